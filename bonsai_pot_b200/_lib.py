@@ -16,6 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libbonsai_attn.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "bonsai_attn.h")
 MODEL_HEADER = os.path.join(os.path.dirname(HERE), "include", "bonsai_model.h")
+PAGED_HEADER = os.path.join(os.path.dirname(HERE), "include", "bonsai_paged.h")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -31,7 +32,7 @@ def needs_build() -> bool:
     if not os.path.exists(LIB_PATH):
         return True
     built = os.path.getmtime(LIB_PATH)
-    deps = sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + [HEADER, MODEL_HEADER]
+    deps = sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + [HEADER, MODEL_HEADER, PAGED_HEADER]
     return any(os.path.getmtime(p) > built for p in deps)
 
 
@@ -173,6 +174,50 @@ MODEL_SIGNATURES = {
     "bp_session_restore": (_int, [_vp, _vp, _u64]),
 }
 
+
+class RopeTableStruct(C.Structure):
+    """`bp_rope_table` of include/bonsai_paged.h."""
+    _fields_ = [("cos_sin", C.c_void_p), ("n_pos", C.c_uint32), ("rot_dim", C.c_uint32), ("layout", C.c_uint32)]
+
+
+class RopeConfigStruct(C.Structure):
+    """`bp_rope_config` of include/bonsai_paged.h."""
+    _fields_ = [("n_pos", C.c_uint32), ("rot_dim", C.c_uint32), ("scaling", C.c_uint32), ("freq_base", C.c_float), ("factor", C.c_float),
+                ("beta_fast", C.c_float), ("beta_slow", C.c_float), ("orig_ctx", C.c_uint32)]
+
+
+class RowsStruct(C.Structure):
+    """`bp_rows` of include/bonsai_paged.h."""
+    _fields_ = [("data", C.c_void_p), ("tok_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class PoolStruct(C.Structure):
+    """`bp_kv4_pool` of include/bonsai_paged.h."""
+    _fields_ = [("data", C.c_void_p), ("n_pages", C.c_uint32), ("page_tokens", C.c_uint32), ("n_kv_head", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
+class AttnStruct(C.Structure):
+    """`bp_kv4_attn` of include/bonsai_paged.h."""
+    _fields_ = [("q", RowsStruct), ("out", RowsStruct), ("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p)] + \
+               [(k, C.c_uint32) for k in ("n_req", "n_head", "total_q", "max_q", "max_kv", "table_stride", "window")] + [("scale", C.c_float)]
+
+
+_rows, _pool, _rope = C.POINTER(RowsStruct), C.POINTER(PoolStruct), C.POINTER(RopeTableStruct)
+
+# name -> (restype, argtypes); must list every symbol include/bonsai_paged.h declares.
+PAGED_SIGNATURES = {
+    "bp_paged_create": (_int, [C.c_int32, _pp]),
+    "bp_paged_destroy": (None, [_vp]),
+    "bp_paged_status": (_int, [_vp, _vp]),
+    "bp_paged_last_error": (C.c_char_p, [_vp]),
+    "bp_rope_fill": (_int, [_vp, _vp, C.POINTER(RopeConfigStruct), _vp]),
+    "bp_rope": (_int, [_vp, _vp, _u32, _rows, _rows, _u32, _u32, _u32, _vp, _rope, _vp, C.c_float, _u32]),
+    "bp_kv4_pool_bytes": (_u64, [_pool]),
+    "bp_kv4_append": (_int, [_vp, _vp, _u32, _pool, _rows, _rows, _u32, _vp, _vp, _rope, _vp, C.c_float]),
+    "bp_kv4_read": (_int, [_vp, _vp, _u32, _pool, _vp, _u32, _rows, _rows]),
+    "bp_kv4_attention": (_int, [_vp, _vp, _u32, _pool, C.POINTER(AttnStruct)]),
+}
+
 _LIB = None
 
 
@@ -189,7 +234,7 @@ def load() -> C.CDLL:
             if not os.path.exists(LIB_PATH):
                 raise ImportError(f"libbonsai_attn.so is missing and could not be built: {e}") from e
     lib = C.CDLL(path)
-    for name, (res, args) in list(SIGNATURES.items()) + list(MODEL_SIGNATURES.items()):
+    for name, (res, args) in [*SIGNATURES.items(), *MODEL_SIGNATURES.items(), *PAGED_SIGNATURES.items()]:
         fn = getattr(lib, name)  # AttributeError here = the header and the library disagree
         fn.restype = res
         fn.argtypes = args

@@ -11,6 +11,8 @@ use std::os::raw::{c_char, c_int, c_void};
 
 /// `include/bonsai_model.h`: operators, model directory, forward passes, sampler, session.
 pub mod model;
+/// `include/bonsai_paged.h`: many requests over one paged KV cache held in 4 bits.
+pub mod paged;
 
 /// Opaque context: owns `kv_k`, `kv_v`, the RoPE table and the split-KV scratch
 /// (what `Model` owns for this path, src/model.rs:1148-1248).
