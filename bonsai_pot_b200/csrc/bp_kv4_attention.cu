@@ -10,6 +10,13 @@
 //                              movmatrix makes from the S^T fragments
 // with a running maximum and sum per row. Queries are scaled per row by a power of two so that the largest element lies in
 // [1, 2): bf16 queries then fit f16.
+//
+// Work is cut into units of 64 keys of one item (request, KV head, 8 NT rows), all of them in one line, of which every CTA takes
+// an equal stretch and every warp of it an equal part: batches of any lengths fill the device evenly. A warp fetches its own keys and
+// values (cp.async.bulk into one K and one V buffer, the next unit's K while V is worked on and the other way round) and waits for nobody.
+// Where an item ends inside a warp's stretch its rows are written at once; pieces of an item are joined, first those of a CTA's warps
+// in shared memory, then those of several CTAs by the CTA that comes last (a counter per item; nobody waits), always in the order of
+// the keys, so that results do not depend on who comes when.
 #include "bp_paged.cuh"
 
 namespace {
@@ -52,24 +59,27 @@ struct Seen {
   int lo, hi;
 };
 
-// State of one warp for one tile of eight rows.
-template <int D>
+// State of one warp for NT tiles of eight rows.
+template <int D, int NT>
 struct WarpState {
   static constexpr int NB = D / 32;
-  uint32_t q[NB][4];  // B fragments of S^T: dims 32 b + 8 t + {0,1}, {2,3} / 16, {4,5}, {6,7} / 16 of row g
-  uint32_t qsum;      // B fragment of the m's: block sums of row g
-  float s_scale[2];   // rows 2 t, 2 t + 1: softmax scale (log2) times the row's power of two
-  Seen seen[2];
-  float m[2], l[2];   // running maximum (log2 units) and this lane's part of the sum, of rows 2 t, 2 t + 1
-  float o[2 * NB][4]; // [m-tile i][dims 32 (i / 2) + 4 g + 2 (i % 2) + {0, 1}] x rows 2 t, 2 t + 1: {d0 r0, d0 r1, d1 r0, d1 r1}
+  uint32_t q[NT][NB][4];  // B fragments of S^T: dims 32 b + 8 t + {0,1}, {2,3} / 16, {4,5}, {6,7} / 16 of row g
+  uint32_t qsum[NT];      // B fragment of the m's: block sums of row g
+  float s_scale[NT][2];   // rows 2 t, 2 t + 1: softmax scale (log2) times the row's power of two
+  Seen seen[NT][2];
+  float m[NT][2], l[NT][2];   // running maximum (log2 units) and this lane's part of the sum, of rows 2 t, 2 t + 1
+  float o[NT][2 * NB][4]; // [m-tile i][dims 32 (i / 2) + 4 g + 2 (i % 2) + {0, 1}] x rows 2 t, 2 t + 1: {d0 r0, d0 r1, d1 r0, d1 r1}
 };
 
 // Loads row g's queries; `row` counts the rows of this (request, KV head), n_rows of them.
-template <int D, bool BF>
-__device__ __forceinline__ void load_queries(WarpState<D>& w, const AttnArgs& a, uint32_t kv_head, uint32_t row0, uint32_t n_rows, uint32_t q0,
+template <int D, bool BF, int NT>
+__device__ __forceinline__ void load_queries(WarpState<D, NT>& w, const AttnArgs& a, uint32_t kv_head, uint32_t tile0, uint32_t n_rows, uint32_t q0,
                                              int q_len, int kv_len, uint32_t lane) {
   constexpr int NB = D / 32;
-  const uint32_t g = lane >> 2, t = lane & 3, row = row0 + g;
+  const uint32_t g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int e = 0; e < NT; e++) {
+  const uint32_t row0 = tile0 + 8 * e, row = row0 + g;
   float x[NB][8], big = 0.f;
 #pragma unroll
   for (int b = 0; b < NB; b++)
@@ -99,7 +109,7 @@ __device__ __forceinline__ void load_queries(WarpState<D>& w, const AttnArgs& a,
     for (int j = 0; j < 4; j++) {
       const __half2 h = __floats2half2_rn(x[b][2 * j] * up, x[b][2 * j + 1] * up);
       sum[b] += __low2float(h) + __high2float(h);
-      w.q[b][j] = u2((j & 1) ? __hmul2(h, __float2half2_rn(0.0625f)) : h);
+      w.q[e][b][j] = u2((j & 1) ? __hmul2(h, __float2half2_rn(0.0625f)) : h);
     }
     sum[b] += __shfl_xor_sync(FULL, sum[b], 1);
     sum[b] += __shfl_xor_sync(FULL, sum[b], 2);
@@ -113,26 +123,28 @@ __device__ __forceinline__ void load_queries(WarpState<D>& w, const AttnArgs& a,
   const __half2 hi = __floats2half2_rn(a0, a1);
   const __half2 lo = __floats2half2_rn(a0 - __low2float(hi), a1 - __high2float(hi));
   const uint32_t lo_from = NB == 4 ? 2 : 1;
-  w.qsum = t < lo_from ? u2(hi) : t < 2 * lo_from ? u2(lo) : 0u;
+  w.qsum[e] = t < lo_from ? u2(hi) : t < 2 * lo_from ? u2(lo) : 0u;
 #pragma unroll
   for (int c = 0; c < 2; c++) {
-    w.s_scale[c] = a.scale_log2 * __shfl_sync(FULL, down, 4 * (2 * t + c));
+    w.s_scale[e][c] = a.scale_log2 * __shfl_sync(FULL, down, 4 * (2 * t + c));
     const uint32_t r = row0 + 2 * t + c;
     const int pos = kv_len - q_len + static_cast<int>(r / a.group);
-    w.seen[c].hi = r < n_rows ? min(pos + 1, kv_len) : 0;
-    w.seen[c].lo = a.window ? max(pos + 1 - static_cast<int>(min(a.window, 0x7fffffffu)), 0) : 0;
-    w.m[c] = NEG_BIG;
-    w.l[c] = 0.f;
+    // (columns without a row see all, so that they ask for no masks; nobody reads them)
+    w.seen[e][c].hi = r < n_rows ? min(pos + 1, kv_len) : 0x7fffffff;
+    w.seen[e][c].lo = a.window && r < n_rows ? max(pos + 1 - static_cast<int>(min(a.window, 0x7fffffffu)), 0) : 0;
+    w.m[e][c] = NEG_BIG;
+    w.l[e][c] = 0.f;
   }
 #pragma unroll
   for (int i = 0; i < 2 * NB; i++)
 #pragma unroll
-    for (int k = 0; k < 4; k++) w.o[i][k] = 0.f;
+    for (int k = 0; k < 4; k++) w.o[e][i][k] = 0.f;
+  }
 }
 
-// S^T of 16 tokens: K codes at kc (rows of ROW bytes), d and m at kd, km (rows of 2 NB bytes).
-template <int D>
-__device__ __forceinline__ void scores16(const WarpState<D>& w, const uint8_t* kc, const uint8_t* kd, const uint8_t* km, uint32_t lane, float (&s)[4]) {
+// S^T of 16 tokens, the k-th of the unit: K codes at kc (rows of ROW bytes), d and m at kd, km (rows of 2 NB bytes).
+template <int D, int NT>
+__device__ __forceinline__ void scores16(const WarpState<D, NT>& w, const uint8_t* kc, const uint8_t* kd, const uint8_t* km, uint32_t lane, float (&s)[NT][4][4], int k) {
   using L = PoolLayout<D>;
   constexpr int NB = D / 32;
   const uint32_t g = lane >> 2, t = lane & 3, ta = tile_token(g), tb = ta + 8;
@@ -159,27 +171,30 @@ __device__ __forceinline__ void scores16(const WarpState<D>& w, const uint8_t* k
     ma = *reinterpret_cast<const uint32_t*>(km + ta * 4);
     mb = *reinterpret_cast<const uint32_t*>(km + tb * 4);
   }
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, low[4] = {0.f, 0.f, 0.f, 0.f};
-  mma_1688(low, ma, mb, w.qsum);
 #pragma unroll
-  for (int b = 0; b < NB; b++) {
-    float p[4] = {0.f, 0.f, 0.f, 0.f};
-    mma_16816(p, wa[b] & 0x000f000fu, wb[b] & 0x000f000fu, wa[b] & 0x00f000f0u, wb[b] & 0x00f000f0u, w.q[b][0], w.q[b][1]);
-    const uint32_t xa = wa[b] >> 8, xb = wb[b] >> 8;
-    mma_16816(p, xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u, w.q[b][2], w.q[b][3]);
-    acc[0] = fmaf(da[b], p[0], acc[0]);
-    acc[1] = fmaf(da[b], p[1], acc[1]);
-    acc[2] = fmaf(db[b], p[2], acc[2]);
-    acc[3] = fmaf(db[b], p[3], acc[3]);
+  for (int e = 0; e < NT; e++) {
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, low[4] = {0.f, 0.f, 0.f, 0.f};
+    mma_1688(low, ma, mb, w.qsum[e]);
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      float p[4] = {0.f, 0.f, 0.f, 0.f};
+      mma_16816(p, wa[b] & 0x000f000fu, wb[b] & 0x000f000fu, wa[b] & 0x00f000f0u, wb[b] & 0x00f000f0u, w.q[e][b][0], w.q[e][b][1]);
+      const uint32_t xa = wa[b] >> 8, xb = wb[b] >> 8;
+      mma_16816(p, xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u, w.q[e][b][2], w.q[e][b][3]);
+      acc[0] = fmaf(da[b], p[0], acc[0]);
+      acc[1] = fmaf(da[b], p[1], acc[1]);
+      acc[2] = fmaf(db[b], p[2], acc[2]);
+      acc[3] = fmaf(db[b], p[3], acc[3]);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c++) s[e][k][c] = fmaf(acc[c], 0x1p24f, low[c]) * w.s_scale[e][c & 1];
   }
-#pragma unroll
-  for (int k = 0; k < 4; k++) s[k] = fmaf(acc[k], 0x1p24f, low[k]) * w.s_scale[k & 1];
 }
 
-// O^T += V^T P^T of 16 tokens of which the first `valid` (>= 16: all) have been written. p0, p1: B fragments of P^T.
-template <int D>
-__device__ __forceinline__ void values16(WarpState<D>& w, const uint8_t* vc, const uint8_t* vd, const uint8_t* vm, uint32_t place, uint32_t valid,
-                                         uint32_t lane, uint32_t p0, uint32_t p1) {
+// O^T += V^T P^T of 16 tokens of which those in [from, to) are the request's (0 and 16 or beyond: all). s: P as S^T fragments.
+template <int D, int NT>
+__device__ __forceinline__ void values16(WarpState<D, NT>& w, const uint8_t* vc, const uint8_t* vd, const uint8_t* vm, uint32_t place, int from, int to,
+                                         uint32_t lane, const float (&s)[NT][4][4], int k) {
   using L = PoolLayout<D>;
   constexpr int NB = D / 32;
   const uint32_t g = lane >> 2, t = lane & 3;
@@ -207,8 +222,8 @@ __device__ __forceinline__ void values16(WarpState<D>& w, const uint8_t* vc, con
       am[0] = *reinterpret_cast<const uint32_t*>(vm + ta * 4);
       bm[0] = *reinterpret_cast<const uint32_t*>(vm + tb * 4);
     }
-    if (valid < 16) {  // places that nobody has written may hold any bits: P is 0 there, the values must be numbers
-      const bool za = ta >= valid, zb = tb >= valid;
+    if (from > 0 || to < 16) {  // the other places may hold any bits: P is 0 there, the values must be numbers
+      const bool za = static_cast<int>(ta) < from || static_cast<int>(ta) >= to, zb = static_cast<int>(tb) < from || static_cast<int>(tb) >= to;
 #pragma unroll
       for (int i = 0; i < NB / 2; i++) {
         ad[i] = za ? 0u : ad[i];
@@ -233,138 +248,501 @@ __device__ __forceinline__ void values16(WarpState<D>& w, const uint8_t* vc, con
     }
   }
 #pragma unroll
-  for (int bl = 0; bl < NB; bl++) {
-    mma_16816(w.o[2 * bl], av[0][bl][0], av[0][bl][1], av[1][bl][0], av[1][bl][1], p0, p1);
-    mma_16816(w.o[2 * bl + 1], av[0][bl][2], av[0][bl][3], av[1][bl][2], av[1][bl][3], p0, p1);
+  for (int e = 0; e < NT; e++) {
+    const uint32_t p0 = movmatrix(pack2<false>(s[e][k][0], s[e][k][1])), p1 = movmatrix(pack2<false>(s[e][k][2], s[e][k][3]));
+#pragma unroll
+    for (int bl = 0; bl < NB; bl++) {
+      mma_16816(w.o[e][2 * bl], av[0][bl][0], av[0][bl][1], av[1][bl][0], av[1][bl][1], p0, p1);
+      mma_16816(w.o[e][2 * bl + 1], av[0][bl][2], av[0][bl][3], av[1][bl][2], av[1][bl][3], p0, p1);
+    }
   }
 }
 
-// P, still as the S^T fragments of up to four tiles, from the scores: masks, maximum, exponentials, sums; O is rescaled.
-template <int D>
-__device__ __forceinline__ void softmax64(WarpState<D>& w, float (&s)[4][4], int key0, uint32_t lane) {
+// P, still as the S^T fragments of four tiles, from the scores: masks, maximum, exponentials, sums; O is rescaled.
+template <int D, int NT>
+__device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4][4], int key0, uint32_t lane) {
   constexpr int NB = D / 32;
   const uint32_t g = lane >> 2;
-  const bool cut = key0 + static_cast<int>(UNIT) > min(w.seen[0].hi, w.seen[1].hi) || key0 < max(w.seen[0].lo, w.seen[1].lo);
-  if (__any_sync(FULL, cut)) {
+#pragma unroll
+  for (int e = 0; e < NT; e++) {
+    const bool cut = key0 + static_cast<int>(UNIT) > min(w.seen[e][0].hi, w.seen[e][1].hi) || key0 < max(w.seen[e][0].lo, w.seen[e][1].lo);
+    if (__any_sync(FULL, cut)) {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int key = key0 + 16 * i + static_cast<int>(tile_token(g + 8 * (k >> 1)));
+          if (key < w.seen[e][k & 1].lo || key >= w.seen[e][k & 1].hi) s[e][i][k] = __int_as_float(0xff800000);
+        }
+    }
+    float mx[2];
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      mx[c] = fmaxf(s[e][0][c], s[e][0][c + 2]);
+#pragma unroll
+      for (int i = 1; i < 4; i++) mx[c] = fmaxf(mx[c], fmaxf(s[e][i][c], s[e][i][c + 2]));
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(FULL, mx[c], o));
+    }
+    if (__any_sync(FULL, mx[0] > w.m[e][0] || mx[1] > w.m[e][1])) {
+      float corr[2];
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        const float m_new = fmaxf(w.m[e][c], mx[c]);
+        corr[c] = ex2(w.m[e][c] - m_new);
+        w.m[e][c] = m_new;
+        w.l[e][c] *= corr[c];
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * NB; i++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) w.o[e][i][k] *= corr[k & 1];
+    }
+    const float top[2] = {w.m[e][0] - P_UP, w.m[e][1] - P_UP};
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        const int key = key0 + 16 * i + static_cast<int>(tile_token(g + 8 * (k >> 1)));
-        if (key < w.seen[k & 1].lo || key >= w.seen[k & 1].hi) s[i][k] = __int_as_float(0xff800000);
+        s[e][i][k] = ex2(s[e][i][k] - top[k & 1]);
+        w.l[e][k & 1] += s[e][i][k];
       }
   }
-  float mx[2];
-#pragma unroll
-  for (int c = 0; c < 2; c++) {
-    mx[c] = fmaxf(s[0][c], s[0][c + 2]);
-#pragma unroll
-    for (int i = 1; i < 4; i++) mx[c] = fmaxf(mx[c], fmaxf(s[i][c], s[i][c + 2]));
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(FULL, mx[c], o));
-  }
-  if (__any_sync(FULL, mx[0] > w.m[0] || mx[1] > w.m[1])) {
-    float corr[2];
-#pragma unroll
-    for (int c = 0; c < 2; c++) {
-      const float m_new = fmaxf(w.m[c], mx[c]);
-      corr[c] = ex2(w.m[c] - m_new);
-      w.m[c] = m_new;
-      w.l[c] *= corr[c];
-    }
-#pragma unroll
-    for (int i = 0; i < 2 * NB; i++)
-#pragma unroll
-      for (int k = 0; k < 4; k++) w.o[i][k] *= corr[k & 1];
-  }
-  const float top[2] = {w.m[0] - P_UP, w.m[1] - P_UP};
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      s[i][k] = ex2(s[i][k] - top[k & 1]);
-      w.l[k & 1] += s[i][k];
-    }
 }
 
-// One warp per (eight rows, KV head, request), all keys one behind the other.
-template <int D, bool BF>
-__global__ void __launch_bounds__(32) kv4_attention_plain_kernel(const AttnArgs a) {
+constexpr uint32_t NWARP = 8, THREADS = 32 * NWARP;
+constexpr uint32_t WAIT_LIMIT = 1u << 20;  // polls before a warp gives up on a copy
+
+template <int D, int NT>
+struct Shape {
+  static constexpr uint32_t ROWS = 8 * NT;                               // rows of an item
+  static constexpr uint32_t PART = UNIT * PoolLayout<D>::TOK / 2;        // bytes of a unit's K (or V)
+  static constexpr uint32_t STRIDE = D + 4;                              // floats of a row of a partial result: o, m, l
+  static constexpr uint32_t PARTIAL = ROWS * STRIDE;                     // floats of one
+  static constexpr uint32_t SMEM = NWARP * 2 * PART;
+  static constexpr int CTAS = NT == 1 || D == 64 ? 2 : 1;                // per SM: two where 128 registers do
+  static_assert(PARTIAL * 4 <= 2 * PART, "a warp's partial result goes over its buffers");
+};
+
+// What one request asks for.
+struct Request {
+  int q0, q_len, kv_len, low;    // low: no query sees a key before it
+  __device__ int first() const { return low & ~static_cast<int>(UNIT - 1); }
+  uint32_t units, tiles;         // units of 64 keys of an item; items per KV head
+};
+template <int NT>
+__device__ __forceinline__ Request request(const AttnArgs& a, uint32_t r, bool report) {
+  Request q;
+  q.q0 = max(a.q_start[r], 0);
+  const int given_q = max(min(a.q_start[r + 1], static_cast<int>(a.total_q)) - q.q0, 0), given_kv = max(a.kv_len[r], 0);
+  q.q_len = min(given_q, static_cast<int>(a.max_q));
+  q.kv_len = min(given_kv, static_cast<int>(min(a.max_kv, a.table_stride << a.pool.log_page)));
+  if (report && (given_q > q.q_len || given_kv > q.kv_len)) note_range(a.err);
+  const int from = a.window ? q.kv_len - q.q_len + 1 - static_cast<int>(min(a.window, 0x40000000u)) : 0;
+  q.low = max(min(from, q.kv_len), 0);
+  q.units = max((static_cast<uint32_t>(q.kv_len - q.first()) + UNIT - 1) / UNIT, 1u);  // (an item without keys still has its zeros to write)
+  q.tiles = (static_cast<uint32_t>(q.q_len) * a.group + 8 * NT - 1) / (8 * NT);
+  return q;
+}
+
+// A place in the line of units.
+struct Cursor {
+  Request q;
+  uint32_t r, head, tile, unit;
+};
+template <int NT>
+__device__ __forceinline__ void next_item(Cursor& c, const AttnArgs& a) {
+  c.unit = 0;
+  if (++c.tile < c.q.tiles) return;
+  c.tile = 0;
+  if (++c.head < a.pool.n_kv_head) return;
+  c.head = 0;
+  do {
+    if (++c.r >= a.n_req) return;
+    c.q = request<NT>(a, c.r, false);
+  } while (c.q.tiles == 0);
+}
+
+// A piece of an item that one warp has worked on.
+struct Piece {
+  uint32_t used, r, head, tile, units;
+  unsigned long long start;  // the item's first unit in the line
+};
+
+// Fetches K or V of a unit, one lane per page. ids: lane l has the page id of page `base + l` of the request.
+struct Fetch {
+  uint32_t ids, base;
+};
+__device__ __forceinline__ void load_ids(Fetch& f, const AttnArgs& a, const Cursor& c, uint32_t first_page, uint32_t lane) {
+  const uint32_t pages = (static_cast<uint32_t>(c.q.kv_len) + a.pool.page - 1) >> a.pool.log_page;
+  f.base = first_page;
+  f.ids = 0xffffffffu;
+  if (first_page + lane < pages) f.ids = static_cast<uint32_t>(a.page_table[static_cast<size_t>(c.r) * a.table_stride + first_page + lane]);
+}
+// Returns which of the unit's pages are on their way: those that hold keys of [low, kv_len) and have a good id.
+template <int D>
+__device__ __forceinline__ uint32_t fetch(Fetch& f, const AttnArgs& a, const Cursor& c, uint32_t v, uint32_t dst, uint32_t bar, uint32_t lane) {
+  using L = PoolLayout<D>;
+  const int key0 = c.q.first() + static_cast<int>(c.unit * UNIT), key = key0 + static_cast<int>(lane << a.pool.log_page);
+  const uint32_t page0 = static_cast<uint32_t>(key0) >> a.pool.log_page, n = UNIT >> a.pool.log_page;
+  if (page0 - f.base >= 32) load_ids(f, a, c, page0, lane);
+  const uint32_t id = __shfl_sync(FULL, f.ids, (page0 - f.base + lane) & 31);
+  const bool there = lane < n && key < c.q.kv_len && key + static_cast<int>(a.pool.page) > c.q.low, good = there && id < a.pool.n_pages;
+  if (there && !good) note_range(a.err);
+  const uint32_t bytes = a.pool.page * (L::TOK / 2), pages = __ballot_sync(FULL, good);
+  if (lane == 0) mbar_arrive_expect_tx(bar, __popc(pages) * bytes);
+  __syncwarp();
+  if (good) {
+    const uint8_t* src = a.pool.data + (static_cast<size_t>(id) * a.pool.n_kv_head + c.head) * (static_cast<size_t>(a.pool.page) * L::TOK) + v * bytes;
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + lane * bytes), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+  }
+  return pages;
+}
+
+// Four dims of an output row.
+template <bool BF>
+__device__ __forceinline__ void store4(uint16_t* p, float a, float b, float c, float d) {
+  const uint32_t x = pack2<BF>(a, b), y = pack2<BF>(c, d);
+  if ((reinterpret_cast<uintptr_t>(p) & 7) == 0) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(x, y);
+  } else {
+    p[0] = static_cast<uint16_t>(x);
+    p[1] = static_cast<uint16_t>(x >> 16);
+    p[2] = static_cast<uint16_t>(y);
+    p[3] = static_cast<uint16_t>(y >> 16);
+  }
+}
+__device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, int q0, uint32_t head, uint32_t row) {
+  return a.out.data + static_cast<int64_t>(q0 + row / a.group) * a.out.tok + static_cast<int64_t>(head * a.group + row % a.group) * a.out.head;
+}
+
+// Pieces of one item, given by `at(i)`, i = from, from + step, ... < n: the running result of four dims of one row.
+struct Joined {
+  float m, l;
+  float4 o;
+  __device__ void add(float m2, float l2, float4 o2) {
+    const float top = fmaxf(m, m2), w1 = ex2(m - top), w2 = ex2(m2 - top);
+    m = top;
+    l = l * w1 + l2 * w2;
+    o = make_float4(o.x * w1 + o2.x * w2, o.y * w1 + o2.y * w2, o.z * w1 + o2.z * w2, o.w * w1 + o2.w * w2);
+  }
+};
+
+template <int D, bool BF, int NT>
+__global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_kernel(const AttnArgs a, float* __restrict__ scratch, uint32_t* __restrict__ counters) {
+  using S = Shape<D, NT>;
   using L = PoolLayout<D>;
   constexpr int NB = D / 32;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t bars[NWARP][2];
+  __shared__ unsigned long long line[THREADS + 1];  // units before the requests of thread t's part
+  __shared__ Piece pieces[NWARP][2];
+  __shared__ uint32_t items_s, most_s, last_s;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  uint8_t* buf[2] = {smem + warp * 2 * S::PART, smem + warp * 2 * S::PART + S::PART};
+  const uint32_t bar[2] = {smem_u32(&bars[warp][0]), smem_u32(&bars[warp][1])};
+  if (lane == 0) {
+    mbar_init(bar[0], 1);
+    mbar_init(bar[1], 1);
+    fence_barrier_init();
+  }
+  if (lane < 2) pieces[warp][lane].used = 0;
+  if (threadIdx.x == 0) items_s = most_s = 0;
+  __syncthreads();
   pdl_launch_dependents();
   pdl_wait();
-  const uint32_t lane = threadIdx.x, r = blockIdx.z, head = blockIdx.y, row0 = blockIdx.x * 8;
-  int q0 = max(a.q_start[r], 0), q1 = min(a.q_start[r + 1], static_cast<int>(a.total_q));
-  const int q_given = max(q1 - q0, 0), q_len = min(q_given, static_cast<int>(a.max_q));
-  const uint32_t n_rows = q_len * a.group;
-  if (row0 >= n_rows) return;
-  const uint32_t most = min(a.max_kv, a.table_stride << a.pool.log_page);
-  const int given = max(a.kv_len[r], 0), kv_len = min(given, static_cast<int>(most));
-  if ((given > kv_len || q_given > q_len) && lane == 0) note_range(a.err);
-  WarpState<D> w;
-  load_queries<D, BF>(w, a, head, row0, n_rows, q0, q_len, kv_len, lane);
-  const uint32_t page = a.pool.page;
-  int lo = min(w.seen[0].lo, w.seen[1].lo), hi = max(w.seen[0].hi, w.seen[1].hi);
+
+  // ---- this warp's stretch of the line ----
+  const uint32_t per = (a.n_req + THREADS - 1) / THREADS;
+  unsigned long long mine = 0;
+  {
+    uint32_t items = 0, most = 0;
+    for (uint32_t r = threadIdx.x * per; r < min((threadIdx.x + 1) * per, a.n_req); r++) {
+      const Request q = request<NT>(a, r, blockIdx.x == 0);
+      items += q.tiles * a.pool.n_kv_head;
+      if (q.tiles) most = max(most, q.units);
+      mine += static_cast<unsigned long long>(q.tiles) * a.pool.n_kv_head * q.units;
+    }
+    unsigned long long up = mine;
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    lo = min(lo, __shfl_xor_sync(FULL, lo, o));
-    hi = max(hi, __shfl_xor_sync(FULL, hi, o));
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long x = __shfl_up_sync(FULL, up, o);
+      if (lane >= o) up += x;
+    }
+    line[threadIdx.x + 1] = up;  // within the warp
+    items = __reduce_add_sync(FULL, items);
+    most = __reduce_max_sync(FULL, most);
+    if (lane == 0) {
+      atomicAdd(&items_s, items);
+      atomicMax(&most_s, most);
+    }
   }
-  for (int key0 = lo / static_cast<int>(UNIT) * static_cast<int>(UNIT); key0 < hi; key0 += UNIT) {
-    float s[4][4];
-    const uint8_t* rec[4];
+  __syncthreads();
+  unsigned long long before = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int key = key0 + 16 * i;
-      rec[i] = nullptr;
-#pragma unroll
-      for (int k = 0; k < 4; k++) s[i][k] = __int_as_float(0xff800000);
-      if (key >= kv_len) continue;
-      const uint32_t id = static_cast<uint32_t>(a.page_table[static_cast<size_t>(r) * a.table_stride + (key >> a.pool.log_page)]);
-      if (id >= a.pool.n_pages) {
-        if (lane == 0 && key + 16 > lo) note_range(a.err);
-        continue;
+  for (uint32_t w = 0; w < NWARP; w++) before += w < warp ? line[32 * (w + 1)] : 0;
+  __syncthreads();
+  line[threadIdx.x + 1] += before;
+  if (threadIdx.x == 0) line[0] = 0;
+  __syncthreads();
+  const unsigned long long total = line[THREADS];
+  // One item per CTA where that takes at most one round of the warps more than equal stretches, which need their pieces
+  // joined; else equal stretches, of one unit per warp at least.
+  const uint32_t n_cta = gridDim.x;
+  const unsigned long long even = (total + n_cta - 1) / n_cta, share = max(even, static_cast<unsigned long long>(NWARP));
+  const bool whole = items_s <= n_cta && (most_s + NWARP - 1) / NWARP <= (share + NWARP - 1) / NWARP + 1;
+  unsigned long long c0, c1;
+  Cursor cur;
+  cur.r = cur.head = cur.tile = cur.unit = 0;
+  cur.q = Request{};
+  auto locate = [&](unsigned long long x) {  // x < total
+    uint32_t lo = 0, hi = THREADS;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (line[mid] <= x) lo = mid;
+      else hi = mid;
+    }
+    unsigned long long left = x - line[lo];
+    for (uint32_t r = lo * per; r < a.n_req; r++) {
+      const Request q = request<NT>(a, r, false);
+      const unsigned long long n = static_cast<unsigned long long>(q.tiles) * a.pool.n_kv_head * q.units;
+      if (left < n) {
+        const uint32_t item = static_cast<uint32_t>(left / q.units);
+        cur.q = q;
+        cur.r = r;
+        cur.unit = static_cast<uint32_t>(left % q.units);
+        cur.head = item / q.tiles;
+        cur.tile = item % q.tiles;
+        return;
       }
-      rec[i] = a.pool.data + (static_cast<size_t>(id) * a.pool.n_kv_head + head) * (static_cast<size_t>(page) * L::TOK);
-      const uint32_t place = key & (page - 1);
-      scores16<D>(w, rec[i] + place * L::ROW, rec[i] + L::kd(page) + place * 2 * NB, rec[i] + L::km(page) + place * 2 * NB, lane, s[i]);
+      left -= n;
     }
-    softmax64<D>(w, s, key0, lane);
+  };
+  if (whole) {  // item blockIdx.x: its place in the line
+    c0 = c1 = 0;
+    if (blockIdx.x < items_s) {
+      uint32_t left = blockIdx.x;
+      for (uint32_t r = 0; r < a.n_req; r++) {
+        const Request q = request<NT>(a, r, false);
+        const uint32_t n = q.tiles * a.pool.n_kv_head;
+        if (left < n) {
+          c0 += static_cast<unsigned long long>(left) * q.units;
+          c1 = c0 + q.units;
+          break;
+        }
+        left -= n;
+        c0 += static_cast<unsigned long long>(n) * q.units;
+      }
+    }
+  } else {
+    c0 = min(blockIdx.x * share, total);
+    c1 = min(c0 + share, total);
+  }
+  if (c0 >= c1) return;  // (all threads)
+  const uint32_t cta_units = static_cast<uint32_t>(c1 - c0);
+  const unsigned long long x0 = c0 + static_cast<unsigned long long>(cta_units) * warp / NWARP;
+  const uint32_t n = static_cast<uint32_t>(c0 + static_cast<unsigned long long>(cta_units) * (warp + 1) / NWARP - x0);
+
+  if (n > 0) {
+    locate(x0);
+    Cursor next = cur;  // the unit that is fetched
+    Fetch f;
+    load_ids(f, a, next, (next.q.first() + next.unit * UNIT) >> a.pool.log_page, lane);
+    uint32_t pages = fetch<D>(f, a, next, 0, smem_u32(buf[0]), bar[0], lane), next_pages = 0;
+    (void)fetch<D>(f, a, next, 1, smem_u32(buf[1]), bar[1], lane);
+    WarpState<D, NT> w;
+    bool fresh = true, from_start = false, ok = true;
+    const uint32_t lp = a.pool.log_page, page = a.pool.page, half = page * (L::TOK / 2);
+    for (uint32_t i = 0; i < n; i++) {
+      if (fresh) {
+        load_queries<D, BF, NT>(w, a, cur.head, cur.tile * S::ROWS, cur.q.q_len * a.group, cur.q.q0, cur.q.q_len, cur.q.kv_len, lane);
+        from_start = cur.unit == 0;
+        fresh = false;
+      }
+      const int key0 = cur.q.first() + cur.unit * UNIT, left = cur.q.kv_len - key0;
+      const bool more = i + 1 < n;
+      bool moved = false;
+      if (more) {
+        if (++next.unit == next.q.units) {
+          next_item<NT>(next, a);
+          moved = true;
+        }
+      }
+      float s[NT][4][4];
+      ok = ok && mbar_wait(bar[0], i & 1, WAIT_LIMIT);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      if (!rec[i]) continue;
-      const int key = key0 + 16 * i;
-      const uint32_t place = key & (page - 1);
-      const uint8_t* v = rec[i] + L::v(page);
-      const uint32_t p0 = movmatrix(pack2<false>(s[i][0], s[i][1])), p1 = movmatrix(pack2<false>(s[i][2], s[i][3]));
-      values16<D>(w, v + place * L::ROW, v + L::kd(page) + place * 2 * NB, v + L::km(page) + place * 2 * NB, place, kv_len - key, lane, p0, p1);
+      for (int k = 0; k < 4; k++) {
+        const uint32_t pg = (16 * k) >> lp, place = (16 * k) & (page - 1);
+        const uint8_t* p = buf[0] + pg * half;
+        if (pages >> pg & 1)
+          scores16<D, NT>(w, p + place * L::ROW, p + L::kd(page) + place * 2 * NB, p + L::km(page) + place * 2 * NB, lane, s, k);
+        else
+#pragma unroll
+          for (int e = 0; e < NT; e++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) s[e][k][c] = __int_as_float(0xff800000);
+      }
+      __syncwarp();
+      if (more && ok) {
+        if (moved) load_ids(f, a, next, (next.q.first() + next.unit * UNIT) >> lp, lane);
+        next_pages = fetch<D>(f, a, next, 0, smem_u32(buf[0]), bar[0], lane);
+      }
+      softmax64<D, NT>(w, s, key0, lane);
+      ok = ok && mbar_wait(bar[1], i & 1, WAIT_LIMIT);
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const uint32_t pg = (16 * k) >> lp, place = (16 * k) & (page - 1);
+        if (!(pages >> pg & 1)) continue;
+        const uint8_t* p = buf[1] + pg * half;
+        values16<D, NT>(w, p + place * L::ROW, p + L::kd(page) + place * 2 * NB, p + L::km(page) + place * 2 * NB, place, cur.q.low - key0 - 16 * k, left - 16 * k, lane, s, k);
+      }
+      __syncwarp();
+      if (more && ok) (void)fetch<D>(f, a, next, 1, smem_u32(buf[1]), bar[1], lane);
+      pages = next_pages;
+      if (!ok) break;
+
+      const bool ends = cur.unit + 1 == cur.q.units;
+      if (ends || !more) {
+        // sums over the lanes of a row
+#pragma unroll
+        for (int e = 0; e < NT; e++)
+#pragma unroll
+          for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) w.l[e][c] += __shfl_xor_sync(FULL, w.l[e][c], o);
+        const uint32_t row0 = cur.tile * S::ROWS, n_rows = cur.q.q_len * a.group;
+        if (ends && from_start) {
+#pragma unroll
+          for (int e = 0; e < NT; e++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+              const uint32_t row = row0 + 8 * e + 2 * t + c;
+              if (row >= n_rows) continue;
+              const float inv = w.l[e][c] == 0.f ? 0.f : 1.f / w.l[e][c];
+              uint16_t* out = out_row(a, cur.q.q0, cur.head, row);
+#pragma unroll
+              for (int b = 0; b < NB; b++)
+                store4<BF>(out + 32 * b + 4 * g, w.o[e][2 * b][c] * inv, w.o[e][2 * b][c + 2] * inv, w.o[e][2 * b + 1][c] * inv, w.o[e][2 * b + 1][c + 2] * inv);
+            }
+        } else {
+          // an item's end goes to memory (the buffers are in use), the stretch's end over the buffers
+          float* part = ends ? scratch + (static_cast<size_t>(blockIdx.x) * NWARP + warp) * S::PARTIAL : reinterpret_cast<float*>(buf[0]);
+#pragma unroll
+          for (int e = 0; e < NT; e++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+              float* p = part + (8 * e + 2 * t + c) * S::STRIDE;
+#pragma unroll
+              for (int b = 0; b < NB; b++)
+                *reinterpret_cast<float4*>(p + 32 * b + 4 * g) = make_float4(w.o[e][2 * b][c], w.o[e][2 * b][c + 2], w.o[e][2 * b + 1][c], w.o[e][2 * b + 1][c + 2]);
+              if (g == 0) *reinterpret_cast<float2*>(p + D) = make_float2(w.m[e][c], w.l[e][c]);
+            }
+          if (lane == 0) pieces[warp][ends ? 0 : 1] = Piece{1, cur.r, cur.head, cur.tile, cur.q.units, x0 + i - cur.unit};
+        }
+        fresh = true;
+      }
+      if (more) {
+        if (ends) next_item<NT>(cur, a);
+        else cur.unit++;
+      }
+    }
+    if (!ok) {  // the wait gave up: what is on its way comes before the buffers are given back
+      if (lane == 0) reinterpret_cast<volatile uint32_t*>(a.err)[1] = 1;
+      for (uint32_t k = 0; k < 2; k++)
+        for (uint32_t ph = 0; ph < 2; ph++) (void)mbar_wait(bar[k], ph, DRAIN_LIMIT);
     }
   }
-  const uint32_t g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int c = 0; c < 2; c++) {
-    float l = w.l[c];
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(FULL, l, o);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const uint32_t row = row0 + 2 * t + c;
-    if (row >= n_rows) continue;
-    uint16_t* out = a.out.data + static_cast<int64_t>(q0 + row / a.group) * a.out.tok + static_cast<int64_t>(head * a.group + row % a.group) * a.out.head;
-#pragma unroll
-    for (int i = 0; i < 2 * NB; i++) {
-      const uint32_t h = pack2<BF>(w.o[i][c] * inv, w.o[i][c + 2] * inv), dim = 32 * (i >> 1) + 4 * g + 2 * (i & 1);
-      out[dim] = static_cast<uint16_t>(h);
-      out[dim + 1] = static_cast<uint16_t>(h >> 16);
+  __syncthreads();
+
+  // ---- the CTA's pieces ----
+  float* exchange = scratch + static_cast<size_t>(gridDim.x) * NWARP * S::PARTIAL;
+  for (uint32_t i = 0; i < 2 * NWARP;) {
+    const Piece& p = pieces[i >> 1][i & 1];
+    if (!p.used) {
+      i++;
+      continue;
     }
+    uint32_t end = i + 1;  // pieces [i, end) that are used belong to one item
+    for (uint32_t k = i + 1; k < 2 * NWARP; k++) {
+      const Piece& o = pieces[k >> 1][k & 1];
+      if (!o.used) continue;
+      if (o.start != p.start) break;
+      end = k + 1;
+    }
+    const int q0 = max(a.q_start[p.r], 0);
+    const uint32_t n_rows = static_cast<uint32_t>(min(max(min(a.q_start[p.r + 1], static_cast<int>(a.total_q)) - q0, 0), static_cast<int>(a.max_q))) * a.group;
+    const uint32_t row0 = p.tile * S::ROWS, rows = min(S::ROWS, n_rows - row0), cols = rows * (D / 4);
+    const bool all = p.start >= c0 && p.start + p.units <= c1;
+    const uint32_t first_cta = all ? 0 : static_cast<uint32_t>(p.start / share), n_parts = all ? 1 : static_cast<uint32_t>((p.start + p.units - 1) / share) - first_cta + 1;
+    float* mine_out = exchange + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PARTIAL;
+    for (uint32_t x = threadIdx.x; x < cols; x += THREADS) {
+      const uint32_t row = x / (D / 4), col = x % (D / 4) * 4;
+      Joined j{NEG_BIG, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+      for (uint32_t k = i; k < end; k++) {
+        if (!pieces[k >> 1][k & 1].used) continue;
+        const float* part = (k & 1) ? reinterpret_cast<const float*>(smem + (k >> 1) * 2 * S::PART) : scratch + (static_cast<size_t>(blockIdx.x) * NWARP + (k >> 1)) * S::PARTIAL;
+        const float2 ml = *reinterpret_cast<const float2*>(part + row * S::STRIDE + D);
+        j.add(ml.x, ml.y, *reinterpret_cast<const float4*>(part + row * S::STRIDE + col));
+      }
+      if (all) {
+        const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
+        store4<BF>(out_row(a, q0, p.head, row0 + row) + col, j.o.x * inv, j.o.y * inv, j.o.z * inv, j.o.w * inv);
+      } else {
+        *reinterpret_cast<float4*>(mine_out + row * S::STRIDE + col) = j.o;
+        if (col == 0) *reinterpret_cast<float2*>(mine_out + row * S::STRIDE + D) = make_float2(j.m, j.l);
+      }
+    }
+    if (!all) {
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const uint32_t seen = atomicAdd(&counters[first_cta], 1u);
+        last_s = seen == n_parts - 1;
+        if (last_s) counters[first_cta] = 0;  // for the next launch
+        __threadfence();
+      }
+      __syncthreads();
+      if (last_s) {
+        for (uint32_t x = threadIdx.x; x < cols; x += THREADS) {
+          const uint32_t row = x / (D / 4), col = x % (D / 4) * 4;
+          Joined j{NEG_BIG, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 4
+          for (uint32_t k = 0; k < n_parts; k++) {
+            const float* part = exchange + static_cast<size_t>(2 * (first_cta + k) + (k == 0)) * S::PARTIAL + row * S::STRIDE;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + D));
+            j.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(part + col)));
+          }
+          const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
+          store4<BF>(out_row(a, q0, p.head, row0 + row) + col, j.o.x * inv, j.o.y * inv, j.o.z * inv, j.o.w * inv);
+        }
+      }
+      __syncthreads();
+    }
+    i = end;
   }
+}
+
+template <int D, bool BF, int NT>
+cudaError_t allow() {
+  return cudaFuncSetAttribute(kv4_attention_kernel<D, BF, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<D, NT>::SMEM));
 }
 
 }  // namespace
 
 cudaError_t bp_kv4_attention_init(bp_paged_ctx* c) {
-  (void)c;
-  return cudaSuccess;
+  cudaError_t e;
+  if ((e = allow<128, false, 1>()) != cudaSuccess || (e = allow<128, true, 1>()) != cudaSuccess || (e = allow<64, false, 1>()) != cudaSuccess ||
+      (e = allow<64, true, 1>()) != cudaSuccess || (e = allow<128, false, 2>()) != cudaSuccess || (e = allow<128, true, 2>()) != cudaSuccess ||
+      (e = allow<64, false, 2>()) != cudaSuccess || (e = allow<64, true, 2>()) != cudaSuccess)
+    return e;
+  // a piece per warp and two per CTA, of the instance that needs most
+  const size_t one = 2 * static_cast<size_t>(c->sm_count) * (NWARP + 2);
+  const size_t floats = one * Shape<128, 2>::PARTIAL;
+  e = cudaMalloc(&c->partials, floats * sizeof(float));
+  if (e != cudaSuccess) return e;
+  e = cudaMalloc(&c->counters, 2 * static_cast<size_t>(c->sm_count) * sizeof(uint32_t));
+  if (e != cudaSuccess) return e;
+  return cudaMemset(c->counters, 0, 2 * static_cast<size_t>(c->sm_count) * sizeof(uint32_t));
 }
 
 cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, const Pool& pool, uint32_t head_dim, const bp_kv4_attn& in) {
@@ -385,7 +763,14 @@ cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, co
   a.table_stride = in.table_stride < (0x7fffffffu >> pool.log_page) ? in.table_stride : (0x7fffffffu >> pool.log_page);
   a.window = in.window;
   a.scale_log2 = in.scale * 1.4426950408889634f;
-  const dim3 grid((a.max_q * a.group + 7) / 8, pool.n_kv_head, in.n_req);
-  if (head_dim == 128) return bp_launch(true, bf ? kv4_attention_plain_kernel<128, true> : kv4_attention_plain_kernel<128, false>, grid, dim3(32), 0, s, a);
-  return bp_launch(true, bf ? kv4_attention_plain_kernel<64, true> : kv4_attention_plain_kernel<64, false>, grid, dim3(32), 0, s, a);
+  auto go = [&](auto kernel, uint32_t smem, uint32_t ctas) {
+    return bp_launch(true, kernel, dim3(ctas * static_cast<uint32_t>(c->sm_count)), dim3(THREADS), smem, s, a, c->partials, c->counters);
+  };
+  const bool two = a.max_q * a.group > 8;
+  if (head_dim == 128) {
+    if (two) return go(bf ? kv4_attention_kernel<128, true, 2> : kv4_attention_kernel<128, false, 2>, Shape<128, 2>::SMEM, Shape<128, 2>::CTAS);
+    return go(bf ? kv4_attention_kernel<128, true, 1> : kv4_attention_kernel<128, false, 1>, Shape<128, 1>::SMEM, Shape<128, 1>::CTAS);
+  }
+  if (two) return go(bf ? kv4_attention_kernel<64, true, 2> : kv4_attention_kernel<64, false, 2>, Shape<64, 2>::SMEM, Shape<64, 2>::CTAS);
+  return go(bf ? kv4_attention_kernel<64, true, 1> : kv4_attention_kernel<64, false, 1>, Shape<64, 1>::SMEM, Shape<64, 1>::CTAS);
 }
