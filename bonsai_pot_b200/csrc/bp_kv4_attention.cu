@@ -17,6 +17,8 @@
 // Where an item ends inside a warp's stretch its rows are written at once; pieces of an item are joined, first those of a CTA's warps
 // in shared memory, then those of several CTAs by the CTA that comes last (a counter per item; nobody waits), always in the order of
 // the keys, so that results do not depend on who comes when.
+#include <type_traits>
+
 #include "bp_paged.cuh"
 
 namespace {
@@ -35,6 +37,8 @@ struct AttnArgs {
   uint32_t* err;
   uint32_t n_req, n_head, group, total_q, max_q, max_kv, table_stride, window;
   float scale_log2;
+  uint32_t bias;  // 0x64006400: two f16 numbers 1024
+  uint32_t bf;    // activations are bfloat16
 };
 
 // The token of a 16-token tile that a lane's MMA row r holds. K rows 2 j and 2 j + 1 then differ in parity and the values of
@@ -46,10 +50,21 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ void mma_1688(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(b0));
+// D = A B, as mma_16816 without C; and of eight k's.
+__device__ __forceinline__ void mma_16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_1688_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
+}
+// (x & mask) | 0x64006400 in one instruction: it has room for one constant, so the other one is a kernel argument
+__device__ __forceinline__ __half2 biased(uint32_t x, uint32_t mask, uint32_t bias) {
+  const uint32_t r = lop3<0xea>(x, mask, bias);
+  return *reinterpret_cast<const __half2*>(&r);
 }
 __device__ __forceinline__ __half2 h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 __device__ __forceinline__ uint32_t u2(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
@@ -65,14 +80,14 @@ struct WarpState {
   static constexpr int NB = D / 32;
   uint32_t q[NT][NB][4];  // B fragments of S^T: dims 32 b + 8 t + {0,1}, {2,3} / 16, {4,5}, {6,7} / 16 of row g
   uint32_t qsum[NT];      // B fragment of the m's: block sums of row g
-  float s_scale[NT][2];   // rows 2 t, 2 t + 1: softmax scale (log2) times the row's power of two
+  float s_scale[NT][2];   // rows 2 t, 2 t + 1: |softmax scale| (log2) times the row's power of two (its sign is the query's)
   Seen seen[NT][2];
   float m[NT][2], l[NT][2];   // running maximum (log2 units) and this lane's part of the sum, of rows 2 t, 2 t + 1
   float o[NT][2 * NB][4]; // [m-tile i][dims 32 (i / 2) + 4 g + 2 (i % 2) + {0, 1}] x rows 2 t, 2 t + 1: {d0 r0, d0 r1, d1 r0, d1 r1}
 };
 
 // Loads row g's queries; `row` counts the rows of this (request, KV head), n_rows of them.
-template <int D, bool BF, int NT>
+template <int D, int NT>
 __device__ __forceinline__ void load_queries(WarpState<D, NT>& w, const AttnArgs& a, uint32_t kv_head, uint32_t tile0, uint32_t n_rows, uint32_t q0,
                                              int q_len, int kv_len, uint32_t lane) {
   constexpr int NB = D / 32;
@@ -90,8 +105,17 @@ __device__ __forceinline__ void load_queries(WarpState<D, NT>& w, const AttnArgs
     const bool vec = (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-      if (vec) load8<BF, true>(p + 32 * b + 8 * t, x[b]);
-      else load8<BF, false>(p + 32 * b + 8 * t, x[b]);
+      uint4 u;
+      if (vec) {
+        u = *reinterpret_cast<const uint4*>(p + 32 * b + 8 * t);
+      } else {
+        uint32_t h[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) h[i] = p[32 * b + 8 * t + i];
+        u = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+      }
+      if (a.bf) unpack8<true>(u, x[b]);
+      else unpack8<false>(u, x[b]);
 #pragma unroll
       for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[b][i]));
     }
@@ -100,14 +124,14 @@ __device__ __forceinline__ void load_queries(WarpState<D, NT>& w, const AttnArgs
   big = fmaxf(big, __shfl_xor_sync(FULL, big, 2));
   // 2^e <= big: its exponent bits; tiny or zero rows keep e = -126
   const uint32_t ebits = min(max(__float_as_uint(big) & 0x7f800000u, 0x00800000u), 0x7e800000u);
-  const float up = __uint_as_float(0x7f000000u - ebits), down = __uint_as_float(ebits);  // 2^-e, 2^e
+  const float up = __uint_as_float(0x7f000000u - ebits), down = __uint_as_float(ebits), turn = copysignf(up, a.scale_log2);  // 2^-e, 2^e
   float sum[NB];
 #pragma unroll
   for (int b = 0; b < NB; b++) {
     sum[b] = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const __half2 h = __floats2half2_rn(x[b][2 * j] * up, x[b][2 * j + 1] * up);
+      const __half2 h = __floats2half2_rn(x[b][2 * j] * turn, x[b][2 * j + 1] * turn);
       sum[b] += __low2float(h) + __high2float(h);
       w.q[e][b][j] = u2((j & 1) ? __hmul2(h, __float2half2_rn(0.0625f)) : h);
     }
@@ -126,7 +150,8 @@ __device__ __forceinline__ void load_queries(WarpState<D, NT>& w, const AttnArgs
   w.qsum[e] = t < lo_from ? u2(hi) : t < 2 * lo_from ? u2(lo) : 0u;
 #pragma unroll
   for (int c = 0; c < 2; c++) {
-    w.s_scale[e][c] = a.scale_log2 * __shfl_sync(FULL, down, 4 * (2 * t + c));
+    // (never 0: a masked score, -infinity, stays what it is)
+    w.s_scale[e][c] = fmaxf(fabsf(a.scale_log2) * __shfl_sync(FULL, down, 4 * (2 * t + c)), 1e-37f);
     const uint32_t r = row0 + 2 * t + c;
     const int pos = kv_len - q_len + static_cast<int>(r / a.group);
     // (columns without a row see all, so that they ask for no masks; nobody reads them)
@@ -142,11 +167,18 @@ __device__ __forceinline__ void load_queries(WarpState<D, NT>& w, const AttnArgs
   }
 }
 
-// S^T of 16 tokens, the k-th of the unit: K codes at kc (rows of ROW bytes), d and m at kd, km (rows of 2 NB bytes).
-template <int D, int NT>
-__device__ __forceinline__ void scores16(const WarpState<D, NT>& w, const uint8_t* kc, const uint8_t* kd, const uint8_t* km, uint32_t lane, float (&s)[NT][4][4], int k) {
+// Where the k-th 16 tokens of a unit's K or V lie: `part` = the offset of a page's codes, d or m, `row` = bytes of a token of it.
+template <int D, uint32_t PAGE>
+__device__ constexpr uint32_t tile_at(int k, uint32_t row, uint32_t part) {
+  return 16u * k / PAGE * (PAGE * (PoolLayout<D>::TOK / 2)) + part + 16u * k % PAGE * row;
+}
+
+// S^T of the k-th 16 tokens of a unit, not scaled.
+template <int D, int NT, uint32_t PAGE>
+__device__ __forceinline__ void scores16(const WarpState<D, NT>& w, const uint8_t* buf, uint32_t lane, float (&s)[NT][4][4], int k) {
   using L = PoolLayout<D>;
   constexpr int NB = D / 32;
+  const uint8_t *kc = buf + tile_at<D, PAGE>(k, L::ROW, 0), *kd = buf + tile_at<D, PAGE>(k, 2 * NB, L::kd(PAGE)), *km = buf + tile_at<D, PAGE>(k, 2 * NB, L::km(PAGE));
   const uint32_t g = lane >> 2, t = lane & 3, ta = tile_token(g), tb = ta + 8;
   uint32_t wa[NB], wb[NB];
   float da[NB], db[NB];
@@ -173,12 +205,12 @@ __device__ __forceinline__ void scores16(const WarpState<D, NT>& w, const uint8_
   }
 #pragma unroll
   for (int e = 0; e < NT; e++) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, low[4] = {0.f, 0.f, 0.f, 0.f};
-    mma_1688(low, ma, mb, w.qsum[e]);
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, low[4];
+    mma_1688_first(low, ma, mb, w.qsum[e]);
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-      float p[4] = {0.f, 0.f, 0.f, 0.f};
-      mma_16816(p, wa[b] & 0x000f000fu, wb[b] & 0x000f000fu, wa[b] & 0x00f000f0u, wb[b] & 0x00f000f0u, w.q[e][b][0], w.q[e][b][1]);
+      float p[4];
+      mma_16816_first(p, wa[b] & 0x000f000fu, wb[b] & 0x000f000fu, wa[b] & 0x00f000f0u, wb[b] & 0x00f000f0u, w.q[e][b][0], w.q[e][b][1]);
       const uint32_t xa = wa[b] >> 8, xb = wb[b] >> 8;
       mma_16816(p, xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u, w.q[e][b][2], w.q[e][b][3]);
       acc[0] = fmaf(da[b], p[0], acc[0]);
@@ -187,73 +219,60 @@ __device__ __forceinline__ void scores16(const WarpState<D, NT>& w, const uint8_
       acc[3] = fmaf(db[b], p[3], acc[3]);
     }
 #pragma unroll
-    for (int c = 0; c < 4; c++) s[e][k][c] = fmaf(acc[c], 0x1p24f, low[c]) * w.s_scale[e][c & 1];
+    for (int c = 0; c < 4; c++) s[e][k][c] = fmaf(acc[c], 0x1p24f, low[c]);
   }
 }
 
-// O^T += V^T P^T of 16 tokens of which those in [from, to) are the request's (0 and 16 or beyond: all). s: P as S^T fragments.
-template <int D, int NT>
-__device__ __forceinline__ void values16(WarpState<D, NT>& w, const uint8_t* vc, const uint8_t* vd, const uint8_t* vm, uint32_t place, int from, int to,
-                                         uint32_t lane, const float (&s)[NT][4][4], int k) {
+// O^T += V^T P^T of the k-th 16 tokens of a unit. s: P as S^T fragments.
+template <int D, int NT, uint32_t PAGE>
+__device__ __forceinline__ void values16(WarpState<D, NT>& w, const uint8_t* buf, uint32_t lane, const float (&s)[NT][4][4], int k, uint32_t bias) {
   using L = PoolLayout<D>;
   constexpr int NB = D / 32;
   const uint32_t g = lane >> 2, t = lane & 3;
-  // pair 0: MMA columns 2 t, 2 t + 1; pair 1: 2 t + 8, 2 t + 9
-  uint32_t av[2][NB][4];
+  const uint8_t *vc = buf + tile_at<D, PAGE>(k, L::ROW, 0), *vd = buf + tile_at<D, PAGE>(k, 2 * NB, L::kd(PAGE)), *vm = buf + tile_at<D, PAGE>(k, 2 * NB, L::km(PAGE));
+  // [pair 0: MMA columns 2 t, 2 t + 1; pair 1: 2 t + 8, 2 t + 9][first, second token]
+  uint32_t codes[2][2][NB / 2], dw[2][2][NB / 2], mw[2][2][NB / 2];
 #pragma unroll
-  for (int pr = 0; pr < 2; pr++) {
-    const uint32_t ta = tile_token(2 * t + 8 * pr), tb = tile_token(2 * t + 1 + 8 * pr);
-    uint32_t a[NB / 2], b[NB / 2], ad[NB / 2], bd[NB / 2], am[NB / 2], bm[NB / 2];
+  for (int i = 0; i < 4; i++) {
+    const uint32_t tok = tile_token(2 * t + (i & 1) + 8 * (i >> 1));
+    uint32_t(&c)[NB / 2] = codes[i >> 1][i & 1], (&d)[NB / 2] = dw[i >> 1][i & 1], (&m)[NB / 2] = mw[i >> 1][i & 1];
     if constexpr (NB == 4) {
-      const uint2 x = *reinterpret_cast<const uint2*>(vc + ta * L::ROW + L::v16(place + ta, g, 0)), y = *reinterpret_cast<const uint2*>(vc + tb * L::ROW + L::v16(place + tb, g, 0));
-      a[0] = x.x; a[1] = x.y;
-      b[0] = y.x; b[1] = y.y;
-      const uint2 e = *reinterpret_cast<const uint2*>(vd + ta * 8), f = *reinterpret_cast<const uint2*>(vd + tb * 8);
-      ad[0] = e.x; ad[1] = e.y;
-      bd[0] = f.x; bd[1] = f.y;
-      const uint2 i = *reinterpret_cast<const uint2*>(vm + ta * 8), j = *reinterpret_cast<const uint2*>(vm + tb * 8);
-      am[0] = i.x; am[1] = i.y;
-      bm[0] = j.x; bm[1] = j.y;
+      const uint2 x = *reinterpret_cast<const uint2*>(vc + tok * L::ROW + L::v16(tok, g, 0)), e = *reinterpret_cast<const uint2*>(vd + tok * 8),
+                  f = *reinterpret_cast<const uint2*>(vm + tok * 8);
+      c[0] = x.x; c[1] = x.y;
+      d[0] = e.x; d[1] = e.y;
+      m[0] = f.x; m[1] = f.y;
     } else {
-      a[0] = *reinterpret_cast<const uint32_t*>(vc + ta * L::ROW + L::v16(place + ta, g, 0));
-      b[0] = *reinterpret_cast<const uint32_t*>(vc + tb * L::ROW + L::v16(place + tb, g, 0));
-      ad[0] = *reinterpret_cast<const uint32_t*>(vd + ta * 4);
-      bd[0] = *reinterpret_cast<const uint32_t*>(vd + tb * 4);
-      am[0] = *reinterpret_cast<const uint32_t*>(vm + ta * 4);
-      bm[0] = *reinterpret_cast<const uint32_t*>(vm + tb * 4);
-    }
-    if (from > 0 || to < 16) {  // the other places may hold any bits: P is 0 there, the values must be numbers
-      const bool za = static_cast<int>(ta) < from || static_cast<int>(ta) >= to, zb = static_cast<int>(tb) < from || static_cast<int>(tb) >= to;
-#pragma unroll
-      for (int i = 0; i < NB / 2; i++) {
-        ad[i] = za ? 0u : ad[i];
-        am[i] = za ? 0u : am[i];
-        bd[i] = zb ? 0u : bd[i];
-        bm[i] = zb ? 0u : bm[i];
-      }
-    }
-    const __half2 off = __float2half2_rn(-1024.f), off16 = __float2half2_rn(-64.f), sixteenth = __float2half2_rn(0.0625f);
-#pragma unroll
-    for (int bl = 0; bl < NB; bl++) {
-      const uint32_t sel = (bl & 1) ? 0x7632u : 0x5410u;
-      const uint32_t x = prmt(a[bl >> 1], b[bl >> 1], sel), y = x >> 8;
-      const __half2 d = h2(prmt(ad[bl >> 1], bd[bl >> 1], sel)), m = h2(prmt(am[bl >> 1], bm[bl >> 1], sel));
-      // 1024 + q and 1024 + 16 q as f16 numbers
-      const __half2 q0 = __hadd2(h2((x & 0x000f000fu) | 0x64006400u), off), q1 = __hfma2(h2((x & 0x00f000f0u) | 0x64006400u), sixteenth, off16);
-      const __half2 q2 = __hadd2(h2((y & 0x000f000fu) | 0x64006400u), off), q3 = __hfma2(h2((y & 0x00f000f0u) | 0x64006400u), sixteenth, off16);
-      av[pr][bl][0] = u2(__hfma2(q0, d, m));
-      av[pr][bl][1] = u2(__hfma2(q1, d, m));
-      av[pr][bl][2] = u2(__hfma2(q2, d, m));
-      av[pr][bl][3] = u2(__hfma2(q3, d, m));
+      c[0] = *reinterpret_cast<const uint32_t*>(vc + tok * L::ROW + L::v16(tok, g, 0));
+      d[0] = *reinterpret_cast<const uint32_t*>(vd + tok * 4);
+      m[0] = *reinterpret_cast<const uint32_t*>(vm + tok * 4);
     }
   }
+  uint32_t p0[NT], p1[NT];
 #pragma unroll
   for (int e = 0; e < NT; e++) {
-    const uint32_t p0 = movmatrix(pack2<false>(s[e][k][0], s[e][k][1])), p1 = movmatrix(pack2<false>(s[e][k][2], s[e][k][3]));
+    p0[e] = movmatrix(pack2<false>(s[e][k][0], s[e][k][1]));
+    p1[e] = movmatrix(pack2<false>(s[e][k][2], s[e][k][3]));
+  }
+  const __half2 off = __float2half2_rn(-1024.f), off16 = __float2half2_rn(-64.f), sixteenth = __float2half2_rn(0.0625f);
 #pragma unroll
-    for (int bl = 0; bl < NB; bl++) {
-      mma_16816(w.o[e][2 * bl], av[0][bl][0], av[0][bl][1], av[1][bl][0], av[1][bl][1], p0, p1);
-      mma_16816(w.o[e][2 * bl + 1], av[0][bl][2], av[0][bl][3], av[1][bl][2], av[1][bl][3], p0, p1);
+  for (int bl = 0; bl < NB; bl++) {
+    const uint32_t sel = (bl & 1) ? 0x7632u : 0x5410u;
+    uint32_t av[2][4];
+#pragma unroll
+    for (int pr = 0; pr < 2; pr++) {
+      const uint32_t x = prmt(codes[pr][0][bl >> 1], codes[pr][1][bl >> 1], sel), y = x >> 8;
+      const __half2 d = h2(prmt(dw[pr][0][bl >> 1], dw[pr][1][bl >> 1], sel)), m = h2(prmt(mw[pr][0][bl >> 1], mw[pr][1][bl >> 1], sel));
+      // 1024 + q and 1024 + 16 q as f16 numbers, then q
+      av[pr][0] = u2(__hfma2(__hadd2(biased(x, 0x000f000fu, bias), off), d, m));
+      av[pr][1] = u2(__hfma2(__hfma2(biased(x, 0x00f000f0u, bias), sixteenth, off16), d, m));
+      av[pr][2] = u2(__hfma2(__hadd2(biased(y, 0x000f000fu, bias), off), d, m));
+      av[pr][3] = u2(__hfma2(__hfma2(biased(y, 0x00f000f0u, bias), sixteenth, off16), d, m));
+    }
+#pragma unroll
+    for (int e = 0; e < NT; e++) {
+      mma_16816(w.o[e][2 * bl], av[0][0], av[0][1], av[1][0], av[1][1], p0[e], p1[e]);
+      mma_16816(w.o[e][2 * bl + 1], av[0][2], av[0][3], av[1][2], av[1][3], p0[e], p1[e]);
     }
   }
 }
@@ -283,6 +302,7 @@ __device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4]
       for (int i = 1; i < 4; i++) mx[c] = fmaxf(mx[c], fmaxf(s[e][i][c], s[e][i][c + 2]));
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(FULL, mx[c], o));
+      mx[c] *= w.s_scale[e][c];
     }
     if (__any_sync(FULL, mx[0] > w.m[e][0] || mx[1] > w.m[e][1])) {
       float corr[2];
@@ -303,7 +323,7 @@ __device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4]
     for (int i = 0; i < 4; i++)
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        s[e][i][k] = ex2(s[e][i][k] - top[k & 1]);
+        s[e][i][k] = ex2(fmaf(s[e][i][k], w.s_scale[e][k & 1], -top[k & 1]));
         w.l[e][k & 1] += s[e][i][k];
       }
   }
@@ -349,8 +369,10 @@ struct Cursor {
   Request q;
   uint32_t r, head, tile, unit;
 };
+// One unit on (a cursor lies in shared memory, one lane moves it).
 template <int NT>
-__device__ __forceinline__ void next_item(Cursor& c, const AttnArgs& a) {
+__device__ __forceinline__ void advance(Cursor& c, const AttnArgs& a) {
+  if (++c.unit < c.q.units) return;
   c.unit = 0;
   if (++c.tile < c.q.tiles) return;
   c.tile = 0;
@@ -368,9 +390,11 @@ struct Piece {
   unsigned long long start;  // the item's first unit in the line
 };
 
-// Fetches K or V of a unit, one lane per page. ids: lane l has the page id of page `base + l` of the request.
+// Fetches the units of a stretch, one lane per page. ids: lane l has the page id of page `base + l` of the request.
 struct Fetch {
   uint32_t ids, base;
+  const uint8_t* src;  // this lane's page of the unit, K
+  uint32_t pages;      // the unit's pages that are fetched: those that hold keys of [low, kv_len) and have a good id
 };
 __device__ __forceinline__ void load_ids(Fetch& f, const AttnArgs& a, const Cursor& c, uint32_t first_page, uint32_t lane) {
   const uint32_t pages = (static_cast<uint32_t>(c.q.kv_len) + a.pool.page - 1) >> a.pool.log_page;
@@ -378,31 +402,48 @@ __device__ __forceinline__ void load_ids(Fetch& f, const AttnArgs& a, const Curs
   f.ids = 0xffffffffu;
   if (first_page + lane < pages) f.ids = static_cast<uint32_t>(a.page_table[static_cast<size_t>(c.r) * a.table_stride + first_page + lane]);
 }
-// Returns which of the unit's pages are on their way: those that hold keys of [low, kv_len) and have a good id.
+__device__ __forceinline__ void copy_pages(const Fetch& f, const uint8_t* src, uint32_t bytes, uint32_t dst, uint32_t bar, uint32_t lane) {
+  if (lane == 0) mbar_arrive_expect_tx(bar, __popc(f.pages) * bytes);
+  __syncwarp();
+  if (f.pages >> lane & 1)
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + lane * bytes), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
 template <int D>
-__device__ __forceinline__ uint32_t fetch(Fetch& f, const AttnArgs& a, const Cursor& c, uint32_t v, uint32_t dst, uint32_t bar, uint32_t lane) {
-  using L = PoolLayout<D>;
+__device__ __forceinline__ void fetch_keys(Fetch& f, const AttnArgs& a, const Cursor& c, bool new_item, uint32_t bytes, uint32_t dst, uint32_t bar, uint32_t lane) {
   const int key0 = c.q.first() + static_cast<int>(c.unit * UNIT), key = key0 + static_cast<int>(lane << a.pool.log_page);
   const uint32_t page0 = static_cast<uint32_t>(key0) >> a.pool.log_page, n = UNIT >> a.pool.log_page;
-  if (page0 - f.base >= 32) load_ids(f, a, c, page0, lane);
+  if (new_item || page0 - f.base >= 32) load_ids(f, a, c, page0, lane);
   const uint32_t id = __shfl_sync(FULL, f.ids, (page0 - f.base + lane) & 31);
   const bool there = lane < n && key < c.q.kv_len && key + static_cast<int>(a.pool.page) > c.q.low, good = there && id < a.pool.n_pages;
   if (there && !good) note_range(a.err);
-  const uint32_t bytes = a.pool.page * (L::TOK / 2), pages = __ballot_sync(FULL, good);
-  if (lane == 0) mbar_arrive_expect_tx(bar, __popc(pages) * bytes);
-  __syncwarp();
-  if (good) {
-    const uint8_t* src = a.pool.data + (static_cast<size_t>(id) * a.pool.n_kv_head + c.head) * (static_cast<size_t>(a.pool.page) * L::TOK) + v * bytes;
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + lane * bytes), "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
+  f.pages = __ballot_sync(FULL, good);
+  f.src = a.pool.data + (static_cast<size_t>(id) * a.pool.n_kv_head + c.head) * (2 * static_cast<size_t>(bytes));
+  copy_pages(f, f.src, bytes, dst, bar, lane);
+}
+
+// Places of a unit's K or V that hold no key of the request may hold any bits: their d and m become 0, so that the values are
+// numbers (P is 0 there). pages: those that have been fetched; tokens [from, to) are the request's.
+template <int D, uint32_t PAGE>
+__device__ __forceinline__ void clear_scales(uint8_t* buf, uint32_t pages, int from, int to, uint32_t lane) {
+  using L = PoolLayout<D>;
+#pragma unroll
+  for (uint32_t tok = lane; tok < UNIT; tok += 32) {
+    if ((pages >> (tok / PAGE) & 1) && static_cast<int>(tok) >= from && static_cast<int>(tok) < to) continue;
+    uint8_t* at = buf + tok / PAGE * (PAGE * (L::TOK / 2)) + L::kd(PAGE) + tok % PAGE * 2 * L::NB;
+#pragma unroll
+    for (uint32_t i = 0; i < L::NB / 2; i++) {
+      reinterpret_cast<uint32_t*>(at)[i] = 0;
+      reinterpret_cast<uint32_t*>(at + L::km(PAGE) - L::kd(PAGE))[i] = 0;
+    }
   }
-  return pages;
+  fence_proxy_async();  // the next copy into the buffer comes behind these
+  __syncwarp();
 }
 
 // Four dims of an output row.
-template <bool BF>
-__device__ __forceinline__ void store4(uint16_t* p, float a, float b, float c, float d) {
-  const uint32_t x = pack2<BF>(a, b), y = pack2<BF>(c, d);
+__device__ __forceinline__ void store4(bool bf, uint16_t* p, float a, float b, float c, float d) {
+  const uint32_t x = bf ? pack2<true>(a, b) : pack2<false>(a, b), y = bf ? pack2<true>(c, d) : pack2<false>(c, d);
   if ((reinterpret_cast<uintptr_t>(p) & 7) == 0) {
     *reinterpret_cast<uint2*>(p) = make_uint2(x, y);
   } else {
@@ -428,8 +469,8 @@ struct Joined {
   }
 };
 
-template <int D, bool BF, int NT>
-__global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_kernel(const AttnArgs a, float* __restrict__ scratch, uint32_t* __restrict__ counters) {
+template <int D, int NT, uint32_t PAGE>
+__global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_kernel(const __grid_constant__ AttnArgs a, float* __restrict__ scratch, uint32_t* __restrict__ counters) {
   using S = Shape<D, NT>;
   using L = PoolLayout<D>;
   constexpr int NB = D / 32;
@@ -437,6 +478,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
   __shared__ __align__(8) uint64_t bars[NWARP][2];
   __shared__ unsigned long long line[THREADS + 1];  // units before the requests of thread t's part
   __shared__ Piece pieces[NWARP][2];
+  __shared__ Cursor cursors[NWARP][2];               // the unit that is worked on, the unit that is fetched
   __shared__ uint32_t items_s, most_s, last_s;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* buf[2] = {smem + warp * 2 * S::PART, smem + warp * 2 * S::PART + S::PART};
@@ -492,9 +534,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
   const unsigned long long even = (total + n_cta - 1) / n_cta, share = max(even, static_cast<unsigned long long>(NWARP));
   const bool whole = items_s <= n_cta && (most_s + NWARP - 1) / NWARP <= (share + NWARP - 1) / NWARP + 1;
   unsigned long long c0, c1;
-  Cursor cur;
-  cur.r = cur.head = cur.tile = cur.unit = 0;
-  cur.q = Request{};
+  Cursor &cur = cursors[warp][0], &next = cursors[warp][1];
   auto locate = [&](unsigned long long x) {  // x < total
     uint32_t lo = 0, hi = THREADS;
     while (hi - lo > 1) {
@@ -544,64 +584,46 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
   const uint32_t n = static_cast<uint32_t>(c0 + static_cast<unsigned long long>(cta_units) * (warp + 1) / NWARP - x0);
 
   if (n > 0) {
-    locate(x0);
-    Cursor next = cur;  // the unit that is fetched
+    if (lane == 0) {
+      locate(x0);
+      next = cur;
+    }
+    __syncwarp();
+    constexpr uint32_t half = PAGE * (L::TOK / 2), ALL_PAGES = (1u << UNIT / PAGE) - 1;
     Fetch f;
-    load_ids(f, a, next, (next.q.first() + next.unit * UNIT) >> a.pool.log_page, lane);
-    uint32_t pages = fetch<D>(f, a, next, 0, smem_u32(buf[0]), bar[0], lane), next_pages = 0;
-    (void)fetch<D>(f, a, next, 1, smem_u32(buf[1]), bar[1], lane);
+    fetch_keys<D>(f, a, next, true, half, smem_u32(buf[0]), bar[0], lane);
+    copy_pages(f, f.src + half, half, smem_u32(buf[1]), bar[1], lane);
+    uint32_t pages = f.pages;
     WarpState<D, NT> w;
     bool fresh = true, from_start = false, ok = true;
-    const uint32_t lp = a.pool.log_page, page = a.pool.page, half = page * (L::TOK / 2);
     for (uint32_t i = 0; i < n; i++) {
       if (fresh) {
-        load_queries<D, BF, NT>(w, a, cur.head, cur.tile * S::ROWS, cur.q.q_len * a.group, cur.q.q0, cur.q.q_len, cur.q.kv_len, lane);
+        load_queries<D, NT>(w, a, cur.head, cur.tile * S::ROWS, cur.q.q_len * a.group, cur.q.q0, cur.q.q_len, cur.q.kv_len, lane);
         from_start = cur.unit == 0;
         fresh = false;
       }
       const int key0 = cur.q.first() + cur.unit * UNIT, left = cur.q.kv_len - key0;
-      const bool more = i + 1 < n;
-      bool moved = false;
-      if (more) {
-        if (++next.unit == next.q.units) {
-          next_item<NT>(next, a);
-          moved = true;
-        }
-      }
+      const int low = cur.q.low - key0;
+      const bool more = i + 1 < n, ends = cur.unit + 1 == cur.q.units;
+      if (more && lane == 0) advance<NT>(next, a);
       float s[NT][4][4];
       ok = ok && mbar_wait(bar[0], i & 1, WAIT_LIMIT);
+      const bool part = pages != ALL_PAGES || low > 0 || left < static_cast<int>(UNIT);
+      if (part) clear_scales<D, PAGE>(buf[0], pages, 0, UNIT, lane);
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const uint32_t pg = (16 * k) >> lp, place = (16 * k) & (page - 1);
-        const uint8_t* p = buf[0] + pg * half;
-        if (pages >> pg & 1)
-          scores16<D, NT>(w, p + place * L::ROW, p + L::kd(page) + place * 2 * NB, p + L::km(page) + place * 2 * NB, lane, s, k);
-        else
-#pragma unroll
-          for (int e = 0; e < NT; e++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) s[e][k][c] = __int_as_float(0xff800000);
-      }
+      for (int k = 0; k < 4; k++) scores16<D, NT, PAGE>(w, buf[0], lane, s, k);
       __syncwarp();
-      if (more && ok) {
-        if (moved) load_ids(f, a, next, (next.q.first() + next.unit * UNIT) >> lp, lane);
-        next_pages = fetch<D>(f, a, next, 0, smem_u32(buf[0]), bar[0], lane);
-      }
+      if (more && ok) fetch_keys<D>(f, a, next, ends, half, smem_u32(buf[0]), bar[0], lane);
       softmax64<D, NT>(w, s, key0, lane);
       ok = ok && mbar_wait(bar[1], i & 1, WAIT_LIMIT);
+      if (part) clear_scales<D, PAGE>(buf[1], pages, low, left, lane);
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const uint32_t pg = (16 * k) >> lp, place = (16 * k) & (page - 1);
-        if (!(pages >> pg & 1)) continue;
-        const uint8_t* p = buf[1] + pg * half;
-        values16<D, NT>(w, p + place * L::ROW, p + L::kd(page) + place * 2 * NB, p + L::km(page) + place * 2 * NB, place, cur.q.low - key0 - 16 * k, left - 16 * k, lane, s, k);
-      }
+      for (int k = 0; k < 4; k++) values16<D, NT, PAGE>(w, buf[1], lane, s, k, a.bias);
       __syncwarp();
-      if (more && ok) (void)fetch<D>(f, a, next, 1, smem_u32(buf[1]), bar[1], lane);
-      pages = next_pages;
+      if (more && ok) copy_pages(f, f.src + half, half, smem_u32(buf[1]), bar[1], lane);
+      pages = f.pages;
       if (!ok) break;
 
-      const bool ends = cur.unit + 1 == cur.q.units;
       if (ends || !more) {
         // sums over the lanes of a row
 #pragma unroll
@@ -622,7 +644,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
               uint16_t* out = out_row(a, cur.q.q0, cur.head, row);
 #pragma unroll
               for (int b = 0; b < NB; b++)
-                store4<BF>(out + 32 * b + 4 * g, w.o[e][2 * b][c] * inv, w.o[e][2 * b][c + 2] * inv, w.o[e][2 * b + 1][c] * inv, w.o[e][2 * b + 1][c + 2] * inv);
+                store4(a.bf, out + 32 * b + 4 * g, w.o[e][2 * b][c] * inv, w.o[e][2 * b][c + 2] * inv, w.o[e][2 * b + 1][c] * inv, w.o[e][2 * b + 1][c + 2] * inv);
             }
         } else {
           // an item's end goes to memory (the buffers are in use), the stretch's end over the buffers
@@ -641,10 +663,9 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
         }
         fresh = true;
       }
-      if (more) {
-        if (ends) next_item<NT>(cur, a);
-        else cur.unit++;
-      }
+      __syncwarp();
+      if (more && lane == 0) advance<NT>(cur, a);
+      __syncwarp();
     }
     if (!ok) {  // the wait gave up: what is on its way comes before the buffers are given back
       if (lane == 0) reinterpret_cast<volatile uint32_t*>(a.err)[1] = 1;
@@ -686,7 +707,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
       }
       if (all) {
         const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
-        store4<BF>(out_row(a, q0, p.head, row0 + row) + col, j.o.x * inv, j.o.y * inv, j.o.z * inv, j.o.w * inv);
+        store4(a.bf, out_row(a, q0, p.head, row0 + row) + col, j.o.x * inv, j.o.y * inv, j.o.z * inv, j.o.w * inv);
       } else {
         *reinterpret_cast<float4*>(mine_out + row * S::STRIDE + col) = j.o;
         if (col == 0) *reinterpret_cast<float2*>(mine_out + row * S::STRIDE + D) = make_float2(j.m, j.l);
@@ -713,7 +734,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
             j.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(part + col)));
           }
           const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
-          store4<BF>(out_row(a, q0, p.head, row0 + row) + col, j.o.x * inv, j.o.y * inv, j.o.z * inv, j.o.w * inv);
+          store4(a.bf, out_row(a, q0, p.head, row0 + row) + col, j.o.x * inv, j.o.y * inv, j.o.z * inv, j.o.w * inv);
         }
       }
       __syncthreads();
@@ -722,19 +743,28 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
   }
 }
 
-template <int D, bool BF, int NT>
-cudaError_t allow() {
-  return cudaFuncSetAttribute(kv4_attention_kernel<D, BF, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<D, NT>::SMEM));
+// f(kernel, shape) for the instance of (head_dim, rows of an item, page).
+template <typename F>
+cudaError_t with_kernel(uint32_t head_dim, bool two, uint32_t page, F f) {
+  auto by_page = [&](auto d, auto nt) {
+    constexpr int D = decltype(d)::value, NT = decltype(nt)::value;
+    return page == 16 ? f(kv4_attention_kernel<D, NT, 16>, Shape<D, NT>()) : page == 32 ? f(kv4_attention_kernel<D, NT, 32>, Shape<D, NT>()) : f(kv4_attention_kernel<D, NT, 64>, Shape<D, NT>());
+  };
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  if (head_dim == 128) return two ? by_page(std::integral_constant<int, 128>(), I2()) : by_page(std::integral_constant<int, 128>(), I1());
+  return two ? by_page(std::integral_constant<int, 64>(), I2()) : by_page(std::integral_constant<int, 64>(), I1());
 }
 
 }  // namespace
 
 cudaError_t bp_kv4_attention_init(bp_paged_ctx* c) {
-  cudaError_t e;
-  if ((e = allow<128, false, 1>()) != cudaSuccess || (e = allow<128, true, 1>()) != cudaSuccess || (e = allow<64, false, 1>()) != cudaSuccess ||
-      (e = allow<64, true, 1>()) != cudaSuccess || (e = allow<128, false, 2>()) != cudaSuccess || (e = allow<128, true, 2>()) != cudaSuccess ||
-      (e = allow<64, false, 2>()) != cudaSuccess || (e = allow<64, true, 2>()) != cudaSuccess)
-    return e;
+  cudaError_t e = cudaSuccess;
+  for (uint32_t i = 0; i < 12 && e == cudaSuccess; i++)
+    e = with_kernel(i & 1 ? 128 : 64, i & 2, 16u << (i >> 2), [](auto kernel, auto shape) {
+      return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shape.SMEM));
+    });
+  if (e != cudaSuccess) return e;
   // a piece per warp and two per CTA, of the instance that needs most
   const size_t one = 2 * static_cast<size_t>(c->sm_count) * (NWARP + 2);
   const size_t floats = one * Shape<128, 2>::PARTIAL;
@@ -763,14 +793,9 @@ cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, co
   a.table_stride = in.table_stride < (0x7fffffffu >> pool.log_page) ? in.table_stride : (0x7fffffffu >> pool.log_page);
   a.window = in.window;
   a.scale_log2 = in.scale * 1.4426950408889634f;
-  auto go = [&](auto kernel, uint32_t smem, uint32_t ctas) {
-    return bp_launch(true, kernel, dim3(ctas * static_cast<uint32_t>(c->sm_count)), dim3(THREADS), smem, s, a, c->partials, c->counters);
-  };
-  const bool two = a.max_q * a.group > 8;
-  if (head_dim == 128) {
-    if (two) return go(bf ? kv4_attention_kernel<128, true, 2> : kv4_attention_kernel<128, false, 2>, Shape<128, 2>::SMEM, Shape<128, 2>::CTAS);
-    return go(bf ? kv4_attention_kernel<128, true, 1> : kv4_attention_kernel<128, false, 1>, Shape<128, 1>::SMEM, Shape<128, 1>::CTAS);
-  }
-  if (two) return go(bf ? kv4_attention_kernel<64, true, 2> : kv4_attention_kernel<64, false, 2>, Shape<64, 2>::SMEM, Shape<64, 2>::CTAS);
-  return go(bf ? kv4_attention_kernel<64, true, 1> : kv4_attention_kernel<64, false, 1>, Shape<64, 1>::SMEM, Shape<64, 1>::CTAS);
+  a.bias = 0x64006400u;
+  a.bf = bf;
+  return with_kernel(head_dim, a.max_q * a.group > 8, pool.page, [&](auto kernel, auto shape) {
+    return bp_launch(true, kernel, dim3(shape.CTAS * static_cast<uint32_t>(c->sm_count)), dim3(THREADS), shape.SMEM, s, a, c->partials, c->counters);
+  });
 }
