@@ -69,11 +69,6 @@ __device__ __forceinline__ __half2 biased(uint32_t x, uint32_t mask, uint32_t bi
 __device__ __forceinline__ __half2 h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 __device__ __forceinline__ uint32_t u2(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-// Which keys a row sees: j in [lo, hi).
-struct Seen {
-  int lo, hi;
-};
-
 // State of one warp for NT tiles of eight rows.
 template <int D, int NT>
 struct WarpState {
@@ -81,7 +76,6 @@ struct WarpState {
   uint32_t q[NT][NB][4];  // B fragments of S^T: dims 32 b + 8 t + {0,1}, {2,3} / 16, {4,5}, {6,7} / 16 of row g
   uint32_t qsum[NT];      // B fragment of the m's: block sums of row g
   float s_scale[NT][2];   // rows 2 t, 2 t + 1: |softmax scale| (log2) times the row's power of two (its sign is the query's)
-  Seen seen[NT][2];
   float m[NT][2], l[NT][2];   // running maximum (log2 units) and this lane's part of the sum, of rows 2 t, 2 t + 1
   float o[NT][2 * NB][4]; // [m-tile i][dims 32 (i / 2) + 4 g + 2 (i % 2) + {0, 1}] x rows 2 t, 2 t + 1: {d0 r0, d0 r1, d1 r0, d1 r1}
 };
@@ -89,7 +83,7 @@ struct WarpState {
 // Loads row g's queries; `row` counts the rows of this (request, KV head), n_rows of them.
 template <int D, int NT>
 __device__ __forceinline__ void load_queries(WarpState<D, NT>& w, const AttnArgs& a, uint32_t kv_head, uint32_t tile0, uint32_t n_rows, uint32_t q0,
-                                             int q_len, int kv_len, uint32_t lane) {
+                                             uint32_t lane) {
   constexpr int NB = D / 32;
   const uint32_t g = lane >> 2, t = lane & 3;
 #pragma unroll
@@ -152,11 +146,6 @@ __device__ __forceinline__ void load_queries(WarpState<D, NT>& w, const AttnArgs
   for (int c = 0; c < 2; c++) {
     // (never 0: a masked score, -infinity, stays what it is)
     w.s_scale[e][c] = fmaxf(fabsf(a.scale_log2) * __shfl_sync(FULL, down, 4 * (2 * t + c)), 1e-37f);
-    const uint32_t r = row0 + 2 * t + c;
-    const int pos = kv_len - q_len + static_cast<int>(r / a.group);
-    // (columns without a row see all, so that they ask for no masks; nobody reads them)
-    w.seen[e][c].hi = r < n_rows ? min(pos + 1, kv_len) : 0x7fffffff;
-    w.seen[e][c].lo = a.window && r < n_rows ? max(pos + 1 - static_cast<int>(min(a.window, 0x7fffffffu)), 0) : 0;
     w.m[e][c] = NEG_BIG;
     w.l[e][c] = 0.f;
   }
@@ -277,22 +266,27 @@ __device__ __forceinline__ void values16(WarpState<D, NT>& w, const uint8_t* buf
   }
 }
 
-// P, still as the S^T fragments of four tiles, from the scores: masks, maximum, exponentials, sums; O is rescaled.
+// P, still as the S^T fragments of four tiles, from the scores: masks (cut: some row may not see all of the unit, of which `left` keys are there), maximum, exponentials, sums; O is rescaled.
 template <int D, int NT>
-__device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4][4], int key0, uint32_t lane) {
+__device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4][4], bool cut, int left, uint32_t tile0, int q_len, const AttnArgs& a, uint32_t lane) {
   constexpr int NB = D / 32;
   const uint32_t g = lane >> 2;
 #pragma unroll
   for (int e = 0; e < NT; e++) {
-    const bool cut = key0 + static_cast<int>(UNIT) > min(w.seen[e][0].hi, w.seen[e][1].hi) || key0 < max(w.seen[e][0].lo, w.seen[e][1].lo);
-    if (__any_sync(FULL, cut)) {
+    if (cut) {
 #pragma unroll
-      for (int i = 0; i < 4; i++)
+      for (int c = 0; c < 2; c++) {
+        // the keys of the unit that row 2 t + c sees are [lo, hi); columns behind the request's rows are left as they are, nobody reads them
+        const int behind = q_len - 1 - static_cast<int>((tile0 + 8 * e + 2 * (lane & 3) + c) / a.group);  // queries behind this one
+        const int hi = behind < 0 ? left : left - behind, lo = a.window && behind >= 0 ? hi - static_cast<int>(min(a.window, 0x40000000u)) : 0;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const int key = key0 + 16 * i + static_cast<int>(tile_token(g + 8 * (k >> 1)));
-          if (key < w.seen[e][k & 1].lo || key >= w.seen[e][k & 1].hi) s[e][i][k] = __int_as_float(0xff800000);
-        }
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int k = c; k < 4; k += 2) {
+            const int key = 16 * i + static_cast<int>(tile_token(g + 8 * (k >> 1)));
+            if (key < lo || key >= hi) s[e][i][k] = __int_as_float(0xff800000);
+          }
+      }
     }
     float mx[2];
 #pragma unroll
@@ -330,6 +324,7 @@ __device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4]
 }
 
 constexpr uint32_t NWARP = 8, THREADS = 32 * NWARP;
+constexpr uint32_t MOST_SMS = 160;         // SMs that a launch uses at most (a B200 has 148)
 constexpr uint32_t WAIT_LIMIT = 1u << 20;  // polls before a warp gives up on a copy
 
 template <int D, int NT>
@@ -338,7 +333,8 @@ struct Shape {
   static constexpr uint32_t PART = UNIT * PoolLayout<D>::TOK / 2;        // bytes of a unit's K (or V)
   static constexpr uint32_t STRIDE = D + 4;                              // floats of a row of a partial result: o, m, l
   static constexpr uint32_t PARTIAL = ROWS * STRIDE;                     // floats of one
-  static constexpr uint32_t SMEM = NWARP * 2 * PART;
+  static constexpr uint32_t BUFFERS = NWARP * 2 * PART, JOIN = ROWS * 2 * MOST_SMS * 8 + THREADS * 16;  // what joining an item over all CTAs takes
+  static constexpr uint32_t SMEM = BUFFERS > JOIN ? BUFFERS : JOIN;
   static constexpr int CTAS = NT == 1 || D == 64 ? 2 : 1;                // per SM: two where 128 registers do
   static_assert(PARTIAL * 4 <= 2 * PART, "a warp's partial result goes over its buffers");
 };
@@ -369,10 +365,9 @@ struct Cursor {
   Request q;
   uint32_t r, head, tile, unit;
 };
-// One unit on (a cursor lies in shared memory, one lane moves it).
+// The next item (a cursor lies in shared memory, one lane moves it).
 template <int NT>
-__device__ __forceinline__ void advance(Cursor& c, const AttnArgs& a) {
-  if (++c.unit < c.q.units) return;
+__device__ __forceinline__ void next_item(Cursor& c, const AttnArgs& a) {
   c.unit = 0;
   if (++c.tile < c.q.tiles) return;
   c.tile = 0;
@@ -390,18 +385,14 @@ struct Piece {
   unsigned long long start;  // the item's first unit in the line
 };
 
-// Fetches the units of a stretch, one lane per page. ids: lane l has the page id of page `base + l` of the request.
+// The unit that is fetched, one lane per page.
 struct Fetch {
-  uint32_t ids, base;
-  const uint8_t* src;  // this lane's page of the unit, K
-  uint32_t pages;      // the unit's pages that are fetched: those that hold keys of [low, kv_len) and have a good id
+  int key0, kv_len, low;
+  uint32_t rem;          // units of the item from this one on
+  uint32_t ids, base;    // ids: lane l has the page id of page `base + l` of the request
+  const uint8_t* src;    // this lane's page, K
+  uint32_t pages;        // those that are fetched: they hold keys of [low, kv_len) and have a good id
 };
-__device__ __forceinline__ void load_ids(Fetch& f, const AttnArgs& a, const Cursor& c, uint32_t first_page, uint32_t lane) {
-  const uint32_t pages = (static_cast<uint32_t>(c.q.kv_len) + a.pool.page - 1) >> a.pool.log_page;
-  f.base = first_page;
-  f.ids = 0xffffffffu;
-  if (first_page + lane < pages) f.ids = static_cast<uint32_t>(a.page_table[static_cast<size_t>(c.r) * a.table_stride + first_page + lane]);
-}
 __device__ __forceinline__ void copy_pages(const Fetch& f, const uint8_t* src, uint32_t bytes, uint32_t dst, uint32_t bar, uint32_t lane) {
   if (lane == 0) mbar_arrive_expect_tx(bar, __popc(f.pages) * bytes);
   __syncwarp();
@@ -409,17 +400,33 @@ __device__ __forceinline__ void copy_pages(const Fetch& f, const uint8_t* src, u
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + lane * bytes), "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
 }
-template <int D>
-__device__ __forceinline__ void fetch_keys(Fetch& f, const AttnArgs& a, const Cursor& c, bool new_item, uint32_t bytes, uint32_t dst, uint32_t bar, uint32_t lane) {
-  const int key0 = c.q.first() + static_cast<int>(c.unit * UNIT), key = key0 + static_cast<int>(lane << a.pool.log_page);
-  const uint32_t page0 = static_cast<uint32_t>(key0) >> a.pool.log_page, n = UNIT >> a.pool.log_page;
-  if (new_item || page0 - f.base >= 32) load_ids(f, a, c, page0, lane);
+template <uint32_t PAGE>
+__device__ __forceinline__ void load_ids(Fetch& f, const AttnArgs& a, uint32_t r, uint32_t lane) {
+  f.base = static_cast<uint32_t>(f.key0) / PAGE;
+  f.ids = 0xffffffffu;
+  if (f.base + lane < (static_cast<uint32_t>(f.kv_len) + PAGE - 1) / PAGE) f.ids = static_cast<uint32_t>(a.page_table[static_cast<size_t>(r) * a.table_stride + f.base + lane]);
+}
+template <uint32_t PAGE>
+__device__ __forceinline__ void start_item(Fetch& f, const AttnArgs& a, const Cursor& c, uint32_t lane) {
+  f.key0 = c.q.first() + static_cast<int>(c.unit * UNIT);
+  f.kv_len = c.q.kv_len;
+  f.low = c.q.low;
+  f.rem = c.q.units - c.unit;
+  f.src = a.pool.data;
+  load_ids<PAGE>(f, a, c.r, lane);
+}
+template <int D, uint32_t PAGE>
+__device__ __forceinline__ void fetch_keys(Fetch& f, const AttnArgs& a, const Cursor& c, uint32_t dst, uint32_t bar, uint32_t lane) {
+  constexpr uint32_t N = UNIT / PAGE, BYTES = PAGE * (PoolLayout<D>::TOK / 2);
+  const uint32_t page0 = static_cast<uint32_t>(f.key0) / PAGE;
+  if (page0 - f.base >= 32) load_ids<PAGE>(f, a, c.r, lane);
   const uint32_t id = __shfl_sync(FULL, f.ids, (page0 - f.base + lane) & 31);
-  const bool there = lane < n && key < c.q.kv_len && key + static_cast<int>(a.pool.page) > c.q.low, good = there && id < a.pool.n_pages;
+  const int key = f.key0 + static_cast<int>(lane * PAGE);
+  const bool there = lane < N && key < f.kv_len && key + static_cast<int>(PAGE) > f.low, good = there && id < a.pool.n_pages;
   if (there && !good) note_range(a.err);
   f.pages = __ballot_sync(FULL, good);
-  f.src = a.pool.data + (static_cast<size_t>(id) * a.pool.n_kv_head + c.head) * (2 * static_cast<size_t>(bytes));
-  copy_pages(f, f.src, bytes, dst, bar, lane);
+  f.src = a.pool.data + (static_cast<uint64_t>(id) * a.pool.n_kv_head + c.head) * (2 * BYTES);
+  copy_pages(f, f.src, BYTES, dst, bar, lane);
 }
 
 // Places of a unit's K or V that hold no key of the request may hold any bits: their d and m become 0, so that the values are
@@ -457,6 +464,22 @@ __device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, int q0, uint32_t
   return a.out.data + static_cast<int64_t>(q0 + row / a.group) * a.out.tok + static_cast<int64_t>(head * a.group + row % a.group) * a.out.head;
 }
 
+// The rows of a piece's item.
+struct Item {
+  int q0;
+  uint32_t row0, rows, cols;  // cols: fours of values of all rows
+};
+template <int D, int NT>
+__device__ __forceinline__ Item item_of(const AttnArgs& a, const Piece& p) {
+  const Request q = request<NT>(a, p.r, false);
+  const uint32_t row0 = p.tile * 8 * NT, rows = min(8u * NT, static_cast<uint32_t>(q.q_len) * a.group - row0);
+  return Item{q.q0, row0, rows, rows * (D / 4)};
+}
+// An item whose pieces lie in several CTAs: which of this CTA's pieces is one, where it begins, over how many CTAs it goes.
+struct Join {
+  uint32_t piece, first_cta, n, last;
+};
+
 // Pieces of one item, given by `at(i)`, i = from, from + step, ... < n: the running result of four dims of one row.
 struct Joined {
   float m, l;
@@ -479,7 +502,9 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
   __shared__ unsigned long long line[THREADS + 1];  // units before the requests of thread t's part
   __shared__ Piece pieces[NWARP][2];
   __shared__ Cursor cursors[NWARP][2];               // the unit that is worked on, the unit that is fetched
-  __shared__ uint32_t items_s, most_s, last_s;
+  __shared__ unsigned long long plan[3];             // the CTA's stretch [0, 1) of the line; units of a stretch
+  __shared__ Join joins[2];
+  __shared__ uint32_t items_s, most_s;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* buf[2] = {smem + warp * 2 * S::PART, smem + warp * 2 * S::PART + S::PART};
   const uint32_t bar[2] = {smem_u32(&bars[warp][0]), smem_u32(&bars[warp][1])};
@@ -579,33 +604,43 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
     c1 = min(c0 + share, total);
   }
   if (c0 >= c1) return;  // (all threads)
-  const uint32_t cta_units = static_cast<uint32_t>(c1 - c0);
-  const unsigned long long x0 = c0 + static_cast<unsigned long long>(cta_units) * warp / NWARP;
-  const uint32_t n = static_cast<uint32_t>(c0 + static_cast<unsigned long long>(cta_units) * (warp + 1) / NWARP - x0);
+  if (threadIdx.x == 0) {
+    plan[0] = c0;
+    plan[1] = c1;
+    plan[2] = share;
+  }
+  const uint32_t cta_units = static_cast<uint32_t>(c1 - c0), begin = static_cast<uint32_t>(static_cast<unsigned long long>(cta_units) * warp / NWARP);
+  const uint32_t n = static_cast<uint32_t>(static_cast<unsigned long long>(cta_units) * (warp + 1) / NWARP) - begin;
 
+  __syncthreads();
   if (n > 0) {
     if (lane == 0) {
-      locate(x0);
+      locate(c0 + begin);
       next = cur;
     }
     __syncwarp();
     constexpr uint32_t half = PAGE * (L::TOK / 2), ALL_PAGES = (1u << UNIT / PAGE) - 1;
     Fetch f;
-    fetch_keys<D>(f, a, next, true, half, smem_u32(buf[0]), bar[0], lane);
+    start_item<PAGE>(f, a, next, lane);
+    fetch_keys<D, PAGE>(f, a, next, smem_u32(buf[0]), bar[0], lane);
     copy_pages(f, f.src + half, half, smem_u32(buf[1]), bar[1], lane);
-    uint32_t pages = f.pages;
     WarpState<D, NT> w;
     bool fresh = true, from_start = false, ok = true;
+    uint32_t first = 0;  // of this piece; cur.unit is its place in the item
     for (uint32_t i = 0; i < n; i++) {
       if (fresh) {
-        load_queries<D, NT>(w, a, cur.head, cur.tile * S::ROWS, cur.q.q_len * a.group, cur.q.q0, cur.q.q_len, cur.q.kv_len, lane);
+        load_queries<D, NT>(w, a, cur.head, cur.tile * S::ROWS, cur.q.q_len * a.group, cur.q.q0, lane);
         from_start = cur.unit == 0;
+        first = i;
         fresh = false;
       }
-      const int key0 = cur.q.first() + cur.unit * UNIT, left = cur.q.kv_len - key0;
-      const int low = cur.q.low - key0;
-      const bool more = i + 1 < n, ends = cur.unit + 1 == cur.q.units;
-      if (more && lane == 0) advance<NT>(next, a);
+      const int key0 = f.key0, left = f.kv_len - key0, low = f.low - key0;
+      const uint32_t pages = f.pages;
+      const bool more = i + 1 < n, ends = f.rem == 1;
+      if (more && !ends) {
+        f.key0 += UNIT;
+        f.rem--;
+      }
       float s[NT][4][4];
       ok = ok && mbar_wait(bar[0], i & 1, WAIT_LIMIT);
       const bool part = pages != ALL_PAGES || low > 0 || left < static_cast<int>(UNIT);
@@ -613,15 +648,22 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
 #pragma unroll
       for (int k = 0; k < 4; k++) scores16<D, NT, PAGE>(w, buf[0], lane, s, k);
       __syncwarp();
-      if (more && ok) fetch_keys<D>(f, a, next, ends, half, smem_u32(buf[0]), bar[0], lane);
-      softmax64<D, NT>(w, s, key0, lane);
+      if (more && ok) {
+        if (ends) {
+          if (lane == 0) next_item<NT>(next, a);
+          __syncwarp();
+          start_item<PAGE>(f, a, next, lane);
+        }
+        fetch_keys<D, PAGE>(f, a, next, smem_u32(buf[0]), bar[0], lane);
+      }
+      const int q_len = cur.q.q_len;
+      softmax64<D, NT>(w, s, left - static_cast<int>(UNIT) < q_len - 1 || (a.window && left > static_cast<int>(min(a.window, 0x40000000u))), left, cur.tile * S::ROWS, q_len, a, lane);
       ok = ok && mbar_wait(bar[1], i & 1, WAIT_LIMIT);
       if (part) clear_scales<D, PAGE>(buf[1], pages, low, left, lane);
 #pragma unroll
       for (int k = 0; k < 4; k++) values16<D, NT, PAGE>(w, buf[1], lane, s, k, a.bias);
       __syncwarp();
       if (more && ok) copy_pages(f, f.src + half, half, smem_u32(buf[1]), bar[1], lane);
-      pages = f.pages;
       if (!ok) break;
 
       if (ends || !more) {
@@ -659,13 +701,15 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
                 *reinterpret_cast<float4*>(p + 32 * b + 4 * g) = make_float4(w.o[e][2 * b][c], w.o[e][2 * b][c + 2], w.o[e][2 * b + 1][c], w.o[e][2 * b + 1][c + 2]);
               if (g == 0) *reinterpret_cast<float2*>(p + D) = make_float2(w.m[e][c], w.l[e][c]);
             }
-          if (lane == 0) pieces[warp][ends ? 0 : 1] = Piece{1, cur.r, cur.head, cur.tile, cur.q.units, x0 + i - cur.unit};
+          if (lane == 0) pieces[warp][ends ? 0 : 1] = Piece{1, cur.r, cur.head, cur.tile, cur.q.units, plan[0] + begin + first - cur.unit};
         }
         fresh = true;
       }
-      __syncwarp();
-      if (more && lane == 0) advance<NT>(cur, a);
-      __syncwarp();
+      if (more && ends) {
+        __syncwarp();
+        if (lane == 0) cur = next;
+        __syncwarp();
+      }
     }
     if (!ok) {  // the wait gave up: what is on its way comes before the buffers are given back
       if (lane == 0) reinterpret_cast<volatile uint32_t*>(a.err)[1] = 1;
@@ -675,8 +719,9 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
   }
   __syncthreads();
 
-  // ---- the CTA's pieces ----
+  // ---- the CTA's pieces: joined; items that lie in this CTA alone are written ----
   float* exchange = scratch + static_cast<size_t>(gridDim.x) * NWARP * S::PARTIAL;
+  uint32_t n_joins = 0;
   for (uint32_t i = 0; i < 2 * NWARP;) {
     const Piece& p = pieces[i >> 1][i & 1];
     if (!p.used) {
@@ -690,13 +735,11 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
       if (o.start != p.start) break;
       end = k + 1;
     }
-    const int q0 = max(a.q_start[p.r], 0);
-    const uint32_t n_rows = static_cast<uint32_t>(min(max(min(a.q_start[p.r + 1], static_cast<int>(a.total_q)) - q0, 0), static_cast<int>(a.max_q))) * a.group;
-    const uint32_t row0 = p.tile * S::ROWS, rows = min(S::ROWS, n_rows - row0), cols = rows * (D / 4);
-    const bool all = p.start >= c0 && p.start + p.units <= c1;
-    const uint32_t first_cta = all ? 0 : static_cast<uint32_t>(p.start / share), n_parts = all ? 1 : static_cast<uint32_t>((p.start + p.units - 1) / share) - first_cta + 1;
+    const Item it = item_of<D, NT>(a, p);
+    const bool all = p.start >= plan[0] && p.start + p.units <= plan[1];
+    const uint32_t first_cta = all ? 0 : static_cast<uint32_t>(p.start / plan[2]);
     float* mine_out = exchange + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PARTIAL;
-    for (uint32_t x = threadIdx.x; x < cols; x += THREADS) {
+    for (uint32_t x = threadIdx.x; x < it.cols; x += THREADS) {
       const uint32_t row = x / (D / 4), col = x % (D / 4) * 4;
       Joined j{NEG_BIG, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
       for (uint32_t k = i; k < end; k++) {
@@ -707,39 +750,89 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
       }
       if (all) {
         const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
-        store4(a.bf, out_row(a, q0, p.head, row0 + row) + col, j.o.x * inv, j.o.y * inv, j.o.z * inv, j.o.w * inv);
+        store4(a.bf, out_row(a, it.q0, p.head, it.row0 + row) + col, j.o.x * inv, j.o.y * inv, j.o.z * inv, j.o.w * inv);
       } else {
         *reinterpret_cast<float4*>(mine_out + row * S::STRIDE + col) = j.o;
         if (col == 0) *reinterpret_cast<float2*>(mine_out + row * S::STRIDE + D) = make_float2(j.m, j.l);
       }
     }
-    if (!all) {
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        const uint32_t seen = atomicAdd(&counters[first_cta], 1u);
-        last_s = seen == n_parts - 1;
-        if (last_s) counters[first_cta] = 0;  // for the next launch
-        __threadfence();
-      }
-      __syncthreads();
-      if (last_s) {
-        for (uint32_t x = threadIdx.x; x < cols; x += THREADS) {
-          const uint32_t row = x / (D / 4), col = x % (D / 4) * 4;
-          Joined j{NEG_BIG, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-#pragma unroll 4
-          for (uint32_t k = 0; k < n_parts; k++) {
-            const float* part = exchange + static_cast<size_t>(2 * (first_cta + k) + (k == 0)) * S::PARTIAL + row * S::STRIDE;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + D));
-            j.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(part + col)));
-          }
-          const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
-          store4(a.bf, out_row(a, q0, p.head, row0 + row) + col, j.o.x * inv, j.o.y * inv, j.o.z * inv, j.o.w * inv);
-        }
-      }
-      __syncthreads();
+    if (!all) {  // an item that began before the stretch, one that goes on behind it
+      if (threadIdx.x == 0) joins[n_joins] = Join{i, first_cta, static_cast<uint32_t>((p.start + p.units - 1) / plan[2]) - first_cta + 1, 0};
+      n_joins++;
     }
     i = end;
+  }
+  if (n_joins == 0) return;  // (all threads)
+
+  // ---- items of several CTAs: the one that comes last joins them ----
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x < n_joins) {
+    Join& j = joins[threadIdx.x];
+    j.last = atomicAdd(&counters[j.first_cta], 1u) == j.n - 1;
+    if (j.last) counters[j.first_cta] = 0;  // for the next launch
+    __threadfence();
+  }
+  __syncthreads();
+  for (uint32_t q = 0; q < n_joins; q++) {
+    if (!joins[q].last) continue;
+    const Piece& p = pieces[joins[q].piece >> 1][joins[q].piece & 1];
+    const Item it = item_of<D, NT>(a, p);
+    const uint32_t first_cta = joins[q].first_cta, n_parts = joins[q].n, rows = it.rows, cols = it.cols;
+    // weights of the pieces, then their sum: `ways` threads per four dims, each a part of the pieces, all loads on their way at once
+    float2* ml = reinterpret_cast<float2*>(smem);
+    const float* from = exchange + static_cast<size_t>(2 * first_cta) * S::PARTIAL;
+    for (uint32_t x = threadIdx.x; x < rows * n_parts; x += THREADS) {
+      const uint32_t k = x / rows, row = x % rows;
+      ml[row * n_parts + k] = __ldcg(reinterpret_cast<const float2*>(from + (2 * k + (k == 0)) * S::PARTIAL + row * S::STRIDE + D));
+    }
+    __syncthreads();
+    for (uint32_t row = warp; row < rows; row += NWARP) {
+      float m = NEG_BIG, l = 0.f;
+      for (uint32_t k = lane; k < n_parts; k += 32) m = fmaxf(m, ml[row * n_parts + k].x);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
+      for (uint32_t k = lane; k < n_parts; k += 32) {
+        const float2 e = ml[row * n_parts + k];
+        const float weight = ex2(e.x - m);
+        l += weight * e.y;
+        ml[row * n_parts + k].x = weight;
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(FULL, l, o);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      __syncwarp();
+      for (uint32_t k = lane; k < n_parts; k += 32) ml[row * n_parts + k].x *= inv;
+    }
+    __syncthreads();
+    const uint32_t ways = cols <= THREADS / 8 ? 8 : cols <= THREADS / 4 ? 4 : cols <= THREADS / 2 ? 2 : 1;
+    float4* sums = reinterpret_cast<float4*>(ml + ((rows * n_parts + 1) & ~1u));
+    for (uint32_t x = threadIdx.x; x < cols * ways; x += THREADS) {
+      const uint32_t way = x / cols, c = x % cols, row = c / (D / 4), col = c % (D / 4) * 4;
+      const float* part = from + row * S::STRIDE + col;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (uint32_t k = way; k < n_parts; k += ways) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(part + (2 * k + (k == 0)) * S::PARTIAL));
+        const float weight = ml[row * n_parts + k].x;
+        o = make_float4(fmaf(v.x, weight, o.x), fmaf(v.y, weight, o.y), fmaf(v.z, weight, o.z), fmaf(v.w, weight, o.w));
+      }
+      if (ways == 1) store4(a.bf, out_row(a, it.q0, p.head, it.row0 + row) + col, o.x, o.y, o.z, o.w);
+      else sums[x] = o;
+    }
+    if (ways > 1) {
+      __syncthreads();
+      if (threadIdx.x < cols) {
+        const uint32_t row = threadIdx.x / (D / 4), col = threadIdx.x % (D / 4) * 4;
+        float4 o = sums[threadIdx.x];
+        for (uint32_t k = 1; k < ways; k++) {
+          const float4 v = sums[k * cols + threadIdx.x];
+          o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+        }
+        store4(a.bf, out_row(a, it.q0, p.head, it.row0 + row) + col, o.x, o.y, o.z, o.w);
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -766,13 +859,14 @@ cudaError_t bp_kv4_attention_init(bp_paged_ctx* c) {
     });
   if (e != cudaSuccess) return e;
   // a piece per warp and two per CTA, of the instance that needs most
-  const size_t one = 2 * static_cast<size_t>(c->sm_count) * (NWARP + 2);
+  c->attn_sms = c->sm_count < static_cast<int>(MOST_SMS) ? c->sm_count : MOST_SMS;
+  const size_t one = 2 * static_cast<size_t>(c->attn_sms) * (NWARP + 2);
   const size_t floats = one * Shape<128, 2>::PARTIAL;
   e = cudaMalloc(&c->partials, floats * sizeof(float));
   if (e != cudaSuccess) return e;
-  e = cudaMalloc(&c->counters, 2 * static_cast<size_t>(c->sm_count) * sizeof(uint32_t));
+  e = cudaMalloc(&c->counters, 2 * static_cast<size_t>(c->attn_sms) * sizeof(uint32_t));
   if (e != cudaSuccess) return e;
-  return cudaMemset(c->counters, 0, 2 * static_cast<size_t>(c->sm_count) * sizeof(uint32_t));
+  return cudaMemset(c->counters, 0, 2 * static_cast<size_t>(c->attn_sms) * sizeof(uint32_t));
 }
 
 cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, const Pool& pool, uint32_t head_dim, const bp_kv4_attn& in) {
@@ -796,6 +890,6 @@ cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, co
   a.bias = 0x64006400u;
   a.bf = bf;
   return with_kernel(head_dim, a.max_q * a.group > 8, pool.page, [&](auto kernel, auto shape) {
-    return bp_launch(true, kernel, dim3(shape.CTAS * static_cast<uint32_t>(c->sm_count)), dim3(THREADS), shape.SMEM, s, a, c->partials, c->counters);
+    return bp_launch(true, kernel, dim3(shape.CTAS * c->attn_sms), dim3(THREADS), shape.SMEM, s, a, c->partials, c->counters);
   });
 }

@@ -14,6 +14,7 @@
 struct bp_paged_ctx {
   int device;
   int sm_count;
+  uint32_t attn_sms;   // of them, those that split attention uses
   int status;          // latched: BP_ERR_DEVICE_LOST or BP_ERR_TIMEOUT
   uint32_t* err_host;  // pinned, mapped: [0] a token or page out of range, [1] a bounded wait gave up
   uint32_t* err_dev;   // device alias
