@@ -39,6 +39,7 @@ struct AttnArgs {
   float scale_log2;
   uint32_t bias;  // 0x64006400: two f16 numbers 1024
   uint32_t bf;    // activations are bfloat16
+  uint32_t q_vec; // rows of q are 16-byte aligned
 };
 
 // The token of a 16-token tile that a lane's MMA row r holds. K rows 2 j and 2 j + 1 then differ in parity and the values of
@@ -80,40 +81,54 @@ struct WarpState {
   float o[NT][2 * NB][4]; // [m-tile i][dims 32 (i / 2) + 4 g + 2 (i % 2) + {0, 1}] x rows 2 t, 2 t + 1: {d0 r0, d0 r1, d1 r0, d1 r1}
 };
 
-// Loads row g's queries; `row` counts the rows of this (request, KV head), n_rows of them.
+// Row g's queries as they are in memory, then as fragments. Rows of this (request, KV head) are counted from tile0, n_rows of them.
 template <int D, int NT>
-__device__ __forceinline__ void load_queries(WarpState<D, NT>& w, const AttnArgs& a, uint32_t kv_head, uint32_t tile0, uint32_t n_rows, uint32_t q0,
-                                             uint32_t lane) {
+struct RawQueries {
+  uint4 u[NT][D / 32];
+};
+template <int D, int NT>
+__device__ __forceinline__ void ask_queries(RawQueries<D, NT>& raw, const AttnArgs& a, uint32_t kv_head, uint32_t tile0, uint32_t n_rows, uint32_t q0, uint32_t lane) {
+#pragma unroll
+  for (int e = 0; e < NT; e++) {
+    const uint32_t r = min(tile0 + 8 * e + (lane >> 2), n_rows - 1);
+    const uint16_t* p = a.q.data + static_cast<int64_t>(q0 + r / a.group) * a.q.tok + static_cast<int64_t>(kv_head * a.group + r % a.group) * a.q.head + 8 * (lane & 3);
+    if (a.q_vec) {
+#pragma unroll
+      for (int b = 0; b < D / 32; b++) raw.u[e][b] = *reinterpret_cast<const uint4*>(p + 32 * b);
+    } else {
+#pragma unroll
+      for (int b = 0; b < D / 32; b++) {
+        uint32_t h[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) h[i] = p[32 * b + i];
+        raw.u[e][b] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+      }
+    }
+  }
+}
+template <int D, int NT>
+__device__ __forceinline__ void set_queries(WarpState<D, NT>& w, RawQueries<D, NT>& raw, const AttnArgs& a, uint32_t tile0, uint32_t n_rows, uint32_t lane) {
   constexpr int NB = D / 32;
   const uint32_t g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int e = 0; e < NT; e++) {
   const uint32_t row0 = tile0 + 8 * e, row = row0 + g;
   float x[NB][8], big = 0.f;
+  if (row >= n_rows) {
+#pragma unroll
+    for (int b = 0; b < NB; b++) raw.u[e][b] = make_uint4(0, 0, 0, 0);
+  }
+  if (a.bf) {
+#pragma unroll
+    for (int b = 0; b < NB; b++) unpack8<true>(raw.u[e][b], x[b]);
+  } else {
+#pragma unroll
+    for (int b = 0; b < NB; b++) unpack8<false>(raw.u[e][b], x[b]);
+  }
 #pragma unroll
   for (int b = 0; b < NB; b++)
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[b][i] = 0.f;
-  if (row < n_rows) {
-    const uint16_t* p = a.q.data + static_cast<int64_t>(q0 + row / a.group) * a.q.tok + static_cast<int64_t>(kv_head * a.group + row % a.group) * a.q.head;
-    const bool vec = (reinterpret_cast<uintptr_t>(p) & 15) == 0;
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-      uint4 u;
-      if (vec) {
-        u = *reinterpret_cast<const uint4*>(p + 32 * b + 8 * t);
-      } else {
-        uint32_t h[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) h[i] = p[32 * b + 8 * t + i];
-        u = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-      }
-      if (a.bf) unpack8<true>(u, x[b]);
-      else unpack8<false>(u, x[b]);
-#pragma unroll
-      for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[b][i]));
-    }
-  }
+    for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[b][i]));
   big = fmaxf(big, __shfl_xor_sync(FULL, big, 1));
   big = fmaxf(big, __shfl_xor_sync(FULL, big, 2));
   // 2^e <= big: its exponent bits; tiny or zero rows keep e = -126
@@ -323,40 +338,41 @@ __device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4]
   }
 }
 
-constexpr uint32_t NWARP = 8, THREADS = 32 * NWARP;
-constexpr uint32_t MOST_SMS = 160;         // SMs that a launch uses at most (a B200 has 148)
 constexpr uint32_t WAIT_LIMIT = 1u << 20;  // polls before a warp gives up on a copy
 
+// One CTA per SM. A warp fetches ahead into RING buffers, K and V of its units in turn: one is worked on, the others are on
+// their way. With two (16 warps of 128 registers) the buffers in flight did not cover the latency of a loaded memory.
 template <int D, int NT>
 struct Shape {
   static constexpr uint32_t ROWS = 8 * NT;                               // rows of an item
+  static constexpr uint32_t NWARP = D == 128 ? (NT == 1 ? 12 : 8) : (NT == 1 ? 16 : 12), THREADS = 32 * NWARP;
+  static constexpr uint32_t RING = D == 128 && NT == 1 ? 3 : 4;
   static constexpr uint32_t PART = UNIT * PoolLayout<D>::TOK / 2;        // bytes of a unit's K (or V)
   static constexpr uint32_t STRIDE = D + 4;                              // floats of a row of a partial result: o, m, l
   static constexpr uint32_t PARTIAL = ROWS * STRIDE;                     // floats of one
-  static constexpr uint32_t BUFFERS = NWARP * 2 * PART, JOIN = ROWS * 2 * MOST_SMS * 8 + THREADS * 16;  // what joining an item over all CTAs takes
-  static constexpr uint32_t SMEM = BUFFERS > JOIN ? BUFFERS : JOIN;
-  static constexpr int CTAS = NT == 1 || D == 64 ? 2 : 1;                // per SM: two where 128 registers do
-  static_assert(PARTIAL * 4 <= 2 * PART, "a warp's partial result goes over its buffers");
+  static constexpr uint32_t SMEM = NWARP * RING * PART;
+  static_assert(PARTIAL * 4 <= RING * PART && 2 * NWARP <= 32, "a partial result goes over its warp's buffers; a lane per piece");
 };
 
 // What one request asks for.
 struct Request {
-  int q0, q_len, kv_len, low;    // low: no query sees a key before it
+  int q0, q_len, kv_len, low;  // low: no query sees a key before it
+  uint32_t units, tiles;       // units of 64 keys of an item; items per KV head (none without keys: there are only zeros to write)
   __device__ int first() const { return low & ~static_cast<int>(UNIT - 1); }
-  uint32_t units, tiles;         // units of 64 keys of an item; items per KV head
 };
 template <int NT>
 __device__ __forceinline__ Request request(const AttnArgs& a, uint32_t r, bool report) {
   Request q;
-  q.q0 = max(a.q_start[r], 0);
-  const int given_q = max(min(a.q_start[r + 1], static_cast<int>(a.total_q)) - q.q0, 0), given_kv = max(a.kv_len[r], 0);
+  const int start = a.q_start[r], stop = a.q_start[r + 1], keys = a.kv_len[r];
+  q.q0 = max(start, 0);
+  const int given_q = max(min(stop, static_cast<int>(a.total_q)) - q.q0, 0), given_kv = max(keys, 0);
   q.q_len = min(given_q, static_cast<int>(a.max_q));
   q.kv_len = min(given_kv, static_cast<int>(min(a.max_kv, a.table_stride << a.pool.log_page)));
   if (report && (given_q > q.q_len || given_kv > q.kv_len)) note_range(a.err);
   const int from = a.window ? q.kv_len - q.q_len + 1 - static_cast<int>(min(a.window, 0x40000000u)) : 0;
   q.low = max(min(from, q.kv_len), 0);
-  q.units = max((static_cast<uint32_t>(q.kv_len - q.first()) + UNIT - 1) / UNIT, 1u);  // (an item without keys still has its zeros to write)
-  q.tiles = (static_cast<uint32_t>(q.q_len) * a.group + 8 * NT - 1) / (8 * NT);
+  q.units = (static_cast<uint32_t>(q.kv_len - q.first()) + UNIT - 1) / UNIT;
+  q.tiles = q.kv_len ? (static_cast<uint32_t>(q.q_len) * a.group + 8 * NT - 1) / (8 * NT) : 0;
   return q;
 }
 
@@ -365,9 +381,9 @@ struct Cursor {
   Request q;
   uint32_t r, head, tile, unit;
 };
-// The next item (a cursor lies in shared memory, one lane moves it).
+// The next item (a cursor lies in shared memory, one lane moves it). known: the requests, or null if there are too many.
 template <int NT>
-__device__ __forceinline__ void next_item(Cursor& c, const AttnArgs& a) {
+__device__ __forceinline__ void next_item(Cursor& c, const AttnArgs& a, const Request* known) {
   c.unit = 0;
   if (++c.tile < c.q.tiles) return;
   c.tile = 0;
@@ -375,28 +391,38 @@ __device__ __forceinline__ void next_item(Cursor& c, const AttnArgs& a) {
   c.head = 0;
   do {
     if (++c.r >= a.n_req) return;
-    c.q = request<NT>(a, c.r, false);
+    c.q = known ? known[c.r] : request<NT>(a, c.r, false);
   } while (c.q.tiles == 0);
 }
 
-// A piece of an item that one warp has worked on.
+// A piece of an item that one warp has worked on: the item's first unit in the line and its units; its rows.
 struct Piece {
-  uint32_t used, r, head, tile, units;
-  unsigned long long start;  // the item's first unit in the line
+  uint32_t used, start, units, head, row0, rows;
+  int q0;
+};
+// An item whose pieces lie in several CTAs: one of this CTA's pieces of it, where it begins, over how many CTAs it goes.
+struct Join {
+  uint32_t piece, first_cta, n, last;
 };
 
 // The unit that is fetched, one lane per page.
 struct Fetch {
   int key0, kv_len, low;
-  uint32_t rem;          // units of the item from this one on
-  uint32_t ids, base;    // ids: lane l has the page id of page `base + l` of the request
-  const uint8_t* src;    // this lane's page, K
-  uint32_t pages;        // those that are fetched: they hold keys of [low, kv_len) and have a good id
+  uint32_t rem;        // units of the item from this one on
+  uint32_t ids, base;  // ids: lane l has the page id of page `base + l` of the request
+  uint32_t pages;      // those that are fetched: they hold keys of [low, kv_len) and have a good id
+  const uint8_t* src;  // this lane's page, K
 };
-__device__ __forceinline__ void copy_pages(const Fetch& f, const uint8_t* src, uint32_t bytes, uint32_t dst, uint32_t bar, uint32_t lane) {
-  if (lane == 0) mbar_arrive_expect_tx(bar, __popc(f.pages) * bytes);
+// What the warp has to know of a unit when it works on it: keys from its first one to the last one, keys before the first that
+// is looked at (both relative to the unit), the pages that were fetched, whether the item ends with it.
+struct Unit {
+  int left, low;
+  uint32_t pages, ends;
+};
+__device__ __forceinline__ void copy_pages(uint32_t pages, const uint8_t* src, uint32_t bytes, uint32_t dst, uint32_t bar, uint32_t lane) {
+  if (lane == 0) mbar_arrive_expect_tx(bar, __popc(pages) * bytes);
   __syncwarp();
-  if (f.pages >> lane & 1)
+  if (pages >> lane & 1)
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + lane * bytes), "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
 }
@@ -412,11 +438,10 @@ __device__ __forceinline__ void start_item(Fetch& f, const AttnArgs& a, const Cu
   f.kv_len = c.q.kv_len;
   f.low = c.q.low;
   f.rem = c.q.units - c.unit;
-  f.src = a.pool.data;
   load_ids<PAGE>(f, a, c.r, lane);
 }
 template <int D, uint32_t PAGE>
-__device__ __forceinline__ void fetch_keys(Fetch& f, const AttnArgs& a, const Cursor& c, uint32_t dst, uint32_t bar, uint32_t lane) {
+__device__ __forceinline__ void fetch_keys(Fetch& f, const AttnArgs& a, const Cursor& c, Unit& info, uint32_t dst, uint32_t bar, uint32_t lane) {
   constexpr uint32_t N = UNIT / PAGE, BYTES = PAGE * (PoolLayout<D>::TOK / 2);
   const uint32_t page0 = static_cast<uint32_t>(f.key0) / PAGE;
   if (page0 - f.base >= 32) load_ids<PAGE>(f, a, c.r, lane);
@@ -425,20 +450,19 @@ __device__ __forceinline__ void fetch_keys(Fetch& f, const AttnArgs& a, const Cu
   const bool there = lane < N && key < f.kv_len && key + static_cast<int>(PAGE) > f.low, good = there && id < a.pool.n_pages;
   if (there && !good) note_range(a.err);
   f.pages = __ballot_sync(FULL, good);
+  if (lane == 0) info = Unit{f.kv_len - f.key0, f.low - f.key0, f.pages, f.rem == 1};
   f.src = a.pool.data + (static_cast<uint64_t>(id) * a.pool.n_kv_head + c.head) * (2 * BYTES);
-  copy_pages(f, f.src, BYTES, dst, bar, lane);
+  copy_pages(f.pages, f.src, BYTES, dst, bar, lane);
 }
 
 // Places of a unit's K or V that hold no key of the request may hold any bits: their d and m become 0, so that the values are
 // numbers (P is 0 there). pages: those that have been fetched; tokens [from, to) are the request's.
 template <int D, uint32_t PAGE>
-__device__ __forceinline__ void clear_scales(uint8_t* buf, uint32_t pages, int from, int to, uint32_t lane) {
+__device__ __noinline__ void clear_scales(uint8_t* buf, uint32_t pages, int from, int to) {
   using L = PoolLayout<D>;
-#pragma unroll
-  for (uint32_t tok = lane; tok < UNIT; tok += 32) {
+  for (uint32_t tok = threadIdx.x & 31; tok < UNIT; tok += 32) {
     if ((pages >> (tok / PAGE) & 1) && static_cast<int>(tok) >= from && static_cast<int>(tok) < to) continue;
     uint8_t* at = buf + tok / PAGE * (PAGE * (L::TOK / 2)) + L::kd(PAGE) + tok % PAGE * 2 * L::NB;
-#pragma unroll
     for (uint32_t i = 0; i < L::NB / 2; i++) {
       reinterpret_cast<uint32_t*>(at)[i] = 0;
       reinterpret_cast<uint32_t*>(at + L::km(PAGE) - L::kd(PAGE))[i] = 0;
@@ -464,144 +488,183 @@ __device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, int q0, uint32_t
   return a.out.data + static_cast<int64_t>(q0 + row / a.group) * a.out.tok + static_cast<int64_t>(head * a.group + row % a.group) * a.out.head;
 }
 
-// The rows of a piece's item.
-struct Item {
-  int q0;
-  uint32_t row0, rows, cols;  // cols: fours of values of all rows
-};
-template <int D, int NT>
-__device__ __forceinline__ Item item_of(const AttnArgs& a, const Piece& p) {
-  const Request q = request<NT>(a, p.r, false);
-  const uint32_t row0 = p.tile * 8 * NT, rows = min(8u * NT, static_cast<uint32_t>(q.q_len) * a.group - row0);
-  return Item{q.q0, row0, rows, rows * (D / 4)};
-}
-// An item whose pieces lie in several CTAs: which of this CTA's pieces is one, where it begins, over how many CTAs it goes.
-struct Join {
-  uint32_t piece, first_cta, n, last;
-};
-
-// Pieces of one item, given by `at(i)`, i = from, from + step, ... < n: the running result of four dims of one row.
-struct Joined {
-  float m, l;
-  float4 o;
-  __device__ void add(float m2, float l2, float4 o2) {
-    const float top = fmaxf(m, m2), w1 = ex2(m - top), w2 = ex2(m2 - top);
+// A warp: row `row` of the `n` partial results at part(k) of an item, in order, becomes the output's row (to == null) or that of the
+// partial result `to`.
+template <int D, int NT, typename Part>
+__device__ __forceinline__ void join_row(const AttnArgs& a, const Piece& p, uint32_t row, uint32_t n, Part part, float* to, uint32_t lane) {
+  using S = Shape<D, NT>;
+  constexpr int V = D / 32;  // dims of a lane
+  float m = NEG_BIG, l = 0.f, o[V] = {};
+  for (uint32_t k0 = 0; k0 < n; k0 += 32) {
+    const uint32_t some = min(n - k0, 32u);
+    const float2 ml = lane < some ? *reinterpret_cast<const float2*>(part(k0 + lane) + row * S::STRIDE + D) : make_float2(NEG_BIG, 0.f);
+    float top = ml.x;
+#pragma unroll
+    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, x));
+    top = fmaxf(top, m);
+    const float before = ex2(m - top), weight = ex2(ml.x - top);
+    float sum = weight * ml.y;
+#pragma unroll
+    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(FULL, sum, x);
+    l = l * before + sum;
     m = top;
-    l = l * w1 + l2 * w2;
-    o = make_float4(o.x * w1 + o2.x * w2, o.y * w1 + o2.y * w2, o.z * w1 + o2.z * w2, o.w * w1 + o2.w * w2);
+#pragma unroll
+    for (int x = 0; x < V; x++) o[x] *= before;
+#pragma unroll 8
+    for (uint32_t k = 0; k < some; k++) {
+      const float* v = part(k0 + k) + row * S::STRIDE + V * lane;
+      const float wk = __shfl_sync(FULL, weight, k);
+      if constexpr (V == 4) {
+        const float4 e = *reinterpret_cast<const float4*>(v);
+        o[0] = fmaf(e.x, wk, o[0]);
+        o[1] = fmaf(e.y, wk, o[1]);
+        o[2] = fmaf(e.z, wk, o[2]);
+        o[3] = fmaf(e.w, wk, o[3]);
+      } else {
+        const float2 e = *reinterpret_cast<const float2*>(v);
+        o[0] = fmaf(e.x, wk, o[0]);
+        o[1] = fmaf(e.y, wk, o[1]);
+      }
+    }
   }
-};
+  if (to) {
+    float* v = to + row * S::STRIDE + V * lane;
+    if constexpr (V == 4) *reinterpret_cast<float4*>(v) = make_float4(o[0], o[1], o[2], o[3]);
+    else *reinterpret_cast<float2*>(v) = make_float2(o[0], o[1]);
+    if (lane == 0) *reinterpret_cast<float2*>(to + row * S::STRIDE + D) = make_float2(m, l);
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* out = out_row(a, p.q0, p.head, p.row0 + row) + V * lane;
+  if constexpr (V == 4) {
+    store4(a.bf, out, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  } else {
+    const uint32_t h = a.bf ? pack2<true>(o[0] * inv, o[1] * inv) : pack2<false>(o[0] * inv, o[1] * inv);
+    out[0] = static_cast<uint16_t>(h);
+    out[1] = static_cast<uint16_t>(h >> 16);
+  }
+}
 
 template <int D, int NT, uint32_t PAGE>
-__global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_kernel(const __grid_constant__ AttnArgs a, float* __restrict__ scratch, uint32_t* __restrict__ counters) {
+__global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel(const __grid_constant__ AttnArgs a, float* __restrict__ scratch, uint32_t* __restrict__ counters) {
   using S = Shape<D, NT>;
   using L = PoolLayout<D>;
   constexpr int NB = D / 32;
+  constexpr uint32_t NWARP = S::NWARP, THREADS = S::THREADS, RING = S::RING, HALF = PAGE * (L::TOK / 2), ALL_PAGES = (1u << UNIT / PAGE) - 1;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t bars[NWARP][2];
-  __shared__ unsigned long long line[THREADS + 1];  // units before the requests of thread t's part
-  __shared__ Piece pieces[NWARP][2];
-  __shared__ Cursor cursors[NWARP][2];               // the unit that is worked on, the unit that is fetched
-  __shared__ unsigned long long plan[3];             // the CTA's stretch [0, 1) of the line; units of a stretch
+  __shared__ __align__(8) uint64_t bars[NWARP][RING];
+  __shared__ uint32_t line[THREADS + 1];     // units before the requests of thread t's part
+  __shared__ Request requests[THREADS];      // all of them if there are no more than threads
+  __shared__ Cursor cursors[NWARP][2];       // the item that is worked on, the item that is fetched
+  __shared__ Unit infos[NWARP][4];
+  __shared__ Piece pieces[2 * NWARP];        // of a warp: where an item ended that had begun before its stretch; what its stretch ended with
   __shared__ Join joins[2];
-  __shared__ uint32_t items_s, most_s;
+  __shared__ uint32_t items_s, most_s, plan[3];  // plan: the CTA's stretch [0, 1) of the line; units of a stretch
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  uint8_t* buf[2] = {smem + warp * 2 * S::PART, smem + warp * 2 * S::PART + S::PART};
-  const uint32_t bar[2] = {smem_u32(&bars[warp][0]), smem_u32(&bars[warp][1])};
-  if (lane == 0) {
-    mbar_init(bar[0], 1);
-    mbar_init(bar[1], 1);
-    fence_barrier_init();
-  }
-  if (lane < 2) pieces[warp][lane].used = 0;
+  uint8_t* const buf = smem + warp * RING * S::PART;
+  const uint32_t buf_at = smem_u32(buf), bar = smem_u32(&bars[warp][0]);
+  if (lane < RING) mbar_init(bar + 8 * lane, 1);
+  if (lane == 0) fence_barrier_init();
+  if (lane < 2) pieces[2 * warp + lane].used = 0;
   if (threadIdx.x == 0) items_s = most_s = 0;
   __syncthreads();
   pdl_launch_dependents();
   pdl_wait();
 
-  // ---- this warp's stretch of the line ----
+  // ---- the line of units ----
   const uint32_t per = (a.n_req + THREADS - 1) / THREADS;
-  unsigned long long mine = 0;
+  const Request* known = per == 1 ? requests : nullptr;
   {
-    uint32_t items = 0, most = 0;
+    uint32_t units = 0, items = 0, most = 0;
     for (uint32_t r = threadIdx.x * per; r < min((threadIdx.x + 1) * per, a.n_req); r++) {
       const Request q = request<NT>(a, r, blockIdx.x == 0);
+      if (known) requests[r] = q;
       items += q.tiles * a.pool.n_kv_head;
       if (q.tiles) most = max(most, q.units);
-      mine += static_cast<unsigned long long>(q.tiles) * a.pool.n_kv_head * q.units;
+      units += q.tiles * a.pool.n_kv_head * q.units;
     }
-    unsigned long long up = mine;
+    uint32_t up = units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long x = __shfl_up_sync(FULL, up, o);
+      const uint32_t x = __shfl_up_sync(FULL, up, o);
       if (lane >= o) up += x;
     }
     line[threadIdx.x + 1] = up;  // within the warp
     items = __reduce_add_sync(FULL, items);
     most = __reduce_max_sync(FULL, most);
-    if (lane == 0) {
+    if (lane == 0 && items) {
       atomicAdd(&items_s, items);
       atomicMax(&most_s, most);
     }
   }
   __syncthreads();
-  unsigned long long before = 0;
-#pragma unroll
-  for (uint32_t w = 0; w < NWARP; w++) before += w < warp ? line[32 * (w + 1)] : 0;
-  __syncthreads();
-  line[threadIdx.x + 1] += before;
-  if (threadIdx.x == 0) line[0] = 0;
-  __syncthreads();
-  const unsigned long long total = line[THREADS];
+  if (a.n_req > 32) {
+    uint32_t before = 0;
+    for (uint32_t w = 0; w < warp; w++) before += line[32 * (w + 1)];
+    __syncthreads();
+    line[threadIdx.x + 1] += before;
+    __syncthreads();
+  }
+  // (with 32 requests or fewer the first warp's part is the line)
+  const uint32_t total = line[a.n_req > 32 ? THREADS : 32], n_cta = gridDim.x;
+  auto locate = [&](uint32_t x, Cursor& c) {  // the warp: unit x < total
+    uint32_t at = 0;                          // the last part that begins at x or before it
+    for (uint32_t i = 0; i < (a.n_req > 32 ? THREADS : 32u); i += 32) {
+      const uint32_t n = __popc(__ballot_sync(FULL, line[i + lane + 1] <= x));
+      at += n;
+      if (n < 32) break;
+    }
+    if (lane == 0) {
+      uint32_t left = at ? x - line[at] : x;
+      for (uint32_t r = at * per; r < a.n_req; r++) {
+        const Request q = known ? known[r] : request<NT>(a, r, false);
+        const uint32_t n = q.tiles * a.pool.n_kv_head * q.units;
+        if (left >= n) {
+          left -= n;
+          continue;
+        }
+        const uint32_t item = left / q.units;
+        c.q = q;
+        c.r = r;
+        c.unit = left - item * q.units;
+        c.head = item / q.tiles;
+        c.tile = item - c.head * q.tiles;
+        break;
+      }
+    }
+    __syncwarp();
+  };
+  for (uint32_t r = blockIdx.x; r < a.n_req; r += n_cta) {
+    const Request q = known ? known[r] : request<NT>(a, r, false);
+    if (q.kv_len) continue;
+    for (uint32_t x = threadIdx.x; x < static_cast<uint32_t>(q.q_len) * a.n_head * (D / 4); x += THREADS) {
+      const uint32_t row = x / (D / 4);
+      store4(false, a.out.data + static_cast<int64_t>(q.q0 + row / a.n_head) * a.out.tok + static_cast<int64_t>(row % a.n_head) * a.out.head + x % (D / 4) * 4, 0.f, 0.f, 0.f, 0.f);
+    }
+  }
   // One item per CTA where that takes at most one round of the warps more than equal stretches, which need their pieces
   // joined; else equal stretches, of one unit per warp at least.
-  const uint32_t n_cta = gridDim.x;
-  const unsigned long long even = (total + n_cta - 1) / n_cta, share = max(even, static_cast<unsigned long long>(NWARP));
-  const bool whole = items_s <= n_cta && (most_s + NWARP - 1) / NWARP <= (share + NWARP - 1) / NWARP + 1;
-  unsigned long long c0, c1;
-  Cursor &cur = cursors[warp][0], &next = cursors[warp][1];
-  auto locate = [&](unsigned long long x) {  // x < total
-    uint32_t lo = 0, hi = THREADS;
-    while (hi - lo > 1) {
-      const uint32_t mid = (lo + hi) / 2;
-      if (line[mid] <= x) lo = mid;
-      else hi = mid;
-    }
-    unsigned long long left = x - line[lo];
-    for (uint32_t r = lo * per; r < a.n_req; r++) {
-      const Request q = request<NT>(a, r, false);
-      const unsigned long long n = static_cast<unsigned long long>(q.tiles) * a.pool.n_kv_head * q.units;
-      if (left < n) {
-        const uint32_t item = static_cast<uint32_t>(left / q.units);
-        cur.q = q;
-        cur.r = r;
-        cur.unit = static_cast<uint32_t>(left % q.units);
-        cur.head = item / q.tiles;
-        cur.tile = item % q.tiles;
-        return;
-      }
-      left -= n;
-    }
-  };
-  if (whole) {  // item blockIdx.x: its place in the line
+  uint32_t c0, c1;
+  const uint32_t share = max((total + n_cta - 1) / n_cta, NWARP);
+  if (items_s <= n_cta && (most_s + NWARP - 1) / NWARP <= (share + NWARP - 1) / NWARP + 1) {
     c0 = c1 = 0;
     if (blockIdx.x < items_s) {
       uint32_t left = blockIdx.x;
       for (uint32_t r = 0; r < a.n_req; r++) {
-        const Request q = request<NT>(a, r, false);
+        const Request q = known ? known[r] : request<NT>(a, r, false);
         const uint32_t n = q.tiles * a.pool.n_kv_head;
         if (left < n) {
-          c0 += static_cast<unsigned long long>(left) * q.units;
+          c0 += left * q.units;
           c1 = c0 + q.units;
           break;
         }
         left -= n;
-        c0 += static_cast<unsigned long long>(n) * q.units;
+        c0 += n * q.units;
       }
     }
   } else {
-    c0 = min(blockIdx.x * share, total);
-    c1 = min(c0 + share, total);
+    c0 = min(static_cast<uint64_t>(blockIdx.x) * share, static_cast<uint64_t>(total));
+    c1 = c0 + min(share, total - c0);
   }
   if (c0 >= c1) return;  // (all threads)
   if (threadIdx.x == 0) {
@@ -609,64 +672,102 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
     plan[1] = c1;
     plan[2] = share;
   }
-  const uint32_t cta_units = static_cast<uint32_t>(c1 - c0), begin = static_cast<uint32_t>(static_cast<unsigned long long>(cta_units) * warp / NWARP);
-  const uint32_t n = static_cast<uint32_t>(static_cast<unsigned long long>(cta_units) * (warp + 1) / NWARP) - begin;
-
+  const uint32_t begin = static_cast<uint64_t>(c1 - c0) * warp / NWARP, n = static_cast<uint64_t>(c1 - c0) * (warp + 1) / NWARP - begin;
   __syncthreads();
+
   if (n > 0) {
-    if (lane == 0) {
-      locate(c0 + begin);
-      next = cur;
-    }
+    Cursor &cur = cursors[warp][0], &next = cursors[warp][1];
+    locate(plan[0] + begin, cur);
+    if (lane == 0) next = cur;
     __syncwarp();
-    constexpr uint32_t half = PAGE * (L::TOK / 2), ALL_PAGES = (1u << UNIT / PAGE) - 1;
     Fetch f;
+    uint32_t asked = 1, nb = 0, flying = 0;  // units asked for; the buffer (and its barrier) that is filled next; filled ones
+    auto fetch_k = [&]() {       // of unit asked - 1
+      fetch_keys<D, PAGE>(f, a, next, infos[warp][(asked - 1) & 3], buf_at + nb * S::PART, bar + 8 * nb, lane);
+      if (++nb == RING) nb = 0;
+      flying++;
+    };
+    auto fetch_v = [&]() {
+      copy_pages(f.pages, f.src + HALF, HALF, buf_at + nb * S::PART, bar + 8 * nb, lane);
+      if (++nb == RING) nb = 0;
+      flying++;
+    };
+    auto next_unit = [&]() {
+      asked++;
+      if (f.rem > 1) {
+        f.rem--;
+        f.key0 += UNIT;
+      } else {
+        if (lane == 0) next_item<NT>(next, a, known);
+        __syncwarp();
+        start_item<PAGE>(f, a, next, lane);
+      }
+    };
+    RawQueries<D, NT> raw;
+    ask_queries<D, NT>(raw, a, cur.head, cur.tile * S::ROWS, cur.q.q_len * a.group, cur.q.q0, lane);
     start_item<PAGE>(f, a, next, lane);
-    fetch_keys<D, PAGE>(f, a, next, smem_u32(buf[0]), bar[0], lane);
-    copy_pages(f, f.src + half, half, smem_u32(buf[1]), bar[1], lane);
+    fetch_k();
+    fetch_v();
+    if (n > 1) {
+      next_unit();
+      fetch_k();
+      if (RING == 4) fetch_v();
+    }
     WarpState<D, NT> w;
     bool fresh = true, from_start = false, ok = true;
-    uint32_t first = 0;  // of this piece; cur.unit is its place in the item
+    uint32_t first = 0;          // of this piece; cur.unit is its place in the item
+    uint32_t b = 0, phase = 0;   // the buffer that is worked on, the phases of the barriers' next use
+    auto wait = [&]() { return mbar_wait(bar + 8 * b, phase >> b & 1, WAIT_LIMIT); };
+    auto done = [&]() {
+      phase ^= 1u << b;
+      if (++b == RING) b = 0;
+      flying--;
+      __syncwarp();
+    };
     for (uint32_t i = 0; i < n; i++) {
       if (fresh) {
-        load_queries<D, NT>(w, a, cur.head, cur.tile * S::ROWS, cur.q.q_len * a.group, cur.q.q0, lane);
+        if (i) ask_queries<D, NT>(raw, a, cur.head, cur.tile * S::ROWS, cur.q.q_len * a.group, cur.q.q0, lane);
+        set_queries<D, NT>(w, raw, a, cur.tile * S::ROWS, cur.q.q_len * a.group, lane);
         from_start = cur.unit == 0;
         first = i;
         fresh = false;
       }
-      const int key0 = f.key0, left = f.kv_len - key0, low = f.low - key0;
-      const uint32_t pages = f.pages;
-      const bool more = i + 1 < n, ends = f.rem == 1;
-      if (more && !ends) {
-        f.key0 += UNIT;
-        f.rem--;
-      }
       float s[NT][4][4];
-      ok = ok && mbar_wait(bar[0], i & 1, WAIT_LIMIT);
-      const bool part = pages != ALL_PAGES || low > 0 || left < static_cast<int>(UNIT);
-      if (part) clear_scales<D, PAGE>(buf[0], pages, 0, UNIT, lane);
+      ok = ok && wait();
+      if (!ok) break;
+      const Unit u = infos[warp][i & 3];
+      const bool part = u.pages != ALL_PAGES || u.low > 0 || u.left < static_cast<int>(UNIT);
+      {
+        uint8_t* kb = buf + b * S::PART;
+        if (part) clear_scales<D, PAGE>(kb, u.pages, 0, UNIT);
 #pragma unroll
-      for (int k = 0; k < 4; k++) scores16<D, NT, PAGE>(w, buf[0], lane, s, k);
-      __syncwarp();
-      if (more && ok) {
-        if (ends) {
-          if (lane == 0) next_item<NT>(next, a);
-          __syncwarp();
-          start_item<PAGE>(f, a, next, lane);
-        }
-        fetch_keys<D, PAGE>(f, a, next, smem_u32(buf[0]), bar[0], lane);
+        for (int k = 0; k < 4; k++) scores16<D, NT, PAGE>(w, kb, lane, s, k);
+      }
+      done();
+      if (RING == 3 && i + 1 < n) fetch_v();  // of unit i + 1
+      if (RING == 4 && i + 2 < n) {
+        next_unit();
+        fetch_k();
       }
       const int q_len = cur.q.q_len;
-      softmax64<D, NT>(w, s, left - static_cast<int>(UNIT) < q_len - 1 || (a.window && left > static_cast<int>(min(a.window, 0x40000000u))), left, cur.tile * S::ROWS, q_len, a, lane);
-      ok = ok && mbar_wait(bar[1], i & 1, WAIT_LIMIT);
-      if (part) clear_scales<D, PAGE>(buf[1], pages, low, left, lane);
-#pragma unroll
-      for (int k = 0; k < 4; k++) values16<D, NT, PAGE>(w, buf[1], lane, s, k, a.bias);
-      __syncwarp();
-      if (more && ok) copy_pages(f, f.src + half, half, smem_u32(buf[1]), bar[1], lane);
+      softmax64<D, NT>(w, s, u.left - static_cast<int>(UNIT) < q_len - 1 || (a.window && u.left > static_cast<int>(min(a.window, 0x40000000u))), u.left,
+                       cur.tile * S::ROWS, q_len, a, lane);
+      ok = wait();
       if (!ok) break;
+      {
+        uint8_t* vb = buf + b * S::PART;
+        if (part) clear_scales<D, PAGE>(vb, u.pages, u.low, u.left);
+#pragma unroll
+        for (int k = 0; k < 4; k++) values16<D, NT, PAGE>(w, vb, lane, s, k, a.bias);
+      }
+      done();
+      if (RING == 3 && i + 2 < n) {
+        next_unit();
+        fetch_k();
+      }
+      if (RING == 4 && i + 2 < n) fetch_v();
 
-      if (ends || !more) {
+      if (u.ends || i + 1 == n) {
         // sums over the lanes of a row
 #pragma unroll
         for (int e = 0; e < NT; e++)
@@ -674,8 +775,8 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
           for (int c = 0; c < 2; c++)
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) w.l[e][c] += __shfl_xor_sync(FULL, w.l[e][c], o);
-        const uint32_t row0 = cur.tile * S::ROWS, n_rows = cur.q.q_len * a.group;
-        if (ends && from_start) {
+        const uint32_t row0 = cur.tile * S::ROWS, n_rows = static_cast<uint32_t>(q_len) * a.group;
+        if (u.ends && from_start) {
 #pragma unroll
           for (int e = 0; e < NT; e++)
 #pragma unroll
@@ -685,154 +786,92 @@ __global__ void __launch_bounds__(THREADS, Shape<D, NT>::CTAS) kv4_attention_ker
               const float inv = w.l[e][c] == 0.f ? 0.f : 1.f / w.l[e][c];
               uint16_t* out = out_row(a, cur.q.q0, cur.head, row);
 #pragma unroll
-              for (int b = 0; b < NB; b++)
-                store4(a.bf, out + 32 * b + 4 * g, w.o[e][2 * b][c] * inv, w.o[e][2 * b][c + 2] * inv, w.o[e][2 * b + 1][c] * inv, w.o[e][2 * b + 1][c + 2] * inv);
+              for (int x = 0; x < NB; x++)
+                store4(a.bf, out + 32 * x + 4 * g, w.o[e][2 * x][c] * inv, w.o[e][2 * x][c + 2] * inv, w.o[e][2 * x + 1][c] * inv, w.o[e][2 * x + 1][c + 2] * inv);
             }
         } else {
           // an item's end goes to memory (the buffers are in use), the stretch's end over the buffers
-          float* part = ends ? scratch + (static_cast<size_t>(blockIdx.x) * NWARP + warp) * S::PARTIAL : reinterpret_cast<float*>(buf[0]);
+          const bool last = i + 1 == n;
+          float* to = last ? reinterpret_cast<float*>(buf) : scratch + (static_cast<size_t>(blockIdx.x) * NWARP + warp) * S::PARTIAL;
 #pragma unroll
           for (int e = 0; e < NT; e++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-              float* p = part + (8 * e + 2 * t + c) * S::STRIDE;
+              float* p = to + (8 * e + 2 * t + c) * S::STRIDE;
 #pragma unroll
-              for (int b = 0; b < NB; b++)
-                *reinterpret_cast<float4*>(p + 32 * b + 4 * g) = make_float4(w.o[e][2 * b][c], w.o[e][2 * b][c + 2], w.o[e][2 * b + 1][c], w.o[e][2 * b + 1][c + 2]);
+              for (int x = 0; x < NB; x++)
+                *reinterpret_cast<float4*>(p + 32 * x + 4 * g) = make_float4(w.o[e][2 * x][c], w.o[e][2 * x][c + 2], w.o[e][2 * x + 1][c], w.o[e][2 * x + 1][c + 2]);
               if (g == 0) *reinterpret_cast<float2*>(p + D) = make_float2(w.m[e][c], w.l[e][c]);
             }
-          if (lane == 0) pieces[warp][ends ? 0 : 1] = Piece{1, cur.r, cur.head, cur.tile, cur.q.units, plan[0] + begin + first - cur.unit};
+          if (lane == 0)
+            pieces[2 * warp + (last ? 1 : 0)] = Piece{1, plan[0] + begin + first - cur.unit, cur.q.units, cur.head, row0, min(S::ROWS, n_rows - row0), cur.q.q0};
         }
         fresh = true;
-      }
-      if (more && ends) {
-        __syncwarp();
-        if (lane == 0) cur = next;
-        __syncwarp();
+        if (i + 1 < n) {
+          if (lane == 0) next_item<NT>(cur, a, known);
+          __syncwarp();
+        }
       }
     }
     if (!ok) {  // the wait gave up: what is on its way comes before the buffers are given back
       if (lane == 0) reinterpret_cast<volatile uint32_t*>(a.err)[1] = 1;
-      for (uint32_t k = 0; k < 2; k++)
-        for (uint32_t ph = 0; ph < 2; ph++) (void)mbar_wait(bar[k], ph, DRAIN_LIMIT);
+      for (; flying > 0; flying--) {
+        (void)mbar_wait(bar + 8 * b, phase >> b & 1, DRAIN_LIMIT);
+        if (++b == RING) b = 0;
+      }
     }
   }
   __syncthreads();
 
   // ---- the CTA's pieces: joined; items that lie in this CTA alone are written ----
-  float* exchange = scratch + static_cast<size_t>(gridDim.x) * NWARP * S::PARTIAL;
-  uint32_t n_joins = 0;
-  for (uint32_t i = 0; i < 2 * NWARP;) {
-    const Piece& p = pieces[i >> 1][i & 1];
-    if (!p.used) {
-      i++;
-      continue;
-    }
-    uint32_t end = i + 1;  // pieces [i, end) that are used belong to one item
-    for (uint32_t k = i + 1; k < 2 * NWARP; k++) {
-      const Piece& o = pieces[k >> 1][k & 1];
-      if (!o.used) continue;
-      if (o.start != p.start) break;
-      end = k + 1;
-    }
-    const Item it = item_of<D, NT>(a, p);
+  float* exchange = scratch + static_cast<size_t>(n_cta) * NWARP * S::PARTIAL;
+  const bool used = lane < 2 * NWARP && pieces[lane].used;
+  const uint32_t start = used ? pieces[lane].start : 0, all_used = __ballot_sync(FULL, used), under = all_used & ((1u << lane) - 1);
+  const uint32_t prev = __shfl_sync(FULL, start, under ? 31 - __clz(under) : 0);
+  uint32_t heads = __ballot_sync(FULL, used && (!under || prev != start)), n_joins = 0, turn = 0;  // the first piece of every item
+  while (heads) {
+    const uint32_t i = __ffs(heads) - 1;
+    heads &= heads - 1;
+    const uint32_t run = all_used & ~((1u << i) - 1) & (heads ? (1u << (__ffs(heads) - 1)) - 1 : FULL), n_run = __popc(run);
+    const Piece& p = pieces[i];
     const bool all = p.start >= plan[0] && p.start + p.units <= plan[1];
-    const uint32_t first_cta = all ? 0 : static_cast<uint32_t>(p.start / plan[2]);
-    float* mine_out = exchange + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PARTIAL;
-    for (uint32_t x = threadIdx.x; x < it.cols; x += THREADS) {
-      const uint32_t row = x / (D / 4), col = x % (D / 4) * 4;
-      Joined j{NEG_BIG, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-      for (uint32_t k = i; k < end; k++) {
-        if (!pieces[k >> 1][k & 1].used) continue;
-        const float* part = (k & 1) ? reinterpret_cast<const float*>(smem + (k >> 1) * 2 * S::PART) : scratch + (static_cast<size_t>(blockIdx.x) * NWARP + (k >> 1)) * S::PARTIAL;
-        const float2 ml = *reinterpret_cast<const float2*>(part + row * S::STRIDE + D);
-        j.add(ml.x, ml.y, *reinterpret_cast<const float4*>(part + row * S::STRIDE + col));
-      }
-      if (all) {
-        const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
-        store4(a.bf, out_row(a, it.q0, p.head, it.row0 + row) + col, j.o.x * inv, j.o.y * inv, j.o.z * inv, j.o.w * inv);
-      } else {
-        *reinterpret_cast<float4*>(mine_out + row * S::STRIDE + col) = j.o;
-        if (col == 0) *reinterpret_cast<float2*>(mine_out + row * S::STRIDE + D) = make_float2(j.m, j.l);
-      }
+    const uint32_t first_cta = all ? 0 : p.start / plan[2];
+    float* to = all ? nullptr : exchange + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PARTIAL;
+    for (uint32_t row = 0; row < p.rows; row++) {  // the warps take the rows of all items in turn
+      if (turn == warp)
+        join_row<D, NT>(a, p, row, n_run, [&](uint32_t k) {
+          const uint32_t x = __fns(run, 0, k + 1);
+          return (x & 1) ? reinterpret_cast<const float*>(smem + (x >> 1) * (RING * S::PART)) : scratch + (static_cast<size_t>(blockIdx.x) * NWARP + (x >> 1)) * S::PARTIAL;
+        }, to, lane);
+      if (++turn == NWARP) turn = 0;
     }
     if (!all) {  // an item that began before the stretch, one that goes on behind it
-      if (threadIdx.x == 0) joins[n_joins] = Join{i, first_cta, static_cast<uint32_t>((p.start + p.units - 1) / plan[2]) - first_cta + 1, 0};
+      if (threadIdx.x == 0) joins[n_joins] = Join{i, first_cta, (p.start + p.units - 1) / plan[2] - first_cta + 1, 0};
       n_joins++;
     }
-    i = end;
   }
   if (n_joins == 0) return;  // (all threads)
 
   // ---- items of several CTAs: the one that comes last joins them ----
-  __threadfence();
   __syncthreads();
   if (threadIdx.x < n_joins) {
     Join& j = joins[threadIdx.x];
+    __threadfence();
     j.last = atomicAdd(&counters[j.first_cta], 1u) == j.n - 1;
     if (j.last) counters[j.first_cta] = 0;  // for the next launch
     __threadfence();
   }
   __syncthreads();
+  turn = 0;
   for (uint32_t q = 0; q < n_joins; q++) {
-    if (!joins[q].last) continue;
-    const Piece& p = pieces[joins[q].piece >> 1][joins[q].piece & 1];
-    const Item it = item_of<D, NT>(a, p);
-    const uint32_t first_cta = joins[q].first_cta, n_parts = joins[q].n, rows = it.rows, cols = it.cols;
-    // weights of the pieces, then their sum: `ways` threads per four dims, each a part of the pieces, all loads on their way at once
-    float2* ml = reinterpret_cast<float2*>(smem);
-    const float* from = exchange + static_cast<size_t>(2 * first_cta) * S::PARTIAL;
-    for (uint32_t x = threadIdx.x; x < rows * n_parts; x += THREADS) {
-      const uint32_t k = x / rows, row = x % rows;
-      ml[row * n_parts + k] = __ldcg(reinterpret_cast<const float2*>(from + (2 * k + (k == 0)) * S::PARTIAL + row * S::STRIDE + D));
+    const Join j = joins[q];
+    if (!j.last) continue;
+    const float* from = exchange + static_cast<size_t>(2 * j.first_cta) * S::PARTIAL;
+    const Piece& p = pieces[j.piece];
+    for (uint32_t row = 0; row < p.rows; row++) {
+      if (turn == warp) join_row<D, NT>(a, p, row, j.n, [&](uint32_t k) { return from + (2 * k + (k == 0)) * S::PARTIAL; }, nullptr, lane);
+      if (++turn == NWARP) turn = 0;
     }
-    __syncthreads();
-    for (uint32_t row = warp; row < rows; row += NWARP) {
-      float m = NEG_BIG, l = 0.f;
-      for (uint32_t k = lane; k < n_parts; k += 32) m = fmaxf(m, ml[row * n_parts + k].x);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
-      for (uint32_t k = lane; k < n_parts; k += 32) {
-        const float2 e = ml[row * n_parts + k];
-        const float weight = ex2(e.x - m);
-        l += weight * e.y;
-        ml[row * n_parts + k].x = weight;
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(FULL, l, o);
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      __syncwarp();
-      for (uint32_t k = lane; k < n_parts; k += 32) ml[row * n_parts + k].x *= inv;
-    }
-    __syncthreads();
-    const uint32_t ways = cols <= THREADS / 8 ? 8 : cols <= THREADS / 4 ? 4 : cols <= THREADS / 2 ? 2 : 1;
-    float4* sums = reinterpret_cast<float4*>(ml + ((rows * n_parts + 1) & ~1u));
-    for (uint32_t x = threadIdx.x; x < cols * ways; x += THREADS) {
-      const uint32_t way = x / cols, c = x % cols, row = c / (D / 4), col = c % (D / 4) * 4;
-      const float* part = from + row * S::STRIDE + col;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (uint32_t k = way; k < n_parts; k += ways) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(part + (2 * k + (k == 0)) * S::PARTIAL));
-        const float weight = ml[row * n_parts + k].x;
-        o = make_float4(fmaf(v.x, weight, o.x), fmaf(v.y, weight, o.y), fmaf(v.z, weight, o.z), fmaf(v.w, weight, o.w));
-      }
-      if (ways == 1) store4(a.bf, out_row(a, it.q0, p.head, it.row0 + row) + col, o.x, o.y, o.z, o.w);
-      else sums[x] = o;
-    }
-    if (ways > 1) {
-      __syncthreads();
-      if (threadIdx.x < cols) {
-        const uint32_t row = threadIdx.x / (D / 4), col = threadIdx.x % (D / 4) * 4;
-        float4 o = sums[threadIdx.x];
-        for (uint32_t k = 1; k < ways; k++) {
-          const float4 v = sums[k * cols + threadIdx.x];
-          o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
-        }
-        store4(a.bf, out_row(a, it.q0, p.head, it.row0 + row) + col, o.x, o.y, o.z, o.w);
-      }
-    }
-    __syncthreads();
   }
 }
 
@@ -859,14 +898,18 @@ cudaError_t bp_kv4_attention_init(bp_paged_ctx* c) {
     });
   if (e != cudaSuccess) return e;
   // a piece per warp and two per CTA, of the instance that needs most
-  c->attn_sms = c->sm_count < static_cast<int>(MOST_SMS) ? c->sm_count : MOST_SMS;
-  const size_t one = 2 * static_cast<size_t>(c->attn_sms) * (NWARP + 2);
-  const size_t floats = one * Shape<128, 2>::PARTIAL;
+  size_t floats = 0;
+  for (uint32_t i = 0; i < 4; i++)
+    (void)with_kernel(i & 1 ? 128 : 64, i & 2, 16, [&](auto, auto shape) {
+      const size_t need = static_cast<size_t>(c->sm_count) * (shape.NWARP + 2) * shape.PARTIAL;
+      if (need > floats) floats = need;
+      return cudaSuccess;
+    });
   e = cudaMalloc(&c->partials, floats * sizeof(float));
   if (e != cudaSuccess) return e;
-  e = cudaMalloc(&c->counters, 2 * static_cast<size_t>(c->attn_sms) * sizeof(uint32_t));
+  e = cudaMalloc(&c->counters, static_cast<size_t>(c->sm_count) * sizeof(uint32_t));
   if (e != cudaSuccess) return e;
-  return cudaMemset(c->counters, 0, 2 * static_cast<size_t>(c->attn_sms) * sizeof(uint32_t));
+  return cudaMemset(c->counters, 0, static_cast<size_t>(c->sm_count) * sizeof(uint32_t));
 }
 
 cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, const Pool& pool, uint32_t head_dim, const bp_kv4_attn& in) {
@@ -889,7 +932,8 @@ cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, co
   a.scale_log2 = in.scale * 1.4426950408889634f;
   a.bias = 0x64006400u;
   a.bf = bf;
+  a.q_vec = reinterpret_cast<uintptr_t>(in.q.data) % 16 == 0 && in.q.tok_stride % 8 == 0 && in.q.head_stride % 8 == 0;
   return with_kernel(head_dim, a.max_q * a.group > 8, pool.page, [&](auto kernel, auto shape) {
-    return bp_launch(true, kernel, dim3(shape.CTAS * c->attn_sms), dim3(THREADS), shape.SMEM, s, a, c->partials, c->counters);
+    return bp_launch(true, kernel, dim3(c->sm_count), dim3(shape.THREADS), shape.SMEM, s, a, c->partials, c->counters);
   });
 }

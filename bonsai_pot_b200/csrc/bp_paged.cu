@@ -267,6 +267,9 @@ int bp_kv4_attention(bp_paged_ctx* c, void* stream, uint32_t dtype, const bp_kv4
   if (a->n_req == 0 || a->total_q == 0 || a->max_q == 0) return BP_OK;
   if (a->n_req > 65535) return fail_config(c, "at most 65535 requests");
   if (static_cast<uint64_t>(a->total_q) * a->n_head > 0x7fffffffull || a->max_kv > 0x7fffff00u) return fail_config(c, "total_q * n_head and max_kv must be < 2^31");
+  // units of 64 keys of 8 rows are counted in 32 bits
+  const uint64_t tiles = static_cast<uint64_t>(a->total_q) * (a->n_head / p.n_kv_head) / 8 + a->n_req;
+  if (tiles * p.n_kv_head > 0xffffffffull / (a->max_kv / 64 + 1)) return fail_config(c, "total_q * n_head * max_kv is too large for one call");
   if (!rq.data || !ro.data || !a->q_start || !a->kv_len || (a->max_kv != 0 && (!p.data || !a->page_table))) return fail(c, BP_ERR_NULL, "null pointer argument");
   OnDevice on(c->device);
   BP_TRY(c, on.err);
