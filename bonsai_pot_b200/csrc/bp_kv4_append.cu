@@ -11,62 +11,62 @@ namespace {
 
 using namespace bp;
 
-__device__ __forceinline__ float min_nan(float a, float b) {
+// A NaN among them is the result.
+__device__ __forceinline__ float min3(float a, float b, float c) {
   float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
+__device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
-// Eight dims of a block, of which four neighbouring lanes hold a quarter each: the codes, dim i at bits 4 i, and d, m.
-__device__ __forceinline__ uint32_t quantise8(const float* x, __half* d_out, __half* m_out) {
+// Bits of a code of dim i: in a K word even dims are in the low half, odd ones in the high half; in a V word in order.
+template <bool K>
+__host__ __device__ constexpr int code_at(int i) {
+  return K ? 4 * (i >> 1) + 16 * (i & 1) : 4 * i;
+}
+constexpr float MAGIC = 12582912.f;  // 1.5 2^23: the low bits of x + MAGIC are rint(x)
+constexpr uint32_t MAGIC_BITS = 0x4b400000u;
+
+// Eight dims of a block, of which four neighbouring lanes hold a quarter each: the codes, and the block's d, m.
+template <bool K>
+__device__ __forceinline__ uint32_t quantise8(float* x, __half* d_out, __half* m_out) {
   constexpr float LIM = 64512.f;
-  float v[8], lo, hi;
-#pragma unroll
-  for (int i = 0; i < 8; i++) v[i] = min_nan(max_nan(x[i], -LIM), LIM);
-  lo = min_nan(min_nan(min_nan(v[0], v[1]), min_nan(v[2], v[3])), min_nan(min_nan(v[4], v[5]), min_nan(v[6], v[7])));
-  hi = max_nan(max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])), max_nan(max_nan(v[4], v[5]), max_nan(v[6], v[7])));
+  float lo = min3(min3(x[0], x[1], x[2]), min3(x[3], x[4], x[5]), min3(x[6], x[7], x[7]));
+  float hi = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[7]));
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = min3(lo, __shfl_xor_sync(0xffffffffu, lo, o), lo);
+    hi = max3(hi, __shfl_xor_sync(0xffffffffu, hi, o), hi);
+  }
+  if (!(lo >= -LIM && hi <= LIM)) {  // rare: values beyond the limit, infinities, a NaN (which stays)
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = min3(max3(x[i], -LIM, -LIM), LIM, LIM);
+    lo = min3(max3(lo, -LIM, -LIM), LIM, LIM);
+    hi = min3(max3(hi, -LIM, -LIM), LIM, LIM);
   }
   // u = 2^(e - 10), e the exponent of the largest magnitude and a 64th: a power of two, so that * u and / u are exact
   const float top = __fmul_rn(fmaxf(fabsf(lo), fabsf(hi)), 1.015625f);
   const float u = fmaxf(__uint_as_float(__float_as_uint(top) & 0x7f800000u) * 0x1p-10f, 0x1p-24f);
-  const float inv_u = __fdiv_rn(1.f, u);
+  const float inv_u = __uint_as_float(0x7f000000u - __float_as_uint(u));  // (of a NaN: anything, m is one)
   const float m = __fmul_rn(rintf(__fmul_rn(lo, inv_u)), u);
   const float d = __fmul_rn(rintf(__fmul_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f), inv_u)), u);
   const float inv = d > 0.f ? __fdiv_rn(1.f, d) : 0.f;
-  uint32_t codes = 0;
+  // q = rint((x - m) inv) is at least -0.5, which rounds to 0: m is at most u / 2 above the least value and d at least u. The low
+  // bits of q + MAGIC are the code; what the other bits add up to is taken off at the end.
+  uint32_t codes = 0, off = 0;
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    const float q = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(v[i], m), inv)), 0.f), 15.f);
-    codes |= static_cast<uint32_t>(q) << (4 * i);
+    const float q = fminf(__fadd_rn(__fmul_rn(__fsub_rn(x[i], m), inv), MAGIC), MAGIC + 15.f);
+    codes += __float_as_uint(q) << code_at<K>(i);
+    off += MAGIC_BITS << code_at<K>(i);
   }
   *d_out = __float2half_rn(d);
   *m_out = __float2half_rn(m);
-  return codes;
-}
-
-// dims 0 .. 7 at bits 4 i -> the order of a K word: even dims in the low half, odd ones in the high half
-__device__ __forceinline__ uint32_t k_word(uint32_t w) {
-  uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
-  even = (even | even >> 4) & 0x00ff00ffu;
-  odd = (odd | odd >> 4) & 0x00ff00ffu;
-  return ((even | even >> 8) & 0xffffu) | (((odd | odd >> 8) & 0xffffu) << 16);
-}
-__device__ __forceinline__ uint32_t k_word_back(uint32_t w) {
-  uint32_t even = w & 0xffffu, odd = w >> 16;
-  even = (even | even << 8) & 0x00ff00ffu;
-  odd = (odd | odd << 8) & 0x00ff00ffu;
-  even = (even | even << 4) & 0x0f0f0f0fu;
-  odd = (odd | odd << 4) & 0x0f0f0f0fu;
-  return even | odd << 4;
+  return codes - off;
 }
 
 struct AppendArgs {
@@ -79,7 +79,18 @@ struct AppendArgs {
   Rope rope;
   uint32_t n_tok;
   float eps;
+  FastDiv heads;
+  uint32_t table_vec;  // rows of the table are 16-byte aligned
 };
+
+template <bool VEC>
+__device__ __forceinline__ uint4 load_raw(const uint16_t* p) {
+  if (VEC) return *reinterpret_cast<const uint4*>(p);
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) h[i] = p[i];
+  return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+}
 
 template <bool BF, bool VEC, int D>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
@@ -91,7 +102,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
   const uint32_t row = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   // (lanes without a row stay for the shuffles, on row 0's data)
   const bool in = row < a.n_tok * a.pool.n_kv_head;
-  const uint32_t tok = in ? row / a.pool.n_kv_head : 0, head = in ? row % a.pool.n_kv_head : 0;
+  const uint32_t tok = in ? a.heads.quotient(row) : 0, head = in ? row - tok * a.pool.n_kv_head : 0;
   const int64_t slot = a.slots[tok];
   const int32_t pos = a.positions ? a.positions[tok] : 0;
   const bool over = slot >= static_cast<int64_t>(a.pool.n_pages) << a.pool.log_page || (a.positions && pos >= 0 && static_cast<uint32_t>(pos) >= a.rope.n_pos);
@@ -99,9 +110,12 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
   if (in && over && slot >= 0 && pos >= 0 && c == 0) note_range(a.err);
   const uint16_t* k = a.k.data + tok * a.k.tok + head * a.k.head;
   const uint16_t* v = a.v.data + tok * a.v.tok + head * a.v.head;
+  uint4 raw[4];  // K, K, V, V: every load is on its way before the first is used
+#pragma unroll
+  for (int i = 0; i < 4; i++) raw[i] = load_raw<VEC>((i < 2 ? k : v) + (i & 1) * (D / 2) + 8 * c);
   float x[2][8], y[2][8];
-  load8<BF, VEC>(k + 8 * c, x[0]);
-  load8<BF, VEC>(k + D / 2 + 8 * c, x[1]);
+  unpack8<BF>(raw[0], x[0]);
+  unpack8<BF>(raw[1], x[1]);
   float scale = 1.f;
   if (a.w) {
     float s[2];
@@ -118,7 +132,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       float w[8];
-      load8<BF, false>(a.w + h * (D / 2) + 8 * c, w);
+      if (reinterpret_cast<uintptr_t>(a.w) % 16 == 0) load8<BF, true>(a.w + h * (D / 2) + 8 * c, w);
+      else load8<BF, false>(a.w + h * (D / 2) + 8 * c, w);
 #pragma unroll
       for (int i = 0; i < 8; i++) x[h][i] = __fmul_rn(__fmul_rn(x[h][i], scale), w[i]);
     }
@@ -135,18 +150,41 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const uint32_t p0 = (h * (D / 2) + 8 * c) / 2;
+        float2 four[4];
+        if (p0 + 4 <= half && a.table_vec) {
+          const float4 e = *reinterpret_cast<const float4*>(cs + p0), f = *reinterpret_cast<const float4*>(cs + p0 + 2);
+          four[0] = make_float2(e.x, e.y);
+          four[1] = make_float2(e.z, e.w);
+          four[2] = make_float2(f.x, f.y);
+          four[3] = make_float2(f.z, f.w);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++) four[i] = p0 + i < half ? cs[p0 + i] : make_float2(1.f, 0.f);
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           if (p0 + i >= half) continue;
-          const float2 t = cs[p0 + i];
+          const float2 t = four[i];
           y[h][2 * i] = turn(x[h][2 * i], x[h][2 * i + 1], t.x, -t.y);
           y[h][2 * i + 1] = turn(x[h][2 * i + 1], x[h][2 * i], t.x, t.y);
         }
       }
     } else if (a.rope.rot == D) {
+      float2 eight[8];
+      if (a.table_vec) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float4 e = reinterpret_cast<const float4*>(cs + 8 * c)[i];
+          eight[2 * i] = make_float2(e.x, e.y);
+          eight[2 * i + 1] = make_float2(e.z, e.w);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) eight[i] = cs[8 * c + i];
+      }
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        const float2 t = cs[8 * c + i];
+        const float2 t = eight[i];
         y[0][i] = turn(x[0][i], x[1][i], t.x, -t.y);
         y[1][i] = turn(x[1][i], x[0][i], t.x, t.y);
       }
@@ -167,32 +205,61 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
       }
     }
   }
-  load8<BF, VEC>(v + 8 * c, x[0]);
-  load8<BF, VEC>(v + D / 2 + 8 * c, x[1]);
+  unpack8<BF>(raw[2], x[0]);
+  unpack8<BF>(raw[3], x[1]);
   const uint32_t page = a.pool.page, place = static_cast<uint32_t>(slot) & (page - 1);
   uint8_t* rec = a.pool.data;
   if (store) rec += (static_cast<size_t>(slot >> a.pool.log_page) * a.pool.n_kv_head + head) * (static_cast<size_t>(page) * L::TOK);
-#pragma unroll
-  for (int h = 0; h < 2; h++) {
-    const uint32_t j = c + h * LANES, b = j >> 2, q = j & 3;  // chunk j is quarter q of block b
-    __half d, m;
-    const uint32_t kw = k_word(quantise8(y[h], &d, &m));
-    if (store) {
-      *reinterpret_cast<uint32_t*>(rec + place * L::ROW + (q * L::NB + b) * 4) = kw;
-      if (q == 0) {
-        *reinterpret_cast<__half*>(rec + L::kd(page) + (place * L::NB + b) * 2) = d;
-        *reinterpret_cast<__half*>(rec + L::km(page) + (place * L::NB + b) * 2) = m;
-      }
+  // this lane's two blocks: chunk c is quarter q of block b, chunk c + LANES the same quarter of block b + NB / 2
+  __half2 kd, km, vd, vm;
+  uint32_t kw[2], vw[2];
+  {
+    __half d0, m0, d1, m1;
+    kw[0] = quantise8<true>(y[0], &d0, &m0);
+    kw[1] = quantise8<true>(y[1], &d1, &m1);
+    kd = __halves2half2(d0, d1);
+    km = __halves2half2(m0, m1);
+    vw[0] = quantise8<false>(x[0], &d0, &m0);
+    vw[1] = quantise8<false>(x[1], &d1, &m1);
+    vd = __halves2half2(d0, d1);
+    vm = __halves2half2(m0, m1);
+  }
+  const uint32_t at = place * 2 * L::NB;
+  if constexpr (D == 128) {
+    // Lanes c and c + 4 have the blocks 0, 2 and 1, 3 of the same quarter: the first takes the K words of both, the other the V
+    // words, and each writes 16 bytes; the lanes of quarter 0 the four d's and m's as well.
+    const bool upper = c & 4;
+    auto swap = [&](uint32_t mine_k, uint32_t mine_v) { return __shfl_xor_sync(0xffffffffu, upper ? mine_k : mine_v, 4); };
+    const uint32_t w0 = swap(kw[0], vw[0]), w1 = swap(kw[1], vw[1]), sd = swap(u2(kd), u2(vd)), sm = swap(u2(km), u2(vm));
+    if (!store) return;
+    uint8_t* part = rec + (upper ? L::v(page) : 0);
+    const uint32_t q = c & 3;
+    // blocks 0 .. 3 in order: the lower lane's first, the upper lane's first, the lower lane's second, the upper lane's second
+    uint4 w;
+    uint32_t da, db, ma, mb;
+    if (upper) {
+      const uint32_t b0 = w0, b1 = vw[0], b2 = w1, b3 = vw[1];
+      w = make_uint4(prmt(b0, b1, 0x5410), prmt(b2, b3, 0x5410), prmt(b0, b1, 0x7632), prmt(b2, b3, 0x7632));
+      da = prmt(sd, u2(vd), 0x5410), db = prmt(sd, u2(vd), 0x7632), ma = prmt(sm, u2(vm), 0x5410), mb = prmt(sm, u2(vm), 0x7632);
+    } else {
+      w = make_uint4(kw[0], w0, kw[1], w1);
+      da = prmt(u2(kd), sd, 0x5410), db = prmt(u2(kd), sd, 0x7632), ma = prmt(u2(km), sm, 0x5410), mb = prmt(u2(km), sm, 0x7632);
     }
-    const uint32_t vw = quantise8(x[h], &d, &m);
-    if (store) {
-      uint8_t* rv = rec + L::v(page);
-      *reinterpret_cast<uint16_t*>(rv + place * L::ROW + L::v16(place, 2 * q, b)) = static_cast<uint16_t>(vw);
-      *reinterpret_cast<uint16_t*>(rv + place * L::ROW + L::v16(place, 2 * q + 1, b)) = static_cast<uint16_t>(vw >> 16);
-      if (q == 0) {
-        *reinterpret_cast<__half*>(rv + L::kd(page) + (place * L::NB + b) * 2) = d;
-        *reinterpret_cast<__half*>(rv + L::km(page) + (place * L::NB + b) * 2) = m;
-      }
+    *reinterpret_cast<uint4*>(part + place * L::ROW + (upper ? L::v16(place, 2 * q, 0) : 16 * q)) = w;
+    if (q == 0) {
+      *reinterpret_cast<uint2*>(part + L::kd(page) + at) = make_uint2(da, db);
+      *reinterpret_cast<uint2*>(part + L::km(page) + at) = make_uint2(ma, mb);
+    }
+  } else {
+    if (!store) return;
+    uint8_t* rv = rec + L::v(page);
+    *reinterpret_cast<uint2*>(rec + place * L::ROW + 8 * c) = make_uint2(kw[0], kw[1]);
+    *reinterpret_cast<uint2*>(rv + place * L::ROW + 8 * c) = make_uint2(prmt(vw[0], vw[1], 0x5410), prmt(vw[0], vw[1], 0x7632));
+    if (c == 0) {
+      *reinterpret_cast<__half2*>(rec + L::kd(page) + at) = kd;
+      *reinterpret_cast<__half2*>(rec + L::km(page) + at) = km;
+      *reinterpret_cast<__half2*>(rv + L::kd(page) + at) = vd;
+      *reinterpret_cast<__half2*>(rv + L::km(page) + at) = vm;
     }
   }
 }
@@ -203,41 +270,98 @@ struct ReadArgs {
   const int64_t* slots;
   uint32_t* err;
   uint32_t n_tok;
+  FastDiv heads;
+  uint32_t bias;  // 0x64006400: two f16 numbers 1024
 };
 
-// A lane has one chunk of eight dims of K and of V.
+template <bool BF>
+__device__ __forceinline__ uint32_t from_half2(__half2 h) {
+  if (!BF) return u2(h);
+  const float2 f = __half22float2(h);
+  return pack2<true>(f.x, f.y);
+}
+template <bool VEC>
+__device__ __forceinline__ void store_words(uint16_t* p, const uint32_t (&w)[4]) {
+  if (VEC) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) p[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+  }
+}
+
+// Eight lanes per row: lane t < 4 has 16 (head_dim 64: 8) bytes of the K codes, a quarter of every block, lane 4 + t the same of V.
+// A lane has READ rows, whose loads are on their way together. m + d q in f16 does not round, see the format.
+constexpr int READ = 2;
 template <bool BF, bool VEC, int D>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const ReadArgs a) {
   using L = PoolLayout<D>;
-  constexpr uint32_t LANES = D / 8;
+  constexpr uint32_t ROWS = 256 / 8, NB = L::NB;
   pdl_launch_dependents();
+  const uint32_t kind = threadIdx.x >> 2 & 1, t = threadIdx.x & 3, page = a.pool.page, n_rows = a.n_tok * a.pool.n_kv_head;
+  const Rows& to = kind ? a.v : a.k;
+  uint32_t tok[READ], head[READ], codes[READ][NB], d[READ][NB / 2], m[READ][NB / 2];
+  int64_t slot[READ];
   pdl_wait();
-  const uint32_t j = threadIdx.x % LANES, row = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-  if (row >= a.n_tok * a.pool.n_kv_head) return;
-  const uint32_t tok = row / a.pool.n_kv_head, head = row % a.pool.n_kv_head;
-  const int64_t slot = a.slots[tok];
-  if (slot < 0) return;
-  if (slot >= static_cast<int64_t>(a.pool.n_pages) << a.pool.log_page) {
-    if (j == 0) note_range(a.err);
-    return;
-  }
-  const uint32_t page = a.pool.page, place = static_cast<uint32_t>(slot) & (page - 1), b = j >> 2, q = j & 3;
-  const uint8_t* rec = a.pool.data + (static_cast<size_t>(slot >> a.pool.log_page) * a.pool.n_kv_head + head) * (static_cast<size_t>(page) * L::TOK);
-  const uint8_t* rv = rec + L::v(page);
-  const uint32_t at = (place * L::NB + b) * 2;
-  const uint32_t kw = k_word_back(*reinterpret_cast<const uint32_t*>(rec + place * L::ROW + (q * L::NB + b) * 4));
-  const uint32_t vw = *reinterpret_cast<const uint16_t*>(rv + place * L::ROW + L::v16(place, 2 * q, b)) |
-                      static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(rv + place * L::ROW + L::v16(place, 2 * q + 1, b))) << 16;
-  const float kd = __half2float(*reinterpret_cast<const __half*>(rec + L::kd(page) + at)), km = __half2float(*reinterpret_cast<const __half*>(rec + L::km(page) + at));
-  const float vd = __half2float(*reinterpret_cast<const __half*>(rv + L::kd(page) + at)), vm = __half2float(*reinterpret_cast<const __half*>(rv + L::km(page) + at));
-  float x[8], y[8];
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    x[i] = fmaf(kd, static_cast<float>((kw >> (4 * i)) & 15), km);  // (exact: the product has 15 bits, the sum is an f16 number)
-    y[i] = fmaf(vd, static_cast<float>((vw >> (4 * i)) & 15), vm);
+  for (int r = 0; r < READ; r++) {
+    const uint32_t row = blockIdx.x * (ROWS * READ) + r * ROWS + threadIdx.x / 8;
+    tok[r] = a.heads.quotient(row);
+    head[r] = row - tok[r] * a.pool.n_kv_head;
+    slot[r] = row < n_rows ? a.slots[tok[r]] : -1;
+    if (slot[r] >= static_cast<int64_t>(a.pool.n_pages) << a.pool.log_page) {
+      note_range(a.err);
+      slot[r] = -1;
+    }
   }
-  store8<BF, VEC>(a.k.data + tok * a.k.tok + head * a.k.head + 8 * j, x);
-  store8<BF, VEC>(a.v.data + tok * a.v.tok + head * a.v.head + 8 * j, y);
+#pragma unroll
+  for (int r = 0; r < READ; r++) {
+    if (slot[r] < 0) continue;
+    const uint32_t place = static_cast<uint32_t>(slot[r]) & (page - 1);
+    const uint8_t* part = a.pool.data + (static_cast<uint64_t>(slot[r] >> a.pool.log_page) * a.pool.n_kv_head + head[r]) * (page * L::TOK) + kind * L::v(page);
+    const uint8_t *p = part + place * L::ROW + (kind ? L::v16(place, 2 * t, 0) : 4 * NB * t), *pd = part + L::kd(page) + place * 2 * NB, *pm = part + L::km(page) + place * 2 * NB;
+    if constexpr (NB == 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      const uint2 e = *reinterpret_cast<const uint2*>(pd), f = *reinterpret_cast<const uint2*>(pm);
+      codes[r][0] = u.x, codes[r][1] = u.y, codes[r][2] = u.z, codes[r][3] = u.w;
+      d[r][0] = e.x, d[r][1] = e.y, m[r][0] = f.x, m[r][1] = f.y;
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      codes[r][0] = u.x, codes[r][1] = u.y;
+      d[r][0] = *reinterpret_cast<const uint32_t*>(pd), m[r][0] = *reinterpret_cast<const uint32_t*>(pm);
+    }
+  }
+  const __half2 off = __float2half2_rn(-1024.f), off16 = __float2half2_rn(-64.f), sixteenth = __float2half2_rn(0.0625f);
+#pragma unroll
+  for (int r = 0; r < READ; r++) {
+    if (slot[r] < 0) continue;
+    uint16_t* out = to.data + tok[r] * to.tok + head[r] * to.head + 8 * t;
+    if (kind) {  // words: dims 0 .. 3 of two blocks, dims 4 .. 7 of them -> a word per block
+#pragma unroll
+      for (uint32_t i = 0; i < NB / 2; i++) {
+        const uint32_t lo = codes[r][i], hi = codes[r][NB / 2 + i];
+        // (in place: block 2 i in i, block 2 i + 1 in NB / 2 + i)
+        codes[r][i] = prmt(lo, hi, 0x5410);
+        codes[r][NB / 2 + i] = prmt(lo, hi, 0x7632);
+      }
+    }
+#pragma unroll
+    for (uint32_t b = 0; b < NB; b++) {
+      const uint32_t w = kind ? codes[r][(b & 1) * (NB / 2) + (b >> 1)] : codes[r][b], w8 = w >> 8, sel = b & 1 ? 0x3232u : 0x1010u;
+      const __half2 dd = h2(prmt(d[r][b >> 1], 0, sel)), mm = h2(prmt(m[r][b >> 1], 0, sel));
+      // the codes at bits 4 i of both halves
+      uint32_t x[4] = {u2(__hfma2(__hadd2(biased(w, 0x000f000fu, a.bias), off), dd, mm)), u2(__hfma2(__hfma2(biased(w, 0x00f000f0u, a.bias), sixteenth, off16), dd, mm)),
+                       u2(__hfma2(__hadd2(biased(w8, 0x000f000fu, a.bias), off), dd, mm)), u2(__hfma2(__hfma2(biased(w8, 0x00f000f0u, a.bias), sixteenth, off16), dd, mm))};
+      if (kind) {  // dims (i, i + 4) -> in order; K has (2 i, 2 i + 1)
+        const uint32_t y[4] = {prmt(x[0], x[1], 0x5410), prmt(x[2], x[3], 0x5410), prmt(x[0], x[1], 0x7632), prmt(x[2], x[3], 0x7632)};
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = y[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] = from_half2<BF>(h2(x[i]));
+      store_words<VEC>(out + 32 * b, x);
+    }
+  }
 }
 
 bool vec8(const Rows& r) { return reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && r.tok % 8 == 0 && r.head % 8 == 0; }
@@ -246,7 +370,8 @@ bool vec8(const Rows& r) { return reinterpret_cast<uintptr_t>(r.data) % 16 == 0 
 
 cudaError_t bp_launch_kv4_append(bp_paged_ctx* c, cudaStream_t s, bool bf, const Pool& pool, uint32_t head_dim, const Rows& k, const Rows& v,
                                  uint32_t n_tok, const int32_t* positions, const int64_t* slots, const Rope& rope, const uint16_t* w_norm, float eps) {
-  const AppendArgs a{pool, k, v, rope.table ? positions : nullptr, slots, w_norm, c->err_dev, rope, n_tok, eps};
+  const AppendArgs a{pool, k, v, rope.table ? positions : nullptr, slots, w_norm, c->err_dev, rope, n_tok, eps, FastDiv(pool.n_kv_head),
+                     reinterpret_cast<uintptr_t>(rope.table) % 16 == 0 && rope.rot % 4 == 0};
   auto go = [&](auto kernel, uint32_t lanes) {
     const uint32_t rows = n_tok * pool.n_kv_head, per = 256 / lanes;
     return bp_launch(true, kernel, dim3((rows + per - 1) / per), dim3(256), 0, s, a);
@@ -261,15 +386,15 @@ cudaError_t bp_launch_kv4_append(bp_paged_ctx* c, cudaStream_t s, bool bf, const
 
 cudaError_t bp_launch_kv4_read(bp_paged_ctx* c, cudaStream_t s, bool bf, const Pool& pool, uint32_t head_dim, const int64_t* slots, uint32_t n_tok,
                                const Rows& k, const Rows& v) {
-  const ReadArgs a{pool, k, v, slots, c->err_dev, n_tok};
-  auto go = [&](auto kernel, uint32_t lanes) {
-    const uint32_t rows = n_tok * pool.n_kv_head, per = 256 / lanes;
+  const ReadArgs a{pool, k, v, slots, c->err_dev, n_tok, FastDiv(pool.n_kv_head), 0x64006400u};
+  auto go = [&](auto kernel) {
+    const uint32_t rows = n_tok * pool.n_kv_head, per = 256 / 8 * READ;
     return bp_launch(true, kernel, dim3((rows + per - 1) / per), dim3(256), 0, s, a);
   };
   const bool vec = vec8(k) && vec8(v);
   if (head_dim == 128)
-    return vec ? (bf ? go(kv4_read_kernel<true, true, 128>, 16) : go(kv4_read_kernel<false, true, 128>, 16))
-               : (bf ? go(kv4_read_kernel<true, false, 128>, 16) : go(kv4_read_kernel<false, false, 128>, 16));
-  return vec ? (bf ? go(kv4_read_kernel<true, true, 64>, 8) : go(kv4_read_kernel<false, true, 64>, 8))
-             : (bf ? go(kv4_read_kernel<true, false, 64>, 8) : go(kv4_read_kernel<false, false, 64>, 8));
+    return vec ? (bf ? go(kv4_read_kernel<true, true, 128>) : go(kv4_read_kernel<false, true, 128>))
+               : (bf ? go(kv4_read_kernel<true, false, 128>) : go(kv4_read_kernel<false, false, 128>));
+  return vec ? (bf ? go(kv4_read_kernel<true, true, 64>) : go(kv4_read_kernel<false, true, 64>))
+             : (bf ? go(kv4_read_kernel<true, false, 64>) : go(kv4_read_kernel<false, false, 64>));
 }

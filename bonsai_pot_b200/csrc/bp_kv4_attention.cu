@@ -62,14 +62,6 @@ __device__ __forceinline__ void mma_1688_first(float (&d)[4], uint32_t a0, uint3
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
 }
-// (x & mask) | 0x64006400 in one instruction: it has room for one constant, so the other one is a kernel argument
-__device__ __forceinline__ __half2 biased(uint32_t x, uint32_t mask, uint32_t bias) {
-  const uint32_t r = lop3<0xea>(x, mask, bias);
-  return *reinterpret_cast<const __half2*>(&r);
-}
-__device__ __forceinline__ __half2 h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-__device__ __forceinline__ uint32_t u2(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-
 // State of one warp for NT tiles of eight rows.
 template <int D, int NT>
 struct WarpState {

@@ -104,6 +104,23 @@ __device__ __forceinline__ void store8(uint16_t* p, const float* x) {
   }
 }
 
+// Division of numbers below 2^31 by one divisor: with l = ceil(log2 d) and m = floor(2^32 (2^l - d) / d) + 1 the quotient is
+// (mulhi(m, n) + n) >> l (Granlund and Montgomery, 1994).
+struct FastDiv {
+  uint32_t d, m, l;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t by) : d(by), l(0) {
+    while ((1ull << l) < by) l++;
+    m = static_cast<uint32_t>((((1ull << l) - by) << 32) / by + 1);
+  }
+  __device__ uint32_t quotient(uint32_t n) const { return (__umulhi(m, n) + n) >> l; }
+};
+
+__device__ __forceinline__ __half2 h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+__device__ __forceinline__ uint32_t u2(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// (x & mask) | 0x64006400 in one instruction: it has room for one constant, so the other one comes as a kernel argument
+__device__ __forceinline__ __half2 biased(uint32_t x, uint32_t mask, uint32_t bias) { return h2(lop3<0xea>(x, mask, bias)); }
+
 __device__ __forceinline__ void note_range(uint32_t* err) { *reinterpret_cast<volatile uint32_t*>(err) = 1; }
 
 }  // namespace bp

@@ -44,6 +44,106 @@ struct RopeArgs {
   float eps, sign;  // sign: -1 turns back
 };
 
+// Rows of 16-byte aligned chunks of eight dims, of which no pair's two dims share a chunk with another layout's: a thread has one
+// slot of 16 dims (chunks c and c + rot / 16 of the half layout, neighbours of the interleaved one, what is only copied behind) of R heads of
+// a token, so that the table's row is read once for them and R rows are on their way at a time.
+// G: lanes per row, the slots rounded up to a power of two, for the norm's sum.
+template <bool BF, bool NORM, int R>
+__global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs a, const uint32_t log_g, const FastDiv groups_by) {
+  pdl_launch_dependents();
+  const uint32_t at = blockIdx.x * 256 + threadIdx.x, slot = at & ((1u << log_g) - 1), item = at >> log_g;
+  const uint32_t groups = groups_by.d, tok = groups_by.quotient(item), head0 = item - tok * groups, slots = a.dim / 16, turned = a.rope.rot / 16;
+  const bool in = tok < a.n_tok && slot < slots;
+  // the two chunks of the slot
+  uint32_t c0 = 2 * slot, c1 = 2 * slot + 1;
+  if (slot < turned && a.rope.layout == BP_ROPE_HALF) {
+    c0 = slot;
+    c1 = slot + turned;
+  }
+  pdl_wait();
+  int32_t pos = in ? a.positions[tok] : -1;
+  if (pos >= 0 && static_cast<uint32_t>(pos) >= a.rope.n_pos) {
+    note_range(a.err);
+    pos = -1;
+  }
+  const bool go = pos >= 0;
+  uint4 raw[R][2];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const uint32_t head = head0 + r * groups;
+    if (go && head < a.n_head) {
+      const uint16_t* x = a.x.data + tok * a.x.tok + head * a.x.head;
+      raw[r][0] = *reinterpret_cast<const uint4*>(x + 8 * c0);
+      raw[r][1] = *reinterpret_cast<const uint4*>(x + 8 * c1);
+    } else {
+      raw[r][0] = raw[r][1] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  float cs[8], sn[8];  // of the slot's eight pairs
+  const bool turns = go && slot < turned;
+  if (turns) {
+    const float4* row = reinterpret_cast<const float4*>(a.rope.table + static_cast<size_t>(pos) * (a.rope.rot / 2) + 8 * slot);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float4 t = row[i];
+      cs[2 * i] = t.x;
+      sn[2 * i] = t.y * a.sign;
+      cs[2 * i + 1] = t.z;
+      sn[2 * i + 1] = t.w * a.sign;
+    }
+  }
+  float w[16];
+  if (NORM && go) {
+    if (reinterpret_cast<uintptr_t>(a.w) % 16 == 0) {
+      load8<BF, true>(a.w + 8 * c0, w);
+      load8<BF, true>(a.w + 8 * c1, w + 8);
+    } else {
+      load8<BF, false>(a.w + 8 * c0, w);
+      load8<BF, false>(a.w + 8 * c1, w + 8);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const uint32_t head = head0 + r * groups;
+    float x[16];
+    unpack8<BF>(raw[r][0], x);
+    unpack8<BF>(raw[r][1], x + 8);
+    if (NORM) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; i++) sum += x[i] * x[i];
+      for (uint32_t o = 1; o < 1u << log_g; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const float scale = __fdiv_rn(1.f, __fsqrt_rn(sum / a.dim + a.eps));
+      if (go) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) x[i] = x[i] * scale * w[i];
+      }
+    }
+    if (turns) {
+      if (a.rope.layout == BP_ROPE_HALF) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float y = x[i] * cs[i] - x[8 + i] * sn[i];
+          x[8 + i] = x[8 + i] * cs[i] + x[i] * sn[i];
+          x[i] = y;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float y = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i];
+          x[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
+          x[2 * i] = y;
+        }
+      }
+    }
+    if (go && head < a.n_head) {
+      uint16_t* out = a.out.data + tok * a.out.tok + head * a.out.head;
+      *reinterpret_cast<uint4*>(out + 8 * c0) = pack8<BF>(x);
+      *reinterpret_cast<uint4*>(out + 8 * c1) = pack8<BF>(x + 8);
+    }
+  }
+}
+
 // Any even dims, strides and alignment: a warp per row, a lane per pair, two bytes at a time.
 template <bool BF>
 __global__ void __launch_bounds__(256) rope_any_kernel(const RopeArgs a) {
@@ -116,6 +216,20 @@ cudaError_t bp_launch_rope_fill(cudaStream_t s, const bp_rope_config& cfg, float
 cudaError_t bp_launch_rope(bp_paged_ctx* c, cudaStream_t s, bool bf, const Rows& x, const Rows& out, uint32_t n_tok, uint32_t n_head,
                            uint32_t head_dim, const int32_t* positions, const Rope& rope, const uint16_t* w_norm, float eps, bool inverse) {
   const RopeArgs a{x, out, positions, w_norm, c->err_dev, rope, n_tok, n_head, head_dim, eps, inverse ? -1.f : 1.f};
+  auto chunked = [](const Rows& r) { return reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && r.tok % 8 == 0 && r.head % 8 == 0; };
+  if (head_dim % 16 == 0 && rope.rot % 16 == 0 && chunked(x) && chunked(out) && reinterpret_cast<uintptr_t>(rope.table) % 16 == 0) {
+    uint32_t log_g = 0;
+    while (1u << log_g < head_dim / 16) log_g++;
+    // heads of a thread: several where there are rows enough to fill the device with one wave of such threads
+    auto go = [&](auto kernel, uint32_t r) {
+      const uint32_t groups = (n_head + r - 1) / r;
+      const uint64_t blocks = ((static_cast<uint64_t>(n_tok) * groups << log_g) + 255) / 256;
+      return bp_launch(true, kernel, dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, s, a, log_g, FastDiv(groups));
+    };
+    const bool many = (static_cast<uint64_t>(n_tok) * n_head << log_g) / 4 >= 2048ull * c->sm_count;
+    if (w_norm) return many ? go(bf ? rope_rows_kernel<true, true, 4> : rope_rows_kernel<false, true, 4>, 4) : go(bf ? rope_rows_kernel<true, true, 1> : rope_rows_kernel<false, true, 1>, 1);
+    return many ? go(bf ? rope_rows_kernel<true, false, 4> : rope_rows_kernel<false, false, 4>, 4) : go(bf ? rope_rows_kernel<true, false, 1> : rope_rows_kernel<false, false, 1>, 1);
+  }
   const uint32_t rows = n_tok * n_head;
   return bp_launch(true, bf ? rope_any_kernel<true> : rope_any_kernel<false>, dim3((rows + 7) / 8), dim3(256), 0, s, a);
 }
