@@ -19,28 +19,14 @@
 // the keys, so that results do not depend on who comes when.
 #include <type_traits>
 
-#include "bp_paged.cuh"
+#include "bp_kv4_attention.cuh"
 
 namespace {
 
 using namespace bp;
+using namespace bp::kv4;
 
-constexpr unsigned FULL = 0xffffffffu;
-constexpr float NEG_BIG = -1e30f;
-constexpr float P_UP = 10.f;   // P is stored as f16 times 2^10: it keeps its bits down to 2^-24 of the maximum
 constexpr uint32_t UNIT = 64;  // keys a warp works on between two looks at the maximum
-
-struct AttnArgs {
-  Pool pool;
-  Rows q, out;
-  const int32_t *q_start, *kv_len, *page_table;
-  uint32_t* err;
-  uint32_t n_req, n_head, group, total_q, max_q, max_kv, table_stride, window;
-  float scale_log2;
-  uint32_t bias;  // 0x64006400: two f16 numbers 1024
-  uint32_t bf;    // activations are bfloat16
-  uint32_t q_vec; // rows of q are 16-byte aligned
-};
 
 // The token of a 16-token tile that a lane's MMA row r holds. K rows 2 j and 2 j + 1 then differ in parity and the values of
 // MMA columns 2 t (t = 0 .. 3) lie in tokens that differ mod 4: no shared-memory bank is met twice (rows of 64 bytes).
@@ -330,7 +316,6 @@ __device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4]
   }
 }
 
-constexpr uint32_t WAIT_LIMIT = 1u << 20;  // polls before a warp gives up on a copy
 
 // One CTA per SM. A warp fetches ahead into RING buffers, K and V of its units in turn: one is worked on, the others are on
 // their way. With two (16 warps of 128 registers) the buffers in flight did not cover the latency of a loaded memory.
@@ -462,22 +447,6 @@ __device__ __noinline__ void clear_scales(uint8_t* buf, uint32_t pages, int from
   }
   fence_proxy_async();  // the next copy into the buffer comes behind these
   __syncwarp();
-}
-
-// Four dims of an output row.
-__device__ __forceinline__ void store4(bool bf, uint16_t* p, float a, float b, float c, float d) {
-  const uint32_t x = bf ? pack2<true>(a, b) : pack2<false>(a, b), y = bf ? pack2<true>(c, d) : pack2<false>(c, d);
-  if ((reinterpret_cast<uintptr_t>(p) & 7) == 0) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(x, y);
-  } else {
-    p[0] = static_cast<uint16_t>(x);
-    p[1] = static_cast<uint16_t>(x >> 16);
-    p[2] = static_cast<uint16_t>(y);
-    p[3] = static_cast<uint16_t>(y >> 16);
-  }
-}
-__device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, int q0, uint32_t head, uint32_t row) {
-  return a.out.data + static_cast<int64_t>(q0 + row / a.group) * a.out.tok + static_cast<int64_t>(head * a.group + row % a.group) * a.out.head;
 }
 
 // A warp: row `row` of the `n` partial results at part(k) of an item, in order, becomes the output's row (to == null) or that of the
@@ -709,7 +678,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
     bool fresh = true, from_start = false, ok = true;
     uint32_t first = 0;          // of this piece; cur.unit is its place in the item
     uint32_t b = 0, phase = 0;   // the buffer that is worked on, the phases of the barriers' next use
-    auto wait = [&]() { return mbar_wait(bar + 8 * b, phase >> b & 1, WAIT_LIMIT); };
+    auto wait = [&]() { return wait_phase(bar + 8 * b, phase >> b & 1); };
     auto done = [&]() {
       phase ^= 1u << b;
       if (++b == RING) b = 0;
@@ -808,7 +777,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
     if (!ok) {  // the wait gave up: what is on its way comes before the buffers are given back
       if (lane == 0) reinterpret_cast<volatile uint32_t*>(a.err)[1] = 1;
       for (; flying > 0; flying--) {
-        (void)mbar_wait(bar + 8 * b, phase >> b & 1, DRAIN_LIMIT);
+        (void)wait_phase(bar + 8 * b, phase >> b & 1);
         if (++b == RING) b = 0;
       }
     }
@@ -904,6 +873,8 @@ cudaError_t bp_kv4_attention_init(bp_paged_ctx* c) {
   return cudaMemset(c->counters, 0, static_cast<size_t>(c->sm_count) * sizeof(uint32_t));
 }
 
+constexpr uint32_t FEW_ROWS = 48;
+
 cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, const Pool& pool, uint32_t head_dim, const bp_kv4_attn& in) {
   AttnArgs a;
   a.pool = pool;
@@ -925,6 +896,7 @@ cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, co
   a.bias = 0x64006400u;
   a.bf = bf;
   a.q_vec = reinterpret_cast<uintptr_t>(in.q.data) % 16 == 0 && in.q.tok_stride % 8 == 0 && in.q.head_stride % 8 == 0;
+  if (static_cast<uint64_t>(a.max_q) * a.group > FEW_ROWS) return bp_launch_kv4_prefill(c, s, head_dim, a);
   return with_kernel(head_dim, a.max_q * a.group > 8, pool.page, [&](auto kernel, auto shape) {
     return bp_launch(true, kernel, dim3(c->sm_count), dim3(shape.THREADS), shape.SMEM, s, a, c->partials, c->counters);
   });

@@ -1,0 +1,59 @@
+// What the two attention kernels over 4-bit pages share (bp_kv4_attention.cu: few rows per request; bp_kv4_prefill.cu: many).
+#pragma once
+
+#include "bp_paged.cuh"
+
+namespace bp {
+namespace kv4 {
+
+constexpr unsigned FULL = 0xffffffffu;
+constexpr float NEG_BIG = -1e30f;
+constexpr float P_UP = 10.f;   // P is stored as f16 times 2^10: it keeps its bits down to 2^-24 of the maximum
+
+struct AttnArgs {
+  Pool pool;
+  Rows q, out;
+  const int32_t *q_start, *kv_len, *page_table;
+  uint32_t* err;
+  uint32_t n_req, n_head, group, total_q, max_q, max_kv, table_stride, window;
+  float scale_log2;
+  uint32_t bias;  // 0x64006400: two f16 numbers 1024
+  uint32_t bf;    // activations are bfloat16
+  uint32_t q_vec; // rows of q are 16-byte aligned
+};
+// A bounded wait for a barrier's phase: false after 2^20 polls or two seconds (a poll may suspend its thread for long).
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity) {
+  if (mbar_test(bar, parity)) return true;
+  unsigned long long t0 = 0, t;
+  for (uint32_t i = 0; i < 1u << 20; i++) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 15) == 0) {
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+      if (t0 == 0) t0 = t;
+      if (t - t0 > 2000000000ull) return false;
+    }
+  }
+  return false;
+}
+
+// Four dims of an output row.
+__device__ __forceinline__ void store4(bool bf, uint16_t* p, float a, float b, float c, float d) {
+  const uint32_t x = bf ? pack2<true>(a, b) : pack2<false>(a, b), y = bf ? pack2<true>(c, d) : pack2<false>(c, d);
+  if ((reinterpret_cast<uintptr_t>(p) & 7) == 0) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(x, y);
+  } else {
+    p[0] = static_cast<uint16_t>(x);
+    p[1] = static_cast<uint16_t>(x >> 16);
+    p[2] = static_cast<uint16_t>(y);
+    p[3] = static_cast<uint16_t>(y >> 16);
+  }
+}
+__device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, int q0, uint32_t head, uint32_t row) {
+  return a.out.data + static_cast<int64_t>(q0 + row / a.group) * a.out.tok + static_cast<int64_t>(head * a.group + row % a.group) * a.out.head;
+}
+
+}  // namespace kv4
+}  // namespace bp
+
+cudaError_t bp_kv4_prefill_init(bp_paged_ctx* c);
+cudaError_t bp_launch_kv4_prefill(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, const bp::kv4::AttnArgs& a);

@@ -1,0 +1,625 @@
+// Attention of many queries per request over a paged 4-bit cache, on the 5th-generation tensor cores (include/bonsai_paged.h;
+// few queries: bp_kv4_attention.cu).
+//
+// An item is one KV head of one request and NQ query tiles of 128 rows (a row is a query head of a token). Keys come in tiles of
+// 64. Roles of a CTA, one CTA per SM:
+//   expanders (4 warps)     codes -> f16 operand tiles in shared memory, K and V, once for all query tiles of the item. Every
+//                           value is an f16 number (the format's choice of m and d): nothing rounds. The next tile's codes are
+//                           on their way in registers meanwhile. Places that hold no key of the request become zeros.
+//   S issuer X (1 thread)   S_X = Q_X K^T (tcgen05.mma kind::f16, M 128, N 64) into one of two 64-column buffers in TMEM
+//   softmax X (4 warps)     thread = row = TMEM lane: masks, running maximum and sum, P as f16 over the tile's S buffer; O_X is
+//                           rescaled in TMEM only when a row's maximum grew by more than 2^5 (P stays below 2^15 meanwhile)
+//   O issuer X (1 thread)   O_X += P_X V (P from TMEM as the A operand, V as the MN-major B operand)
+// The key tiles of all items lie in one line, of which every CTA takes an equal stretch; an item that lies in several CTAs is joined by the
+// one that comes last, in the order of its keys (as in bp_kv4_attention.cu). Every wait is bounded; a timeout sets the context's error word and
+// the CTA winds down and frees its TMEM.
+#include <type_traits>
+
+#include "bp_kv4_attention.cuh"
+
+namespace {
+
+using namespace bp;
+using namespace bp::kv4;
+
+constexpr uint32_t BM = 128, BN = 64;  // query rows of a tile, keys of a tile
+constexpr uint32_t SLOTS = 4;          // K and V tiles in shared memory
+constexpr float GROW = 5.f;            // log2 by which a maximum may grow before O is rescaled; P_UP + GROW stays below 16
+
+template <int D, uint32_t NQ>
+struct Shape {
+  static constexpr uint32_t ROWS = BM * NQ;
+  static constexpr uint32_t Q_B = BM * D * 2, KV_B = BN * D * 2;          // operand tiles: D / 64 chunks of rows of 128 bytes
+  static constexpr uint32_t OFF_K = NQ * Q_B, OFF_V = OFF_K + SLOTS * KV_B, SMEM = OFF_V + SLOTS * KV_B + 1024;
+  static constexpr uint32_t TM_O = 128 * NQ, TMEM_COLS = 256 * NQ;        // S_X at 128 X, O_X at TM_O + 128 X
+  static constexpr uint32_t FIRST_EXPANDER = 4, FIRST_SOFTMAX = 8;        // warps 0, 1: O issuers, 2, 3: S issuers
+  static constexpr uint32_t NWARP = FIRST_SOFTMAX + 4 * NQ, THREADS = 32 * NWARP;
+  static constexpr uint32_t STRIDE = D + 4, PARTIAL = ROWS * STRIDE;      // floats of a row of a partial result (o, m, l), of one
+};
+
+struct Request {
+  int q0, q_len, kv_len;
+  uint32_t rows;
+};
+__device__ __forceinline__ Request request(const AttnArgs& a, uint32_t r, bool report) {
+  Request q;
+  const int start = a.q_start[r], stop = a.q_start[r + 1], keys = a.kv_len[r];
+  q.q0 = max(start, 0);
+  const int given_q = max(min(stop, static_cast<int>(a.total_q)) - q.q0, 0), given_kv = max(keys, 0);
+  q.q_len = min(given_q, static_cast<int>(a.max_q));
+  q.kv_len = min(given_kv, static_cast<int>(min(a.max_kv, a.table_stride << a.pool.log_page)));
+  if (report && (given_q > q.q_len || given_kv > q.kv_len)) note_range(a.err);
+  q.rows = static_cast<uint32_t>(q.q_len) * a.group;
+  return q;
+}
+// Keys [low, high) that the rows [row0, row0 + rows) of a request see, of all of them together; key tiles from low's on, one at least (its
+// rows have zeros to write).
+struct Keys {
+  int low, high;
+  uint32_t tiles;
+  __device__ int first() const { return low & ~static_cast<int>(BN - 1); }
+};
+__device__ __forceinline__ Keys keys_of(const AttnArgs& a, const Request& q, uint32_t row0, uint32_t rows) {
+  Keys k;
+  const int t0 = static_cast<int>(row0 / a.group), t1 = static_cast<int>((min(row0 + rows, q.rows) - 1) / a.group), past = q.kv_len - q.q_len;
+  k.high = max(past + t1 + 1, 0);
+  k.low = a.window ? min(max(past + t0 + 1 - static_cast<int>(min(a.window, 0x40000000u)), 0), k.high) : 0;
+  k.tiles = max((static_cast<uint32_t>(k.high - k.first()) + BN - 1) / BN, 1u);
+  return k;
+}
+
+// A place in the line: item (r, x, head) of `keys.tiles` tiles, tile `at` of it, the item's first tile being the line's `start`.
+struct Cursor {
+  Request q;
+  Keys keys;
+  uint32_t r, x, head, at, start;
+};
+
+// Byte offset of 16-byte unit u of row r in an operand tile of `rows` rows: chunks of 64 dims, 128-byte swizzle.
+__device__ __forceinline__ uint32_t oper_off(uint32_t rows, uint32_t r, uint32_t u) { return (u >> 3) * (rows * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4); }
+
+// A quarter of the codes of one token's K and V (an expander warp has the same quarter of every token), and their scales.
+template <int D>
+struct Raw {
+  static constexpr int NB = D / 32;
+  uint32_t k[NB], v[NB], kd[NB / 2], km[NB / 2], vd[NB / 2], vm[NB / 2];
+};
+template <int D>
+__device__ __forceinline__ void ask(Raw<D>& w, const AttnArgs& a, uint32_t id, int key, uint32_t head, uint32_t quarter) {
+  using L = PoolLayout<D>;
+  constexpr int NB = D / 32;
+  if (id >= a.pool.n_pages) {  // no key of the request, or a page id outside the pool
+#pragma unroll
+    for (int i = 0; i < NB; i++) w.k[i] = w.v[i] = 0;
+#pragma unroll
+    for (int i = 0; i < NB / 2; i++) w.kd[i] = w.km[i] = w.vd[i] = w.vm[i] = 0;
+    return;
+  }
+  const uint32_t page = a.pool.page, tok = static_cast<uint32_t>(key) & (page - 1);
+  const uint8_t* k = a.pool.data + (static_cast<uint64_t>(id) * a.pool.n_kv_head + head) * (page * L::TOK);
+  const uint8_t* v = k + L::v(page);
+  const uint32_t scales = L::kd(page) + tok * 2 * NB, kv = tok * L::ROW, gap = page * 2 * NB;
+  if constexpr (NB == 4) {
+    const uint4 x = *reinterpret_cast<const uint4*>(k + kv + 16 * quarter), y = *reinterpret_cast<const uint4*>(v + kv + L::v16(tok, 2 * quarter, 0));
+    w.k[0] = x.x, w.k[1] = x.y, w.k[2] = x.z, w.k[3] = x.w;
+    w.v[0] = y.x, w.v[1] = y.y, w.v[2] = y.z, w.v[3] = y.w;
+    const uint2 e = *reinterpret_cast<const uint2*>(k + scales), f = *reinterpret_cast<const uint2*>(k + scales + gap);
+    const uint2 g = *reinterpret_cast<const uint2*>(v + scales), h = *reinterpret_cast<const uint2*>(v + scales + gap);
+    w.kd[0] = e.x, w.kd[1] = e.y, w.km[0] = f.x, w.km[1] = f.y;
+    w.vd[0] = g.x, w.vd[1] = g.y, w.vm[0] = h.x, w.vm[1] = h.y;
+  } else {
+    const uint2 x = *reinterpret_cast<const uint2*>(k + kv + 8 * quarter), y = *reinterpret_cast<const uint2*>(v + kv + 8 * quarter);
+    w.k[0] = x.x, w.k[1] = x.y;
+    w.v[0] = y.x, w.v[1] = y.y;
+    w.kd[0] = *reinterpret_cast<const uint32_t*>(k + scales), w.km[0] = *reinterpret_cast<const uint32_t*>(k + scales + gap);
+    w.vd[0] = *reinterpret_cast<const uint32_t*>(v + scales), w.vm[0] = *reinterpret_cast<const uint32_t*>(v + scales + gap);
+  }
+}
+// Eight codes at bits 4 i of both halves -> four words of two f16 values m + d q.
+__device__ __forceinline__ uint4 expand8(uint32_t w, __half2 d, __half2 m, uint32_t bias) {
+  const __half2 off = __float2half2_rn(-1024.f), off16 = __float2half2_rn(-64.f), sixteenth = __float2half2_rn(0.0625f);
+  const uint32_t y = w >> 8;
+  return make_uint4(u2(__hfma2(__hadd2(biased(w, 0x000f000fu, bias), off), d, m)), u2(__hfma2(__hfma2(biased(w, 0x00f000f0u, bias), sixteenth, off16), d, m)),
+                    u2(__hfma2(__hadd2(biased(y, 0x000f000fu, bias), off), d, m)), u2(__hfma2(__hfma2(biased(y, 0x00f000f0u, bias), sixteenth, off16), d, m)));
+}
+// One token's quarter into the K or V operand tile. A V word's halves are dims i and i + 4 of a group of eight: that order stays, and
+// the end of an item puts it right.
+template <int D, bool V>
+__device__ __forceinline__ void put(const Raw<D>& w, uint8_t* tile, uint32_t row, uint32_t quarter, uint32_t bias) {
+  constexpr int NB = D / 32;
+#pragma unroll
+  for (int b = 0; b < NB; b++) {
+    const uint32_t sel = b & 1 ? 0x3232u : 0x1010u;
+    const __half2 d = h2(prmt(V ? w.vd[b >> 1] : w.kd[b >> 1], 0, sel)), m = h2(prmt(V ? w.vm[b >> 1] : w.km[b >> 1], 0, sel));
+    const uint32_t codes = V ? prmt(w.v[b >> 1], w.v[NB / 2 + (b >> 1)], b & 1 ? 0x7632u : 0x5410u) : w.k[b];
+    *reinterpret_cast<uint4*>(tile + oper_off(BN, row, 4 * b + quarter)) = expand8(codes, d, m, bias);
+  }
+}
+// Column of O that holds dim i of a group of eight.
+__host__ __device__ constexpr int column_of(int i) { return i < 4 ? 2 * i : 2 * (i - 4) + 1; }
+
+// What several CTAs have of one item: the first of them, how many.
+struct Join {
+  uint32_t first_cta, n, last;
+};
+
+template <int D, uint32_t NQ>
+__global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(const __grid_constant__ AttnArgs a, float* __restrict__ scratch, uint32_t* __restrict__ counters) {
+  using S = Shape<D, NQ>;
+  constexpr uint32_t THREADS = S::THREADS;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t k_full[SLOTS], v_full[SLOTS], k_empty[NQ][SLOTS], v_empty[NQ][SLOTS];
+  __shared__ __align__(8) uint64_t s_ready[NQ][2], p_ready[NQ][2], p_free[NQ][2], o_done[NQ], drained;
+  __shared__ float row_scale[S::ROWS];  // of a row's queries: the power of two that they were divided by
+  __shared__ uint32_t line[THREADS + 1];
+  __shared__ Cursor cur;
+  __shared__ Join join_s;
+  __shared__ uint32_t tmem_base_s;
+  __shared__ volatile uint32_t abort_s;
+
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (uint32_t i = 0; i < SLOTS; i++) {
+      mbar_init(smem_u32(&k_full[i]), 4);
+      mbar_init(smem_u32(&v_full[i]), 4);
+      for (uint32_t x = 0; x < NQ; x++) {
+        mbar_init(smem_u32(&k_empty[x][i]), 1);
+        mbar_init(smem_u32(&v_empty[x][i]), 1);
+      }
+    }
+    for (uint32_t x = 0; x < NQ; x++) {
+      for (uint32_t b = 0; b < 2; b++) {
+        mbar_init(smem_u32(&s_ready[x][b]), 1);
+        mbar_init(smem_u32(&p_ready[x][b]), 4);
+        mbar_init(smem_u32(&p_free[x][b]), 1);
+      }
+      mbar_init(smem_u32(&o_done[x]), 1);
+    }
+    abort_s = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(smem_u32(&tmem_base_s), S::TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_s;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // (after one wait has given up no other one waits)
+  auto waitx = [&](uint64_t* bar, uint32_t parity) {
+    if (abort_s) return;
+    if (!wait_phase(smem_u32(bar), parity)) {
+      abort_s = 1;
+      reinterpret_cast<volatile uint32_t*>(a.err)[1] = 1;
+    }
+  };
+
+  // ---- the line of key tiles, and this CTA's stretch [c0, c1) of it ----
+  const uint32_t per = (a.n_req + THREADS - 1) / THREADS;
+  auto tiles_of = [&](const Request& q) {  // of all items of a request
+    uint32_t n = 0;
+    for (uint32_t row0 = 0; row0 < q.rows; row0 += S::ROWS) n += keys_of(a, q, row0, S::ROWS).tiles;
+    return n * a.pool.n_kv_head;
+  };
+  {
+    uint32_t units = 0;
+    for (uint32_t r = threadIdx.x * per; r < min((threadIdx.x + 1) * per, a.n_req); r++) units += tiles_of(request(a, r, blockIdx.x == 0));
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(FULL, units, o);
+      if (lane >= o) units += x;
+    }
+    line[threadIdx.x + 1] = units;  // within the warp
+    __syncthreads();
+    uint32_t before = 0;
+    for (uint32_t w = 0; w < warp; w++) before += line[32 * (w + 1)];
+    __syncthreads();
+    line[threadIdx.x + 1] += before;
+    if (threadIdx.x == 0) line[0] = 0;
+    __syncthreads();
+  }
+  const uint32_t total = line[THREADS], share = (total + gridDim.x - 1) / gridDim.x;
+  const uint32_t c0 = min(static_cast<uint64_t>(blockIdx.x) * share, static_cast<uint64_t>(total)), c1 = c0 + min(share, total - c0);
+  if (threadIdx.x == 0 && c0 < c1) {
+    uint32_t at = 0;
+    while (line[at + 1] <= c0) at++;
+    uint32_t left = c0 - line[at];
+    bool found = false;
+    for (uint32_t r = at * per; r < a.n_req && !found; r++) {
+      const Request q = request(a, r, false);
+      for (uint32_t x = 0; x * S::ROWS < q.rows; x++) {
+        const Keys k = keys_of(a, q, x * S::ROWS, S::ROWS);
+        const uint32_t n = k.tiles * a.pool.n_kv_head;
+        if (left < n) {
+          const uint32_t head = left / k.tiles, tile = left - head * k.tiles;
+          cur = Cursor{q, k, r, x, head, tile, c0 - tile};
+          found = true;
+          break;
+        }
+        left -= n;
+      }
+    }
+  }
+  __syncthreads();
+
+  // Barrier phases count on across items: done = key tiles so far, pieces = pieces so far.
+  uint32_t done = 0, pieces = 0;
+  for (uint32_t pos = c0; pos < c1;) {
+    const Request q = cur.q;
+    const Keys keys = cur.keys;
+    const uint32_t head = cur.head, row0 = cur.x * S::ROWS, first = cur.at, n = min(keys.tiles - first, c1 - pos);
+    const uint32_t start = cur.start;
+    const int key_first = keys.first() + static_cast<int>(first * BN);
+    // ---- queries -> f16, each row divided by the power of two of its largest element ----
+    {
+      constexpr uint32_t U = D / 8, ITERS = (S::ROWS * U + THREADS - 1) / THREADS;
+      static_assert(THREADS % U == 0 && (S::ROWS * U) % 32 == 0, "rows are groups of U lanes");
+#pragma unroll
+      for (uint32_t k = 0; k < ITERS; k++) {
+        const uint32_t i = threadIdx.x + k * THREADS, r = i / U, u = i % U;
+        if (i >= S::ROWS * U) break;  // (whole warps)
+        uint4 raw = make_uint4(0, 0, 0, 0);
+        if (row0 + r < q.rows) {
+          const uint16_t* p = a.q.data + static_cast<int64_t>(q.q0 + (row0 + r) / a.group) * a.q.tok + static_cast<int64_t>(head * a.group + (row0 + r) % a.group) * a.q.head + 8 * u;
+          if (a.q_vec) {
+            raw = *reinterpret_cast<const uint4*>(p);
+          } else {
+            uint32_t h[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) h[e] = p[e];
+            raw = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+          }
+        }
+        float x[8], big = 0.f;
+        if (a.bf) unpack8<true>(raw, x);
+        else unpack8<false>(raw, x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[e]));
+#pragma unroll
+        for (uint32_t o = 1; o < U; o <<= 1) big = fmaxf(big, __shfl_xor_sync(FULL, big, o));
+        const uint32_t ebits = min(max(__float_as_uint(big) & 0x7f800000u, 0x00800000u), 0x7e800000u);
+        const float up = copysignf(__uint_as_float(0x7f000000u - ebits), a.scale_log2);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] *= up;
+        *reinterpret_cast<uint4*>(smem + (r / BM) * S::Q_B + oper_off(BM, r % BM, u)) = pack8<false>(x);
+        // (never 0: a masked score, -infinity, stays what it is)
+        if (u == 0) row_scale[r] = fmaxf(fabsf(a.scale_log2) * __uint_as_float(ebits), 1e-37f);
+      }
+    }
+    fence_proxy_async();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+
+    if (warp < 2) {
+      // ---------------- O_X += P_X V ----------------
+      const uint32_t x = warp;
+      if (x < NQ && elect_one()) {
+        constexpr uint32_t IDESC = umma_idesc(1, 0, 0, 0, 1, BM, D);              // f32 += f16 (TMEM) x f16 (MN-major)
+        const uint64_t dmn = umma_desc_sw128(0, BN * 128, 1024);                  // the next 64 dims a chunk on, 8 keys 1 KB
+        const uint32_t s_col = tmem + x * 128, o_col = tmem + S::TM_O + x * 128;
+        for (uint32_t i = 0; i < n; i++) {
+          const uint32_t c = done + i, s = c % SLOTS, b = c & 1;
+          waitx(&p_ready[x][b], (c >> 1) & 1);
+          waitx(&v_full[s], (c / SLOTS) & 1);
+          if (abort_s) break;
+          tc_fence_after();
+          const uint64_t vb = dmn + ((smem_base + S::OFF_V + s * S::KV_B) >> 4);
+#pragma unroll
+          for (uint32_t ks = 0; ks < BN / 16; ks++) umma_f16_ts(o_col, s_col + 64 * b + 8 * ks, vb + ks * (16 * 128 >> 4), IDESC, (i | ks) ? 1u : 0u);
+          umma_commit(smem_u32(&p_free[x][b]));
+          umma_commit(smem_u32(&v_empty[x][s]));
+        }
+        umma_commit(smem_u32(&o_done[x]));
+      }
+    } else if (warp < S::FIRST_EXPANDER) {
+      // ---------------- S_X = Q_X K^T, up to two tiles ahead of P V ----------------
+      const uint32_t x = warp - 2;
+      if (x < NQ && elect_one()) {
+        constexpr uint32_t IDESC = umma_idesc(1, 0, 0, 0, 0, BM, BN);
+        const uint64_t dk = umma_desc_sw128(0, 16, 1024);
+        const uint64_t qa = dk + ((smem_base + x * S::Q_B) >> 4);
+        for (uint32_t i = 0; i < n; i++) {
+          const uint32_t c = done + i, s = c % SLOTS, b = c & 1;
+          waitx(&k_full[s], (c / SLOTS) & 1);
+          if (c >= 2) waitx(&p_free[x][b], ((c >> 1) - 1) & 1);
+          if (abort_s) break;
+          tc_fence_after();
+          const uint64_t kb = dk + ((smem_base + S::OFF_K + s * S::KV_B) >> 4);
+#pragma unroll
+          for (uint32_t ks = 0; ks < D / 16; ks++)  // chunk ks / 4, 32 bytes per step inside it
+            umma_f16(tmem + x * 128 + 64 * b, qa + (ks >> 2) * (BM * 128 >> 4) + (ks & 3) * 2, kb + (ks >> 2) * (BN * 128 >> 4) + (ks & 3) * 2, IDESC, ks);
+          umma_commit(smem_u32(&s_ready[x][b]));
+        }
+      }
+    } else if (warp < S::FIRST_SOFTMAX) {
+      // ---------------- codes -> operand tiles ----------------
+      const uint32_t quarter = warp - S::FIRST_EXPANDER;
+      const int32_t* table = a.page_table + static_cast<size_t>(cur.r) * a.table_stride;
+      auto id_of = [&](int key) {
+        if (key < keys.low || key >= keys.high) return 0xffffffffu;  // keys behind `high` are nobody's here: their columns are masked
+        const uint32_t id = static_cast<uint32_t>(table[key >> a.pool.log_page]);
+        if (id >= a.pool.n_pages) note_range(a.err);
+        return id;
+      };
+      Raw<D> raw[2];
+      uint32_t ids[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) ask<D>(raw[h], a, id_of(key_first + static_cast<int>(lane + 32 * h)), key_first + static_cast<int>(lane + 32 * h), head, quarter);
+#pragma unroll
+      for (int h = 0; h < 2; h++) ids[h] = n > 1 ? id_of(key_first + static_cast<int>(BN + lane + 32 * h)) : 0xffffffffu;
+      for (uint32_t i = 0; i < n; i++) {
+        const uint32_t c = done + i, s = c % SLOTS;
+        Raw<D> mine[2] = {raw[0], raw[1]};
+        const int key = key_first + static_cast<int>((i + 1) * BN + lane);
+        if (i + 1 < n) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) ask<D>(raw[h], a, ids[h], key + 32 * h, head, quarter);
+        }
+        if (i + 2 < n) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) ids[h] = id_of(key + static_cast<int>(BN) + 32 * h);
+        }
+        if (c >= SLOTS)
+          for (uint32_t x = 0; x < NQ; x++) waitx(&k_empty[x][s], (c / SLOTS - 1) & 1);
+        if (__any_sync(FULL, abort_s)) break;
+#pragma unroll
+        for (int h = 0; h < 2; h++) put<D, false>(mine[h], smem + S::OFF_K + s * S::KV_B, lane + 32 * h, quarter, a.bias);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&k_full[s]));
+        if (c >= SLOTS)
+          for (uint32_t x = 0; x < NQ; x++) waitx(&v_empty[x][s], (c / SLOTS - 1) & 1);
+        if (__any_sync(FULL, abort_s)) break;
+#pragma unroll
+        for (int h = 0; h < 2; h++) put<D, true>(mine[h], smem + S::OFF_V + s * S::KV_B, lane + 32 * h, quarter, a.bias);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&v_full[s]));
+      }
+    } else {
+      // ---------------- softmax X ----------------
+      const uint32_t x = (warp - S::FIRST_SOFTMAX) >> 2, quad = warp & 3, r = quad * 32 + lane;
+      const uint32_t lane_addr = (quad * 32) << 16, s_addr = tmem + lane_addr + x * 128, o_addr = tmem + lane_addr + S::TM_O + x * 128;
+      const uint32_t tile_row = row0 + x * BM, row = tile_row + r;
+      const float scale = row_scale[x * BM + r];
+      // this row sees the keys [lo, hi); the tile's first row sees none from hi0 on, its last row none before lo1
+      const int window = static_cast<int>(min(a.window, 0x40000000u)), past = q.kv_len - q.q_len;
+      const int hi = row < q.rows ? past + static_cast<int>(row / a.group) + 1 : 0, lo = a.window ? hi - window : 0;
+      const int hi0 = past + static_cast<int>(tile_row / a.group) + 1;
+      const int lo1 = a.window ? past + static_cast<int>(min(tile_row + BM - 1, q.rows - 1) / a.group) + 1 - window : 0;
+      float m_run = NEG_BIG, l_run = 0.f;
+      for (uint32_t i = 0; i < n; i++) {
+        const uint32_t c = done + i, b = c & 1, s = c % SLOTS;
+        waitx(&s_ready[x][b], (c >> 1) & 1);
+        if (__any_sync(FULL, abort_s)) break;
+        tc_fence_after();
+        if (quad == 0 && lane == 0) mbar_arrive(smem_u32(&k_empty[x][s]));  // Q K^T of the tile is complete
+        uint32_t raw[64];
+        tmem_ld32(s_addr + 64 * b, raw);
+        tmem_ld32(s_addr + 64 * b + 32, raw + 32);
+        tmem_ld_wait();
+        const int key0 = key_first + static_cast<int>(i * BN);
+        if (key0 + static_cast<int>(BN) > hi0 || key0 < lo1) {
+#pragma unroll
+          for (int k = 0; k < 64; k++)
+            if (key0 + k >= hi || key0 + k < lo) raw[k] = 0xff800000u;
+        }
+        float mx[4] = {__uint_as_float(raw[0]), __uint_as_float(raw[1]), __uint_as_float(raw[2]), __uint_as_float(raw[3])};
+#pragma unroll
+        for (int k = 4; k < 64; k += 4)
+#pragma unroll
+          for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], __uint_as_float(raw[k + e]));
+        const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+        const bool grow = m_tile > m_run + GROW;
+        const float m_new = grow ? m_tile : m_run, corr = grow ? ex2(m_run - m_new) : 1.f;
+        m_run = m_new;
+        if (i > 0 && __any_sync(FULL, grow)) {
+          // O_X may be rescaled only between two P V: the previous tile's must be complete
+          waitx(&v_empty[x][(c - 1) % SLOTS], ((c - 1) / SLOTS) & 1);
+          __syncwarp();
+          tc_fence_after();
+#pragma unroll 1
+          for (uint32_t k = 0; k < D / 16; k++) {
+            uint32_t o[16];
+            tmem_ld16(o_addr + 16 * k, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+            tmem_st16(o_addr + 16 * k, o);
+          }
+        }
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t ph[32];
+        const float off = P_UP - m_new;
+#pragma unroll
+        for (int k = 0; k < 32; k++) {
+          float e0, e1;
+          fma2(e0, e1, __uint_as_float(raw[2 * k]), __uint_as_float(raw[2 * k + 1]), scale, off);
+          const float p0 = ex2(e0), p1 = ex2(e1);
+          add2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], p0, p1);
+          ph[k] = pack2<false>(p0, p1);
+        }
+        tmem_st32(s_addr + 64 * b, ph);  // (every S value of this row is in registers)
+        l_run = l_run * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&p_ready[x][b]));
+      }
+      waitx(&o_done[x], pieces & 1);
+      tc_fence_after();
+      if (!__any_sync(FULL, abort_s)) {
+        if (first == 0 && n == keys.tiles) {
+          // ---- the whole item: O / l through the dead Q tile, whole rows of it to memory ----
+          const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+          uint8_t* stage = smem + x * S::Q_B;
+#pragma unroll
+          for (uint32_t k = 0; k < D / 32; k++) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + 32 * k, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              float v[8];
+#pragma unroll
+              for (int j = 0; j < 8; j++) v[j] = __uint_as_float(o[8 * e + column_of(j)]) * inv;
+              *reinterpret_cast<uint4*>(stage + r * (D * 2) + (((4 * k + e) ^ (r & (D / 8 - 1))) << 4)) = a.bf ? pack8<true>(v) : pack8<false>(v);
+            }
+          }
+          __syncwarp();  // a warp reads back the 32 rows that its own lanes have written
+          constexpr uint32_t U = D / 8;
+#pragma unroll 4
+          for (uint32_t k = lane; k < 32 * U; k += 32) {
+            const uint32_t rr = quad * 32 + k / U, u = k % U, row_r = tile_row + rr;
+            if (row_r >= q.rows) continue;
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * (D * 2) + ((u ^ (rr & (U - 1))) << 4));
+            uint16_t* out = out_row(a, q.q0, head, row_r) + 8 * u;
+            if ((reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+              *reinterpret_cast<uint4*>(out) = v;
+            } else {
+              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int e = 0; e < 8; e++) out[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+            }
+          }
+        } else {
+          // ---- a part of an item: as it is, to be joined ----
+          const uint32_t first_cta = start / share;
+          float* to = scratch + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PARTIAL + (x * BM + r) * S::STRIDE;
+#pragma unroll 1
+          for (uint32_t k = 0; k < D / 16; k++) {
+            uint32_t o[16];
+            tmem_ld16(o_addr + 16 * k, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              float v[8];
+#pragma unroll
+              for (int j = 0; j < 8; j++) v[j] = __uint_as_float(o[8 * e + column_of(j)]);
+              if (row < q.rows) {  // (the loads are the whole warp's)
+                *reinterpret_cast<float4*>(to + 16 * k + 8 * e) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4*>(to + 16 * k + 8 * e + 4) = make_float4(v[4], v[5], v[6], v[7]);
+              }
+            }
+          }
+          if (row < q.rows) *reinterpret_cast<float2*>(to + D) = make_float2(m_run, l_run);
+        }
+      }
+    }
+    done += n;
+    pieces++;
+    pos += n;
+    tc_fence_before();
+    __syncthreads();  // the piece is finished by every role: Q, S and O can be reused
+    tc_fence_after();
+    if (abort_s) break;
+
+    // ---- an item of several CTAs is joined by the one that comes last ----
+    const bool whole = first == 0 && n == keys.tiles;
+    if (threadIdx.x == 0) {
+      if (!whole) {
+        const uint32_t first_cta = start / share, parts = (start + keys.tiles - 1) / share - first_cta + 1;
+        __threadfence();
+        const bool last = atomicAdd(&counters[first_cta], 1u) == parts - 1;
+        if (last) counters[first_cta] = 0;  // for the next launch
+        __threadfence();
+        join_s = Join{first_cta, parts, last};
+      }
+      if (pos < c1) {
+        Cursor c = cur;
+        c.at = 0;
+        c.start = pos;
+        if (++c.head == a.pool.n_kv_head) {
+          c.head = 0;
+          if (++c.x * S::ROWS >= c.q.rows) {
+            c.x = 0;
+            do c.q = request(a, ++c.r, false);  // (there is a further item in the line)
+            while (c.q.rows == 0);
+          }
+          c.keys = keys_of(a, c.q, c.x * S::ROWS, S::ROWS);
+        }
+        cur = c;
+      }
+    }
+    __syncthreads();
+    if (!whole && join_s.last) {
+      const Join j = join_s;
+      constexpr int V = D / 32;
+      const float* from = scratch + static_cast<size_t>(2 * j.first_cta) * S::PARTIAL;
+      const uint32_t rows = min(S::ROWS, q.rows - row0);
+      for (uint32_t r = warp; r < rows; r += S::NWARP) {
+        float m = NEG_BIG, l = 0.f, o[V] = {};
+#pragma unroll 4
+        for (uint32_t k = 0; k < j.n; k++) {
+          const float* p = from + static_cast<size_t>(2 * k + (k == 0)) * S::PARTIAL + r * S::STRIDE;
+          const float2 ml = *reinterpret_cast<const float2*>(p + D);
+          float v[V];
+#pragma unroll
+          for (int e = 0; e < V; e += 2) {
+            const float2 f = *reinterpret_cast<const float2*>(p + V * lane + e);
+            v[e] = f.x;
+            v[e + 1] = f.y;
+          }
+          const float top = fmaxf(m, ml.x), w0 = ex2(m - top), w1 = ex2(ml.x - top);
+          m = top;
+          l = l * w0 + ml.y * w1;
+#pragma unroll
+          for (int e = 0; e < V; e++) o[e] = o[e] * w0 + v[e] * w1;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint16_t* out = out_row(a, q.q0, head, row0 + r) + V * lane;
+        if constexpr (V == 4) {
+          store4(a.bf, out, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+        } else {
+          const uint32_t h = a.bf ? pack2<true>(o[0] * inv, o[1] * inv) : pack2<false>(o[0] * inv, o[1] * inv);
+          out[0] = static_cast<uint16_t>(h);
+          out[1] = static_cast<uint16_t>(h >> 16);
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  if (abort_s) {  // (all threads) the MMAs on their way are complete before TMEM and shared memory are given back
+    if (threadIdx.x == 0) {
+      mbar_init(smem_u32(&drained), 4);
+      fence_barrier_init();
+    }
+    __syncthreads();
+    if (warp < 4 && elect_one()) umma_commit(smem_u32(&drained));  // (the threads that issued them)
+    if (threadIdx.x == 0) (void)wait_phase(smem_u32(&drained), 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, S::TMEM_COLS);
+}
+
+template <typename F>
+cudaError_t with_kernel(uint32_t head_dim, bool two, F f) {
+  if (head_dim == 128) return two ? f(kv4_prefill_kernel<128, 2>, Shape<128, 2>()) : f(kv4_prefill_kernel<128, 1>, Shape<128, 1>());
+  return two ? f(kv4_prefill_kernel<64, 2>, Shape<64, 2>()) : f(kv4_prefill_kernel<64, 1>, Shape<64, 1>());
+}
+
+}  // namespace
+
+cudaError_t bp_kv4_prefill_init(bp_paged_ctx* c) {
+  size_t floats = 0;
+  cudaError_t e = cudaSuccess;
+  for (uint32_t i = 0; i < 4 && e == cudaSuccess; i++)
+    e = with_kernel(i & 1 ? 128 : 64, i & 2, [&](auto kernel, auto shape) {
+      const size_t need = 2 * static_cast<size_t>(c->sm_count) * shape.PARTIAL;  // two pieces per CTA
+      if (need > floats) floats = need;
+      return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shape.SMEM));
+    });
+  return e != cudaSuccess ? e : cudaMalloc(&c->prefill_partials, floats * sizeof(float));
+}
+
+cudaError_t bp_launch_kv4_prefill(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, const AttnArgs& a) {
+  return with_kernel(head_dim, a.max_q * a.group > BM, [&](auto kernel, auto shape) {
+    return bp_launch(true, kernel, dim3(c->sm_count), dim3(shape.THREADS), shape.SMEM, s, a, c->prefill_partials, c->counters);
+  });
+}

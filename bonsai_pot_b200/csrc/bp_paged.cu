@@ -4,7 +4,7 @@
 
 #include <new>
 
-#include "bp_paged.cuh"
+#include "bp_kv4_attention.cuh"
 
 namespace {
 
@@ -116,6 +116,7 @@ int bp_paged_create(int32_t device, bp_paged_ctx** out) {
   if (major != 10) return fail(c, BP_ERR_CUDA, "this library is built for sm_100a (B200) only");
   BP_TRY(c, cudaDeviceGetAttribute(&c->sm_count, cudaDevAttrMultiProcessorCount, device));
   BP_TRY(c, bp_kv4_attention_init(c));
+  BP_TRY(c, bp_kv4_prefill_init(c));
   BP_TRY(c, cudaHostAlloc(&c->err_host, 2 * sizeof(uint32_t), cudaHostAllocMapped));
   c->err_host[0] = c->err_host[1] = 0;
   void* dev = nullptr;
@@ -130,6 +131,7 @@ void bp_paged_destroy(bp_paged_ctx* c) {
     OnDevice on(c->device);
     if (on.err == cudaSuccess) {
       if (c->partials) (void)cudaFree(c->partials);  // waits for launches that still use it
+      if (c->prefill_partials) (void)cudaFree(c->prefill_partials);
       if (c->counters) (void)cudaFree(c->counters);
       if (c->err_host) (void)cudaFreeHost(c->err_host);
     }

@@ -14,11 +14,11 @@
 struct bp_paged_ctx {
   int device;
   int sm_count;
-  uint32_t attn_sms;   // of them, those that split attention uses
   int status;          // latched: BP_ERR_DEVICE_LOST or BP_ERR_TIMEOUT
   uint32_t* err_host;  // pinned, mapped: [0] a token or page out of range, [1] a bounded wait gave up
   uint32_t* err_dev;   // device alias
   float* partials;     // split attention: partial results of the CTAs
+  float* prefill_partials;  // the same of the kernel for many queries
   uint32_t* counters;  // split attention: partials that have arrived, zero between launches
   char msg[256];
 };
