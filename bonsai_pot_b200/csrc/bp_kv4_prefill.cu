@@ -24,6 +24,7 @@ using namespace bp::kv4;
 
 constexpr uint32_t BM = 128, BN = 64;  // query rows of a tile, keys of a tile
 constexpr uint32_t SLOTS = 4;          // K and V tiles in shared memory
+constexpr uint32_t ITEM_COST = 6;      // what beginning and ending an item costs, in key tiles
 constexpr float GROW = 5.f;            // log2 by which a maximum may grow before O is rescaled; P_UP + GROW stays below 16
 
 template <int D, uint32_t NQ>
@@ -34,7 +35,7 @@ struct Shape {
   static constexpr uint32_t TM_O = 128 * NQ, TMEM_COLS = 256 * NQ;        // S_X at 128 X, O_X at TM_O + 128 X
   static constexpr uint32_t FIRST_EXPANDER = 4, FIRST_SOFTMAX = 8;        // warps 0, 1: O issuers, 2, 3: S issuers
   static constexpr uint32_t NWARP = FIRST_SOFTMAX + 4 * NQ, THREADS = 32 * NWARP;
-  static constexpr uint32_t STRIDE = D + 4, PARTIAL = ROWS * STRIDE;      // floats of a row of a partial result (o, m, l), of one
+  static constexpr uint32_t PARTIAL = ROWS * (D + 2);                     // floats of a partial result: o as fours [dims / 4][row], (m, l) [row]
 };
 
 struct Request {
@@ -68,7 +69,8 @@ __device__ __forceinline__ Keys keys_of(const AttnArgs& a, const Request& q, uin
   return k;
 }
 
-// A place in the line: item (r, x, head) of `keys.tiles` tiles, tile `at` of it, the item's first tile being the line's `start`.
+// A place in the line, in which an item takes ITEM_COST places before those of its tiles: item (r, x, head) of `keys.tiles` tiles, tile
+// `at` of it, the item's first tile lying at place `start`.
 struct Cursor {
   Request q;
   Keys keys;
@@ -143,6 +145,25 @@ struct Join {
   uint32_t first_cta, n, last;
 };
 
+// `rows` staged output rows (16-byte chunks xor-ed with the row) from row0 of a request on to memory, by `n` threads.
+template <int D>
+__device__ __forceinline__ void store_rows(const AttnArgs& a, int q0, uint32_t head, uint32_t row0, uint32_t rows, const uint8_t* stage, uint32_t me, uint32_t n) {
+  constexpr uint32_t U = D / 8;
+#pragma unroll 4
+  for (uint32_t k = me; k < rows * U; k += n) {
+    const uint32_t r = k / U, u = k % U;
+    const uint4 v = *reinterpret_cast<const uint4*>(stage + r * (D * 2) + ((u ^ (r & (U - 1))) << 4));
+    uint16_t* out = out_row(a, q0, head, row0 + r) + 8 * u;
+    if ((reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+      *reinterpret_cast<uint4*>(out) = v;
+    } else {
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; e++) out[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+    }
+  }
+}
+
 template <int D, uint32_t NQ>
 __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(const __grid_constant__ AttnArgs a, float* __restrict__ scratch, uint32_t* __restrict__ counters) {
   using S = Shape<D, NQ>;
@@ -201,7 +222,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   const uint32_t per = (a.n_req + THREADS - 1) / THREADS;
   auto tiles_of = [&](const Request& q) {  // of all items of a request
     uint32_t n = 0;
-    for (uint32_t row0 = 0; row0 < q.rows; row0 += S::ROWS) n += keys_of(a, q, row0, S::ROWS).tiles;
+    for (uint32_t row0 = 0; row0 < q.rows; row0 += S::ROWS) n += keys_of(a, q, row0, S::ROWS).tiles + ITEM_COST;
     return n * a.pool.n_kv_head;
   };
   {
@@ -232,10 +253,10 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       const Request q = request(a, r, false);
       for (uint32_t x = 0; x * S::ROWS < q.rows; x++) {
         const Keys k = keys_of(a, q, x * S::ROWS, S::ROWS);
-        const uint32_t n = k.tiles * a.pool.n_kv_head;
+        const uint32_t places = k.tiles + ITEM_COST, n = places * a.pool.n_kv_head;
         if (left < n) {
-          const uint32_t head = left / k.tiles, tile = left - head * k.tiles;
-          cur = Cursor{q, k, r, x, head, tile, c0 - tile};
+          const uint32_t head = left / places, in = left - head * places;
+          cur = Cursor{q, k, r, x, head, in > ITEM_COST ? in - ITEM_COST : 0, c0 - in + ITEM_COST};
           found = true;
           break;
         }
@@ -248,6 +269,8 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   // Barrier phases count on across items: done = key tiles so far, pieces = pieces so far.
   uint32_t done = 0, pieces = 0;
   for (uint32_t pos = c0; pos < c1;) {
+    pos = max(pos, cur.start);
+    if (pos >= c1) break;  // (the stretch ends before the item's first tile)
     const Request q = cur.q;
     const Keys keys = cur.keys;
     const uint32_t head = cur.head, row0 = cur.x * S::ROWS, first = cur.at, n = min(keys.tiles - first, c1 - pos);
@@ -257,25 +280,28 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     {
       constexpr uint32_t U = D / 8, ITERS = (S::ROWS * U + THREADS - 1) / THREADS;
       static_assert(THREADS % U == 0 && (S::ROWS * U) % 32 == 0, "rows are groups of U lanes");
+      uint4 raw[ITERS];  // every load is on its way before the first is used
+#pragma unroll
+      for (uint32_t k = 0; k < ITERS; k++) {
+        const uint32_t i = threadIdx.x + k * THREADS, r = min(row0 + min(i / U, S::ROWS - 1), q.rows - 1), u = i % U;
+        const uint16_t* p = a.q.data + static_cast<int64_t>(q.q0 + r / a.group) * a.q.tok + static_cast<int64_t>(head * a.group + r % a.group) * a.q.head + 8 * u;
+        if (a.q_vec) {
+          raw[k] = *reinterpret_cast<const uint4*>(p);
+        } else {
+          uint32_t h[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) h[e] = p[e];
+          raw[k] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+        }
+      }
 #pragma unroll
       for (uint32_t k = 0; k < ITERS; k++) {
         const uint32_t i = threadIdx.x + k * THREADS, r = i / U, u = i % U;
         if (i >= S::ROWS * U) break;  // (whole warps)
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (row0 + r < q.rows) {
-          const uint16_t* p = a.q.data + static_cast<int64_t>(q.q0 + (row0 + r) / a.group) * a.q.tok + static_cast<int64_t>(head * a.group + (row0 + r) % a.group) * a.q.head + 8 * u;
-          if (a.q_vec) {
-            raw = *reinterpret_cast<const uint4*>(p);
-          } else {
-            uint32_t h[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) h[e] = p[e];
-            raw = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-          }
-        }
+        if (row0 + r >= q.rows) raw[k] = make_uint4(0, 0, 0, 0);
         float x[8], big = 0.f;
-        if (a.bf) unpack8<true>(raw, x);
-        else unpack8<false>(raw, x);
+        if (a.bf) unpack8<true>(raw[k], x);
+        else unpack8<false>(raw[k], x);
 #pragma unroll
         for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[e]));
 #pragma unroll
@@ -471,42 +497,26 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
             }
           }
           __syncwarp();  // a warp reads back the 32 rows that its own lanes have written
-          constexpr uint32_t U = D / 8;
-#pragma unroll 4
-          for (uint32_t k = lane; k < 32 * U; k += 32) {
-            const uint32_t rr = quad * 32 + k / U, u = k % U, row_r = tile_row + rr;
-            if (row_r >= q.rows) continue;
-            const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * (D * 2) + ((u ^ (rr & (U - 1))) << 4));
-            uint16_t* out = out_row(a, q.q0, head, row_r) + 8 * u;
-            if ((reinterpret_cast<uintptr_t>(out) & 15) == 0) {
-              *reinterpret_cast<uint4*>(out) = v;
-            } else {
-              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-              for (int e = 0; e < 8; e++) out[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
-            }
-          }
+          if (tile_row + quad * 32 < q.rows)
+            store_rows<D>(a, q.q0, head, tile_row + quad * 32, min(32u, q.rows - tile_row - quad * 32), stage + quad * 32 * (D * 2), lane, 32);
         } else {
           // ---- a part of an item: as it is, to be joined ----
           const uint32_t first_cta = start / share;
-          float* to = scratch + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PARTIAL + (x * BM + r) * S::STRIDE;
-#pragma unroll 1
+          float4* to = reinterpret_cast<float4*>(scratch + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PARTIAL) + x * BM + r;
+#pragma unroll 2
           for (uint32_t k = 0; k < D / 16; k++) {
             uint32_t o[16];
             tmem_ld16(o_addr + 16 * k, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-              float v[8];
+            for (int e = 0; e < 4; e++) {
+              float v[4];
 #pragma unroll
-              for (int j = 0; j < 8; j++) v[j] = __uint_as_float(o[8 * e + column_of(j)]);
-              if (row < q.rows) {  // (the loads are the whole warp's)
-                *reinterpret_cast<float4*>(to + 16 * k + 8 * e) = make_float4(v[0], v[1], v[2], v[3]);
-                *reinterpret_cast<float4*>(to + 16 * k + 8 * e + 4) = make_float4(v[4], v[5], v[6], v[7]);
-              }
+              for (int j = 0; j < 4; j++) v[j] = __uint_as_float(o[8 * (e >> 1) + column_of(4 * (e & 1) + j)]);
+              to[(4 * k + e) * S::ROWS] = make_float4(v[0], v[1], v[2], v[3]);  // (a warp's 32 rows are 512 bytes)
             }
           }
-          if (row < q.rows) *reinterpret_cast<float2*>(to + D) = make_float2(m_run, l_run);
+          reinterpret_cast<float2*>(to - (x * BM + r) + (D / 4) * S::ROWS)[x * BM + r] = make_float2(m_run, l_run);
         }
       }
     }
@@ -532,7 +542,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       if (pos < c1) {
         Cursor c = cur;
         c.at = 0;
-        c.start = pos;
+        c.start = pos + ITEM_COST;
         if (++c.head == a.pool.n_kv_head) {
           c.head = 0;
           if (++c.x * S::ROWS >= c.q.rows) {
@@ -548,38 +558,41 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     __syncthreads();
     if (!whole && join_s.last) {
       const Join j = join_s;
-      constexpr int V = D / 32;
       const float* from = scratch + static_cast<size_t>(2 * j.first_cta) * S::PARTIAL;
       const uint32_t rows = min(S::ROWS, q.rows - row0);
-      for (uint32_t r = warp; r < rows; r += S::NWARP) {
-        float m = NEG_BIG, l = 0.f, o[V] = {};
+      auto piece = [&](uint32_t k) { return from + static_cast<size_t>(2 * k + (k == 0)) * S::PARTIAL; };
+      auto ml = [&](uint32_t k, uint32_t r) { return reinterpret_cast<const float2*>(piece(k) + D * S::ROWS)[r]; };
+      // the rows' maxima and 1 / sums, in the dead K tiles; then a thread per four dims of a row, the rows of a warp side by side
+      float2* joined = reinterpret_cast<float2*>(smem + S::OFF_K);
+      for (uint32_t r = threadIdx.x; r < S::ROWS; r += THREADS) {
+        float m = NEG_BIG, l = 0.f;
 #pragma unroll 4
         for (uint32_t k = 0; k < j.n; k++) {
-          const float* p = from + static_cast<size_t>(2 * k + (k == 0)) * S::PARTIAL + r * S::STRIDE;
-          const float2 ml = *reinterpret_cast<const float2*>(p + D);
-          float v[V];
-#pragma unroll
-          for (int e = 0; e < V; e += 2) {
-            const float2 f = *reinterpret_cast<const float2*>(p + V * lane + e);
-            v[e] = f.x;
-            v[e + 1] = f.y;
-          }
-          const float top = fmaxf(m, ml.x), w0 = ex2(m - top), w1 = ex2(ml.x - top);
+          const float2 e = ml(k, r);
+          const float top = fmaxf(m, e.x);
+          l = l * ex2(m - top) + e.y * ex2(e.x - top);
           m = top;
-          l = l * w0 + ml.y * w1;
-#pragma unroll
-          for (int e = 0; e < V; e++) o[e] = o[e] * w0 + v[e] * w1;
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        uint16_t* out = out_row(a, q.q0, head, row0 + r) + V * lane;
-        if constexpr (V == 4) {
-          store4(a.bf, out, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-        } else {
-          const uint32_t h = a.bf ? pack2<true>(o[0] * inv, o[1] * inv) : pack2<false>(o[0] * inv, o[1] * inv);
-          out[0] = static_cast<uint16_t>(h);
-          out[1] = static_cast<uint16_t>(h >> 16);
-        }
+        joined[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
       }
+      __syncthreads();
+#pragma unroll 4
+      for (uint32_t i = threadIdx.x; i < S::ROWS * (D / 4); i += THREADS) {
+        const uint32_t r = i % S::ROWS, c = i / S::ROWS;
+        const float2 all = joined[r];
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+        for (uint32_t k = 0; k < j.n; k++) {
+          const float4 v = reinterpret_cast<const float4*>(piece(k))[c * S::ROWS + r];
+          const float w = ex2(ml(k, r).x - all.x) * all.y;
+          o = make_float4(fmaf(v.x, w, o.x), fmaf(v.y, w, o.y), fmaf(v.z, w, o.z), fmaf(v.w, w, o.w));
+        }
+        // staged in the dead Q tiles: whole rows go to memory
+        const uint32_t lo = a.bf ? pack2<true>(o.x, o.y) : pack2<false>(o.x, o.y), hi = a.bf ? pack2<true>(o.z, o.w) : pack2<false>(o.z, o.w);
+        *reinterpret_cast<uint2*>(smem + r * (D * 2) + (((c >> 1) ^ (r & (D / 8 - 1))) << 4) + 8 * (c & 1)) = make_uint2(lo, hi);
+      }
+      __syncthreads();
+      store_rows<D>(a, q.q0, head, row0, rows, smem, threadIdx.x, THREADS);
     }
     __syncthreads();
   }
