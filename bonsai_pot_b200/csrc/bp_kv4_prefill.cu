@@ -3,12 +3,13 @@
 //
 // An item is one KV head of one request and NQ query tiles of 128 rows (a row is a query head of a token). Keys come in tiles of
 // 64. Roles of a CTA, one CTA per SM:
-//   expanders (4 warps)     codes -> f16 operand tiles in shared memory, K and V, once for all query tiles of the item. Every
+//   expanders (8 warps)     codes -> f16 operand tiles in shared memory, K and V, once for all query tiles of the item. Every
 //                           value is an f16 number (the format's choice of m and d): nothing rounds. The next tile's codes are
 //                           on their way in registers meanwhile. Places that hold no key of the request become zeros.
 //   S issuer X (1 thread)   S_X = Q_X K^T (tcgen05.mma kind::f16, M 128, N 64) into one of two 64-column buffers in TMEM
-//   softmax X (4 warps)     thread = row = TMEM lane: masks, running maximum and sum, P as f16 over the tile's S buffer; O_X is
-//                           rescaled in TMEM only when a row's maximum grew by more than 2^5 (P stays below 2^15 meanwhile)
+//   softmax X (8 warps)     two threads per row = TMEM lane, 32 keys each: masks, running maximum (they agree on it through shared memory) and
+//                           sum, P as f16 over the tile's S buffer; O_X is rescaled in TMEM only when a row's maximum grew by more
+//                           than 2^5 (P stays below 2^15 meanwhile). One thread per row (64 keys) took 1.55 us per tile
 //   O issuer X (1 thread)   O_X += P_X V (P from TMEM as the A operand, V as the MN-major B operand)
 // The key tiles of all items lie in one line, of which every CTA takes an equal stretch; an item that lies in several CTAs is joined by the
 // one that comes last, in the order of its keys (as in bp_kv4_attention.cu). Every wait is bounded; a timeout sets the context's error word and
@@ -33,8 +34,8 @@ struct Shape {
   static constexpr uint32_t Q_B = BM * D * 2, KV_B = BN * D * 2;          // operand tiles: D / 64 chunks of rows of 128 bytes
   static constexpr uint32_t OFF_K = NQ * Q_B, OFF_V = OFF_K + SLOTS * KV_B, SMEM = OFF_V + SLOTS * KV_B + 1024;
   static constexpr uint32_t TM_O = 128 * NQ, TMEM_COLS = 256 * NQ;        // S_X at 128 X, O_X at TM_O + 128 X
-  static constexpr uint32_t FIRST_EXPANDER = 4, FIRST_SOFTMAX = 8;        // warps 0, 1: O issuers, 2, 3: S issuers
-  static constexpr uint32_t NWARP = FIRST_SOFTMAX + 4 * NQ, THREADS = 32 * NWARP;
+  static constexpr uint32_t FIRST_EXPANDER = 4, FIRST_SOFTMAX = 12;       // warps 0, 1: O issuers, 2, 3: S issuers
+  static constexpr uint32_t NWARP = FIRST_SOFTMAX + 8 * NQ, THREADS = 32 * NWARP;
   static constexpr uint32_t PARTIAL = ROWS * (D + 2);                     // floats of a partial result: o as fours [dims / 4][row], (m, l) [row]
 };
 
@@ -137,6 +138,11 @@ __device__ __forceinline__ void put(const Raw<D>& w, uint8_t* tile, uint32_t row
     *reinterpret_cast<uint4*>(tile + oper_off(BN, row, 4 * b + quarter)) = expand8(codes, d, m, bias);
   }
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // Column of O that holds dim i of a group of eight.
 __host__ __device__ constexpr int column_of(int i) { return i < 4 ? 2 * i : 2 * (i - 4) + 1; }
 
@@ -171,6 +177,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t k_full[SLOTS], v_full[SLOTS], k_empty[NQ][SLOTS], v_empty[NQ][SLOTS];
   __shared__ __align__(8) uint64_t s_ready[NQ][2], p_ready[NQ][2], p_free[NQ][2], o_done[NQ], drained;
+  __shared__ float shared_max[NQ][2][2][BM];  // [query tile][tile & 1][half][row]
   __shared__ float row_scale[S::ROWS];  // of a row's queries: the power of two that they were divided by
   __shared__ uint32_t line[THREADS + 1];
   __shared__ Cursor cur;
@@ -183,8 +190,8 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < SLOTS; i++) {
-      mbar_init(smem_u32(&k_full[i]), 4);
-      mbar_init(smem_u32(&v_full[i]), 4);
+      mbar_init(smem_u32(&k_full[i]), 8);
+      mbar_init(smem_u32(&v_full[i]), 8);
       for (uint32_t x = 0; x < NQ; x++) {
         mbar_init(smem_u32(&k_empty[x][i]), 1);
         mbar_init(smem_u32(&v_empty[x][i]), 1);
@@ -193,7 +200,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     for (uint32_t x = 0; x < NQ; x++) {
       for (uint32_t b = 0; b < 2; b++) {
         mbar_init(smem_u32(&s_ready[x][b]), 1);
-        mbar_init(smem_u32(&p_ready[x][b]), 4);
+        mbar_init(smem_u32(&p_ready[x][b]), 8);
         mbar_init(smem_u32(&p_free[x][b]), 1);
       }
       mbar_init(smem_u32(&o_done[x]), 1);
@@ -363,7 +370,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       }
     } else if (warp < S::FIRST_SOFTMAX) {
       // ---------------- codes -> operand tiles ----------------
-      const uint32_t quarter = warp - S::FIRST_EXPANDER;
+      const uint32_t quarter = warp & 3, row = lane + 32 * ((warp - S::FIRST_EXPANDER) >> 2);
       const int32_t* table = a.page_table + static_cast<size_t>(cur.r) * a.table_stride;
       auto id_of = [&](int key) {
         if (key < keys.low || key >= keys.high) return 0xffffffffu;  // keys behind `high` are nobody's here: their columns are masked
@@ -371,45 +378,36 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         if (id >= a.pool.n_pages) note_range(a.err);
         return id;
       };
-      Raw<D> raw[2];
-      uint32_t ids[2];
-#pragma unroll
-      for (int h = 0; h < 2; h++) ask<D>(raw[h], a, id_of(key_first + static_cast<int>(lane + 32 * h)), key_first + static_cast<int>(lane + 32 * h), head, quarter);
-#pragma unroll
-      for (int h = 0; h < 2; h++) ids[h] = n > 1 ? id_of(key_first + static_cast<int>(BN + lane + 32 * h)) : 0xffffffffu;
+      Raw<D> raw;
+      int key = key_first + static_cast<int>(row);
+      ask<D>(raw, a, id_of(key), key, head, quarter);
+      uint32_t id = n > 1 ? id_of(key + static_cast<int>(BN)) : 0xffffffffu;
       for (uint32_t i = 0; i < n; i++) {
         const uint32_t c = done + i, s = c % SLOTS;
-        Raw<D> mine[2] = {raw[0], raw[1]};
-        const int key = key_first + static_cast<int>((i + 1) * BN + lane);
-        if (i + 1 < n) {
-#pragma unroll
-          for (int h = 0; h < 2; h++) ask<D>(raw[h], a, ids[h], key + 32 * h, head, quarter);
-        }
-        if (i + 2 < n) {
-#pragma unroll
-          for (int h = 0; h < 2; h++) ids[h] = id_of(key + static_cast<int>(BN) + 32 * h);
-        }
+        const Raw<D> mine = raw;
+        key += BN;
+        if (i + 1 < n) ask<D>(raw, a, id, key, head, quarter);
+        if (i + 2 < n) id = id_of(key + static_cast<int>(BN));
         if (c >= SLOTS)
           for (uint32_t x = 0; x < NQ; x++) waitx(&k_empty[x][s], (c / SLOTS - 1) & 1);
         if (__any_sync(FULL, abort_s)) break;
-#pragma unroll
-        for (int h = 0; h < 2; h++) put<D, false>(mine[h], smem + S::OFF_K + s * S::KV_B, lane + 32 * h, quarter, a.bias);
+        put<D, false>(mine, smem + S::OFF_K + s * S::KV_B, row, quarter, a.bias);
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&k_full[s]));
         if (c >= SLOTS)
           for (uint32_t x = 0; x < NQ; x++) waitx(&v_empty[x][s], (c / SLOTS - 1) & 1);
         if (__any_sync(FULL, abort_s)) break;
-#pragma unroll
-        for (int h = 0; h < 2; h++) put<D, true>(mine[h], smem + S::OFF_V + s * S::KV_B, lane + 32 * h, quarter, a.bias);
+        put<D, true>(mine, smem + S::OFF_V + s * S::KV_B, row, quarter, a.bias);
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&v_full[s]));
       }
     } else {
       // ---------------- softmax X ----------------
-      const uint32_t x = (warp - S::FIRST_SOFTMAX) >> 2, quad = warp & 3, r = quad * 32 + lane;
-      const uint32_t lane_addr = (quad * 32) << 16, s_addr = tmem + lane_addr + x * 128, o_addr = tmem + lane_addr + S::TM_O + x * 128;
+      // (after a wait that gave up the warps go on to the end without waiting: they meet at named barriers)
+      const uint32_t x = (warp - S::FIRST_SOFTMAX) >> 3, half = warp >> 2 & 1, quad = warp & 3, r = quad * 32 + lane;
+      const uint32_t lane_addr = (quad * 32) << 16, s_addr = tmem + lane_addr + x * 128, o_addr = tmem + lane_addr + S::TM_O + x * 128 + half * (D / 2);
       const uint32_t tile_row = row0 + x * BM, row = tile_row + r;
       const float scale = row_scale[x * BM + r];
       // this row sees the keys [lo, hi); the tile's first row sees none from hi0 on, its last row none before lo1
@@ -421,25 +419,32 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       for (uint32_t i = 0; i < n; i++) {
         const uint32_t c = done + i, b = c & 1, s = c % SLOTS;
         waitx(&s_ready[x][b], (c >> 1) & 1);
-        if (__any_sync(FULL, abort_s)) break;
+        __syncwarp();
         tc_fence_after();
-        if (quad == 0 && lane == 0) mbar_arrive(smem_u32(&k_empty[x][s]));  // Q K^T of the tile is complete
-        uint32_t raw[64];
-        tmem_ld32(s_addr + 64 * b, raw);
-        tmem_ld32(s_addr + 64 * b + 32, raw + 32);
+        if (half == 0 && quad == 0 && lane == 0) mbar_arrive(smem_u32(&k_empty[x][s]));  // Q K^T of the tile is complete
+        uint32_t raw[32];
+        tmem_ld32(s_addr + 64 * b + 32 * half, raw);
         tmem_ld_wait();
         const int key0 = key_first + static_cast<int>(i * BN);
         if (key0 + static_cast<int>(BN) > hi0 || key0 < lo1) {
+          const int from = lo - key0 - static_cast<int>(32 * half), to = hi - key0 - static_cast<int>(32 * half);
 #pragma unroll
-          for (int k = 0; k < 64; k++)
-            if (key0 + k >= hi || key0 + k < lo) raw[k] = 0xff800000u;
+          for (int k = 0; k < 32; k++)
+            if (k >= to || k < from) raw[k] = 0xff800000u;
         }
         float mx[4] = {__uint_as_float(raw[0]), __uint_as_float(raw[1]), __uint_as_float(raw[2]), __uint_as_float(raw[3])};
 #pragma unroll
-        for (int k = 4; k < 64; k += 4)
+        for (int k = 4; k < 28; k += 8)
 #pragma unroll
-          for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], __uint_as_float(raw[k + e]));
-        const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+          for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], __uint_as_float(raw[k + e]), __uint_as_float(raw[k + 4 + e]));
+#pragma unroll
+        for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], __uint_as_float(raw[28 + e]));
+        const float m_half = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        shared_max[x][i & 1][half][r] = m_half;
+        tc_fence_before();
+        named_bar_sync(1 + x, 256);  // (both halves have read their S, too: P goes over it)
+        tc_fence_after();
+        const float m_tile = fmaxf(m_half, shared_max[x][i & 1][half ^ 1][r]) * scale;
         const bool grow = m_tile > m_run + GROW;
         const float m_new = grow ? m_tile : m_run, corr = grow ? ex2(m_run - m_new) : 1.f;
         m_run = m_new;
@@ -449,7 +454,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
           __syncwarp();
           tc_fence_after();
 #pragma unroll 1
-          for (uint32_t k = 0; k < D / 16; k++) {
+          for (uint32_t k = 0; k < D / 32; k++) {
             uint32_t o[16];
             tmem_ld16(o_addr + 16 * k, o);
             tmem_ld_wait();
@@ -459,65 +464,68 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
           }
         }
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t ph[32];
+        uint32_t ph[16];
         const float off = P_UP - m_new;
 #pragma unroll
-        for (int k = 0; k < 32; k++) {
+        for (int k = 0; k < 16; k++) {
           float e0, e1;
           fma2(e0, e1, __uint_as_float(raw[2 * k]), __uint_as_float(raw[2 * k + 1]), scale, off);
           const float p0 = ex2(e0), p1 = ex2(e1);
           add2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], p0, p1);
           ph[k] = pack2<false>(p0, p1);
         }
-        tmem_st32(s_addr + 64 * b, ph);  // (every S value of this row is in registers)
+        tmem_st16(s_addr + 64 * b + 16 * half, ph);
         l_run = l_run * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&p_ready[x][b]));
       }
+      // the row's sum over both halves
+      shared_max[x][n & 1][half][r] = l_run;
       waitx(&o_done[x], pieces & 1);
+      named_bar_sync(1 + x, 256);
+      l_run += shared_max[x][n & 1][half ^ 1][r];
       tc_fence_after();
-      if (!__any_sync(FULL, abort_s)) {
-        if (first == 0 && n == keys.tiles) {
-          // ---- the whole item: O / l through the dead Q tile, whole rows of it to memory ----
-          const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-          uint8_t* stage = smem + x * S::Q_B;
+      if (first == 0 && n == keys.tiles) {
+        // ---- the whole item: O / l through the dead Q tile, whole rows of it to memory ----
+        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+        uint8_t* stage = smem + x * S::Q_B;
+#pragma unroll 1
+        for (uint32_t k = 0; k < D / 32; k++) {
+          uint32_t o[16];
+          tmem_ld16(o_addr + 16 * k, o);
+          tmem_ld_wait();
 #pragma unroll
-          for (uint32_t k = 0; k < D / 32; k++) {
-            uint32_t o[32];
-            tmem_ld32(o_addr + 32 * k, o);
-            tmem_ld_wait();
+          for (int e = 0; e < 2; e++) {
+            float v[8];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-              float v[8];
-#pragma unroll
-              for (int j = 0; j < 8; j++) v[j] = __uint_as_float(o[8 * e + column_of(j)]) * inv;
-              *reinterpret_cast<uint4*>(stage + r * (D * 2) + (((4 * k + e) ^ (r & (D / 8 - 1))) << 4)) = a.bf ? pack8<true>(v) : pack8<false>(v);
-            }
+            for (int j = 0; j < 8; j++) v[j] = __uint_as_float(o[8 * e + column_of(j)]) * inv;
+            const uint32_t u = half * (D / 16) + 2 * k + e;
+            *reinterpret_cast<uint4*>(stage + r * (D * 2) + ((u ^ (r & (D / 8 - 1))) << 4)) = a.bf ? pack8<true>(v) : pack8<false>(v);
           }
-          __syncwarp();  // a warp reads back the 32 rows that its own lanes have written
-          if (tile_row + quad * 32 < q.rows)
-            store_rows<D>(a, q.q0, head, tile_row + quad * 32, min(32u, q.rows - tile_row - quad * 32), stage + quad * 32 * (D * 2), lane, 32);
-        } else {
-          // ---- a part of an item: as it is, to be joined ----
-          const uint32_t first_cta = start / share;
-          float4* to = reinterpret_cast<float4*>(scratch + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PARTIAL) + x * BM + r;
-#pragma unroll 2
-          for (uint32_t k = 0; k < D / 16; k++) {
-            uint32_t o[16];
-            tmem_ld16(o_addr + 16 * k, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              float v[4];
-#pragma unroll
-              for (int j = 0; j < 4; j++) v[j] = __uint_as_float(o[8 * (e >> 1) + column_of(4 * (e & 1) + j)]);
-              to[(4 * k + e) * S::ROWS] = make_float4(v[0], v[1], v[2], v[3]);  // (a warp's 32 rows are 512 bytes)
-            }
-          }
-          reinterpret_cast<float2*>(to - (x * BM + r) + (D / 4) * S::ROWS)[x * BM + r] = make_float2(m_run, l_run);
         }
+        named_bar_sync(1 + x, 256);
+        if (tile_row < q.rows && !abort_s) store_rows<D>(a, q.q0, head, tile_row, min(BM, q.rows - tile_row), stage, (half * 4 + quad) * 32 + lane, 256);
+      } else {
+        // ---- a part of an item: as it is, to be joined ----
+        const uint32_t first_cta = start / share;
+        float* mine = scratch + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PARTIAL;
+        float4* to = reinterpret_cast<float4*>(mine) + half * (D / 8) * S::ROWS + x * BM + r;
+#pragma unroll 1
+        for (uint32_t k = 0; k < D / 32; k++) {
+          uint32_t o[16];
+          tmem_ld16(o_addr + 16 * k, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = __uint_as_float(o[8 * (e >> 1) + column_of(4 * (e & 1) + j)]);
+            to[(4 * k + e) * S::ROWS] = make_float4(v[0], v[1], v[2], v[3]);  // (a warp's 32 rows are 512 bytes)
+          }
+        }
+        if (half == 0) reinterpret_cast<float2*>(mine + D * S::ROWS)[x * BM + r] = make_float2(m_run, l_run);
       }
     }
     done += n;
