@@ -35,7 +35,8 @@ struct Shape {
   static constexpr uint32_t OFF_K = NQ * Q_B, OFF_V = OFF_K + SLOTS * KV_B, SMEM = OFF_V + SLOTS * KV_B + 1024;
   static constexpr uint32_t TM_O = 128 * NQ, TMEM_COLS = 256 * NQ;        // S_X at 128 X, O_X at TM_O + 128 X
   static constexpr uint32_t FIRST_EXPANDER = 4, FIRST_SOFTMAX = 12;       // warps 0, 1: O issuers, 2, 3: S issuers
-  static constexpr uint32_t NWARP = FIRST_SOFTMAX + 8 * NQ, THREADS = 32 * NWARP;
+  static constexpr uint32_t H = 1, C = BN / H;                            // softmax threads per row, keys of each
+  static constexpr uint32_t NWARP = FIRST_SOFTMAX + 4 * H * NQ, THREADS = 32 * NWARP;
   static constexpr uint32_t PARTIAL = ROWS * (D + 2);                     // floats of a partial result: o as fours [dims / 4][row], (m, l) [row]
 };
 
@@ -81,7 +82,8 @@ struct Cursor {
 // Byte offset of 16-byte unit u of row r in an operand tile of `rows` rows: chunks of 64 dims, 128-byte swizzle.
 __device__ __forceinline__ uint32_t oper_off(uint32_t rows, uint32_t r, uint32_t u) { return (u >> 3) * (rows * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4); }
 
-// A quarter of the codes of one token's K and V (an expander warp has the same quarter of every token), and their scales.
+// A quarter of the codes of one token's K and V (an expander warp has the same quarter of every token), and their scales; `id` is a page of the
+// pool.
 template <int D>
 struct Raw {
   static constexpr int NB = D / 32;
@@ -91,13 +93,6 @@ template <int D>
 __device__ __forceinline__ void ask(Raw<D>& w, const AttnArgs& a, uint32_t id, int key, uint32_t head, uint32_t quarter) {
   using L = PoolLayout<D>;
   constexpr int NB = D / 32;
-  if (id >= a.pool.n_pages) {  // no key of the request, or a page id outside the pool
-#pragma unroll
-    for (int i = 0; i < NB; i++) w.k[i] = w.v[i] = 0;
-#pragma unroll
-    for (int i = 0; i < NB / 2; i++) w.kd[i] = w.km[i] = w.vd[i] = w.vm[i] = 0;
-    return;
-  }
   const uint32_t page = a.pool.page, tok = static_cast<uint32_t>(key) & (page - 1);
   const uint8_t* k = a.pool.data + (static_cast<uint64_t>(id) * a.pool.n_kv_head + head) * (page * L::TOK);
   const uint8_t* v = k + L::v(page);
@@ -177,7 +172,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t k_full[SLOTS], v_full[SLOTS], k_empty[NQ][SLOTS], v_empty[NQ][SLOTS];
   __shared__ __align__(8) uint64_t s_ready[NQ][2], p_ready[NQ][2], p_free[NQ][2], o_done[NQ], drained;
-  __shared__ float shared_max[NQ][2][2][BM];  // [query tile][tile & 1][half][row]
+  __shared__ float shared_max[NQ][2][S::H][BM];  // [query tile][tile & 1][half][row]
   __shared__ float row_scale[S::ROWS];  // of a row's queries: the power of two that they were divided by
   __shared__ uint32_t line[THREADS + 1];
   __shared__ Cursor cur;
@@ -200,7 +195,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     for (uint32_t x = 0; x < NQ; x++) {
       for (uint32_t b = 0; b < 2; b++) {
         mbar_init(smem_u32(&s_ready[x][b]), 1);
-        mbar_init(smem_u32(&p_ready[x][b]), 8);
+        mbar_init(smem_u32(&p_ready[x][b]), 4 * S::H);
         mbar_init(smem_u32(&p_free[x][b]), 1);
       }
       mbar_init(smem_u32(&o_done[x]), 1);
@@ -372,22 +367,31 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       // ---------------- codes -> operand tiles ----------------
       const uint32_t quarter = warp & 3, row = lane + 32 * ((warp - S::FIRST_EXPANDER) >> 2);
       const int32_t* table = a.page_table + static_cast<size_t>(cur.r) * a.table_stride;
-      auto id_of = [&](int key) {
-        if (key < keys.low || key >= keys.high) return 0xffffffffu;  // keys behind `high` are nobody's here: their columns are masked
-        const uint32_t id = static_cast<uint32_t>(table[key >> a.pool.log_page]);
-        if (id >= a.pool.n_pages) note_range(a.err);
-        return id;
-      };
+      // Page ids are asked for two tiles ahead and looked at one tile ahead, when the codes are asked for: nothing here waits for memory.
+      // A token that holds no key of the request (or lies in a page outside the pool) gets page 0's codes, and zeros for its scales.
+      auto has_key = [&](int key) { return key >= keys.low && key < keys.high; };
+      auto ask_id = [&](int key) { return has_key(key) ? static_cast<uint32_t>(table[key >> a.pool.log_page]) : 0u; };
       Raw<D> raw;
       int key = key_first + static_cast<int>(row);
-      ask<D>(raw, a, id_of(key), key, head, quarter);
-      uint32_t id = n > 1 ? id_of(key + static_cast<int>(BN)) : 0xffffffffu;
+      uint32_t id = ask_id(key), id_next = n > 1 ? ask_id(key + static_cast<int>(BN)) : 0u;
+      bool there;
+      auto ask_codes = [&]() {  // of the tile that `key` lies in
+        there = has_key(key) && id < a.pool.n_pages;
+        if (has_key(key) && !there) note_range(a.err);
+        ask<D>(raw, a, there ? id : 0u, key, head, quarter);
+      };
+      ask_codes();
       for (uint32_t i = 0; i < n; i++) {
         const uint32_t c = done + i, s = c % SLOTS;
-        const Raw<D> mine = raw;
+        Raw<D> mine = raw;
+        if (!there) {
+#pragma unroll
+          for (int e = 0; e < D / 64; e++) mine.kd[e] = mine.km[e] = mine.vd[e] = mine.vm[e] = 0;
+        }
         key += BN;
-        if (i + 1 < n) ask<D>(raw, a, id, key, head, quarter);
-        if (i + 2 < n) id = id_of(key + static_cast<int>(BN));
+        id = id_next;
+        if (i + 1 < n) ask_codes();
+        if (i + 2 < n) id_next = ask_id(key + static_cast<int>(BN));
         if (c >= SLOTS)
           for (uint32_t x = 0; x < NQ; x++) waitx(&k_empty[x][s], (c / SLOTS - 1) & 1);
         if (__any_sync(FULL, abort_s)) break;
@@ -406,8 +410,9 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     } else {
       // ---------------- softmax X ----------------
       // (after a wait that gave up the warps go on to the end without waiting: they meet at named barriers)
-      const uint32_t x = (warp - S::FIRST_SOFTMAX) >> 3, half = warp >> 2 & 1, quad = warp & 3, r = quad * 32 + lane;
-      const uint32_t lane_addr = (quad * 32) << 16, s_addr = tmem + lane_addr + x * 128, o_addr = tmem + lane_addr + S::TM_O + x * 128 + half * (D / 2);
+      constexpr uint32_t H = S::H, C = S::C;
+      const uint32_t x = (warp - S::FIRST_SOFTMAX) / (4 * H), half = warp / 4 % H, quad = warp & 3, r = quad * 32 + lane;
+      const uint32_t lane_addr = (quad * 32) << 16, s_addr = tmem + lane_addr + x * 128, o_addr = tmem + lane_addr + S::TM_O + x * 128 + half * (D / H);
       const uint32_t tile_row = row0 + x * BM, row = tile_row + r;
       const float scale = row_scale[x * BM + r];
       // this row sees the keys [lo, hi); the tile's first row sees none from hi0 on, its last row none before lo1
@@ -422,29 +427,33 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         __syncwarp();
         tc_fence_after();
         if (half == 0 && quad == 0 && lane == 0) mbar_arrive(smem_u32(&k_empty[x][s]));  // Q K^T of the tile is complete
-        uint32_t raw[32];
-        tmem_ld32(s_addr + 64 * b + 32 * half, raw);
+        uint32_t raw[C];
+#pragma unroll
+        for (uint32_t k = 0; k < C; k += 32) tmem_ld32(s_addr + 64 * b + C * half + k, raw + k);
         tmem_ld_wait();
         const int key0 = key_first + static_cast<int>(i * BN);
         if (key0 + static_cast<int>(BN) > hi0 || key0 < lo1) {
-          const int from = lo - key0 - static_cast<int>(32 * half), to = hi - key0 - static_cast<int>(32 * half);
+          const int from = lo - key0 - static_cast<int>(C * half), to = hi - key0 - static_cast<int>(C * half);
 #pragma unroll
-          for (int k = 0; k < 32; k++)
+          for (int k = 0; k < static_cast<int>(C); k++)
             if (k >= to || k < from) raw[k] = 0xff800000u;
         }
         float mx[4] = {__uint_as_float(raw[0]), __uint_as_float(raw[1]), __uint_as_float(raw[2]), __uint_as_float(raw[3])};
 #pragma unroll
-        for (int k = 4; k < 28; k += 8)
+        for (uint32_t k = 4; k < C - 4; k += 8)
 #pragma unroll
-          for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], __uint_as_float(raw[k + e]), __uint_as_float(raw[k + 4 + e]));
+          for (uint32_t e = 0; e < 4; e++) mx[e] = max3(mx[e], __uint_as_float(raw[k + e]), __uint_as_float(raw[k + 4 + e]));
 #pragma unroll
-        for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], __uint_as_float(raw[28 + e]));
-        const float m_half = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        shared_max[x][i & 1][half][r] = m_half;
-        tc_fence_before();
-        named_bar_sync(1 + x, 256);  // (both halves have read their S, too: P goes over it)
-        tc_fence_after();
-        const float m_tile = fmaxf(m_half, shared_max[x][i & 1][half ^ 1][r]) * scale;
+        for (uint32_t e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], __uint_as_float(raw[C - 4 + e]));
+        float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if constexpr (H == 2) {
+          shared_max[x][i & 1][half][r] = m_tile;
+          tc_fence_before();
+          named_bar_sync(1 + x, 256);  // (both halves have read their S, too: P goes over it)
+          tc_fence_after();
+          m_tile = fmaxf(m_tile, shared_max[x][i & 1][half ^ 1][r]);
+        }
+        m_tile *= scale;
         const bool grow = m_tile > m_run + GROW;
         const float m_new = grow ? m_tile : m_run, corr = grow ? ex2(m_run - m_new) : 1.f;
         m_run = m_new;
@@ -454,7 +463,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
           __syncwarp();
           tc_fence_after();
 #pragma unroll 1
-          for (uint32_t k = 0; k < D / 32; k++) {
+          for (uint32_t k = 0; k < D / (16 * H); k++) {
             uint32_t o[16];
             tmem_ld16(o_addr + 16 * k, o);
             tmem_ld_wait();
@@ -464,35 +473,40 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
           }
         }
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t ph[16];
         const float off = P_UP - m_new;
 #pragma unroll
-        for (int k = 0; k < 16; k++) {
-          float e0, e1;
-          fma2(e0, e1, __uint_as_float(raw[2 * k]), __uint_as_float(raw[2 * k + 1]), scale, off);
-          const float p0 = ex2(e0), p1 = ex2(e1);
-          add2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], p0, p1);
-          ph[k] = pack2<false>(p0, p1);
+        for (uint32_t k0 = 0; k0 < C; k0 += 32) {
+          uint32_t ph[16];
+#pragma unroll
+          for (uint32_t k = 0; k < 16; k++) {
+            float e0, e1;
+            fma2(e0, e1, __uint_as_float(raw[k0 + 2 * k]), __uint_as_float(raw[k0 + 2 * k + 1]), scale, off);
+            const float p0 = ex2(e0), p1 = ex2(e1);
+            add2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], p0, p1);
+            ph[k] = pack2<false>(p0, p1);
+          }
+          tmem_st16(s_addr + 64 * b + (C * half + k0) / 2, ph);  // (every S value of this row is in registers)
         }
-        tmem_st16(s_addr + 64 * b + 16 * half, ph);
         l_run = l_run * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&p_ready[x][b]));
       }
-      // the row's sum over both halves
-      shared_max[x][n & 1][half][r] = l_run;
+      if constexpr (H == 2) shared_max[x][n & 1][half][r] = l_run;
       waitx(&o_done[x], pieces & 1);
-      named_bar_sync(1 + x, 256);
-      l_run += shared_max[x][n & 1][half ^ 1][r];
+      if constexpr (H == 2) {  // the row's sum over both halves
+        named_bar_sync(1 + x, 256);
+        l_run += shared_max[x][n & 1][half ^ 1][r];
+      }
+      __syncwarp();
       tc_fence_after();
       if (first == 0 && n == keys.tiles) {
         // ---- the whole item: O / l through the dead Q tile, whole rows of it to memory ----
         const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
         uint8_t* stage = smem + x * S::Q_B;
 #pragma unroll 1
-        for (uint32_t k = 0; k < D / 32; k++) {
+        for (uint32_t k = 0; k < D / (16 * H); k++) {
           uint32_t o[16];
           tmem_ld16(o_addr + 16 * k, o);
           tmem_ld_wait();
@@ -501,19 +515,19 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = __uint_as_float(o[8 * e + column_of(j)]) * inv;
-            const uint32_t u = half * (D / 16) + 2 * k + e;
+            const uint32_t u = half * (D / (8 * H)) + 2 * k + e;
             *reinterpret_cast<uint4*>(stage + r * (D * 2) + ((u ^ (r & (D / 8 - 1))) << 4)) = a.bf ? pack8<true>(v) : pack8<false>(v);
           }
         }
-        named_bar_sync(1 + x, 256);
-        if (tile_row < q.rows && !abort_s) store_rows<D>(a, q.q0, head, tile_row, min(BM, q.rows - tile_row), stage, (half * 4 + quad) * 32 + lane, 256);
+        named_bar_sync(1 + x, 128 * H);
+        if (tile_row < q.rows && !abort_s) store_rows<D>(a, q.q0, head, tile_row, min(BM, q.rows - tile_row), stage, (half * 4 + quad) * 32 + lane, 128 * H);
       } else {
         // ---- a part of an item: as it is, to be joined ----
         const uint32_t first_cta = start / share;
         float* mine = scratch + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PARTIAL;
-        float4* to = reinterpret_cast<float4*>(mine) + half * (D / 8) * S::ROWS + x * BM + r;
+        float4* to = reinterpret_cast<float4*>(mine) + half * (D / (4 * H)) * S::ROWS + x * BM + r;
 #pragma unroll 1
-        for (uint32_t k = 0; k < D / 32; k++) {
+        for (uint32_t k = 0; k < D / (16 * H); k++) {
           uint32_t o[16];
           tmem_ld16(o_addr + 16 * k, o);
           tmem_ld_wait();
