@@ -21,21 +21,14 @@ struct AttnArgs {
   uint32_t bf;    // activations are bfloat16
   uint32_t q_vec; // rows of q are 16-byte aligned
 };
-// A bounded wait for a barrier's phase: false after 2^20 polls or two seconds. A poll suspends its thread until the phase is complete, 5 us
-// at most: polls without that time took two thirds of the issue slots of the kernel for many queries.
-__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity) {
+// A bounded wait for a barrier's phase: false after 2^20 polls or two seconds, or when *stop (may be null) is set.
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const volatile uint32_t* stop = nullptr) {
   if (mbar_test(bar, parity)) return true;
   unsigned long long t0 = 0, t;
   for (uint32_t i = 0; i < 1u << 20; i++) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity), "r"(5000u)
-        : "memory");
-    if (ok) return true;
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 15) != 15) continue;
+    if (stop && *stop) return false;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     if (t0 == 0) t0 = t;
     if (t - t0 > 2000000000ull) return false;

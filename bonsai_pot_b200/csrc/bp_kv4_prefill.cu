@@ -82,7 +82,7 @@ struct Cursor {
 // Byte offset of 16-byte unit u of row r in an operand tile of `rows` rows: chunks of 64 dims, 128-byte swizzle.
 __device__ __forceinline__ uint32_t oper_off(uint32_t rows, uint32_t r, uint32_t u) { return (u >> 3) * (rows * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4); }
 
-// A quarter of the codes of one token's K and V (an expander warp has the same quarter of every token), and their scales; `id` is a page of the
+// A quarter of the codes of one token's K and V and their scales; `id` is a page of the
 // pool.
 template <int D>
 struct Raw {
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   using S = Shape<D, NQ>;
   constexpr uint32_t THREADS = S::THREADS;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t k_full[SLOTS], v_full[SLOTS], k_empty[NQ][SLOTS], v_empty[NQ][SLOTS];
+  __shared__ __align__(8) uint64_t k_full[SLOTS], v_full[SLOTS], k_empty[SLOTS], v_empty[SLOTS], pv_done[NQ][SLOTS];
   __shared__ __align__(8) uint64_t s_ready[NQ][2], p_ready[NQ][2], p_free[NQ][2], o_done[NQ], drained;
   __shared__ float shared_max[NQ][2][S::H][BM];  // [query tile][tile & 1][half][row]
   __shared__ float row_scale[S::ROWS];  // of a row's queries: the power of two that they were divided by
@@ -187,10 +187,9 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     for (uint32_t i = 0; i < SLOTS; i++) {
       mbar_init(smem_u32(&k_full[i]), 8);
       mbar_init(smem_u32(&v_full[i]), 8);
-      for (uint32_t x = 0; x < NQ; x++) {
-        mbar_init(smem_u32(&k_empty[x][i]), 1);
-        mbar_init(smem_u32(&v_empty[x][i]), 1);
-      }
+      mbar_init(smem_u32(&k_empty[i]), NQ);
+      mbar_init(smem_u32(&v_empty[i]), NQ);
+      for (uint32_t x = 0; x < NQ; x++) mbar_init(smem_u32(&pv_done[x][i]), 1);
     }
     for (uint32_t x = 0; x < NQ; x++) {
       for (uint32_t b = 0; b < 2; b++) {
@@ -211,13 +210,15 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   pdl_launch_dependents();
   pdl_wait();
 
-  // (after one wait has given up no other one waits)
+  // After one wait has given up no other one waits.
   auto waitx = [&](uint64_t* bar, uint32_t parity) {
-    if (abort_s) return;
-    if (!wait_phase(smem_u32(bar), parity)) {
+    if (mbar_test(smem_u32(bar), parity)) return true;
+    if (!abort_s && wait_phase(smem_u32(bar), parity, &abort_s)) return true;
+    if (!abort_s) {
       abort_s = 1;
       reinterpret_cast<volatile uint32_t*>(a.err)[1] = 1;
     }
+    return false;
   };
 
   // ---- the line of key tiles, and this CTA's stretch [c0, c1) of it ----
@@ -331,15 +332,14 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         const uint32_t s_col = tmem + x * 128, o_col = tmem + S::TM_O + x * 128;
         for (uint32_t i = 0; i < n; i++) {
           const uint32_t c = done + i, s = c % SLOTS, b = c & 1;
-          waitx(&p_ready[x][b], (c >> 1) & 1);
-          waitx(&v_full[s], (c / SLOTS) & 1);
-          if (abort_s) break;
+          if (!waitx(&p_ready[x][b], (c >> 1) & 1) || !waitx(&v_full[s], (c / SLOTS) & 1)) break;
           tc_fence_after();
           const uint64_t vb = dmn + ((smem_base + S::OFF_V + s * S::KV_B) >> 4);
 #pragma unroll
           for (uint32_t ks = 0; ks < BN / 16; ks++) umma_f16_ts(o_col, s_col + 64 * b + 8 * ks, vb + ks * (16 * 128 >> 4), IDESC, (i | ks) ? 1u : 0u);
           umma_commit(smem_u32(&p_free[x][b]));
-          umma_commit(smem_u32(&v_empty[x][s]));
+          umma_commit(smem_u32(&pv_done[x][s]));
+          umma_commit(smem_u32(&v_empty[s]));
         }
         umma_commit(smem_u32(&o_done[x]));
       }
@@ -352,9 +352,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         const uint64_t qa = dk + ((smem_base + x * S::Q_B) >> 4);
         for (uint32_t i = 0; i < n; i++) {
           const uint32_t c = done + i, s = c % SLOTS, b = c & 1;
-          waitx(&k_full[s], (c / SLOTS) & 1);
-          if (c >= 2) waitx(&p_free[x][b], ((c >> 1) - 1) & 1);
-          if (abort_s) break;
+          if (!waitx(&k_full[s], (c / SLOTS) & 1) || (c >= 2 && !waitx(&p_free[x][b], ((c >> 1) - 1) & 1))) break;
           tc_fence_after();
           const uint64_t kb = dk + ((smem_base + S::OFF_K + s * S::KV_B) >> 4);
 #pragma unroll
@@ -365,7 +363,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       }
     } else if (warp < S::FIRST_SOFTMAX) {
       // ---------------- codes -> operand tiles ----------------
-      const uint32_t quarter = warp & 3, row = lane + 32 * ((warp - S::FIRST_EXPANDER) >> 2);
+      const uint32_t quarter = lane >> 3, row = 8 * (warp - S::FIRST_EXPANDER) + (lane & 7);  // a warp: all of eight tokens, eight rows per 16-byte phase
       const int32_t* table = a.page_table + static_cast<size_t>(cur.r) * a.table_stride;
       // Page ids are asked for two tiles ahead and looked at one tile ahead, when the codes are asked for: nothing here waits for memory.
       // A token that holds no key of the request (or lies in a page outside the pool) gets page 0's codes, and zeros for its scales.
@@ -392,16 +390,12 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         id = id_next;
         if (i + 1 < n) ask_codes();
         if (i + 2 < n) id_next = ask_id(key + static_cast<int>(BN));
-        if (c >= SLOTS)
-          for (uint32_t x = 0; x < NQ; x++) waitx(&k_empty[x][s], (c / SLOTS - 1) & 1);
-        if (__any_sync(FULL, abort_s)) break;
+        if (c >= SLOTS && !__all_sync(FULL, waitx(&k_empty[s], (c / SLOTS - 1) & 1))) break;
         put<D, false>(mine, smem + S::OFF_K + s * S::KV_B, row, quarter, a.bias);
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&k_full[s]));
-        if (c >= SLOTS)
-          for (uint32_t x = 0; x < NQ; x++) waitx(&v_empty[x][s], (c / SLOTS - 1) & 1);
-        if (__any_sync(FULL, abort_s)) break;
+        if (c >= SLOTS && !__all_sync(FULL, waitx(&v_empty[s], (c / SLOTS - 1) & 1))) break;
         put<D, true>(mine, smem + S::OFF_V + s * S::KV_B, row, quarter, a.bias);
         fence_proxy_async();
         __syncwarp();
@@ -423,10 +417,10 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       float m_run = NEG_BIG, l_run = 0.f;
       for (uint32_t i = 0; i < n; i++) {
         const uint32_t c = done + i, b = c & 1, s = c % SLOTS;
-        waitx(&s_ready[x][b], (c >> 1) & 1);
+        (void)waitx(&s_ready[x][b], (c >> 1) & 1);
         __syncwarp();
         tc_fence_after();
-        if (half == 0 && quad == 0 && lane == 0) mbar_arrive(smem_u32(&k_empty[x][s]));  // Q K^T of the tile is complete
+        if (half == 0 && quad == 0 && lane == 0) mbar_arrive(smem_u32(&k_empty[s]));  // Q K^T of the tile is complete
         uint32_t raw[C];
 #pragma unroll
         for (uint32_t k = 0; k < C; k += 32) tmem_ld32(s_addr + 64 * b + C * half + k, raw + k);
@@ -459,7 +453,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         m_run = m_new;
         if (i > 0 && __any_sync(FULL, grow)) {
           // O_X may be rescaled only between two P V: the previous tile's must be complete
-          waitx(&v_empty[x][(c - 1) % SLOTS], ((c - 1) / SLOTS) & 1);
+          (void)waitx(&pv_done[x][(c - 1) % SLOTS], ((c - 1) / SLOTS) & 1);
           __syncwarp();
           tc_fence_after();
 #pragma unroll 1
@@ -494,7 +488,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         if (lane == 0) mbar_arrive(smem_u32(&p_ready[x][b]));
       }
       if constexpr (H == 2) shared_max[x][n & 1][half][r] = l_run;
-      waitx(&o_done[x], pieces & 1);
+      (void)waitx(&o_done[x], pieces & 1);
       if constexpr (H == 2) {  // the row's sum over both halves
         named_bar_sync(1 + x, 256);
         l_run += shared_max[x][n & 1][half ^ 1][r];
