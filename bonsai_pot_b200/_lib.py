@@ -202,20 +202,19 @@ class AttnStruct(C.Structure):
                [(k, C.c_uint32) for k in ("n_req", "n_head", "total_q", "max_q", "max_kv", "table_stride", "window")] + [("scale", C.c_float)]
 
 
-_rows, _pool, _rope = C.POINTER(RowsStruct), C.POINTER(PoolStruct), C.POINTER(RopeTableStruct)
-
-# name -> (restype, argtypes); must list every symbol include/bonsai_paged.h declares.
+# name -> (restype, argtypes); must list every symbol include/bonsai_paged.h declares. Structs go by address (an int is converted
+# fastest, and these calls are made several times per layer and token).
 PAGED_SIGNATURES = {
     "bp_paged_create": (_int, [C.c_int32, _pp]),
     "bp_paged_destroy": (None, [_vp]),
     "bp_paged_status": (_int, [_vp, _vp]),
     "bp_paged_last_error": (C.c_char_p, [_vp]),
     "bp_rope_fill": (_int, [_vp, _vp, C.POINTER(RopeConfigStruct), _vp]),
-    "bp_rope": (_int, [_vp, _vp, _u32, _rows, _rows, _u32, _u32, _u32, _vp, _rope, _vp, C.c_float, _u32]),
-    "bp_kv4_pool_bytes": (_u64, [_pool]),
-    "bp_kv4_append": (_int, [_vp, _vp, _u32, _pool, _rows, _rows, _u32, _vp, _vp, _rope, _vp, C.c_float]),
-    "bp_kv4_read": (_int, [_vp, _vp, _u32, _pool, _vp, _u32, _rows, _rows]),
-    "bp_kv4_attention": (_int, [_vp, _vp, _u32, _pool, C.POINTER(AttnStruct)]),
+    "bp_rope": (_int, [_vp, _vp, _u32, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, C.c_float, _u32]),
+    "bp_kv4_pool_bytes": (_u64, [_vp]),
+    "bp_kv4_append": (_int, [_vp, _vp, _u32, _vp, _vp, _vp, _u32, _vp, _vp, _vp, _vp, C.c_float]),
+    "bp_kv4_read": (_int, [_vp, _vp, _u32, _vp, _vp, _u32, _vp, _vp]),
+    "bp_kv4_attention": (_int, [_vp, _vp, _u32, _vp, _vp]),
 }
 
 _LIB = None

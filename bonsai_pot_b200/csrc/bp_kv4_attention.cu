@@ -449,10 +449,9 @@ __device__ __noinline__ void clear_scales(uint8_t* buf, uint32_t pages, int from
   __syncwarp();
 }
 
-// A warp: row `row` of the `n` partial results at part(k) of an item, in order, becomes the output's row (to == null) or that of the
-// partial result `to`.
+// A warp: row `row` of the `n` partial results at part(k) of an item, in order, becomes the output's row.
 template <int D, int NT, typename Part>
-__device__ __forceinline__ void join_row(const AttnArgs& a, const Piece& p, uint32_t row, uint32_t n, Part part, float* to, uint32_t lane) {
+__device__ __forceinline__ void join_row(const AttnArgs& a, const Piece& p, uint32_t row, uint32_t n, Part part, uint32_t lane) {
   using S = Shape<D, NT>;
   constexpr int V = D / 32;  // dims of a lane
   float m = NEG_BIG, l = 0.f, o[V] = {};
@@ -488,13 +487,6 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, const Piece& p, uint
       }
     }
   }
-  if (to) {
-    float* v = to + row * S::STRIDE + V * lane;
-    if constexpr (V == 4) *reinterpret_cast<float4*>(v) = make_float4(o[0], o[1], o[2], o[3]);
-    else *reinterpret_cast<float2*>(v) = make_float2(o[0], o[1]);
-    if (lane == 0) *reinterpret_cast<float2*>(to + row * S::STRIDE + D) = make_float2(m, l);
-    return;
-  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* out = out_row(a, p.q0, p.head, p.row0 + row) + V * lane;
   if constexpr (V == 4) {
@@ -504,6 +496,43 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, const Piece& p, uint
     out[0] = static_cast<uint16_t>(h);
     out[1] = static_cast<uint16_t>(h >> 16);
   }
+}
+
+// The same of four rows at a time, eight lanes each, for few partial results, one after the other; into the output (to == null) or the partial
+// result `to`.
+template <int D, int NT, typename Part>
+__device__ __forceinline__ void join_rows4(const AttnArgs& a, const Piece& p, uint32_t row0, uint32_t n, Part part, float* to, uint32_t lane) {
+  using S = Shape<D, NT>;
+  constexpr int V = D / 32;  // fours of dims of a lane
+  const uint32_t row = min(row0 + (lane >> 3), p.rows - 1), at = row * S::STRIDE, col = 4 * (lane & 7);
+  float m = NEG_BIG, l = 0.f;
+  float4 o[V];
+#pragma unroll
+  for (int x = 0; x < V; x++) o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+  for (uint32_t k = 0; k < n; k++) {
+    const float* v = part(k) + at;
+    const float2 ml = *reinterpret_cast<const float2*>(v + D);
+    float4 e[V];
+#pragma unroll
+    for (int x = 0; x < V; x++) e[x] = *reinterpret_cast<const float4*>(v + 32 * x + col);
+    const float top = fmaxf(m, ml.x), w0 = ex2(m - top), w1 = ex2(ml.x - top);
+    m = top;
+    l = l * w0 + ml.y * w1;
+#pragma unroll
+    for (int x = 0; x < V; x++) o[x] = make_float4(o[x].x * w0 + e[x].x * w1, o[x].y * w0 + e[x].y * w1, o[x].z * w0 + e[x].z * w1, o[x].w * w0 + e[x].w * w1);
+  }
+  if (row0 + (lane >> 3) >= p.rows) return;
+  if (to) {
+#pragma unroll
+    for (int x = 0; x < V; x++) *reinterpret_cast<float4*>(to + at + 32 * x + col) = o[x];
+    if ((lane & 7) == 0) *reinterpret_cast<float2*>(to + at + D) = make_float2(m, l);
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* out = out_row(a, p.q0, p.head, p.row0 + row) + col;
+#pragma unroll
+  for (int x = 0; x < V; x++) store4(a.bf, out + 32 * x, o[x].x * inv, o[x].y * inv, o[x].z * inv, o[x].w * inv);
 }
 
 template <int D, int NT, uint32_t PAGE>
@@ -798,9 +827,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
     const bool all = p.start >= plan[0] && p.start + p.units <= plan[1];
     const uint32_t first_cta = all ? 0 : p.start / plan[2];
     float* to = all ? nullptr : exchange + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PARTIAL;
-    for (uint32_t row = 0; row < p.rows; row++) {  // the warps take the rows of all items in turn
+    for (uint32_t row = 0; row < p.rows; row += 4) {  // the warps take the rows of all items in turn
       if (turn == warp)
-        join_row<D, NT>(a, p, row, n_run, [&](uint32_t k) {
+        join_rows4<D, NT>(a, p, row, n_run, [&](uint32_t k) {
           const uint32_t x = __fns(run, 0, k + 1);
           return (x & 1) ? reinterpret_cast<const float*>(smem + (x >> 1) * (RING * S::PART)) : scratch + (static_cast<size_t>(blockIdx.x) * NWARP + (x >> 1)) * S::PARTIAL;
         }, to, lane);
@@ -817,10 +846,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
   __syncthreads();
   if (threadIdx.x < n_joins) {
     Join& j = joins[threadIdx.x];
-    __threadfence();
-    j.last = atomicAdd(&counters[j.first_cta], 1u) == j.n - 1;
+    j.last = arrive(&counters[j.first_cta]) == j.n - 1;
     if (j.last) counters[j.first_cta] = 0;  // for the next launch
-    __threadfence();
   }
   __syncthreads();
   turn = 0;
@@ -829,8 +856,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
     if (!j.last) continue;
     const float* from = exchange + static_cast<size_t>(2 * j.first_cta) * S::PARTIAL;
     const Piece& p = pieces[j.piece];
-    for (uint32_t row = 0; row < p.rows; row++) {
-      if (turn == warp) join_row<D, NT>(a, p, row, j.n, [&](uint32_t k) { return from + (2 * k + (k == 0)) * S::PARTIAL; }, nullptr, lane);
+    auto part = [&](uint32_t k) { return from + (2 * k + (k == 0)) * S::PARTIAL; };
+    const uint32_t step = j.n <= 4 ? 4 : 1;
+    for (uint32_t row = 0; row < p.rows; row += step) {
+      if (turn == warp) {
+        if (step == 4) join_rows4<D, NT>(a, p, row, j.n, part, nullptr, lane);
+        else join_row<D, NT>(a, p, row, j.n, part, lane);
+      }
       if (++turn == NWARP) turn = 0;
     }
   }
@@ -873,8 +905,6 @@ cudaError_t bp_kv4_attention_init(bp_paged_ctx* c) {
   return cudaMemset(c->counters, 0, static_cast<size_t>(c->sm_count) * sizeof(uint32_t));
 }
 
-constexpr uint32_t FEW_ROWS = 48;
-
 cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, const Pool& pool, uint32_t head_dim, const bp_kv4_attn& in) {
   AttnArgs a;
   a.pool = pool;
@@ -896,7 +926,12 @@ cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, co
   a.bias = 0x64006400u;
   a.bf = bf;
   a.q_vec = reinterpret_cast<uintptr_t>(in.q.data) % 16 == 0 && in.q.tok_stride % 8 == 0 && in.q.head_stride % 8 == 0;
-  if (static_cast<uint64_t>(a.max_q) * a.group > FEW_ROWS) return bp_launch_kv4_prefill(c, s, head_dim, a);
+  // Which kernel. Up to 16 rows (tokens x query heads per KV head) a request is two tiles of eight here, and every tile more expands the
+  // codes again; there a row costs nothing up to 128. us, this kernel / the other one, D = 128, 8 KV heads: 16 requests of 4096 keys, 12 rows
+  // 42.5 / 73.7, 16 rows 42.6 / 73.8, 24 rows 77 / 74, 32 rows 80 / 74; with few items the line moves up, 1 request of 2000 keys, 32 rows
+  // 20 / 29.5, of 30000 keys 51.9 / 63.6 (48 rows 65.5 / 64.2). D = 64: 16 x 4096, 15 rows 31 / 58, 20 rows 52 / 59, 30 rows 55 / 59, 40 rows 68 / 59.
+  const uint64_t rows = static_cast<uint64_t>(a.max_q) * a.group;
+  if (rows > 32 || (rows > 16 && 2 * static_cast<uint64_t>(a.n_req) * pool.n_kv_head > static_cast<uint64_t>(c->sm_count))) return bp_launch_kv4_prefill(c, s, head_dim, a);
   return with_kernel(head_dim, a.max_q * a.group > 8, pool.page, [&](auto kernel, auto shape) {
     return bp_launch(true, kernel, dim3(c->sm_count), dim3(shape.THREADS), shape.SMEM, s, a, c->partials, c->counters);
   });

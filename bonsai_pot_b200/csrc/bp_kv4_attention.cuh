@@ -36,6 +36,14 @@ __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const 
   return false;
 }
 
+// One more piece of an item has been written (by threads that have met this one at a barrier since); the count before it. What the other
+// pieces' writers had written is visible to whoever meets this thread at a barrier afterwards.
+__device__ __forceinline__ uint32_t arrive(uint32_t* counter) {
+  uint32_t before;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+  return before;
+}
+
 // Four dims of an output row.
 __device__ __forceinline__ void store4(bool bf, uint16_t* p, float a, float b, float c, float d) {
   const uint32_t x = bf ? pack2<true>(a, b) : pack2<false>(a, b), y = bf ? pack2<true>(c, d) : pack2<false>(c, d);

@@ -549,10 +549,8 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     if (threadIdx.x == 0) {
       if (!whole) {
         const uint32_t first_cta = start / share, parts = (start + keys.tiles - 1) / share - first_cta + 1;
-        __threadfence();
-        const bool last = atomicAdd(&counters[first_cta], 1u) == parts - 1;
+        const bool last = arrive(&counters[first_cta]) == parts - 1;
         if (last) counters[first_cta] = 0;  // for the next launch
-        __threadfence();
         join_s = Join{first_cta, parts, last};
       }
       if (pos < c1) {

@@ -15,42 +15,57 @@ from .errors import ConfigError, raise_for_status
 
 _LAYOUTS = {"half": 0, "interleaved": 1}
 _SCALINGS = {None: 0, "linear": 1, "ntk": 2, "yarn": 3}
-_DTYPES = {}
+_DTYPES, _I32, _I64 = {}, None, None
+
+
+def _types():
+    """The torch types (the package itself does not import torch; whoever calls with tensors has)."""
+    global _I32, _I64
+    import torch
+    _DTYPES.update({torch.float16: 0, torch.bfloat16: 1})
+    _I32, _I64 = torch.int32, torch.int64
+
+
+def _bad(text):
+    raise ConfigError("invalid config: " + text)
 
 
 def _dtype(t):
     code = _DTYPES.get(t.dtype)
     if code is None:
-        code = {"torch.float16": 0, "torch.bfloat16": 1}.get(str(t.dtype))
+        _types()
+        code = _DTYPES.get(t.dtype)
         if code is None:
-            raise ConfigError(f"invalid config: rows are float16 or bfloat16, not {t.dtype}")
-        _DTYPES[t.dtype] = code
+            _bad(f"rows are float16 or bfloat16, not {t.dtype}")
     return code
 
 
-def _rows(t, what, like=None):
-    shape = t.shape
-    if len(shape) != 3:
-        raise ConfigError(f"invalid config: {what} must be [tokens, heads, head_dim], not {tuple(shape)}")
-    if like is not None and (shape != like.shape or t.dtype != like.dtype):
-        raise ConfigError(f"invalid config: {what} must have the shape and type of the rows it goes with: {tuple(shape)} {t.dtype}, not {tuple(like.shape)} {like.dtype}")
-    a, b, c = t.stride()
-    if c != 1 and shape[2] > 1:
-        raise ConfigError(f"invalid config: a row of {what} must be dense")
-    return _lib.RowsStruct(t.data_ptr(), a, b)
+# The checks below are on the path of every call (a decoded token makes three of them per layer), hence as few tensor methods as will do.
+def _rows(to, t, what):
+    """t's address and strides into a RowsStruct."""
+    strides = t.stride()
+    if len(strides) != 3:
+        _bad(f"{what} must be [tokens, heads, head_dim], not {tuple(t.shape)}")
+    to.tok_stride, to.head_stride, dense = strides
+    if dense != 1 and t.shape[2] > 1:
+        _bad(f"a row of {what} must be dense")
+    to.data = t.data_ptr()
 
 
-def _index(t, what, n, dtype="torch.int32"):
-    if str(t.dtype) != dtype or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
-        raise ConfigError(f"invalid config: {what} must be {n} dense {dtype} values, not {tuple(t.shape)} {t.dtype}")
+def _like(t, rows, what):
+    if t.dtype is not rows.dtype or t.shape != rows.shape:
+        _bad(f"{what} must have the shape and type of the rows it goes with: {tuple(t.shape)} {t.dtype}, not {tuple(rows.shape)} {rows.dtype}")
+
+
+def _index(t, what, n, slots=False):
+    if t.dtype is not (_I64 if slots else _I32) or t.shape != (n,) or not t.is_contiguous():
+        _bad(f"{what} must be {n} dense values of {_I64 if slots else _I32}, not {tuple(t.shape)} {t.dtype}")
     return t.data_ptr()
 
 
 def _weight(w, rows, what):
-    if w is None:
-        return None
-    if w.dtype != rows.dtype or w.numel() != rows.shape[2] or not w.is_contiguous():
-        raise ConfigError(f"invalid config: {what} must be {rows.shape[2]} dense values of the rows' type")
+    if w.dtype is not rows.dtype or w.numel() != rows.shape[2] or not w.is_contiguous():
+        _bad(f"{what} must be {rows.shape[2]} dense values of the rows' type")
     return w.data_ptr()
 
 
@@ -64,6 +79,7 @@ class RopeTable:
             raise ConfigError("invalid config: a RoPE table is a dense float32 tensor [positions, rot_dim / 2, 2]")
         self.data = data
         self._c = _lib.RopeTableStruct(data.data_ptr(), data.shape[0], 2 * data.shape[1], _LAYOUTS[layout])
+        self._p = C.addressof(self._c)
 
 
 class KV4Pool:
@@ -73,12 +89,13 @@ class KV4Pool:
         need = KV4Pool.bytes(n_pages, page_tokens, n_kv_head, head_dim)
         if str(data.dtype) != "torch.uint8" or not data.is_contiguous() or data.numel() < need:
             raise ConfigError(f"invalid config: a pool of this shape is a dense uint8 tensor of at least {need} bytes")
-        self.data, self.n_kv_head, self.head_dim = data, n_kv_head, head_dim
+        self.data, self.page_tokens, self.n_kv_head, self.head_dim = data, page_tokens, n_kv_head, head_dim
         self._c = _lib.PoolStruct(data.data_ptr(), n_pages, page_tokens, n_kv_head, head_dim)
+        self._p = C.addressof(self._c)
 
     @staticmethod
     def bytes(n_pages, page_tokens, n_kv_head, head_dim):
-        n = _lib.load().bp_kv4_pool_bytes(_lib.PoolStruct(None, n_pages, page_tokens, n_kv_head, head_dim)) if min(n_pages, page_tokens, n_kv_head, head_dim) > 0 else 0
+        n = _lib.load().bp_kv4_pool_bytes(C.byref(_lib.PoolStruct(None, n_pages, page_tokens, n_kv_head, head_dim))) if min(n_pages, page_tokens, n_kv_head, head_dim) > 0 else 0
         if n == 0:
             raise ConfigError("invalid config: a pool has n_pages >= 1, page_tokens 16, 32 or 64, n_kv_head >= 1 and head_dim 64 or 128")
         return n
@@ -90,11 +107,18 @@ class PagedContext:
     def __init__(self, device=0):
         self._lib = _lib.load()
         self._h = C.c_void_p()
+        self._setup()
         st = self._lib.bp_paged_create(device, C.byref(self._h))
         if st != 0:
             msg = self._message()
             self.close()
             raise_for_status(st, msg)
+
+    def _setup(self):
+        # arguments of a call, filled anew by every one (a context is not thread-safe)
+        self._a, self._b, self._attn = _lib.RowsStruct(), _lib.RowsStruct(), _lib.AttnStruct()
+        self._q, self._o = self._attn.q, self._attn.out
+        self._pa, self._pb, self._pattn = C.addressof(self._a), C.addressof(self._b), C.addressof(self._attn)
 
     def _message(self):
         return (self._lib.bp_paged_last_error(self._h) or b"").decode() if self._h else ""
@@ -134,48 +158,65 @@ class PagedContext:
 
     def rope(self, x, out, positions, table, w_norm=None, eps=1e-6, inverse=False, stream=None):
         """x [tokens, heads, head_dim] -> out (may be x): RMS norm over the head if w_norm is given, then the rotation by `positions`."""
-        rx, ro = _rows(x, "x"), _rows(out, "out", x)
+        dtype = _dtype(x)
+        _rows(self._a, x, "x")
+        _like(out, x, "out")
+        _rows(self._b, out, "out")
         n, heads, dim = x.shape
-        self._check(self._lib.bp_rope(self._h, _stream(stream), _dtype(x), rx, ro, n, heads, dim, _index(positions, "positions", n), table._c,
-                                      _weight(w_norm, x, "w_norm"), eps, inverse))
+        st = self._lib.bp_rope(self._h, stream if stream is None else _stream(stream), dtype, self._pa, self._pb, n, heads, dim, _index(positions, "positions", n), table._p,
+                               None if w_norm is None else _weight(w_norm, x, "w_norm"), eps, inverse)
+        if st:
+            self._check(st)
 
     def append(self, pool, k, v, positions, slots, table=None, w_k_norm=None, eps=1e-6, stream=None):
         """k, v [tokens, KV heads, head_dim] -> the pool at `slots`; K is normalised (w_k_norm) and rotated (table) on the way."""
-        rk, rv = _rows(k, "k"), _rows(v, "v", k)
-        n = self._fits(pool, k)
-        self._check(self._lib.bp_kv4_append(self._h, _stream(stream), _dtype(k), pool._c, rk, rv, n,
-                                            None if positions is None else _index(positions, "positions", n), _index(slots, "slots", n, "torch.int64"),
-                                            None if table is None else table._c, _weight(w_k_norm, k, "w_k_norm"), eps))
+        dtype, n = self._kv(pool, k, v)
+        st = self._lib.bp_kv4_append(self._h, stream if stream is None else _stream(stream), dtype, pool._p, self._pa, self._pb, n,
+                                     None if positions is None else _index(positions, "positions", n), _index(slots, "slots", n, True),
+                                     None if table is None else table._p, None if w_k_norm is None else _weight(w_k_norm, k, "w_k_norm"), eps)
+        if st:
+            self._check(st)
 
     def read(self, pool, slots, k, v, stream=None):
         """The pool's rows at `slots` -> k, v [tokens, KV heads, head_dim]; keys are as they were stored."""
-        rk, rv = _rows(k, "k"), _rows(v, "v", k)
-        n = self._fits(pool, k)
-        self._check(self._lib.bp_kv4_read(self._h, _stream(stream), _dtype(k), pool._c, _index(slots, "slots", n, "torch.int64"), n, rk, rv))
+        dtype, n = self._kv(pool, k, v)
+        st = self._lib.bp_kv4_read(self._h, stream if stream is None else _stream(stream), dtype, pool._p, _index(slots, "slots", n, True), n, self._pa, self._pb)
+        if st:
+            self._check(st)
 
     def attention(self, pool, q, out, q_start, kv_len, page_table, max_q, max_kv, scale=None, window=0, stream=None):
         """q [tokens of all requests, heads, head_dim] -> out. Request r has the rows q_start[r] .. q_start[r + 1] and sees kv_len[r] keys in
         the pages page_table[r]; max_q, max_kv: no request has more. scale: 1 / sqrt(head_dim) if None; window: 0 = none."""
-        rq, ro = _rows(q, "q"), _rows(out, "out", q)
+        dtype, a = _dtype(q), self._attn
+        _rows(self._q, q, "q")
+        _like(out, q, "out")
+        _rows(self._o, out, "out")
         n, heads, dim = q.shape
         if dim != pool.head_dim:
-            raise ConfigError(f"invalid config: q has head_dim {dim}, the pool {pool.head_dim}")
-        n_req = kv_len.shape[0]
-        if page_table.dim() != 2 or page_table.shape[0] != n_req or str(page_table.dtype) != "torch.int32" or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-            raise ConfigError(f"invalid config: page_table must be int32 [{n_req}, pages] with dense rows")
-        if min(max_q, max_kv, window) < 0:
-            raise ConfigError("invalid config: max_q, max_kv and window must be >= 0")
-        if n_req > 1 and page_table.stride(0) < page_table.shape[1]:
-            raise ConfigError("invalid config: the rows of page_table must not overlap")
+            _bad(f"q has head_dim {dim}, the pool {pool.head_dim}")
+        if page_table.dtype is not _I32 or page_table.dim() != 2:
+            _bad("page_table must be int32 [requests, pages]")
+        (n_req, pages), (stride, dense) = page_table.shape, page_table.stride()
+        if (dense != 1 and pages > 1) or (stride < pages and n_req > 1):
+            _bad("the rows of page_table must be dense and not overlap")
+        if max_q < 0 or max_kv < 0 or window < 0:
+            _bad("max_q, max_kv and window must be >= 0")
         # (what a row of the table holds bounds the keys that are looked at, not the distance of two rows)
-        cap = page_table.shape[1] * pool._c.page_tokens
-        a = _lib.AttnStruct(rq, ro, _index(q_start, "q_start", n_req + 1), _index(kv_len, "kv_len", n_req), page_table.data_ptr(),
-                            n_req, heads, n, max_q, min(max_kv, cap), page_table.stride(0) if n_req > 1 else page_table.shape[1], window,
-                            dim ** -0.5 if scale is None else scale)
-        self._check(self._lib.bp_kv4_attention(self._h, _stream(stream), _dtype(q), pool._c, a))
+        cap = pages * pool.page_tokens
+        a.q_start, a.kv_len, a.page_table = _index(q_start, "q_start", n_req + 1), _index(kv_len, "kv_len", n_req), page_table.data_ptr()
+        a.n_req, a.n_head, a.total_q, a.max_q, a.max_kv, a.window = n_req, heads, n, max_q, max_kv if max_kv < cap else cap, window
+        a.table_stride = stride if n_req > 1 else pages
+        a.scale = dim ** -0.5 if scale is None else scale
+        st = self._lib.bp_kv4_attention(self._h, stream if stream is None else _stream(stream), dtype, pool._p, self._pattn)
+        if st:
+            self._check(st)
 
-    @staticmethod
-    def _fits(pool, rows):
-        if rows.shape[1] != pool.n_kv_head or rows.shape[2] != pool.head_dim:
-            raise ConfigError(f"invalid config: the pool holds {pool.n_kv_head} heads of {pool.head_dim}, the rows have {tuple(rows.shape[1:])}")
-        return rows.shape[0]
+    def _kv(self, pool, k, v):
+        dtype = _dtype(k)
+        _rows(self._a, k, "k")
+        _like(v, k, "v")
+        _rows(self._b, v, "v")
+        n, heads, dim = k.shape
+        if heads != pool.n_kv_head or dim != pool.head_dim:
+            _bad(f"the pool holds {pool.n_kv_head} heads of {pool.head_dim}, the rows have {heads} of {dim}")
+        return dtype, n

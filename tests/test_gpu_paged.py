@@ -490,13 +490,13 @@ def test_refusals(ctx):
         with pytest.raises(bp.ConfigError) as e:
             call()
         assert str(e.value).startswith("invalid config: "), i
-    lib, rows = ctx._lib, bp.paged._lib.RowsStruct(x.data_ptr(), 128, 64)
-    assert lib.bp_rope(ctx._h, None, 0, rows, rows, 3, 2, 64, None, tab._c, None, 0.0, 0) == 7
-    assert lib.bp_kv4_append(ctx._h, None, 0, pool._c, rows, rows, 3, pos.data_ptr(), None, tab._c, None, 0.0) == 7
-    assert lib.bp_kv4_append(ctx._h, None, 0, pool._c, rows, rows, 3, None, slots.data_ptr(), tab._c, None, 0.0) == 7
+    lib, rows = ctx._lib, C.byref(bp.paged._lib.RowsStruct(x.data_ptr(), 128, 64))
+    assert lib.bp_rope(ctx._h, None, 0, rows, rows, 3, 2, 64, None, tab._p, None, 0.0, 0) == 7
+    assert lib.bp_kv4_append(ctx._h, None, 0, pool._p, rows, rows, 3, pos.data_ptr(), None, tab._p, None, 0.0) == 7
+    assert lib.bp_kv4_append(ctx._h, None, 0, pool._p, rows, rows, 3, None, slots.data_ptr(), tab._p, None, 0.0) == 7
     assert lib.bp_kv4_read(ctx._h, None, 0, None, slots.data_ptr(), 3, rows, rows) == 7
-    assert lib.bp_kv4_attention(ctx._h, None, 0, pool._c, None) == 7
-    assert lib.bp_kv4_attention(ctx._h, None, 2, pool._c, bp.paged._lib.AttnStruct()) == 1
+    assert lib.bp_kv4_attention(ctx._h, None, 0, pool._p, None) == 7
+    assert lib.bp_kv4_attention(ctx._h, None, 2, pool._p, C.byref(bp.paged._lib.AttnStruct())) == 1
     with pytest.raises(bp.ConfigError):
         bp.PagedContext(device=99)
     empty = C.c_void_p()
