@@ -931,7 +931,8 @@ cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, co
   // 42.5 / 73.7, 16 rows 42.6 / 73.8, 24 rows 77 / 74, 32 rows 80 / 74; with few items the line moves up, 1 request of 2000 keys, 32 rows
   // 20 / 29.5, of 30000 keys 51.9 / 63.6 (48 rows 65.5 / 64.2). D = 64: 16 x 4096, 15 rows 31 / 58, 20 rows 52 / 59, 30 rows 55 / 59, 40 rows 68 / 59.
   const uint64_t rows = static_cast<uint64_t>(a.max_q) * a.group;
-  if (rows > 32 || (rows > 16 && 2 * static_cast<uint64_t>(a.n_req) * pool.n_kv_head > static_cast<uint64_t>(c->sm_count))) return bp_launch_kv4_prefill(c, s, head_dim, a);
+  // (Without any key there are only zeros to write, and there may be no pool: this kernel looks at none.)
+  if (a.max_kv != 0 && (rows > 32 || (rows > 16 && 2 * static_cast<uint64_t>(a.n_req) * pool.n_kv_head > static_cast<uint64_t>(c->sm_count)))) return bp_launch_kv4_prefill(c, s, head_dim, a);
   return with_kernel(head_dim, a.max_q * a.group > 8, pool.page, [&](auto kernel, auto shape) {
     return bp_launch(true, kernel, dim3(c->sm_count), dim3(shape.THREADS), shape.SMEM, s, a, c->partials, c->counters);
   });

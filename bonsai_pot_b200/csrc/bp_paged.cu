@@ -189,7 +189,7 @@ int bp_rope(bp_paged_ctx* c, void* stream, uint32_t dtype, const bp_rows* x, con
   if (!aligned_to(positions, 4) || !aligned_to(w_norm, 2)) return fail_config(c, "positions must be 4-byte, a norm weight 2-byte aligned");
   if (n_tok == 0) return BP_OK;
   if (!rx.data || !ro.data || !positions || !rope.table) return fail(c, BP_ERR_NULL, "null pointer argument");
-  if (static_cast<uint64_t>(n_tok) * n_head > 0x7fffffffull) return fail_config(c, "n_tok * n_head must be < 2^31");
+  if (static_cast<uint64_t>(n_tok) * n_head > 1ull << 28) return fail_config(c, "n_tok * n_head must be <= 2^28");
   OnDevice on(c->device);
   BP_TRY(c, on.err);
   BP_TRY(c, bp_launch_rope(c, static_cast<cudaStream_t>(stream), dtype == BP_DTYPE_BF16, rx, ro, n_tok, n_head, head_dim,
@@ -269,9 +269,9 @@ int bp_kv4_attention(bp_paged_ctx* c, void* stream, uint32_t dtype, const bp_kv4
   if (a->n_req == 0 || a->total_q == 0 || a->max_q == 0) return BP_OK;
   if (a->n_req > 65535) return fail_config(c, "at most 65535 requests");
   if (static_cast<uint64_t>(a->total_q) * a->n_head > 0x7fffffffull || a->max_kv > 0x7fffff00u) return fail_config(c, "total_q * n_head and max_kv must be < 2^31");
-  // units of 64 keys of 8 rows are counted in 32 bits
+  // units of 64 keys of 8 rows, and what an item of the kernel for many queries costs besides, are counted in 32 bits
   const uint64_t tiles = static_cast<uint64_t>(a->total_q) * (a->n_head / p.n_kv_head) / 8 + a->n_req;
-  if (tiles * p.n_kv_head > 0xffffffffull / (a->max_kv / 64 + 1)) return fail_config(c, "total_q * n_head * max_kv is too large for one call");
+  if (tiles * p.n_kv_head > 0xffffffffull / (a->max_kv / 64 + 8)) return fail_config(c, "total_q * n_head * max_kv is too large for one call");
   if (!rq.data || !ro.data || !a->q_start || !a->kv_len || (a->max_kv != 0 && (!p.data || !a->page_table))) return fail(c, BP_ERR_NULL, "null pointer argument");
   OnDevice on(c->device);
   BP_TRY(c, on.err);

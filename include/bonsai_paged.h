@@ -67,7 +67,7 @@ int bp_rope_fill(bp_paged_ctx* ctx, void* stream, const bp_rope_config* cfg, voi
 
 /* x rows -> out rows (the same memory, or memory that does not overlap): an RMS norm over the head first if w_norm (activation type,
  * [head_dim]) is given, then the rotation by positions[token] (device int32); inverse != 0 turns back, which is the
- * gradient with respect to x (not with w_norm). head_dim even, <= 256. Tokens with a negative position are padding: their
+ * gradient with respect to x (not with w_norm). head_dim even, <= 256; n_tok * n_head <= 2^28. Tokens with a negative position are padding: their
  * rows are not written. */
 typedef struct bp_rows {
   void* data;
@@ -85,7 +85,8 @@ uint64_t bp_kv4_pool_bytes(const bp_kv4_pool* pool);
 /* k, v rows -> the pool, at slots[token] (device int64; negative: padding, nothing is written). K is normalised first if
  * w_k_norm is given and rotated by positions[token] if table is; the squares of a row are summed as a binary tree over
  * neighbouring dims, 1 / sqrt is correctly rounded, nothing is contracted: a cache does not depend on the batch. With a table,
- * tokens with a negative position are padding too. Two tokens with the same slot: one of them is there afterwards. */
+ * tokens with a negative position are padding too. A slot may occur once in a call (the bytes
+ * of one that occurs twice are of both tokens). */
 int bp_kv4_append(bp_paged_ctx* ctx, void* stream, uint32_t dtype, const bp_kv4_pool* pool, const bp_rows* k, const bp_rows* v,
                   uint32_t n_tok, const void* positions, const void* slots, const bp_rope_table* table, const void* w_k_norm, float eps);
 /* The pool's rows at slots[token] -> k, v rows (negative slots: not written). */

@@ -430,6 +430,20 @@ def test_other_streams_and_graphs(ctx, q, kv):
     ctx.status()
 
 
+@pytest.mark.parametrize("q", [1, 200])
+def test_no_keys_at_all(ctx, q):
+    """Zeros for every query, without a look at a pool or a page table (the C entry takes neither)."""
+    rows = normal(1, (2 * q, 4, 64), "f16")
+    out = torch.full_like(rows, float("nan"))
+    start, kv = torch.tensor([0, q, 2 * q], dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    lib = bp.paged._lib
+    r = [lib.RowsStruct(t.data_ptr(), 256, 64) for t in (rows, out)]
+    a = lib.AttnStruct(*r, start.data_ptr(), kv.data_ptr(), None, 2, 4, 2 * q, q, 0, 0, 0, 0.125)
+    assert ctx._lib.bp_kv4_attention(ctx._h, None, 0, C.byref(lib.PoolStruct(None, 1, 16, 2, 64)), C.byref(a)) == 0
+    assert (out == 0).all()
+    ctx.status()
+
+
 def test_nothing_to_do(ctx):
     pool = bp.KV4Pool(torch.zeros(bp.KV4Pool.bytes(1, 16, 2, 64), dtype=torch.uint8, device="cuda"), 1, 16, 2, 64)
     q = torch.zeros(0, 4, 64, dtype=torch.float16, device="cuda")
@@ -504,3 +518,10 @@ def test_refusals(ctx):
     assert lib.bp_paged_status(empty, None) == 5
     lib.bp_paged_destroy(empty)
     ctx.status()
+
+
+def test_the_serving_example(ctx):
+    """Prompts in chunks, decoded tokens, pages that change owners: the outputs are the plain softmax's over what the cache holds. bf16 outputs below 4
+    in magnitude: half a unit is 2^-7 at most, and P's rounding 2^-11 of at most 4."""
+    from examples import paged_serving
+    assert paged_serving.run(steps=20) <= 2.0 ** -7 + 2.0 ** -8
