@@ -7,13 +7,18 @@
 //                           value is an f16 number (the format's choice of m and d): nothing rounds. The next tile's codes are
 //                           on their way in registers meanwhile. Places that hold no key of the request become zeros.
 //   S issuer X (1 thread)   S_X = Q_X K^T (tcgen05.mma kind::f16, M 128, N 64) into one of two 64-column buffers in TMEM
-//   softmax X (8 warps)     two threads per row = TMEM lane, 32 keys each: masks, running maximum (they agree on it through shared memory) and
-//                           sum, P as f16 over the tile's S buffer; O_X is rescaled in TMEM only when a row's maximum grew by more
-//                           than 2^5 (P stays below 2^15 meanwhile). One thread per row (64 keys) took 1.55 us per tile
+//   softmax X (4 warps)     thread = row = TMEM lane: masks, running maximum and sum, P as f16 over the tile's S buffer; O_X is
+//                           rescaled in TMEM only when a row's maximum grew by more than 2^5 (P stays below 2^15 meanwhile)
 //   O issuer X (1 thread)   O_X += P_X V (P from TMEM as the A operand, V as the MN-major B operand)
 // The key tiles of all items lie in one line, of which every CTA takes an equal stretch; an item that lies in several CTAs is joined by the
 // one that comes last, in the order of its keys (as in bp_kv4_attention.cu). Every wait is bounded; a timeout sets the context's error word and
 // the CTA winds down and frees its TMEM.
+//
+// Bound by the expanders: of the some 2500 cycles of a tile of 64 keys and 256 rows the S issuers wait most for K (the MMAs alone would take about
+// 1450 at the measured rate of a library product). 2048 queries behind 32768 keys, 32 / 8 heads of 128: 1.22 ms, 872 TFLOP/s, 53 % of that rate
+// (floor 0.65 ms). Four expander warps whose page ids were waited for took 1.39 ms; eight of them, with two softmax threads per row, 1.38; with one softmax
+// thread per row 1.25; with whole lines read and one barrier per slot 1.23. 4 requests of up to 512 queries behind up to 4099 keys: 96 us (floor 32): a tile costs the
+// same, beginning and ending an item about 14 us; before the line weighted items and the partial results had whole-warp accesses it was 216.
 #include <type_traits>
 
 #include "bp_kv4_attention.cuh"
@@ -35,8 +40,7 @@ struct Shape {
   static constexpr uint32_t OFF_K = NQ * Q_B, OFF_V = OFF_K + SLOTS * KV_B, SMEM = OFF_V + SLOTS * KV_B + 1024;
   static constexpr uint32_t TM_O = 128 * NQ, TMEM_COLS = 256 * NQ;        // S_X at 128 X, O_X at TM_O + 128 X
   static constexpr uint32_t FIRST_EXPANDER = 4, FIRST_SOFTMAX = 12;       // warps 0, 1: O issuers, 2, 3: S issuers
-  static constexpr uint32_t H = 1, C = BN / H;                            // softmax threads per row, keys of each
-  static constexpr uint32_t NWARP = FIRST_SOFTMAX + 4 * H * NQ, THREADS = 32 * NWARP;
+  static constexpr uint32_t NWARP = FIRST_SOFTMAX + 4 * NQ, THREADS = 32 * NWARP;
   static constexpr uint32_t PARTIAL = ROWS * (D + 2);                     // floats of a partial result: o as fours [dims / 4][row], (m, l) [row]
 };
 
@@ -172,7 +176,6 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t k_full[SLOTS], v_full[SLOTS], k_empty[SLOTS], v_empty[SLOTS], pv_done[NQ][SLOTS];
   __shared__ __align__(8) uint64_t s_ready[NQ][2], p_ready[NQ][2], p_free[NQ][2], o_done[NQ], drained;
-  __shared__ float shared_max[NQ][2][S::H][BM];  // [query tile][tile & 1][half][row]
   __shared__ float row_scale[S::ROWS];  // of a row's queries: the power of two that they were divided by
   __shared__ uint32_t line[THREADS + 1];
   __shared__ Cursor cur;
@@ -194,7 +197,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     for (uint32_t x = 0; x < NQ; x++) {
       for (uint32_t b = 0; b < 2; b++) {
         mbar_init(smem_u32(&s_ready[x][b]), 1);
-        mbar_init(smem_u32(&p_ready[x][b]), 4 * S::H);
+        mbar_init(smem_u32(&p_ready[x][b]), 4);
         mbar_init(smem_u32(&p_free[x][b]), 1);
       }
       mbar_init(smem_u32(&o_done[x]), 1);
@@ -403,10 +406,9 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       }
     } else {
       // ---------------- softmax X ----------------
-      // (after a wait that gave up the warps go on to the end without waiting: they meet at named barriers)
-      constexpr uint32_t H = S::H, C = S::C;
-      const uint32_t x = (warp - S::FIRST_SOFTMAX) / (4 * H), half = warp / 4 % H, quad = warp & 3, r = quad * 32 + lane;
-      const uint32_t lane_addr = (quad * 32) << 16, s_addr = tmem + lane_addr + x * 128, o_addr = tmem + lane_addr + S::TM_O + x * 128 + half * (D / H);
+      // (after a wait that gave up the warps go on to the end without waiting: they meet at a named barrier)
+      const uint32_t x = (warp - S::FIRST_SOFTMAX) >> 2, quad = warp & 3, r = quad * 32 + lane;
+      const uint32_t lane_addr = (quad * 32) << 16, s_addr = tmem + lane_addr + x * 128, o_addr = tmem + lane_addr + S::TM_O + x * 128;
       const uint32_t tile_row = row0 + x * BM, row = tile_row + r;
       const float scale = row_scale[x * BM + r];
       // this row sees the keys [lo, hi); the tile's first row sees none from hi0 on, its last row none before lo1
@@ -420,34 +422,26 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         (void)waitx(&s_ready[x][b], (c >> 1) & 1);
         __syncwarp();
         tc_fence_after();
-        if (half == 0 && quad == 0 && lane == 0) mbar_arrive(smem_u32(&k_empty[s]));  // Q K^T of the tile is complete
-        uint32_t raw[C];
+        if (quad == 0 && lane == 0) mbar_arrive(smem_u32(&k_empty[s]));  // Q K^T of the tile is complete
+        uint32_t raw[BN];
 #pragma unroll
-        for (uint32_t k = 0; k < C; k += 32) tmem_ld32(s_addr + 64 * b + C * half + k, raw + k);
+        for (uint32_t k = 0; k < BN; k += 32) tmem_ld32(s_addr + 64 * b + k, raw + k);
         tmem_ld_wait();
         const int key0 = key_first + static_cast<int>(i * BN);
         if (key0 + static_cast<int>(BN) > hi0 || key0 < lo1) {
-          const int from = lo - key0 - static_cast<int>(C * half), to = hi - key0 - static_cast<int>(C * half);
+          const int from = lo - key0, to = hi - key0;
 #pragma unroll
-          for (int k = 0; k < static_cast<int>(C); k++)
+          for (int k = 0; k < static_cast<int>(BN); k++)
             if (k >= to || k < from) raw[k] = 0xff800000u;
         }
         float mx[4] = {__uint_as_float(raw[0]), __uint_as_float(raw[1]), __uint_as_float(raw[2]), __uint_as_float(raw[3])};
 #pragma unroll
-        for (uint32_t k = 4; k < C - 4; k += 8)
+        for (uint32_t k = 4; k < BN - 4; k += 8)
 #pragma unroll
           for (uint32_t e = 0; e < 4; e++) mx[e] = max3(mx[e], __uint_as_float(raw[k + e]), __uint_as_float(raw[k + 4 + e]));
 #pragma unroll
-        for (uint32_t e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], __uint_as_float(raw[C - 4 + e]));
-        float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        if constexpr (H == 2) {
-          shared_max[x][i & 1][half][r] = m_tile;
-          tc_fence_before();
-          named_bar_sync(1 + x, 256);  // (both halves have read their S, too: P goes over it)
-          tc_fence_after();
-          m_tile = fmaxf(m_tile, shared_max[x][i & 1][half ^ 1][r]);
-        }
-        m_tile *= scale;
+        for (uint32_t e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], __uint_as_float(raw[BN - 4 + e]));
+        const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
         const bool grow = m_tile > m_run + GROW;
         const float m_new = grow ? m_tile : m_run, corr = grow ? ex2(m_run - m_new) : 1.f;
         m_run = m_new;
@@ -457,7 +451,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
           __syncwarp();
           tc_fence_after();
 #pragma unroll 1
-          for (uint32_t k = 0; k < D / (16 * H); k++) {
+          for (uint32_t k = 0; k < D / 16; k++) {
             uint32_t o[16];
             tmem_ld16(o_addr + 16 * k, o);
             tmem_ld_wait();
@@ -469,7 +463,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
         const float off = P_UP - m_new;
 #pragma unroll
-        for (uint32_t k0 = 0; k0 < C; k0 += 32) {
+        for (uint32_t k0 = 0; k0 < BN; k0 += 32) {
           uint32_t ph[16];
 #pragma unroll
           for (uint32_t k = 0; k < 16; k++) {
@@ -479,7 +473,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
             add2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], p0, p1);
             ph[k] = pack2<false>(p0, p1);
           }
-          tmem_st16(s_addr + 64 * b + (C * half + k0) / 2, ph);  // (every S value of this row is in registers)
+          tmem_st16(s_addr + 64 * b + k0 / 2, ph);  // (every S value of this row is in registers)
         }
         l_run = l_run * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
         tmem_st_wait();
@@ -487,12 +481,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&p_ready[x][b]));
       }
-      if constexpr (H == 2) shared_max[x][n & 1][half][r] = l_run;
       (void)waitx(&o_done[x], pieces & 1);
-      if constexpr (H == 2) {  // the row's sum over both halves
-        named_bar_sync(1 + x, 256);
-        l_run += shared_max[x][n & 1][half ^ 1][r];
-      }
       __syncwarp();
       tc_fence_after();
       if (first == 0 && n == keys.tiles) {
@@ -500,7 +489,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
         uint8_t* stage = smem + x * S::Q_B;
 #pragma unroll 1
-        for (uint32_t k = 0; k < D / (16 * H); k++) {
+        for (uint32_t k = 0; k < D / 16; k++) {
           uint32_t o[16];
           tmem_ld16(o_addr + 16 * k, o);
           tmem_ld_wait();
@@ -509,19 +498,19 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = __uint_as_float(o[8 * e + column_of(j)]) * inv;
-            const uint32_t u = half * (D / (8 * H)) + 2 * k + e;
+            const uint32_t u = 2 * k + e;
             *reinterpret_cast<uint4*>(stage + r * (D * 2) + ((u ^ (r & (D / 8 - 1))) << 4)) = a.bf ? pack8<true>(v) : pack8<false>(v);
           }
         }
-        named_bar_sync(1 + x, 128 * H);
-        if (tile_row < q.rows && !abort_s) store_rows<D>(a, q.q0, head, tile_row, min(BM, q.rows - tile_row), stage, (half * 4 + quad) * 32 + lane, 128 * H);
+        named_bar_sync(1 + x, 128);
+        if (tile_row < q.rows && !abort_s) store_rows<D>(a, q.q0, head, tile_row, min(BM, q.rows - tile_row), stage, r, 128);
       } else {
         // ---- a part of an item: as it is, to be joined ----
         const uint32_t first_cta = start / share;
         float* mine = scratch + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PARTIAL;
-        float4* to = reinterpret_cast<float4*>(mine) + half * (D / (4 * H)) * S::ROWS + x * BM + r;
+        float4* to = reinterpret_cast<float4*>(mine) + x * BM + r;
 #pragma unroll 1
-        for (uint32_t k = 0; k < D / (16 * H); k++) {
+        for (uint32_t k = 0; k < D / 16; k++) {
           uint32_t o[16];
           tmem_ld16(o_addr + 16 * k, o);
           tmem_ld_wait();
@@ -533,7 +522,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
             to[(4 * k + e) * S::ROWS] = make_float4(v[0], v[1], v[2], v[3]);  // (a warp's 32 rows are 512 bytes)
           }
         }
-        if (half == 0) reinterpret_cast<float2*>(mine + D * S::ROWS)[x * BM + r] = make_float2(m_run, l_run);
+        reinterpret_cast<float2*>(mine + D * S::ROWS)[x * BM + r] = make_float2(m_run, l_run);
       }
     }
     done += n;

@@ -2,6 +2,8 @@
 //
 // y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin for every pair of dims that turn together; the inverse turns by -angle, which
 // is the transpose and so the gradient. Bound by HBM: 2 bytes in and 2 out per value, 4 rot bytes of table per token.
+// Measured: 16383 tokens x 24 heads x 64, 18.8 us = 5.6 TB/s, 85 % of the measured copy (102.6 us with a warp per row and two bytes per lane, which
+// rows of other shapes still get); 2048 x 32 x 128, 7.8 us = 4.4 TB/s (22.3 us). One token: 6.3 us from call to call, which is its issue from Python.
 #include "bp_paged.cuh"
 
 namespace {
@@ -44,7 +46,7 @@ struct RopeArgs {
   float eps, sign;  // sign: -1 turns back
 };
 
-// Rows of 16-byte aligned chunks of eight dims, of which no pair's two dims share a chunk with another layout's: a thread has one
+// Rows of 16-byte aligned chunks of eight dims, head_dim and rot_dim multiples of 16: a thread has one
 // slot of 16 dims (chunks c and c + rot / 16 of the half layout, neighbours of the interleaved one, what is only copied behind) of R heads of
 // a token, so that the table's row is read once for them and R rows are on their way at a time.
 // G: lanes per row, the slots rounded up to a power of two, for the norm's sum.
@@ -220,7 +222,7 @@ cudaError_t bp_launch_rope(bp_paged_ctx* c, cudaStream_t s, bool bf, const Rows&
   if (head_dim % 16 == 0 && rope.rot % 16 == 0 && chunked(x) && chunked(out) && reinterpret_cast<uintptr_t>(rope.table) % 16 == 0) {
     uint32_t log_g = 0;
     while (1u << log_g < head_dim / 16) log_g++;
-    // heads of a thread: several where there are rows enough to fill the device with one wave of such threads
+    // heads of a thread: four where that still leaves every SM 2048 threads (the table's row is then read once for them), else one
     auto go = [&](auto kernel, uint32_t r) {
       const uint32_t groups = (n_head + r - 1) / r;
       const uint64_t blocks = ((static_cast<uint64_t>(n_tok) * groups << log_g) + 255) / 256;
