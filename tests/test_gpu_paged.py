@@ -343,6 +343,17 @@ def test_many_requests(ctx):
     r.check(r.run(ctx))
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q", [1, 6])
+def test_more_requests_than_threads(ctx, dim, q):
+    """A thread then counts the work of several requests; some have no queries, some no keys."""
+    rng = np.random.default_rng(dim + q)
+    kv = [int(x) for x in rng.integers(0, 90, 1100)]
+    r = Requests(12, "f16", [int(x) for x in rng.integers(0, q + 1, 1100)], kv, 4, 1, dim, 16)
+    r.check(r.run(ctx))
+    ctx.status()
+
+
 def test_pages_behind_four_gigabytes(ctx):
     heads, hkv, dim, page = 4, 2, 128, 64
     record = hkv * page * dim * 5 // 4
