@@ -806,6 +806,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
         }
         fresh = true;
         if (i + 1 < n) {
+          __syncwarp();  // (every lane has read the item that ends)
           if (lane == 0) next_item<NT>(cur, a, known);
           __syncwarp();
         }

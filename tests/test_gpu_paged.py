@@ -326,6 +326,14 @@ def test_small_and_large_queries(ctx, dtype, gain, q):
         r.check(out, scale=scale)
 
 
+@pytest.mark.parametrize("q", [1, 130])
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+@pytest.mark.parametrize("window", [0, 50])
+def test_scales_that_turn_or_level_the_scores(ctx, q, scale, window):
+    r = Requests(13, "bf16", [q, q], [300, 140], 8, 2, 64, 16)
+    r.check(r.run(ctx, scale=scale, window=window), scale=scale, window=window)
+
+
 @pytest.mark.parametrize("heads,hkv,dim,kv", [(32, 8, 128, 9000), (4, 1, 128, 20011), (8, 8, 64, 5000)])
 def test_long_contexts_are_split(ctx, heads, hkv, dim, kv):
     r = Requests(6, "f16", [1, 1, 2], [kv, 10, 3000], heads, hkv, dim, 64)
