@@ -191,6 +191,28 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
         y[0][i] = turn(x[0][i], x[1][i], t.x, -t.y);
         y[1][i] = turn(x[1][i], x[0][i], t.x, t.y);
       }
+    } else if (half % 8 == 0) {  // part of a head, whole chunks of eight: the chunk that this one turns with is read again
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const uint32_t dim = h * (D / 2) + 8 * c;
+        if (dim >= 2 * half) continue;
+        const bool first = dim < half;
+        const uint32_t other = first ? dim + half : dim - half, pair = first ? dim : other;
+        float z[8];
+        unpack8<BF>(load_raw<VEC>(k + other), z);
+        if (a.w) {
+          float w[8];
+          if (reinterpret_cast<uintptr_t>(a.w) % 16 == 0) load8<BF, true>(a.w + other, w);
+          else load8<BF, false>(a.w + other, w);
+#pragma unroll
+          for (int i = 0; i < 8; i++) z[i] = __fmul_rn(__fmul_rn(z[i], scale), w[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float2 t = cs[pair + i];
+          y[h][i] = turn(x[h][i], z[i], t.x, first ? -t.y : t.y);
+        }
+      }
     } else {  // part of a head: the other dim of a pair is read again
 #pragma unroll
       for (int h = 0; h < 2; h++) {

@@ -92,18 +92,6 @@ __device__ __forceinline__ void load8(const uint16_t* p, float* x) {
     for (int i = 0; i < 8; i++) x[i] = to_f32<BF>(p[i]);
   }
 }
-template <bool BF, bool VEC>
-__device__ __forceinline__ void store8(uint16_t* p, const float* x) {
-  const uint4 u = pack8<BF>(x);
-  if (VEC) {
-    *reinterpret_cast<uint4*>(p) = u;
-  } else {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 8; i++) p[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
-  }
-}
-
 // Division of numbers below 2^31 by one divisor: with l = ceil(log2 d) and m = floor(2^32 (2^l - d) / d) + 1 the quotient is
 // (mulhi(m, n) + n) >> l (Granlund and Montgomery, 1994).
 struct FastDiv {
