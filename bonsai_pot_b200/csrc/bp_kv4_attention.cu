@@ -715,7 +715,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
     bool fresh = true, from_start = false, ok = true;
     uint32_t first = 0;          // of this piece; cur.unit is its place in the item
     uint32_t b = 0, phase = 0;   // the buffer that is worked on, the phases of the barriers' next use
-    auto wait = [&]() { return wait_phase(bar + 8 * b, phase >> b & 1); };
+    // (the lanes decide together: what follows shuffles and multiplies with the whole warp, and one lane may see the phase that another one gave up on)
+    auto wait = [&]() { return __all_sync(FULL, wait_phase(bar + 8 * b, phase >> b & 1)); };
     auto done = [&]() {
       phase ^= 1u << b;
       if (++b == RING) b = 0;
