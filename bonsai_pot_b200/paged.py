@@ -41,8 +41,15 @@ def _dtype(t):
 
 
 # The checks below are on the path of every call (a decoded token makes three of them per layer), hence as few tensor methods as will do.
-def _rows(to, t, what):
+def _elsewhere(t, what, device):
+    """An address of host memory or of another device must not reach a kernel."""
+    _bad(f"{what} must be on cuda:{device}, not on {t.device}")
+
+
+def _rows(to, t, what, device):
     """t's address and strides into a RowsStruct."""
+    if t.get_device() != device:
+        _elsewhere(t, what, device)
     strides = t.stride()
     if len(strides) != 3:
         _bad(f"{what} must be [tokens, heads, head_dim], not {tuple(t.shape)}")
@@ -57,13 +64,17 @@ def _like(t, rows, what):
         _bad(f"{what} must have the shape and type of the rows it goes with: {tuple(t.shape)} {t.dtype}, not {tuple(rows.shape)} {rows.dtype}")
 
 
-def _index(t, what, n, slots=False):
+def _index(t, what, n, device, slots=False):
+    if t.get_device() != device:
+        _elsewhere(t, what, device)
     if t.dtype is not (_I64 if slots else _I32) or t.shape != (n,) or not t.is_contiguous():
         _bad(f"{what} must be {n} dense values of {_I64 if slots else _I32}, not {tuple(t.shape)} {t.dtype}")
     return t.data_ptr()
 
 
-def _weight(w, rows, what):
+def _weight(w, rows, what, device):
+    if w.get_device() != device:
+        _elsewhere(w, what, device)
     if w.dtype is not rows.dtype or w.numel() != rows.shape[2] or not w.is_contiguous():
         _bad(f"{what} must be {rows.shape[2]} dense values of the rows' type")
     return w.data_ptr()
@@ -77,7 +88,9 @@ class RopeTable:
             raise ConfigError(f"invalid config: layout must be one of {sorted(_LAYOUTS)}, not {layout!r}")
         if str(data.dtype) != "torch.float32" or data.dim() != 3 or data.shape[2] != 2 or not data.is_contiguous():
             raise ConfigError("invalid config: a RoPE table is a dense float32 tensor [positions, rot_dim / 2, 2]")
-        self.data = data
+        if not data.is_cuda:
+            _bad(f"a RoPE table must be on a CUDA device, not on {data.device}")
+        self.data, self.device = data, data.get_device()
         self._c = _lib.RopeTableStruct(data.data_ptr(), data.shape[0], 2 * data.shape[1], _LAYOUTS[layout])
         self._p = C.addressof(self._c)
 
@@ -89,7 +102,10 @@ class KV4Pool:
         need = KV4Pool.bytes(n_pages, page_tokens, n_kv_head, head_dim)
         if str(data.dtype) != "torch.uint8" or not data.is_contiguous() or data.numel() < need:
             raise ConfigError(f"invalid config: a pool of this shape is a dense uint8 tensor of at least {need} bytes")
-        self.data, self.page_tokens, self.n_kv_head, self.head_dim = data, page_tokens, n_kv_head, head_dim
+        if not data.is_cuda:
+            _bad(f"a pool must be on a CUDA device, not on {data.device}")
+        self.data, self.device = data, data.get_device()
+        self.page_tokens, self.n_kv_head, self.head_dim = page_tokens, n_kv_head, head_dim
         self._c = _lib.PoolStruct(data.data_ptr(), n_pages, page_tokens, n_kv_head, head_dim)
         self._p = C.addressof(self._c)
 
@@ -102,11 +118,12 @@ class KV4Pool:
 
 
 class PagedContext:
-    """Scratch memory and errors of the paged operators on one device."""
+    """Scratch memory and errors of the paged operators on one device, on which every tensor of a call must lie."""
 
     def __init__(self, device=0):
         self._lib = _lib.load()
         self._h = C.c_void_p()
+        self._device = device
         self._setup()
         st = self._lib.bp_paged_create(device, C.byref(self._h))
         if st != 0:
@@ -152,45 +169,54 @@ class PagedContext:
         """Fills a float32 tensor [positions, rot_dim / 2, 2]; scaling: None, "linear", "ntk" or "yarn"."""
         if scaling not in _SCALINGS:
             raise ConfigError(f"invalid config: scaling must be one of None, 'linear', 'ntk', 'yarn', not {scaling!r}")
-        RopeTable(out)
+        if RopeTable(out).device != self._device:
+            _elsewhere(out, "a RoPE table", self._device)
         cfg = _lib.RopeConfigStruct(out.shape[0], 2 * out.shape[1], _SCALINGS[scaling], freq_base, factor, beta_fast, beta_slow, orig_ctx)
         self._check(self._lib.bp_rope_fill(self._h, _stream(stream), C.byref(cfg), out.data_ptr()))
 
     def rope(self, x, out, positions, table, w_norm=None, eps=1e-6, inverse=False, stream=None):
         """x [tokens, heads, head_dim] -> out (may be x): RMS norm over the head if w_norm is given, then the rotation by `positions`."""
-        dtype = _dtype(x)
-        _rows(self._a, x, "x")
+        dtype, device = _dtype(x), self._device
+        _rows(self._a, x, "x", device)
         _like(out, x, "out")
-        _rows(self._b, out, "out")
+        _rows(self._b, out, "out", device)
+        if table.device != device:
+            _elsewhere(table.data, "the RoPE table", device)
         n, heads, dim = x.shape
-        st = self._lib.bp_rope(self._h, stream if stream is None else _stream(stream), dtype, self._pa, self._pb, n, heads, dim, _index(positions, "positions", n), table._p,
-                               None if w_norm is None else _weight(w_norm, x, "w_norm"), eps, inverse)
+        st = self._lib.bp_rope(self._h, stream if stream is None else _stream(stream), dtype, self._pa, self._pb, n, heads, dim, _index(positions, "positions", n, device), table._p,
+                               None if w_norm is None else _weight(w_norm, x, "w_norm", device), eps, inverse)
         if st:
             self._check(st)
 
     def append(self, pool, k, v, positions, slots, table=None, w_k_norm=None, eps=1e-6, stream=None):
         """k, v [tokens, KV heads, head_dim] -> the pool at `slots`; K is normalised (w_k_norm) and rotated (table) on the way."""
-        dtype, n = self._kv(pool, k, v)
+        dtype, n, device = self._kv(pool, k, v)
+        if table is not None and table.device != device:
+            _elsewhere(table.data, "the RoPE table", device)
         st = self._lib.bp_kv4_append(self._h, stream if stream is None else _stream(stream), dtype, pool._p, self._pa, self._pb, n,
-                                     None if positions is None else _index(positions, "positions", n), _index(slots, "slots", n, True),
-                                     None if table is None else table._p, None if w_k_norm is None else _weight(w_k_norm, k, "w_k_norm"), eps)
+                                     None if positions is None else _index(positions, "positions", n, device), _index(slots, "slots", n, device, True),
+                                     None if table is None else table._p, None if w_k_norm is None else _weight(w_k_norm, k, "w_k_norm", device), eps)
         if st:
             self._check(st)
 
     def read(self, pool, slots, k, v, stream=None):
         """The pool's rows at `slots` -> k, v [tokens, KV heads, head_dim]; keys are as they were stored."""
-        dtype, n = self._kv(pool, k, v)
-        st = self._lib.bp_kv4_read(self._h, stream if stream is None else _stream(stream), dtype, pool._p, _index(slots, "slots", n, True), n, self._pa, self._pb)
+        dtype, n, device = self._kv(pool, k, v)
+        st = self._lib.bp_kv4_read(self._h, stream if stream is None else _stream(stream), dtype, pool._p, _index(slots, "slots", n, device, True), n, self._pa, self._pb)
         if st:
             self._check(st)
 
     def attention(self, pool, q, out, q_start, kv_len, page_table, max_q, max_kv, scale=None, window=0, stream=None):
         """q [tokens of all requests, heads, head_dim] -> out. Request r has the rows q_start[r] .. q_start[r + 1] and sees kv_len[r] keys in
         the pages page_table[r]; max_q, max_kv: no request has more. scale: 1 / sqrt(head_dim) if None; window: 0 = none."""
-        dtype, a = _dtype(q), self._attn
-        _rows(self._q, q, "q")
+        dtype, a, device = _dtype(q), self._attn, self._device
+        _rows(self._q, q, "q", device)
         _like(out, q, "out")
-        _rows(self._o, out, "out")
+        _rows(self._o, out, "out", device)
+        if pool.device != device:
+            _elsewhere(pool.data, "the pool", device)
+        if page_table.get_device() != device:
+            _elsewhere(page_table, "page_table", device)
         n, heads, dim = q.shape
         if dim != pool.head_dim:
             _bad(f"q has head_dim {dim}, the pool {pool.head_dim}")
@@ -203,7 +229,7 @@ class PagedContext:
             _bad("max_q, max_kv and window must be >= 0")
         # (what a row of the table holds bounds the keys that are looked at, not the distance of two rows)
         cap = pages * pool.page_tokens
-        a.q_start, a.kv_len, a.page_table = _index(q_start, "q_start", n_req + 1), _index(kv_len, "kv_len", n_req), page_table.data_ptr()
+        a.q_start, a.kv_len, a.page_table = _index(q_start, "q_start", n_req + 1, device), _index(kv_len, "kv_len", n_req, device), page_table.data_ptr()
         a.n_req, a.n_head, a.total_q, a.max_q, a.max_kv, a.window = n_req, heads, n, max_q, max_kv if max_kv < cap else cap, window
         a.table_stride = stride if n_req > 1 else pages
         a.scale = dim ** -0.5 if scale is None else scale
@@ -212,11 +238,13 @@ class PagedContext:
             self._check(st)
 
     def _kv(self, pool, k, v):
-        dtype = _dtype(k)
-        _rows(self._a, k, "k")
+        dtype, device = _dtype(k), self._device
+        _rows(self._a, k, "k", device)
         _like(v, k, "v")
-        _rows(self._b, v, "v")
+        _rows(self._b, v, "v", device)
+        if pool.device != device:
+            _elsewhere(pool.data, "the pool", device)
         n, heads, dim = k.shape
         if heads != pool.n_kv_head or dim != pool.head_dim:
             _bad(f"the pool holds {pool.n_kv_head} heads of {pool.head_dim}, the rows have {heads} of {dim}")
-        return dtype, n
+        return dtype, n, device

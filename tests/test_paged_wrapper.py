@@ -1,0 +1,100 @@
+"""What PagedContext refuses, and what it hands to the C entry, without a GPU: the library is a stand-in that records its calls."""
+import ctypes as C
+
+import pytest
+
+import bonsai_pot_b200 as bp
+from bonsai_pot_b200 import paged
+
+torch = pytest.importorskip("torch")
+
+
+class Recorder:
+    """Every entry of the library: notes its arguments and says that all went well."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def entry(*args):
+            self.calls.append((name, args))
+            return 0
+        return entry
+
+
+class Owner:
+    """A table or pool as the context sees it."""
+    _p, n_kv_head, head_dim, page_tokens = 0, 2, 64, 16
+
+    def __init__(self, device=0):
+        self.device = device
+
+
+@pytest.fixture
+def ctx():
+    c = paged.PagedContext.__new__(paged.PagedContext)
+    c._lib, c._h, c._device = Recorder(), C.c_void_p(), 0
+    c._setup()
+    return c
+
+
+@pytest.mark.parametrize("name", ["rope", "append", "read", "attention"])
+def test_host_tensors_do_not_reach_a_kernel(ctx, name):
+    x, i32, slots = torch.zeros(3, 2, 64, dtype=torch.float16), torch.zeros(3, dtype=torch.int32), torch.arange(3)
+    owner = Owner()
+    call = {
+        "rope": lambda: ctx.rope(x, x, i32, owner),
+        "append": lambda: ctx.append(owner, x, x, i32, slots, owner),
+        "read": lambda: ctx.read(owner, slots, x, x),
+        "attention": lambda: ctx.attention(owner, x, x, i32[:2], i32[:1], i32[:2].view(1, 2), max_q=3, max_kv=3),
+    }[name]
+    with pytest.raises(bp.ConfigError, match="^invalid config: .* must be on cuda:0, not on cpu"):
+        call()
+    assert ctx._lib.calls == []
+
+
+def test_tables_and_pools_are_device_memory(ctx):
+    with pytest.raises(bp.ConfigError, match="^invalid config: "):
+        bp.RopeTable(torch.zeros(4, 32, 2))
+    with pytest.raises(bp.ConfigError, match="^invalid config: "):
+        bp.KV4Pool(torch.zeros(bp.KV4Pool.bytes(1, 16, 2, 64), dtype=torch.uint8), 1, 16, 2, 64)
+    with pytest.raises(bp.ConfigError, match="^invalid config: "):
+        ctx.fill_rope(torch.zeros(4, 32, 2))
+    assert ctx._lib.calls == []
+
+
+@pytest.mark.gpu
+def test_every_tensor_of_a_call_is_looked_at():
+    """One tensor at a time is on the host; nothing is launched."""
+    cuda = {"x": torch.zeros(3, 2, 64, dtype=torch.float16), "out": torch.zeros(3, 2, 64, dtype=torch.float16), "pos": torch.zeros(3, dtype=torch.int32),
+            "slots": torch.arange(3), "w": torch.ones(64, dtype=torch.float16), "table": torch.zeros(1, 2, dtype=torch.int32),
+            "start": torch.tensor([0, 3], dtype=torch.int32), "kv": torch.tensor([3], dtype=torch.int32)}
+    cuda = {k: v.cuda() for k, v in cuda.items()}
+    tab = bp.RopeTable(torch.zeros(4, 32, 2, device="cuda"))
+    pool = bp.KV4Pool(torch.zeros(bp.KV4Pool.bytes(1, 16, 2, 64), dtype=torch.uint8, device="cuda"), 1, 16, 2, 64)
+    c = bp.PagedContext()
+    calls = {
+        ("x", "out", "pos", "w"): lambda t: c.rope(t["x"], t["out"], t["pos"], tab, w_norm=t["w"]),
+        ("x", "out", "pos", "slots", "w"): lambda t: c.append(pool, t["x"], t["out"], t["pos"], t["slots"], tab, w_k_norm=t["w"]),
+        ("x", "out", "slots"): lambda t: c.read(pool, t["slots"], t["x"], t["out"]),
+        ("x", "out", "start", "kv", "table"): lambda t: c.attention(pool, t["x"], t["out"], t["start"], t["kv"], t["table"], max_q=3, max_kv=3),
+    }
+    real, c._lib = c._lib, Recorder()
+    for names, call in calls.items():
+        for name in names:
+            with pytest.raises(bp.ConfigError, match="must be on cuda:0, not on cpu"):
+                call({**cuda, name: cuda[name].cpu()})
+        assert c._lib.calls == []
+        call(cuda)
+        assert len(c._lib.calls) == 1
+        c._lib.calls.clear()
+    other = bp.PagedContext.__new__(bp.PagedContext)  # a context of the next device: tables and pools of this one are refused too
+    other._lib, other._h, other._device = Recorder(), C.c_void_p(), 1
+    other._setup()
+    with pytest.raises(bp.ConfigError, match="must be on cuda:1, not on cuda:0"):
+        other.fill_rope(tab.data)
+    with pytest.raises(bp.ConfigError, match="must be on cuda:1, not on cuda:0"):
+        other.rope(cuda["x"], cuda["out"], cuda["pos"], tab)
+    assert other._lib.calls == []
+    c._lib = real
+    c.close()
