@@ -3,7 +3,8 @@
 `PagedContext` owns scratch memory only; cache, RoPE table and activations are the caller's CUDA tensors. Every method calls
 straight into the C ABI of include/bonsai_paged.h, which says what each operator computes and how a pool's bytes are laid
 out. Rows are tensors [tokens, heads, head_dim] of float16 or bfloat16 with any strides between tokens and heads; index
-tensors are int32, slots int64.
+tensors are int32, slots int64. A call without a `stream` goes to torch's current stream of the context's device (the C entries' null
+stream is CUDA's legacy default stream, for which torch's other streams do not wait).
 """
 from __future__ import annotations
 
@@ -24,6 +25,14 @@ def _types():
     import torch
     _DTYPES.update({torch.float16: 0, torch.bfloat16: 1})
     _I32, _I64 = torch.int32, torch.int64
+
+
+def _current(device):
+    """The handle of torch's current stream; the first call puts torch's own function here."""
+    global _current
+    import torch
+    _current = torch._C._cuda_getCurrentRawStream
+    return _current(device)
 
 
 def _bad(text):
@@ -163,7 +172,7 @@ class PagedContext:
 
     def status(self, stream=None):
         """Waits for `stream`; raises if a position, slot, page id or number of keys was out of range since the last call."""
-        self._check(self._lib.bp_paged_status(self._h, _stream(stream)))
+        self._check(self._lib.bp_paged_status(self._h, _current(self._device) if stream is None else _stream(stream)))
 
     def fill_rope(self, out, freq_base=1e6, scaling=None, factor=1.0, beta_fast=32.0, beta_slow=1.0, orig_ctx=0, stream=None):
         """Fills a float32 tensor [positions, rot_dim / 2, 2]; scaling: None, "linear", "ntk" or "yarn"."""
@@ -172,7 +181,7 @@ class PagedContext:
         if RopeTable(out).device != self._device:
             _elsewhere(out, "a RoPE table", self._device)
         cfg = _lib.RopeConfigStruct(out.shape[0], 2 * out.shape[1], _SCALINGS[scaling], freq_base, factor, beta_fast, beta_slow, orig_ctx)
-        self._check(self._lib.bp_rope_fill(self._h, _stream(stream), C.byref(cfg), out.data_ptr()))
+        self._check(self._lib.bp_rope_fill(self._h, _current(self._device) if stream is None else _stream(stream), C.byref(cfg), out.data_ptr()))
 
     def rope(self, x, out, positions, table, w_norm=None, eps=1e-6, inverse=False, stream=None):
         """x [tokens, heads, head_dim] -> out (may be x): RMS norm over the head if w_norm is given, then the rotation by `positions`."""
@@ -183,7 +192,7 @@ class PagedContext:
         if table.device != device:
             _elsewhere(table.data, "the RoPE table", device)
         n, heads, dim = x.shape
-        st = self._lib.bp_rope(self._h, stream if stream is None else _stream(stream), dtype, self._pa, self._pb, n, heads, dim, _index(positions, "positions", n, device), table._p,
+        st = self._lib.bp_rope(self._h, _current(device) if stream is None else _stream(stream), dtype, self._pa, self._pb, n, heads, dim, _index(positions, "positions", n, device), table._p,
                                None if w_norm is None else _weight(w_norm, x, "w_norm", device), eps, inverse)
         if st:
             self._check(st)
@@ -193,7 +202,7 @@ class PagedContext:
         dtype, n, device = self._kv(pool, k, v)
         if table is not None and table.device != device:
             _elsewhere(table.data, "the RoPE table", device)
-        st = self._lib.bp_kv4_append(self._h, stream if stream is None else _stream(stream), dtype, pool._p, self._pa, self._pb, n,
+        st = self._lib.bp_kv4_append(self._h, _current(device) if stream is None else _stream(stream), dtype, pool._p, self._pa, self._pb, n,
                                      None if positions is None else _index(positions, "positions", n, device), _index(slots, "slots", n, device, True),
                                      None if table is None else table._p, None if w_k_norm is None else _weight(w_k_norm, k, "w_k_norm", device), eps)
         if st:
@@ -202,7 +211,7 @@ class PagedContext:
     def read(self, pool, slots, k, v, stream=None):
         """The pool's rows at `slots` -> k, v [tokens, KV heads, head_dim]; keys are as they were stored."""
         dtype, n, device = self._kv(pool, k, v)
-        st = self._lib.bp_kv4_read(self._h, stream if stream is None else _stream(stream), dtype, pool._p, _index(slots, "slots", n, device, True), n, self._pa, self._pb)
+        st = self._lib.bp_kv4_read(self._h, _current(device) if stream is None else _stream(stream), dtype, pool._p, _index(slots, "slots", n, device, True), n, self._pa, self._pb)
         if st:
             self._check(st)
 
@@ -233,7 +242,7 @@ class PagedContext:
         a.n_req, a.n_head, a.total_q, a.max_q, a.max_kv, a.window = n_req, heads, n, max_q, max_kv if max_kv < cap else cap, window
         a.table_stride = stride if n_req > 1 else pages
         a.scale = dim ** -0.5 if scale is None else scale
-        st = self._lib.bp_kv4_attention(self._h, stream if stream is None else _stream(stream), dtype, pool._p, self._pattn)
+        st = self._lib.bp_kv4_attention(self._h, _current(device) if stream is None else _stream(stream), dtype, pool._p, self._pattn)
         if st:
             self._check(st)
 

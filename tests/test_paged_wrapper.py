@@ -98,3 +98,53 @@ def test_every_tensor_of_a_call_is_looked_at():
     assert other._lib.calls == []
     c._lib = real
     c.close()
+
+
+def test_without_a_stream_a_call_goes_to_the_current_one(ctx, monkeypatch):
+    ctx._device = -1  # where host tensors lie: nothing here is refused
+    x, i32, slots, owner = torch.zeros(3, 2, 64, dtype=torch.float16), torch.zeros(3, dtype=torch.int32), torch.arange(3), Owner(-1)
+    asked = []
+    monkeypatch.setattr(paged, "_current", lambda device: asked.append(device) or 4711, raising=False)
+    monkeypatch.setattr(bp.RopeTable, "__init__", lambda self, data, layout="half": setattr(self, "device", -1))
+    for stream, want in ((None, 4711), (99, 99), (0, 0)):
+        ctx.rope(x, x, i32, owner, stream=stream)
+        ctx.append(owner, x, x, i32, slots, owner, stream=stream)
+        ctx.read(owner, slots, x, x, stream=stream)
+        ctx.attention(owner, x, x, i32[:2], i32[:1], i32[:2].view(1, 2), max_q=3, max_kv=3, stream=stream)
+        ctx.fill_rope(torch.zeros(4, 32, 2), stream=stream)
+        ctx.status(stream=stream)
+        assert [args[1] for _, args in ctx._lib.calls] == [want] * 6
+        ctx._lib.calls.clear()
+    assert asked == [-1] * 6
+
+
+@pytest.mark.gpu
+def test_calls_follow_the_current_stream():
+    """On a stream of torch's own the rows are made late: a call that did not wait for them would take what was there before. And a call
+    without a stream is captured like any other."""
+    c = bp.PagedContext()
+    tab = torch.empty(64, 32, 2, device="cuda")
+    side = torch.cuda.Stream()
+    x, out, pos = torch.zeros(4, 2, 64, dtype=torch.float16, device="cuda"), torch.zeros(4, 2, 64, dtype=torch.float16, device="cuda"), torch.arange(4, dtype=torch.int32, device="cuda")
+    ones = torch.ones_like(x)
+    c.fill_rope(tab)
+    table = bp.RopeTable(tab)
+    want = torch.empty_like(x)
+    c.rope(ones, want, pos, table)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)  # some 25 ms
+        x.copy_(ones)
+        c.rope(x, out, pos, table)
+        c.status()  # waits for the same stream
+        assert side.query()
+    assert torch.equal(out, want)
+    out.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.rope(x, out, pos, table)
+    assert (out == 0).all()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    c.close()
