@@ -17,6 +17,7 @@ from .errors import ConfigError, raise_for_status
 _LAYOUTS = {"half": 0, "interleaved": 1}
 _SCALINGS = {None: 0, "linear": 1, "ntk": 2, "yarn": 3}
 _DTYPES, _I32, _I64 = {}, None, None
+_U32 = 0xFFFFFFFF
 
 
 def _types():
@@ -120,7 +121,7 @@ class KV4Pool:
 
     @staticmethod
     def bytes(n_pages, page_tokens, n_kv_head, head_dim):
-        n = _lib.load().bp_kv4_pool_bytes(C.byref(_lib.PoolStruct(None, n_pages, page_tokens, n_kv_head, head_dim))) if min(n_pages, page_tokens, n_kv_head, head_dim) > 0 else 0
+        n = _lib.load().bp_kv4_pool_bytes(C.byref(_lib.PoolStruct(None, n_pages, page_tokens, n_kv_head, head_dim))) if 0 < min(n_pages, page_tokens, n_kv_head, head_dim) and max(n_pages, page_tokens, n_kv_head, head_dim) <= _U32 else 0
         if n == 0:
             raise ConfigError("invalid config: a pool has n_pages >= 1, page_tokens 16, 32 or 64, n_kv_head >= 1 and head_dim 64 or 128")
         return n
@@ -238,9 +239,15 @@ class PagedContext:
             _bad("max_q, max_kv and window must be >= 0")
         # (what a row of the table holds bounds the keys that are looked at, not the distance of two rows)
         cap = pages * pool.page_tokens
+        if max_kv > cap:
+            max_kv = cap
+        pitch = stride if n_req > 1 else pages
+        if max_kv > _U32 or pitch > _U32:  # (the C entry's numbers have 32 bits: what is longer would arrive as another number)
+            _bad("max_kv and the distance of two rows of page_table must be below 2^32")
         a.q_start, a.kv_len, a.page_table = _index(q_start, "q_start", n_req + 1, device), _index(kv_len, "kv_len", n_req, device), page_table.data_ptr()
-        a.n_req, a.n_head, a.total_q, a.max_q, a.max_kv, a.window = n_req, heads, n, max_q, max_kv if max_kv < cap else cap, window
-        a.table_stride = stride if n_req > 1 else pages
+        a.n_req, a.n_head, a.total_q, a.max_q, a.max_kv = n_req, heads, n, max_q if max_q < n else n, max_kv
+        a.window = window if window < max_kv else 0  # (a window over all keys is none)
+        a.table_stride = pitch
         a.scale = dim ** -0.5 if scale is None else scale
         st = self._lib.bp_kv4_attention(self._h, _current(device) if stream is None else _stream(stream), dtype, pool._p, self._pattn)
         if st:

@@ -118,6 +118,32 @@ def test_without_a_stream_a_call_goes_to_the_current_one(ctx, monkeypatch):
     assert asked == [-1] * 6
 
 
+def test_sizes_beyond_32_bits_are_not_cut_to_other_ones(ctx, monkeypatch):
+    ctx._device = -1
+    monkeypatch.setattr(paged, "_current", lambda device: 0)
+    x, i32, owner = torch.zeros(3, 2, 64, dtype=torch.float16), torch.zeros(3, dtype=torch.int32), Owner(-1)
+    taken = []
+    monkeypatch.setattr(ctx, "_lib", type("L", (), {"bp_kv4_attention": lambda self, *a: taken.append((ctx._attn.max_q, ctx._attn.max_kv, ctx._attn.window)) and 0})())
+
+    def call(max_q=3, max_kv=3, window=0, page_table=i32[:2].view(1, 2)):
+        ctx.attention(owner, x, x, i32[:2], i32[:1], page_table, max_q=max_q, max_kv=max_kv, window=window)
+        return taken[-1]
+
+    assert call() == (3, 3, 0) and call(window=2) == (3, 3, 2)
+    assert call(max_q=1 << 32) == (3, 3, 0)  # no more queries than rows
+    assert call(max_kv=1 << 32) == (3, 32, 0)  # no more keys than the table's pages hold
+    assert call(window=(1 << 32) + 1) == (3, 3, 0) and call(window=3) == (3, 3, 0)  # a window over all keys is none
+    n = len(taken)
+    with pytest.raises(bp.ConfigError, match="^invalid config: "):
+        call(max_kv=1 << 40, page_table=torch.empty(1, 1 << 28, dtype=torch.int32))  # pages of 2^32 tokens (nobody touches them)
+    assert len(taken) == n
+    for bad in ((1 << 32) + 1, 1 << 40):
+        with pytest.raises(bp.ConfigError, match="^invalid config: "):
+            bp.KV4Pool.bytes(bad, 16, 1, 64)
+        with pytest.raises(bp.ConfigError, match="^invalid config: "):
+            bp.KV4Pool.bytes(1, 16, bad, 64)
+
+
 @pytest.mark.gpu
 def test_calls_follow_the_current_stream():
     """On a stream of torch's own the rows are made late: a call that did not wait for them would take what was there before. And a call
