@@ -352,7 +352,7 @@ __device__ __forceinline__ Request request(const AttnArgs& a, uint32_t r, bool r
   q.q0 = max(start, 0);
   const int given_q = max(min(stop, static_cast<int>(a.total_q)) - q.q0, 0), given_kv = max(keys, 0);
   q.q_len = min(given_q, static_cast<int>(a.max_q));
-  q.kv_len = min(given_kv, static_cast<int>(min(a.max_kv, a.table_stride << a.pool.log_page)));
+  q.kv_len = min(given_kv, static_cast<int>(min(a.max_kv, a.table_pages << a.pool.log_page)));
   if (report && (given_q > q.q_len || given_kv > q.kv_len)) note_range(a.err);
   const int from = a.window ? q.kv_len - q.q_len + 1 - static_cast<int>(min(a.window, 0x40000000u)) : 0;
   q.low = max(min(from, q.kv_len), 0);
@@ -930,7 +930,8 @@ cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, co
   a.total_q = in.total_q;
   a.max_q = in.max_q < in.total_q ? in.max_q : in.total_q;
   a.max_kv = in.max_kv;
-  a.table_stride = in.table_stride < (0x7fffffffu >> pool.log_page) ? in.table_stride : (0x7fffffffu >> pool.log_page);
+  a.table_stride = in.table_stride;
+  a.table_pages = in.table_stride < (0x7fffffffu >> pool.log_page) ? in.table_stride : (0x7fffffffu >> pool.log_page);
   a.window = in.window;
   a.scale_log2 = in.scale * 1.4426950408889634f;
   a.bias = 0x64006400u;

@@ -16,6 +16,7 @@ struct AttnArgs {
   const int32_t *q_start, *kv_len, *page_table;
   uint32_t* err;
   uint32_t n_req, n_head, group, total_q, max_q, max_kv, table_stride, window;
+  uint32_t table_pages;  // of a row of the page table that are looked at: what 31 bits of keys fill at most (rows may lie further apart)
   float scale_log2;
   uint32_t bias;  // 0x64006400: two f16 numbers 1024
   uint32_t bf;    // activations are bfloat16
