@@ -278,7 +278,7 @@ __device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4]
       for (int c = 0; c < 2; c++) {
         // the keys of the unit that row 2 t + c sees are [lo, hi); columns behind the request's rows are left as they are, nobody reads them
         const int behind = q_len - 1 - static_cast<int>((tile0 + 8 * e + 2 * (lane & 3) + c) / a.group);  // queries behind this one
-        const int hi = behind < 0 ? left : left - behind, lo = a.window && behind >= 0 ? hi - static_cast<int>(min(a.window, 0x40000000u)) : 0;
+        const int hi = behind < 0 ? left : left - behind, lo = a.window && behind >= 0 ? hi - static_cast<int>(a.window) : 0;
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -354,8 +354,7 @@ __device__ __forceinline__ Request request(const AttnArgs& a, uint32_t r, bool r
   q.q_len = min(given_q, static_cast<int>(a.max_q));
   q.kv_len = min(given_kv, static_cast<int>(min(a.max_kv, a.table_pages << a.pool.log_page)));
   if (report && (given_q > q.q_len || given_kv > q.kv_len)) note_range(a.err);
-  const int from = a.window ? q.kv_len - q.q_len + 1 - static_cast<int>(min(a.window, 0x40000000u)) : 0;
-  q.low = max(min(from, q.kv_len), 0);
+  q.low = min(first_seen(q.kv_len - q.q_len + 1, a.window), q.kv_len);
   q.units = (static_cast<uint32_t>(q.kv_len - q.first()) + UNIT - 1) / UNIT;
   q.tiles = q.kv_len ? (static_cast<uint32_t>(q.q_len) * a.group + 8 * NT - 1) / (8 * NT) : 0;
   return q;
@@ -749,7 +748,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
         fetch_k();
       }
       const int q_len = cur.q.q_len;
-      softmax64<D, NT>(w, s, u.left - static_cast<int>(UNIT) < q_len - 1 || (a.window && u.left > static_cast<int>(min(a.window, 0x40000000u))), u.left,
+      softmax64<D, NT>(w, s, u.left - static_cast<int>(UNIT) < q_len - 1 || (a.window && u.left > static_cast<int>(a.window)), u.left,
                        cur.tile * S::ROWS, q_len, a, lane);
       ok = wait();
       if (!ok) break;
@@ -932,7 +931,7 @@ cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, co
   a.max_kv = in.max_kv;
   a.table_stride = in.table_stride;
   a.table_pages = in.table_stride < (0x7fffffffu >> pool.log_page) ? in.table_stride : (0x7fffffffu >> pool.log_page);
-  a.window = in.window;
+  a.window = in.window < in.max_kv ? in.window : 0;  // (nobody has more keys)
   a.scale_log2 = in.scale * 1.4426950408889634f;
   a.bias = 0x64006400u;
   a.bf = bf;

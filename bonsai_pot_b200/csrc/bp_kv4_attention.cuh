@@ -22,6 +22,9 @@ struct AttnArgs {
   uint32_t bf;    // activations are bfloat16
   uint32_t q_vec; // rows of q are 16-byte aligned
 };
+// The first key that a query sees to which `keys` of its request are visible without a window (none or fewer: it lies before them all).
+// Nothing here may pass 31 bits: windows are shorter than max_kv (a longer one is none).
+__device__ __forceinline__ int first_seen(int keys, uint32_t window) { return window && keys > static_cast<int>(window) ? keys - static_cast<int>(window) : 0; }
 // A bounded wait for a barrier's phase: false after 2^20 polls or two seconds, or when *stop (may be null) is set.
 __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const volatile uint32_t* stop = nullptr) {
   if (mbar_test(bar, parity)) return true;

@@ -70,7 +70,7 @@ __device__ __forceinline__ Keys keys_of(const AttnArgs& a, const Request& q, uin
   Keys k;
   const int t0 = static_cast<int>(row0 / a.group), t1 = static_cast<int>((min(row0 + rows, q.rows) - 1) / a.group), past = q.kv_len - q.q_len;
   k.high = max(past + t1 + 1, 0);
-  k.low = a.window ? min(max(past + t0 + 1 - static_cast<int>(min(a.window, 0x40000000u)), 0), k.high) : 0;
+  k.low = first_seen(past + t0 + 1, a.window);
   k.tiles = max((static_cast<uint32_t>(k.high - k.first()) + BN - 1) / BN, 1u);
   return k;
 }
@@ -412,10 +412,10 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       const uint32_t tile_row = row0 + x * BM, row = tile_row + r;
       const float scale = row_scale[x * BM + r];
       // this row sees the keys [lo, hi); the tile's first row sees none from hi0 on, its last row none before lo1
-      const int window = static_cast<int>(min(a.window, 0x40000000u)), past = q.kv_len - q.q_len;
-      const int hi = row < q.rows ? past + static_cast<int>(row / a.group) + 1 : 0, lo = a.window ? hi - window : 0;
+      const int past = q.kv_len - q.q_len;
+      const int hi = row < q.rows ? past + static_cast<int>(row / a.group) + 1 : 0, lo = first_seen(hi, a.window);
       const int hi0 = past + static_cast<int>(tile_row / a.group) + 1;
-      const int lo1 = a.window ? past + static_cast<int>(min(tile_row + BM - 1, q.rows - 1) / a.group) + 1 - window : 0;
+      const int lo1 = first_seen(past + static_cast<int>(min(tile_row + BM - 1, q.rows - 1) / a.group) + 1, a.window);
       float m_run = NEG_BIG, l_run = 0.f;
       for (uint32_t i = 0; i < n; i++) {
         const uint32_t c = done + i, b = c & 1, s = c % SLOTS;

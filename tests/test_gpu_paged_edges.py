@@ -23,3 +23,42 @@ def test_page_tables_whose_rows_lie_apart(ctx, q, pitch):
     r.args[2] = view
     r.check(r.run(ctx))
     ctx.status()
+
+
+@pytest.mark.parametrize("heads", [1, 40])
+def test_windows_beyond_a_billion_keys(ctx, heads):
+    """All pages are the same one but the first, whose keys have so large a score that one of them outweighs all the others together: a window
+    that reaches it must not be cut shorter, one that does not reach it must not see it."""
+    kv, page, dim = (1 << 30) + 5000, 64, 64
+    rng = np.random.default_rng(15)
+    k, v = (rng.standard_normal((2 * page, 1, dim)).astype(np.float32) for _ in range(2))
+    k[:, :, 0] = 0.0
+    k[:page, :, 0] = 64.0
+    ref = R.Pool(2, page, 1, dim)
+    for kind, x in ((0, k), (1, v)):
+        ref.write(kind, np.arange(2 * page), *R.quantise(x))
+    pool = bp.KV4Pool(torch.from_numpy(ref.bytes).cuda(), 2, page, 1, dim)
+    table = torch.ones(1, -(-kv // page), dtype=torch.int32, device="cuda")
+    table[0, 0] = 0
+    q = torch.zeros(1, heads, dim, dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 10.0  # a score of 80 (natural logarithm) against 0 for a billion others
+    out = torch.empty_like(q)
+    start, length = torch.tensor([0, 1], dtype=torch.int32, device="cuda"), torch.tensor([kv], dtype=torch.int32, device="cuda")
+    keys, values = (R.dequantise(*R.quantise(x))[:, 0] for x in (k, v))
+    score = keys @ f64(q[0, 0]) * dim ** -0.5
+    place = np.arange(page)
+    for window, first in ((kv - 3, 3), (kv - 63, 63), (0, 0), (kv, 0), (kv - 64, page)):
+        ctx.attention(pool, q, out, start, length, table, max_q=1, max_kv=kv, window=window)
+        # how often each place of the two pages is seen
+        times = np.concatenate([place >= first, (kv - page - 1 - place) // page + 1]).astype(np.float64)
+        p = times * np.exp(score - score[times > 0].max())
+        p /= p.sum()
+        want, weight = p @ values, p @ np.abs(values)
+        if first < page:  # (binary32 sums of the rest do not count)
+            assert (np.abs(f64(out[0]) - want) <= HALF_UNIT["f16"] * np.abs(want) + (2.0 ** -11 + 2.0 ** -13) * weight + 2.0 ** -24).all(), window
+        else:
+            # a tensor core's binary32 sum may be cut, not rounded, at each of its steps of 16 keys: 2^-23 of it per step, and a CTA has
+            # 2^26 / SMs steps in a row
+            steps = (1 << 26) / torch.cuda.get_device_properties(0).multi_processor_count
+            assert (np.abs(f64(out[0]) - want) <= (2.0 ** -10 + steps * 2.0 ** -23) * weight).all(), window
+    ctx.status()
