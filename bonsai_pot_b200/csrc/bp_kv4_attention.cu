@@ -542,6 +542,22 @@ __device__ __forceinline__ void join_rows4(const AttnArgs& a, const Piece& p, ui
   for (int x = 0; x < V; x++) store4(a.bf, out + 32 * x, o[x].x * inv, o[x].y * inv, o[x].z * inv, o[x].w * inv);
 }
 
+// Zeros for the `n_tok` tokens of a request without keys, by a CTA. (Their values can be more than 32 bits count.)
+template <int D>
+__device__ __noinline__ void zero_rows(const AttnArgs& a, int q0, uint32_t n_tok) {
+  const uint32_t step = blockDim.x / (D / 4), dt = step / a.n_head, dh = step % a.n_head;  // rows that the CTA writes at a time
+  const uint32_t row = threadIdx.x / (D / 4);
+  for (uint32_t t = row / a.n_head, h = row % a.n_head; t < n_tok;) {
+    store4(false, a.out.data + static_cast<int64_t>(q0 + t) * a.out.tok + static_cast<int64_t>(h) * a.out.head + threadIdx.x % (D / 4) * 4, 0.f, 0.f, 0.f, 0.f);
+    t += dt;
+    h += dh;
+    if (h >= a.n_head) {
+      h -= a.n_head;
+      t++;
+    }
+  }
+}
+
 template <int D, int NT, uint32_t PAGE>
 __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel(const __grid_constant__ AttnArgs a, float* __restrict__ scratch, uint32_t* __restrict__ counters) {
   using S = Shape<D, NT>;
@@ -633,11 +649,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
   };
   for (uint32_t r = blockIdx.x; r < a.n_req; r += n_cta) {
     const Request q = known ? known[r] : request<NT>(a, r, false);
-    if (q.kv_len) continue;
-    for (uint32_t x = threadIdx.x; x < static_cast<uint32_t>(q.q_len) * a.n_head * (D / 4); x += THREADS) {
-      const uint32_t row = x / (D / 4);
-      store4(false, a.out.data + static_cast<int64_t>(q.q0 + row / a.n_head) * a.out.tok + static_cast<int64_t>(row % a.n_head) * a.out.head + x % (D / 4) * 4, 0.f, 0.f, 0.f, 0.f);
-    }
+    if (q.kv_len == 0) zero_rows<D>(a, q.q0, q.q_len);
   }
   // One item per CTA where that takes at most one round of the warps more than equal stretches, which need their pieces
   // joined; else equal stretches, of one unit per warp at least.

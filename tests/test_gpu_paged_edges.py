@@ -62,3 +62,16 @@ def test_windows_beyond_a_billion_keys(ctx, heads):
             steps = (1 << 26) / torch.cuda.get_device_properties(0).multi_processor_count
             assert (np.abs(f64(out[0]) - want) <= (2.0 ** -10 + steps * 2.0 ** -23) * weight).all(), window
     ctx.status()
+
+
+@pytest.mark.parametrize("dim,n", [(128, 1 << 23), (128, (1 << 23) + 3), (64, 1 << 24)])
+def test_zeros_for_more_rows_than_32_bits_of_values(ctx, dim, n):
+    """16 heads of n queries without any key. The queries are one row, the outputs lie four values apart (all are zeros), so that 2^27 rows fit."""
+    q = torch.zeros(1, 1, dim, dtype=torch.float16, device="cuda").expand(n, 16, dim)
+    store = torch.ones(n * 64 + dim - 4, dtype=torch.float16, device="cuda")
+    out = store.as_strided((n, 16, dim), (64, 4, 1))
+    pool = bp.KV4Pool(torch.zeros(bp.KV4Pool.bytes(1, 16, 4, dim), dtype=torch.uint8, device="cuda"), 1, 16, 4, dim)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    ctx.attention(pool, q, out, torch.tensor([0, n], **i32), torch.zeros(1, **i32), torch.zeros(1, 1, **i32), max_q=n, max_kv=0)
+    assert not store.any()
+    ctx.status()
