@@ -5,7 +5,9 @@
 //   S^T[token][row] = K Q^T    mma m16n8k16, A = the codes themselves: a nibble in an f16's low bits is the number q 2^-24
 //                              (q 2^-20 one nibble up; the query's dims there are scaled by 1/16), exact in the tensor core.
 //                              A block's sum is then multiplied by its d in binary32; the m's go through one m16n8k8 with the
-//                              query's block sums (f16 high and low part).
+//                              query's block sums (f16 high and low part). The mantissa of the softmax scale comes in with these two, so
+//                              that a power of two per row is left: taking the maximum off is then one operation that rounds the product of
+//                              no score, and scores may be of any size (2^24 and more, where a rounded maximum is off by powers of two).
 //   O^T[dim][row] += V^T P^T   A = V as f16 (m + d q, which does not round by the format's choice of m and d), B = P^T, which
 //                              movmatrix makes from the S^T fragments
 // with a running maximum and sum per row. Queries are scaled per row by a power of two so that the largest element lies in
@@ -24,6 +26,8 @@
 // at the end (the warps of a CTA end 1 to 3 us apart, joining a CTA's pieces takes 3, meeting the other CTAs 2, joining theirs 1 to 3). One request of 32768 keys:
 // 22.5 us (floor 6.4), 11 of them streaming. Why so: with one warp per item and no split these took 772 and 3064 us; with two CTAs of eight warps and two
 // buffers per warp 70 and 28; with joins by all threads of a CTA behind barriers, one item after the other, 86 and 31.
+#include <math.h>
+
 #include <type_traits>
 
 #include "bp_kv4_attention.cuh"
@@ -61,7 +65,7 @@ struct WarpState {
   static constexpr int NB = D / 32;
   uint32_t q[NT][NB][4];  // B fragments of S^T: dims 32 b + 8 t + {0,1}, {2,3} / 16, {4,5}, {6,7} / 16 of row g
   uint32_t qsum[NT];      // B fragment of the m's: block sums of row g
-  float s_scale[NT][2];   // rows 2 t, 2 t + 1: |softmax scale| (log2) times the row's power of two (its sign is the query's)
+  float s_scale[NT][2];   // rows 2 t, 2 t + 1: the softmax scale's power of two (log2 units) times the row's (its sign is the query's, its mantissa in the scores)
   float m[NT][2], l[NT][2];   // running maximum (log2 units) and this lane's part of the sum, of rows 2 t, 2 t + 1
   float o[NT][2 * NB][4]; // [m-tile i][dims 32 (i / 2) + 4 g + 2 (i % 2) + {0, 1}] x rows 2 t, 2 t + 1: {d0 r0, d0 r1, d1 r0, d1 r1}
 };
@@ -131,6 +135,7 @@ __device__ __forceinline__ void set_queries(WarpState<D, NT>& w, RawQueries<D, N
     }
     sum[b] += __shfl_xor_sync(FULL, sum[b], 1);
     sum[b] += __shfl_xor_sync(FULL, sum[b], 2);
+    sum[b] *= a.mantissa;
   }
   // k slots 2 t, 2 t + 1 of the m's MMA: blocks (0, 1), (2, 3) in the high part, then the low part
   float a0 = sum[0], a1 = sum[1];
@@ -145,7 +150,7 @@ __device__ __forceinline__ void set_queries(WarpState<D, NT>& w, RawQueries<D, N
 #pragma unroll
   for (int c = 0; c < 2; c++) {
     // (never 0: a masked score, -infinity, stays what it is)
-    w.s_scale[e][c] = fmaxf(fabsf(a.scale_log2) * __shfl_sync(FULL, down, 4 * (2 * t + c)), 1e-37f);
+    w.s_scale[e][c] = fmaxf(a.power * __shfl_sync(FULL, down, 4 * (2 * t + c)), 0x1p-122f);
     w.m[e][c] = NEG_BIG;
     w.l[e][c] = 0.f;
   }
@@ -162,9 +167,9 @@ __device__ constexpr uint32_t tile_at(int k, uint32_t row, uint32_t part) {
   return 16u * k / PAGE * (PAGE * (PoolLayout<D>::TOK / 2)) + part + 16u * k % PAGE * row;
 }
 
-// S^T of the k-th 16 tokens of a unit, not scaled.
+// S^T of the k-th 16 tokens of a unit, times the softmax scale's mantissa.
 template <int D, int NT, uint32_t PAGE>
-__device__ __forceinline__ void scores16(const WarpState<D, NT>& w, const uint8_t* buf, uint32_t lane, float (&s)[NT][4][4], int k) {
+__device__ __forceinline__ void scores16(const WarpState<D, NT>& w, const uint8_t* buf, uint32_t lane, float (&s)[NT][4][4], int k, float mantissa) {
   using L = PoolLayout<D>;
   constexpr int NB = D / 32;
   const uint8_t *kc = buf + tile_at<D, PAGE>(k, L::ROW, 0), *kd = buf + tile_at<D, PAGE>(k, 2 * NB, L::kd(PAGE)), *km = buf + tile_at<D, PAGE>(k, 2 * NB, L::km(PAGE));
@@ -208,7 +213,7 @@ __device__ __forceinline__ void scores16(const WarpState<D, NT>& w, const uint8_
       acc[3] = fmaf(db[b], p[3], acc[3]);
     }
 #pragma unroll
-    for (int c = 0; c < 4; c++) s[e][k][c] = fmaf(acc[c], 0x1p24f, low[c]);
+    for (int c = 0; c < 4; c++) s[e][k][c] = fmaf(acc[c], 0x1p24f * mantissa, low[c]);
   }
 }
 
@@ -751,7 +756,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
         uint8_t* kb = buf + b * S::PART;
         if (part) clear_scales<D, PAGE>(kb, u.pages, 0, UNIT);
 #pragma unroll
-        for (int k = 0; k < 4; k++) scores16<D, NT, PAGE>(w, kb, lane, s, k);
+        for (int k = 0; k < 4; k++) scores16<D, NT, PAGE>(w, kb, lane, s, k, a.mantissa);
       }
       done();
       if (RING == 3 && i + 1 < n) fetch_v();  // of unit i + 1
@@ -945,6 +950,11 @@ cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, co
   a.table_pages = in.table_stride < (0x7fffffffu >> pool.log_page) ? in.table_stride : (0x7fffffffu >> pool.log_page);
   a.window = in.window < in.max_kv ? in.window : 0;  // (nobody has more keys)
   a.scale_log2 = in.scale * 1.4426950408889634f;
+  int exponent = 0;
+  const float fraction = frexpf(fabsf(a.scale_log2), &exponent);
+  const bool split = fraction > 0.f && fraction < 1.f;  // (not of 0 and infinity)
+  a.mantissa = split ? 2.f * fraction : 1.f;
+  a.power = split ? ldexpf(1.f, exponent - 1) : fraction;
   a.bias = 0x64006400u;
   a.bf = bf;
   a.q_vec = reinterpret_cast<uintptr_t>(in.q.data) % 16 == 0 && in.q.tok_stride % 8 == 0 && in.q.head_stride % 8 == 0;

@@ -7,7 +7,7 @@ namespace bp {
 namespace kv4 {
 
 constexpr unsigned FULL = 0xffffffffu;
-constexpr float NEG_BIG = -1e30f;
+constexpr float NEG_BIG = -3e38f;  // the maximum of no score, below every score that 32 bits hold but the last few
 constexpr float P_UP = 10.f;   // P is stored as f16 times 2^10: it keeps its bits down to 2^-24 of the maximum
 
 struct AttnArgs {
@@ -18,6 +18,7 @@ struct AttnArgs {
   uint32_t n_req, n_head, group, total_q, max_q, max_kv, table_stride, window;
   uint32_t table_pages;  // of a row of the page table that are looked at: what 31 bits of keys fill at most (rows may lie further apart)
   float scale_log2;
+  float mantissa, power;  // their product: 1 <= mantissa < 2, power is one of two or 0
   uint32_t bias;  // 0x64006400: two f16 numbers 1024
   uint32_t bf;    // activations are bfloat16
   uint32_t q_vec; // rows of q are 16-byte aligned

@@ -441,9 +441,11 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
           for (uint32_t e = 0; e < 4; e++) mx[e] = max3(mx[e], __uint_as_float(raw[k + e]), __uint_as_float(raw[k + 4 + e]));
 #pragma unroll
         for (uint32_t e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], __uint_as_float(raw[BN - 4 + e]));
-        const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-        const bool grow = m_tile > m_run + GROW;
-        const float m_new = grow ? m_tile : m_run, corr = grow ? ex2(m_run - m_new) : 1.f;
+        const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) ;
+        // (The maximum is kept as it comes and taken off before the scale: scores may be of any size. A scaled one would be rounded, from 2^24 on by
+        // more than f16 has room for. One packed addition per two scores: 1.20 -> 1.23 ms for the prompt above.)
+        const bool grow = (m_tile - m_run) * scale > GROW;
+        const float m_new = grow ? m_tile : m_run, corr = grow ? ex2((m_run - m_new) * scale) : 1.f;
         m_run = m_new;
         if (i > 0 && __any_sync(FULL, grow)) {
           // O_X may be rescaled only between two P V: the previous tile's must be complete
@@ -461,14 +463,15 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
           }
         }
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        const float off = P_UP - m_new;
+        const float down = -m_new;
 #pragma unroll
         for (uint32_t k0 = 0; k0 < BN; k0 += 32) {
           uint32_t ph[16];
 #pragma unroll
           for (uint32_t k = 0; k < 16; k++) {
-            float e0, e1;
-            fma2(e0, e1, __uint_as_float(raw[k0 + 2 * k]), __uint_as_float(raw[k0 + 2 * k + 1]), scale, off);
+            float e0 = down, e1 = down;
+            add2(e0, e1, __uint_as_float(raw[k0 + 2 * k]), __uint_as_float(raw[k0 + 2 * k + 1]));
+            fma2(e0, e1, e0, e1, scale, P_UP);
             const float p0 = ex2(e0), p1 = ex2(e1);
             add2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], p0, p1);
             ph[k] = pack2<false>(p0, p1);
@@ -522,7 +525,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
             to[(4 * k + e) * S::ROWS] = make_float4(v[0], v[1], v[2], v[3]);  // (a warp's 32 rows are 512 bytes)
           }
         }
-        reinterpret_cast<float2*>(mine + D * S::ROWS)[x * BM + r] = make_float2(m_run, l_run);
+        reinterpret_cast<float2*>(mine + D * S::ROWS)[x * BM + r] = make_float2(l_run == 0.f ? NEG_BIG : m_run * scale, l_run);
       }
     }
     done += n;

@@ -75,3 +75,35 @@ def test_zeros_for_more_rows_than_32_bits_of_values(ctx, dim, n):
     ctx.attention(pool, q, out, torch.tensor([0, n], **i32), torch.zeros(1, **i32), torch.zeros(1, 1, **i32), max_q=n, max_kv=0)
     assert not store.any()
     ctx.status()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("scale", [1e4, 3e7, -2e9, 1e33])
+@pytest.mark.parametrize("q,heads,hkv,dim,kv", [(1, 8, 2, 128, 700), (3, 10, 2, 64, 90), (1, 4, 1, 128, 9000), (70, 8, 2, 128, 300), (130, 4, 1, 64, 200)])
+def test_scores_of_any_size(ctx, dtype, scale, q, heads, hkv, dim, kv):
+    """With such scales one key has all the weight of a row; rows whose two largest scores lie nearer than 32 bits can tell are left out."""
+    r = Requests(16, dtype, [q, q], [kv, kv // 2], heads, hkv, dim, 32)
+    out = f64(r.run(ctx, scale=scale))
+    told = asked = 0
+    for i in range(2):
+        keys, values, rows = r.keys[i], r.values[i], f64(r.q[r.start[i]:r.start[i + 1]])
+        for j in range(q):
+            n = len(keys) - q + j + 1
+            if n <= 0:
+                assert (out[r.start[i] + j] == 0).all()
+                continue
+            asked += heads
+            for h in range(heads):
+                s = keys[:n, h // (heads // hkv)] @ rows[j, h] * scale
+                best = int(s.argmax())
+                second = np.partition(s, -2)[-2] if n > 1 else -np.inf
+                # binary32 sums of some 130 terms: 2^-22 of the sum of magnitudes; what the second has is exp(-gap) of the weight, below 2^-24
+                noise = 2.0 ** -22 * (np.abs(keys[:n, h // (heads // hkv)]) @ np.abs(rows[j, h])).max() * abs(scale)
+                if s[best] - second < 2 * noise + 17:
+                    continue
+                told += 1
+                want = values[best, h // (heads // hkv)]
+                got = out[r.start[i] + j, h]
+                assert (np.abs(got - want) <= (HALF_UNIT[dtype] + 2.0 ** -11) * np.abs(want) + 2.0 ** -24 + 2.0 ** -22).all(), (i, j, h)
+    assert told >= 0.8 * asked
+    ctx.status()
