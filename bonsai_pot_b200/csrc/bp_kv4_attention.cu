@@ -461,6 +461,52 @@ __device__ __noinline__ void clear_scales(uint8_t* buf, uint32_t pages, int from
   __syncwarp();
 }
 
+// A token's d's in a buffer with a unit's K or V; bits of its blocks that have a scale that is no finite number.
+template <int D, uint32_t PAGE>
+__device__ __forceinline__ uint16_t* scales_at(uint8_t* buf, uint32_t tok) {
+  using L = PoolLayout<D>;
+  return reinterpret_cast<uint16_t*>(buf + tok / PAGE * (PAGE * (L::TOK / 2)) + L::kd(PAGE) + tok % PAGE * 2 * L::NB);
+}
+template <int D, uint32_t PAGE>
+__device__ __forceinline__ uint32_t blocks_without_numbers(uint8_t* buf, uint32_t tok) {
+  using L = PoolLayout<D>;
+  const uint32_t *d = reinterpret_cast<const uint32_t*>(scales_at<D, PAGE>(buf, tok)), *m = d + (L::km(PAGE) - L::kd(PAGE)) / 4;
+  uint32_t bad = 0;
+#pragma unroll
+  for (uint32_t b = 0; b < L::NB / 2; b++) bad |= no_numbers(d[b], m[b]) << (2 * b);
+  return bad;
+}
+// Values that are no numbers, in a unit of which an item's rows see different keys: 0 times such a value is not 0, so the blocks become zeros in the buffer
+// and are counted here, for the rows that see them. Returns what to write over: bit 2 NB e + NB c + b is block b of row 2 t + c of tile e.
+template <int D, int NT, uint32_t PAGE>
+__device__ __noinline__ uint32_t take_no_numbers(uint8_t* buf, int left, uint32_t tile0, int q_len, uint32_t group, uint32_t window) {
+  using L = PoolLayout<D>;
+  constexpr uint32_t NB = L::NB;
+  const uint32_t lane = threadIdx.x & 31;
+  uint32_t found = 0;
+#pragma unroll 1
+  for (uint32_t k = 0; k < UNIT; k += 32) {
+    const uint32_t tok = k + lane;
+    uint16_t *d = scales_at<D, PAGE>(buf, tok), *m = d + (L::km(PAGE) - L::kd(PAGE)) / 2;
+    const uint32_t bad = blocks_without_numbers<D, PAGE>(buf, tok);
+#pragma unroll
+    for (uint32_t b = 0; b < NB; b++)
+      if (bad >> b & 1) d[b] = m[b] = 0;
+    for (uint32_t who = __ballot_sync(FULL, bad != 0); who; who &= who - 1) {
+      const int at = __ffs(who) - 1, key = static_cast<int>(k) + at;
+      const uint32_t blocks = __shfl_sync(FULL, bad, at);
+      for (uint32_t e = 0; e < NT; e++)
+        for (uint32_t c = 0; c < 2; c++) {
+          const int behind = q_len - 1 - static_cast<int>((tile0 + 8 * e + 2 * (lane & 3) + c) / group), hi = left - behind;
+          if (behind >= 0 && key < hi && (window == 0 || key >= hi - static_cast<int>(window))) found |= blocks << (NB * (2 * e + c));
+        }
+    }
+  }
+  fence_proxy_async();  // the next copy into the buffer comes behind these
+  __syncwarp();
+  return found;
+}
+
 // A warp: row `row` of the `n` partial results at part(k) of an item, in order, becomes the output's row.
 template <int D, int NT, typename Part>
 __device__ __forceinline__ void join_row(const AttnArgs& a, const Piece& p, uint32_t row, uint32_t n, Part part, uint32_t lane) {
@@ -765,13 +811,23 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
         fetch_k();
       }
       const int q_len = cur.q.q_len;
-      softmax64<D, NT>(w, s, u.left - static_cast<int>(UNIT) < q_len - 1 || (a.window && u.left > static_cast<int>(a.window)), u.left,
-                       cur.tile * S::ROWS, q_len, a, lane);
+      const bool cut = u.left - static_cast<int>(UNIT) < q_len - 1 || (a.window && u.left > static_cast<int>(a.window));
+      softmax64<D, NT>(w, s, cut, u.left, cur.tile * S::ROWS, q_len, a, lane);
       ok = wait();
       if (!ok) break;
       {
         uint8_t* vb = buf + b * S::PART;
         if (part) clear_scales<D, PAGE>(vb, u.pages, u.low, u.left);
+        if (cut && q_len > 1 && __any_sync(FULL, (blocks_without_numbers<D, PAGE>(vb, lane) | blocks_without_numbers<D, PAGE>(vb, lane + 32)) != 0)) {
+          const uint32_t spoiled = take_no_numbers<D, NT, PAGE>(vb, u.left, cur.tile * S::ROWS, q_len, a.group, a.window);
+#pragma unroll
+          for (int e = 0; e < NT; e++)
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++)
+#pragma unroll
+              for (int c = 0; c < 4; c++)
+                if (spoiled >> (NB * (2 * e + (c & 1)) + i / 2) & 1) w.o[e][i][c] = __int_as_float(0x7fffffff);
+        }
 #pragma unroll
         for (int k = 0; k < 4; k++) values16<D, NT, PAGE>(w, vb, lane, s, k, a.bias);
       }

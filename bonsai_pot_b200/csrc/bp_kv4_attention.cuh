@@ -49,6 +49,11 @@ __device__ __forceinline__ uint32_t arrive(uint32_t* counter) {
   return before;
 }
 
+// Which of the two blocks whose d's and m's are the halves of d and m have a scale that is no finite number.
+__device__ __forceinline__ uint32_t no_numbers(uint32_t d, uint32_t m) {
+  constexpr uint32_t LO = 0x7c00u, HI = 0x7c000000u;
+  return ((d & LO) == LO || (m & LO) == LO ? 1u : 0u) | ((d & HI) == HI || (m & HI) == HI ? 2u : 0u);
+}
 // Four dims of an output row.
 __device__ __forceinline__ void store4(bool bf, uint16_t* p, float a, float b, float c, float d) {
   const uint32_t x = bf ? pack2<true>(a, b) : pack2<false>(a, b), y = bf ? pack2<true>(c, d) : pack2<false>(c, d);

@@ -30,6 +30,9 @@ using namespace bp::kv4;
 
 constexpr uint32_t BM = 128, BN = 64;  // query rows of a tile, keys of a tile
 constexpr uint32_t SLOTS = 4;          // K and V tiles in shared memory
+// Tiles of which some rows of an item see only a part: its rows are 256 tokens at most, so these are 5 tiles at each end of the keys that they see; where a
+// window is so short that no tile lies between the two ends, the two overlap or are less than two tiles apart: 11 tiles.
+constexpr uint32_t MIXED = 11;
 constexpr uint32_t ITEM_COST = 6;      // what beginning and ending an item costs, in key tiles
 constexpr float GROW = 5.f;            // log2 by which a maximum may grow before O is rescaled; P_UP + GROW stays below 16
 
@@ -63,6 +66,7 @@ __device__ __forceinline__ Request request(const AttnArgs& a, uint32_t r, bool r
 // rows have zeros to write).
 struct Keys {
   int low, high;
+  int all_from, all_to;  // every row sees the keys in between
   uint32_t tiles;
   __device__ int first() const { return low & ~static_cast<int>(BN - 1); }
 };
@@ -71,6 +75,8 @@ __device__ __forceinline__ Keys keys_of(const AttnArgs& a, const Request& q, uin
   const int t0 = static_cast<int>(row0 / a.group), t1 = static_cast<int>((min(row0 + rows, q.rows) - 1) / a.group), past = q.kv_len - q.q_len;
   k.high = max(past + t1 + 1, 0);
   k.low = first_seen(past + t0 + 1, a.window);
+  k.all_from = first_seen(past + t1 + 1, a.window);
+  k.all_to = past + t0 + 1;
   k.tiles = max((static_cast<uint32_t>(k.high - k.first()) + BN - 1) / BN, 1u);
   return k;
 }
@@ -176,6 +182,9 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t k_full[SLOTS], v_full[SLOTS], k_empty[SLOTS], v_empty[SLOTS], pv_done[NQ][SLOTS];
   __shared__ __align__(8) uint64_t s_ready[NQ][2], p_ready[NQ][2], p_free[NQ][2], o_done[NQ], drained;
+  // Values that are no numbers, in tiles of which the item's rows see different keys (0 times such a value is not 0): such blocks become zeros in
+  // V, `bad` has them by key (a bit per block), and a piece's end writes them over in the rows that see them.
+  __shared__ __align__(16) uint8_t bad[MIXED][BN];
   __shared__ float row_scale[S::ROWS];  // of a row's queries: the power of two that they were divided by
   __shared__ uint32_t line[THREADS + 1];
   __shared__ Cursor cur;
@@ -282,6 +291,9 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     const uint32_t head = cur.head, row0 = cur.x * S::ROWS, first = cur.at, n = min(keys.tiles - first, c1 - pos);
     const uint32_t start = cur.start;
     const int key_first = keys.first() + static_cast<int>(first * BN);
+    // the piece's tiles [plain0, plain0 + plain_n) are seen whole by every row
+    const uint32_t plain0 = static_cast<uint32_t>(max(keys.all_from - key_first + static_cast<int>(BN) - 1, 0)) / BN;
+    const uint32_t plain_n = static_cast<uint32_t>(max((keys.all_to - key_first) / static_cast<int>(BN) - static_cast<int>(plain0), 0));
     // ---- queries -> f16, each row divided by the power of two of its largest element ----
     {
       constexpr uint32_t U = D / 8, ITERS = (S::ROWS * U + THREADS - 1) / THREADS;
@@ -384,10 +396,19 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       ask_codes();
       for (uint32_t i = 0; i < n; i++) {
         const uint32_t c = done + i, s = c % SLOTS;
+        const bool mixed = i - plain0 >= plain_n;
         Raw<D> mine = raw;
-        if (!there) {
+        if (!there || mixed) {
+          uint32_t found = 0;
 #pragma unroll
-          for (int e = 0; e < D / 64; e++) mine.kd[e] = mine.km[e] = mine.vd[e] = mine.vm[e] = 0;
+          for (int e = 0; e < D / 64; e++) {
+            const uint32_t two = no_numbers(mine.vd[e], mine.vm[e]), keep = (two & 1 ? 0u : 0xffffu) | (two & 2 ? 0u : 0xffff0000u);
+            if (!there) mine.kd[e] = mine.km[e] = 0;
+            mine.vd[e] &= there ? keep : 0u;
+            mine.vm[e] &= there ? keep : 0u;
+            found |= two << (2 * e);
+          }
+          if (mixed && quarter == 0) bad[i < plain0 ? i : i - plain_n][row] = there ? static_cast<uint8_t>(found) : 0;
         }
         key += BN;
         id = id_next;
@@ -411,14 +432,13 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       const uint32_t lane_addr = (quad * 32) << 16, s_addr = tmem + lane_addr + x * 128, o_addr = tmem + lane_addr + S::TM_O + x * 128;
       const uint32_t tile_row = row0 + x * BM, row = tile_row + r;
       const float scale = row_scale[x * BM + r];
-      // this row sees the keys [lo, hi); the tile's first row sees none from hi0 on, its last row none before lo1
+      // this row sees the keys [lo, hi)
       const int past = q.kv_len - q.q_len;
       const int hi = row < q.rows ? past + static_cast<int>(row / a.group) + 1 : 0, lo = first_seen(hi, a.window);
-      const int hi0 = past + static_cast<int>(tile_row / a.group) + 1;
-      const int lo1 = first_seen(past + static_cast<int>(min(tile_row + BM - 1, q.rows - 1) / a.group) + 1, a.window);
       float m_run = NEG_BIG, l_run = 0.f;
       for (uint32_t i = 0; i < n; i++) {
         const uint32_t c = done + i, b = c & 1, s = c % SLOTS;
+        const bool mixed = i - plain0 >= plain_n;
         (void)waitx(&s_ready[x][b], (c >> 1) & 1);
         __syncwarp();
         tc_fence_after();
@@ -428,7 +448,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         for (uint32_t k = 0; k < BN; k += 32) tmem_ld32(s_addr + 64 * b + k, raw + k);
         tmem_ld_wait();
         const int key0 = key_first + static_cast<int>(i * BN);
-        if (key0 + static_cast<int>(BN) > hi0 || key0 < lo1) {
+        if (mixed) {
           const int from = lo - key0, to = hi - key0;
 #pragma unroll
           for (int k = 0; k < static_cast<int>(BN); k++)
@@ -443,7 +463,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         for (uint32_t e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], __uint_as_float(raw[BN - 4 + e]));
         const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) ;
         // (The maximum is kept as it comes and taken off before the scale: scores may be of any size. A scaled one would be rounded, from 2^24 on by
-        // more than f16 has room for. One packed addition per two scores: 1.20 -> 1.23 ms for the prompt above.)
+        // more than f16 has room for. One packed addition per two scores, 2 % of a prompt.)
         const bool grow = (m_tile - m_run) * scale > GROW;
         const float m_new = grow ? m_tile : m_run, corr = grow ? ex2((m_run - m_new) * scale) : 1.f;
         m_run = m_new;
@@ -484,18 +504,33 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&p_ready[x][b]));
       }
+      (void)waitx(&v_full[(done + n - 1) % SLOTS], ((done + n - 1) / SLOTS) & 1);  // (`bad` is complete)
+      uint32_t over = 0;
+#pragma unroll 1
+      for (uint32_t at = 0, i; (i = at < plain0 ? at : at + plain_n) < n; at++) {
+        const uint4* look = reinterpret_cast<const uint4*>(bad[at]);
+        uint32_t any = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < BN / 16; k++) any |= look[k].x | look[k].y | look[k].z | look[k].w;
+        const int key0 = key_first + static_cast<int>(i * BN);
+        if (any) {
+#pragma unroll 1
+          for (int k = max(lo - key0, 0); k < min(hi - key0, static_cast<int>(BN)); k++) over |= bad[at][k];
+        }
+      }
       (void)waitx(&o_done[x], pieces & 1);
       __syncwarp();
       tc_fence_after();
       if (first == 0 && n == keys.tiles) {
         // ---- the whole item: O / l through the dead Q tile, whole rows of it to memory ----
-        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+        const float inv_l = l_run == 0.f ? 0.f : 1.f / l_run;
         uint8_t* stage = smem + x * S::Q_B;
 #pragma unroll 1
         for (uint32_t k = 0; k < D / 16; k++) {
           uint32_t o[16];
           tmem_ld16(o_addr + 16 * k, o);
           tmem_ld_wait();
+          const float inv = over >> (k >> 1) & 1 ? __int_as_float(0x7fffffff) : inv_l;
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             float v[8];
@@ -517,6 +552,10 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
           uint32_t o[16];
           tmem_ld16(o_addr + 16 * k, o);
           tmem_ld_wait();
+          if (over >> (k >> 1) & 1) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[e] = 0x7fffffffu;
+          }
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             float v[4];

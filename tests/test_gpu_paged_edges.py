@@ -107,3 +107,35 @@ def test_scores_of_any_size(ctx, dtype, scale, q, heads, hkv, dim, kv):
                 assert (np.abs(got - want) <= (HALF_UNIT[dtype] + 2.0 ** -11) * np.abs(want) + 2.0 ** -24 + 2.0 ** -22).all(), (i, j, h)
     assert told >= 0.8 * asked
     ctx.status()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,hkv,dim", [(4, 1, 128), (10, 2, 64), (16, 2, 128), (3, 3, 64)])
+@pytest.mark.parametrize("q,kv,window,at", [(2, 70, 0, [69]), (4, 200, 0, [199, 198, 3]), (3, 129, 0, [127, 128]), (4, 300, 100, [198, 199, 200, 299, 100, 150]),
+                                            (3, 64, 64, [63, 1]), (130, 500, 0, [499, 450, 401, 370, 20]), (130, 130, 0, [0, 64, 129]), (200, 700, 90, [499, 411, 412, 640, 699]),
+                                            (520, 1400, 0, [1399, 1100]), (300, 2000, 65, [1700, 1900, 1635])])
+def test_values_that_are_no_numbers_reach_who_sees_them(ctx, dtype, heads, hkv, dim, q, kv, window, at):
+    """NaN in one block of a value at some keys: only queries that see such a key have it in their outputs, and only in the block's dims."""
+    r = Requests(17, dtype, [q, 1], [kv, 90], heads, hkv, dim, 16)
+    for i, key in enumerate(at):  # by append, as a layer would
+        k = torch.from_numpy(r.keys[0][key]).half().cuda()[None]
+        v = torch.from_numpy(r.values[0][key]).half().cuda()[None]
+        block = i % (dim // 32)
+        v[0, i % hkv, 32 * block + 5] = float("nan")
+        ctx.append(r.pool, k, v, None, torch.tensor([int(r.table[0, key // 16]) * 16 + key % 16], device="cuda"))
+        ks, vs = torch.empty_like(k), torch.empty_like(v)  # quantised anew: what the cache now holds
+        ctx.read(r.pool, torch.tensor([int(r.table[0, key // 16]) * 16 + key % 16], device="cuda"), ks, vs)
+        r.keys[0][key], r.values[0][key] = f64(ks[0]), f64(vs[0])
+    out = r.run(ctx, window=window)
+    none = np.isnan(r.values[0])
+    r.values[0] = np.where(none, 0.0, r.values[0])
+    place = np.arange(kv - q, kv)[:, None]
+    seen = (np.arange(kv) <= place) & ((np.arange(kv) > place - window) if window else True)
+    spoiled = np.repeat(np.einsum("qk,khd->qhd", seen.astype(np.int64), none.astype(np.int64)) > 0, heads // hkv, axis=1)
+    got = f64(out)
+    assert np.array_equal(np.isnan(got[:q]), spoiled) and spoiled.any() and not spoiled.all()
+    want, weight = R.attention(f64(r.q[:q]), r.keys[0], r.values[0], dim ** -0.5, window)
+    tol = HALF_UNIT[dtype] * np.abs(want) + (2.0 ** -11 + 2.0 ** -13) * weight + 2.0 ** -24
+    assert (np.abs(got[:q] - want) <= tol)[~spoiled].all()
+    r.check(out, window=window, only=[1])
+    ctx.status()
