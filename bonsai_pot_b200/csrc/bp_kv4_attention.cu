@@ -10,8 +10,7 @@
 //                              no score, and scores may be of any size (2^24 and more, where a rounded maximum is off by powers of two).
 //   O^T[dim][row] += V^T P^T   A = V as f16 (m + d q, which does not round by the format's choice of m and d), B = P^T, which
 //                              movmatrix makes from the S^T fragments
-// with a running maximum and sum per row. Queries are scaled per row by a power of two so that the largest element lies in
-// [1, 2): bf16 queries then fit f16.
+// with a running maximum and sum per row. Queries are multiplied per row by a power of two (RowPower): bf16 queries then fit f16.
 //
 // Work is cut into units of 64 keys of one item (request, KV head, 8 NT rows), all of them in one line, of which every CTA takes
 // an equal stretch and every warp of it an equal part: batches of any lengths fill the device evenly. A warp fetches its own keys and
@@ -120,9 +119,8 @@ __device__ __forceinline__ void set_queries(WarpState<D, NT>& w, RawQueries<D, N
     for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[b][i]));
   big = fmaxf(big, __shfl_xor_sync(FULL, big, 1));
   big = fmaxf(big, __shfl_xor_sync(FULL, big, 2));
-  // 2^e <= big: its exponent bits; tiny or zero rows keep e = -126
-  const uint32_t ebits = min(max(__float_as_uint(big) & 0x7f800000u, 0x00800000u), 0x7e800000u);
-  const float up = __uint_as_float(0x7f000000u - ebits), down = __uint_as_float(ebits), turn = copysignf(up, a.scale_log2);  // 2^-e, 2^e
+  const RowPower power = RowPower::of(big);
+  const float down = power.down(), turn = copysignf(power.up(), a.scale_log2);
   float sum[NB];
 #pragma unroll
   for (int b = 0; b < NB; b++) {

@@ -23,6 +23,15 @@ struct AttnArgs {
   uint32_t bf;    // activations are bfloat16
   uint32_t q_vec; // rows of q are 16-byte aligned
 };
+// Queries become f16 numbers, each row multiplied by the power of two that brings its largest element into [2^8, 2^9): the most for which 32 of them
+// times a mantissa add up within f16, as bp_kv4_attention.cu wants. f16 and bf16 queries keep all their bits down to 2^-18 of the row's largest element,
+// smaller ones are off by 2^-29 of it at most: f16 because the keys' values are f16 numbers, which a tensor core multiplies by nothing wider.
+struct RowPower {
+  uint32_t bits;  // exponent bits of the largest element; of zeros, tiny rows and infinities the nearest that leave 2^(8 - e) and 2^(e - 8) normal numbers
+  static __device__ RowPower of(float largest) { return RowPower{min(max(__float_as_uint(largest) & 0x7f800000u, 9u << 23), 254u << 23)}; }
+  __device__ float up() const { return __uint_as_float((262u << 23) - bits); }
+  __device__ float down() const { return __uint_as_float(bits - (8u << 23)); }
+};
 // The first key that a query sees to which `keys` of its request are visible without a window (none or fewer: it lies before them all).
 // Nothing here may pass 31 bits: windows are shorter than max_kv (a longer one is none).
 __device__ __forceinline__ int first_seen(int keys, uint32_t window) { return window && keys > static_cast<int>(window) ? keys - static_cast<int>(window) : 0; }

@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   // Values that are no numbers, in tiles of which the item's rows see different keys (0 times such a value is not 0): such blocks become zeros in
   // V, `bad` has them by key (a bit per block), and a piece's end writes them over in the rows that see them.
   __shared__ __align__(16) uint8_t bad[MIXED][BN];
-  __shared__ float row_scale[S::ROWS];  // of a row's queries: the power of two that they were divided by
+  __shared__ float row_scale[S::ROWS];  // the softmax scale in log2 units over the power of two of a row's queries
   __shared__ uint32_t line[THREADS + 1];
   __shared__ Cursor cur;
   __shared__ Join join_s;
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     // the piece's tiles [plain0, plain0 + plain_n) are seen whole by every row
     const uint32_t plain0 = static_cast<uint32_t>(max(keys.all_from - key_first + static_cast<int>(BN) - 1, 0)) / BN;
     const uint32_t plain_n = static_cast<uint32_t>(max((keys.all_to - key_first) / static_cast<int>(BN) - static_cast<int>(plain0), 0));
-    // ---- queries -> f16, each row divided by the power of two of its largest element ----
+    // ---- queries -> f16, each row times its power of two ----
     {
       constexpr uint32_t U = D / 8, ITERS = (S::ROWS * U + THREADS - 1) / THREADS;
       static_assert(THREADS % U == 0 && (S::ROWS * U) % 32 == 0, "rows are groups of U lanes");
@@ -324,13 +324,13 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[e]));
 #pragma unroll
         for (uint32_t o = 1; o < U; o <<= 1) big = fmaxf(big, __shfl_xor_sync(FULL, big, o));
-        const uint32_t ebits = min(max(__float_as_uint(big) & 0x7f800000u, 0x00800000u), 0x7e800000u);
-        const float up = copysignf(__uint_as_float(0x7f000000u - ebits), a.scale_log2);
+        const RowPower power = RowPower::of(big);
+        const float up = copysignf(power.up(), a.scale_log2);
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] *= up;
         *reinterpret_cast<uint4*>(smem + (r / BM) * S::Q_B + oper_off(BM, r % BM, u)) = pack8<false>(x);
         // (never 0: a masked score, -infinity, stays what it is)
-        if (u == 0) row_scale[r] = fmaxf(fabsf(a.scale_log2) * __uint_as_float(ebits), 1e-37f);
+        if (u == 0) row_scale[r] = fmaxf(fabsf(a.scale_log2) * power.down(), 1e-37f);
       }
     }
     fence_proxy_async();

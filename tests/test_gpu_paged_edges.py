@@ -139,3 +139,27 @@ def test_values_that_are_no_numbers_reach_who_sees_them(ctx, dtype, heads, hkv, 
     assert (np.abs(got[:q] - want) <= tol)[~spoiled].all()
     r.check(out, window=window, only=[1])
     ctx.status()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,hkv,dim", [(4, 1, 128), (10, 2, 64), (16, 1, 128)])
+@pytest.mark.parametrize("q", [1, 5, 130])
+def test_queries_with_a_wide_range_within_a_row(ctx, dtype, heads, hkv, dim, q):
+    """The first 32 dims of all keys are zeros, and those of the queries larger than the others by 2^17: what counts are the small ones, whose bits
+    must have been kept. (The sums that the zeros are in have no share in an error.)"""
+    r = Requests(18, dtype, [q, q], [300, 170], heads, hkv, dim, 32)
+    for i in range(2):
+        k, v = (torch.from_numpy(x).half().cuda() for x in (r.keys[i], r.values[i]))
+        k[:, :, :32] = 0
+        at = np.arange(len(k))
+        slots = torch.from_numpy(r.table[i, at // 32].astype(np.int64) * 32 + at % 32).cuda()
+        ctx.append(r.pool, k, v, None, slots)
+        ks, vs = torch.empty_like(k), torch.empty_like(v)
+        ctx.read(r.pool, slots, ks, vs)
+        r.keys[i], r.values[i] = f64(ks), f64(vs)
+        assert (r.keys[i][:, :, :32] == 0).all()
+    small = 1.0 if dtype == "bf16" else 0.125
+    r.q *= small
+    r.q[:, :, :32] = 2.0 ** 17 * small
+    out = r.run(ctx, scale=dim ** -0.5 / small)
+    r.check(out, scale=dim ** -0.5 / small)
