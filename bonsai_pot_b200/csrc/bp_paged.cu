@@ -121,6 +121,8 @@ int bp_paged_create(int32_t device, bp_paged_ctx** out) {
   c->err_host[0] = c->err_host[1] = 0;
   void* dev = nullptr;
   BP_TRY(c, cudaHostGetDevicePointer(&dev, c->err_host, 0));
+  // the counters' zeros are written on the legacy stream, for which a first call's stream need not wait
+  BP_TRY(c, cudaStreamSynchronize(cudaStreamLegacy));
   c->err_dev = static_cast<uint32_t*>(dev);
   return BP_OK;
 }

@@ -163,3 +163,15 @@ def test_queries_with_a_wide_range_within_a_row(ctx, dtype, heads, hkv, dim, q):
     r.q[:, :, :32] = 2.0 ** 17 * small
     out = r.run(ctx, scale=dim ** -0.5 / small)
     r.check(out, scale=dim ** -0.5 / small)
+
+
+def test_a_new_context_is_ready_for_every_stream():
+    """Its counters are zeroed behind what the legacy stream still has to do: creation waits for that."""
+    bp.PagedContext().close()  # (what is loaded once has been)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)  # some 100 ms
+    before = torch.cuda.Event()
+    before.record()
+    c = bp.PagedContext()
+    assert before.query()
+    c.close()
