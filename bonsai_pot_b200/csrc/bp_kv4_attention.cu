@@ -1012,13 +1012,17 @@ cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, co
   a.bias = 0x64006400u;
   a.bf = bf;
   a.q_vec = reinterpret_cast<uintptr_t>(in.q.data) % 16 == 0 && in.q.tok_stride % 8 == 0 && in.q.head_stride % 8 == 0;
-  // Which kernel. Up to 16 rows (tokens x query heads per KV head) a request is two tiles of eight here, and every tile more expands the
-  // codes again; there a row costs nothing up to 128. us, this kernel / the other one, D = 128, 8 KV heads: 16 requests of 4096 keys, 12 rows
-  // 42.5 / 73.7, 16 rows 42.6 / 73.8, 24 rows 77 / 74, 32 rows 80 / 74; with few items the line moves up, 1 request of 2000 keys, 32 rows
-  // 20 / 29.5, of 30000 keys 51.9 / 63.6 (48 rows 65.5 / 64.2). D = 64: 16 x 4096, 15 rows 31 / 58, 20 rows 52 / 59, 30 rows 55 / 59, 40 rows 68 / 59.
+  // Which kernel. Here the codes are expanded once per 16 rows (tokens x query heads per KV head) of a request, there once for up to 128, with some 14 us
+  // for an item's beginning and end. us, this kernel / the other one:
+  //   head_dim 128, 32 / 8 heads         16 rows  32 rows  48 rows     head_dim 64, 40 / 8 heads    15 rows  30 rows  40 rows  50 rows
+  //   16 requests of 4096 keys           41/75    68/75    97/76                                    28/60    47/61    60/61    78/61
+  //   the same, window 1024              19/36    31/36    38/36                                    15/28    24/29    26/29    30/29
+  //   64 requests of 1000 keys           46/85    78/87    113/88                                   29/70    50/70    65/71    85/72
+  //   1 request of 30000 keys            33/64    48/63    62/64                                    27/45    36/45    42/45    50/45
+  // and as much apart with 2, 4 and 8 requests of 4096 keys and with 2 KV heads; so 32 rows is the line for both.
   const uint64_t rows = static_cast<uint64_t>(a.max_q) * a.group;
   // (Without any key there are only zeros to write, and there may be no pool: this kernel looks at none.)
-  if (a.max_kv != 0 && (rows > 32 || (rows > 16 && 2 * static_cast<uint64_t>(a.n_req) * pool.n_kv_head > static_cast<uint64_t>(c->sm_count)))) return bp_launch_kv4_prefill(c, s, head_dim, a);
+  if (a.max_kv != 0 && rows > 32) return bp_launch_kv4_prefill(c, s, head_dim, a);
   return with_kernel(head_dim, a.max_q * a.group > 8, pool.page, [&](auto kernel, auto shape) {
     return bp_launch(true, kernel, dim3(c->sm_count), dim3(shape.THREADS), shape.SMEM, s, a, c->partials, c->counters);
   });
