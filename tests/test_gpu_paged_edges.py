@@ -175,3 +175,149 @@ def test_a_new_context_is_ready_for_every_stream():
     c = bp.PagedContext()
     assert before.query()
     c.close()
+
+
+# ---- long stretches: every warp or CTA works on many units of several items ------------------------------------------
+
+class Shared(Requests):
+    """Requests whose pages are drawn from a few hundred, many of them several times: long contexts that cost little to make. rising: a request's pages
+    lie in the order of the size of their keys, so that a running maximum grows again and again on the way."""
+
+    def __init__(self, seed, dtype, q_len, kv_len, heads, hkv, dim, page, rising=False, pages=150):
+        rng = np.random.default_rng(seed)
+        self.q_len, self.kv_len, self.dtype, self.dim, self.page, self.hkv = q_len, kv_len, dtype, dim, page, hkv
+        self.ref = R.Pool(pages, page, hkv, dim)
+        x = rng.standard_normal((2, pages * page, hkv, dim)).astype(np.float32)
+        if rising:
+            x[0] *= np.linspace(0.2, 3.0, pages, dtype=np.float32).repeat(page)[:, None, None]
+        self.rows = []
+        for kind in range(2):
+            parts = R.quantise(x[kind])
+            self.ref.write(kind, np.arange(pages * page), *parts)
+            self.rows.append(R.dequantise(*parts).reshape(pages, page, hkv, dim))
+        self.table = rng.integers(0, pages, (len(kv_len), max(-(-max(kv_len) // page), 1))).astype(np.int32)
+        if rising:
+            for row, k in zip(self.table, kv_len):
+                row[:-(-k // page)].sort()
+        self.pool = bp.KV4Pool(torch.from_numpy(self.ref.bytes).cuda(), pages, page, hkv, dim)
+        self.q = normal(seed + 1, (sum(q_len), heads, dim), dtype, 1.5)
+        self.start = np.concatenate([[0], np.cumsum(q_len)]).astype(np.int32)
+        self.args = [torch.from_numpy(a).cuda() for a in (self.start, np.array(kv_len, np.int32), self.table)]
+
+    def gathered(self, kind):
+        class Rows:
+            def __getitem__(_, r):
+                k = self.kv_len[r]
+                return self.rows[kind][self.table[r, :-(-k // self.page)]].reshape(-1, self.hkv, self.dim)[:k]
+        return Rows()
+
+    keys = property(lambda self: self.gathered(0))
+    values = property(lambda self: self.gathered(1))
+
+
+def sms():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+# (heads, KV heads, head_dim, tokens, page, warps of a CTA): one and two tiles of eight rows, both dims; pages of 16: more than 32 of them per warp
+@pytest.mark.parametrize("heads,hkv,dim,q,page,warps", [(32, 8, 128, 1, 16, 12), (32, 8, 128, 1, 64, 12), (16, 8, 64, 1, 16, 16), (16, 8, 64, 4, 32, 16), (32, 8, 128, 4, 32, 8),
+                                                        (32, 4, 128, 2, 16, 8), (14, 2, 64, 2, 16, 12), (40, 8, 64, 5, 64, 12)])
+@pytest.mark.parametrize("window", [0, 1500])
+@pytest.mark.parametrize("rising", [False, True])
+def test_many_units_per_warp(ctx, heads, hkv, dim, q, page, warps, window, rising):
+    """Some 12 (pages of 16) or 6 units of 64 keys for every warp of the device, of ragged requests: rings are filled again and again, items change within
+    a warp's stretch and end in the middle of it, page ids are read anew."""
+    rng = np.random.default_rng(heads + q)
+    rows = q * heads // hkv
+    tiles = -(-rows // 8) if rows <= 8 else -(-rows // 16)
+    units = (12 if page == 16 else 6) * warps * sms()
+    kv = []
+    while sum(min(k, window or k) for k in kv) * hkv * tiles < units * 64:
+        kv.append(int(rng.integers(1, 4300)))
+    kv[3] = 0
+    r = Shared(19, "bf16", [q] * len(kv), kv, heads, hkv, dim, page, rising)
+    out = r.run(ctx, window=window)
+    r.check(out, window=window, only=sorted({0, 3, len(kv) - 1, int(np.argmax(kv)), *(int(x) for x in rng.integers(0, len(kv), 12))}))
+    assert torch.equal(out, r.run(ctx, window=window))
+    ctx.status()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,hkv,dim,q,kv", [(16, 8, 128, [100], [12100]), (16, 8, 64, [110], [12100]), (32, 8, 128, [20], [12100]), (24, 8, 64, [33], [12500]),
+                                                (8, 4, 128, [150, 7, 60, 1, 129], [9000, 7000, 4100, 8000, 6000])])
+@pytest.mark.parametrize("rising", [False, True])
+def test_many_key_tiles_per_cta(ctx, dtype, heads, hkv, dim, q, kv, rising):
+    """Ten tiles of 64 keys and more of one item per CTA (all slots several times), one and two query tiles; rising: O is rescaled on the way."""
+    r = Shared(20, dtype, q, kv, heads, hkv, dim, 32, rising)
+    out = r.run(ctx)
+    r.check(out)
+    assert torch.equal(out, r.run(ctx))
+    ctx.status()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_tokens_and_chunks_in_one_call(ctx, dim):
+    """What a server with chunked prompts issues: hundreds of requests with one token beside a few with a chunk."""
+    rng = np.random.default_rng(dim)
+    q = [1] * 300 + [200, 77, 1, 300]
+    kv = [int(x) for x in rng.integers(1, 1500, 300)] + [900, 77, 0, 1300]
+    order = rng.permutation(len(q))
+    q, kv = [q[i] for i in order], [kv[i] for i in order]
+    r = Shared(21, "bf16", q, kv, 8, 2, dim, 16)
+    out = r.run(ctx)
+    r.check(out, only=[i for i in range(len(q)) if q[i] > 1 or kv[i] == 0 or i % 9 == 0])
+    r.check(r.run(ctx, window=333), window=333, only=[i for i in range(len(q)) if q[i] > 1 or i % 9 == 0])
+    ctx.status()
+
+
+def test_two_contexts_at_once(ctx):
+    """Each has its own scratch memory: calls on two streams do not meet."""
+    a, b = Shared(22, "f16", [1] * 3, [30000, 5000, 20000], 32, 8, 128, 32), Shared(23, "f16", [70, 3], [9000, 4000], 16, 4, 128, 32)
+    want = [x.run(ctx) for x in (a, b)]
+    a.check(want[0])
+    b.check(want[1])
+    torch.cuda.synchronize()
+    with bp.PagedContext() as other:
+        streams, outs = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+        for _ in range(10):
+            for i, (c, x) in enumerate(((ctx, a), (other, b))):
+                with torch.cuda.stream(streams[i]):
+                    outs[i].append(x.run(c, out=torch.zeros_like(x.q)))
+        for i, c in enumerate((ctx, other)):
+            c.status(stream=streams[i])
+            assert all(torch.equal(o, want[i]) for o in outs[i])
+
+
+# ---- rope: several heads per thread ----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n,heads,dim,rot,layout,norm,dtype", [(30500, 5, 80, 80, "half", True, "bf16"), (30500, 5, 128, 64, "interleaved", False, "f16"), (17000, 9, 128, 128, "half", False, "bf16"),
+                                                              (17000, 9, 80, 32, "interleaved", True, "f16"), (6400, 24, 128, 128, "half", True, "f16"), (13000, 24, 64, 64, "interleaved", True, "bf16"),
+                                                              (20000, 2, 256, 256, "half", False, "f16")])
+def test_rope_of_long_prompts(ctx, n, heads, dim, rot, layout, norm, dtype):
+    """So many rows that a thread has four heads of a token (or as many as are left); out of place, in place, tokens that are padding."""
+    lanes = 1 << (dim // 16 - 1).bit_length()
+    assert n * heads * lanes // 4 >= 2048 * sms() or heads < 3
+    x = normal(n, (n, heads + 1, dim), dtype, 2.0)[:, 1:]
+    tab = R.table(500, rot)
+    pos = np.random.default_rng(6).integers(0, 500, n).astype(np.int32)
+    pos[[0, 7, n - 1]] = -1
+    w = normal(8, (dim,), dtype) if norm else None
+    want = f64(x)
+    if norm:
+        want = R.norm64(want, f64(w), 1e-6)
+    full = R.rotate(want, tab, np.maximum(pos, 0), layout)
+    near = np.abs(want)
+    p1, p2 = R.pairs(rot, layout)
+    near[..., p1] = near[..., p2] = near[..., p1] + near[..., p2]
+    table, at = bp.RopeTable(torch.from_numpy(tab).cuda(), layout), torch.from_numpy(pos).cuda()
+    out = torch.full((n, heads, dim), 3.0, dtype=TYPES[dtype], device="cuda")
+    ctx.rope(x, out, at, table, w_norm=w)
+    there = pos >= 0
+    assert (out[torch.from_numpy(~there).cuda()] == 3.0).all()
+    err = np.abs(f64(out) - full)[there]
+    assert (err <= (HALF_UNIT[dtype] * np.abs(full) + 2.0 ** -25 + 2.0 ** -20 * near)[there]).all(), err.max()
+    before = x.clone()
+    ctx.rope(x, x, at, table, w_norm=w)
+    keep = torch.from_numpy(~there).cuda()
+    assert torch.equal(x[keep], before[keep]) and torch.equal(x[~keep], out[~keep])
+    ctx.status()
