@@ -2,8 +2,8 @@
 
 One attention layer of the 8B shape (32 query / 8 KV heads of 128) on made-up activations stands for a model's layers: what a layer
 does with its cache is complete (norm, rotary positions, append, attention), the projections around it are not there. A request
-gets pages as it grows and gives them back when it ends. At the end the decoded outputs are compared with a plain softmax over
-the keys and values that the cache says it holds.
+gets pages as it grows and gives them back when it ends. The outputs of every prompt chunk and of the last step are compared with a
+plain softmax over the keys and values that the cache says it holds.
 
     python examples/paged_serving.py [--steps 64]
 """
@@ -75,29 +75,48 @@ def projections(n):
     return torch.randn(n, N_HEAD + 2 * N_KV_HEAD, HEAD_DIM, device="cuda").bfloat16()
 
 
+def deviation(server, request, q, out):
+    """Of `out`, the outputs of the request's last tokens q, from the plain softmax: the largest, and the largest in parts of sum p |v|."""
+    k, v = (t.repeat_interleave(N_HEAD // N_KV_HEAD, 1) for t in server.keys(request))
+    n, total = q.shape[0], k.shape[0]
+    scores = torch.einsum("qhd,thd->qht", q.float(), k) / HEAD_DIM ** 0.5
+    hidden = torch.arange(total, device="cuda") > torch.arange(total - n, total, device="cuda")[:, None]
+    p = torch.softmax(scores.masked_fill(hidden[:, None], float("-inf")), -1)
+    off = (torch.einsum("qht,thd->qhd", p, v) - out.float()).abs()
+    return off.max().item(), (off / torch.einsum("qht,thd->qhd", p, v.abs())).max().item()
+
+
 def run(steps=64, prompts=(700, 37, 1, 1300), seed=0):
     """Serves the prompts for `steps` tokens each; returns the largest deviation of the last step's outputs from the plain softmax."""
+    return serve(steps, prompts, seed)[0]
+
+
+def serve(steps, prompts, seed=0):
+    """The same; returns that deviation, and the largest of the prompts' outputs in parts of sum p |v|."""
     torch.manual_seed(seed)
+    of_prompts = 0.0
     server = Server()
     for r, n in enumerate(prompts):
         server.add(r)
         for at in range(0, n, CHUNK):
-            server.layer([r], [min(CHUNK, n - at)], projections(min(CHUNK, n - at)))
+            q, out = server.layer([r], [min(CHUNK, n - at)], projections(min(CHUNK, n - at)))
+            of_prompts = max(of_prompts, deviation(server, r, q, out)[1])
     live, worst = list(range(len(prompts))), 0.0
     for step in range(steps):
         q, out = server.layer(live, [1] * len(live), projections(len(live)))
+        rows = list(live)
         if step == steps // 2 and len(live) > 1:  # a request ends, its pages serve the others
             server.drop(live.pop(1))
-    live_rows = list(range(q.shape[0]))
-    for row, r in zip(live_rows, live):
-        k, v = (t.repeat_interleave(N_HEAD // N_KV_HEAD, 1) for t in server.keys(r))
-        p = torch.softmax(torch.einsum("hd,thd->ht", q[row].float(), k) / HEAD_DIM ** 0.5, -1)
-        worst = max(worst, (torch.einsum("ht,thd->hd", p, v) - out[row].float()).abs().max().item())
+    for row, r in enumerate(rows if steps else []):
+        if r not in live:
+            continue
+        worst = max(worst, deviation(server, r, q[row:row + 1], out[row:row + 1])[0])
     server.ctx.status()
-    return worst
+    return worst, of_prompts
 
 
 if __name__ == "__main__":
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--steps", type=int, default=64)
-    print("largest deviation from a plain softmax: %.2g" % run(ap.parse_args().steps))
+    decoded, of_prompts = serve(ap.parse_args().steps, (700, 37, 1, 1300))
+    print("largest deviation from a plain softmax: %.2g decoded, %.2g of sum p |v| in prompts" % (decoded, of_prompts))

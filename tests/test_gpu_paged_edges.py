@@ -321,3 +321,11 @@ def test_rope_of_long_prompts(ctx, n, heads, dim, rot, layout, norm, dtype):
     keep = torch.from_numpy(~there).cuda()
     assert torch.equal(x[keep], before[keep]) and torch.equal(x[~keep], out[~keep])
     ctx.status()
+
+
+def test_the_prompts_of_the_serving_example(ctx):
+    """bf16 outputs: half a unit is 2^-8 of the value at most, which is no larger than sum p |v|; P's rounding and the binary32 sums as everywhere."""
+    from examples import paged_serving
+    decoded, of_prompts = paged_serving.serve(1, (700, 37, 1, 1300), seed=1)
+    assert decoded <= 2.0 ** -7 + 2.0 ** -8
+    assert of_prompts <= 2.0 ** -8 + 2.0 ** -11 + 2.0 ** -13
