@@ -167,7 +167,7 @@ __device__ constexpr uint32_t tile_at(int k, uint32_t row, uint32_t part) {
 
 // S^T of the k-th 16 tokens of a unit, times the softmax scale's mantissa.
 template <int D, int NT, uint32_t PAGE>
-__device__ __forceinline__ void scores16(const WarpState<D, NT>& w, const uint8_t* buf, uint32_t lane, float (&s)[NT][4][4], int k, float mantissa) {
+__device__ __forceinline__ void scores16(const WarpState<D, NT>& w, const uint8_t* buf, uint32_t lane, float (&s)[NT][4][4], int k, float mantissa24) {
   using L = PoolLayout<D>;
   constexpr int NB = D / 32;
   const uint8_t *kc = buf + tile_at<D, PAGE>(k, L::ROW, 0), *kd = buf + tile_at<D, PAGE>(k, 2 * NB, L::kd(PAGE)), *km = buf + tile_at<D, PAGE>(k, 2 * NB, L::km(PAGE));
@@ -211,7 +211,7 @@ __device__ __forceinline__ void scores16(const WarpState<D, NT>& w, const uint8_
       acc[3] = fmaf(db[b], p[3], acc[3]);
     }
 #pragma unroll
-    for (int c = 0; c < 4; c++) s[e][k][c] = fmaf(acc[c], 0x1p24f * mantissa, low[c]);
+    for (int c = 0; c < 4; c++) s[e][k][c] = fmaf(acc[c], mantissa24, low[c]);
   }
 }
 
@@ -800,7 +800,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
         uint8_t* kb = buf + b * S::PART;
         if (part) clear_scales<D, PAGE>(kb, u.pages, 0, UNIT);
 #pragma unroll
-        for (int k = 0; k < 4; k++) scores16<D, NT, PAGE>(w, kb, lane, s, k, a.mantissa);
+        for (int k = 0; k < 4; k++) scores16<D, NT, PAGE>(w, kb, lane, s, k, a.mantissa24);
       }
       done();
       if (RING == 3 && i + 1 < n) fetch_v();  // of unit i + 1
@@ -1008,6 +1008,7 @@ cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, co
   const float fraction = frexpf(fabsf(a.scale_log2), &exponent);
   const bool split = fraction > 0.f && fraction < 1.f;  // (not of 0 and infinity)
   a.mantissa = split ? 2.f * fraction : 1.f;
+  a.mantissa24 = a.mantissa * 0x1p24f;
   a.power = split ? ldexpf(1.f, exponent - 1) : fraction;
   a.bias = 0x64006400u;
   a.bf = bf;

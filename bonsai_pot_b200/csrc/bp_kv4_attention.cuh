@@ -19,6 +19,7 @@ struct AttnArgs {
   uint32_t table_pages;  // of a row of the page table that are looked at: what 31 bits of keys fill at most (rows may lie further apart)
   float scale_log2;
   float mantissa, power;  // their product: 1 <= mantissa < 2, power is one of two or 0
+  float mantissa24;       // the mantissa times 2^24
   uint32_t bias;  // 0x64006400: two f16 numbers 1024
   uint32_t bf;    // activations are bfloat16
   uint32_t q_vec; // rows of q are 16-byte aligned
