@@ -36,6 +36,18 @@ struct RowPower {
 // The first key that a query sees to which `keys` of its request are visible without a window (none or fewer: it lies before them all).
 // Nothing here may pass 31 bits: windows are shorter than max_kv (a longer one is none).
 __device__ __forceinline__ int first_seen(int keys, uint32_t window) { return window && keys > static_cast<int>(window) ? keys - static_cast<int>(window) : 0; }
+// What a request has, cut to what there is: its first row of q, its queries, its keys. report: a cut is reported.
+struct Lengths {
+  int q0, q_len, kv_len;
+};
+__device__ __forceinline__ Lengths lengths_of(const AttnArgs& a, uint32_t r, bool report) {
+  const int start = a.q_start[r], stop = a.q_start[r + 1], keys = a.kv_len[r], q0 = max(start, 0);
+  const int given_q = max(stop, q0) - q0, given_kv = max(keys, 0);
+  const Lengths n{q0, min(min(given_q, static_cast<int>(a.max_q)), max(static_cast<int>(a.total_q) - q0, 0)),
+                  min(given_kv, static_cast<int>(min(a.max_kv, a.table_pages << a.pool.log_page)))};
+  if (report && (given_q > n.q_len || given_kv > n.kv_len || (start < 0 && stop > start))) note_range(a.err);
+  return n;
+}
 // A bounded wait for a barrier's phase: false after 2^20 polls or two seconds, or when *stop (may be null) is set.
 __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const volatile uint32_t* stop = nullptr) {
   if (mbar_test(bar, parity)) return true;

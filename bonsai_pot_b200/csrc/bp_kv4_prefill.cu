@@ -53,12 +53,10 @@ struct Request {
 };
 __device__ __forceinline__ Request request(const AttnArgs& a, uint32_t r, bool report) {
   Request q;
-  const int start = a.q_start[r], stop = a.q_start[r + 1], keys = a.kv_len[r];
-  q.q0 = max(start, 0);
-  const int given_q = max(min(stop, static_cast<int>(a.total_q)) - q.q0, 0), given_kv = max(keys, 0);
-  q.q_len = min(given_q, static_cast<int>(a.max_q));
-  q.kv_len = min(given_kv, static_cast<int>(min(a.max_kv, a.table_pages << a.pool.log_page)));
-  if (report && (given_q > q.q_len || given_kv > q.kv_len)) note_range(a.err);
+  const Lengths n = lengths_of(a, r, report);
+  q.q0 = n.q0;
+  q.q_len = n.q_len;
+  q.kv_len = n.kv_len;
   q.rows = static_cast<uint32_t>(q.q_len) * a.group;
   return q;
 }

@@ -40,8 +40,9 @@ typedef struct bp_paged_ctx bp_paged_ctx;
 int bp_paged_create(int32_t device, bp_paged_ctx** out);
 void bp_paged_destroy(bp_paged_ctx* ctx);
 /* Waits for `stream`, then: BP_OK; BP_ERR_CONTEXT_OVERFLOW once if a token's position lay behind the table, its slot behind
- * the pool, a page id outside the pool, or a request had more keys than its row of the page table holds (such rows were
- * left out or cut, nothing outside the caller's buffers was touched); or the latched BP_ERR_TIMEOUT / BP_ERR_DEVICE_LOST. */
+ * the pool, a page id outside the pool, or a request had more keys than its row of the page table holds or max_kv says, more
+ * queries than max_q says or some outside the rows of q (they were left out or cut, nothing outside the caller's buffers was
+ * touched); or the latched BP_ERR_TIMEOUT / BP_ERR_DEVICE_LOST. */
 int bp_paged_status(bp_paged_ctx* ctx, void* stream);
 const char* bp_paged_last_error(const bp_paged_ctx* ctx);
 
@@ -94,11 +95,15 @@ int bp_kv4_read(bp_paged_ctx* ctx, void* stream, uint32_t dtype, const bp_kv4_po
                 const bp_rows* k, const bp_rows* v);
 
 /* Attention of several requests. q, out: rows of n_head heads, the requests' queries one behind the other: request r has
- * rows [q_start[r], q_start[r + 1]) (device int32 [n_req + 1]) and kv_len[r] keys (device int32), in the pages
- * page_table[r * table_stride + i] (device int32), i = 0 .. ceil(kv_len / page_tokens) - 1. Its last query sees all its
- * keys, the one before all but the last, and so on; with window > 0 each sees the last `window` of those. A query that
- * sees none gives zeros. total_q = rows of q; max_q, max_kv: no request has more queries or keys (they only size the
- * launches; more keys than max_kv or than table_stride pages are not looked at). scale multiplies q.k. */
+ * rows [q_start[r], q_start[r + 1]) (device int32 [n_req + 1], no entry below the one before it) and kv_len[r] keys (device
+ * int32), in the pages page_table[r * table_stride + i] (device int32), i = 0 .. ceil(kv_len / page_tokens) - 1. Its last query
+ * sees all its keys, the one before all but the last, and so on; with window > 0 each sees the last `window` of those. A query
+ * that sees none gives zeros; one that sees a value that is no number gives none in that value's block of dims. out may be q
+ * itself. total_q = rows of q; max_q, max_kv: no request has more queries or keys (they only size the launches; more keys
+ * than max_kv or than table_stride pages are not looked at). scale multiplies q.k.
+ * Scores, maxima and sums are binary32. Two things have fewer bits: queries become f16 numbers times a power of two per row
+ * (both types keep all their bits down to 2^-18 of a row's largest element), and the exponentials that weigh the values are
+ * rounded to f16 once (2^-11 of each; they are summed before). */
 typedef struct bp_kv4_attn {
   bp_rows q, out;
   const void *q_start, *kv_len, *page_table;

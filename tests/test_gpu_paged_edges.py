@@ -329,3 +329,35 @@ def test_the_prompts_of_the_serving_example(ctx):
     decoded, of_prompts = paged_serving.serve(1, (700, 37, 1, 1300), seed=1)
     assert decoded <= 2.0 ** -7 + 2.0 ** -8
     assert of_prompts <= 2.0 ** -8 + 2.0 ** -11 + 2.0 ** -13
+
+
+@pytest.mark.parametrize("q", [1, 70])
+def test_queries_behind_the_rows_are_reported(ctx, q):
+    r = Requests(24, "f16", [q, q, q], [200, 150, 90], 8, 2, 64, 16)
+    want = r.run(ctx)
+    r.check(want)
+    for at, value, right in ((3, 3 * q + 2, [0, 1]), (3, (1 << 31) - 1, [0, 1]), (0, -3, [1, 2]), (0, -(1 << 31), [1, 2])):
+        starts = r.args[0].clone()
+        starts[at] = value
+        keep, r.args[0] = r.args[0], starts
+        out = r.run(ctx, max_q=q + 5)
+        with pytest.raises(bp.ContextOverflow):
+            ctx.status()
+        r.check(out, only=right)
+        r.args[0] = keep
+    # entries for nobody: as many as there are, all behind the last request
+    more = torch.cat([r.args[0], r.args[0][-1:].repeat(5)])
+    lengths = torch.cat([r.args[1], torch.tensor([0, -1, 3, 0, -9], dtype=torch.int32, device="cuda")])
+    r.args = [more, lengths, torch.cat([r.args[2], r.args[2][:1].repeat(5, 1)])]
+    assert torch.equal(r.run(ctx), want)
+    ctx.status()
+
+
+@pytest.mark.parametrize("q,kv", [(1, 9000), (5, 700), (64, 3000), (300, 2000)])
+def test_outputs_over_the_queries(ctx, q, kv):
+    """out may be q: whoever writes a row has read it, and so have the others."""
+    r = Shared(25, "bf16", [q, 1, q], [kv, 300, kv // 2], 32, 8, 128, 16)
+    want = r.run(ctx)
+    r.q = r.q.clone()
+    r.run(ctx, out=r.q)
+    assert torch.equal(r.q, want)
