@@ -95,11 +95,6 @@ __device__ __forceinline__ uint32_t oper_off(uint32_t r, uint32_t u16) {
   return (u16 >> 3) * 16384 + r * 128 + (((u16 & 7) ^ (r & 7)) << 4);
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 // ---------------------------------------------------------------------------------------------
 // Expansion of rows [0, rows_pad) of one layer: rows below m get int8 * scale (product in FP32,
 // rounded once to f16, clamped to the finite range); rows m .. rows_pad - 1 get zeros, so that a

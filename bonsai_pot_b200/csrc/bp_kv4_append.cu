@@ -15,12 +15,12 @@ namespace {
 using namespace bp;
 
 // A NaN among them is the result.
-__device__ __forceinline__ float min3(float a, float b, float c) {
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
   float r;
   asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
@@ -38,18 +38,18 @@ constexpr uint32_t MAGIC_BITS = 0x4b400000u;
 template <bool K>
 __device__ __forceinline__ uint32_t quantise8(float* x, __half* d_out, __half* m_out) {
   constexpr float LIM = 64512.f;
-  float lo = min3(min3(x[0], x[1], x[2]), min3(x[3], x[4], x[5]), min3(x[6], x[7], x[7]));
-  float hi = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[7]));
+  float lo = min3_nan(min3_nan(x[0], x[1], x[2]), min3_nan(x[3], x[4], x[5]), min3_nan(x[6], x[7], x[7]));
+  float hi = max3_nan(max3_nan(x[0], x[1], x[2]), max3_nan(x[3], x[4], x[5]), max3_nan(x[6], x[7], x[7]));
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
-    lo = min3(lo, __shfl_xor_sync(0xffffffffu, lo, o), lo);
-    hi = max3(hi, __shfl_xor_sync(0xffffffffu, hi, o), hi);
+    lo = min3_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o), lo);
+    hi = max3_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o), hi);
   }
   if (!(lo >= -LIM && hi <= LIM)) {  // rare: values beyond the limit, infinities, a NaN (which stays)
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = min3(max3(x[i], -LIM, -LIM), LIM, LIM);
-    lo = min3(max3(lo, -LIM, -LIM), LIM, LIM);
-    hi = min3(max3(hi, -LIM, -LIM), LIM, LIM);
+    for (int i = 0; i < 8; i++) x[i] = min3_nan(max3_nan(x[i], -LIM, -LIM), LIM, LIM);
+    lo = min3_nan(max3_nan(lo, -LIM, -LIM), LIM, LIM);
+    hi = min3_nan(max3_nan(hi, -LIM, -LIM), LIM, LIM);
   }
   // u = 2^(e - 10), e the exponent of the largest magnitude and a 64th: a power of two, so that * u and / u are exact
   const float top = __fmul_rn(fmaxf(fabsf(lo), fabsf(hi)), 1.015625f);

@@ -100,62 +100,62 @@ __device__ __forceinline__ void set_queries(WarpState<D, NT>& w, RawQueries<D, N
   const uint32_t g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int e = 0; e < NT; e++) {
-  const uint32_t row0 = tile0 + 8 * e, row = row0 + g;
-  float x[NB][8], big = 0.f;
-  if (row >= n_rows) {
+    const uint32_t row = tile0 + 8 * e + g;
+    float x[NB][8], big = 0.f;
+    if (row >= n_rows) {
 #pragma unroll
-    for (int b = 0; b < NB; b++) raw.u[e][b] = make_uint4(0, 0, 0, 0);
-  }
-  if (a.bf) {
-#pragma unroll
-    for (int b = 0; b < NB; b++) unpack8<true>(raw.u[e][b], x[b]);
-  } else {
-#pragma unroll
-    for (int b = 0; b < NB; b++) unpack8<false>(raw.u[e][b], x[b]);
-  }
-#pragma unroll
-  for (int b = 0; b < NB; b++)
-#pragma unroll
-    for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[b][i]));
-  big = fmaxf(big, __shfl_xor_sync(FULL, big, 1));
-  big = fmaxf(big, __shfl_xor_sync(FULL, big, 2));
-  const RowPower power = RowPower::of(big);
-  const float down = power.down(), turn = copysignf(power.up(), a.scale_log2);
-  float sum[NB];
-#pragma unroll
-  for (int b = 0; b < NB; b++) {
-    sum[b] = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const __half2 h = __floats2half2_rn(x[b][2 * j] * turn, x[b][2 * j + 1] * turn);
-      sum[b] += __low2float(h) + __high2float(h);
-      w.q[e][b][j] = u2((j & 1) ? __hmul2(h, __float2half2_rn(0.0625f)) : h);
+      for (int b = 0; b < NB; b++) raw.u[e][b] = make_uint4(0, 0, 0, 0);
     }
-    sum[b] += __shfl_xor_sync(FULL, sum[b], 1);
-    sum[b] += __shfl_xor_sync(FULL, sum[b], 2);
-    sum[b] *= a.mantissa;
-  }
-  // k slots 2 t, 2 t + 1 of the m's MMA: blocks (0, 1), (2, 3) in the high part, then the low part
-  float a0 = sum[0], a1 = sum[1];
-  if (NB == 4 && (t & 1)) {
-    a0 = sum[NB - 2];
-    a1 = sum[NB - 1];
-  }
-  const __half2 hi = __floats2half2_rn(a0, a1);
-  const __half2 lo = __floats2half2_rn(a0 - __low2float(hi), a1 - __high2float(hi));
-  const uint32_t lo_from = NB == 4 ? 2 : 1;
-  w.qsum[e] = t < lo_from ? u2(hi) : t < 2 * lo_from ? u2(lo) : 0u;
+    if (a.bf) {
 #pragma unroll
-  for (int c = 0; c < 2; c++) {
-    // (never 0: a masked score, -infinity, stays what it is)
-    w.s_scale[e][c] = fmaxf(a.power * __shfl_sync(FULL, down, 4 * (2 * t + c)), 0x1p-122f);
-    w.m[e][c] = NEG_BIG;
-    w.l[e][c] = 0.f;
-  }
+      for (int b = 0; b < NB; b++) unpack8<true>(raw.u[e][b], x[b]);
+    } else {
 #pragma unroll
-  for (int i = 0; i < 2 * NB; i++)
+      for (int b = 0; b < NB; b++) unpack8<false>(raw.u[e][b], x[b]);
+    }
 #pragma unroll
-    for (int k = 0; k < 4; k++) w.o[e][i][k] = 0.f;
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[b][i]));
+    big = fmaxf(big, __shfl_xor_sync(FULL, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(FULL, big, 2));
+    const RowPower power = RowPower::of(big);
+    const float down = power.down(), turn = copysignf(power.up(), a.scale_log2);
+    float sum[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      sum[b] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const __half2 h = __floats2half2_rn(x[b][2 * j] * turn, x[b][2 * j + 1] * turn);
+        sum[b] += __low2float(h) + __high2float(h);
+        w.q[e][b][j] = u2((j & 1) ? __hmul2(h, __float2half2_rn(0.0625f)) : h);
+      }
+      sum[b] += __shfl_xor_sync(FULL, sum[b], 1);
+      sum[b] += __shfl_xor_sync(FULL, sum[b], 2);
+      sum[b] *= a.mantissa;
+    }
+    // k slots 2 t, 2 t + 1 of the m's MMA: blocks (0, 1), (2, 3) in the high part, then the low part
+    float a0 = sum[0], a1 = sum[1];
+    if (NB == 4 && (t & 1)) {
+      a0 = sum[NB - 2];
+      a1 = sum[NB - 1];
+    }
+    const __half2 hi = __floats2half2_rn(a0, a1);
+    const __half2 lo = __floats2half2_rn(a0 - __low2float(hi), a1 - __high2float(hi));
+    const uint32_t lo_from = NB == 4 ? 2 : 1;
+    w.qsum[e] = t < lo_from ? u2(hi) : t < 2 * lo_from ? u2(lo) : 0u;
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      // (never 0: a masked score, -infinity, stays what it is)
+      w.s_scale[e][c] = fmaxf(a.power * __shfl_sync(FULL, down, 4 * (2 * t + c)), 0x1p-122f);
+      w.m[e][c] = NEG_BIG;
+      w.l[e][c] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NB; i++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) w.o[e][i][k] = 0.f;
   }
 }
 

@@ -141,11 +141,6 @@ __device__ __forceinline__ void put(const Raw<D>& w, uint8_t* tile, uint32_t row
     *reinterpret_cast<uint4*>(tile + oper_off(BN, row, 4 * b + quarter)) = expand8(codes, d, m, bias);
   }
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 // Column of O that holds dim i of a group of eight.
 __host__ __device__ constexpr int column_of(int i) { return i < 4 ? 2 * i : 2 * (i - 4) + 1; }
 

@@ -119,6 +119,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // Shared-memory loads by 32-bit shared-window address. They are ordinary C++
 // loads (the compiler may schedule them freely between barriers and knows they
 // read memory), not opaque asm.
