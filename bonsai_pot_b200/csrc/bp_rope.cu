@@ -1,9 +1,11 @@
 // Rotary positions on rows of heads, and the table they read (include/bonsai_paged.h).
 //
 // y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin for every pair of dims that turn together; the inverse turns by -angle, which
-// is the transpose and so the gradient. Bound by HBM: 2 bytes in and 2 out per value, 4 rot bytes of table per token.
-// Measured: 16383 tokens x 24 heads x 64, 18.8 us = 5.6 TB/s, 85 % of the measured copy (102.6 us with a warp per row and two bytes per lane, which
-// rows of other shapes still get); 2048 x 32 x 128, 7.8 us = 4.4 TB/s (22.3 us). One token: 6.3 us from call to call, which is its issue from Python.
+// is the transpose and so the gradient (a factor in cos and sin, as a YaRN table has, is applied either way). Moves 2 bytes in and 2 out per value, 4 rot bytes
+// of table per token, and is bound by the latency of its loads with what fits on an SM (counters: 7.6 of 10 stalled warps per issue wait for memory).
+// Measured: 16383 tokens x 24 heads x 64, 18.6 us = 5.6 TB/s of those bytes, 85 % of the rate of the measured copy; DRAM sees 62 of the 105 MB, the output stays in
+// L2 (102.6 us with a warp per row and two bytes per lane, which rows of other shapes still get); 2048 x 32 x 128, 7.8 us = 4.4 TB/s (22.3 us). One token: 6.4 us
+// from call to call, which is its issue from Python.
 #include "bp_paged.cuh"
 
 namespace {

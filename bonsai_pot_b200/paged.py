@@ -185,7 +185,8 @@ class PagedContext:
         self._check(self._lib.bp_rope_fill(self._h, _current(self._device) if stream is None else _stream(stream), C.byref(cfg), out.data_ptr()))
 
     def rope(self, x, out, positions, table, w_norm=None, eps=1e-6, inverse=False, stream=None):
-        """x [tokens, heads, head_dim] -> out (may be x): RMS norm over the head if w_norm is given, then the rotation by `positions`."""
+        """x [tokens, heads, head_dim] -> out (may be x): RMS norm over the head if w_norm is given, then the rotation by `positions`; inverse:
+        its transpose, the gradient with respect to x."""
         dtype, device = _dtype(x), self._device
         _rows(self._a, x, "x", device)
         _like(out, x, "out")

@@ -66,10 +66,11 @@ typedef struct bp_rope_config {
 /* Fills a table on the device, in binary64, rounded once. */
 int bp_rope_fill(bp_paged_ctx* ctx, void* stream, const bp_rope_config* cfg, void* table_out);
 
-/* x rows -> out rows (the same memory, or memory that does not overlap): an RMS norm over the head first if w_norm (activation type,
- * [head_dim]) is given, then the rotation by positions[token] (device int32); inverse != 0 turns back, which is the
- * gradient with respect to x (not with w_norm). head_dim even, <= 256; n_tok * n_head <= 2^28. Tokens with a negative position are padding: their
- * rows are not written. */
+/* x rows -> out rows (the same memory, or memory that does not overlap): an RMS norm over the head first if w_norm (activation
+ * type, [head_dim]) is given, then the rotation by positions[token] (device int32). inverse != 0 is its transpose, by minus
+ * the angle and with the same factor: the gradient with respect to x (not with w_norm). With a table of cos^2 + sin^2 = 1 it
+ * undoes the rotation; a BP_ROPE_SCALE_YARN table's factor it applies once more. head_dim even, <= 256; n_tok * n_head
+ * <= 2^28. Tokens with a negative position are padding: their rows are not written. */
 typedef struct bp_rows {
   void* data;
   int64_t tok_stride, head_stride;

@@ -361,3 +361,28 @@ def test_outputs_over_the_queries(ctx, q, kv):
     r.q = r.q.clone()
     r.run(ctx, out=r.q)
     assert torch.equal(r.q, want)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dim,rot", [(64, 64), (128, 32), (20, 8)])
+def test_rope_inverse_of_a_table_with_a_factor(ctx, layout, dim, rot):
+    """A YaRN table's cos and sin have a factor: the inverse is the transpose still, <rope(x), y> = <x, inverse(y)>, and undoes the rotation but for
+    the factor's square."""
+    factor = 8.0
+    tab = torch.empty(300, rot // 2, 2, device="cuda")
+    ctx.fill_rope(tab, scaling="yarn", factor=factor, orig_ctx=64)
+    table, pos = bp.RopeTable(tab, layout), torch.tensor([0, 17, 299], dtype=torch.int32, device="cuda")
+    x, y = normal(1, (3, 2, dim), "f16"), normal(2, (3, 2, dim), "f16")
+    rx, iy, back = (torch.empty_like(x) for _ in range(3))
+    ctx.rope(x, rx, pos, table)
+    ctx.rope(y, iy, pos, table, inverse=True)
+    ctx.rope(rx, back, pos, table, inverse=True)
+    left, right = (f64(rx) * f64(y)).sum(-1), (f64(x) * f64(iy)).sum(-1)
+    size = (np.abs(f64(rx) * f64(y)) + np.abs(f64(x) * f64(iy))).sum(-1)
+    assert (np.abs(left - right) <= 2.0 ** -10 * size).all()  # both sides are sums of terms with one rounding to f16 each
+    want = f64(x)
+    p1, p2 = R.pairs(rot, layout)
+    for p in (p1, p2):
+        want[..., p] *= (0.1 * np.log(factor) + 1) ** 2
+    near = np.abs(f64(rx)).max(-1, keepdims=True)
+    assert (np.abs(f64(back) - want) <= 2.0 ** -9 * near * 1.3).all()  # rx and back are rounded to f16 once each, next to values of that size
