@@ -40,17 +40,18 @@ def _bad(text):
     raise ConfigError("invalid config: " + text)
 
 
-def _dtype(t):
-    code = _DTYPES.get(t.dtype)
+def _code(dtype):
+    code = _DTYPES.get(dtype)
     if code is None:
         _types()
-        code = _DTYPES.get(t.dtype)
+        code = _DTYPES.get(dtype)
         if code is None:
-            _bad(f"rows are float16 or bfloat16, not {t.dtype}")
+            _bad(f"rows are float16 or bfloat16, not {dtype}")
     return code
 
 
-# The checks below are on the path of every call (a decoded token makes three of them per layer), hence as few tensor methods as will do.
+# The checks below are on the path of every call (a decoded token makes three of them per layer), hence as few tensor methods as will do (each
+# takes 50 to 130 ns, and a shape is made anew whenever it is asked for).
 def _elsewhere(t, what, device):
     """An address of host memory or of another device must not reach a kernel."""
     _bad(f"{what} must be on cuda:{device}, not on {t.device}")
@@ -69,9 +70,9 @@ def _rows(to, t, what, device):
     to.data = t.data_ptr()
 
 
-def _like(t, rows, what):
-    if t.dtype is not rows.dtype or t.shape != rows.shape:
-        _bad(f"{what} must have the shape and type of the rows it goes with: {tuple(t.shape)} {t.dtype}, not {tuple(rows.shape)} {rows.dtype}")
+def _like(t, dtype, shape, what):
+    if t.dtype is not dtype or t.shape != shape:
+        _bad(f"{what} must have the shape and type of the rows it goes with: {tuple(t.shape)} {t.dtype}, not {tuple(shape)} {dtype}")
 
 
 def _index(t, what, n, device, slots=False):
@@ -82,11 +83,11 @@ def _index(t, what, n, device, slots=False):
     return t.data_ptr()
 
 
-def _weight(w, rows, what, device):
+def _weight(w, dtype, dim, what, device):
     if w.get_device() != device:
         _elsewhere(w, what, device)
-    if w.dtype is not rows.dtype or w.numel() != rows.shape[2] or not w.is_contiguous():
-        _bad(f"{what} must be {rows.shape[2]} dense values of the rows' type")
+    if w.dtype is not dtype or w.numel() != dim or not w.is_contiguous():
+        _bad(f"{what} must be {dim} dense values of the rows' type")
     return w.data_ptr()
 
 
@@ -187,48 +188,50 @@ class PagedContext:
     def rope(self, x, out, positions, table, w_norm=None, eps=1e-6, inverse=False, stream=None):
         """x [tokens, heads, head_dim] -> out (may be x): RMS norm over the head if w_norm is given, then the rotation by `positions`; inverse:
         its transpose, the gradient with respect to x."""
-        dtype, device = _dtype(x), self._device
+        dtype, shape, device = x.dtype, x.shape, self._device
+        code = _code(dtype)
         _rows(self._a, x, "x", device)
-        _like(out, x, "out")
+        _like(out, dtype, shape, "out")
         _rows(self._b, out, "out", device)
         if table.device != device:
             _elsewhere(table.data, "the RoPE table", device)
-        n, heads, dim = x.shape
-        st = self._lib.bp_rope(self._h, _current(device) if stream is None else _stream(stream), dtype, self._pa, self._pb, n, heads, dim, _index(positions, "positions", n, device), table._p,
-                               None if w_norm is None else _weight(w_norm, x, "w_norm", device), eps, inverse)
+        n, heads, dim = shape
+        st = self._lib.bp_rope(self._h, _current(device) if stream is None else _stream(stream), code, self._pa, self._pb, n, heads, dim, _index(positions, "positions", n, device), table._p,
+                               None if w_norm is None else _weight(w_norm, dtype, dim, "w_norm", device), eps, inverse)
         if st:
             self._check(st)
 
     def append(self, pool, k, v, positions, slots, table=None, w_k_norm=None, eps=1e-6, stream=None):
         """k, v [tokens, KV heads, head_dim] -> the pool at `slots`; K is normalised (w_k_norm) and rotated (table) on the way."""
-        dtype, n, device = self._kv(pool, k, v)
+        code, n, device = self._kv(pool, k, v)
         if table is not None and table.device != device:
             _elsewhere(table.data, "the RoPE table", device)
-        st = self._lib.bp_kv4_append(self._h, _current(device) if stream is None else _stream(stream), dtype, pool._p, self._pa, self._pb, n,
+        st = self._lib.bp_kv4_append(self._h, _current(device) if stream is None else _stream(stream), code, pool._p, self._pa, self._pb, n,
                                      None if positions is None else _index(positions, "positions", n, device), _index(slots, "slots", n, device, True),
-                                     None if table is None else table._p, None if w_k_norm is None else _weight(w_k_norm, k, "w_k_norm", device), eps)
+                                     None if table is None else table._p, None if w_k_norm is None else _weight(w_k_norm, k.dtype, pool.head_dim, "w_k_norm", device), eps)
         if st:
             self._check(st)
 
     def read(self, pool, slots, k, v, stream=None):
         """The pool's rows at `slots` -> k, v [tokens, KV heads, head_dim]; keys are as they were stored."""
-        dtype, n, device = self._kv(pool, k, v)
-        st = self._lib.bp_kv4_read(self._h, _current(device) if stream is None else _stream(stream), dtype, pool._p, _index(slots, "slots", n, device, True), n, self._pa, self._pb)
+        code, n, device = self._kv(pool, k, v)
+        st = self._lib.bp_kv4_read(self._h, _current(device) if stream is None else _stream(stream), code, pool._p, _index(slots, "slots", n, device, True), n, self._pa, self._pb)
         if st:
             self._check(st)
 
     def attention(self, pool, q, out, q_start, kv_len, page_table, max_q, max_kv, scale=None, window=0, stream=None):
         """q [tokens of all requests, heads, head_dim] -> out. Request r has the rows q_start[r] .. q_start[r + 1] and sees kv_len[r] keys in
         the pages page_table[r]; max_q, max_kv: no request has more. scale: 1 / sqrt(head_dim) if None; window: 0 = none."""
-        dtype, a, device = _dtype(q), self._attn, self._device
+        dtype, shape, a, device = q.dtype, q.shape, self._attn, self._device
+        code = _code(dtype)
         _rows(self._q, q, "q", device)
-        _like(out, q, "out")
+        _like(out, dtype, shape, "out")
         _rows(self._o, out, "out", device)
         if pool.device != device:
             _elsewhere(pool.data, "the pool", device)
         if page_table.get_device() != device:
             _elsewhere(page_table, "page_table", device)
-        n, heads, dim = q.shape
+        n, heads, dim = shape
         if dim != pool.head_dim:
             _bad(f"q has head_dim {dim}, the pool {pool.head_dim}")
         if page_table.dtype is not _I32 or page_table.dim() != 2:
@@ -250,18 +253,19 @@ class PagedContext:
         a.window = window if window < max_kv else 0  # (a window over all keys is none)
         a.table_stride = pitch
         a.scale = dim ** -0.5 if scale is None else scale
-        st = self._lib.bp_kv4_attention(self._h, _current(device) if stream is None else _stream(stream), dtype, pool._p, self._pattn)
+        st = self._lib.bp_kv4_attention(self._h, _current(device) if stream is None else _stream(stream), code, pool._p, self._pattn)
         if st:
             self._check(st)
 
     def _kv(self, pool, k, v):
-        dtype, device = _dtype(k), self._device
+        dtype, shape, device = k.dtype, k.shape, self._device
+        code = _code(dtype)
         _rows(self._a, k, "k", device)
-        _like(v, k, "v")
+        _like(v, dtype, shape, "v")
         _rows(self._b, v, "v", device)
         if pool.device != device:
             _elsewhere(pool.data, "the pool", device)
-        n, heads, dim = k.shape
+        n, heads, dim = shape
         if heads != pool.n_kv_head or dim != pool.head_dim:
             _bad(f"the pool holds {pool.n_kv_head} heads of {pool.head_dim}, the rows have {heads} of {dim}")
-        return dtype, n, device
+        return code, n, device
