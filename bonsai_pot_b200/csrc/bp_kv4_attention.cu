@@ -623,8 +623,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* const buf = smem + warp * RING * S::PART;
   const uint32_t buf_at = smem_u32(buf), bar = smem_u32(&bars[warp][0]);
-  if (lane < RING) mbar_init(bar + 8 * lane, 1);
-  if (lane == 0) fence_barrier_init();
+  if (lane < RING) {
+    mbar_init(bar + 8 * lane, 1);
+    fence_barrier_init();  // (by whoever made one)
+  }
   if (lane < 2) pieces[2 * warp + lane].used = 0;
   if (threadIdx.x == 0) items_s = most_s = 0;
   __syncthreads();

@@ -25,3 +25,15 @@ def test_the_lanes_of_a_warp_decide_together_whether_a_wait_gave_up():
         assert len(waits) >= 2
         for line in waits:
             assert form in line, line
+
+
+def test_who_makes_a_barrier_fences_it():
+    """A fence orders the barriers that its own thread has made before the copies that arrive on them; another thread's does not."""
+    src = code("bp_kv4_attention.cu")
+    assert src.count("mbar_init(") == src.count("fence_barrier_init(") == 1
+    assert re.search(r"if \(lane < RING\) \{\s*mbar_init\([^\n]*\);\s*fence_barrier_init\(\);\s*\}", src)
+    src = code("bp_kv4_prefill.cu")
+    blocks = re.findall(r"if \(threadIdx\.x == 0\) \{\n((?:    [^\n]*\n)+)  ?(?:  )?\}", src)
+    made = [b for b in blocks if "mbar_init(" in b]
+    assert len(made) == 2 and all("fence_barrier_init();" in b for b in made)
+    assert sum(b.count("mbar_init(") for b in made) == src.count("mbar_init(")
