@@ -14,10 +14,13 @@
 // one that comes last, in the order of its keys (as in bp_kv4_attention.cu). Every wait is bounded; a timeout sets the context's error word and
 // the CTA winds down and frees its TMEM.
 //
-// Bound by the expanders: of the some 2500 cycles of a tile of 64 keys and 256 rows the S issuers wait most for K (the MMAs alone would take about
-// 1450 at the measured rate of a library product). 2048 queries behind 32768 keys, 32 / 8 heads of 128: 1.22 ms, 872 TFLOP/s, 53 % of that rate
+// P is f16 because V is (see bp_kv4_attention.cu).
+//
+// Bound by the softmax warps: of the some 2340 cycles of a tile of 64 keys and 256 rows (clocks read in a copy of the kernel) they wait 250 for S, while the S issuers wait
+// 1600 for a free buffer, the O issuers 1770 for P, and the expanders 490 for free slots. The row exponentials alone take 1024 cycles at 16 per cycle and SM, the MMAs
+// would take about 1450 at the measured rate of a library product. 2048 queries behind 32768 keys, 32 / 8 heads of 128: 1.21 ms, 881 TFLOP/s, 54 % of that rate
 // (floor 0.65 ms). Four expander warps whose page ids were waited for took 1.39 ms; eight of them, with two softmax threads per row, 1.38; with one softmax
-// thread per row 1.25; with whole lines read and one barrier per slot 1.23. 4 requests of up to 512 queries behind up to 4099 keys: 96 us (floor 32): a tile costs the
+// thread per row 1.25; with whole lines read and one barrier per slot 1.23. 4 requests of up to 512 queries behind up to 4099 keys: 97 us (floor 32): a tile costs the
 // same, beginning and ending an item about 14 us; before the line weighted items and the partial results had whole-warp accesses it was 216.
 #include <type_traits>
 
