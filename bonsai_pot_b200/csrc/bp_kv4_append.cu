@@ -4,7 +4,7 @@
 // step is an explicitly rounded binary32 operation in a fixed order, so that a token's bytes do not depend on what else is
 // in the batch and a plain program can reproduce them. 4 D bytes in, 1.25 D out per (token, KV head).
 // Measured: 16383 tokens x 8 heads x 128 appended and read back 47 us (floor 27.5 at the measured copy rate): about 30 for the append, bound by instruction
-// issue (72 % of the slots: five per code, the tree of squares, the rotation), 17 for the read-back, bound by the latency of slot -> row. With
+// issue (71 % of the slots: five per code, the tree of squares, the rotation), 17 for the read-back, bound by the latency of slot -> row. With
 // narrower loads and stores and codes rounded by conversions it was 56.
 // A row of D dims is D / 16 lanes: lane c has the eight dims of chunk c (8 c ..) and the eight of chunk c + D / 16, so that with
 // the half layout over whole heads the two dims that turn together are in one lane, and a block is four lanes.
