@@ -7,9 +7,9 @@ from .errors import (ConfigError, ContextOverflow, CudaError, DeviceLost, Device
 from .attention import AttnContext  # noqa: F401
 from .kv_snapshot import KvSnapshot  # noqa: F401
 from .errors import IoError  # noqa: F401
-from .paged import KV4Pool, PagedContext, RopeTable  # noqa: F401
+from .paged import BlockSummary, KV4Pool, KV4Pools, PagedContext, PageTables, RopeTable  # noqa: F401
 from .model import GenerateOptions, Model, Sampler, Session, StopReason  # noqa: F401
 
 __all__ = ["AttnContext", "KvSnapshot", "PotError", "ConfigError", "ContextOverflow", "PrefillTooLarge",
            "DeviceLost", "CudaError", "DeviceTimeout", "IoError", "Model", "Session", "Sampler", "GenerateOptions", "StopReason",
-           "PagedContext", "KV4Pool", "RopeTable"]
+           "PagedContext", "KV4Pool", "KV4Pools", "PageTables", "BlockSummary", "RopeTable"]

@@ -17,10 +17,11 @@ LIB_PATH = os.path.join(HERE, "libbonsai_attn.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "bonsai_attn.h")
 MODEL_HEADER = os.path.join(os.path.dirname(HERE), "include", "bonsai_model.h")
 PAGED_HEADER = os.path.join(os.path.dirname(HERE), "include", "bonsai_paged.h")
+PAGES_HEADER = os.path.join(os.path.dirname(HERE), "include", "bonsai_pages.h")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-shared", "-Xcompiler", "-fPIC", "--threads", "0",
 ]
 
 
@@ -32,7 +33,7 @@ def needs_build() -> bool:
     if not os.path.exists(LIB_PATH):
         return True
     built = os.path.getmtime(LIB_PATH)
-    deps = sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + [HEADER, MODEL_HEADER, PAGED_HEADER]
+    deps = sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + [HEADER, MODEL_HEADER, PAGED_HEADER, PAGES_HEADER]
     return any(os.path.getmtime(p) > built for p in deps)
 
 
@@ -217,6 +218,57 @@ PAGED_SIGNATURES = {
     "bp_kv4_attention": (_int, [_vp, _vp, _u32, _vp, _vp]),
 }
 
+
+
+class PageTablesStruct(C.Structure):
+    """`bp_page_tables` of include/bonsai_pages.h."""
+    _fields_ = [("table", C.c_void_p), ("kv_len", C.c_void_p), ("refs", C.c_void_p)] + \
+               [(k, C.c_uint32) for k in ("n_rows", "row_pages", "table_stride", "n_pages", "page_tokens")]
+
+
+class PageArrayStruct(C.Structure):
+    """`bp_page_array` of include/bonsai_pages.h."""
+    _fields_ = [("data", C.c_void_p), ("page_bytes", C.c_uint64)]
+
+
+class SharedStruct(C.Structure):
+    """`bp_kv4_shared` of include/bonsai_pages.h."""
+    _fields_ = [("q", RowsStruct), ("out", RowsStruct)] + \
+               [(k, C.c_void_p) for k in ("q_start", "kv_len", "page_table", "prefix_start", "prefix_len", "prefix_table", "work")] + \
+               [(k, C.c_uint32) for k in ("n_req", "n_head", "total_q", "max_q", "max_kv", "table_stride", "n_prefix", "max_prefix", "prefix_stride")] + [("scale", C.c_float)]
+
+
+class SummaryStruct(C.Structure):
+    """`bp_block_summary` of include/bonsai_pages.h."""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p)]
+
+
+class ChoiceStruct(C.Structure):
+    """`bp_kv4_choice` of include/bonsai_pages.h."""
+    _fields_ = [("q", RowsStruct)] + [(k, C.c_void_p) for k in ("q_start", "kv_len", "page_table", "pages", "keys")] + \
+               [(k, C.c_uint32) for k in ("n_req", "n_head", "total_q", "max_q", "max_kv", "table_stride", "chosen", "first", "last")]
+
+
+class ChosenStruct(C.Structure):
+    """`bp_kv4_chosen` of include/bonsai_pages.h."""
+    _fields_ = [("q", RowsStruct), ("out", RowsStruct), ("pages", C.c_void_p), ("keys", C.c_void_p)] + \
+               [(k, C.c_uint32) for k in ("n_head", "total_q", "chosen")] + [("scale", C.c_float)]
+
+
+# name -> (restype, argtypes); must list every symbol include/bonsai_pages.h declares. Structs go by address, as above.
+PAGES_SIGNATURES = {
+    "bp_pages_grow": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32]),
+    "bp_pages_release": (_int, [_vp, _vp, _vp, _vp, _u32]),
+    "bp_pages_fork": (_int, [_vp, _vp, _vp, _vp, _vp, _u32, _vp, _vp]),
+    "bp_pages_compact": (_int, [_vp, _vp, _vp, _vp, _vp, _u32]),
+    "bp_pages_copy": (_int, [_vp, _vp, _vp, _u32, _u32, _vp, _vp, _u32]),
+    "bp_kv4_shared_work": (_u64, [_u32, _u32, _u32]),
+    "bp_kv4_attention_shared": (_int, [_vp, _vp, _u32, _vp, _vp]),
+    "bp_kv4_summarise": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _u32]),
+    "bp_kv4_select": (_int, [_vp, _vp, _u32, _vp, _vp, _vp]),
+    "bp_kv4_attention_selected": (_int, [_vp, _vp, _u32, _vp, _vp]),
+}
+
 _LIB = None
 
 
@@ -233,7 +285,7 @@ def load() -> C.CDLL:
             if not os.path.exists(LIB_PATH):
                 raise ImportError(f"libbonsai_attn.so is missing and could not be built: {e}") from e
     lib = C.CDLL(path)
-    for name, (res, args) in [*SIGNATURES.items(), *MODEL_SIGNATURES.items(), *PAGED_SIGNATURES.items()]:
+    for name, (res, args) in [*SIGNATURES.items(), *MODEL_SIGNATURES.items(), *PAGED_SIGNATURES.items(), *PAGES_SIGNATURES.items()]:
         fn = getattr(lib, name)  # AttributeError here = the header and the library disagree
         fn.restype = res
         fn.argtypes = args

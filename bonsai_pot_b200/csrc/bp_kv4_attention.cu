@@ -274,7 +274,7 @@ __device__ __forceinline__ void values16(WarpState<D, NT>& w, const uint8_t* buf
 }
 
 // P, still as the S^T fragments of four tiles, from the scores: masks (cut: some row may not see all of the unit, of which `left` keys are there), maximum, exponentials, sums; O is rescaled.
-template <int D, int NT>
+template <int D, int NT, int MODE>
 __device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4][4], bool cut, int left, uint32_t tile0, int q_len, const AttnArgs& a, uint32_t lane) {
   constexpr int NB = D / 32;
   const uint32_t g = lane >> 2;
@@ -284,7 +284,7 @@ __device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4]
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         // the keys of the unit that row 2 t + c sees are [lo, hi); columns behind the request's rows are left as they are, nobody reads them
-        const int behind = q_len - 1 - static_cast<int>((tile0 + 8 * e + 2 * (lane & 3) + c) / a.group);  // queries behind this one
+        const int behind = MODE == PREFIX ? 0 : q_len - 1 - static_cast<int>((tile0 + 8 * e + 2 * (lane & 3) + c) / a.group);  // queries behind this one
         const int hi = behind < 0 ? left : left - behind, lo = a.window && behind >= 0 ? hi - static_cast<int>(a.window) : 0;
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -352,14 +352,14 @@ struct Request {
   uint32_t units, tiles;       // units of 64 keys of an item; items per KV head (none without keys: there are only zeros to write)
   __device__ int first() const { return low & ~static_cast<int>(UNIT - 1); }
 };
-template <int NT>
+template <int NT, int MODE>
 __device__ __forceinline__ Request request(const AttnArgs& a, uint32_t r, bool report) {
   Request q;
-  const Lengths n = lengths_of(a, r, report);
+  const Lengths n = lengths_of<MODE>(a, r, report);
   q.q0 = n.q0;
   q.q_len = n.q_len;
   q.kv_len = n.kv_len;
-  q.low = min(first_seen(q.kv_len - q.q_len + 1, a.window), q.kv_len);
+  q.low = MODE == PREFIX ? 0 : min(first_seen(q.kv_len - q.q_len + 1, a.window), q.kv_len);
   q.units = (static_cast<uint32_t>(q.kv_len - q.first()) + UNIT - 1) / UNIT;
   q.tiles = q.kv_len ? (static_cast<uint32_t>(q.q_len) * a.group + 8 * NT - 1) / (8 * NT) : 0;
   return q;
@@ -371,7 +371,7 @@ struct Cursor {
   uint32_t r, head, tile, unit;
 };
 // The next item (a cursor lies in shared memory, one lane moves it). known: the requests, or null if there are too many.
-template <int NT>
+template <int NT, int MODE>
 __device__ __forceinline__ void next_item(Cursor& c, const AttnArgs& a, const Request* known) {
   c.unit = 0;
   if (++c.tile < c.q.tiles) return;
@@ -380,7 +380,7 @@ __device__ __forceinline__ void next_item(Cursor& c, const AttnArgs& a, const Re
   c.head = 0;
   do {
     if (++c.r >= a.n_req) return;
-    c.q = known ? known[c.r] : request<NT>(a, c.r, false);
+    c.q = known ? known[c.r] : request<NT, MODE>(a, c.r, false);
   } while (c.q.tiles == 0);
 }
 
@@ -415,25 +415,25 @@ __device__ __forceinline__ void copy_pages(uint32_t pages, const uint8_t* src, u
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + lane * bytes), "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
 }
-template <uint32_t PAGE>
-__device__ __forceinline__ void load_ids(Fetch& f, const AttnArgs& a, uint32_t r, uint32_t lane) {
+template <uint32_t PAGE, int MODE>
+__device__ __forceinline__ void load_ids(Fetch& f, const AttnArgs& a, const Cursor& c, uint32_t lane) {
   f.base = static_cast<uint32_t>(f.key0) / PAGE;
   f.ids = 0xffffffffu;
-  if (f.base + lane < (static_cast<uint32_t>(f.kv_len) + PAGE - 1) / PAGE) f.ids = static_cast<uint32_t>(a.page_table[static_cast<size_t>(r) * a.table_stride + f.base + lane]);
+  if (f.base + lane < (static_cast<uint32_t>(f.kv_len) + PAGE - 1) / PAGE) f.ids = static_cast<uint32_t>(a.page_table[(MODE == CHOSEN ? static_cast<size_t>(c.r) * a.pool.n_kv_head + c.head : c.r) * a.table_stride + f.base + lane]);
 }
-template <uint32_t PAGE>
+template <uint32_t PAGE, int MODE>
 __device__ __forceinline__ void start_item(Fetch& f, const AttnArgs& a, const Cursor& c, uint32_t lane) {
   f.key0 = c.q.first() + static_cast<int>(c.unit * UNIT);
   f.kv_len = c.q.kv_len;
   f.low = c.q.low;
   f.rem = c.q.units - c.unit;
-  load_ids<PAGE>(f, a, c.r, lane);
+  load_ids<PAGE, MODE>(f, a, c, lane);
 }
-template <int D, uint32_t PAGE>
+template <int D, uint32_t PAGE, int MODE>
 __device__ __forceinline__ void fetch_keys(Fetch& f, const AttnArgs& a, const Cursor& c, Unit& info, uint32_t dst, uint32_t bar, uint32_t lane) {
   constexpr uint32_t N = UNIT / PAGE, BYTES = PAGE * (PoolLayout<D>::TOK / 2);
   const uint32_t page0 = static_cast<uint32_t>(f.key0) / PAGE;
-  if (page0 - f.base >= 32) load_ids<PAGE>(f, a, c.r, lane);
+  if (page0 - f.base >= 32) load_ids<PAGE, MODE>(f, a, c, lane);
   const uint32_t id = __shfl_sync(FULL, f.ids, (page0 - f.base + lane) & 31);
   const int key = f.key0 + static_cast<int>(lane * PAGE);
   const bool there = lane < N && key < f.kv_len && key + static_cast<int>(PAGE) > f.low, good = there && id < a.pool.n_pages;
@@ -508,7 +508,7 @@ __device__ __noinline__ uint32_t take_no_numbers(uint8_t* buf, int left, uint32_
 }
 
 // A warp: row `row` of the `n` partial results at part(k) of an item, in order, becomes the output's row.
-template <int D, int NT, typename Part>
+template <int D, int NT, int MODE, typename Part>
 __device__ __forceinline__ void join_row(const AttnArgs& a, const Piece& p, uint32_t row, uint32_t n, Part part, uint32_t lane) {
   using S = Shape<D, NT>;
   constexpr int V = D / 32;  // dims of a lane
@@ -545,6 +545,13 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, const Piece& p, uint
       }
     }
   }
+  if constexpr (in_parts(MODE)) {
+    const size_t at = part_row(a, p.q0, p.head, p.row0 + row);
+#pragma unroll
+    for (int x = 0; x < V; x++) a.part[at * D + V * lane + x] = o[x];
+    if (lane == 0) a.part_ml[at] = make_float2(m, l);
+    return;
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* out = out_row(a, p.q0, p.head, p.row0 + row) + V * lane;
   if constexpr (V == 4) {
@@ -558,7 +565,7 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, const Piece& p, uint
 
 // The same of four rows at a time, eight lanes each, for few partial results, one after the other; into the output (to == null) or the partial
 // result `to`.
-template <int D, int NT, typename Part>
+template <int D, int NT, int MODE, typename Part>
 __device__ __forceinline__ void join_rows4(const AttnArgs& a, const Piece& p, uint32_t row0, uint32_t n, Part part, float* to, uint32_t lane) {
   using S = Shape<D, NT>;
   constexpr int V = D / 32;  // fours of dims of a lane
@@ -587,15 +594,26 @@ __device__ __forceinline__ void join_rows4(const AttnArgs& a, const Piece& p, ui
     if ((lane & 7) == 0) *reinterpret_cast<float2*>(to + at + D) = make_float2(m, l);
     return;
   }
+  if constexpr (in_parts(MODE)) {
+    const size_t where = part_row(a, p.q0, p.head, p.row0 + row);
+#pragma unroll
+    for (int x = 0; x < V; x++) *reinterpret_cast<float4*>(a.part + where * D + 32 * x + col) = o[x];
+    if ((lane & 7) == 0) a.part_ml[where] = make_float2(m, l);
+    return;
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* out = out_row(a, p.q0, p.head, p.row0 + row) + col;
 #pragma unroll
   for (int x = 0; x < V; x++) store4(a.bf, out + 32 * x, o[x].x * inv, o[x].y * inv, o[x].z * inv, o[x].w * inv);
 }
 
-// Zeros for the `n_tok` tokens of a request without keys, by a CTA. (Their values can be more than 32 bits count.)
-template <int D>
+// Zeros for the `n_tok` tokens of a request without keys, by a CTA. (Their values can be more than 32 bits count.) In parts: no weights.
+template <int D, int MODE>
 __device__ __noinline__ void zero_rows(const AttnArgs& a, int q0, uint32_t n_tok) {
+  if constexpr (in_parts(MODE)) {
+    for (size_t i = threadIdx.x; i < static_cast<size_t>(n_tok) * a.n_head; i += blockDim.x) a.part_ml[static_cast<size_t>(q0) * a.n_head + i] = make_float2(NEG_BIG, 0.f);
+    return;
+  }
   const uint32_t step = blockDim.x / (D / 4), dt = step / a.n_head, dh = step % a.n_head;  // rows that the CTA writes at a time
   const uint32_t row = threadIdx.x / (D / 4);
   for (uint32_t t = row / a.n_head, h = row % a.n_head; t < n_tok;) {
@@ -609,7 +627,7 @@ __device__ __noinline__ void zero_rows(const AttnArgs& a, int q0, uint32_t n_tok
   }
 }
 
-template <int D, int NT, uint32_t PAGE>
+template <int D, int NT, uint32_t PAGE, int MODE>
 __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel(const __grid_constant__ AttnArgs a, float* __restrict__ scratch, uint32_t* __restrict__ counters) {
   using S = Shape<D, NT>;
   using L = PoolLayout<D>;
@@ -643,7 +661,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
   {
     uint32_t units = 0, items = 0, most = 0;
     for (uint32_t r = threadIdx.x * per; r < min((threadIdx.x + 1) * per, a.n_req); r++) {
-      const Request q = request<NT>(a, r, blockIdx.x == 0);
+      const Request q = request<NT, MODE>(a, r, blockIdx.x == 0);
       if (known) requests[r] = q;
       items += q.tiles * a.pool.n_kv_head;
       if (q.tiles) most = max(most, q.units);
@@ -683,7 +701,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
     if (lane == 0) {
       uint32_t left = at ? x - line[at] : x;
       for (uint32_t r = at * per; r < a.n_req; r++) {
-        const Request q = known ? known[r] : request<NT>(a, r, false);
+        const Request q = known ? known[r] : request<NT, MODE>(a, r, false);
         const uint32_t n = q.tiles * a.pool.n_kv_head * q.units;
         if (left >= n) {
           left -= n;
@@ -701,8 +719,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
     __syncwarp();
   };
   for (uint32_t r = blockIdx.x; r < a.n_req; r += n_cta) {
-    const Request q = known ? known[r] : request<NT>(a, r, false);
-    if (q.kv_len == 0) zero_rows<D>(a, q.q0, q.q_len);
+    const Request q = known ? known[r] : request<NT, MODE>(a, r, false);
+    if (q.kv_len == 0) zero_rows<D, MODE>(a, q.q0, q.q_len);
   }
   // One item per CTA where that takes at most one round of the warps more than equal stretches, which need their pieces
   // joined; else equal stretches, of one unit per warp at least.
@@ -713,7 +731,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
     if (blockIdx.x < items_s) {
       uint32_t left = blockIdx.x;
       for (uint32_t r = 0; r < a.n_req; r++) {
-        const Request q = known ? known[r] : request<NT>(a, r, false);
+        const Request q = known ? known[r] : request<NT, MODE>(a, r, false);
         const uint32_t n = q.tiles * a.pool.n_kv_head;
         if (left < n) {
           c0 += left * q.units;
@@ -745,7 +763,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
     Fetch f;
     uint32_t asked = 1, nb = 0, flying = 0;  // units asked for; the buffer (and its barrier) that is filled next; filled ones
     auto fetch_k = [&]() {       // of unit asked - 1
-      fetch_keys<D, PAGE>(f, a, next, infos[warp][(asked - 1) & 3], buf_at + nb * S::PART, bar + 8 * nb, lane);
+      fetch_keys<D, PAGE, MODE>(f, a, next, infos[warp][(asked - 1) & 3], buf_at + nb * S::PART, bar + 8 * nb, lane);
       if (++nb == RING) nb = 0;
       flying++;
     };
@@ -760,14 +778,14 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
         f.rem--;
         f.key0 += UNIT;
       } else {
-        if (lane == 0) next_item<NT>(next, a, known);
+        if (lane == 0) next_item<NT, MODE>(next, a, known);
         __syncwarp();
-        start_item<PAGE>(f, a, next, lane);
+        start_item<PAGE, MODE>(f, a, next, lane);
       }
     };
     RawQueries<D, NT> raw;
     ask_queries<D, NT>(raw, a, cur.head, cur.tile * S::ROWS, cur.q.q_len * a.group, cur.q.q0, lane);
-    start_item<PAGE>(f, a, next, lane);
+    start_item<PAGE, MODE>(f, a, next, lane);
     fetch_k();
     fetch_v();
     if (n > 1) {
@@ -813,14 +831,15 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
         fetch_k();
       }
       const int q_len = cur.q.q_len;
-      const bool cut = u.left - static_cast<int>(UNIT) < q_len - 1 || (a.window && u.left > static_cast<int>(a.window));
-      softmax64<D, NT>(w, s, cut, u.left, cur.tile * S::ROWS, q_len, a, lane);
+      // (every row of a prefix sees the same keys)
+      const bool cut = MODE == PREFIX ? u.left < static_cast<int>(UNIT) : u.left - static_cast<int>(UNIT) < q_len - 1 || (a.window && u.left > static_cast<int>(a.window));
+      softmax64<D, NT, MODE>(w, s, cut, u.left, cur.tile * S::ROWS, q_len, a, lane);
       ok = wait();
       if (!ok) break;
       {
         uint8_t* vb = buf + b * S::PART;
         if (part) clear_scales<D, PAGE>(vb, u.pages, u.low, u.left);
-        if (cut && q_len > 1 && __any_sync(FULL, (blocks_without_numbers<D, PAGE>(vb, lane) | blocks_without_numbers<D, PAGE>(vb, lane + 32)) != 0)) {
+        if (MODE != PREFIX && cut && q_len > 1 && __any_sync(FULL, (blocks_without_numbers<D, PAGE>(vb, lane) | blocks_without_numbers<D, PAGE>(vb, lane + 32)) != 0)) {
           const uint32_t spoiled = take_no_numbers<D, NT, PAGE>(vb, u.left, cur.tile * S::ROWS, q_len, a.group, a.window);
 #pragma unroll
           for (int e = 0; e < NT; e++)
@@ -856,6 +875,14 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
             for (int c = 0; c < 2; c++) {
               const uint32_t row = row0 + 8 * e + 2 * t + c;
               if (row >= n_rows) continue;
+              if constexpr (in_parts(MODE)) {
+                const size_t at = part_row(a, cur.q.q0, cur.head, row);
+#pragma unroll
+                for (int x = 0; x < NB; x++)
+                  *reinterpret_cast<float4*>(a.part + at * D + 32 * x + 4 * g) = make_float4(w.o[e][2 * x][c], w.o[e][2 * x][c + 2], w.o[e][2 * x + 1][c], w.o[e][2 * x + 1][c + 2]);
+                if (g == 0) a.part_ml[at] = make_float2(w.m[e][c], w.l[e][c]);
+                continue;
+              }
               const float inv = w.l[e][c] == 0.f ? 0.f : 1.f / w.l[e][c];
               uint16_t* out = out_row(a, cur.q.q0, cur.head, row);
 #pragma unroll
@@ -882,7 +909,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
         fresh = true;
         if (i + 1 < n) {
           __syncwarp();  // (every lane has read the item that ends)
-          if (lane == 0) next_item<NT>(cur, a, known);
+          if (lane == 0) next_item<NT, MODE>(cur, a, known);
           __syncwarp();
         }
       }
@@ -913,7 +940,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
     float* to = all ? nullptr : exchange + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PARTIAL;
     for (uint32_t row = 0; row < p.rows; row += 4) {  // the warps take the rows of all items in turn
       if (turn == warp)
-        join_rows4<D, NT>(a, p, row, n_run, [&](uint32_t k) {
+        join_rows4<D, NT, MODE>(a, p, row, n_run, [&](uint32_t k) {
           const uint32_t x = __fns(run, 0, k + 1);
           return (x & 1) ? reinterpret_cast<const float*>(smem + (x >> 1) * (RING * S::PART)) : scratch + (static_cast<size_t>(blockIdx.x) * NWARP + (x >> 1)) * S::PARTIAL;
         }, to, lane);
@@ -944,8 +971,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
     const uint32_t step = j.n <= 4 ? 4 : 1;
     for (uint32_t row = 0; row < p.rows; row += step) {
       if (turn == warp) {
-        if (step == 4) join_rows4<D, NT>(a, p, row, j.n, part, nullptr, lane);
-        else join_row<D, NT>(a, p, row, j.n, part, lane);
+        if (step == 4) join_rows4<D, NT, MODE>(a, p, row, j.n, part, nullptr, lane);
+        else join_row<D, NT, MODE>(a, p, row, j.n, part, lane);
       }
       if (++turn == NWARP) turn = 0;
     }
@@ -953,31 +980,41 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
 }
 
 // f(kernel, shape) for the instance of (head_dim, rows of an item, page).
-template <typename F>
+template <int MODE, typename F>
 cudaError_t with_kernel(uint32_t head_dim, bool two, uint32_t page, F f) {
   auto by_page = [&](auto d, auto nt) {
     constexpr int D = decltype(d)::value, NT = decltype(nt)::value;
-    return page == 16 ? f(kv4_attention_kernel<D, NT, 16>, Shape<D, NT>()) : page == 32 ? f(kv4_attention_kernel<D, NT, 32>, Shape<D, NT>()) : f(kv4_attention_kernel<D, NT, 64>, Shape<D, NT>());
+    return page == 16   ? f(kv4_attention_kernel<D, NT, 16, MODE>, Shape<D, NT>())
+           : page == 32 ? f(kv4_attention_kernel<D, NT, 32, MODE>, Shape<D, NT>())
+                        : f(kv4_attention_kernel<D, NT, 64, MODE>, Shape<D, NT>());
   };
   using I1 = std::integral_constant<int, 1>;
   using I2 = std::integral_constant<int, 2>;
   if (head_dim == 128) return two ? by_page(std::integral_constant<int, 128>(), I2()) : by_page(std::integral_constant<int, 128>(), I1());
   return two ? by_page(std::integral_constant<int, 64>(), I2()) : by_page(std::integral_constant<int, 64>(), I1());
 }
+template <int MODE>
+cudaError_t allow_shared_memory() {
+  cudaError_t e = cudaSuccess;
+  for (uint32_t i = 0; i < 12 && e == cudaSuccess; i++)
+    e = with_kernel<MODE>(i & 1 ? 128 : 64, i & 2, 16u << (i >> 2), [](auto kernel, auto shape) {
+      return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shape.SMEM));
+    });
+  return e;
+}
 
 }  // namespace
 
 cudaError_t bp_kv4_attention_init(bp_paged_ctx* c) {
-  cudaError_t e = cudaSuccess;
-  for (uint32_t i = 0; i < 12 && e == cudaSuccess; i++)
-    e = with_kernel(i & 1 ? 128 : 64, i & 2, 16u << (i >> 2), [](auto kernel, auto shape) {
-      return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shape.SMEM));
-    });
+  cudaError_t e = allow_shared_memory<PLAIN>();
+  if (e == cudaSuccess) e = allow_shared_memory<PREFIX>();
+  if (e == cudaSuccess) e = allow_shared_memory<OWN>();
+  if (e == cudaSuccess) e = allow_shared_memory<CHOSEN>();
   if (e != cudaSuccess) return e;
   // a piece per warp and two per CTA, of the instance that needs most
   size_t floats = 0;
   for (uint32_t i = 0; i < 4; i++)
-    (void)with_kernel(i & 1 ? 128 : 64, i & 2, 16, [&](auto, auto shape) {
+    (void)with_kernel<PLAIN>(i & 1 ? 128 : 64, i & 2, 16, [&](auto, auto shape) {
       const size_t need = static_cast<size_t>(c->sm_count) * (shape.NWARP + 2) * shape.PARTIAL;
       if (need > floats) floats = need;
       return cudaSuccess;
@@ -989,34 +1026,27 @@ cudaError_t bp_kv4_attention_init(bp_paged_ctx* c) {
   return cudaMemset(c->counters, 0, static_cast<size_t>(c->sm_count) * sizeof(uint32_t));
 }
 
-cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, const Pool& pool, uint32_t head_dim, const bp_kv4_attn& in) {
-  AttnArgs a;
-  a.pool = pool;
-  a.q = Rows{static_cast<uint16_t*>(in.q.data), in.q.tok_stride, in.q.head_stride};
-  a.out = Rows{static_cast<uint16_t*>(in.out.data), in.out.tok_stride, in.out.head_stride};
-  a.q_start = static_cast<const int32_t*>(in.q_start);
-  a.kv_len = static_cast<const int32_t*>(in.kv_len);
-  a.page_table = static_cast<const int32_t*>(in.page_table);
-  a.err = c->err_dev;
-  a.n_req = in.n_req;
-  a.n_head = in.n_head;
-  a.group = in.n_head / pool.n_kv_head;
-  a.total_q = in.total_q;
-  a.max_q = in.max_q < in.total_q ? in.max_q : in.total_q;
-  a.max_kv = in.max_kv;
-  a.table_stride = in.table_stride;
-  a.table_pages = in.table_stride < (0x7fffffffu >> pool.log_page) ? in.table_stride : (0x7fffffffu >> pool.log_page);
-  a.window = in.window < in.max_kv ? in.window : 0;  // (nobody has more keys)
-  a.scale_log2 = in.scale * 1.4426950408889634f;
+void bp_kv4_attention_args(const bp_paged_ctx* c, bool bf, const Pool& pool, const bp_rows& q, const bp_rows& out, uint32_t n_head, float scale, AttnArgs* a) {
+  *a = AttnArgs{};
+  a->pool = pool;
+  a->q = Rows{static_cast<uint16_t*>(q.data), q.tok_stride, q.head_stride};
+  a->out = Rows{static_cast<uint16_t*>(out.data), out.tok_stride, out.head_stride};
+  a->err = c->err_dev;
+  a->n_head = n_head;
+  a->group = n_head / pool.n_kv_head;
+  a->scale_log2 = scale * 1.4426950408889634f;
   int exponent = 0;
-  const float fraction = frexpf(fabsf(a.scale_log2), &exponent);
+  const float fraction = frexpf(fabsf(a->scale_log2), &exponent);
   const bool split = fraction > 0.f && fraction < 1.f;  // (not of 0 and infinity)
-  a.mantissa = split ? 2.f * fraction : 1.f;
-  a.mantissa24 = a.mantissa * 0x1p24f;
-  a.power = split ? ldexpf(1.f, exponent - 1) : fraction;
-  a.bias = 0x64006400u;
-  a.bf = bf;
-  a.q_vec = reinterpret_cast<uintptr_t>(in.q.data) % 16 == 0 && in.q.tok_stride % 8 == 0 && in.q.head_stride % 8 == 0;
+  a->mantissa = split ? 2.f * fraction : 1.f;
+  a->mantissa24 = a->mantissa * 0x1p24f;
+  a->power = split ? ldexpf(1.f, exponent - 1) : fraction;
+  a->bias = 0x64006400u;
+  a->bf = bf;
+  a->q_vec = reinterpret_cast<uintptr_t>(q.data) % 16 == 0 && q.tok_stride % 8 == 0 && q.head_stride % 8 == 0;
+}
+
+cudaError_t bp_launch_kv4_rows(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, int mode, uint64_t rows, const AttnArgs& a) {
   // Which kernel. Here the codes are expanded once per 16 rows (tokens x query heads per KV head) of a request, there once for up to 128, with some 14 us
   // for an item's beginning and end. us, this kernel / the other one:
   //   head_dim 128, 32 / 8 heads         16 rows  32 rows  48 rows     head_dim 64, 40 / 8 heads    15 rows  30 rows  40 rows  50 rows
@@ -1025,10 +1055,33 @@ cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, co
   //   64 requests of 1000 keys           46/85    78/87    113/88                                   29/70    50/70    65/71    85/72
   //   1 request of 30000 keys            33/64    48/63    62/64                                    27/45    36/45    42/45    50/45
   // and as much apart with 2, 4 and 8 requests of 4096 keys and with 2 KV heads; so 32 rows is the line for both.
-  const uint64_t rows = static_cast<uint64_t>(a.max_q) * a.group;
-  // (Without any key there are only zeros to write, and there may be no pool: this kernel looks at none.)
-  if (a.max_kv != 0 && rows > 32) return bp_launch_kv4_prefill(c, s, head_dim, a);
-  return with_kernel(head_dim, a.max_q * a.group > 8, pool.page, [&](auto kernel, auto shape) {
+  // (Without any key there are only zeros to write, and there may be no pool: this kernel looks at none. Chosen pages are those of one token.)
+  if (a.max_kv != 0 && rows > 32 && mode != CHOSEN) return bp_launch_kv4_prefill(c, s, head_dim, mode, a);
+  auto launch = [&](auto kernel, auto shape) {
     return bp_launch(true, kernel, dim3(c->sm_count), dim3(shape.THREADS), shape.SMEM, s, a, c->partials, c->counters);
-  });
+  };
+  const bool two = rows > 8;
+  return mode == PLAIN    ? with_kernel<PLAIN>(head_dim, two, a.pool.page, launch)
+         : mode == PREFIX ? with_kernel<PREFIX>(head_dim, two, a.pool.page, launch)
+         : mode == OWN    ? with_kernel<OWN>(head_dim, two, a.pool.page, launch)
+                          : with_kernel<CHOSEN>(head_dim, two, a.pool.page, launch);
+}
+
+// Pages of a row of a page table that are looked at: what 31 bits of keys fill at most.
+uint32_t bp_kv4_table_pages(const Pool& pool, uint32_t stride) { return stride < (0x7fffffffu >> pool.log_page) ? stride : (0x7fffffffu >> pool.log_page); }
+
+cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, const Pool& pool, uint32_t head_dim, const bp_kv4_attn& in) {
+  AttnArgs a;
+  bp_kv4_attention_args(c, bf, pool, in.q, in.out, in.n_head, in.scale, &a);
+  a.q_start = static_cast<const int32_t*>(in.q_start);
+  a.kv_len = static_cast<const int32_t*>(in.kv_len);
+  a.page_table = static_cast<const int32_t*>(in.page_table);
+  a.n_req = in.n_req;
+  a.total_q = in.total_q;
+  a.max_q = in.max_q < in.total_q ? in.max_q : in.total_q;
+  a.max_kv = in.max_kv;
+  a.table_stride = in.table_stride;
+  a.table_pages = bp_kv4_table_pages(pool, in.table_stride);
+  a.window = in.window < in.max_kv ? in.window : 0;  // (nobody has more keys)
+  return bp_launch_kv4_rows(c, s, head_dim, PLAIN, static_cast<uint64_t>(a.max_q) * a.group, a);
 }

@@ -10,6 +10,17 @@ constexpr unsigned FULL = 0xffffffffu;
 constexpr float NEG_BIG = -3e38f;  // the maximum of no score, below every score that 32 bits hold but the last few
 constexpr float P_UP = 10.f;   // P is stored as f16 times 2^10: it keeps its bits down to 2^-24 of the maximum
 
+// What a kernel's line of requests is.
+enum Mode {
+  PLAIN,    // requests, their outputs are written
+  PREFIX,   // prefixes that several requests have in common: their rows are those of all these requests, each sees every key; parts
+  OWN,      // requests behind their prefixes; parts
+  CHOSEN,   // tokens that see every key of pages chosen for each KV head; their outputs are written
+};
+// Where a part of the keys is all that a kernel sees, its rows become partial results in memory instead of outputs: the sums as they are, their
+// maximum (log2 units) and the sum of the weights. bp_kv4_shared.cu puts them together.
+__host__ __device__ constexpr bool in_parts(int mode) { return mode == PREFIX || mode == OWN; }
+
 struct AttnArgs {
   Pool pool;
   Rows q, out;
@@ -23,6 +34,11 @@ struct AttnArgs {
   uint32_t bias;  // 0x64006400: two f16 numbers 1024
   uint32_t bf;    // activations are bfloat16
   uint32_t q_vec; // rows of q are 16-byte aligned
+  // in parts
+  float* part;          // [rows of q][n_head][head_dim]
+  float2* part_ml;      // [rows of q][n_head]
+  const int32_t* prefix_start;  // PREFIX: request r is a prefix, of the requests [prefix_start[r], prefix_start[r + 1]) of n_all
+  uint32_t n_all;
 };
 // Queries become f16 numbers, each row multiplied by the power of two that brings its largest element into [2^8, 2^9): the most for which 32 of them
 // times a mantissa add up within f16, as bp_kv4_attention.cu wants. f16 and bf16 queries keep all their bits down to 2^-18 of the row's largest element,
@@ -40,8 +56,23 @@ __device__ __forceinline__ int first_seen(int keys, uint32_t window) { return wi
 struct Lengths {
   int q0, q_len, kv_len;
 };
+template <int MODE>
 __device__ __forceinline__ Lengths lengths_of(const AttnArgs& a, uint32_t r, bool report) {
-  const int start = a.q_start[r], stop = a.q_start[r + 1], keys = a.kv_len[r], q0 = max(start, 0);
+  const int keys = a.kv_len[r];
+  int start, stop;
+  if constexpr (MODE == PREFIX) {
+    const int from = a.prefix_start[r], to = a.prefix_start[r + 1], last = static_cast<int>(a.n_all), f = min(max(from, 0), last), t = min(max(to, f), last);
+    if (report && (f != from || t != to)) note_range(a.err);
+    start = a.q_start[f];
+    stop = a.q_start[t];
+  } else if constexpr (MODE == CHOSEN) {  // (a negative number of keys: a token of no request)
+    start = static_cast<int>(r);
+    stop = start + (keys >= 0);
+  } else {
+    start = a.q_start[r];
+    stop = a.q_start[r + 1];
+  }
+  const int q0 = max(start, 0);
   const int given_q = max(stop, q0) - q0, given_kv = max(keys, 0);
   const Lengths n{q0, min(min(given_q, static_cast<int>(a.max_q)), max(static_cast<int>(a.total_q) - q0, 0)),
                   min(given_kv, static_cast<int>(min(a.max_kv, a.table_pages << a.pool.log_page)))};
@@ -91,9 +122,17 @@ __device__ __forceinline__ void store4(bool bf, uint16_t* p, float a, float b, f
 __device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, int q0, uint32_t head, uint32_t row) {
   return a.out.data + static_cast<int64_t>(q0 + row / a.group) * a.out.tok + static_cast<int64_t>(head * a.group + row % a.group) * a.out.head;
 }
+// The same row among the partial results.
+__device__ __forceinline__ size_t part_row(const AttnArgs& a, int q0, uint32_t head, uint32_t row) {
+  return static_cast<size_t>(q0 + row / a.group) * a.n_head + head * a.group + row % a.group;
+}
 
 }  // namespace kv4
 }  // namespace bp
 
 cudaError_t bp_kv4_prefill_init(bp_paged_ctx* c);
-cudaError_t bp_launch_kv4_prefill(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, const bp::kv4::AttnArgs& a);
+cudaError_t bp_launch_kv4_prefill(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, int mode, const bp::kv4::AttnArgs& a);
+// The scale and what belongs to the context and the pool; then either kernel, by the rows of an item (`rows` of a request at most).
+uint32_t bp_kv4_table_pages(const bp::Pool& pool, uint32_t stride);
+void bp_kv4_attention_args(const bp_paged_ctx* c, bool bf, const bp::Pool& pool, const bp_rows& q, const bp_rows& out, uint32_t n_head, float scale, bp::kv4::AttnArgs* a);
+cudaError_t bp_launch_kv4_rows(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, int mode, uint64_t rows, const bp::kv4::AttnArgs& a);

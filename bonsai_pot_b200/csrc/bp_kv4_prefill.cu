@@ -54,9 +54,10 @@ struct Request {
   int q0, q_len, kv_len;
   uint32_t rows;
 };
+template <int MODE>
 __device__ __forceinline__ Request request(const AttnArgs& a, uint32_t r, bool report) {
   Request q;
-  const Lengths n = lengths_of(a, r, report);
+  const Lengths n = lengths_of<MODE>(a, r, report);
   q.q0 = n.q0;
   q.q_len = n.q_len;
   q.kv_len = n.kv_len;
@@ -71,8 +72,15 @@ struct Keys {
   uint32_t tiles;
   __device__ int first() const { return low & ~static_cast<int>(BN - 1); }
 };
+template <int MODE>
 __device__ __forceinline__ Keys keys_of(const AttnArgs& a, const Request& q, uint32_t row0, uint32_t rows) {
   Keys k;
+  if constexpr (MODE == PREFIX) {
+    k.low = k.all_from = 0;
+    k.high = k.all_to = q.kv_len;
+    k.tiles = max((static_cast<uint32_t>(q.kv_len) + BN - 1) / BN, 1u);
+    return k;
+  }
   const int t0 = static_cast<int>(row0 / a.group), t1 = static_cast<int>((min(row0 + rows, q.rows) - 1) / a.group), past = q.kv_len - q.q_len;
   k.high = max(past + t1 + 1, 0);
   k.low = first_seen(past + t0 + 1, a.window);
@@ -171,7 +179,7 @@ __device__ __forceinline__ void store_rows(const AttnArgs& a, int q0, uint32_t h
   }
 }
 
-template <int D, uint32_t NQ>
+template <int D, uint32_t NQ, int MODE>
 __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(const __grid_constant__ AttnArgs a, float* __restrict__ scratch, uint32_t* __restrict__ counters) {
   using S = Shape<D, NQ>;
   constexpr uint32_t THREADS = S::THREADS;
@@ -233,12 +241,12 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   const uint32_t per = (a.n_req + THREADS - 1) / THREADS;
   auto tiles_of = [&](const Request& q) {  // of all items of a request
     uint32_t n = 0;
-    for (uint32_t row0 = 0; row0 < q.rows; row0 += S::ROWS) n += keys_of(a, q, row0, S::ROWS).tiles + ITEM_COST;
+    for (uint32_t row0 = 0; row0 < q.rows; row0 += S::ROWS) n += keys_of<MODE>(a, q, row0, S::ROWS).tiles + ITEM_COST;
     return n * a.pool.n_kv_head;
   };
   {
     uint32_t units = 0;
-    for (uint32_t r = threadIdx.x * per; r < min((threadIdx.x + 1) * per, a.n_req); r++) units += tiles_of(request(a, r, blockIdx.x == 0));
+    for (uint32_t r = threadIdx.x * per; r < min((threadIdx.x + 1) * per, a.n_req); r++) units += tiles_of(request<MODE>(a, r, blockIdx.x == 0));
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t x = __shfl_up_sync(FULL, units, o);
@@ -261,9 +269,9 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     uint32_t left = c0 - line[at];
     bool found = false;
     for (uint32_t r = at * per; r < a.n_req && !found; r++) {
-      const Request q = request(a, r, false);
+      const Request q = request<MODE>(a, r, false);
       for (uint32_t x = 0; x * S::ROWS < q.rows; x++) {
-        const Keys k = keys_of(a, q, x * S::ROWS, S::ROWS);
+        const Keys k = keys_of<MODE>(a, q, x * S::ROWS, S::ROWS);
         const uint32_t places = k.tiles + ITEM_COST, n = places * a.pool.n_kv_head;
         if (left < n) {
           const uint32_t head = left / places, in = left - head * places;
@@ -430,7 +438,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       const float scale = row_scale[x * BM + r];
       // this row sees the keys [lo, hi)
       const int past = q.kv_len - q.q_len;
-      const int hi = row < q.rows ? past + static_cast<int>(row / a.group) + 1 : 0, lo = first_seen(hi, a.window);
+      const int hi = row >= q.rows ? 0 : MODE == PREFIX ? q.kv_len : past + static_cast<int>(row / a.group) + 1, lo = MODE == PREFIX ? 0 : first_seen(hi, a.window);
       float m_run = NEG_BIG, l_run = 0.f;
       for (uint32_t i = 0; i < n; i++) {
         const uint32_t c = done + i, b = c & 1, s = c % SLOTS;
@@ -517,7 +525,26 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       (void)waitx(&o_done[x], pieces & 1);
       __syncwarp();
       tc_fence_after();
-      if (first == 0 && n == keys.tiles) {
+      if (in_parts(MODE) && first == 0 && n == keys.tiles) {
+        // ---- the whole item, as a partial result of its rows ----
+        const size_t at = row < q.rows ? part_row(a, q.q0, head, row) : 0;
+#pragma unroll 1
+        for (uint32_t k = 0; k < D / 16; k++) {
+          uint32_t o[16];
+          tmem_ld16(o_addr + 16 * k, o);
+          tmem_ld_wait();
+          if (row >= q.rows || abort_s) continue;
+          const bool none = over >> (k >> 1) & 1;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = none ? __int_as_float(0x7fffffff) : __uint_as_float(o[8 * (e >> 1) + column_of(4 * (e & 1) + j)]);
+            *reinterpret_cast<float4*>(a.part + at * D + 16 * k + 4 * e) = make_float4(v[0], v[1], v[2], v[3]);
+          }
+        }
+        if (row < q.rows && !abort_s) a.part_ml[at] = make_float2(l_run == 0.f ? NEG_BIG : m_run * scale, l_run);
+      } else if (first == 0 && n == keys.tiles) {
         // ---- the whole item: O / l through the dead Q tile, whole rows of it to memory ----
         const float inv_l = l_run == 0.f ? 0.f : 1.f / l_run;
         uint8_t* stage = smem + x * S::Q_B;
@@ -588,10 +615,10 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
           c.head = 0;
           if (++c.x * S::ROWS >= c.q.rows) {
             c.x = 0;
-            do c.q = request(a, ++c.r, false);  // (there is a further item in the line)
+            do c.q = request<MODE>(a, ++c.r, false);  // (there is a further item in the line)
             while (c.q.rows == 0);
           }
-          c.keys = keys_of(a, c.q, c.x * S::ROWS, S::ROWS);
+          c.keys = keys_of<MODE>(a, c.q, c.x * S::ROWS, S::ROWS);
         }
         cur = c;
       }
@@ -614,7 +641,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
           l = l * ex2(m - top) + e.y * ex2(e.x - top);
           m = top;
         }
-        joined[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
+        joined[r] = make_float2(m, in_parts(MODE) ? l : l == 0.f ? 0.f : 1.f / l);
       }
       __syncthreads();
 #pragma unroll 4
@@ -625,15 +652,23 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
 #pragma unroll 2
         for (uint32_t k = 0; k < j.n; k++) {
           const float4 v = reinterpret_cast<const float4*>(piece(k))[c * S::ROWS + r];
-          const float w = ex2(ml(k, r).x - all.x) * all.y;
+          const float w = in_parts(MODE) ? ex2(ml(k, r).x - all.x) : ex2(ml(k, r).x - all.x) * all.y;
           o = make_float4(fmaf(v.x, w, o.x), fmaf(v.y, w, o.y), fmaf(v.z, w, o.z), fmaf(v.w, w, o.w));
+        }
+        if constexpr (in_parts(MODE)) {
+          if (r < rows) {
+            const size_t at = part_row(a, q.q0, head, row0 + r);
+            *reinterpret_cast<float4*>(a.part + at * D + 4 * c) = o;
+            if (c == 0) a.part_ml[at] = all;
+          }
+          continue;
         }
         // staged in the dead Q tiles: whole rows go to memory
         const uint32_t lo = a.bf ? pack2<true>(o.x, o.y) : pack2<false>(o.x, o.y), hi = a.bf ? pack2<true>(o.z, o.w) : pack2<false>(o.z, o.w);
         *reinterpret_cast<uint2*>(smem + r * (D * 2) + (((c >> 1) ^ (r & (D / 8 - 1))) << 4) + 8 * (c & 1)) = make_uint2(lo, hi);
       }
       __syncthreads();
-      store_rows<D>(a, q.q0, head, row0, rows, smem, threadIdx.x, THREADS);
+      if constexpr (!in_parts(MODE)) store_rows<D>(a, q.q0, head, row0, rows, smem, threadIdx.x, THREADS);
     }
     __syncthreads();
   }
@@ -652,10 +687,10 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   if (warp == 1) tmem_dealloc(tmem, S::TMEM_COLS);
 }
 
-template <typename F>
+template <int MODE, typename F>
 cudaError_t with_kernel(uint32_t head_dim, bool two, F f) {
-  if (head_dim == 128) return two ? f(kv4_prefill_kernel<128, 2>, Shape<128, 2>()) : f(kv4_prefill_kernel<128, 1>, Shape<128, 1>());
-  return two ? f(kv4_prefill_kernel<64, 2>, Shape<64, 2>()) : f(kv4_prefill_kernel<64, 1>, Shape<64, 1>());
+  if (head_dim == 128) return two ? f(kv4_prefill_kernel<128, 2, MODE>, Shape<128, 2>()) : f(kv4_prefill_kernel<128, 1, MODE>, Shape<128, 1>());
+  return two ? f(kv4_prefill_kernel<64, 2, MODE>, Shape<64, 2>()) : f(kv4_prefill_kernel<64, 1, MODE>, Shape<64, 1>());
 }
 
 }  // namespace
@@ -663,17 +698,25 @@ cudaError_t with_kernel(uint32_t head_dim, bool two, F f) {
 cudaError_t bp_kv4_prefill_init(bp_paged_ctx* c) {
   size_t floats = 0;
   cudaError_t e = cudaSuccess;
-  for (uint32_t i = 0; i < 4 && e == cudaSuccess; i++)
-    e = with_kernel(i & 1 ? 128 : 64, i & 2, [&](auto kernel, auto shape) {
-      const size_t need = 2 * static_cast<size_t>(c->sm_count) * shape.PARTIAL;  // two pieces per CTA
-      if (need > floats) floats = need;
-      return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shape.SMEM));
-    });
+  auto allow = [&](auto kernel, auto shape) {
+    const size_t need = 2 * static_cast<size_t>(c->sm_count) * shape.PARTIAL;  // two pieces per CTA
+    if (need > floats) floats = need;
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shape.SMEM));
+  };
+  for (uint32_t i = 0; i < 4 && e == cudaSuccess; i++) {
+    e = with_kernel<PLAIN>(i & 1 ? 128 : 64, i & 2, allow);
+    if (e == cudaSuccess) e = with_kernel<PREFIX>(i & 1 ? 128 : 64, i & 2, allow);
+    if (e == cudaSuccess) e = with_kernel<OWN>(i & 1 ? 128 : 64, i & 2, allow);
+  }
   return e != cudaSuccess ? e : cudaMalloc(&c->prefill_partials, floats * sizeof(float));
 }
 
-cudaError_t bp_launch_kv4_prefill(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, const AttnArgs& a) {
-  return with_kernel(head_dim, a.max_q * a.group > BM, [&](auto kernel, auto shape) {
+cudaError_t bp_launch_kv4_prefill(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, int mode, const AttnArgs& a) {
+  auto launch = [&](auto kernel, auto shape) {
     return bp_launch(true, kernel, dim3(c->sm_count), dim3(shape.THREADS), shape.SMEM, s, a, c->prefill_partials, c->counters);
-  });
+  };
+  const bool two = static_cast<uint64_t>(a.max_q) * a.group > BM;
+  return mode == PLAIN    ? with_kernel<PLAIN>(head_dim, two, launch)
+         : mode == PREFIX ? with_kernel<PREFIX>(head_dim, two, launch)
+                          : with_kernel<OWN>(head_dim, two, launch);
 }

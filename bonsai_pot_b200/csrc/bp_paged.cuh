@@ -20,6 +20,7 @@ struct bp_paged_ctx {
   float* partials;     // split attention: partial results of the CTAs
   float* prefill_partials;  // the same of the kernel for many queries
   uint32_t* counters;  // split attention: partials that have arrived, zero between launches
+  uint32_t* page_counter;  // page tables: CTAs that have ended, zero between launches
   char msg[256];
 };
 
@@ -122,5 +123,7 @@ cudaError_t bp_launch_kv4_append(bp_paged_ctx* c, cudaStream_t s, bool bf, const
                                  const uint16_t* w_norm, float eps);
 cudaError_t bp_launch_kv4_read(bp_paged_ctx* c, cudaStream_t s, bool bf, const bp::Pool& pool, uint32_t head_dim, const int64_t* slots,
                                uint32_t n_tok, const bp::Rows& k, const bp::Rows& v);
+cudaError_t bp_pages_init(bp_paged_ctx* c);
+cudaError_t bp_kv4_select_init(bp_paged_ctx* c);
 cudaError_t bp_kv4_attention_init(bp_paged_ctx* c);
 cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, const bp::Pool& pool, uint32_t head_dim, const bp_kv4_attn& a);

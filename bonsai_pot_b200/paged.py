@@ -1,7 +1,8 @@
-"""Many requests at once over one paged KV cache held in 4 bits: rotary positions, append, read-back, attention.
+"""Many requests at once over one paged KV cache held in 4 bits: rotary positions, append, read-back, attention; page tables on the device,
+prefixes that requests have in common, attention over chosen pages.
 
 `PagedContext` owns scratch memory only; cache, RoPE table and activations are the caller's CUDA tensors. Every method calls
-straight into the C ABI of include/bonsai_paged.h, which says what each operator computes and how a pool's bytes are laid
+straight into the C ABI of include/bonsai_paged.h and include/bonsai_pages.h, which say what each operator computes and how a pool's bytes are laid
 out. Rows are tensors [tokens, heads, head_dim] of float16 or bfloat16 with any strides between tokens and heads; index
 tensors are int32, slots int64. A call without a `stream` goes to torch's current stream of the context's device (the C entries' null
 stream is CUDA's legacy default stream, for which torch's other streams do not wait).
@@ -76,6 +77,8 @@ def _like(t, dtype, shape, what):
 
 
 def _index(t, what, n, device, slots=False):
+    if _I32 is None:
+        _types()
     if t.get_device() != device:
         _elsewhere(t, what, device)
     if t.dtype is not (_I64 if slots else _I32) or t.shape != (n,) or not t.is_contiguous():
@@ -128,6 +131,66 @@ class KV4Pool:
         return n
 
 
+class KV4Pools:
+    """The pools of a model's layers, of one shape, and their summaries: what copy_pages copies in one call."""
+
+    def __init__(self, pools, summaries=()):
+        self.pools, self.summaries = list(pools), list(summaries)
+        if not self.pools:
+            _bad("at least one pool")
+        one = self.pools[0]
+        self.device, self.n_pages = one.device, one._c.n_pages
+        for p in self.pools:
+            if p.device != self.device or (p._c.n_pages, p.page_tokens, p.n_kv_head, p.head_dim) != (self.n_pages, one.page_tokens, one.n_kv_head, one.head_dim):
+                _bad("the pools must have one shape and lie on one device")
+        arrays = [(p.data.data_ptr(), one.page_tokens * one.n_kv_head * one.head_dim * 5 // 4) for p in self.pools]
+        for s in self.summaries:
+            if s.device != self.device or s.codes.shape[0] != self.n_pages:
+                _bad("the summaries must have the pools' number of pages and lie on their device")
+            arrays += [(s.codes.data_ptr(), s.codes[0].numel()), (s.scales.data_ptr(), 4 * s.scales.shape[1])]
+        self.n_arrays = len(arrays)
+        self._c = (_lib.PageArrayStruct * self.n_arrays)(*[_lib.PageArrayStruct(*a) for a in arrays])
+        self._p = C.addressof(self._c)
+
+
+class PageTables:
+    """int32 CUDA tensors: table [rows, pages of a row], kv_len [rows], refs [pages of the pool] (how often a page is held; 0 is free)."""
+
+    def __init__(self, table, kv_len, refs, page_tokens):
+        for t, what, n in ((table, "table", 2), (kv_len, "kv_len", 1), (refs, "refs", 1)):
+            if str(t.dtype) != "torch.int32" or t.dim() != n:
+                _bad(f"{what} must be an int32 tensor of {n} dimension{'s' * (n > 1)}, not {tuple(t.shape)} {t.dtype}")
+            if not t.is_cuda or t.get_device() != table.get_device():
+                _bad(f"{what} must be on the CUDA device of the others, not on {t.device}")
+        n_rows, row_pages = table.shape
+        if (table.stride(1) != 1 and row_pages > 1) or (n_rows > 1 and table.stride(0) < row_pages) or not kv_len.is_contiguous() or not refs.is_contiguous():
+            _bad("the rows of table must be dense and not overlap, kv_len and refs dense")
+        if kv_len.shape[0] != n_rows or page_tokens not in (16, 32, 64):
+            _bad("kv_len must have an entry per row of table, page_tokens must be 16, 32 or 64")
+        pitch = table.stride(0) if n_rows > 1 else row_pages
+        if max(n_rows, row_pages, pitch, refs.shape[0]) > _U32:
+            _bad("page tables have fewer than 2^32 rows, pages and elements between rows")
+        self.table, self.kv_len, self.refs, self.page_tokens, self.device = table, kv_len, refs, page_tokens, table.get_device()
+        self._c = _lib.PageTablesStruct(table.data_ptr(), kv_len.data_ptr(), refs.data_ptr(), n_rows, row_pages, pitch, refs.shape[0], page_tokens)
+        self._p, self.n_rows = C.addressof(self._c), n_rows
+
+
+class BlockSummary:
+    """What select() goes by: int8 CUDA tensor codes [pages, KV heads, 2, head_dim] and float32 scales [pages, KV heads]."""
+
+    def __init__(self, codes, scales):
+        if str(codes.dtype) != "torch.int8" or codes.dim() != 4 or codes.shape[2] != 2 or not codes.is_contiguous():
+            _bad("codes are a dense int8 tensor [pages, KV heads, 2, head_dim]")
+        if str(scales.dtype) != "torch.float32" or scales.shape != codes.shape[:2] or not scales.is_contiguous():
+            _bad("scales are a dense float32 tensor [pages, KV heads]")
+        if not codes.is_cuda or codes.get_device() != scales.get_device():
+            _bad("codes and scales must be on one CUDA device")
+        self.codes, self.scales, self.device = codes, scales, codes.get_device()
+        self.shape = (codes.shape[0], codes.shape[1], codes.shape[3])
+        self._c = _lib.SummaryStruct(codes.data_ptr(), scales.data_ptr())
+        self._p = C.addressof(self._c)
+
+
 class PagedContext:
     """Scratch memory and errors of the paged operators on one device, on which every tensor of a call must lie."""
 
@@ -147,6 +210,8 @@ class PagedContext:
         self._a, self._b, self._attn = _lib.RowsStruct(), _lib.RowsStruct(), _lib.AttnStruct()
         self._q, self._o = self._attn.q, self._attn.out
         self._pa, self._pb, self._pattn = C.addressof(self._a), C.addressof(self._b), C.addressof(self._attn)
+        self._shared, self._choice, self._chosen = _lib.SharedStruct(), _lib.ChoiceStruct(), _lib.ChosenStruct()
+        self._pshared, self._pchoice, self._pchosen = C.addressof(self._shared), C.addressof(self._choice), C.addressof(self._chosen)
 
     def _message(self):
         return (self._lib.bp_paged_last_error(self._h) or b"").decode() if self._h else ""
@@ -269,3 +334,170 @@ class PagedContext:
         if heads != pool.n_kv_head or dim != pool.head_dim:
             _bad(f"the pool holds {pool.n_kv_head} heads of {pool.head_dim}, the rows have {heads} of {dim}")
         return code, n, device
+
+    # ---- page tables ----
+
+    def _tables(self, tables):
+        if tables.device != self._device:
+            _elsewhere(tables.table, "the page tables", self._device)
+        return tables._p
+
+    def _pairs(self, a, b, what_a, what_b):
+        """Two int32 tensors of one length; the length and the addresses."""
+        n = a.shape[0] if a.dim() == 1 else -1
+        return n, _index(a, what_a, n, self._device), _index(b, what_b, n, self._device)
+
+    def grow(self, tables, n_new, q_start, positions, slots, stream=None):
+        """Every row gets n_new[row] further tokens and the pages for them; q_start [rows + 1], positions and (int64) slots [at least the
+        new tokens] are written for what is done with the tokens, -1 behind the last."""
+        device, n = self._device, positions.shape[0] if positions.dim() == 1 else -1
+        p, rows = self._tables(tables), tables.n_rows
+        st = self._lib.bp_pages_grow(self._h, _current(device) if stream is None else _stream(stream), p, _index(n_new, "n_new", rows, device), _index(q_start, "q_start", rows + 1, device),
+                                     _index(positions, "positions", n, device), _index(slots, "slots", n, device, True), n)
+        if st:
+            self._check(st)
+
+    def release(self, tables, rows, stream=None):
+        """The rows (int32; negative: none) give their pages back and are empty."""
+        device, n = self._device, rows.shape[0] if rows.dim() == 1 else -1
+        st = self._lib.bp_pages_release(self._h, _current(device) if stream is None else _stream(stream), self._tables(tables), _index(rows, "rows", n, device), n)
+        if st:
+            self._check(st)
+
+    def fork(self, tables, parents, children, src, dst, stream=None):
+        """Empty rows `children` become what `parents` are: full pages are shared, src and dst say which pages are to be copied (copy_pages)."""
+        n, parents, children = self._pairs(parents, children, "parents", "children")
+        device = self._device
+        st = self._lib.bp_pages_fork(self._h, _current(device) if stream is None else _stream(stream), self._tables(tables), parents, children, n, _index(src, "src", n, device),
+                                     _index(dst, "dst", n, device))
+        if st:
+            self._check(st)
+
+    def compact(self, tables, src, dst, stream=None):
+        """The highest used pages move into the lowest free ones, as many as src and dst have places; these say which pages are to be copied (copy_pages)."""
+        n, src, dst = self._pairs(src, dst, "src", "dst")
+        st = self._lib.bp_pages_compact(self._h, _current(self._device) if stream is None else _stream(stream), self._tables(tables), src, dst, n)
+        if st:
+            self._check(st)
+
+    def copy_pages(self, pools, src, dst, stream=None):
+        """Page src[i] of every pool and summary of a KV4Pools goes to page dst[i] (int32; a negative one of either: nothing)."""
+        if pools.device != self._device:
+            _elsewhere(pools.pools[0].data, "the pools", self._device)
+        n, src, dst = self._pairs(src, dst, "src", "dst")
+        st = self._lib.bp_pages_copy(self._h, _current(self._device) if stream is None else _stream(stream), pools._p, pools.n_arrays, pools.n_pages, src, dst, n)
+        if st:
+            self._check(st)
+
+    # ---- a prefix in common; chosen pages ----
+
+    def _table(self, t, what, page_tokens, most):
+        """A page table's requests, address and pitch, and `most` cut to the keys that a row has pages for."""
+        if t.get_device() != self._device:
+            _elsewhere(t, what, self._device)
+        if t.dtype is not _I32 or t.dim() != 2:
+            _bad(f"{what} must be int32 [rows, pages]")
+        (n, pages), (stride, dense) = t.shape, t.stride()
+        if (dense != 1 and pages > 1) or (stride < pages and n > 1):
+            _bad(f"the rows of {what} must be dense and not overlap")
+        if most < 0:
+            _bad("the largest numbers of queries and keys must be >= 0")
+        most, pitch = min(most, pages * page_tokens), stride if n > 1 else pages
+        if most > _U32 or pitch > _U32:
+            _bad(f"the keys and the distance of two rows of {what} must be below 2^32")
+        return n, t.data_ptr(), pitch, most
+
+    def _queries(self, pool, q, out, to):
+        """q and out into a struct; their type's code."""
+        dtype, shape = q.dtype, q.shape
+        code = _code(dtype)
+        _rows(to.q, q, "q", self._device)
+        if out is not None:
+            _like(out, dtype, shape, "out")
+            _rows(to.out, out, "out", self._device)
+        if pool.device != self._device:
+            _elsewhere(pool.data, "the pool", self._device)
+        if shape[2] != pool.head_dim:
+            _bad(f"q has head_dim {shape[2]}, the pool {pool.head_dim}")
+        to.total_q, to.n_head = shape[0], shape[1]
+        return code
+
+    def shared_work(self, total_q, n_head, head_dim):
+        """float32 values of attention_shared's `work` for that many rows."""
+        if not (0 <= total_q <= _U32 and 0 <= n_head <= _U32 and 0 <= head_dim <= _U32):
+            _bad("total_q, n_head and head_dim must be >= 0 and below 2^32")
+        return self._lib.bp_kv4_shared_work(total_q, n_head, head_dim)
+
+    def attention_shared(self, pool, q, out, q_start, kv_len, page_table, prefix_start, prefix_len, prefix_table, work, max_q, max_kv, max_prefix, scale=None, stream=None):
+        """attention() for requests behind prefixes in common: the requests prefix_start[g] .. prefix_start[g + 1] see the prefix_len[g] keys in the
+        pages prefix_table[g], then their own. work: a float32 tensor of at least shared_work(...) values, for this call's partial results."""
+        a, device = self._shared, self._device
+        code = self._queries(pool, q, out, a)
+        n_req, a.page_table, a.table_stride, a.max_kv = self._table(page_table, "page_table", pool.page_tokens, max_kv)
+        n_prefix, a.prefix_table, a.prefix_stride, a.max_prefix = self._table(prefix_table, "prefix_table", pool.page_tokens, max_prefix)
+        if max_q < 0:
+            _bad("max_q must be >= 0")
+        total, heads = a.total_q, a.n_head
+        if work.get_device() != device:
+            _elsewhere(work, "work", device)
+        if str(work.dtype) != "torch.float32" or not work.is_contiguous() or work.numel() < self._lib.bp_kv4_shared_work(total, heads, pool.head_dim):
+            _bad("work must be dense float32 of at least shared_work(total_q, n_head, head_dim) values")
+        a.q_start, a.kv_len = _index(q_start, "q_start", n_req + 1, device), _index(kv_len, "kv_len", n_req, device)
+        a.prefix_start, a.prefix_len = _index(prefix_start, "prefix_start", n_prefix + 1, device), _index(prefix_len, "prefix_len", n_prefix, device)
+        a.work, a.n_req, a.n_prefix, a.max_q = work.data_ptr(), n_req, n_prefix, max_q if max_q < total else total
+        a.scale = pool.head_dim ** -0.5 if scale is None else scale
+        st = self._lib.bp_kv4_attention_shared(self._h, _current(device) if stream is None else _stream(stream), code, pool._p, self._pshared)
+        if st:
+            self._check(st)
+
+    def _summary(self, pool, summary):
+        if summary.device != self._device:
+            _elsewhere(summary.codes, "the summary", self._device)
+        if pool.device != self._device:
+            _elsewhere(pool.data, "the pool", self._device)
+        if summary.shape != (pool._c.n_pages, pool.n_kv_head, pool.head_dim):
+            _bad(f"the summary is of {summary.shape} pages, KV heads and dims, the pool of {(pool._c.n_pages, pool.n_kv_head, pool.head_dim)}")
+        return summary._p
+
+    def summarise(self, pool, summary, pages, n_tok=None, stream=None):
+        """The summaries of `pages` (int32; negative: none), of all their tokens or the first n_tok (int32) of each."""
+        p, n, device = self._summary(pool, summary), pages.shape[0] if pages.dim() == 1 else -1, self._device
+        st = self._lib.bp_kv4_summarise(self._h, _current(device) if stream is None else _stream(stream), pool._p, p, _index(pages, "pages", n, device),
+                                        None if n_tok is None else _index(n_tok, "n_tok", n, device), n)
+        if st:
+            self._check(st)
+
+    def select(self, pool, summary, q, pages, keys, q_start, kv_len, page_table, max_q, max_kv, first=1, last=1, stream=None):
+        """For every token and KV head the pages with the highest scores among those it sees, as many as pages [tokens, KV heads, pages] (int32) has
+        places, the first `first` and last `last` always; keys [tokens] (int32): the keys in them."""
+        p, a, device = self._summary(pool, summary), self._choice, self._device
+        code = self._queries(pool, q, None, a)
+        n_req, a.page_table, a.table_stride, a.max_kv = self._table(page_table, "page_table", pool.page_tokens, max_kv)
+        total = a.total_q
+        a.pages, a.chosen = self._lists(pool, pages, total)
+        if max_q < 0 or not (0 <= first <= _U32 and 0 <= last <= _U32):
+            _bad("max_q, first and last must be >= 0")
+        a.keys = _index(keys, "keys", total, device)
+        a.q_start, a.kv_len = _index(q_start, "q_start", n_req + 1, device), _index(kv_len, "kv_len", n_req, device)
+        a.n_req, a.max_q, a.first, a.last = n_req, max_q if max_q < total else total, first, last
+        st = self._lib.bp_kv4_select(self._h, _current(device) if stream is None else _stream(stream), code, pool._p, p, self._pchoice)
+        if st:
+            self._check(st)
+
+    def _lists(self, pool, pages, n):
+        if pages.get_device() != self._device:
+            _elsewhere(pages, "pages", self._device)
+        if pages.dtype is not _I32 or pages.dim() != 3 or pages.shape[0] != n or pages.shape[1] != pool.n_kv_head or not pages.is_contiguous():
+            _bad(f"pages must be dense int32 [{n}, {pool.n_kv_head}, pages], not {tuple(pages.shape)} {pages.dtype}")
+        return pages.data_ptr(), pages.shape[2]
+
+    def attention_selected(self, pool, q, out, pages, keys, scale=None, stream=None):
+        """Attention of every token of q [tokens, heads, head_dim] over the pages that select() has chosen for it."""
+        a, device = self._chosen, self._device
+        code = self._queries(pool, q, out, a)
+        a.pages, a.chosen = self._lists(pool, pages, a.total_q)
+        a.keys = _index(keys, "keys", a.total_q, device)
+        a.scale = pool.head_dim ** -0.5 if scale is None else scale
+        st = self._lib.bp_kv4_attention_selected(self._h, _current(device) if stream is None else _stream(stream), code, pool._p, self._pchosen)
+        if st:
+            self._check(st)
