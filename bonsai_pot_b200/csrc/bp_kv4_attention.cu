@@ -319,7 +319,13 @@ __device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4]
 #pragma unroll
         for (int k = 0; k < 4; k++) w.o[e][i][k] *= corr[k & 1];
     }
-    const float top[2] = {w.m[e][0] - P_UP, w.m[e][1] - P_UP};
+    // (where neighbouring numbers are 16 apart the difference may be 16, and f16 has no 2^16)
+    float top[2];
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      top[c] = w.m[e][c] - P_UP;
+      if (w.m[e][c] - top[c] > 15.f) top[c] = w.m[e][c];
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll

@@ -386,3 +386,16 @@ def test_rope_inverse_of_a_table_with_a_factor(ctx, layout, dim, rot):
         want[..., p] *= (0.1 * np.log(factor) + 1) ** 2
     near = np.abs(f64(rx)).max(-1, keepdims=True)
     assert (np.abs(f64(back) - want) <= 2.0 ** -9 * near * 1.3).all()  # rx and back are rounded to f16 once each, next to values of that size
+
+
+@pytest.mark.parametrize("top", [2.0 ** 24.5, 2.0 ** 25.5, 2.0 ** 26.5, 2.0 ** 27.5, 2.0 ** 28.5, 2.0 ** 30.5])
+@pytest.mark.parametrize("q", [1, 4])
+def test_weights_are_f16_numbers_whatever_the_largest_score(ctx, top, q):
+    """The largest score (log2 units) lies where neighbouring binary32 numbers are 2 to 128 apart: the weights' common factor must not pass f16. All
+    keys are one and the same: the output is its value."""
+    r = Requests(15, "f16", [q], [100], 4, 2, 64, 16)
+    k = torch.ones(100, 2, 64, dtype=torch.float16, device="cuda")
+    slots = torch.tensor([int(r.table[0, i // 16]) * 16 + i % 16 for i in range(100)], device="cuda")
+    ctx.append(r.pool, k, 3 * k, None, slots)
+    r.q.fill_(1.0)
+    assert (r.run(ctx, scale=top / 64 / 1.4426950408889634) == 3).all()
