@@ -352,31 +352,33 @@ class PagedContext:
         new tokens] are written for what is done with the tokens, -1 behind the last."""
         device, n = self._device, positions.shape[0] if positions.dim() == 1 else -1
         p, rows = self._tables(tables), tables.n_rows
-        st = self._lib.bp_pages_grow(self._h, _current(device) if stream is None else _stream(stream), p, _index(n_new, "n_new", rows, device), _index(q_start, "q_start", rows + 1, device),
-                                     _index(positions, "positions", n, device), _index(slots, "slots", n, device, True), n)
+        at = (_index(n_new, "n_new", rows, device), _index(q_start, "q_start", rows + 1, device), _index(positions, "positions", n, device), _index(slots, "slots", n, device, True))
+        st = self._lib.bp_pages_grow(self._h, _current(device) if stream is None else _stream(stream), p, *at, n)
         if st:
             self._check(st)
 
     def release(self, tables, rows, stream=None):
         """The rows (int32; negative: none) give their pages back and are empty."""
-        device, n = self._device, rows.shape[0] if rows.dim() == 1 else -1
-        st = self._lib.bp_pages_release(self._h, _current(device) if stream is None else _stream(stream), self._tables(tables), _index(rows, "rows", n, device), n)
+        device, n, p = self._device, rows.shape[0] if rows.dim() == 1 else -1, self._tables(tables)
+        rows = _index(rows, "rows", n, device)
+        st = self._lib.bp_pages_release(self._h, _current(device) if stream is None else _stream(stream), p, rows, n)
         if st:
             self._check(st)
 
     def fork(self, tables, parents, children, src, dst, stream=None):
         """Empty rows `children` become what `parents` are: full pages are shared, src and dst say which pages are to be copied (copy_pages)."""
+        p, device = self._tables(tables), self._device
         n, parents, children = self._pairs(parents, children, "parents", "children")
-        device = self._device
-        st = self._lib.bp_pages_fork(self._h, _current(device) if stream is None else _stream(stream), self._tables(tables), parents, children, n, _index(src, "src", n, device),
-                                     _index(dst, "dst", n, device))
+        src, dst = _index(src, "src", n, device), _index(dst, "dst", n, device)
+        st = self._lib.bp_pages_fork(self._h, _current(device) if stream is None else _stream(stream), p, parents, children, n, src, dst)
         if st:
             self._check(st)
 
     def compact(self, tables, src, dst, stream=None):
         """The highest used pages move into the lowest free ones, as many as src and dst have places; these say which pages are to be copied (copy_pages)."""
+        p = self._tables(tables)
         n, src, dst = self._pairs(src, dst, "src", "dst")
-        st = self._lib.bp_pages_compact(self._h, _current(self._device) if stream is None else _stream(stream), self._tables(tables), src, dst, n)
+        st = self._lib.bp_pages_compact(self._h, _current(self._device) if stream is None else _stream(stream), p, src, dst, n)
         if st:
             self._check(st)
 
@@ -462,8 +464,8 @@ class PagedContext:
     def summarise(self, pool, summary, pages, n_tok=None, stream=None):
         """The summaries of `pages` (int32; negative: none), of all their tokens or the first n_tok (int32) of each."""
         p, n, device = self._summary(pool, summary), pages.shape[0] if pages.dim() == 1 else -1, self._device
-        st = self._lib.bp_kv4_summarise(self._h, _current(device) if stream is None else _stream(stream), pool._p, p, _index(pages, "pages", n, device),
-                                        None if n_tok is None else _index(n_tok, "n_tok", n, device), n)
+        pages, n_tok = _index(pages, "pages", n, device), None if n_tok is None else _index(n_tok, "n_tok", n, device)
+        st = self._lib.bp_kv4_summarise(self._h, _current(device) if stream is None else _stream(stream), pool._p, p, pages, n_tok, n)
         if st:
             self._check(st)
 

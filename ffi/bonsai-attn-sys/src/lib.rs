@@ -13,6 +13,8 @@ use std::os::raw::{c_char, c_int, c_void};
 pub mod model;
 /// `include/bonsai_paged.h`: many requests over one paged KV cache held in 4 bits.
 pub mod paged;
+/// `include/bonsai_pages.h`: page tables, attention behind a prefix in common, attention over chosen pages.
+pub mod pages;
 
 /// Opaque context: owns `kv_k`, `kv_v`, the RoPE table and the split-KV scratch
 /// (what `Model` owns for this path, src/model.rs:1148-1248).
