@@ -275,7 +275,7 @@ __device__ __forceinline__ void values16(WarpState<D, NT>& w, const uint8_t* buf
 
 // P, still as the S^T fragments of four tiles, from the scores: masks (cut: some row may not see all of the unit, of which `left` keys are there), maximum, exponentials, sums; O is rescaled.
 template <int D, int NT, int MODE>
-__device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4][4], bool cut, int left, uint32_t tile0, int q_len, const AttnArgs& a, uint32_t lane) {
+__device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4][4], bool cut, int left, uint32_t tile0, int q_len, bool causal, const AttnArgs& a, uint32_t lane) {
   constexpr int NB = D / 32;
   const uint32_t g = lane >> 2;
 #pragma unroll
@@ -284,7 +284,7 @@ __device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4]
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         // the keys of the unit that row 2 t + c sees are [lo, hi); columns behind the request's rows are left as they are, nobody reads them
-        const int behind = MODE == PREFIX ? 0 : q_len - 1 - static_cast<int>((tile0 + 8 * e + 2 * (lane & 3) + c) / a.group);  // queries behind this one
+        const int behind = MODE == PARTS && !causal ? 0 : q_len - 1 - static_cast<int>((tile0 + 8 * e + 2 * (lane & 3) + c) / a.group);  // queries behind this one
         const int hi = behind < 0 ? left : left - behind, lo = a.window && behind >= 0 ? hi - static_cast<int>(a.window) : 0;
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -356,6 +356,7 @@ struct Shape {
 struct Request {
   int q0, q_len, kv_len, low;  // low: no query sees a key before it
   uint32_t units, tiles;       // units of 64 keys of an item; items per KV head (none without keys: there are only zeros to write)
+  uint32_t causal;
   __device__ int first() const { return low & ~static_cast<int>(UNIT - 1); }
 };
 template <int NT, int MODE>
@@ -365,7 +366,8 @@ __device__ __forceinline__ Request request(const AttnArgs& a, uint32_t r, bool r
   q.q0 = n.q0;
   q.q_len = n.q_len;
   q.kv_len = n.kv_len;
-  q.low = MODE == PREFIX ? 0 : min(first_seen(q.kv_len - q.q_len + 1, a.window), q.kv_len);
+  q.causal = is_causal<MODE>(a, r);
+  q.low = q.causal ? min(first_seen(q.kv_len - q.q_len + 1, a.window), q.kv_len) : 0;
   q.units = (static_cast<uint32_t>(q.kv_len - q.first()) + UNIT - 1) / UNIT;
   q.tiles = q.kv_len ? (static_cast<uint32_t>(q.q_len) * a.group + 8 * NT - 1) / (8 * NT) : 0;
   return q;
@@ -394,6 +396,7 @@ __device__ __forceinline__ void next_item(Cursor& c, const AttnArgs& a, const Re
 struct Piece {
   uint32_t used, start, units, head, row0, rows;
   int q0;
+  uint32_t prefix;
 };
 // An item whose pieces lie in several CTAs: one of this CTA's pieces of it, where it begins, over how many CTAs it goes.
 struct Join {
@@ -425,7 +428,7 @@ template <uint32_t PAGE, int MODE>
 __device__ __forceinline__ void load_ids(Fetch& f, const AttnArgs& a, const Cursor& c, uint32_t lane) {
   f.base = static_cast<uint32_t>(f.key0) / PAGE;
   f.ids = 0xffffffffu;
-  if (f.base + lane < (static_cast<uint32_t>(f.kv_len) + PAGE - 1) / PAGE) f.ids = static_cast<uint32_t>(a.page_table[(MODE == CHOSEN ? static_cast<size_t>(c.r) * a.pool.n_kv_head + c.head : c.r) * a.table_stride + f.base + lane]);
+  if (f.base + lane < (static_cast<uint32_t>(f.kv_len) + PAGE - 1) / PAGE) f.ids = static_cast<uint32_t>(pages_of<MODE>(a, c.r, c.head)[f.base + lane]);
 }
 template <uint32_t PAGE, int MODE>
 __device__ __forceinline__ void start_item(Fetch& f, const AttnArgs& a, const Cursor& c, uint32_t lane) {
@@ -514,7 +517,7 @@ __device__ __noinline__ uint32_t take_no_numbers(uint8_t* buf, int left, uint32_
 }
 
 // A warp: row `row` of the `n` partial results at part(k) of an item, in order, becomes the output's row.
-template <int D, int NT, int MODE, typename Part>
+template <int D, int NT, typename Part>
 __device__ __forceinline__ void join_row(const AttnArgs& a, const Piece& p, uint32_t row, uint32_t n, Part part, uint32_t lane) {
   using S = Shape<D, NT>;
   constexpr int V = D / 32;  // dims of a lane
@@ -550,13 +553,6 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, const Piece& p, uint
         o[1] = fmaf(e.y, wk, o[1]);
       }
     }
-  }
-  if constexpr (in_parts(MODE)) {
-    const size_t at = part_row(a, p.q0, p.head, p.row0 + row);
-#pragma unroll
-    for (int x = 0; x < V; x++) a.part[at * D + V * lane + x] = o[x];
-    if (lane == 0) a.part_ml[at] = make_float2(m, l);
-    return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* out = out_row(a, p.q0, p.head, p.row0 + row) + V * lane;
@@ -600,11 +596,11 @@ __device__ __forceinline__ void join_rows4(const AttnArgs& a, const Piece& p, ui
     if ((lane & 7) == 0) *reinterpret_cast<float2*>(to + at + D) = make_float2(m, l);
     return;
   }
-  if constexpr (in_parts(MODE)) {
-    const size_t where = part_row(a, p.q0, p.head, p.row0 + row);
+  if constexpr (MODE == PARTS) {
+    float* record = record_of<D>(a, p.prefix, p.q0, p.head, p.row0 + row);
 #pragma unroll
-    for (int x = 0; x < V; x++) *reinterpret_cast<float4*>(a.part + where * D + 32 * x + col) = o[x];
-    if ((lane & 7) == 0) a.part_ml[where] = make_float2(m, l);
+    for (int x = 0; x < V; x++) *reinterpret_cast<float4*>(record + 32 * x + col) = o[x];
+    if ((lane & 7) == 0) end_record<D>(record, m, l);
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -615,9 +611,10 @@ __device__ __forceinline__ void join_rows4(const AttnArgs& a, const Piece& p, ui
 
 // Zeros for the `n_tok` tokens of a request without keys, by a CTA. (Their values can be more than 32 bits count.) In parts: no weights.
 template <int D, int MODE>
-__device__ __noinline__ void zero_rows(const AttnArgs& a, int q0, uint32_t n_tok) {
-  if constexpr (in_parts(MODE)) {
-    for (size_t i = threadIdx.x; i < static_cast<size_t>(n_tok) * a.n_head; i += blockDim.x) a.part_ml[static_cast<size_t>(q0) * a.n_head + i] = make_float2(NEG_BIG, 0.f);
+__device__ __noinline__ void zero_rows(const AttnArgs& a, int q0, uint32_t n_tok, bool prefix) {
+  if constexpr (MODE == PARTS) {
+    float* record = a.part + ((prefix ? 0 : static_cast<size_t>(a.total_q) * a.n_head) + static_cast<size_t>(q0) * a.n_head) * RECORD<D>;
+    for (size_t i = threadIdx.x; i < static_cast<size_t>(n_tok) * a.n_head; i += blockDim.x) end_record<D>(record + i * RECORD<D>, NEG_BIG, 0.f);
     return;
   }
   const uint32_t step = blockDim.x / (D / 4), dt = step / a.n_head, dh = step % a.n_head;  // rows that the CTA writes at a time
@@ -658,8 +655,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
   if (lane < 2) pieces[2 * warp + lane].used = 0;
   if (threadIdx.x == 0) items_s = most_s = 0;
   __syncthreads();
-  pdl_launch_dependents();
-  pdl_wait();
+  const bool beside = MODE == PARTS && a.beside;
+  if (!(MODE == PARTS && a.first)) pdl_launch_dependents();
+  if (!beside) pdl_wait();
+  if (MODE == PARTS && a.first) pdl_launch_dependents();
 
   // ---- the line of units ----
   const uint32_t per = (a.n_req + THREADS - 1) / THREADS;
@@ -726,7 +725,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
   };
   for (uint32_t r = blockIdx.x; r < a.n_req; r += n_cta) {
     const Request q = known ? known[r] : request<NT, MODE>(a, r, false);
-    if (q.kv_len == 0) zero_rows<D, MODE>(a, q.q0, q.q_len);
+    if (q.kv_len == 0) zero_rows<D, MODE>(a, q.q0, q.q_len, !q.causal);
   }
   // One item per CTA where that takes at most one round of the warps more than equal stretches, which need their pieces
   // joined; else equal stretches, of one unit per warp at least.
@@ -752,7 +751,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
     c0 = min(static_cast<uint64_t>(blockIdx.x) * share, static_cast<uint64_t>(total));
     c1 = c0 + min(share, total - c0);
   }
-  if (c0 >= c1) return;  // (all threads)
+  if (c0 >= c1) {  // (all threads)
+    if (beside) pdl_wait();
+    return;
+  }
   if (threadIdx.x == 0) {
     plan[0] = c0;
     plan[1] = c1;
@@ -838,14 +840,15 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
       }
       const int q_len = cur.q.q_len;
       // (every row of a prefix sees the same keys)
-      const bool cut = MODE == PREFIX ? u.left < static_cast<int>(UNIT) : u.left - static_cast<int>(UNIT) < q_len - 1 || (a.window && u.left > static_cast<int>(a.window));
-      softmax64<D, NT, MODE>(w, s, cut, u.left, cur.tile * S::ROWS, q_len, a, lane);
+      const bool causal = MODE != PARTS || cur.q.causal;
+      const bool cut = u.left - static_cast<int>(UNIT) < (causal ? q_len - 1 : 0) || (a.window && u.left > static_cast<int>(a.window));
+      softmax64<D, NT, MODE>(w, s, cut, u.left, cur.tile * S::ROWS, q_len, causal, a, lane);
       ok = wait();
       if (!ok) break;
       {
         uint8_t* vb = buf + b * S::PART;
         if (part) clear_scales<D, PAGE>(vb, u.pages, u.low, u.left);
-        if (MODE != PREFIX && cut && q_len > 1 && __any_sync(FULL, (blocks_without_numbers<D, PAGE>(vb, lane) | blocks_without_numbers<D, PAGE>(vb, lane + 32)) != 0)) {
+        if (cut && causal && q_len > 1 && __any_sync(FULL, (blocks_without_numbers<D, PAGE>(vb, lane) | blocks_without_numbers<D, PAGE>(vb, lane + 32)) != 0)) {
           const uint32_t spoiled = take_no_numbers<D, NT, PAGE>(vb, u.left, cur.tile * S::ROWS, q_len, a.group, a.window);
 #pragma unroll
           for (int e = 0; e < NT; e++)
@@ -881,12 +884,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
             for (int c = 0; c < 2; c++) {
               const uint32_t row = row0 + 8 * e + 2 * t + c;
               if (row >= n_rows) continue;
-              if constexpr (in_parts(MODE)) {
-                const size_t at = part_row(a, cur.q.q0, cur.head, row);
+              if constexpr (MODE == PARTS) {
+                float* record = record_of<D>(a, !cur.q.causal, cur.q.q0, cur.head, row);
 #pragma unroll
                 for (int x = 0; x < NB; x++)
-                  *reinterpret_cast<float4*>(a.part + at * D + 32 * x + 4 * g) = make_float4(w.o[e][2 * x][c], w.o[e][2 * x][c + 2], w.o[e][2 * x + 1][c], w.o[e][2 * x + 1][c + 2]);
-                if (g == 0) a.part_ml[at] = make_float2(w.m[e][c], w.l[e][c]);
+                  *reinterpret_cast<float4*>(record + 32 * x + 4 * g) = make_float4(w.o[e][2 * x][c], w.o[e][2 * x][c + 2], w.o[e][2 * x + 1][c], w.o[e][2 * x + 1][c + 2]);
+                if (g == 0) end_record<D>(record, w.m[e][c], w.l[e][c]);
                 continue;
               }
               const float inv = w.l[e][c] == 0.f ? 0.f : 1.f / w.l[e][c];
@@ -910,7 +913,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
               if (g == 0) *reinterpret_cast<float2*>(p + D) = make_float2(w.m[e][c], w.l[e][c]);
             }
           if (lane == 0)
-            pieces[2 * warp + (last ? 1 : 0)] = Piece{1, plan[0] + begin + first - cur.unit, cur.q.units, cur.head, row0, min(S::ROWS, n_rows - row0), cur.q.q0};
+            pieces[2 * warp + (last ? 1 : 0)] = Piece{1, plan[0] + begin + first - cur.unit, cur.q.units, cur.head, row0, min(S::ROWS, n_rows - row0), cur.q.q0, !cur.q.causal};
         }
         fresh = true;
         if (i + 1 < n) {
@@ -952,11 +955,17 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
         }, to, lane);
       if (++turn == NWARP) turn = 0;
     }
+    if constexpr (MODE == PARTS) {  // (the CTA with an item's first piece says where they all are)
+      if (!all && blockIdx.x == first_cta && threadIdx.x < p.rows)
+        end_record<D>(record_of<D>(a, p.prefix, p.q0, p.head, p.row0 + threadIdx.x), NEG_BIG, 0.f, first_cta, (p.start + p.units - 1) / plan[2] - first_cta + 1, threadIdx.x);
+      continue;
+    }
     if (!all) {  // an item that began before the stretch, one that goes on behind it
       if (threadIdx.x == 0) joins[n_joins] = Join{i, first_cta, (p.start + p.units - 1) / plan[2] - first_cta + 1, 0};
       n_joins++;
     }
   }
+  if (beside) pdl_wait();
   if (n_joins == 0) return;  // (all threads)
 
   // ---- items of several CTAs: the one that comes last joins them ----
@@ -978,7 +987,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
     for (uint32_t row = 0; row < p.rows; row += step) {
       if (turn == warp) {
         if (step == 4) join_rows4<D, NT, MODE>(a, p, row, j.n, part, nullptr, lane);
-        else join_row<D, NT, MODE>(a, p, row, j.n, part, lane);
+        else join_row<D, NT>(a, p, row, j.n, part, lane);
       }
       if (++turn == NWARP) turn = 0;
     }
@@ -1013,8 +1022,7 @@ cudaError_t allow_shared_memory() {
 
 cudaError_t bp_kv4_attention_init(bp_paged_ctx* c) {
   cudaError_t e = allow_shared_memory<PLAIN>();
-  if (e == cudaSuccess) e = allow_shared_memory<PREFIX>();
-  if (e == cudaSuccess) e = allow_shared_memory<OWN>();
+  if (e == cudaSuccess) e = allow_shared_memory<PARTS>();
   if (e == cudaSuccess) e = allow_shared_memory<CHOSEN>();
   if (e != cudaSuccess) return e;
   // a piece per warp and two per CTA, of the instance that needs most
@@ -1052,25 +1060,16 @@ void bp_kv4_attention_args(const bp_paged_ctx* c, bool bf, const Pool& pool, con
   a->q_vec = reinterpret_cast<uintptr_t>(q.data) % 16 == 0 && q.tok_stride % 8 == 0 && q.head_stride % 8 == 0;
 }
 
-cudaError_t bp_launch_kv4_rows(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, int mode, uint64_t rows, const AttnArgs& a) {
-  // Which kernel. Here the codes are expanded once per 16 rows (tokens x query heads per KV head) of a request, there once for up to 128, with some 14 us
-  // for an item's beginning and end. us, this kernel / the other one:
-  //   head_dim 128, 32 / 8 heads         16 rows  32 rows  48 rows     head_dim 64, 40 / 8 heads    15 rows  30 rows  40 rows  50 rows
-  //   16 requests of 4096 keys           41/75    68/75    97/76                                    28/60    47/61    60/61    78/61
-  //   the same, window 1024              19/36    31/36    38/36                                    15/28    24/29    26/29    30/29
-  //   64 requests of 1000 keys           46/85    78/87    113/88                                   29/70    50/70    65/71    85/72
-  //   1 request of 30000 keys            33/64    48/63    62/64                                    27/45    36/45    42/45    50/45
-  // and as much apart with 2, 4 and 8 requests of 4096 keys and with 2 KV heads; so 32 rows is the line for both.
-  // (Without any key there are only zeros to write, and there may be no pool: this kernel looks at none. Chosen pages are those of one token.)
-  if (a.max_kv != 0 && rows > 32 && mode != CHOSEN) return bp_launch_kv4_prefill(c, s, head_dim, mode, a);
+cudaError_t bp_launch_kv4_few_rows(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, int mode, uint64_t rows, uint32_t ctas, const AttnArgs& a, const float** slots, uint32_t* piece) {
+  const uint32_t grid = ctas ? ctas : c->sm_count;
   auto launch = [&](auto kernel, auto shape) {
-    return bp_launch(true, kernel, dim3(c->sm_count), dim3(shape.THREADS), shape.SMEM, s, a, c->partials, c->counters);
+    using S = decltype(shape);
+    if (slots) *slots = c->partials + static_cast<size_t>(grid) * S::NWARP * S::PARTIAL;
+    if (piece) *piece = S::PARTIAL;
+    return bp_launch(true, kernel, dim3(grid), dim3(S::THREADS), S::SMEM, s, a, c->partials, c->counters);
   };
   const bool two = rows > 8;
-  return mode == PLAIN    ? with_kernel<PLAIN>(head_dim, two, a.pool.page, launch)
-         : mode == PREFIX ? with_kernel<PREFIX>(head_dim, two, a.pool.page, launch)
-         : mode == OWN    ? with_kernel<OWN>(head_dim, two, a.pool.page, launch)
-                          : with_kernel<CHOSEN>(head_dim, two, a.pool.page, launch);
+  return mode == PLAIN ? with_kernel<PLAIN>(head_dim, two, a.pool.page, launch) : mode == PARTS ? with_kernel<PARTS>(head_dim, two, a.pool.page, launch) : with_kernel<CHOSEN>(head_dim, two, a.pool.page, launch);
 }
 
 // Pages of a row of a page table that are looked at: what 31 bits of keys fill at most.
@@ -1089,5 +1088,16 @@ cudaError_t bp_launch_kv4_attention(bp_paged_ctx* c, cudaStream_t s, bool bf, co
   a.table_stride = in.table_stride;
   a.table_pages = bp_kv4_table_pages(pool, in.table_stride);
   a.window = in.window < in.max_kv ? in.window : 0;  // (nobody has more keys)
-  return bp_launch_kv4_rows(c, s, head_dim, PLAIN, static_cast<uint64_t>(a.max_q) * a.group, a);
+  // Which kernel. Here the codes are expanded once per 16 rows (tokens x query heads per KV head) of a request, there once for up to 128, with some 14 us
+  // for an item's beginning and end. us, this kernel / the other one:
+  //   head_dim 128, 32 / 8 heads         16 rows  32 rows  48 rows     head_dim 64, 40 / 8 heads    15 rows  30 rows  40 rows  50 rows
+  //   16 requests of 4096 keys           41/75    68/75    97/76                                    28/60    47/61    60/61    78/61
+  //   the same, window 1024              19/36    31/36    38/36                                    15/28    24/29    26/29    30/29
+  //   64 requests of 1000 keys           46/85    78/87    113/88                                   29/70    50/70    65/71    85/72
+  //   1 request of 30000 keys            33/64    48/63    62/64                                    27/45    36/45    42/45    50/45
+  // and as much apart with 2, 4 and 8 requests of 4096 keys and with 2 KV heads; so 32 rows is the line for both.
+  const uint64_t rows = static_cast<uint64_t>(a.max_q) * a.group;
+  // (Without any key there are only zeros to write, and there may be no pool: this kernel looks at none.)
+  if (a.max_kv != 0 && rows > BP_KV4_FEW_ROWS) return bp_launch_kv4_prefill(c, s, head_dim, PLAIN, rows, 0, a);
+  return bp_launch_kv4_few_rows(c, s, head_dim, PLAIN, rows, 0, a);
 }

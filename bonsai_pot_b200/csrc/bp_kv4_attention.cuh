@@ -12,14 +12,18 @@ constexpr float P_UP = 10.f;   // P is stored as f16 times 2^10: it keeps its bi
 
 // What a kernel's line of requests is.
 enum Mode {
-  PLAIN,    // requests, their outputs are written
-  PREFIX,   // prefixes that several requests have in common: their rows are those of all these requests, each sees every key; parts
-  OWN,      // requests behind their prefixes; parts
-  CHOSEN,   // tokens that see every key of pages chosen for each KV head; their outputs are written
+  PLAIN,   // requests, their outputs are written
+  PARTS,   // prefixes that several requests have in common (their rows are those of all these requests, each sees every key), then requests behind
+           // their prefixes: either sees a part of a row's keys only, and what comes out are partial results
+  CHOSEN,  // tokens that see every key of pages chosen for each KV head; their outputs are written
 };
-// Where a part of the keys is all that a kernel sees, its rows become partial results in memory instead of outputs: the sums as they are, their
-// maximum (log2 units) and the sum of the weights. bp_kv4_shared.cu puts them together.
-__host__ __device__ constexpr bool in_parts(int mode) { return mode == PREFIX || mode == OWN; }
+// A partial result of a row: [0, D) the values' sum, [D] the largest score (log2 units), [D + 1] the sum of the weights, then as whole numbers [D + 2] c and
+// [D + 3] n << 16 | r. n = 0: that is it. n > 0: n CTAs from c on have a piece of it each, at row r of their place for pieces (piece_at).
+// bp_kv4_shared.cu puts them together.
+template <int D>
+constexpr uint32_t RECORD = D + 4;
+// CTA c + k's place for pieces is the k-th of an item's: a CTA has at most two, of the item that ends in it and of the one that goes on behind it.
+__host__ __device__ constexpr uint32_t piece_at(uint32_t c, uint32_t k) { return 2 * (c + k) + (k == 0); }
 
 struct AttnArgs {
   Pool pool;
@@ -34,11 +38,12 @@ struct AttnArgs {
   uint32_t bias;  // 0x64006400: two f16 numbers 1024
   uint32_t bf;    // activations are bfloat16
   uint32_t q_vec; // rows of q are 16-byte aligned
-  // in parts
-  float* part;          // [rows of q][n_head][head_dim]
-  float2* part_ml;      // [rows of q][n_head]
-  const int32_t* prefix_start;  // PREFIX: request r is a prefix, of the requests [prefix_start[r], prefix_start[r + 1]) of n_all
-  uint32_t n_all;
+  // PARTS: requests [0, n_prefix) are prefixes, prefix g that of the requests [prefix_start[g], prefix_start[g + 1]) of n_req - n_prefix
+  const int32_t *prefix_start, *prefix_len, *prefix_table;
+  uint32_t n_prefix, n_own, max_prefix, prefix_stride, prefix_pages;
+  float* part;  // [prefix, own][rows of q][n_head] records
+  // The launch before this one has waited for what is read here and runs at the same time; it is waited for at the end. (first: this is that launch)
+  uint32_t beside, first;
 };
 // Queries become f16 numbers, each row multiplied by the power of two that brings its largest element into [2^8, 2^9): the most for which 32 of them
 // times a mantissa add up within f16, as bp_kv4_attention.cu wants. f16 and bf16 queries keep all their bits down to 2^-18 of the row's largest element,
@@ -58,26 +63,42 @@ struct Lengths {
 };
 template <int MODE>
 __device__ __forceinline__ Lengths lengths_of(const AttnArgs& a, uint32_t r, bool report) {
-  const int keys = a.kv_len[r];
-  int start, stop;
-  if constexpr (MODE == PREFIX) {
-    const int from = a.prefix_start[r], to = a.prefix_start[r + 1], last = static_cast<int>(a.n_all), f = min(max(from, 0), last), t = min(max(to, f), last);
+  int keys, start, stop;
+  uint32_t most = a.max_q, most_keys = min(a.max_kv, a.table_pages << a.pool.log_page);
+  if (MODE == PARTS && r < a.n_prefix) {
+    const int from = a.prefix_start[r], to = a.prefix_start[r + 1], last = static_cast<int>(a.n_own), f = min(max(from, 0), last), t = min(max(to, f), last);
     if (report && (f != from || t != to)) note_range(a.err);
+    keys = a.prefix_len[r];
     start = a.q_start[f];
     stop = a.q_start[t];
+    most = a.total_q;
+    most_keys = min(a.max_prefix, a.prefix_pages << a.pool.log_page);
   } else if constexpr (MODE == CHOSEN) {  // (a negative number of keys: a token of no request)
+    keys = a.kv_len[r];
     start = static_cast<int>(r);
     stop = start + (keys >= 0);
   } else {
+    if (MODE == PARTS) r -= a.n_prefix;
+    keys = a.kv_len[r];
     start = a.q_start[r];
     stop = a.q_start[r + 1];
   }
   const int q0 = max(start, 0);
   const int given_q = max(stop, q0) - q0, given_kv = max(keys, 0);
-  const Lengths n{q0, min(min(given_q, static_cast<int>(a.max_q)), max(static_cast<int>(a.total_q) - q0, 0)),
-                  min(given_kv, static_cast<int>(min(a.max_kv, a.table_pages << a.pool.log_page)))};
+  const Lengths n{q0, min(min(given_q, static_cast<int>(most)), max(static_cast<int>(a.total_q) - q0, 0)), min(given_kv, static_cast<int>(most_keys))};
   if (report && (given_q > n.q_len || given_kv > n.kv_len || (start < 0 && stop > start))) note_range(a.err);
   return n;
+}
+// Whether the queries of request r see its keys up to their own (or all of them); its row of pages, for KV head `head`.
+template <int MODE>
+__device__ __forceinline__ bool is_causal(const AttnArgs& a, uint32_t r) {
+  return MODE != PARTS || r >= a.n_prefix;
+}
+template <int MODE>
+__device__ __forceinline__ const int32_t* pages_of(const AttnArgs& a, uint32_t r, uint32_t head) {
+  if (MODE == PARTS && r < a.n_prefix) return a.prefix_table + static_cast<size_t>(r) * a.prefix_stride;
+  const size_t row = MODE == CHOSEN ? static_cast<size_t>(r) * a.pool.n_kv_head + head : MODE == PARTS ? r - a.n_prefix : r;
+  return a.page_table + row * a.table_stride;
 }
 // A bounded wait for a barrier's phase: false after 2^20 polls or two seconds, or when *stop (may be null) is set.
 __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const volatile uint32_t* stop = nullptr) {
@@ -122,17 +143,27 @@ __device__ __forceinline__ void store4(bool bf, uint16_t* p, float a, float b, f
 __device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, int q0, uint32_t head, uint32_t row) {
   return a.out.data + static_cast<int64_t>(q0 + row / a.group) * a.out.tok + static_cast<int64_t>(head * a.group + row % a.group) * a.out.head;
 }
-// The same row among the partial results.
-__device__ __forceinline__ size_t part_row(const AttnArgs& a, int q0, uint32_t head, uint32_t row) {
-  return static_cast<size_t>(q0 + row / a.group) * a.n_head + head * a.group + row % a.group;
+// The same row's record, of the prefix or the own keys.
+template <int D>
+__device__ __forceinline__ float* record_of(const AttnArgs& a, bool prefix, int q0, uint32_t head, uint32_t row) {
+  const size_t at = static_cast<size_t>(q0 + row / a.group) * a.n_head + head * a.group + row % a.group;
+  return a.part + ((prefix ? 0 : static_cast<size_t>(a.total_q) * a.n_head) + at) * RECORD<D>;
+}
+template <int D>
+__device__ __forceinline__ void end_record(float* record, float m, float l, uint32_t c = 0, uint32_t n = 0, uint32_t r = 0) {
+  *reinterpret_cast<float4*>(record + D) = make_float4(m, l, __uint_as_float(c), __uint_as_float(n << 16 | r));
 }
 
 }  // namespace kv4
 }  // namespace bp
 
 cudaError_t bp_kv4_prefill_init(bp_paged_ctx* c);
-cudaError_t bp_launch_kv4_prefill(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, int mode, const bp::kv4::AttnArgs& a);
-// The scale and what belongs to the context and the pool; then either kernel, by the rows of an item (`rows` of a request at most).
+// Launches over `ctas` CTAs (0: all); rows: of an item at most. In PARTS pieces go to *slots, `piece` floats each.
+cudaError_t bp_launch_kv4_prefill(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, int mode, uint64_t rows, uint32_t ctas, const bp::kv4::AttnArgs& a,
+                                  const float** slots = nullptr, uint32_t* piece = nullptr);
+cudaError_t bp_launch_kv4_few_rows(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, int mode, uint64_t rows, uint32_t ctas, const bp::kv4::AttnArgs& a,
+                                   const float** slots = nullptr, uint32_t* piece = nullptr);
+constexpr uint64_t BP_KV4_FEW_ROWS = 32;  // of a request, that the kernel for few rows takes (bp_kv4_attention.cu has the reason)
+// The scale and what belongs to the context and the pool.
 uint32_t bp_kv4_table_pages(const bp::Pool& pool, uint32_t stride);
 void bp_kv4_attention_args(const bp_paged_ctx* c, bool bf, const bp::Pool& pool, const bp_rows& q, const bp_rows& out, uint32_t n_head, float scale, bp::kv4::AttnArgs* a);
-cudaError_t bp_launch_kv4_rows(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, int mode, uint64_t rows, const bp::kv4::AttnArgs& a);

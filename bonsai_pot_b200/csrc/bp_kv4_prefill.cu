@@ -36,7 +36,9 @@ constexpr uint32_t SLOTS = 4;          // K and V tiles in shared memory
 // Tiles of which some rows of an item see only a part: its rows are 256 tokens at most, so these are 5 tiles at each end of the keys that they see; where a
 // window is so short that no tile lies between the two ends, the two overlap or are less than two tiles apart: 11 tiles.
 constexpr uint32_t MIXED = 11;
-constexpr uint32_t ITEM_COST = 6;      // what beginning and ending an item costs, in key tiles
+// What beginning and ending an item costs, in key tiles.
+template <int MODE>
+constexpr uint32_t ITEM_COST = MODE == PARTS ? 14 : 6;
 constexpr float GROW = 5.f;            // log2 by which a maximum may grow before O is rescaled; P_UP + GROW stays below 16
 
 template <int D, uint32_t NQ>
@@ -48,11 +50,12 @@ struct Shape {
   static constexpr uint32_t FIRST_EXPANDER = 4, FIRST_SOFTMAX = 12;       // warps 0, 1: O issuers, 2, 3: S issuers
   static constexpr uint32_t NWARP = FIRST_SOFTMAX + 4 * NQ, THREADS = 32 * NWARP;
   static constexpr uint32_t PARTIAL = ROWS * (D + 2);                     // floats of a partial result: o as fours [dims / 4][row], (m, l) [row]
+  static constexpr uint32_t PIECE = ROWS * RECORD<D>;                     // the same in PARTS: a record per row
 };
 
 struct Request {
   int q0, q_len, kv_len;
-  uint32_t rows;
+  uint32_t rows, causal;
 };
 template <int MODE>
 __device__ __forceinline__ Request request(const AttnArgs& a, uint32_t r, bool report) {
@@ -62,6 +65,7 @@ __device__ __forceinline__ Request request(const AttnArgs& a, uint32_t r, bool r
   q.q_len = n.q_len;
   q.kv_len = n.kv_len;
   q.rows = static_cast<uint32_t>(q.q_len) * a.group;
+  q.causal = is_causal<MODE>(a, r);
   return q;
 }
 // Keys [low, high) that the rows [row0, row0 + rows) of a request see, of all of them together; key tiles from low's on, one at least (its
@@ -75,7 +79,7 @@ struct Keys {
 template <int MODE>
 __device__ __forceinline__ Keys keys_of(const AttnArgs& a, const Request& q, uint32_t row0, uint32_t rows) {
   Keys k;
-  if constexpr (MODE == PREFIX) {
+  if (MODE == PARTS && !q.causal) {
     k.low = k.all_from = 0;
     k.high = k.all_to = q.kv_len;
     k.tiles = max((static_cast<uint32_t>(q.kv_len) + BN - 1) / BN, 1u);
@@ -223,8 +227,9 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base_s;
-  pdl_launch_dependents();
+  if (!(MODE == PARTS && a.first)) pdl_launch_dependents();
   pdl_wait();
+  if (MODE == PARTS && a.first) pdl_launch_dependents();
 
   // After one wait has given up no other one waits.
   auto waitx = [&](uint64_t* bar, uint32_t parity) {
@@ -241,7 +246,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   const uint32_t per = (a.n_req + THREADS - 1) / THREADS;
   auto tiles_of = [&](const Request& q) {  // of all items of a request
     uint32_t n = 0;
-    for (uint32_t row0 = 0; row0 < q.rows; row0 += S::ROWS) n += keys_of<MODE>(a, q, row0, S::ROWS).tiles + ITEM_COST;
+    for (uint32_t row0 = 0; row0 < q.rows; row0 += S::ROWS) n += keys_of<MODE>(a, q, row0, S::ROWS).tiles + ITEM_COST<MODE>;
     return n * a.pool.n_kv_head;
   };
   {
@@ -272,10 +277,10 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       const Request q = request<MODE>(a, r, false);
       for (uint32_t x = 0; x * S::ROWS < q.rows; x++) {
         const Keys k = keys_of<MODE>(a, q, x * S::ROWS, S::ROWS);
-        const uint32_t places = k.tiles + ITEM_COST, n = places * a.pool.n_kv_head;
+        const uint32_t places = k.tiles + ITEM_COST<MODE>, n = places * a.pool.n_kv_head;
         if (left < n) {
           const uint32_t head = left / places, in = left - head * places;
-          cur = Cursor{q, k, r, x, head, in > ITEM_COST ? in - ITEM_COST : 0, c0 - in + ITEM_COST};
+          cur = Cursor{q, k, r, x, head, in > ITEM_COST<MODE> ? in - ITEM_COST<MODE> : 0, c0 - in + ITEM_COST<MODE>};
           found = true;
           break;
         }
@@ -383,7 +388,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     } else if (warp < S::FIRST_SOFTMAX) {
       // ---------------- codes -> operand tiles ----------------
       const uint32_t quarter = lane >> 3, row = 8 * (warp - S::FIRST_EXPANDER) + (lane & 7);  // a warp: all of eight tokens, eight rows per 16-byte phase
-      const int32_t* table = a.page_table + static_cast<size_t>(cur.r) * a.table_stride;
+      const int32_t* table = pages_of<MODE>(a, cur.r, head);
       // Page ids are asked for two tiles ahead and looked at one tile ahead, when the codes are asked for: nothing here waits for memory.
       // A token that holds no key of the request (or lies in a page outside the pool) gets page 0's codes, and zeros for its scales.
       auto has_key = [&](int key) { return key >= keys.low && key < keys.high; };
@@ -438,7 +443,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       const float scale = row_scale[x * BM + r];
       // this row sees the keys [lo, hi)
       const int past = q.kv_len - q.q_len;
-      const int hi = row >= q.rows ? 0 : MODE == PREFIX ? q.kv_len : past + static_cast<int>(row / a.group) + 1, lo = MODE == PREFIX ? 0 : first_seen(hi, a.window);
+      const int hi = row >= q.rows ? 0 : MODE == PARTS && !q.causal ? q.kv_len : past + static_cast<int>(row / a.group) + 1, lo = MODE == PARTS ? 0 : first_seen(hi, a.window);
       float m_run = NEG_BIG, l_run = 0.f;
       for (uint32_t i = 0; i < n; i++) {
         const uint32_t c = done + i, b = c & 1, s = c % SLOTS;
@@ -525,25 +530,48 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       (void)waitx(&o_done[x], pieces & 1);
       __syncwarp();
       tc_fence_after();
-      if (in_parts(MODE) && first == 0 && n == keys.tiles) {
-        // ---- the whole item, as a partial result of its rows ----
-        const size_t at = row < q.rows ? part_row(a, q.q0, head, row) : 0;
+      if constexpr (MODE == PARTS) {
+        // ---- a record per row: in its own place, or as a piece of an item that several CTAs have, whose first one says where they are ----
+        const uint32_t first_cta = start / share, parts = (start + keys.tiles - 1) / share - first_cta + 1;
+        const bool all = first == 0 && n == keys.tiles;
+        float* record = row < q.rows ? record_of<D>(a, !q.causal, q.q0, head, row) : nullptr;
+        float* to = all ? record : scratch + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PIECE + (x * BM + r) * RECORD<D>;
+        const bool there = record && !abort_s;
+        // half the dims at a time through the dead Q tile, so that a row's 2 D bytes go to memory together
+        constexpr uint32_t U = D / 8;
+        uint8_t* stage = smem + x * S::Q_B;
+        const uint32_t rows = min(BM, q.rows - min(tile_row, q.rows));
 #pragma unroll 1
-        for (uint32_t k = 0; k < D / 16; k++) {
-          uint32_t o[16];
-          tmem_ld16(o_addr + 16 * k, o);
-          tmem_ld_wait();
-          if (row >= q.rows || abort_s) continue;
-          const bool none = over >> (k >> 1) & 1;
+        for (uint32_t half = 0; half < 2; half++) {
+          if (half) named_bar_sync(1 + x, 128);  // (what was staged before has gone)
+#pragma unroll 1
+          for (uint32_t k = 0; k < D / 32; k++) {
+            uint32_t o[16];
+            tmem_ld16(o_addr + D / 2 * half + 16 * k, o);
+            tmem_ld_wait();
+            const bool none = over >> (D / 64 * half + (k >> 1)) & 1;
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            float v[4];
+            for (int e = 0; e < 4; e++) {
+              float v[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = none ? __int_as_float(0x7fffffff) : __uint_as_float(o[8 * (e >> 1) + column_of(4 * (e & 1) + j)]);
-            *reinterpret_cast<float4*>(a.part + at * D + 16 * k + 4 * e) = make_float4(v[0], v[1], v[2], v[3]);
+              for (int j = 0; j < 4; j++) v[j] = none ? __int_as_float(0x7fffffff) : __uint_as_float(o[8 * (e >> 1) + column_of(4 * (e & 1) + j)]);
+              *reinterpret_cast<float4*>(stage + r * (2 * D) + (((4 * k + e) ^ (r & (U - 1))) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+          }
+          named_bar_sync(1 + x, 128);
+          if (!abort_s) {
+#pragma unroll 4
+            for (uint32_t k = r; k < rows * U; k += 128) {
+              const uint32_t row_in = k / U, u = k % U;
+              float* row_to = all ? record_of<D>(a, !q.causal, q.q0, head, tile_row + row_in) : scratch + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PIECE + (x * BM + row_in) * RECORD<D>;
+              *reinterpret_cast<float4*>(row_to + D / 2 * half + 4 * u) = *reinterpret_cast<const float4*>(stage + row_in * (2 * D) + ((u ^ (row_in & (U - 1))) << 4));
+            }
           }
         }
-        if (row < q.rows && !abort_s) a.part_ml[at] = make_float2(l_run == 0.f ? NEG_BIG : m_run * scale, l_run);
+        if (there) {
+          end_record<D>(to, l_run == 0.f ? NEG_BIG : m_run * scale, l_run);
+          if (!all && blockIdx.x == first_cta) end_record<D>(record, NEG_BIG, 0.f, first_cta, parts, x * BM + r);
+        }
       } else if (first == 0 && n == keys.tiles) {
         // ---- the whole item: O / l through the dead Q tile, whole rows of it to memory ----
         const float inv_l = l_run == 0.f ? 0.f : 1.f / l_run;
@@ -599,7 +627,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     if (abort_s) break;
 
     // ---- an item of several CTAs is joined by the one that comes last ----
-    const bool whole = first == 0 && n == keys.tiles;
+    const bool whole = MODE == PARTS || (first == 0 && n == keys.tiles);  // (parts are joined by another kernel)
     if (threadIdx.x == 0) {
       if (!whole) {
         const uint32_t first_cta = start / share, parts = (start + keys.tiles - 1) / share - first_cta + 1;
@@ -610,7 +638,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       if (pos < c1) {
         Cursor c = cur;
         c.at = 0;
-        c.start = pos + ITEM_COST;
+        c.start = pos + ITEM_COST<MODE>;
         if (++c.head == a.pool.n_kv_head) {
           c.head = 0;
           if (++c.x * S::ROWS >= c.q.rows) {
@@ -641,7 +669,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
           l = l * ex2(m - top) + e.y * ex2(e.x - top);
           m = top;
         }
-        joined[r] = make_float2(m, in_parts(MODE) ? l : l == 0.f ? 0.f : 1.f / l);
+        joined[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
       }
       __syncthreads();
 #pragma unroll 4
@@ -652,23 +680,15 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
 #pragma unroll 2
         for (uint32_t k = 0; k < j.n; k++) {
           const float4 v = reinterpret_cast<const float4*>(piece(k))[c * S::ROWS + r];
-          const float w = in_parts(MODE) ? ex2(ml(k, r).x - all.x) : ex2(ml(k, r).x - all.x) * all.y;
+          const float w = ex2(ml(k, r).x - all.x) * all.y;
           o = make_float4(fmaf(v.x, w, o.x), fmaf(v.y, w, o.y), fmaf(v.z, w, o.z), fmaf(v.w, w, o.w));
-        }
-        if constexpr (in_parts(MODE)) {
-          if (r < rows) {
-            const size_t at = part_row(a, q.q0, head, row0 + r);
-            *reinterpret_cast<float4*>(a.part + at * D + 4 * c) = o;
-            if (c == 0) a.part_ml[at] = all;
-          }
-          continue;
         }
         // staged in the dead Q tiles: whole rows go to memory
         const uint32_t lo = a.bf ? pack2<true>(o.x, o.y) : pack2<false>(o.x, o.y), hi = a.bf ? pack2<true>(o.z, o.w) : pack2<false>(o.z, o.w);
         *reinterpret_cast<uint2*>(smem + r * (D * 2) + (((c >> 1) ^ (r & (D / 8 - 1))) << 4) + 8 * (c & 1)) = make_uint2(lo, hi);
       }
       __syncthreads();
-      if constexpr (!in_parts(MODE)) store_rows<D>(a, q.q0, head, row0, rows, smem, threadIdx.x, THREADS);
+      store_rows<D>(a, q.q0, head, row0, rows, smem, threadIdx.x, THREADS);
     }
     __syncthreads();
   }
@@ -699,24 +719,23 @@ cudaError_t bp_kv4_prefill_init(bp_paged_ctx* c) {
   size_t floats = 0;
   cudaError_t e = cudaSuccess;
   auto allow = [&](auto kernel, auto shape) {
-    const size_t need = 2 * static_cast<size_t>(c->sm_count) * shape.PARTIAL;  // two pieces per CTA
+    const size_t need = 2 * static_cast<size_t>(c->sm_count) * shape.PIECE;  // two pieces per CTA
     if (need > floats) floats = need;
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shape.SMEM));
   };
   for (uint32_t i = 0; i < 4 && e == cudaSuccess; i++) {
     e = with_kernel<PLAIN>(i & 1 ? 128 : 64, i & 2, allow);
-    if (e == cudaSuccess) e = with_kernel<PREFIX>(i & 1 ? 128 : 64, i & 2, allow);
-    if (e == cudaSuccess) e = with_kernel<OWN>(i & 1 ? 128 : 64, i & 2, allow);
+    if (e == cudaSuccess) e = with_kernel<PARTS>(i & 1 ? 128 : 64, i & 2, allow);
   }
   return e != cudaSuccess ? e : cudaMalloc(&c->prefill_partials, floats * sizeof(float));
 }
 
-cudaError_t bp_launch_kv4_prefill(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, int mode, const AttnArgs& a) {
+cudaError_t bp_launch_kv4_prefill(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, int mode, uint64_t rows, uint32_t ctas, const AttnArgs& a, const float** slots, uint32_t* piece) {
   auto launch = [&](auto kernel, auto shape) {
-    return bp_launch(true, kernel, dim3(c->sm_count), dim3(shape.THREADS), shape.SMEM, s, a, c->prefill_partials, c->counters);
+    using S = decltype(shape);
+    if (slots) *slots = c->prefill_partials;
+    if (piece) *piece = S::PIECE;
+    return bp_launch(true, kernel, dim3(ctas ? ctas : c->sm_count), dim3(S::THREADS), S::SMEM, s, a, c->prefill_partials, c->counters);
   };
-  const bool two = static_cast<uint64_t>(a.max_q) * a.group > BM;
-  return mode == PLAIN    ? with_kernel<PLAIN>(head_dim, two, launch)
-         : mode == PREFIX ? with_kernel<PREFIX>(head_dim, two, launch)
-                          : with_kernel<OWN>(head_dim, two, launch);
+  return mode == PLAIN ? with_kernel<PLAIN>(head_dim, rows > BM, launch) : with_kernel<PARTS>(head_dim, rows > BM, launch);
 }

@@ -365,7 +365,7 @@ int bp_kv4_attention_selected(bp_paged_ctx* c, void* stream, uint32_t dtype, con
   a.max_q = 1;
   a.max_kv = in->chosen * p.page;
   a.table_stride = a.table_pages = in->chosen;
-  BP_TRY(c, bp_launch_kv4_rows(c, static_cast<cudaStream_t>(stream), pool->head_dim, CHOSEN, a.group, a));
+  BP_TRY(c, bp_launch_kv4_few_rows(c, static_cast<cudaStream_t>(stream), pool->head_dim, CHOSEN, a.group, 0, a));
   return BP_OK;
 }
 

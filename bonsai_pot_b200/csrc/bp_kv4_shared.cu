@@ -1,9 +1,10 @@
 // Attention of requests behind prefixes that several of them have in common (include/bonsai_pages.h).
 //
 // The keys that a query sees are those of its prefix and its request's own. With o_i = sum of 2^(s - m_i) v, l_i = sum of 2^(s - m_i) and m_i = the
-// largest score (log2 units) over part i of the keys, the output is sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, m = max(m_1, m_2). The first part is
-// a prefix whose rows are those of all its requests, so that its codes are read and expanded once for all of them; the second is each request's own. Both are the attention
-// kernels' (bp_kv4_attention.cu, bp_kv4_prefill.cu), which leave (o, m, l) in the caller's work memory in 32 bits; the kernel here joins them.
+// largest score (log2 units) over part i of the keys, the output is sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, m = the largest m_i. Prefixes are items whose rows
+// are those of all their requests, so that their codes are read and expanded once for all of them; own keys are items of each request. Both are the attention
+// kernels' (bp_kv4_attention.cu, bp_kv4_prefill.cu), which leave (o, m, l) of whole items in the caller's work memory and of pieces of items in the context's, in 32 bits;
+// the kernel here joins them all, in the order of the keys.
 #include "bp_kv4_attention.cuh"
 #include "bp_paged_host.cuh"
 
@@ -14,23 +15,24 @@ using namespace bp::kv4;
 using namespace bp::paged;
 
 struct JoinArgs {
-  const float *prefix, *own;
-  const float2 *prefix_ml, *own_ml;
-  const int32_t *q_start, *prefix_start;
-  uint32_t n_prefix;
-  AttnArgs a;  // of the own keys' launch: where the outputs go, what the lengths are cut to
+  AttnArgs a;  // lengths of both parts, outputs
+  const float* slots[2];             // pieces of prefixes, of own keys
+  uint32_t piece[2], ctas[2], rows[2];  // floats of a piece, CTAs that have some, rows of one
 };
 constexpr uint32_t JOIN_THREADS = 256;
 
-// The last i of n with begin[i] <= x, or -1.
-__device__ __forceinline__ int last_begun(const int32_t* begin, uint32_t n, int x) {
-  int lo = -1, hi = static_cast<int>(n);
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (begin[mid] <= x) lo = mid;
-    else hi = mid;
+// The last i of n with begin[i] <= x, or -1, by a warp: 32 places at a time.
+__device__ __forceinline__ int last_begun(const int32_t* begin, uint32_t n, int x, uint32_t lane) {
+  uint32_t lo = 0, len = n;  // it is lo - 1 or one of [lo, lo + len)
+  while (len > 0) {
+    const uint32_t step = (len + 31) / 32, at = lo + min(lane * step, len - 1);
+    const uint32_t begun = __popc(__ballot_sync(FULL, lane * step < len && begin[at] <= x));
+    if (begun == 0) break;
+    const uint32_t from = lo + (begun - 1) * step;  // this one has begun, the next one asked for has not
+    len = min(step, lo + len - from) - 1;
+    lo = from + 1;
   }
-  return lo;
+  return static_cast<int>(lo) - 1;
 }
 
 // A warp per row.
@@ -44,23 +46,73 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(const __grid_con
   pdl_wait();
   if (row >= static_cast<uint64_t>(a.total_q) * a.n_head) return;
   const uint32_t token = static_cast<uint32_t>(row / a.n_head), head = static_cast<uint32_t>(row) - token * a.n_head;
-  const int r = last_begun(j.q_start, a.n_req + 1, static_cast<int>(token));
-  if (r < 0 || r >= static_cast<int>(a.n_req)) return;  // a row of no request
-  const Lengths n = lengths_of<OWN>(a, r, false);
-  if (static_cast<int>(token) >= n.q0 + n.q_len) return;  // (cut, and reported)
-  const int g = last_begun(j.prefix_start, j.n_prefix + 1, r);
-  const float2 none = make_float2(NEG_BIG, 0.f);
-  const float2 x = g >= 0 && g < static_cast<int>(j.n_prefix) ? j.prefix_ml[row] : none, y = j.own_ml[row];
-  const float m = fmaxf(x.x, y.x), wx = x.y == 0.f ? 0.f : ex2(x.x - m), wy = y.y == 0.f ? 0.f : ex2(y.x - m), l = wx * x.y + wy * y.y;
-  float o[V] = {};
-  // (a part without weights has not been written)
-  if (x.y != 0.f) {
+  // where the pieces of either part are (asked for before it is known whether there is anything)
+  const float* record[2] = {a.part + row * RECORD<D>, a.part + (static_cast<size_t>(a.total_q) * a.n_head + row) * RECORD<D>};
+  const uint4 ends[2] = {*reinterpret_cast<const uint4*>(record[0] + D), *reinterpret_cast<const uint4*>(record[1] + D)};
+  const int r = last_begun(a.q_start, a.n_own + 1, static_cast<int>(token), lane);
+  if (r < 0 || r >= static_cast<int>(a.n_own)) return;  // a row of no request
+  const int g = last_begun(a.prefix_start, a.n_prefix + 1, r, lane);
+  const Lengths own = lengths_of<PARTS>(a, a.n_prefix + r, false);
+  if (static_cast<int>(token) >= own.q0 + own.q_len) return;  // (cut, and reported)
+  const bool some = g >= 0 && g < static_cast<int>(a.n_prefix);
+  uint32_t n[2], c[2], at[2];
+  float2 first[2];
 #pragma unroll
-    for (int i = 0; i < V; i++) o[i] = wx * j.prefix[row * D + V * lane + i];
+  for (int p = 0; p < 2; p++) {
+    const bool none = p == 0 && !some;
+    first[p] = none ? make_float2(NEG_BIG, 0.f) : make_float2(__uint_as_float(ends[p].x), __uint_as_float(ends[p].y));
+    c[p] = ends[p].z;
+    n[p] = none ? 0 : ends[p].w >> 16;
+    at[p] = ends[p].w & 0xffff;
+    // (after a wait that gave up nobody may have written this)
+    if (n[p] != 0 && (n[p] > j.ctas[p] || c[p] > j.ctas[p] - n[p] || at[p] >= j.rows[p])) return;
   }
-  if (y.y != 0.f) {
+  const uint32_t n0 = max(n[0], 1u), all = n0 + max(n[1], 1u);
+  auto piece = [&](uint32_t k) -> const float* {
+    const int p = k >= n0;
+    if (n[p] == 0) return record[p];
+    return j.slots[p] + static_cast<size_t>(piece_at(c[p], k - (p ? n0 : 0))) * j.piece[p] + at[p] * RECORD<D>;
+  };
+  float m = NEG_BIG, l = 0.f, o[V] = {};
+  for (uint32_t k0 = 0; k0 < all; k0 += 32) {
+    const uint32_t few = min(all - k0, 32u), k = k0 + lane;
+    float2 ml = make_float2(NEG_BIG, 0.f);
+    if (lane < few) ml = n[k >= n0] == 0 ? first[k >= n0] : *reinterpret_cast<const float2*>(piece(k) + D);
+    float top = ml.x;
 #pragma unroll
-    for (int i = 0; i < V; i++) o[i] = fmaf(wy, j.own[row * D + V * lane + i], o[i]);
+    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, x));
+    top = fmaxf(top, m);
+    const float before = ex2(m - top), weight = ml.y == 0.f ? 0.f : ex2(ml.x - top);
+    float sum = weight * ml.y;
+#pragma unroll
+    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(FULL, sum, x);
+    l = l * before + sum;
+    m = top;
+#pragma unroll
+    for (int x = 0; x < V; x++) o[x] *= before;
+    for (uint32_t q0 = 0; q0 < few; q0 += 4) {  // four pieces on their way (one without weights may not have been written)
+      float e[4][V], w[4];
+#pragma unroll
+      for (uint32_t q = 0; q < 4; q++) {
+        w[q] = __shfl_sync(FULL, weight, q0 + q);  // 0 behind the last
+#pragma unroll
+        for (int x = 0; x < V; x++) e[q][x] = 0.f;
+        if (q0 + q < few && w[q] != 0.f) {
+          const float* v = piece(k0 + q0 + q) + V * lane;
+          if constexpr (V == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(v);
+            e[q][0] = f.x, e[q][1] = f.y, e[q][2] = f.z, e[q][3] = f.w;
+          } else {
+            const float2 f = *reinterpret_cast<const float2*>(v);
+            e[q][0] = f.x, e[q][1] = f.y;
+          }
+        }
+      }
+#pragma unroll
+      for (uint32_t q = 0; q < 4; q++)
+#pragma unroll
+        for (int x = 0; x < V; x++) o[x] = fmaf(e[q][x], w[q], o[x]);
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* out = a.out.data + static_cast<int64_t>(token) * a.out.tok + static_cast<int64_t>(head) * a.out.head + V * lane;
@@ -78,7 +130,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(const __grid_con
 extern "C" {
 
 uint64_t bp_kv4_shared_work(uint32_t total_q, uint32_t n_head, uint32_t head_dim) {
-  return 2 * static_cast<uint64_t>(total_q) * n_head * (static_cast<uint64_t>(head_dim) + 2);
+  return 2 * static_cast<uint64_t>(total_q) * n_head * (static_cast<uint64_t>(head_dim) + 4);
 }
 
 int bp_kv4_attention_shared(bp_paged_ctx* c, void* stream, uint32_t dtype, const bp_kv4_pool* pool, const bp_kv4_shared* in) {
@@ -100,9 +152,9 @@ int bp_kv4_attention_shared(bp_paged_ctx* c, void* stream, uint32_t dtype, const
   if (in->n_req > 65535 || in->n_prefix > 65535) return fail_config(c, "at most 65535 requests and prefixes");
   if (static_cast<uint64_t>(in->total_q) * in->n_head > 0x7fffffffull || in->max_kv > 0x7fffff00u || in->max_prefix > 0x7fffff00u)
     return fail_config(c, "total_q * n_head, max_kv and max_prefix must be < 2^31");
-  // units of 64 keys of 8 rows, and what an item of the kernel for many queries costs besides, are counted in 32 bits
+  // units of 64 keys of 8 rows, and what an item of the kernel for many queries costs besides, are counted in 32 bits, those of both parts together
   const uint64_t rows8 = static_cast<uint64_t>(in->total_q) * (in->n_head / p.n_kv_head) / 8;
-  if ((rows8 + in->n_req) * p.n_kv_head > 0xffffffffull / (in->max_kv / 64 + 8) || (rows8 + in->n_prefix) * p.n_kv_head > 0xffffffffull / (in->max_prefix / 64 + 8))
+  if ((rows8 + in->n_req) * p.n_kv_head > 0x7fffffffull / (in->max_kv / 64 + 8) || (rows8 + in->n_prefix) * p.n_kv_head > 0x7fffffffull / (in->max_prefix / 64 + 8))
     return fail_config(c, "total_q * n_head * max_kv or max_prefix is too large for one call");
   if (!rq.data || !ro.data || !in->q_start || !in->kv_len || !in->work || (in->max_kv != 0 && (!p.data || !in->page_table)) ||
       (in->n_prefix != 0 && (!in->prefix_start || !in->prefix_len || (in->max_prefix != 0 && (!p.data || !in->prefix_table)))))
@@ -110,48 +162,63 @@ int bp_kv4_attention_shared(bp_paged_ctx* c, void* stream, uint32_t dtype, const
   OnDevice on(c->device);
   BP_TRY(c, on.err);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const size_t rows = static_cast<size_t>(in->total_q) * in->n_head;
-  float* work = static_cast<float*>(in->work);
-  AttnArgs a;
+  JoinArgs j = {};
+  AttnArgs& a = j.a;
   bp_kv4_attention_args(c, dtype == BP_DTYPE_BF16, p, in->q, in->out, in->n_head, in->scale, &a);
   a.q_start = static_cast<const int32_t*>(in->q_start);
-  a.total_q = in->total_q;
-  JoinArgs j = {};
-  j.prefix = work;
-  j.own = work + rows * pool->head_dim;
-  j.prefix_ml = reinterpret_cast<float2*>(work + 2 * rows * pool->head_dim);
-  j.own_ml = j.prefix_ml + rows;
-  j.q_start = a.q_start;
-  j.prefix_start = static_cast<const int32_t*>(in->prefix_start);
-  j.n_prefix = in->n_prefix;
-  if (in->n_prefix != 0) {
-    AttnArgs x = a;
-    x.kv_len = static_cast<const int32_t*>(in->prefix_len);
-    x.page_table = static_cast<const int32_t*>(in->prefix_table);
-    x.prefix_start = j.prefix_start;
-    x.n_all = in->n_req;
-    x.n_req = in->n_prefix;
-    x.max_q = in->total_q;
-    x.max_kv = in->max_prefix;
-    x.table_stride = in->prefix_stride;
-    x.table_pages = bp_kv4_table_pages(p, in->prefix_stride);
-    x.part = const_cast<float*>(j.prefix);
-    x.part_ml = const_cast<float2*>(j.prefix_ml);
-    BP_TRY(c, bp_launch_kv4_rows(c, s, pool->head_dim, PREFIX, (static_cast<uint64_t>(in->total_q) * a.group + in->n_prefix - 1) / in->n_prefix, x));
-  }
   a.kv_len = static_cast<const int32_t*>(in->kv_len);
   a.page_table = static_cast<const int32_t*>(in->page_table);
-  a.n_req = in->n_req;
+  a.total_q = in->total_q;
   a.max_q = in->max_q < in->total_q ? in->max_q : in->total_q;
   a.max_kv = in->max_kv;
   a.table_stride = in->table_stride;
   a.table_pages = bp_kv4_table_pages(p, in->table_stride);
-  a.part = const_cast<float*>(j.own);
-  a.part_ml = const_cast<float2*>(j.own_ml);
-  BP_TRY(c, bp_launch_kv4_rows(c, s, pool->head_dim, OWN, static_cast<uint64_t>(a.max_q) * a.group, a));
-  j.a = a;
+  a.prefix_start = static_cast<const int32_t*>(in->prefix_start);
+  a.prefix_len = static_cast<const int32_t*>(in->prefix_len);
+  a.prefix_table = static_cast<const int32_t*>(in->prefix_table);
+  a.n_prefix = in->n_prefix;
+  a.n_own = in->n_req;
+  a.n_req = in->n_prefix + in->n_req;
+  a.max_prefix = in->max_prefix;
+  a.prefix_stride = in->prefix_stride;
+  a.prefix_pages = bp_kv4_table_pages(p, in->prefix_stride);
+  a.part = static_cast<float*>(in->work);
+  // rows of a prefix (on the average) and of a request, by which either part goes to the kernel for few rows or the one for many; without any key there are only zeros
+  const uint64_t own_rows = static_cast<uint64_t>(a.max_q) * a.group, prefix_rows = in->n_prefix ? (static_cast<uint64_t>(in->total_q) * a.group + in->n_prefix - 1) / in->n_prefix : 0;
+  const bool own_many = in->max_kv != 0 && own_rows > BP_KV4_FEW_ROWS, prefix_many = in->max_prefix != 0 && prefix_rows > BP_KV4_FEW_ROWS;
+  const uint32_t D = pool->head_dim;
+  const uint64_t more = own_rows > prefix_rows ? own_rows : prefix_rows;
+  if (own_many || !prefix_many) {  // one launch for both
+    BP_TRY(c, own_many ? bp_launch_kv4_prefill(c, s, D, PARTS, more, 0, a, &j.slots[0], &j.piece[0]) : bp_launch_kv4_few_rows(c, s, D, PARTS, more, 0, a, &j.slots[0], &j.piece[0]));
+    j.slots[1] = j.slots[0];
+    j.piece[1] = j.piece[0];
+    j.ctas[0] = j.ctas[1] = c->sm_count;
+  } else {
+    // Side by side, each on its share of the SMs: what a tile of 64 keys takes there (1.2 us of 256 rows, 0.9 of 128) against 0.18 us for a unit of 64 keys here,
+    // by the lengths that the caller says, and each its beginning and end.
+    const float prefix_tiles = static_cast<float>(in->n_prefix) * p.n_kv_head * ((prefix_rows + 255) / 256) * (in->max_prefix / 64 + 6);
+    const float prefix_cost = prefix_tiles * (prefix_rows > 128 ? 1.2f : 0.9f), own_cost = static_cast<float>(in->n_req) * p.n_kv_head * (in->max_kv / 64 + 1) * 0.18f;
+    const float part = prefix_cost / (prefix_cost + own_cost);
+    const int sms = c->sm_count, most = sms - sms / 8;
+    int here = static_cast<int>(part * sms + 0.5f);
+    here = here < sms / 8 ? sms / 8 : here > most ? most : here;
+    AttnArgs x = a;
+    x.first = 1;
+    x.n_req = x.n_prefix;
+    BP_TRY(c, bp_launch_kv4_prefill(c, s, D, PARTS, prefix_rows, here, x, &j.slots[0], &j.piece[0]));
+    x = a;
+    x.beside = 1;
+    x.n_req = x.n_own;
+    x.n_prefix = 0;
+    BP_TRY(c, bp_launch_kv4_few_rows(c, s, D, PARTS, own_rows, sms - here, x, &j.slots[1], &j.piece[1]));
+    j.ctas[0] = here;
+    j.ctas[1] = sms - here;
+  }
+  j.rows[0] = j.piece[0] / (D + 4);
+  j.rows[1] = j.piece[1] / (D + 4);
+  const uint64_t rows = static_cast<uint64_t>(in->total_q) * in->n_head;
   const dim3 grid(static_cast<uint32_t>((rows + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32)));
-  BP_TRY(c, bp_launch(true, pool->head_dim == 128 ? kv4_join_kernel<128> : kv4_join_kernel<64>, grid, dim3(JOIN_THREADS), 0, s, j));
+  BP_TRY(c, bp_launch(true, D == 128 ? kv4_join_kernel<128> : kv4_join_kernel<64>, grid, dim3(JOIN_THREADS), 0, s, j));
   return BP_OK;
 }
 

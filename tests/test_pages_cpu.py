@@ -58,7 +58,7 @@ def test_nothing_runs_without_a_context():
     assert lib.bp_kv4_summarise(None, None, None, None, None, None, 0) == 7
     assert lib.bp_kv4_select(None, None, 0, None, None, None) == 7
     assert lib.bp_kv4_attention_selected(None, None, 0, None, None) == 7
-    assert lib.bp_kv4_shared_work(3, 4, 64) == 2 * 3 * 4 * 66 and lib.bp_kv4_shared_work(1 << 31, 64, 128) == (1 << 38) * 130
+    assert lib.bp_kv4_shared_work(3, 4, 64) == 2 * 3 * 4 * 68 and lib.bp_kv4_shared_work(1 << 31, 64, 128) == (1 << 38) * 132
 
 
 @pytest.fixture
