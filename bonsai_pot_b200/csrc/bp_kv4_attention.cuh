@@ -100,6 +100,20 @@ __device__ __forceinline__ const int32_t* pages_of(const AttnArgs& a, uint32_t r
   const size_t row = MODE == CHOSEN ? static_cast<size_t>(r) * a.pool.n_kv_head + head : MODE == PARTS ? r - a.n_prefix : r;
   return a.page_table + row * a.table_stride;
 }
+// The last i of n with begin[i] <= x, or -1, by a warp: 32 places at a time.
+__device__ __forceinline__ int last_begun(const int32_t* begin, uint32_t n, int x, uint32_t lane) {
+  uint32_t lo = 0, len = n;  // it is lo - 1 or one of [lo, lo + len)
+  while (len > 0) {
+    const uint32_t step = (len + 31) / 32, at = lo + min(lane * step, len - 1);
+    const uint32_t begun = __popc(__ballot_sync(FULL, lane * step < len && begin[at] <= x));
+    if (begun == 0) break;
+    const uint32_t from = lo + (begun - 1) * step;  // this one has begun, the next one asked for has not
+    len = min(step, lo + len - from) - 1;
+    lo = from + 1;
+  }
+  return static_cast<int>(lo) - 1;
+}
+
 // A bounded wait for a barrier's phase: false after 2^20 polls or two seconds, or when *stop (may be null) is set.
 __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const volatile uint32_t* stop = nullptr) {
   if (mbar_test(bar, parity)) return true;

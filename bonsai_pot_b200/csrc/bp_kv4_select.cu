@@ -104,8 +104,10 @@ struct ChoiceArgs {
   const float* scales;
   int32_t *pages, *keys;
   uint32_t chosen, first, last;
+  uint32_t split;  // CTAs of a cluster, which share a token's pages
 };
 constexpr uint32_t CHOICE_THREADS = 256, MAX_BLOCKS = 49152;
+constexpr uint32_t AT_A_TIME = 4;  // pages that eight lanes ask for together
 
 // Sum of u8 x s8 products of four bytes each, added to c.
 __device__ __forceinline__ int dot4(uint32_t u, uint32_t s, int c) {
@@ -118,57 +120,71 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   const uint32_t b = __float_as_uint(x);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Stores into the shared memory of the cluster's first CTA, at the same place as `at` here.
+__device__ __forceinline__ void store_to_first(uint32_t* at, uint32_t x) {
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(smem_u32(at)));
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(x) : "memory");
+}
 
-// A CTA per token and KV head.
+// A cluster of `split` CTAs per token and KV head. Every CTA scores its part of the pages, eight lanes per page with 2 D / 8 bytes of its summary each; the scores
+// go to the first CTA, which looks for the want-th highest of them: the range in which it lies is cut into up to 256 parts of equal width and counted until one part
+// holds no others than are wanted. Bound by latency: what follows the launch is one chain of a dozen accesses to memory (the token's request, its lengths, page ids, summaries) and
+// as many barriers.
 template <int D>
 __global__ void __launch_bounds__(CHOICE_THREADS) kv4_select_kernel(const __grid_constant__ ChoiceArgs s) {
+  constexpr uint32_t WARPS = CHOICE_THREADS / 32;
   extern __shared__ uint32_t order[];  // scores of the token's pages as ordered numbers
   __shared__ __align__(16) uint8_t query[2 * D];
-  __shared__ float tops[CHOICE_THREADS / 32];
-  __shared__ uint32_t hist[256], sums[CHOICE_THREADS / 32], pick[2];
+  __shared__ float tops[WARPS];
+  __shared__ uint32_t hist[256], sums[WARPS], lows[WARPS], highs[WARPS], pick[3];
   const AttnArgs& a = s.a;
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, token = blockIdx.x, head = blockIdx.y;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, token = blockIdx.x / s.split, rank = blockIdx.x - token * s.split, head = blockIdx.y;
   pdl_launch_dependents();
+  if (s.split > 1) cluster_arrive();  // (nobody stores into a CTA that has not begun)
   pdl_wait();
-  // the token's request
-  uint32_t lo = 0, hi = a.n_req + 1;
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) >> 1;
-    if (a.q_start[mid] <= static_cast<int>(token)) lo = mid;
-    else hi = mid;
-  }
-  int sees = -1;
-  if (lo < a.n_req && a.q_start[lo] <= static_cast<int>(token)) {
-    const Lengths n = lengths_of<PLAIN>(a, lo, head == 0 && threadIdx.x == 0);
-    const int i = static_cast<int>(token) - n.q0;
-    if (i >= 0 && i < n.q_len) sees = max(n.kv_len - n.q_len + i + 1, 0);
-  }
-  const uint32_t blocks = sees > 0 ? (static_cast<uint32_t>(sees) + a.pool.page - 1) >> a.pool.log_page : 0, n = min(blocks, s.chosen);
-  if (head == 0 && threadIdx.x == 0) s.keys[token] = sees < 0 ? -1 : sees - static_cast<int>((blocks - n) << a.pool.log_page);
-  int32_t* out = s.pages + (static_cast<size_t>(token) * a.pool.n_kv_head + head) * s.chosen;
-  const int32_t* table = a.page_table + static_cast<size_t>(lo) * a.table_stride;
-  for (uint32_t i = n + threadIdx.x; i < s.chosen; i += CHOICE_THREADS) out[i] = -1;
-  if (n == blocks) {
-    for (uint32_t i = threadIdx.x; i < n; i += CHOICE_THREADS) out[i] = table[i];
-    return;
-  }
-  // ---- the query in 8 bits ----
+  // ---- the sums of the queries' positive and negative parts, in the order of the heads ----
   float up = 0.f, down = 0.f;
   if (threadIdx.x < D) {
     const uint16_t* q = a.q.data + static_cast<int64_t>(token) * a.q.tok + static_cast<int64_t>(head * a.group) * a.q.head + threadIdx.x;
+#pragma unroll 4
     for (uint32_t g = 0; g < a.group; g++) {
       const float x = a.bf ? to_f32<true>(q[g * a.q.head]) : to_f32<false>(q[g * a.q.head]);
       up += fmaxf(x, 0.f);
       down += fmaxf(-x, 0.f);
     }
   }
+  // ---- what the token sees ----
+  const int r = last_begun(a.q_start, a.n_req + 1, static_cast<int>(token), lane);
+  int sees = -1;
+  if (r >= 0 && r < static_cast<int>(a.n_req)) {
+    const Lengths n = lengths_of<PLAIN>(a, r, head == 0 && threadIdx.x == 0);
+    const int i = static_cast<int>(token) - n.q0;
+    if (i < n.q_len) sees = max(n.kv_len - n.q_len + i + 1, 0);
+  }
+  const uint32_t blocks = sees > 0 ? (static_cast<uint32_t>(sees) + a.pool.page - 1) >> a.pool.log_page : 0, n = min(blocks, s.chosen);
+  int32_t* out = s.pages + (static_cast<size_t>(token) * a.pool.n_kv_head + head) * s.chosen;
+  const int32_t* table = a.page_table + static_cast<size_t>(max(r, 0)) * a.table_stride;
+  if (rank == 0) {
+    if (head == 0 && threadIdx.x == 0) s.keys[token] = sees < 0 ? -1 : sees - static_cast<int>((blocks - n) << a.pool.log_page);
+    for (uint32_t i = n + threadIdx.x; i < s.chosen; i += CHOICE_THREADS) out[i] = -1;
+    if (n == blocks)
+      for (uint32_t i = threadIdx.x; i < n; i += CHOICE_THREADS) out[i] = table[i];
+  }
+  if (n == blocks) {  // (the whole cluster)
+    if (s.split > 1) cluster_wait();
+    return;
+  }
+  // ---- the query in 8 bits ----
   float top = fmaxf(up, down);
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
   if (lane == 0) tops[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (uint32_t w = 0; w < CHOICE_THREADS / 32; w++) top = fmaxf(top, tops[w]);
+  for (uint32_t w = 0; w < WARPS; w++) top = fmaxf(top, tops[w]);
   const uint32_t e = min(max(__float_as_uint(top) & 0x7f800000u, 27u << 23), 254u << 23);  // 2^-100 .. 2^127
   const float inv = __uint_as_float((261u << 23) - e);                                      // 2^(7 - e)
   if (threadIdx.x < D) {
@@ -176,89 +192,142 @@ __global__ void __launch_bounds__(CHOICE_THREADS) kv4_select_kernel(const __grid
     query[D + threadIdx.x] = static_cast<uint8_t>(fminf(rintf(down * inv), 255.f));
   }
   __syncthreads();
-  // ---- scores: eight lanes per page, 2 D / 8 bytes each ----
+  // ---- scores ----
   constexpr uint32_t W = 2 * D / 32;  // words of a lane
   uint32_t mine[W];
 #pragma unroll
   for (uint32_t i = 0; i < W; i++) mine[i] = reinterpret_cast<const uint32_t*>(query)[(lane & 7) * 4 + (i >> 2) * 32 + (i & 3)];
-  for (uint32_t b0 = warp * 4; b0 < blocks; b0 += CHOICE_THREADS / 8) {
-    const uint32_t b = b0 + (lane >> 3);
-    const bool there = b < blocks;
-    const uint32_t page = there ? static_cast<uint32_t>(table[b]) : 0u;
-    const bool good = page < a.pool.n_pages;
-    int sum = 0;
-    float scale = 0.f;
-    if (there && good) {
-      const size_t record = static_cast<size_t>(page) * a.pool.n_kv_head + head;
-      const uint4* codes = reinterpret_cast<const uint4*>(s.codes + record * 2 * D);
-      scale = s.scales[record];
+  const uint32_t per = (blocks + s.split - 1) / s.split, from = min(rank * per, blocks), to = min(from + per, blocks);
+  if (s.split > 1) cluster_wait();
+  constexpr uint32_t STEP = CHOICE_THREADS / 8;
+  uint32_t ids[AT_A_TIME];
+  auto ask_ids = [&](uint32_t b0) {
+#pragma unroll
+    for (uint32_t k = 0; k < AT_A_TIME; k++) ids[k] = b0 + k * STEP < to ? static_cast<uint32_t>(table[b0 + k * STEP]) : 0xffffffffu;
+  };
+  ask_ids(from + (threadIdx.x >> 3));
+  for (uint32_t b0 = from + (threadIdx.x >> 3); __any_sync(FULL, b0 < to); b0 += AT_A_TIME * STEP) {
+    uint4 v[AT_A_TIME][W / 4];
+    float scale[AT_A_TIME];
+    bool good[AT_A_TIME];
+#pragma unroll
+    for (uint32_t k = 0; k < AT_A_TIME; k++) {
+      good[k] = ids[k] < a.pool.n_pages;
+      const size_t record = good[k] ? static_cast<size_t>(ids[k]) * a.pool.n_kv_head + head : 0;
+      const uint4* codes = reinterpret_cast<const uint4*>(s.codes + record * 2 * D) + (lane & 7);
+      scale[k] = s.scales[record];
+#pragma unroll
+      for (uint32_t i = 0; i < W / 4; i++) v[k][i] = codes[8 * i];
+    }
+    ask_ids(b0 + AT_A_TIME * STEP);
+#pragma unroll
+    for (uint32_t k = 0; k < AT_A_TIME; k++) {
+      int sum = 0;
 #pragma unroll
       for (uint32_t i = 0; i < W / 4; i++) {
-        const uint4 v = codes[(lane & 7) + 8 * i];
-        sum = dot4(mine[4 * i], v.x, sum);
-        sum = dot4(mine[4 * i + 1], v.y, sum);
-        sum = dot4(mine[4 * i + 2], v.z, sum);
-        sum = dot4(mine[4 * i + 3], v.w, sum);
+        sum = dot4(mine[4 * i], v[k][i].x, sum);
+        sum = dot4(mine[4 * i + 1], v[k][i].y, sum);
+        sum = dot4(mine[4 * i + 2], v[k][i].z, sum);
+        sum = dot4(mine[4 * i + 3], v[k][i].w, sum);
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(FULL, sum, o);
+      const uint32_t b = b0 + k * STEP;
+      if (b < to && (lane & 7) == k) {
+        if (!good[k]) note_range(a.err);
+        const uint32_t x = good[k] ? ordered(static_cast<float>(sum) * scale[k]) : 0u;
+        if (s.split > 1) store_to_first(&order[b], x);
+        else order[b] = x;
       }
     }
+  }
+  if (s.split > 1) {
+    cluster_arrive();
+    cluster_wait();
+    if (rank) return;
+  } else {
+    __syncthreads();
+  }
+  // ---- the want-th highest of those that are not chosen anyway ----
+  const uint32_t begin = s.first, end = blocks - s.last;
+  uint32_t want = n - s.first - s.last, least = 0xffffffffu, ties = 0;  // chosen are those above `least` and the first `ties` of those equal to it
+  if (want > 0) {
+    uint32_t low = 0xffffffffu, high = 0;
+    for (uint32_t i = begin + threadIdx.x; i < end; i += CHOICE_THREADS) {
+      low = min(low, order[i]);
+      high = max(high, order[i]);
+    }
+    low = __reduce_min_sync(FULL, low);
+    high = __reduce_max_sync(FULL, high);
+    if (lane == 0) {
+      lows[warp] = low;
+      highs[warp] = high;
+    }
+    hist[threadIdx.x] = 0;
+    __syncthreads();
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(FULL, sum, o);
-    if (there && (lane & 7) == 0) {
-      if (!good) note_range(a.err);
-      order[b] = b < s.first || b >= blocks - s.last ? 0xffffffffu : good ? ordered(static_cast<float>(sum) * scale) : 0u;
+    for (uint32_t w = 0; w < WARPS; w++) {
+      low = min(low, lows[w]);
+      high = max(high, highs[w]);
+    }
+    while (true) {
+      const uint32_t range = high - low, bits = 32 - __clz(range), shift = bits > 8 ? bits - 8 : 0;
+      for (uint32_t i = begin + threadIdx.x; i < end; i += CHOICE_THREADS) {
+        const uint32_t x = order[i] - low;
+        if (x <= range) atomicAdd(&hist[x >> shift], 1);
+      }
+      __syncthreads();
+      // thread t: those in part 255 - t or a higher one
+      const uint32_t count = hist[255 - threadIdx.x];
+      uint32_t run = count;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(FULL, run, o);
+        if (lane >= o) run += x;
+      }
+      if (lane == 31) sums[warp] = run;
+      __syncthreads();
+      for (uint32_t w = 0; w < warp; w++) run += sums[w];
+      if (run >= want && run - count < want) {
+        pick[0] = 255 - threadIdx.x;
+        pick[1] = want - (run - count);
+        pick[2] = count;
+      }
+      hist[255 - threadIdx.x] = 0;
+      __syncthreads();
+      low += pick[0] << shift;
+      want = pick[1];
+      if (shift == 0 || pick[2] == want) {
+        least = low;
+        ties = shift == 0 ? want : 0xffffffffu;  // (the whole part)
+        break;
+      }
+      high = low + ((1u << shift) - 1);
     }
   }
+  // ---- in the order of the keys: a thread has `each` pages side by side ----
+  const uint32_t each = (blocks + CHOICE_THREADS - 1) / CHOICE_THREADS, b0 = min(threadIdx.x * each, blocks), b1 = min(b0 + each, blocks);
+  auto kind = [&](uint32_t b) -> uint32_t {  // 1: chosen, 1 << 16: equal to the last one
+    if (b < begin || b >= end) return 1;
+    return order[b] > least ? 1u : ties && order[b] == least ? 1u << 16 : 0u;
+  };
+  uint32_t mine_of = 0;
+  for (uint32_t b = b0; b < b1; b++) mine_of += kind(b);
+  uint32_t upto = mine_of;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t x = __shfl_up_sync(FULL, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) sums[warp] = upto;
   __syncthreads();
-  // ---- the n-th highest: digit by digit ----
-  uint32_t prefix = 0, mask = 0, want = n;  // of those whose bits under mask are prefix, the want-th is looked for
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (uint32_t i = threadIdx.x; i < 256; i += CHOICE_THREADS) hist[i] = 0;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < blocks; i += CHOICE_THREADS) {
-      const uint32_t x = order[i];
-      if ((x & mask) == prefix) atomicAdd(&hist[x >> shift & 255], 1);
-    }
-    __syncthreads();
-    // thread t: those with the digit 255 - t or a higher one
-    const uint32_t count = hist[255 - threadIdx.x];
-    uint32_t run = count;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t x = __shfl_up_sync(FULL, run, o);
-      if (lane >= o) run += x;
-    }
-    if (lane == 31) sums[warp] = run;
-    __syncthreads();
-    for (uint32_t w = 0; w < warp; w++) run += sums[w];
-    if (run >= want && run - count < want) {
-      pick[0] = 255 - threadIdx.x;
-      pick[1] = want - (run - count);
-    }
-    __syncthreads();
-    prefix |= pick[0] << shift;
-    mask |= 255u << shift;
-    want = pick[1];
-    __syncthreads();
-  }
-  // ---- in the order of the keys: those above, and the first `want` of those equal ----
-  uint32_t done_above = 0, done_equal = 0;
-  for (uint32_t b0 = 0; b0 < blocks; b0 += CHOICE_THREADS) {
-    const uint32_t b = b0 + threadIdx.x, x = b < blocks ? order[b] : 0u;
-    const bool above = b < blocks && x > prefix, equal = b < blocks && x == prefix;
-    const uint32_t am = __ballot_sync(FULL, above), em = __ballot_sync(FULL, equal), under = (1u << lane) - 1;
-    if (lane == 0) sums[warp] = __popc(am) | __popc(em) << 16;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < CHOICE_THREADS / 32; w++) {
-      if (w == warp) before = all;
-      all += sums[w];
-    }
-    const uint32_t a_at = done_above + (before & 0xffff) + __popc(am & under), e_at = done_equal + (before >> 16) + __popc(em & under);
-    if (above || (equal && e_at < want)) out[a_at + min(e_at, want)] = table[b];
-    done_above += all & 0xffff;
-    done_equal += all >> 16;
-    __syncthreads();
+  for (uint32_t w = 0; w < warp; w++) upto += sums[w];
+  uint32_t above = (upto - mine_of) & 0xffff, equal = (upto - mine_of) >> 16;
+  for (uint32_t b = b0; b < b1; b++) {
+    const uint32_t k = kind(b);
+    if (k == 1 || (k && equal < ties)) out[above + min(equal, ties)] = table[b];
+    above += k & 0xffff;
+    equal += k >> 16;
   }
 }
 
@@ -332,8 +401,24 @@ int bp_kv4_select(bp_paged_ctx* c, void* stream, uint32_t dtype, const bp_kv4_po
   s.chosen = in->chosen;
   s.first = in->first;
   s.last = in->last;
-  BP_TRY(c, bp_launch(true, pool->head_dim == 128 ? kv4_select_kernel<128> : kv4_select_kernel<64>, dim3(in->total_q, p.n_kv_head), dim3(CHOICE_THREADS), blocks * 4,
-                      static_cast<cudaStream_t>(stream), s));
+  // CTAs per token and head: up to two per SM in all, of 128 pages at least (what they ask for at a time)
+  s.split = 1;
+  while (s.split < 8 && static_cast<uint64_t>(in->total_q) * p.n_kv_head * s.split < static_cast<uint64_t>(c->sm_count) && blocks > 128 * s.split) s.split *= 2;
+  if (static_cast<uint64_t>(in->total_q) * s.split > 0x7fffffffull) return fail_config(c, "total_q is too large for one call");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(in->total_q * s.split, p.n_kv_head);
+  cfg.blockDim = dim3(CHOICE_THREADS);
+  cfg.dynamicSmemBytes = blocks * 4;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = s.split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = s.split > 1 ? 2 : 1;
+  BP_TRY(c, cudaLaunchKernelEx(&cfg, pool->head_dim == 128 ? kv4_select_kernel<128> : kv4_select_kernel<64>, s));
   return BP_OK;
 }
 

@@ -21,20 +21,6 @@ struct JoinArgs {
 };
 constexpr uint32_t JOIN_THREADS = 256;
 
-// The last i of n with begin[i] <= x, or -1, by a warp: 32 places at a time.
-__device__ __forceinline__ int last_begun(const int32_t* begin, uint32_t n, int x, uint32_t lane) {
-  uint32_t lo = 0, len = n;  // it is lo - 1 or one of [lo, lo + len)
-  while (len > 0) {
-    const uint32_t step = (len + 31) / 32, at = lo + min(lane * step, len - 1);
-    const uint32_t begun = __popc(__ballot_sync(FULL, lane * step < len && begin[at] <= x));
-    if (begun == 0) break;
-    const uint32_t from = lo + (begun - 1) * step;  // this one has begun, the next one asked for has not
-    len = min(step, lo + len - from) - 1;
-    lo = from + 1;
-  }
-  return static_cast<int>(lo) - 1;
-}
-
 // A warp per row.
 template <int D>
 __global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(const __grid_constant__ JoinArgs j) {
