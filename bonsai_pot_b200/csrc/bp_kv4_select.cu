@@ -22,43 +22,53 @@ struct SummaryArgs {
 };
 constexpr uint32_t SUMMARY_WARPS = 4;
 
-// A warp per page and KV head: a lane has eight dims (a 32-bit word) of every 32 / (D / 8)-th token. Every value m + d q is an f16 number, so f16 maxima are exact.
+// A warp per 16 tokens of a page and KV head, all of whose loads are on their way at once: a lane has eight dims (a 32-bit word) of every 32 / (D / 8)-th token. The
+// page's first warp goes on. Every value m + d q is an f16 number, so f16 maxima are exact.
 template <int D>
 __global__ void __launch_bounds__(32 * SUMMARY_WARPS) kv4_summary_kernel(const __grid_constant__ SummaryArgs a) {
   using L = PoolLayout<D>;
-  constexpr uint32_t NB = L::NB, LANES = D / 8, STEP = 32 / LANES;
-  const uint32_t lane = threadIdx.x & 31, item = blockIdx.x * SUMMARY_WARPS + (threadIdx.x >> 5), at = item / a.pool.n_kv_head, head = item - at * a.pool.n_kv_head;
+  constexpr uint32_t NB = L::NB, LANES = D / 8, STEP = 32 / LANES, N = 16 / STEP;
+  __shared__ __half2 found[SUMMARY_WARPS][8][LANES];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, log_warps = a.pool.log_page - 4;
+  const uint32_t item = blockIdx.x * (SUMMARY_WARPS >> log_warps) + (warp >> log_warps), at = item / a.pool.n_kv_head, head = item - at * a.pool.n_kv_head;
+  const uint32_t part = warp & ((1u << log_warps) - 1);
   pdl_launch_dependents();
   pdl_wait();
-  if (at >= a.n) return;
-  const int32_t page = a.pages[at];
-  if (page < 0) return;
-  const int32_t given = a.n_tok ? a.n_tok[at] : static_cast<int32_t>(a.pool.page);
-  if (static_cast<uint32_t>(page) >= a.pool.n_pages || given <= 0 || given > static_cast<int32_t>(a.pool.page)) {
-    if (lane == 0) note_range(a.err);
-    return;
-  }
-  const uint32_t n = given, c = lane % LANES / NB, b = lane % NB;
-  const size_t record = static_cast<size_t>(page) * a.pool.n_kv_head + head;
+  const int32_t page = at < a.n ? a.pages[at] : -1;
+  const int32_t given = page < 0 || !a.n_tok ? static_cast<int32_t>(a.pool.page) : a.n_tok[at];
+  const bool good = page >= 0 && static_cast<uint32_t>(page) < a.pool.n_pages && given > 0 && given <= static_cast<int32_t>(a.pool.page);
+  if (page >= 0 && !good && lane == 0 && part == 0) note_range(a.err);
+  const uint32_t n = good ? given : 0, c = lane % LANES / NB, b = lane % NB;
+  const size_t record = good ? static_cast<size_t>(page) * a.pool.n_kv_head + head : 0;
   const uint8_t* k = a.pool.data + record * (a.pool.page * L::TOK);
   const uint8_t *words = k + (c * NB + b) * 4, *ds = k + L::kd(a.pool.page) + 2 * b, *ms = k + L::km(a.pool.page) + 2 * b;
   const __half2 none_hi = __float2half2_rn(-INFINITY), none_lo = __float2half2_rn(INFINITY);
   __half2 hi[4] = {none_hi, none_hi, none_hi, none_hi}, lo[4] = {none_lo, none_lo, none_lo, none_lo};
   const __half2 off = __float2half2_rn(-1024.f), off16 = __float2half2_rn(-64.f), sixteenth = __float2half2_rn(0.0625f);
-#pragma unroll 4
-  for (uint32_t t = lane / LANES; t < n; t += STEP) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(words + t * L::ROW), y = w >> 8;
-    const __half2 d = __half2half2(__ushort_as_half(*reinterpret_cast<const uint16_t*>(ds + t * 2 * NB)));
-    const __half2 m = __half2half2(__ushort_as_half(*reinterpret_cast<const uint16_t*>(ms + t * 2 * NB)));
-    const __half2 v[4] = {__hfma2(__hadd2(biased(w, 0x000f000fu, a.bias), off), d, m), __hfma2(__hfma2(biased(w, 0x00f000f0u, a.bias), sixteenth, off16), d, m),
+  const uint32_t t0 = 16 * part + lane / LANES;
+  uint32_t w[N];
+  uint16_t d16[N], m16[N];
+#pragma unroll
+  for (uint32_t i = 0; i < N; i++) {
+    const uint32_t t = t0 + i * STEP;
+    if (t >= n) continue;
+    w[i] = *reinterpret_cast<const uint32_t*>(words + t * L::ROW);
+    d16[i] = *reinterpret_cast<const uint16_t*>(ds + t * 2 * NB);
+    m16[i] = *reinterpret_cast<const uint16_t*>(ms + t * 2 * NB);
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < N; i++) {
+    if (t0 + i * STEP >= n) continue;
+    const uint32_t x = w[i], y = x >> 8;
+    const __half2 d = __half2half2(__ushort_as_half(d16[i])), m = __half2half2(__ushort_as_half(m16[i]));
+    const __half2 v[4] = {__hfma2(__hadd2(biased(x, 0x000f000fu, a.bias), off), d, m), __hfma2(__hfma2(biased(x, 0x00f000f0u, a.bias), sixteenth, off16), d, m),
                           __hfma2(__hadd2(biased(y, 0x000f000fu, a.bias), off), d, m), __hfma2(__hfma2(biased(y, 0x00f000f0u, a.bias), sixteenth, off16), d, m)};
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      hi[i] = __hmax2(hi[i], v[i]);
-      lo[i] = __hmin2(lo[i], v[i]);
+    for (int e = 0; e < 4; e++) {
+      hi[e] = __hmax2(hi[e], v[e]);
+      lo[e] = __hmin2(lo[e], v[e]);
     }
   }
-  float ends[2][8], top = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
 #pragma unroll
@@ -66,6 +76,28 @@ __global__ void __launch_bounds__(32 * SUMMARY_WARPS) kv4_summary_kernel(const _
       hi[i] = __hmax2(hi[i], h2(__shfl_xor_sync(FULL, u2(hi[i]), o)));
       lo[i] = __hmin2(lo[i], h2(__shfl_xor_sync(FULL, u2(lo[i]), o)));
     }
+  }
+  if (log_warps > 0) {
+    if (part != 0 && lane < LANES) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        found[warp][i][lane] = hi[i];
+        found[warp][4 + i][lane] = lo[i];
+      }
+    }
+    __syncthreads();
+    for (uint32_t p = 1; p < 1u << log_warps; p++) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        hi[i] = __hmax2(hi[i], found[(warp + p) % SUMMARY_WARPS][i][lane % LANES]);
+        lo[i] = __hmin2(lo[i], found[(warp + p) % SUMMARY_WARPS][4 + i][lane % LANES]);
+      }
+    }
+  }
+  if (!good || part != 0) return;
+  float ends[2][8], top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
     const float2 x = __half22float2(hi[i]), z = __half22float2(lo[i]);
     const bool some0 = z.x <= x.x, some1 = z.y <= x.y;
     ends[0][2 * i] = some0 ? x.x : 0.f;
@@ -355,7 +387,8 @@ int bp_kv4_summarise(bp_paged_ctx* c, void* stream, const bp_kv4_pool* pool, con
   BP_TRY(c, on.err);
   const SummaryArgs a{p, static_cast<int8_t*>(summary->codes), static_cast<float*>(summary->scales), static_cast<const int32_t*>(pages), static_cast<const int32_t*>(n_tok), n,
                       c->err_dev, 0x64006400u};
-  const dim3 grid((n * p.n_kv_head + SUMMARY_WARPS - 1) / SUMMARY_WARPS);
+  const uint32_t of_cta = SUMMARY_WARPS * 16 / p.page;
+  const dim3 grid((n * p.n_kv_head + of_cta - 1) / of_cta);
   BP_TRY(c, bp_launch(true, pool->head_dim == 128 ? kv4_summary_kernel<128> : kv4_summary_kernel<64>, grid, dim3(32 * SUMMARY_WARPS), 0, static_cast<cudaStream_t>(stream), a));
   return BP_OK;
 }

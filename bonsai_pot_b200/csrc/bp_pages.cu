@@ -4,6 +4,7 @@
 // result coming (grow, the end of a fork), rows are spread over CTAs where each is for itself (release, a fork's rows, the tables behind a
 // compaction). Free pages are found by looking at the reference counts, 32 per warp and load, in the order of the pages, so results do not depend on
 // who comes when; integer counts do not depend on the order of their atomics.
+#include "bp_kv4_attention.cuh"
 #include "bp_paged_host.cuh"
 
 namespace {
@@ -11,7 +12,7 @@ namespace {
 using namespace bp;
 using namespace bp::paged;
 
-constexpr unsigned FULL = 0xffffffffu;
+using kv4::FULL;
 constexpr uint32_t WORDS = 8;  // words of 32 pages that a warp looks at at a time: as many loads are on their way
 constexpr uint32_t MAX_ROWS = 16384, MAX_OUT = 1u << 24;
 
@@ -109,6 +110,7 @@ struct GrowArgs {
   int32_t *q_start, *positions;
   int64_t* slots;
   uint32_t n_out;
+  uint32_t later;  // the tokens' positions and slots are written by pages_place_kernel; a row's first one gets the position alone
 };
 
 // Whether row r has room for its tokens, which begin at `start` of the output; the pages that it needs.
@@ -174,6 +176,14 @@ __global__ void __launch_bounds__(GROW_THREADS, 1) pages_grow_kernel(const __gri
     }
   }
   __syncthreads();
+  if (g.later) {
+    for (uint32_t r = r0; r < r1; r++) {
+      const bool fits = !(refused[r >> 5] >> (r & 31) & 1);
+      if (g.n_new[r] > 0 && starts[r] < g.n_out) g.positions[starts[r]] = fits ? t.kv_len[r] : -1;
+      if (fits) t.kv_len[r] += g.n_new[r];
+    }
+    return;
+  }
   for (uint32_t i = threadIdx.x; i < g.n_out; i += GROW_THREADS) {
     int32_t pos = -1;
     int64_t slot = -1;
@@ -190,6 +200,35 @@ __global__ void __launch_bounds__(GROW_THREADS, 1) pages_grow_kernel(const __gri
   __syncthreads();
   for (uint32_t r = r0; r < r1; r++)
     if (!(refused[r >> 5] >> (r & 31) & 1)) t.kv_len[r] += g.n_new[r];
+}
+
+// A thread per token. (The row of a warp's first token and of its last one are looked for by the warp.)
+constexpr uint32_t PLACE_THREADS = 256;
+__global__ void __launch_bounds__(PLACE_THREADS) pages_place_kernel(const __grid_constant__ GrowArgs g) {
+  const Tables& t = g.t;
+  const uint32_t lane = threadIdx.x & 31, i = blockIdx.x * PLACE_THREADS + threadIdx.x, i0 = i - lane;
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t total = g.q_start[t.n_rows], last = min(i0 + 31, g.n_out - 1);
+  int32_t pos = -1;
+  int64_t slot = -1;
+  if (i0 < total) {  // (the whole warp; q_start[0] is 0)
+    uint32_t lo = kv4::last_begun(g.q_start, t.n_rows, static_cast<int>(i0), lane), hi = kv4::last_begun(g.q_start, t.n_rows, static_cast<int>(last), lane) + 1;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) >> 1;
+      if (static_cast<uint32_t>(g.q_start[mid]) <= i) lo = mid;
+      else hi = mid;
+    }
+    const uint32_t start = g.q_start[lo];
+    const int32_t base = g.positions[start];
+    if (i <= last && i < total && base >= 0) {
+      pos = base + static_cast<int32_t>(i - start);
+      slot = (static_cast<int64_t>(t.row(lo)[pos >> t.log_page]) << t.log_page) + (pos & (t.page - 1));
+    }
+  }
+  if (i >= g.n_out) return;
+  g.positions[i] = pos;  // (a row's first one: what it is already)
+  g.slots[i] = slot;
 }
 
 // ---- release ---------------------------------------------------------------------------------------------------------
@@ -228,7 +267,25 @@ __global__ void __launch_bounds__(ROW_THREADS) pages_release_kernel(const __grid
   const int32_t tokens = tokens_s;
   if (tokens < 0 && threadIdx.x == 0) note_range(t.err);
   const uint32_t n = entries_of(t, max(tokens, 0));
-  for (uint32_t i = threadIdx.x; i < n; i += ROW_THREADS) let_go(t, t.row(r)[i]);
+  const int32_t* row = t.row(r);
+  for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 4 * ROW_THREADS) {  // four of a thread on their way
+    int32_t page[4], refs[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) page[k] = i0 + k * ROW_THREADS < n ? row[i0 + k * ROW_THREADS] : 0;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) {
+      refs[k] = 1;
+      if (i0 + k * ROW_THREADS >= n) continue;
+      if (static_cast<uint32_t>(page[k]) < t.n_pages) refs[k] = atomicSub(&t.refs[page[k]], 1);
+      else note_range(t.err);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) {
+      if (refs[k] > 0) continue;  // (nobody held it)
+      atomicAdd(&t.refs[page[k]], 1);
+      note_range(t.err);
+    }
+  }
 }
 
 // ---- fork ------------------------------------------------------------------------------------------------------------
@@ -277,6 +334,7 @@ __global__ void __launch_bounds__(ROW_THREADS) pages_fork_kernel(const __grid_co
     if (tokens > 0) {
       const int32_t* from = t.row(parent);
       int32_t* to = t.row(child);
+#pragma unroll 4
       for (uint32_t k = threadIdx.x; k < static_cast<uint32_t>(tokens) >> t.log_page; k += ROW_THREADS) {
         const int32_t page = from[k];
         to[k] = page;
@@ -470,7 +528,10 @@ int bp_pages_grow(bp_paged_ctx* c, void* stream, const bp_page_tables* tables, c
   OnDevice on(c->device);
   BP_TRY(c, on.err);
   const size_t smem = (GROW_THREADS * WORDS + 2 * (g.t.n_rows + 1) + (g.t.n_rows + 31) / 32) * 4;
+  // A second launch costs some 2 us, a thousand tokens in one CTA 0.6.
+  g.later = n_out > 4096;
   BP_TRY(c, bp_launch(true, pages_grow_kernel, dim3(1), dim3(GROW_THREADS), smem, static_cast<cudaStream_t>(stream), g));
+  if (g.later) BP_TRY(c, bp_launch(true, pages_place_kernel, dim3((n_out + PLACE_THREADS - 1) / PLACE_THREADS), dim3(PLACE_THREADS), 0, static_cast<cudaStream_t>(stream), g));
   return BP_OK;
 }
 
