@@ -10,6 +10,7 @@ stream is CUDA's legacy default stream, for which torch's other streams do not w
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 from . import _lib
 from .attention import _stream
@@ -17,16 +18,18 @@ from .errors import ConfigError, raise_for_status
 
 _LAYOUTS = {"half": 0, "interleaved": 1}
 _SCALINGS = {None: 0, "linear": 1, "ntk": 2, "yarn": 3}
-_DTYPES, _I32, _I64 = {}, None, None
+_DTYPES, _I32, _I64, _F32 = {}, None, None, None
 _U32 = 0xFFFFFFFF
+# the structs of include/bonsai_pages.h up to their scale, written at once (a field at a time costs 60 ns each)
+_SHARED, _CHOICE, _CHOSEN = struct.Struct("PqqPqq7P9I").pack_into, struct.Struct("Pqq5P9I").pack_into, struct.Struct("PqqPqq2P3I").pack_into
 
 
 def _types():
     """The torch types (the package itself does not import torch; whoever calls with tensors has)."""
-    global _I32, _I64
+    global _I32, _I64, _F32
     import torch
     _DTYPES.update({torch.float16: 0, torch.bfloat16: 1})
-    _I32, _I64 = torch.int32, torch.int64
+    _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
 
 
 def _current(device):
@@ -397,32 +400,36 @@ class PagedContext:
         """A page table's requests, address and pitch, and `most` cut to the keys that a row has pages for."""
         if t.get_device() != self._device:
             _elsewhere(t, what, self._device)
-        if t.dtype is not _I32 or t.dim() != 2:
+        shape, stride = t.shape, t.stride()
+        if t.dtype is not _I32 or len(shape) != 2:
             _bad(f"{what} must be int32 [rows, pages]")
-        (n, pages), (stride, dense) = t.shape, t.stride()
-        if (dense != 1 and pages > 1) or (stride < pages and n > 1):
+        (n, pages), (pitch, dense) = shape, stride
+        if (dense != 1 and pages > 1) or (pitch < pages and n > 1):
             _bad(f"the rows of {what} must be dense and not overlap")
         if most < 0:
             _bad("the largest numbers of queries and keys must be >= 0")
-        most, pitch = min(most, pages * page_tokens), stride if n > 1 else pages
+        if most > pages * page_tokens:
+            most = pages * page_tokens
+        if n <= 1:
+            pitch = pages
         if most > _U32 or pitch > _U32:
             _bad(f"the keys and the distance of two rows of {what} must be below 2^32")
         return n, t.data_ptr(), pitch, most
 
-    def _queries(self, pool, q, out, to):
-        """q and out into a struct; their type's code."""
-        dtype, shape = q.dtype, q.shape
-        code = _code(dtype)
-        _rows(to.q, q, "q", self._device)
-        if out is not None:
-            _like(out, dtype, shape, "out")
-            _rows(to.out, out, "out", self._device)
+    def _queries(self, pool, q, what="q"):
+        """The shape of q (or out), its address and strides."""
+        if q.get_device() != self._device:
+            _elsewhere(q, what, self._device)
+        shape, stride = q.shape, q.stride()
+        if len(stride) != 3:
+            _bad(f"{what} must be [tokens, heads, head_dim], not {tuple(shape)}")
+        if stride[2] != 1 and shape[2] > 1:
+            _bad(f"a row of {what} must be dense")
         if pool.device != self._device:
             _elsewhere(pool.data, "the pool", self._device)
         if shape[2] != pool.head_dim:
-            _bad(f"q has head_dim {shape[2]}, the pool {pool.head_dim}")
-        to.total_q, to.n_head = shape[0], shape[1]
-        return code
+            _bad(f"{what} has head_dim {shape[2]}, the pool {pool.head_dim}")
+        return shape, q.data_ptr(), stride[0], stride[1]
 
     def shared_work(self, total_q, n_head, head_dim):
         """float32 values of attention_shared's `work` for that many rows."""
@@ -433,21 +440,23 @@ class PagedContext:
     def attention_shared(self, pool, q, out, q_start, kv_len, page_table, prefix_start, prefix_len, prefix_table, work, max_q, max_kv, max_prefix, scale=None, stream=None):
         """attention() for requests behind prefixes in common: the requests prefix_start[g] .. prefix_start[g + 1] see the prefix_len[g] keys in the
         pages prefix_table[g], then their own. work: a float32 tensor of at least shared_work(...) values, for this call's partial results."""
-        a, device = self._shared, self._device
-        code = self._queries(pool, q, out, a)
-        n_req, a.page_table, a.table_stride, a.max_kv = self._table(page_table, "page_table", pool.page_tokens, max_kv)
-        n_prefix, a.prefix_table, a.prefix_stride, a.max_prefix = self._table(prefix_table, "prefix_table", pool.page_tokens, max_prefix)
+        a, device, dtype = self._shared, self._device, q.dtype
+        code = _code(dtype)
+        shape, *rows = self._queries(pool, q)
+        _like(out, dtype, shape, "out")
+        n_req, table, pitch, max_kv = self._table(page_table, "page_table", pool.page_tokens, max_kv)
+        n_prefix, prefix, prefix_pitch, max_prefix = self._table(prefix_table, "prefix_table", pool.page_tokens, max_prefix)
+        total, heads, dim = shape
         if max_q < 0:
             _bad("max_q must be >= 0")
-        total, heads = a.total_q, a.n_head
         if work.get_device() != device:
             _elsewhere(work, "work", device)
-        if str(work.dtype) != "torch.float32" or not work.is_contiguous() or work.numel() < self._lib.bp_kv4_shared_work(total, heads, pool.head_dim):
+        if work.dtype is not _F32 or not work.is_contiguous() or work.numel() < self._lib.bp_kv4_shared_work(total, heads, dim):
             _bad("work must be dense float32 of at least shared_work(total_q, n_head, head_dim) values")
-        a.q_start, a.kv_len = _index(q_start, "q_start", n_req + 1, device), _index(kv_len, "kv_len", n_req, device)
-        a.prefix_start, a.prefix_len = _index(prefix_start, "prefix_start", n_prefix + 1, device), _index(prefix_len, "prefix_len", n_prefix, device)
-        a.work, a.n_req, a.n_prefix, a.max_q = work.data_ptr(), n_req, n_prefix, max_q if max_q < total else total
-        a.scale = pool.head_dim ** -0.5 if scale is None else scale
+        _SHARED(a, 0, *rows, *self._queries(pool, out, "out")[1:], _index(q_start, "q_start", n_req + 1, device), _index(kv_len, "kv_len", n_req, device), table,
+                _index(prefix_start, "prefix_start", n_prefix + 1, device), _index(prefix_len, "prefix_len", n_prefix, device), prefix, work.data_ptr(),
+                n_req, heads, total, max_q if max_q < total else total, max_kv, pitch, n_prefix, max_prefix, prefix_pitch)
+        a.scale = dim ** -0.5 if scale is None else scale
         st = self._lib.bp_kv4_attention_shared(self._h, _current(device) if stream is None else _stream(stream), code, pool._p, self._pshared)
         if st:
             self._check(st)
@@ -472,16 +481,15 @@ class PagedContext:
     def select(self, pool, summary, q, pages, keys, q_start, kv_len, page_table, max_q, max_kv, first=1, last=1, stream=None):
         """For every token and KV head the pages with the highest scores among those it sees, as many as pages [tokens, KV heads, pages] (int32) has
         places, the first `first` and last `last` always; keys [tokens] (int32): the keys in them."""
-        p, a, device = self._summary(pool, summary), self._choice, self._device
-        code = self._queries(pool, q, None, a)
-        n_req, a.page_table, a.table_stride, a.max_kv = self._table(page_table, "page_table", pool.page_tokens, max_kv)
-        total = a.total_q
-        a.pages, a.chosen = self._lists(pool, pages, total)
-        if max_q < 0 or not (0 <= first <= _U32 and 0 <= last <= _U32):
-            _bad("max_q, first and last must be >= 0")
-        a.keys = _index(keys, "keys", total, device)
-        a.q_start, a.kv_len = _index(q_start, "q_start", n_req + 1, device), _index(kv_len, "kv_len", n_req, device)
-        a.n_req, a.max_q, a.first, a.last = n_req, max_q if max_q < total else total, first, last
+        p, device = self._summary(pool, summary), self._device
+        code = _code(q.dtype)
+        (total, heads, _), *rows = self._queries(pool, q)
+        n_req, table, pitch, max_kv = self._table(page_table, "page_table", pool.page_tokens, max_kv)
+        pages, chosen = self._lists(pool, pages, total)
+        if max_q < 0 or not (0 <= first <= _U32 and 0 <= last <= _U32) or chosen > _U32:
+            _bad("max_q, first, last and the places of pages must be >= 0 and below 2^32")
+        _CHOICE(self._choice, 0, *rows, _index(q_start, "q_start", n_req + 1, device), _index(kv_len, "kv_len", n_req, device), table, pages, _index(keys, "keys", total, device),
+                n_req, heads, total, max_q if max_q < total else total, max_kv, pitch, chosen, first, last)
         st = self._lib.bp_kv4_select(self._h, _current(device) if stream is None else _stream(stream), code, pool._p, p, self._pchoice)
         if st:
             self._check(st)
@@ -489,17 +497,23 @@ class PagedContext:
     def _lists(self, pool, pages, n):
         if pages.get_device() != self._device:
             _elsewhere(pages, "pages", self._device)
-        if pages.dtype is not _I32 or pages.dim() != 3 or pages.shape[0] != n or pages.shape[1] != pool.n_kv_head or not pages.is_contiguous():
-            _bad(f"pages must be dense int32 [{n}, {pool.n_kv_head}, pages], not {tuple(pages.shape)} {pages.dtype}")
-        return pages.data_ptr(), pages.shape[2]
+        shape = pages.shape
+        if pages.dtype is not _I32 or len(shape) != 3 or shape[0] != n or shape[1] != pool.n_kv_head or not pages.is_contiguous():
+            _bad(f"pages must be dense int32 [{n}, {pool.n_kv_head}, pages], not {tuple(shape)} {pages.dtype}")
+        return pages.data_ptr(), shape[2]
 
     def attention_selected(self, pool, q, out, pages, keys, scale=None, stream=None):
         """Attention of every token of q [tokens, heads, head_dim] over the pages that select() has chosen for it."""
-        a, device = self._chosen, self._device
-        code = self._queries(pool, q, out, a)
-        a.pages, a.chosen = self._lists(pool, pages, a.total_q)
-        a.keys = _index(keys, "keys", a.total_q, device)
-        a.scale = pool.head_dim ** -0.5 if scale is None else scale
+        a, device, dtype = self._chosen, self._device, q.dtype
+        code = _code(dtype)
+        shape, *rows = self._queries(pool, q)
+        _like(out, dtype, shape, "out")
+        total, heads, dim = shape
+        pages, chosen = self._lists(pool, pages, total)
+        if chosen > _U32:
+            _bad("the places of pages must be below 2^32")
+        _CHOSEN(a, 0, *rows, *self._queries(pool, out, "out")[1:], pages, _index(keys, "keys", total, device), heads, total, chosen)
+        a.scale = dim ** -0.5 if scale is None else scale
         st = self._lib.bp_kv4_attention_selected(self._h, _current(device) if stream is None else _stream(stream), code, pool._p, self._pchosen)
         if st:
             self._check(st)
