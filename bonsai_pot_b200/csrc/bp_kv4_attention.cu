@@ -516,73 +516,6 @@ __device__ __noinline__ uint32_t take_no_numbers(uint8_t* buf, int left, uint32_
   return found;
 }
 
-// One row of an item's partial results, joined by a warp: a lane has V dims. (Looking for the pieces one by one, four rows per warp and one piece after the other, took
-// 2.6 to 4.6 us per CTA, this 0.7 to 1.5.)
-template <int D>
-struct RowJoin {
-  static constexpr int V = D / 32;
-  float m = NEG_BIG, l = 0.f, o[V] = {};
-  // The pieces of the lanes in `mask`, in their order: `at` is the row in the lane's piece.
-  __device__ __forceinline__ void add(uint32_t mask, const float* at, uint32_t lane) {
-    const float2 ml = mask >> lane & 1 ? *reinterpret_cast<const float2*>(at + D) : make_float2(NEG_BIG, 0.f);
-    float top = ml.x;
-#pragma unroll
-    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, x));
-    top = fmaxf(top, m);
-    const float before = ex2(m - top), weight = ex2(ml.x - top);
-    float sum = weight * ml.y;
-#pragma unroll
-    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(FULL, sum, x);
-    l = l * before + sum;
-    m = top;
-#pragma unroll
-    for (int x = 0; x < V; x++) o[x] *= before;
-    while (mask) {  // four on their way
-      float w[4], e[4][V];
-#pragma unroll
-      for (int q = 0; q < 4; q++) {
-        const int x = mask ? __ffs(mask) - 1 : 0;
-        w[q] = __shfl_sync(FULL, weight, x);
-        const float* v = reinterpret_cast<const float*>(__shfl_sync(FULL, reinterpret_cast<unsigned long long>(at), x)) + V * lane;
-        if (!mask) w[q] = 0.f;
-#pragma unroll
-        for (int k = 0; k < V; k++) e[q][k] = 0.f;
-        if (mask) {
-          if constexpr (V == 4) {
-            const float4 f = *reinterpret_cast<const float4*>(v);
-            e[q][0] = f.x, e[q][1] = f.y, e[q][2] = f.z, e[q][3] = f.w;
-          } else {
-            const float2 f = *reinterpret_cast<const float2*>(v);
-            e[q][0] = f.x, e[q][1] = f.y;
-          }
-        }
-        mask &= mask - 1;
-      }
-#pragma unroll
-      for (int q = 0; q < 4; q++)
-#pragma unroll
-        for (int k = 0; k < V; k++) o[k] = fmaf(e[q][k], w[q], o[k]);
-    }
-  }
-  // A partial result again, or the output's dims from `out` on.
-  __device__ __forceinline__ void put(float* to, uint32_t lane) const {
-    if constexpr (V == 4) *reinterpret_cast<float4*>(to + V * lane) = make_float4(o[0], o[1], o[2], o[3]);
-    else *reinterpret_cast<float2*>(to + V * lane) = make_float2(o[0], o[1]);
-    if (lane == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m, l);
-  }
-  __device__ __forceinline__ void put(bool bf, uint16_t* out, uint32_t lane) const {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    out += V * lane;
-    if constexpr (V == 4) {
-      store4(bf, out, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-    } else {
-      const uint32_t h = bf ? pack2<true>(o[0] * inv, o[1] * inv) : pack2<false>(o[0] * inv, o[1] * inv);
-      out[0] = static_cast<uint16_t>(h);
-      out[1] = static_cast<uint16_t>(h >> 16);
-    }
-  }
-};
-
 // Zeros for the `n_tok` tokens of a request without keys, by a CTA. (Their values can be more than 32 bits count.) In parts: no weights.
 template <int D, int MODE>
 __device__ __noinline__ void zero_rows(const AttnArgs& a, int q0, uint32_t n_tok, bool prefix) {

@@ -24,7 +24,6 @@ constexpr uint32_t JOIN_THREADS = 256;
 // A warp per row.
 template <int D>
 __global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(const __grid_constant__ JoinArgs j) {
-  constexpr int V = D / 32;  // dims of a lane
   const AttnArgs& a = j.a;
   const uint32_t lane = threadIdx.x & 31;
   const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (JOIN_THREADS / 32) + (threadIdx.x >> 5);
@@ -59,56 +58,14 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv4_join_kernel(const __grid_con
     if (n[p] == 0) return record[p];
     return j.slots[p] + static_cast<size_t>(piece_at(c[p], k - (p ? n0 : 0))) * j.piece[p] + at[p] * RECORD<D>;
   };
-  float m = NEG_BIG, l = 0.f, o[V] = {};
+  RowJoin<D> join;
   for (uint32_t k0 = 0; k0 < all; k0 += 32) {
-    const uint32_t few = min(all - k0, 32u), k = k0 + lane;
-    float2 ml = make_float2(NEG_BIG, 0.f);
-    if (lane < few) ml = n[k >= n0] == 0 ? first[k >= n0] : *reinterpret_cast<const float2*>(piece(k) + D);
-    float top = ml.x;
-#pragma unroll
-    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, x));
-    top = fmaxf(top, m);
-    const float before = ex2(m - top), weight = ml.y == 0.f ? 0.f : ex2(ml.x - top);
-    float sum = weight * ml.y;
-#pragma unroll
-    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(FULL, sum, x);
-    l = l * before + sum;
-    m = top;
-#pragma unroll
-    for (int x = 0; x < V; x++) o[x] *= before;
-    for (uint32_t q0 = 0; q0 < few; q0 += 4) {  // four pieces on their way (one without weights may not have been written)
-      float e[4][V], w[4];
-#pragma unroll
-      for (uint32_t q = 0; q < 4; q++) {
-        w[q] = __shfl_sync(FULL, weight, q0 + q);  // 0 behind the last
-#pragma unroll
-        for (int x = 0; x < V; x++) e[q][x] = 0.f;
-        if (q0 + q < few && w[q] != 0.f) {
-          const float* v = piece(k0 + q0 + q) + V * lane;
-          if constexpr (V == 4) {
-            const float4 f = *reinterpret_cast<const float4*>(v);
-            e[q][0] = f.x, e[q][1] = f.y, e[q][2] = f.z, e[q][3] = f.w;
-          } else {
-            const float2 f = *reinterpret_cast<const float2*>(v);
-            e[q][0] = f.x, e[q][1] = f.y;
-          }
-        }
-      }
-#pragma unroll
-      for (uint32_t q = 0; q < 4; q++)
-#pragma unroll
-        for (int x = 0; x < V; x++) o[x] = fmaf(e[q][x], w[q], o[x]);
-    }
+    const uint32_t k = k0 + lane;
+    // (a record without weights may not have been written, pieces have)
+    const bool there = k < all && !(n[k >= n0] == 0 && first[k >= n0].y == 0.f);
+    join.add(__ballot_sync(FULL, there), piece(min(k, all - 1)), lane);
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint16_t* out = a.out.data + static_cast<int64_t>(token) * a.out.tok + static_cast<int64_t>(head) * a.out.head + V * lane;
-  if constexpr (V == 4) {
-    store4(a.bf, out, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-  } else {
-    const uint32_t h = a.bf ? pack2<true>(o[0] * inv, o[1] * inv) : pack2<false>(o[0] * inv, o[1] * inv);
-    out[0] = static_cast<uint16_t>(h);
-    out[1] = static_cast<uint16_t>(h >> 16);
-  }
+  join.put(a.bf, a.out.data + static_cast<int64_t>(token) * a.out.tok + static_cast<int64_t>(head) * a.out.head, lane);
 }
 
 }  // namespace
