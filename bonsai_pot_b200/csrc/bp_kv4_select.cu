@@ -274,6 +274,7 @@ __global__ void __launch_bounds__(CHOICE_THREADS) kv4_select_kernel(const __grid
     }
   }
   if (s.split > 1) {
+    __syncwarp();
     cluster_arrive();
     cluster_wait();
     if (rank) return;

@@ -4,7 +4,8 @@
 // result coming (grow, the end of a fork), rows are spread over CTAs where each is for itself (release, a fork's rows, the tables behind a
 // compaction). Free pages are found by looking at the reference counts, 32 per warp and load, in the order of the pages, so results do not depend on
 // who comes when; integer counts do not depend on the order of their atomics.
-#include "bp_kv4_attention.cuh"
+// Where the result is then spread out over many tokens or rows, the CTA has seven others beside it in a cluster, which wait for it at the cluster's barrier: one
+// launch (2.8 us on the host) less.
 #include "bp_paged_host.cuh"
 
 namespace {
@@ -12,7 +13,7 @@ namespace {
 using namespace bp;
 using namespace bp::paged;
 
-using kv4::FULL;
+constexpr unsigned FULL = 0xffffffffu;
 constexpr uint32_t WORDS = 8;  // words of 32 pages that a warp looks at at a time: as many loads are on their way
 constexpr uint32_t MAX_ROWS = 16384, MAX_OUT = 1u << 24;
 
@@ -24,48 +25,62 @@ struct Tables {
   __device__ int32_t* row(uint32_t r) const { return table + static_cast<size_t>(r) * stride; }
 };
 
-// The sum of v over the threads before this one, and of all.
-template <uint32_t THREADS, typename T>
-__device__ __forceinline__ T block_scan(T v, T* sums, T& total) {
+// Sums are limited to 2^30, more than any call takes: nothing wraps.
+constexpr uint32_t MANY = 1u << 30;
+__device__ __forceinline__ uint32_t plus(uint32_t a, uint32_t b) { return min(a + b, MANY); }  // (of two up to MANY)
+
+// The sums of v.x and v.y over the threads before this one, and of all.
+template <uint32_t THREADS>
+__device__ __forceinline__ uint2 block_scan(uint2 v, uint2* sums, uint2& total) {
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  T up = v;
+  uint2 up = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const T x = __shfl_up_sync(FULL, up, o);
-    if (lane >= o) up += x;
+    const uint32_t x = __shfl_up_sync(FULL, up.x, o), y = __shfl_up_sync(FULL, up.y, o);
+    if (lane >= o) up = make_uint2(plus(up.x, x), plus(up.y, y));
   }
   if (lane == 31) sums[warp] = up;
+  uint2 before = make_uint2(__shfl_up_sync(FULL, up.x, 1), __shfl_up_sync(FULL, up.y, 1));
+  if (lane == 0) before = make_uint2(0, 0);
   __syncthreads();
-  T before = 0;
-  total = 0;
+  total = make_uint2(0, 0);
+  uint2 warps = make_uint2(0, 0);
 #pragma unroll
   for (uint32_t w = 0; w < THREADS / 32; w++) {
-    if (w == warp) before = total;
-    total += sums[w];
+    if (w == warp) warps = total;
+    const uint2 s = sums[w];
+    total = make_uint2(plus(total.x, s.x), plus(total.y, s.y));
   }
   __syncthreads();
-  return before + up - v;
+  return make_uint2(plus(warps.x, before.x), plus(warps.y, before.y));
 }
 
+// The counts of the pages that a lane looks at next, from `base` on (or from the last page down).
+template <bool USED_FROM_TOP>
+struct Look {
+  int32_t refs[WORDS];
+  __device__ __forceinline__ void ask(const Tables& t, uint32_t base) {
+#pragma unroll
+    for (uint32_t k = 0; k < WORDS; k++) {
+      const uint32_t at = base + ((threadIdx.x >> 5) * WORDS + k) * 32 + (threadIdx.x & 31);
+      refs[k] = at < t.n_pages ? t.refs[USED_FROM_TOP ? t.n_pages - 1 - at : at] : USED_FROM_TOP ? 0 : 1;
+    }
+  }
+};
 // The first `want` pages that are free (or the last that are used), as use(rank, page), a thread each; how many there are, `want` at most.
-// list: THREADS * WORDS places in shared memory.
+// look: has asked for the first ones. list: THREADS * WORDS places in shared memory.
 template <uint32_t THREADS, bool USED_FROM_TOP, typename Use>
-__device__ __forceinline__ uint32_t find_pages(const Tables& t, uint32_t want, uint32_t* list, uint32_t* sums, Use use) {
+__device__ __forceinline__ uint32_t find_pages(const Tables& t, Look<USED_FROM_TOP>& look, uint32_t want, uint32_t* list, uint32_t* sums, Use use) {
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t found = 0;
   for (uint32_t base = 0; base < t.n_pages && found < want; base += THREADS * WORDS) {
     uint32_t mask[WORDS], mine = 0;
-    int32_t refs[WORDS];
 #pragma unroll
     for (uint32_t k = 0; k < WORDS; k++) {
-      const uint32_t at = base + (warp * WORDS + k) * 32 + lane;
-      refs[k] = at < t.n_pages ? t.refs[USED_FROM_TOP ? t.n_pages - 1 - at : at] : USED_FROM_TOP ? 0 : 1;
-    }
-#pragma unroll
-    for (uint32_t k = 0; k < WORDS; k++) {
-      mask[k] = __ballot_sync(FULL, USED_FROM_TOP ? refs[k] > 0 : refs[k] == 0);
+      mask[k] = __ballot_sync(FULL, USED_FROM_TOP ? look.refs[k] > 0 : look.refs[k] == 0);
       mine += __popc(mask[k]);
     }
+    if (base + THREADS * WORDS < t.n_pages) look.ask(t, base + THREADS * WORDS);
     if (lane == 0) sums[warp] = mine;
     __syncthreads();
     uint32_t before = 0, all = 0;
@@ -110,125 +125,116 @@ struct GrowArgs {
   int32_t *q_start, *positions;
   int64_t* slots;
   uint32_t n_out;
-  uint32_t later;  // the tokens' positions and slots are written by pages_place_kernel; a row's first one gets the position alone
 };
 
-// Whether row r has room for its tokens, which begin at `start` of the output; the pages that it needs.
-__device__ __forceinline__ bool row_fits(const GrowArgs& g, uint32_t r, uint64_t start, uint32_t& need) {
+// Whether row r has room for its tokens; the pages that it needs.
+__device__ __forceinline__ bool row_fits(const GrowArgs& g, uint32_t r, uint32_t& need) {
   const int32_t kv = g.t.kv_len[r], n = g.n_new[r];
   need = 0;
-  if (kv < 0 || n < 0 || start + n > g.n_out) return false;
+  if (kv < 0 || n < 0) return false;
   const uint64_t after = static_cast<uint64_t>(kv) + n;
   if (after > 0x7fffffffu || g.t.pages_of(static_cast<uint32_t>(after)) > g.t.row_pages) return false;
   need = g.t.pages_of(static_cast<uint32_t>(after)) - g.t.pages_of(kv);
   return true;
 }
+// Its tokens, which begin at `start` of the output, have places there.
+__device__ __forceinline__ bool has_places(const GrowArgs& g, uint32_t r, uint32_t start) { return static_cast<uint64_t>(start) + max(g.n_new[r], 0) <= g.n_out; }
 
-// One CTA. A thread has `per` rows side by side; their starts and the ranks of their new pages lie in shared memory, where a new page and a token find their row.
-__global__ void __launch_bounds__(GROW_THREADS, 1) pages_grow_kernel(const __grid_constant__ GrowArgs g) {
-  extern __shared__ uint32_t smem[];
-  uint32_t *list = smem, *starts = list + GROW_THREADS * WORDS, *ranks = starts + g.t.n_rows + 1, *refused = ranks + g.t.n_rows + 1;
-  __shared__ uint64_t sums64[GROW_THREADS / 32];
-  __shared__ uint32_t sums[GROW_THREADS / 32];
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// What the rows get, by one CTA. A thread has `per` rows side by side; where a row's tokens start and the rank of its first new page lie in shared memory, where a new page
+// finds its row. In the end ranks[r] is the row's length before, -1 if it is refused; to the other CTAs its first token's position says so.
+__device__ __forceinline__ void grow_rows(const GrowArgs& g, uint32_t* list, uint32_t* starts, uint32_t* ranks, uint2* sums2, uint32_t* sums) {
   const Tables& t = g.t;
   const uint32_t per = (t.n_rows + GROW_THREADS - 1) / GROW_THREADS, r0 = min(threadIdx.x * per, t.n_rows), r1 = min(r0 + per, t.n_rows);
-  for (uint32_t i = threadIdx.x; i < (t.n_rows + 31) / 32; i += GROW_THREADS) refused[i] = 0;
-  pdl_launch_dependents();
-  pdl_wait();
-  uint64_t n = 0, total, need_all;
-  for (uint32_t r = r0; r < r1; r++) n += max(g.n_new[r], 0);
-  uint64_t at = block_scan<GROW_THREADS>(n, sums64, total);
-  uint64_t need = 0;
+  Look<false> look;
+  look.ask(t, 0);
+  uint2 sum = make_uint2(0, 0), total;
+  uint32_t need;
   for (uint32_t r = r0; r < r1; r++) {
-    uint32_t more;
-    starts[r] = static_cast<uint32_t>(min(at, static_cast<uint64_t>(0x7fffffffu)));
-    if (!row_fits(g, r, at, more)) {
-      atomicOr(&refused[r >> 5], 1u << (r & 31));
-      note_range(t.err);
+    (void)row_fits(g, r, need);
+    sum = make_uint2(plus(sum.x, min(static_cast<uint32_t>(max(g.n_new[r], 0)), MANY)), plus(sum.y, need));
+  }
+  uint2 at = block_scan<GROW_THREADS>(sum, sums2, total);
+  const uint32_t tokens = total.x;
+  if (tokens > g.n_out) {  // some rows' tokens have no places: these rows need no pages
+    uint32_t start = at.x;
+    sum.y = 0;
+    for (uint32_t r = r0; r < r1; r++) {
+      (void)row_fits(g, r, need);
+      if (has_places(g, r, start)) sum.y = plus(sum.y, need);
+      start = plus(start, min(static_cast<uint32_t>(max(g.n_new[r], 0)), MANY));
     }
-    need += more;
-    at += max(g.n_new[r], 0);
+    at.y = block_scan<GROW_THREADS>(sum, sums2, total).y;
   }
-  uint64_t rank = block_scan<GROW_THREADS>(need, sums64, need_all);
   for (uint32_t r = r0; r < r1; r++) {
-    uint32_t more;
-    ranks[r] = static_cast<uint32_t>(min(rank, static_cast<uint64_t>(0xffffffffu)));
-    (void)row_fits(g, r, starts[r], more);
-    rank += more;
-    g.q_start[r] = static_cast<int32_t>(starts[r]);
+    starts[r] = at.x;
+    ranks[r] = at.y;
+    g.q_start[r] = static_cast<int32_t>(at.x);
+    (void)row_fits(g, r, need);
+    at = make_uint2(plus(at.x, min(static_cast<uint32_t>(max(g.n_new[r], 0)), MANY)), has_places(g, r, starts[r]) ? plus(at.y, need) : at.y);
   }
-  if (threadIdx.x == 0) g.q_start[t.n_rows] = static_cast<int32_t>(min(total, static_cast<uint64_t>(0x7fffffffu)));
+  if (threadIdx.x == 0) {
+    starts[t.n_rows] = tokens;
+    g.q_start[t.n_rows] = static_cast<int32_t>(tokens);
+  }
   __syncthreads();
-  const uint32_t want = static_cast<uint32_t>(min(need_all, static_cast<uint64_t>(t.n_pages)));
-  const uint32_t found = find_pages<GROW_THREADS, false>(t, want, list, sums, [&](uint32_t k, uint32_t page) {
+  const uint32_t found = find_pages<GROW_THREADS, false>(t, look, total.y, list, sums, [&](uint32_t k, uint32_t page) {
     const uint32_t r = last_begun(ranks, t.n_rows, k);
     t.row(r)[t.pages_of(t.kv_len[r]) + k - ranks[r]] = static_cast<int32_t>(page);
     t.refs[page] = 1;
   });
-  if (found < need_all) {  // some rows do not get all their pages: they get none
-    __syncthreads();
-    for (uint32_t r = r0; r < r1; r++) {
-      uint32_t more;
-      if (!row_fits(g, r, starts[r], more) || more == 0 || static_cast<uint64_t>(ranks[r]) + more <= found) continue;
-      for (uint32_t k = ranks[r]; k < found; k++) t.refs[t.row(r)[t.pages_of(t.kv_len[r]) + k - ranks[r]]] = 0;
-      atomicOr(&refused[r >> 5], 1u << (r & 31));
-      note_range(t.err);
+  __syncthreads();
+  for (uint32_t r = r0; r < r1; r++) {
+    const int32_t kv = t.kv_len[r];
+    bool fits = row_fits(g, r, need) && has_places(g, r, starts[r]);
+    if (fits && need > 0 && ranks[r] + need > found) {  // it does not get all its pages: it gets none
+      for (uint32_t k = ranks[r]; k < found; k++) t.refs[t.row(r)[t.pages_of(kv) + k - ranks[r]]] = 0;
+      fits = false;
+    }
+    if (!fits) note_range(t.err);
+    ranks[r] = fits ? static_cast<uint32_t>(kv) : 0xffffffffu;
+    if (gridDim.x > 1 && g.n_new[r] > 0 && starts[r] < g.n_out) g.positions[starts[r]] = fits ? kv : -1;
+    if (fits) t.kv_len[r] = kv + g.n_new[r];
+  }
+}
+__global__ void __launch_bounds__(GROW_THREADS, 1) pages_grow_kernel(const __grid_constant__ GrowArgs g) {
+  extern __shared__ uint32_t smem[];
+  uint32_t *list = smem, *starts = list + GROW_THREADS * WORDS, *bases = starts + g.t.n_rows + 1;
+  __shared__ uint2 sums2[GROW_THREADS / 32];
+  __shared__ uint32_t sums[GROW_THREADS / 32];
+  const Tables& t = g.t;
+  pdl_launch_dependents();
+  pdl_wait();
+  if (blockIdx.x == 0) grow_rows(g, list, starts, bases, sums2, sums);
+  if (gridDim.x > 1) cluster_sync();
+  if (blockIdx.x != 0) {
+    for (uint32_t r = threadIdx.x; r <= t.n_rows; r += GROW_THREADS) {
+      const uint32_t start = g.q_start[r];
+      starts[r] = start;
+      if (r < t.n_rows) bases[r] = start < g.n_out ? g.positions[start] : -1;
     }
   }
   __syncthreads();
-  if (g.later) {
-    for (uint32_t r = r0; r < r1; r++) {
-      const bool fits = !(refused[r >> 5] >> (r & 31) & 1);
-      if (g.n_new[r] > 0 && starts[r] < g.n_out) g.positions[starts[r]] = fits ? t.kv_len[r] : -1;
-      if (fits) t.kv_len[r] += g.n_new[r];
-    }
-    return;
-  }
-  for (uint32_t i = threadIdx.x; i < g.n_out; i += GROW_THREADS) {
+  const uint32_t total = starts[t.n_rows];
+#pragma unroll 2
+  for (uint32_t i = blockIdx.x * GROW_THREADS + threadIdx.x; i < g.n_out; i += gridDim.x * GROW_THREADS) {
     int32_t pos = -1;
     int64_t slot = -1;
     if (i < total) {
       const uint32_t r = last_begun(starts, t.n_rows, i);
-      if (!(refused[r >> 5] >> (r & 31) & 1)) {
-        pos = t.kv_len[r] + static_cast<int32_t>(i - starts[r]);
+      if (bases[r] != 0xffffffffu) {
+        pos = static_cast<int32_t>(bases[r] + (i - starts[r]));
         slot = (static_cast<int64_t>(t.row(r)[pos >> t.log_page]) << t.log_page) + (pos & (t.page - 1));
       }
     }
-    g.positions[i] = pos;
+    g.positions[i] = pos;  // (a row's first one: what it is already)
     g.slots[i] = slot;
   }
-  __syncthreads();
-  for (uint32_t r = r0; r < r1; r++)
-    if (!(refused[r >> 5] >> (r & 31) & 1)) t.kv_len[r] += g.n_new[r];
-}
-
-// A thread per token. (The row of a warp's first token and of its last one are looked for by the warp.)
-constexpr uint32_t PLACE_THREADS = 256;
-__global__ void __launch_bounds__(PLACE_THREADS) pages_place_kernel(const __grid_constant__ GrowArgs g) {
-  const Tables& t = g.t;
-  const uint32_t lane = threadIdx.x & 31, i = blockIdx.x * PLACE_THREADS + threadIdx.x, i0 = i - lane;
-  pdl_launch_dependents();
-  pdl_wait();
-  const uint32_t total = g.q_start[t.n_rows], last = min(i0 + 31, g.n_out - 1);
-  int32_t pos = -1;
-  int64_t slot = -1;
-  if (i0 < total) {  // (the whole warp; q_start[0] is 0)
-    uint32_t lo = kv4::last_begun(g.q_start, t.n_rows, static_cast<int>(i0), lane), hi = kv4::last_begun(g.q_start, t.n_rows, static_cast<int>(last), lane) + 1;
-    while (hi - lo > 1) {
-      const uint32_t mid = (lo + hi) >> 1;
-      if (static_cast<uint32_t>(g.q_start[mid]) <= i) lo = mid;
-      else hi = mid;
-    }
-    const uint32_t start = g.q_start[lo];
-    const int32_t base = g.positions[start];
-    if (i <= last && i < total && base >= 0) {
-      pos = base + static_cast<int32_t>(i - start);
-      slot = (static_cast<int64_t>(t.row(lo)[pos >> t.log_page]) << t.log_page) + (pos & (t.page - 1));
-    }
-  }
-  if (i >= g.n_out) return;
-  g.positions[i] = pos;  // (a row's first one: what it is already)
-  g.slots[i] = slot;
 }
 
 // ---- release ---------------------------------------------------------------------------------------------------------
@@ -309,6 +315,7 @@ __global__ void __launch_bounds__(ROW_THREADS) pages_fork_kernel(const __grid_co
   extern __shared__ uint32_t smem[];
   uint32_t *list = smem, *ranks = smem + ROW_THREADS * WORDS;
   int32_t* lengths = reinterpret_cast<int32_t*>(ranks + f.n);  // tokens of the pairs' parents, -1 where there is no pair that holds its child
+  __shared__ uint2 sums2[ROW_THREADS / 32];
   __shared__ uint32_t sums[ROW_THREADS / 32], last_s;
   __shared__ int32_t tokens_s;
   const Tables& t = f.t;
@@ -353,7 +360,10 @@ __global__ void __launch_bounds__(ROW_THREADS) pages_fork_kernel(const __grid_co
 
   // ---- the last CTA ----
   const uint32_t per = (f.n + ROW_THREADS - 1) / ROW_THREADS, i0 = min(threadIdx.x * per, f.n), i1 = min(i0 + per, f.n);
-  uint32_t need = 0, want, parent, child;
+  Look<false> look;
+  look.ask(t, 0);
+  uint32_t need = 0, parent, child;
+  uint2 total;
   for (uint32_t i = i0; i < i1; i++) {
     int32_t tokens = -1;
     if (is_pair(f, i, parent, child) && *reinterpret_cast<volatile int32_t*>(&t.kv_len[child]) == -1 - static_cast<int32_t>(i))
@@ -362,13 +372,13 @@ __global__ void __launch_bounds__(ROW_THREADS) pages_fork_kernel(const __grid_co
     need += tokens > 0 && (tokens & (t.page - 1));
     f.src[i] = f.dst[i] = -1;
   }
-  uint32_t rank = block_scan<ROW_THREADS>(need, sums, want);
+  uint32_t rank = block_scan<ROW_THREADS>(make_uint2(need, 0), sums2, total).x;
   for (uint32_t i = i0; i < i1; i++) {
     ranks[i] = rank;
     rank += lengths[i] > 0 && (lengths[i] & (t.page - 1));
   }
   __syncthreads();
-  const uint32_t found = find_pages<ROW_THREADS, false>(t, want, list, sums, [&](uint32_t k, uint32_t page) {
+  const uint32_t found = find_pages<ROW_THREADS, false>(t, look, total.x, list, sums, [&](uint32_t k, uint32_t page) {
     const uint32_t i = last_begun(ranks, f.n, k), at = static_cast<uint32_t>(lengths[i]) >> t.log_page;
     const int32_t from = t.row(f.parents[i])[at];
     t.row(f.children[i])[at] = static_cast<int32_t>(page);
@@ -401,15 +411,15 @@ struct CompactArgs {
   uint32_t most;
   uint32_t* counter;
 };
-// One CTA: what moves where. The count of a page that moves becomes -1 - (where it goes) for the kernel behind this one.
-__global__ void __launch_bounds__(GROW_THREADS, 1) pages_plan_kernel(const __grid_constant__ CompactArgs c) {
-  extern __shared__ uint32_t smem[];
-  __shared__ uint32_t sums[GROW_THREADS / 32];
+// What moves where, by one CTA. The count of a page that moves becomes -1 - (where it goes) for the tables' entries.
+__device__ __forceinline__ void plan_moves(const CompactArgs& c, uint32_t* smem, uint32_t* sums) {
   const Tables& t = c.t;
-  pdl_launch_dependents();
-  pdl_wait();
-  const uint32_t low = find_pages<GROW_THREADS, false>(t, c.most, smem, sums, [&](uint32_t i, uint32_t page) { c.dst[i] = static_cast<int32_t>(page); });
-  const uint32_t high = find_pages<GROW_THREADS, true>(t, c.most, smem, sums, [&](uint32_t i, uint32_t page) { c.src[i] = static_cast<int32_t>(page); });
+  Look<false> first;
+  Look<true> last;
+  first.ask(t, 0);
+  last.ask(t, 0);
+  const uint32_t low = find_pages<GROW_THREADS, false>(t, first, c.most, smem, sums, [&](uint32_t i, uint32_t page) { c.dst[i] = static_cast<int32_t>(page); });
+  const uint32_t high = find_pages<GROW_THREADS, true>(t, last, c.most, smem, sums, [&](uint32_t i, uint32_t page) { c.src[i] = static_cast<int32_t>(page); });
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < c.most; i += GROW_THREADS) {
     const int32_t from = i < high ? c.src[i] : -1, to = i < low ? c.dst[i] : -1;
@@ -421,26 +431,56 @@ __global__ void __launch_bounds__(GROW_THREADS, 1) pages_plan_kernel(const __gri
     }
   }
 }
-// The tables' entries follow; the CTA that comes last makes the pages that have moved free.
-__global__ void __launch_bounds__(ROW_THREADS) pages_follow_kernel(const __grid_constant__ CompactArgs c) {
-  __shared__ uint32_t last_s;
+// A row's entries follow, four of a lane on their way.
+__device__ __forceinline__ void follow_moves(const CompactArgs& c, uint32_t r, uint32_t lane) {
   const Tables& t = c.t;
-  pdl_launch_dependents();
-  pdl_wait();
-  for (uint32_t r = blockIdx.x; r < t.n_rows; r += gridDim.x) {
-    const int32_t tokens = t.kv_len[r];
-    if (tokens < 0 && threadIdx.x == 0) note_range(t.err);
-    const uint32_t n = entries_of(t, max(tokens, 0));
-    for (uint32_t i = threadIdx.x; i < n; i += ROW_THREADS) {
-      const int32_t page = t.row(r)[i];
-      if (static_cast<uint32_t>(page) >= t.n_pages) {
-        note_range(t.err);
-        continue;
-      }
-      const int32_t refs = t.refs[page];
-      if (refs < 0) t.row(r)[i] = -1 - refs;
+  const int32_t tokens = t.kv_len[r];
+  if (tokens < 0 && lane == 0) note_range(t.err);
+  const uint32_t n = entries_of(t, max(tokens, 0));
+  int32_t* row = t.row(r);
+  for (uint32_t i0 = lane; i0 < n; i0 += 128) {
+    int32_t page[4], refs[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) page[k] = i0 + 32 * k < n ? row[i0 + 32 * k] : 0;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) refs[k] = static_cast<uint32_t>(page[k]) < t.n_pages ? t.refs[page[k]] : 0;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) {
+      if (static_cast<uint32_t>(page[k]) >= t.n_pages) note_range(t.err);
+      if (refs[k] < 0 && i0 + 32 * k < n) row[i0 + 32 * k] = -1 - refs[k];
     }
   }
+}
+__device__ __forceinline__ void free_moved(const CompactArgs& c) {
+  for (uint32_t i = threadIdx.x; i < c.most; i += blockDim.x)
+    if (c.src[i] >= 0) c.t.refs[c.src[i]] = 0;
+}
+// All of it by a cluster, a warp per row: tables of up to COMPACT_ENTRIES entries.
+constexpr uint32_t COMPACT_ENTRIES = 1u << 18;
+__global__ void __launch_bounds__(GROW_THREADS, 1) pages_compact_kernel(const __grid_constant__ CompactArgs c) {
+  extern __shared__ uint32_t smem[];
+  __shared__ uint32_t sums[GROW_THREADS / 32];
+  pdl_launch_dependents();
+  pdl_wait();
+  if (blockIdx.x == 0) plan_moves(c, smem, sums);
+  cluster_sync();
+  for (uint32_t r = blockIdx.x * (GROW_THREADS / 32) + (threadIdx.x >> 5); r < c.t.n_rows; r += gridDim.x * (GROW_THREADS / 32)) follow_moves(c, r, threadIdx.x & 31);
+  cluster_sync();
+  if (blockIdx.x == 0) free_moved(c);
+}
+// Larger ones: the plan, then the rows by all SMs; the CTA that comes last makes the pages that have moved free.
+__global__ void __launch_bounds__(GROW_THREADS, 1) pages_plan_kernel(const __grid_constant__ CompactArgs c) {
+  extern __shared__ uint32_t smem[];
+  __shared__ uint32_t sums[GROW_THREADS / 32];
+  pdl_launch_dependents();
+  pdl_wait();
+  plan_moves(c, smem, sums);
+}
+__global__ void __launch_bounds__(ROW_THREADS) pages_follow_kernel(const __grid_constant__ CompactArgs c) {
+  __shared__ uint32_t last_s;
+  pdl_launch_dependents();
+  pdl_wait();
+  for (uint32_t r = blockIdx.x * (ROW_THREADS / 32) + (threadIdx.x >> 5); r < c.t.n_rows; r += gridDim.x * (ROW_THREADS / 32)) follow_moves(c, r, threadIdx.x & 31);
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) last_s = atomicAdd(c.counter, 1) == gridDim.x - 1;
@@ -448,8 +488,7 @@ __global__ void __launch_bounds__(ROW_THREADS) pages_follow_kernel(const __grid_
   if (!last_s) return;
   __threadfence();
   if (threadIdx.x == 0) *c.counter = 0;
-  for (uint32_t i = threadIdx.x; i < c.most; i += ROW_THREADS)
-    if (c.src[i] >= 0) t.refs[c.src[i]] = 0;
+  free_moved(c);
 }
 
 // ---- copy ------------------------------------------------------------------------------------------------------------
@@ -487,6 +526,25 @@ __global__ void __launch_bounds__(COPY_THREADS) pages_copy_kernel(const __grid_c
     if (w0 + k * COPY_THREADS < words) y[w0 + k * COPY_THREADS] = v[k];
 }
 
+// One cluster of `ctas` CTAs of GROW_THREADS threads.
+template <typename Args>
+cudaError_t launch_cluster(void (*kernel)(Args), uint32_t ctas, uint32_t smem, cudaStream_t s, const Args& args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(GROW_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args);
+}
+
 const char* check_tables(const bp_paged_ctx* c, const bp_page_tables* in, Tables* t) {
   if (in->page_tokens != 16 && in->page_tokens != 32 && in->page_tokens != 64) return "page_tokens must be 16, 32 or 64";
   if (in->n_rows == 0 || in->n_rows > MAX_ROWS) return "page tables have 1 .. 16384 rows";
@@ -502,7 +560,7 @@ const char* check_tables(const bp_paged_ctx* c, const bp_page_tables* in, Tables
 }  // namespace
 
 cudaError_t bp_pages_init(bp_paged_ctx* c) {
-  cudaError_t e = cudaFuncSetAttribute(pages_grow_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (GROW_THREADS * WORDS + 2 * (MAX_ROWS + 1) + MAX_ROWS / 32) * 4);
+  cudaError_t e = cudaFuncSetAttribute(pages_grow_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (GROW_THREADS * WORDS + 2 * (MAX_ROWS + 1)) * 4);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(pages_fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (ROW_THREADS * WORDS + 2 * MAX_ROWS) * 4);
   if (e == cudaSuccess) e = cudaMalloc(&c->page_counter, sizeof(uint32_t));
   if (e == cudaSuccess) e = cudaMemset(c->page_counter, 0, sizeof(uint32_t));
@@ -527,11 +585,8 @@ int bp_pages_grow(bp_paged_ctx* c, void* stream, const bp_page_tables* tables, c
   g.n_out = n_out;
   OnDevice on(c->device);
   BP_TRY(c, on.err);
-  const size_t smem = (GROW_THREADS * WORDS + 2 * (g.t.n_rows + 1) + (g.t.n_rows + 31) / 32) * 4;
-  // A second launch costs some 2 us, a thousand tokens in one CTA 0.6.
-  g.later = n_out > 4096;
-  BP_TRY(c, bp_launch(true, pages_grow_kernel, dim3(1), dim3(GROW_THREADS), smem, static_cast<cudaStream_t>(stream), g));
-  if (g.later) BP_TRY(c, bp_launch(true, pages_place_kernel, dim3((n_out + PLACE_THREADS - 1) / PLACE_THREADS), dim3(PLACE_THREADS), 0, static_cast<cudaStream_t>(stream), g));
+  const uint32_t smem = (GROW_THREADS * WORDS + 2 * (g.t.n_rows + 1)) * 4;
+  BP_TRY(c, launch_cluster(pages_grow_kernel, n_out > 2 * GROW_THREADS ? 8 : 1, smem, static_cast<cudaStream_t>(stream), g));
   return BP_OK;
 }
 
@@ -586,8 +641,13 @@ int bp_pages_compact(bp_paged_ctx* c, void* stream, const bp_page_tables* tables
   a.counter = c->page_counter;
   OnDevice on(c->device);
   BP_TRY(c, on.err);
-  BP_TRY(c, bp_launch(true, pages_plan_kernel, dim3(1), dim3(GROW_THREADS), GROW_THREADS * WORDS * 4, static_cast<cudaStream_t>(stream), a));
-  const uint32_t ctas = a.t.n_rows < 4u * c->sm_count ? a.t.n_rows : 4u * c->sm_count;
+  const uint32_t smem = GROW_THREADS * WORDS * 4;
+  if (static_cast<uint64_t>(a.t.n_rows) * a.t.row_pages <= COMPACT_ENTRIES) {
+    BP_TRY(c, launch_cluster(pages_compact_kernel, 8, smem, static_cast<cudaStream_t>(stream), a));
+    return BP_OK;
+  }
+  BP_TRY(c, bp_launch(true, pages_plan_kernel, dim3(1), dim3(GROW_THREADS), smem, static_cast<cudaStream_t>(stream), a));
+  const uint32_t rows = (a.t.n_rows + ROW_THREADS / 32 - 1) / (ROW_THREADS / 32), ctas = rows < 4u * c->sm_count ? rows : 4u * c->sm_count;
   BP_TRY(c, bp_launch(true, pages_follow_kernel, dim3(ctas), dim3(ROW_THREADS), 0, static_cast<cudaStream_t>(stream), a));
   return BP_OK;
 }

@@ -131,6 +131,17 @@ def test_many_rows_and_pages(ctx):
     ctx.status()
 
 
+@pytest.mark.parametrize("most", [30, 5000])
+def test_compaction_of_large_tables(ctx, most):
+    """More entries than one cluster takes care of."""
+    rows, width, n_pages, page = 300, 1000, 20_000, 16
+    rng = np.random.default_rng(most)
+    b = Both(9, rows, width, n_pages, page, [int(x) for x in rng.integers(0, 900, rows)])
+    b.compact(ctx, most)
+    b.compact(ctx, most)
+    ctx.status()
+
+
 def test_rows_that_are_refused_stay_as_they_were(ctx):
     """No room in the row, no pages in the pool, no places in the output, a negative number: the others grow."""
     page = 16
