@@ -136,6 +136,25 @@ __device__ __forceinline__ void ask(Raw<D>& w, const AttnArgs& a, uint32_t id, i
     w.vd[0] = *reinterpret_cast<const uint32_t*>(v + scales), w.vm[0] = *reinterpret_cast<const uint32_t*>(v + scales + gap);
   }
 }
+// What a thread of the expanders has asked for: the codes of the tile that `key` lies in, the next two page ids.
+template <int D>
+struct Ahead {
+  Raw<D> raw;
+  int key;
+  uint32_t id, id_next;
+  bool there;
+  // Page ids are asked for two tiles ahead and looked at one tile ahead, when the codes are asked for: nothing here waits for memory.
+  // A token that holds no key of the request (or lies in a page outside the pool) gets page 0's codes, and zeros for its scales.
+  static __device__ __forceinline__ bool has_key(const Keys& keys, int key) { return key >= keys.low && key < keys.high; }
+  static __device__ __forceinline__ uint32_t ask_id(const AttnArgs& a, const Keys& keys, const int32_t* table, int key) {
+    return has_key(keys, key) ? static_cast<uint32_t>(table[key >> a.pool.log_page]) : 0u;
+  }
+  __device__ __forceinline__ void ask_codes(const AttnArgs& a, const Keys& keys, uint32_t head, uint32_t quarter) {
+    there = has_key(keys, key) && id < a.pool.n_pages;
+    if (has_key(keys, key) && !there) note_range(a.err);
+    ask<D>(raw, a, there ? id : 0u, key, head, quarter);
+  }
+};
 // Eight codes at bits 4 i of both halves -> four words of two f16 values m + d q.
 __device__ __forceinline__ uint4 expand8(uint32_t w, __half2 d, __half2 m, uint32_t bias) {
   const __half2 off = __float2half2_rn(-1024.f), off16 = __float2half2_rn(-64.f), sixteenth = __float2half2_rn(0.0625f);
@@ -195,6 +214,8 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   __shared__ __align__(16) uint8_t bad[MIXED][BN];
   __shared__ float row_scale[S::ROWS];  // the softmax scale in log2 units over the power of two of a row's queries
   __shared__ uint32_t line[THREADS + 1];
+  __shared__ Request requests[THREADS];  // all of them if there are no more than threads
+  __shared__ float* records[S::ROWS];    // PARTS: where the rows go
   __shared__ Cursor cur;
   __shared__ Join join_s;
   __shared__ uint32_t tmem_base_s;
@@ -251,7 +272,11 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   };
   {
     uint32_t units = 0;
-    for (uint32_t r = threadIdx.x * per; r < min((threadIdx.x + 1) * per, a.n_req); r++) units += tiles_of(request<MODE>(a, r, blockIdx.x == 0));
+    for (uint32_t r = threadIdx.x * per; r < min((threadIdx.x + 1) * per, a.n_req); r++) {
+      const Request q = request<MODE>(a, r, blockIdx.x == 0);
+      if (per == 1) requests[r] = q;
+      units += tiles_of(q);
+    }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t x = __shfl_up_sync(FULL, units, o);
@@ -268,13 +293,20 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
   }
   const uint32_t total = line[THREADS], share = (total + gridDim.x - 1) / gridDim.x;
   const uint32_t c0 = min(static_cast<uint64_t>(blockIdx.x) * share, static_cast<uint64_t>(total)), c1 = c0 + min(share, total - c0);
+  auto request_of = [&](uint32_t r) { return per == 1 ? requests[r] : request<MODE>(a, r, false); };
+  uint32_t at = 0;  // (warp 0)
+  if (warp == 0 && c0 < c1) {
+    for (uint32_t i = 0; i < THREADS; i += 32) {
+      const uint32_t n = __popc(__ballot_sync(FULL, line[i + lane + 1] <= c0));
+      at += n;
+      if (n < 32) break;
+    }
+  }
   if (threadIdx.x == 0 && c0 < c1) {
-    uint32_t at = 0;
-    while (line[at + 1] <= c0) at++;
     uint32_t left = c0 - line[at];
     bool found = false;
     for (uint32_t r = at * per; r < a.n_req && !found; r++) {
-      const Request q = request<MODE>(a, r, false);
+      const Request q = request_of(r);
       for (uint32_t x = 0; x * S::ROWS < q.rows; x++) {
         const Keys k = keys_of<MODE>(a, q, x * S::ROWS, S::ROWS);
         const uint32_t places = k.tiles + ITEM_COST<MODE>, n = places * a.pool.n_kv_head;
@@ -303,6 +335,17 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     // the piece's tiles [plain0, plain0 + plain_n) are seen whole by every row
     const uint32_t plain0 = static_cast<uint32_t>(max(keys.all_from - key_first + static_cast<int>(BN) - 1, 0)) / BN;
     const uint32_t plain_n = static_cast<uint32_t>(max((keys.all_to - key_first) / static_cast<int>(BN) - static_cast<int>(plain0), 0));
+    // the expanders' first codes are on their way while the queries come (where there are registers for both)
+    Ahead<D> ahead;
+    const bool expands = warp >= S::FIRST_EXPANDER && warp < S::FIRST_SOFTMAX;
+    auto ask_first = [&]() {
+      const int32_t* table = pages_of<MODE>(a, cur.r, head);
+      ahead.key = key_first + static_cast<int>(8 * (warp - S::FIRST_EXPANDER) + (lane & 7));
+      ahead.id = ahead.ask_id(a, keys, table, ahead.key);
+      ahead.id_next = n > 1 ? ahead.ask_id(a, keys, table, ahead.key + static_cast<int>(BN)) : 0u;
+      ahead.ask_codes(a, keys, head, lane >> 3);
+    };
+    if (NQ == 1 && expands) ask_first();
     // ---- queries -> f16, each row times its power of two ----
     {
       constexpr uint32_t U = D / 8, ITERS = (S::ROWS * U + THREADS - 1) / THREADS;
@@ -389,24 +432,12 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       // ---------------- codes -> operand tiles ----------------
       const uint32_t quarter = lane >> 3, row = 8 * (warp - S::FIRST_EXPANDER) + (lane & 7);  // a warp: all of eight tokens, eight rows per 16-byte phase
       const int32_t* table = pages_of<MODE>(a, cur.r, head);
-      // Page ids are asked for two tiles ahead and looked at one tile ahead, when the codes are asked for: nothing here waits for memory.
-      // A token that holds no key of the request (or lies in a page outside the pool) gets page 0's codes, and zeros for its scales.
-      auto has_key = [&](int key) { return key >= keys.low && key < keys.high; };
-      auto ask_id = [&](int key) { return has_key(key) ? static_cast<uint32_t>(table[key >> a.pool.log_page]) : 0u; };
-      Raw<D> raw;
-      int key = key_first + static_cast<int>(row);
-      uint32_t id = ask_id(key), id_next = n > 1 ? ask_id(key + static_cast<int>(BN)) : 0u;
-      bool there;
-      auto ask_codes = [&]() {  // of the tile that `key` lies in
-        there = has_key(key) && id < a.pool.n_pages;
-        if (has_key(key) && !there) note_range(a.err);
-        ask<D>(raw, a, there ? id : 0u, key, head, quarter);
-      };
-      ask_codes();
+      if (NQ != 1) ask_first();
       for (uint32_t i = 0; i < n; i++) {
         const uint32_t c = done + i, s = c % SLOTS;
         const bool mixed = i - plain0 >= plain_n;
-        Raw<D> mine = raw;
+        Raw<D> mine = ahead.raw;
+        const bool there = ahead.there;
         if (!there || mixed) {
           uint32_t found = 0;
 #pragma unroll
@@ -419,10 +450,10 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
           }
           if (mixed && quarter == 0) bad[i < plain0 ? i : i - plain_n][row] = there ? static_cast<uint8_t>(found) : 0;
         }
-        key += BN;
-        id = id_next;
-        if (i + 1 < n) ask_codes();
-        if (i + 2 < n) id_next = ask_id(key + static_cast<int>(BN));
+        ahead.key += BN;
+        ahead.id = ahead.id_next;
+        if (i + 1 < n) ahead.ask_codes(a, keys, head, quarter);
+        if (i + 2 < n) ahead.id_next = ahead.ask_id(a, keys, table, ahead.key + static_cast<int>(BN));
         if (c >= SLOTS && !__all_sync(FULL, waitx(&k_empty[s], (c / SLOTS - 1) & 1))) break;
         put<D, false>(mine, smem + S::OFF_K + s * S::KV_B, row, quarter, a.bias);
         fence_proxy_async();
@@ -541,6 +572,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         constexpr uint32_t U = D / 8;
         uint8_t* stage = smem + x * S::Q_B;
         const uint32_t rows = min(BM, q.rows - min(tile_row, q.rows));
+        records[x * BM + r] = to;
 #pragma unroll 1
         for (uint32_t half = 0; half < 2; half++) {
           if (half) named_bar_sync(1 + x, 128);  // (what was staged before has gone)
@@ -563,8 +595,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
 #pragma unroll 4
             for (uint32_t k = r; k < rows * U; k += 128) {
               const uint32_t row_in = k / U, u = k % U;
-              float* row_to = all ? record_of<D>(a, !q.causal, q.q0, head, tile_row + row_in) : scratch + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PIECE + (x * BM + row_in) * RECORD<D>;
-              *reinterpret_cast<float4*>(row_to + D / 2 * half + 4 * u) = *reinterpret_cast<const float4*>(stage + row_in * (2 * D) + ((u ^ (row_in & (U - 1))) << 4));
+              *reinterpret_cast<float4*>(records[x * BM + row_in] + D / 2 * half + 4 * u) = *reinterpret_cast<const float4*>(stage + row_in * (2 * D) + ((u ^ (row_in & (U - 1))) << 4));
             }
           }
         }
@@ -643,7 +674,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
           c.head = 0;
           if (++c.x * S::ROWS >= c.q.rows) {
             c.x = 0;
-            do c.q = request<MODE>(a, ++c.r, false);  // (there is a further item in the line)
+            do c.q = request_of(++c.r);  // (there is a further item in the line)
             while (c.q.rows == 0);
           }
           c.keys = keys_of<MODE>(a, c.q, c.x * S::ROWS, S::ROWS);

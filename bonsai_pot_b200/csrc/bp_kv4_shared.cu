@@ -137,10 +137,10 @@ int bp_kv4_attention_shared(bp_paged_ctx* c, void* stream, uint32_t dtype, const
     j.piece[1] = j.piece[0];
     j.ctas[0] = j.ctas[1] = c->sm_count;
   } else {
-    // Side by side, each on its share of the SMs: what a tile of 64 keys takes there (1.2 us of 256 rows, 0.9 of 128) against 0.18 us for a unit of 64 keys here,
-    // by the lengths that the caller says, and each its beginning and end.
+    // Side by side, each on its share of the SMs: what a tile of 64 keys takes there (1.2 us of 256 rows, 0.9 of 128) against 0.15 us for a unit of 64 keys of 128 dims here
+    // (0.18, but requests are shorter than the longest), by the lengths that the caller says.
     const float prefix_tiles = static_cast<float>(in->n_prefix) * p.n_kv_head * ((prefix_rows + 255) / 256) * (in->max_prefix / 64 + 6);
-    const float prefix_cost = prefix_tiles * (prefix_rows > 128 ? 1.2f : 0.9f), own_cost = static_cast<float>(in->n_req) * p.n_kv_head * (in->max_kv / 64 + 1) * 0.18f;
+    const float prefix_cost = prefix_tiles * (prefix_rows > 128 ? 1.2f : 0.9f), own_cost = static_cast<float>(in->n_req) * p.n_kv_head * (in->max_kv / 64 + 1) * (0.15f / 128) * D;
     const float part = prefix_cost / (prefix_cost + own_cost);
     const int sms = c->sm_count, most = sms - sms / 8;
     int here = static_cast<int>(part * sms + 0.5f);
