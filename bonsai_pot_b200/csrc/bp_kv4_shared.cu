@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, N > 4 ? 3 : 6) kv4_join_kernel(c
   const uint4 ends[2] = {*reinterpret_cast<const uint4*>(record[0] + D), *reinterpret_cast<const uint4*>(record[1] + D)};
   const int r = last_begun(a.q_start, a.n_own + 1, static_cast<int>(token), lane);
   if (r < 0 || r >= static_cast<int>(a.n_own)) return;  // a row of no request
-  const int g = last_begun(a.prefix_start, a.n_prefix + 1, r, lane);
+  const int g = a.n_prefix ? last_begun(a.prefix_start, a.n_prefix + 1, r, lane) : -1;  // (without prefixes there may be no list of them)
   const Lengths own = lengths_of<PARTS>(a, a.n_prefix + r, false);
   if (static_cast<int>(token) >= own.q0 + own.q_len) return;  // (cut, and reported)
   const bool some = g >= 0 && g < static_cast<int>(a.n_prefix);

@@ -342,6 +342,27 @@ def test_other_streams_and_graphs(ctx):
     ctx.status()
 
 
+def test_two_contexts_at_once(ctx):
+    """Choice (in clusters) and attention on two streams at once."""
+    s = Chosen(14, "f16", [1, 1], [3000, 2500], 4, 2, 64, 16, 20)
+    s.select(ctx)
+    s.check_choice()
+    want = [s.pages.clone(), s.keys_n.clone(), s.attend(ctx)]
+    other, streams = bp.PagedContext(), [torch.cuda.Stream() for _ in range(2)]
+    got = [[(torch.zeros_like(want[0]), torch.zeros_like(want[1]), torch.zeros_like(want[2])) for _ in range(20)] for _ in streams]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for c, stream, g in zip((ctx, other), streams, got):
+            with torch.cuda.stream(stream):
+                s.pages, s.keys_n = g[i][:2]
+                s.select(c)
+                s.attend(c, g[i][2])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for x in g for a, b in zip(x, want))
+    other.status()
+    other.close()
+
+
 def test_refusals(ctx):
     s = Chosen(12, "f16", [1, 1], [300, 200], 4, 2, 64, 16, 4)
     lib, at = bp.paged._lib, torch.zeros(64, device="cuda").data_ptr()

@@ -233,15 +233,76 @@ def test_no_prefix_and_no_keys(ctx):
     ctx.status()
 
 
-@pytest.mark.parametrize("q", [1, 30])
-def test_other_streams_and_graphs(ctx, q):
+@pytest.mark.parametrize("n_req", [40, 90])
+def test_a_call_sees_what_was_written_just_before(ctx, n_req):
+    """Appended keys (of the prefix and the requests' own), then attention whose two launches begin early, again and again without waiting: as with a wait in between."""
+    s = Shared(17, "bf16", [1] * n_req, [33] * n_req, [0, n_req], [700], 8, 2, 128, 16)
+    rows = list(range(n_req)) + [s.n]
+    at = [32] * n_req + [699]
+    slots = torch.tensor([int(s.table[r, k // 16]) * 16 + k % 16 for r, k in zip(rows, at)], device="cuda")
+    new = [normal(i, (n_req + 1, 2, 128), "bf16", 3.0) for i in range(40)]
+    work = torch.empty(ctx.shared_work(n_req, 8, 128), device="cuda")
+
+    def go(wait):
+        outs = [torch.empty_like(s.q) for _ in new]
+        for k, out in zip(new, outs):
+            ctx.append(s.pool, k, k.flip(0), None, slots)
+            if wait:
+                torch.cuda.synchronize()
+            s.run(ctx, out, work=work)
+            if wait:
+                torch.cuda.synchronize()
+        return torch.stack(outs)
+
+    assert torch.equal(go(False), go(True))
+    ctx.status()
+
+
+def test_two_contexts_at_once(ctx):
+    """Two streams, a context and a work memory each, the same pool: neither changes the other's results."""
+    s = Shared(18, "f16", [1] * 50, [60] * 50, [0, 50], [900], 8, 2, 64, 32)
+    want = s.run(ctx)
+    other, streams = bp.PagedContext(), [torch.cuda.Stream() for _ in range(2)]
+    outs = [[torch.zeros_like(s.q) for _ in range(20)] for _ in streams]
+    works = [torch.empty(ctx.shared_work(50, 8, 64), device="cuda") for _ in streams]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for c, stream, out, work in zip((ctx, other), streams, outs, works):
+            with torch.cuda.stream(stream):
+                s.run(c, out[i], work=work)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for out in outs for o in out)
+    other.status()
+    other.close()
+
+
+@pytest.mark.parametrize("how", ["dense", "odd", "heads"])
+def test_two_launches_over_strided_rows_and_over_the_queries(ctx, how):
+    """Many rows behind a prefix, few of each request; rows before the first request and behind the last one stay."""
+    s = Shared(19, "f16", [2] * 30, [20 + 5 * i for i in range(30)], [3, 30], [333], 8, 2, 128, 32, how=how)
+    rows = torch.cat([torch.full((2, 8, 128), 5.0, dtype=s.q.dtype, device="cuda"), s.q, torch.full((3, 8, 128), 6.0, dtype=s.q.dtype, device="cuda")])
+    keep = s.q
+    s.args[0] = s.args[0] + 2
+    s.q = strided(rows, how)
+    for out in (strided(torch.full_like(rows, 7.0), how), s.q):
+        before = out.clone()
+        s.run(ctx, out)
+        assert torch.equal(out[:2], before[:2]) and torch.equal(out[-3:], before[-3:])
+        mine, s.q = s.q, keep
+        s.check(out[2:-3])
+        s.q = mine
+    ctx.status()
+
+
+@pytest.mark.parametrize("q,n", [(1, 5), (30, 5), (1, 45)])
+def test_other_streams_and_graphs(ctx, q, n):
     """Captured twice with one work memory, replayed one behind the other: either follows the lengths on the device."""
-    s = Shared(13, "bf16", [q] * 5, [100, 60, 80, 50, 40], [1, 5], [400], 8, 2, 128, 32)
+    s = Shared(13, "bf16", [q] * n, [40 + 12 * (i % 5) for i in range(n)], [1, n], [400], 8, 2, 128, 32)
     want = s.run(ctx)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     outs = [torch.zeros_like(s.q) for _ in range(2)]
-    work = torch.empty(ctx.shared_work(5 * q, 8, 128), device="cuda")
+    work = torch.empty(ctx.shared_work(n * q, 8, 128), device="cuda")
     s.run(ctx, outs[0], work=work, stream=side)
     side.synchronize()
     assert torch.equal(outs[0], want)
@@ -284,6 +345,11 @@ def test_refusals(ctx):
 
     for name in (*ok, "work"):
         assert entry(**{name: None}) == 7 and entry(**{name: (ok.get(name) or work.data_ptr()) + 2}) == 1, name
+    # without prefixes there need be no tables of them, without own keys none of these
+    none = dict(prefix_start=None, prefix_len=None, prefix_table=None, n_prefix=0)
+    assert entry(**none) == 0 and entry(**none, max_prefix=0) == 0 and entry(page_table=None, max_kv=0) == 0
+    with pytest.raises(bp.ContextOverflow):  # (which is reported: the requests say that they have some)
+        ctx.status()
     assert entry(dtype=2) == 1 and entry(n_head=3) == 1 and entry(n_req=65536) == 1 and entry(n_prefix=65536) == 1 and entry(max_kv=1 << 31) == 1 and entry(max_prefix=1 << 31) == 1
     assert entry(total_q=1 << 30) == 1
     ctx.status()
