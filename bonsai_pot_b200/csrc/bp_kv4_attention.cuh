@@ -175,7 +175,7 @@ struct RowJoin {
   float m = NEG_BIG, l = 0.f, o[V] = {};
   // The pieces of the lanes in `mask`, in their order: `at` is the row in the lane's piece. N of them are on their way together, the first before
   // anything is known of their weights.
-  template <int N = 8>
+  template <int N>
   __device__ __forceinline__ void add(uint32_t mask, const float* at, uint32_t lane) {
     const float2 ml = mask >> lane & 1 ? *reinterpret_cast<const float2*>(at + D) : make_float2(NEG_BIG, 0.f);
     float e[N][V];
