@@ -24,11 +24,15 @@
 // Bound by HBM in principle (1.25 head_dim bytes per key and KV head: 31.6 us for a batch of 64 requests of up to 8191 keys, 32 / 8 heads of 128, 207 MB),
 // in practice by the instructions that expand the codes (about 270 per 16 tokens and warp are the formulation's, 330 were counted; the counters have 53 % of the
 // issue slots used, 19 % of the tensor pipe) and by what lies
-// around the stream: measured 57 us for that batch, of which 40 stream at 5.1 TB/s, 4.5 pass before a warp has its first keys and its queries, and 8
+// around the stream: measured 58 us for that batch, of which 40 stream at 5.1 TB/s, 4.5 pass before a warp has its first keys and its queries, and 8
 // at the end (the warps of a CTA end 1 to 3 us apart, joining a CTA's pieces takes 3, meeting the other CTAs 2, joining theirs 1 to 3). One request of 32768 keys:
-// 22.5 us (floor 6.4), 11 of them streaming. Why so: with one warp per item and no split these took 772 and 3064 us; with two CTAs of eight warps and two
+// 22.9 us (floor 6.4), 11 of them streaming. Why so: with one warp per item and no split these took 772 and 3064 us; with two CTAs of eight warps and two
 // buffers per warp 70 and 28; with joins by all threads of a CTA behind barriers, one item after the other, 86 and 31. 16 requests of up to 5 drafted tokens,
-// 5 query heads of 64 per KV head, behind up to 4096 keys of which a window shows 1024: 19.1 us (floor 1.2).
+// 5 query heads of 64 per KV head, behind up to 4096 keys of which a window shows 1024: 19.4 us (floor 1.2).
+//
+// CHOSEN (bp_kv4_select.cu): an item is a token and KV head over a list of pages of its own; lists are about equally long, so a CTA takes whole items and nobody meets: 32 tokens of 32 pages of
+// 64 keys 26 us (floor 13; 11 streaming at 5.5 units per us and SM, which is the instructions' rate, 3.3 to the first keys, 4 to join a CTA's pieces, with 128 of 148 CTAs), one token of 64
+// pages of 32 12 us, most of it the first pass through the code. PARTS (bp_kv4_shared.cu): rows become 32-bit records; 8 tokens behind 2048 keys 10 us.
 #include <math.h>
 
 #include <type_traits>
@@ -982,7 +986,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
     float* to = all ? nullptr : exchange + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == first_cta)) * S::PARTIAL;
     // The warps take the rows of all items in turn. Requests of any lengths leave many items of few pieces each: four rows at a time, one piece after the other. Chosen
     // pages, and the launches in parts, leave few items of up to twelve pieces: a row at a time, its pieces at once (32 tokens of 32 pages of 64 28.0 -> 26.3 us; 64 requests of up
-    // to 8191 keys would take 61.5 instead of 57.5).
+    // to 8191 keys would take 61.5 instead of 57.9).
     if constexpr (MODE == PLAIN) {
       for (uint32_t row = 0; row < p.rows; row += 4) {
         if (turn == warp)

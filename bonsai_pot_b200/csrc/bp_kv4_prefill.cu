@@ -11,7 +11,8 @@
 //                           rescaled in TMEM only when a row's maximum grew by more than 2^5 (P stays below 2^15 meanwhile)
 //   O issuer X (1 thread)   O_X += P_X V (P from TMEM as the A operand, V as the MN-major B operand)
 // The key tiles of all items lie in one line, of which every CTA takes an equal stretch; an item that lies in several CTAs is joined by the
-// one that comes last, in the order of its keys (as in bp_kv4_attention.cu). Every wait is bounded; a timeout sets the context's error word and
+// one that comes last, in the order of its keys (as in bp_kv4_attention.cu). In PARTS (prefixes that several requests have in common, and keys behind them) nobody joins: rows and
+// pieces of rows go to memory as 32-bit records, through the dead Q tile, and bp_kv4_shared.cu joins them. Every wait is bounded; a timeout sets the context's error word and
 // the CTA winds down and frees its TMEM.
 //
 // P is f16 because V is (see bp_kv4_attention.cu).
@@ -21,7 +22,11 @@
 // would take about 1450 at the measured rate of a library product. 2048 queries behind 32768 keys, 32 / 8 heads of 128: 1.21 ms, 881 TFLOP/s, 54 % of that rate
 // (floor 0.65 ms). Four expander warps whose page ids were waited for took 1.39 ms; eight of them, with two softmax threads per row, 1.38; with one softmax
 // thread per row 1.25; with whole lines read and one barrier per slot 1.23. 4 requests of up to 512 queries behind up to 4099 keys: 97 us (floor 32): a tile costs the
-// same, beginning and ending an item about 14 us; before the line weighted items and the partial results had whole-warp accesses it was 216.
+// same, beginning and ending an item about 14 us; before the line weighted items and the partial results had whole-warp accesses it was 216. 4 chunks of up to 512 queries with
+// 16384 keys in common and up to 1030 of their own, both parts in one launch: 425 us, 850 TFLOP/s. One query tile of 128 rows (64 tokens behind 8191 keys in common, 90 CTAs): 33 us, 1.0 to 1.15
+// per key tile (2000 cycles: an expander warp takes 1900 for it, nearly all of them one instruction waiting for another, the softmax 1300), 1.3 before the first item is
+// found, 1.8 for the queries, 2 from there to the first scores, 2.4 to write the rows. (Tried: two key tiles per turn of the expanders, 280 bytes of registers spilled: 45 us; K and V of a tile
+// behind one fence: the same; every 2nd or 4th pair of exponentials by a polynomial on the FMA units: chunks 536 and 487 us instead of 450.)
 #include <type_traits>
 
 #include "bp_kv4_attention.cuh"
@@ -36,9 +41,10 @@ constexpr uint32_t SLOTS = 4;          // K and V tiles in shared memory
 // Tiles of which some rows of an item see only a part: its rows are 256 tokens at most, so these are 5 tiles at each end of the keys that they see; where a
 // window is so short that no tile lies between the two ends, the two overlap or are less than two tiles apart: 11 tiles.
 constexpr uint32_t MIXED = 11;
-// What beginning and ending an item costs, in key tiles.
+// What beginning and ending an item costs, in key tiles. (In parts its rows are 32-bit records. 4 chunks of 512 behind 16384 keys: with 6, 633 us, as the CTAs with
+// the chunks' own keys, a dozen tiles per item, came last; 10: 444, 14: 451, 18: 455.)
 template <int MODE>
-constexpr uint32_t ITEM_COST = MODE == PARTS ? 14 : 6;
+constexpr uint32_t ITEM_COST = MODE == PARTS ? 10 : 6;
 constexpr float GROW = 5.f;            // log2 by which a maximum may grow before O is rescaled; P_UP + GROW stays below 16
 
 template <int D, uint32_t NQ>

@@ -5,6 +5,10 @@
 // are those of all their requests, so that their codes are read and expanded once for all of them; own keys are items of each request. Both are the attention
 // kernels' (bp_kv4_attention.cu, bp_kv4_prefill.cu), which leave (o, m, l) of whole items in the caller's work memory and of pieces of items in the context's, in 32 bits;
 // the kernel here joins them all, in the order of the keys.
+//
+// Floors: prefix and own keys once, 6.2 us for 64 tokens behind two prefixes of up to 8191 keys (32 / 8 heads of 128, up to 1000 keys of their own), the products, 220 us for 4 chunks of up to 512
+// behind 16384. Measured 41 and 444 us, 16 for 8 tokens behind 2048 keys (bp_kv4_attention for the 64 tokens over the same keys in rows of their own: as many keys as 64 requests have together, some 110).
+// Bound by the attention kernels' beginnings and ends and, of chunks, by their softmax. One launch after the other, each joining its items by the CTA that comes last, took 92, 513 and 31.
 #include "bp_kv4_attention.cuh"
 #include "bp_paged_host.cuh"
 

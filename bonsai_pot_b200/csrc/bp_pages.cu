@@ -6,6 +6,8 @@
 // who comes when; integer counts do not depend on the order of their atomics.
 // Where the result is then spread out over many tokens or rows, the CTA has seven others beside it in a cluster, which wait for it at the cluster's barrier: one
 // launch (2.8 us on the host) less.
+// us on the device: 3 rows end and 64 grow 9 (a call's issue from Python takes 4 to 6), 16 rows of up to 30000 tokens end and get up to 2047 again in a pool of 17000 pages, all but 30 of which
+// they need, 13; 4 forks 7, compaction of 300 pages 7. Copied pages go at the rate of memory: 94 MB 18.4 (what is written stays in L2 at first), 708 MB 212, 6.7 TB/s read and written.
 #include "bp_paged_host.cuh"
 
 namespace {
