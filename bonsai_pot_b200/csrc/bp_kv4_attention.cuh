@@ -15,6 +15,7 @@ enum Mode {
   PLAIN,   // requests, their outputs are written
   PARTS,   // prefixes that several requests have in common (their rows are those of all these requests, each sees every key), then requests behind
            // their prefixes: either sees a part of a row's keys only, and what comes out are partial results
+  BEHIND,  // requests whose keys are their prefix's and then their own: two rows of pages; their outputs are written
   CHOSEN,  // tokens that see every key of pages chosen for each KV head; their outputs are written
 };
 // A partial result of a row: [0, D) the values' sum, [D] the largest score (log2 units), [D + 1] the sum of the weights, then as whole numbers [D + 2] c and
@@ -38,7 +39,7 @@ struct AttnArgs {
   uint32_t bias;  // 0x64006400: two f16 numbers 1024
   uint32_t bf;    // activations are bfloat16
   uint32_t q_vec; // rows of q are 16-byte aligned
-  // PARTS: requests [0, n_prefix) are prefixes, prefix g that of the requests [prefix_start[g], prefix_start[g + 1]) of n_req - n_prefix
+  // prefix g is that of the requests [prefix_start[g], prefix_start[g + 1]) of n_own. PARTS: in the line, requests [0, n_prefix) are the prefixes
   const int32_t *prefix_start, *prefix_len, *prefix_table;
   uint32_t n_prefix, n_own, max_prefix, prefix_stride, prefix_pages;
   float* part;  // [prefix, own][rows of q][n_head] records

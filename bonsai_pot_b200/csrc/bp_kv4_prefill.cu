@@ -23,7 +23,7 @@
 // (floor 0.65 ms). Four expander warps whose page ids were waited for took 1.39 ms; eight of them, with two softmax threads per row, 1.38; with one softmax
 // thread per row 1.25; with whole lines read and one barrier per slot 1.23. 4 requests of up to 512 queries behind up to 4099 keys: 97 us (floor 32): a tile costs the
 // same, beginning and ending an item about 14 us; before the line weighted items and the partial results had whole-warp accesses it was 216. 4 chunks of up to 512 queries with
-// 16384 keys in common and up to 1030 of their own, both parts in one launch: 425 us, 850 TFLOP/s. One query tile of 128 rows (64 tokens behind 8191 keys in common, 90 CTAs): 33 us, 1.0 to 1.15
+// 16384 keys in common and up to 1030 of their own: 412 us, 880 TFLOP/s (BEHIND; both parts in one launch 425, and 20 to join them). One query tile of 128 rows (64 tokens behind 8191 keys in common, 90 CTAs): 33 us, 1.0 to 1.15
 // per key tile (2000 cycles: an expander warp takes 1900 for it, nearly all of them one instruction waiting for another, the softmax 1300), 1.3 before the first item is
 // found, 1.8 for the queries, 2 from there to the first scores, 2.4 to write the rows. (Tried: two key tiles per turn of the expanders, 280 bytes of registers spilled: 45 us; K and V of a tile
 // behind one fence: the same; every 2nd or 4th pair of exponentials by a polynomial on the FMA units: chunks 536 and 487 us instead of 450.)
@@ -62,6 +62,8 @@ struct Shape {
 struct Request {
   int q0, q_len, kv_len;
   uint32_t rows, causal;
+  int before;       // BEHIND: keys of its prefix, which come before its own kv_len
+  uint32_t prefix;
 };
 template <int MODE>
 __device__ __forceinline__ Request request(const AttnArgs& a, uint32_t r, bool report) {
@@ -72,6 +74,20 @@ __device__ __forceinline__ Request request(const AttnArgs& a, uint32_t r, bool r
   q.kv_len = n.kv_len;
   q.rows = static_cast<uint32_t>(q.q_len) * a.group;
   q.causal = is_causal<MODE>(a, r);
+  q.before = 0;
+  q.prefix = 0;
+  if (MODE == BEHIND && a.n_prefix) {
+    uint32_t lo = 0, hi = a.n_prefix + 1;  // the last one that has begun is lo, if any has
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) >> 1;
+      if (a.prefix_start[mid] <= static_cast<int>(r)) lo = mid;
+      else hi = mid;
+    }
+    if (lo < a.n_prefix && a.prefix_start[lo] <= static_cast<int>(r)) {
+      q.prefix = lo;
+      q.before = min(max(a.prefix_len[lo], 0), static_cast<int>(min(a.max_prefix, a.prefix_pages << a.pool.log_page)));
+    }
+  }
   return q;
 }
 // Keys [low, high) that the rows [row0, row0 + rows) of a request see, of all of them together; key tiles from low's on, one at least (its
@@ -96,6 +112,11 @@ __device__ __forceinline__ Keys keys_of(const AttnArgs& a, const Request& q, uin
   k.low = first_seen(past + t0 + 1, a.window);
   k.all_from = first_seen(past + t1 + 1, a.window);
   k.all_to = past + t0 + 1;
+  if (MODE == BEHIND) {
+    k.low = k.all_from = 0;
+    k.high += q.before;
+    k.all_to = q.before + max(k.all_to, 0);
+  }
   k.tiles = max((static_cast<uint32_t>(k.high - k.first()) + BN - 1) / BN, 1u);
   return k;
 }
@@ -142,8 +163,8 @@ __device__ __forceinline__ void ask(Raw<D>& w, const AttnArgs& a, uint32_t id, i
     w.vd[0] = *reinterpret_cast<const uint32_t*>(v + scales), w.vm[0] = *reinterpret_cast<const uint32_t*>(v + scales + gap);
   }
 }
-// What a thread of the expanders has asked for: the codes of the tile that `key` lies in, the next two page ids.
-template <int D>
+// What a thread of the expanders has asked for: the codes of the tile that `key` lies in, the next two page ids. TWO: the first `before` keys lie in other pages, of `first`.
+template <int D, bool TWO>
 struct Ahead {
   Raw<D> raw;
   int key;
@@ -152,13 +173,13 @@ struct Ahead {
   // Page ids are asked for two tiles ahead and looked at one tile ahead, when the codes are asked for: nothing here waits for memory.
   // A token that holds no key of the request (or lies in a page outside the pool) gets page 0's codes, and zeros for its scales.
   static __device__ __forceinline__ bool has_key(const Keys& keys, int key) { return key >= keys.low && key < keys.high; }
-  static __device__ __forceinline__ uint32_t ask_id(const AttnArgs& a, const Keys& keys, const int32_t* table, int key) {
-    return has_key(keys, key) ? static_cast<uint32_t>(table[key >> a.pool.log_page]) : 0u;
+  static __device__ __forceinline__ uint32_t ask_id(const AttnArgs& a, const Keys& keys, const int32_t* table, const int32_t* first, int before, int key) {
+    return !has_key(keys, key) ? 0u : static_cast<uint32_t>(TWO && key < before ? first[key >> a.pool.log_page] : table[(TWO ? key - before : key) >> a.pool.log_page]);
   }
-  __device__ __forceinline__ void ask_codes(const AttnArgs& a, const Keys& keys, uint32_t head, uint32_t quarter) {
+  __device__ __forceinline__ void ask_codes(const AttnArgs& a, const Keys& keys, int before, uint32_t head, uint32_t quarter) {
     there = has_key(keys, key) && id < a.pool.n_pages;
     if (has_key(keys, key) && !there) note_range(a.err);
-    ask<D>(raw, a, there ? id : 0u, key, head, quarter);
+    ask<D>(raw, a, there ? id : 0u, TWO && key >= before ? key - before : key, head, quarter);
   }
 };
 // Eight codes at bits 4 i of both halves -> four words of two f16 values m + d q.
@@ -269,6 +290,12 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     return false;
   };
 
+  if (MODE == BEHIND && blockIdx.x == 0) {  // what is wrong with the prefixes is reported
+    for (uint32_t g = threadIdx.x; g < a.n_prefix; g += THREADS) {
+      const int from = a.prefix_start[g], to = a.prefix_start[g + 1];
+      if (from < 0 || to < from || to > static_cast<int>(a.n_own) || a.prefix_len[g] > static_cast<int>(min(a.max_prefix, a.prefix_pages << a.pool.log_page))) note_range(a.err);
+    }
+  }
   // ---- the line of key tiles, and this CTA's stretch [c0, c1) of it ----
   const uint32_t per = (a.n_req + THREADS - 1) / THREADS;
   auto tiles_of = [&](const Request& q) {  // of all items of a request
@@ -342,14 +369,16 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
     const uint32_t plain0 = static_cast<uint32_t>(max(keys.all_from - key_first + static_cast<int>(BN) - 1, 0)) / BN;
     const uint32_t plain_n = static_cast<uint32_t>(max((keys.all_to - key_first) / static_cast<int>(BN) - static_cast<int>(plain0), 0));
     // the expanders' first codes are on their way while the queries come (where there are registers for both)
-    Ahead<D> ahead;
+    Ahead<D, MODE == BEHIND> ahead;
     const bool expands = warp >= S::FIRST_EXPANDER && warp < S::FIRST_SOFTMAX;
+    const int before = MODE == BEHIND ? q.before : 0;
+    const int32_t* first_table = MODE == BEHIND ? a.prefix_table + static_cast<size_t>(q.prefix) * a.prefix_stride : nullptr;
     auto ask_first = [&]() {
       const int32_t* table = pages_of<MODE>(a, cur.r, head);
       ahead.key = key_first + static_cast<int>(8 * (warp - S::FIRST_EXPANDER) + (lane & 7));
-      ahead.id = ahead.ask_id(a, keys, table, ahead.key);
-      ahead.id_next = n > 1 ? ahead.ask_id(a, keys, table, ahead.key + static_cast<int>(BN)) : 0u;
-      ahead.ask_codes(a, keys, head, lane >> 3);
+      ahead.id = ahead.ask_id(a, keys, table, first_table, before, ahead.key);
+      ahead.id_next = n > 1 ? ahead.ask_id(a, keys, table, first_table, before, ahead.key + static_cast<int>(BN)) : 0u;
+      ahead.ask_codes(a, keys, before, head, lane >> 3);
     };
     if (NQ == 1 && expands) ask_first();
     // ---- queries -> f16, each row times its power of two ----
@@ -458,8 +487,8 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         }
         ahead.key += BN;
         ahead.id = ahead.id_next;
-        if (i + 1 < n) ahead.ask_codes(a, keys, head, quarter);
-        if (i + 2 < n) ahead.id_next = ahead.ask_id(a, keys, table, ahead.key + static_cast<int>(BN));
+        if (i + 1 < n) ahead.ask_codes(a, keys, before, head, quarter);
+        if (i + 2 < n) ahead.id_next = ahead.ask_id(a, keys, table, first_table, before, ahead.key + static_cast<int>(BN));
         if (c >= SLOTS && !__all_sync(FULL, waitx(&k_empty[s], (c / SLOTS - 1) & 1))) break;
         put<D, false>(mine, smem + S::OFF_K + s * S::KV_B, row, quarter, a.bias);
         fence_proxy_async();
@@ -480,7 +509,8 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       const float scale = row_scale[x * BM + r];
       // this row sees the keys [lo, hi)
       const int past = q.kv_len - q.q_len;
-      const int hi = row >= q.rows ? 0 : MODE == PARTS && !q.causal ? q.kv_len : past + static_cast<int>(row / a.group) + 1, lo = MODE == PARTS ? 0 : first_seen(hi, a.window);
+      const int own = past + static_cast<int>(row / a.group) + 1;
+      const int hi = row >= q.rows ? 0 : MODE == PARTS && !q.causal ? q.kv_len : MODE == BEHIND ? before + max(own, 0) : own, lo = MODE == PLAIN ? first_seen(hi, a.window) : 0;
       float m_run = NEG_BIG, l_run = 0.f;
       for (uint32_t i = 0; i < n; i++) {
         const uint32_t c = done + i, b = c & 1, s = c % SLOTS;
@@ -763,6 +793,7 @@ cudaError_t bp_kv4_prefill_init(bp_paged_ctx* c) {
   for (uint32_t i = 0; i < 4 && e == cudaSuccess; i++) {
     e = with_kernel<PLAIN>(i & 1 ? 128 : 64, i & 2, allow);
     if (e == cudaSuccess) e = with_kernel<PARTS>(i & 1 ? 128 : 64, i & 2, allow);
+    if (e == cudaSuccess) e = with_kernel<BEHIND>(i & 1 ? 128 : 64, i & 2, allow);
   }
   return e != cudaSuccess ? e : cudaMalloc(&c->prefill_partials, floats * sizeof(float));
 }
@@ -774,5 +805,7 @@ cudaError_t bp_launch_kv4_prefill(bp_paged_ctx* c, cudaStream_t s, uint32_t head
     if (piece) *piece = S::PIECE;
     return bp_launch(true, kernel, dim3(ctas ? ctas : c->sm_count), dim3(S::THREADS), S::SMEM, s, a, c->prefill_partials, c->counters);
   };
-  return mode == PLAIN ? with_kernel<PLAIN>(head_dim, rows > BM, launch) : with_kernel<PARTS>(head_dim, rows > BM, launch);
+  return mode == PLAIN   ? with_kernel<PLAIN>(head_dim, rows > BM, launch)
+         : mode == PARTS ? with_kernel<PARTS>(head_dim, rows > BM, launch)
+                         : with_kernel<BEHIND>(head_dim, rows > BM, launch);
 }

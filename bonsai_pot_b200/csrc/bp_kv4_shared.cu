@@ -7,8 +7,9 @@
 // the kernel here joins them all, in the order of the keys.
 //
 // Floors: prefix and own keys once, 6.2 us for 64 tokens behind two prefixes of up to 8191 keys (32 / 8 heads of 128, up to 1000 keys of their own), the products, 220 us for 4 chunks of up to 512
-// behind 16384. Measured 41 and 444 us, 16 for 8 tokens behind 2048 keys (bp_kv4_attention for the 64 tokens over the same keys in rows of their own: as many keys as 64 requests have together, some 110).
-// Bound by the attention kernels' beginnings and ends and, of chunks, by their softmax. One launch after the other, each joining its items by the CTA that comes last, took 92, 513 and 31.
+// behind 16384. Measured 41 and 412 us, 16 for 8 tokens behind 2048 keys (bp_kv4_attention over the same keys in rows of pages for each request: 116, 403 and 19).
+// Bound by the attention kernels' beginnings and ends and, of chunks, by their softmax. One launch after the other, each joining its items by the CTA that comes last, took 92, 513 and 31; chunks
+// in parts 444.
 #include "bp_kv4_attention.cuh"
 #include "bp_paged_host.cuh"
 
@@ -23,6 +24,13 @@ struct JoinArgs {
   const float* slots[2];             // pieces of prefixes, of own keys
   uint32_t piece[2], ctas[2], rows[2];  // floats of a piece, CTAs that have some, rows of one
 };
+// Rows of a request (on the average) times head_dim above which it has no need to share the expansion of its prefix's codes: its own rows fill a CTA's query tiles, and its keys are its prefix's
+// and its own in one item, without parts. us, in one item / in parts:
+//   head_dim 128, 32 / 8 heads        128 rows  256      512      1024         head_dim 64, 40 / 8 heads  160 rows  320      640      1280
+//   4 requests behind 16384 keys      76/58     101/95   149/154  218/216                                 84/66     114/87   163/139  290/311
+//   16 behind 4096                    76/64     100/93   143/155  212/247                                 86/72     107/86   130/124  175/190
+//   4 behind 1000                     23/24     34/29    35/38    47/63                                   24/21     27/30    32/38    36/51
+constexpr uint64_t BEHIND_VALUES = 57344;
 constexpr uint32_t JOIN_THREADS = 256;
 
 // A warp per row, N pieces of it on their way.
@@ -135,6 +143,12 @@ int bp_kv4_attention_shared(bp_paged_ctx* c, void* stream, uint32_t dtype, const
   const bool own_many = in->max_kv != 0 && own_rows > BP_KV4_FEW_ROWS, prefix_many = in->max_prefix != 0 && prefix_rows > BP_KV4_FEW_ROWS;
   const uint32_t D = pool->head_dim;
   const uint64_t more = own_rows > prefix_rows ? own_rows : prefix_rows;
+  const uint64_t average = static_cast<uint64_t>(in->total_q) * a.group / in->n_req;
+  if (own_many && average * D > BEHIND_VALUES && static_cast<uint64_t>(in->max_prefix) + in->max_kv <= 0x7fffff00u) {
+    a.n_req = a.n_own;
+    BP_TRY(c, bp_launch_kv4_prefill(c, s, D, BEHIND, own_rows, 0, a));
+    return BP_OK;
+  }
   if (own_many || !prefix_many) {  // one launch for both
     BP_TRY(c, own_many ? bp_launch_kv4_prefill(c, s, D, PARTS, more, 0, a, &j.slots[0], &j.piece[0]) : bp_launch_kv4_few_rows(c, s, D, PARTS, more, 0, a, &j.slots[0], &j.piece[0]));
     j.slots[1] = j.slots[0];

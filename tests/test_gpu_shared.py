@@ -75,7 +75,7 @@ def test_one_token_each(ctx, dtype, heads, hkv, dim, page):
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("heads,hkv,dim", HEADS)
-@pytest.mark.parametrize("q", [5, 70])
+@pytest.mark.parametrize("q", [5, 70, 300])
 def test_several_tokens_each(ctx, dtype, heads, hkv, dim, q):
     """Drafts and chunks of odd lengths; a request with more queries than own keys (the first of them see the prefix alone), one without queries, a
     prefix of nobody, an empty prefix."""
@@ -120,7 +120,7 @@ def test_is_attention_over_both(ctx, n_req):
 
 
 @pytest.mark.parametrize("how", ["fused", "odd", "heads"])
-@pytest.mark.parametrize("q", [1, 60])
+@pytest.mark.parametrize("q", [1, 60, 130])
 def test_strided_rows_and_outputs_over_the_queries(ctx, how, q):
     s = Shared(6, "f16", [q, q, q], [300, 170, 60], [0, 3], [200], 8, 2, 128, 64, how=how)
     out = strided(torch.zeros(3 * q, 8, 128, dtype=torch.float16, device="cuda"), how)
@@ -131,7 +131,7 @@ def test_strided_rows_and_outputs_over_the_queries(ctx, how, q):
     s.check(over, scale=0.2)
 
 
-@pytest.mark.parametrize("q", [1, 40])
+@pytest.mark.parametrize("q", [1, 40, 450])
 @pytest.mark.parametrize("scale", [-0.1, 0.0, 3e6, 1e30])
 def test_scales(ctx, q, scale):
     """Scores that are turned or level, and ones of any size: then one key has all the weight, in the one part or the other."""
@@ -155,7 +155,7 @@ def test_scales(ctx, q, scale):
     s.check(s.run(ctx, scale=scale), scale=scale)
 
 
-@pytest.mark.parametrize("q", [1, 40])
+@pytest.mark.parametrize("q", [1, 40, 240])
 def test_values_that_are_no_numbers(ctx, q):
     """One in a prefix reaches all of its requests, one among own keys the queries that see it; in that block of dims alone. (Unused places hold bits that are no numbers in every test.)"""
     s = Shared(8, "f16", [q] * 4, [q + 70] * 4, [0, 2, 4], [100, 90], 8, 2, 64, 16)
@@ -181,7 +181,7 @@ def test_values_that_are_no_numbers(ctx, q):
 
 
 def test_lengths_and_pages_out_of_range(ctx):
-    for q in (1, 50):
+    for q in (1, 50, 240):
         s = Shared(9, "f16", [q] * 4, [200, 150, 60, 90], [0, 2, 4], [100, 300], 8, 2, 64, 16)
         want = s.run(ctx)
 
@@ -294,7 +294,7 @@ def test_two_launches_over_strided_rows_and_over_the_queries(ctx, how):
     ctx.status()
 
 
-@pytest.mark.parametrize("q,n", [(1, 5), (30, 5), (1, 45)])
+@pytest.mark.parametrize("q,n", [(1, 5), (30, 5), (1, 45), (130, 5)])
 def test_other_streams_and_graphs(ctx, q, n):
     """Captured twice with one work memory, replayed one behind the other: either follows the lengths on the device."""
     s = Shared(13, "bf16", [q] * n, [40 + 12 * (i % 5) for i in range(n)], [1, n], [400], 8, 2, 128, 32)
