@@ -744,7 +744,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
   const uint32_t share = max((total + n_cta - 1) / n_cta, NWARP);
   const uint32_t each = MODE == CHOSEN ? (items_s + n_cta - 1) / n_cta : 1;  // items of a CTA
   if (MODE == CHOSEN && each > 0 && (each * most_s + NWARP - 1) / NWARP <= (share + NWARP - 1) / NWARP + 1) {
-    // The same of several items per CTA, which here are about as long as one another. (32 tokens of up to 2048 keys 29.0 -> 28.0 us, 16 drafts of up to 5 tokens of 768 20.3 -> 16.8.)
+    // The same of several items per CTA, which here are about as long as one another. (A round more than equal stretches is worth it: 32 tokens of up to 2048 keys 26.2 us instead of 28.1,
+    // 48 36.3 instead of 37.6; two more are not: one token of 2048 keys 15.5 instead of 12.0.)
     if (warp < 2) {
       const uint32_t x = min((blockIdx.x + warp) * each, items_s);  // the first item of this CTA, and of the next one
       uint32_t at = 0;
