@@ -235,20 +235,28 @@ def test_no_prefix_and_no_keys(ctx):
 
 @pytest.mark.parametrize("n_req", [40, 90])
 def test_a_call_sees_what_was_written_just_before(ctx, n_req):
-    """Appended keys (of the prefix and the requests' own), then attention whose two launches begin early, again and again without waiting: as with a wait in between."""
+    """New lengths, queries turned into place and appended keys (of the prefix and the requests' own), in changing order, then attention whose two launches begin early, again and
+    again without waiting: as with a wait in between."""
     s = Shared(17, "bf16", [1] * n_req, [33] * n_req, [0, n_req], [700], 8, 2, 128, 16)
     rows = list(range(n_req)) + [s.n]
     at = [32] * n_req + [699]
     slots = torch.tensor([int(s.table[r, k // 16]) * 16 + k % 16 for r, k in zip(rows, at)], device="cuda")
     new = [normal(i, (n_req + 1, 2, 128), "bf16", 3.0) for i in range(40)]
     work = torch.empty(ctx.shared_work(n_req, 8, 128), device="cuda")
+    table = bp.RopeTable(torch.from_numpy(R.table(64, 128)).cuda())
+    asked = [normal(100 + i, (n_req, 8, 128), "bf16") for i in range(40)]
+    positions = [torch.randint(0, 64, (n_req,), device="cuda", dtype=torch.int32) for _ in new]
+    lengths = [torch.randint(1, 34, (n_req,), device="cuda", dtype=torch.int32) for _ in new]
+    back = [k.flip(0).contiguous() for k in new]
 
     def go(wait):
         outs = [torch.empty_like(s.q) for _ in new]
-        for k, out in zip(new, outs):
-            ctx.append(s.pool, k, k.flip(0), None, slots)
-            if wait:
-                torch.cuda.synchronize()
+        for i, (k, out) in enumerate(zip(new, outs)):
+            steps = [lambda: s.args[1].copy_(lengths[i]), lambda: ctx.rope(asked[i], s.q, positions[i], table), lambda: ctx.append(s.pool, k, back[i], None, slots)]
+            for at in range(3):
+                steps[(i + at) % 3]()
+                if wait:
+                    torch.cuda.synchronize()
             s.run(ctx, out, work=work)
             if wait:
                 torch.cuda.synchronize()
