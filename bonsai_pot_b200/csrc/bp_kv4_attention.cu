@@ -73,7 +73,9 @@ struct WarpState {
   uint32_t q[NT][NB][4];  // B fragments of S^T: dims 32 b + 8 t + {0,1}, {2,3} / 16, {4,5}, {6,7} / 16 of row g
   uint32_t qsum[NT];      // B fragment of the m's: block sums of row g
   float s_scale[NT][2];   // rows 2 t, 2 t + 1: the softmax scale's power of two (log2 units) times the row's (its sign is the query's, its mantissa in the scores)
-  float m[NT][2], l[NT][2];   // running maximum (log2 units) and this lane's part of the sum, of rows 2 t, 2 t + 1
+  // Of rows 2 t, 2 t + 1: weights are 2^(score - top), scores in log2 units; this lane's part of their sum. top is P_UP below the running maximum, as nearly as
+  // binary32 has it, and it alone is what O and l refer to: where neighbouring numbers are 4 and more apart the maximum lies 0 to 14 above it.
+  float top[NT][2], l[NT][2];
   float o[NT][2 * NB][4]; // [m-tile i][dims 32 (i / 2) + 4 g + 2 (i % 2) + {0, 1}] x rows 2 t, 2 t + 1: {d0 r0, d0 r1, d1 r0, d1 r1}
 };
 
@@ -157,7 +159,7 @@ __device__ __forceinline__ void set_queries(WarpState<D, NT>& w, RawQueries<D, N
     for (int c = 0; c < 2; c++) {
       // (never 0: a masked score, -infinity, stays what it is)
       w.s_scale[e][c] = fmaxf(a.power * __shfl_sync(FULL, down, 4 * (2 * t + c)), 0x1p-122f);
-      w.m[e][c] = NEG_BIG;
+      w.top[e][c] = NEG_BIG;
       w.l[e][c] = 0.f;
     }
 #pragma unroll
@@ -299,7 +301,7 @@ __device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4]
           }
       }
     }
-    float mx[2];
+    float mx[2], above[2];  // the unit's largest scores, before their power of two; by how much they lie above top
 #pragma unroll
     for (int c = 0; c < 2; c++) {
       mx[c] = fmaxf(s[e][0][c], s[e][0][c + 2]);
@@ -307,15 +309,18 @@ __device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4]
       for (int i = 1; i < 4; i++) mx[c] = fmaxf(mx[c], fmaxf(s[e][i][c], s[e][i][c + 2]));
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(FULL, mx[c], o));
-      mx[c] *= w.s_scale[e][c];
+      above[c] = fmaf(mx[c], w.s_scale[e][c], -w.top[e][c]);
     }
-    if (__any_sync(FULL, mx[0] > w.m[e][0] || mx[1] > w.m[e][1])) {
+    if (__any_sync(FULL, above[0] > P_UP || above[1] > P_UP)) {
       float corr[2];
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        const float m_new = fmaxf(w.m[e][c], mx[c]);
-        corr[c] = ex2(w.m[e][c] - m_new);
-        w.m[e][c] = m_new;
+        const float m = mx[c] * w.s_scale[e][c];
+        float top = m - P_UP;
+        if (m - top > 15.f) top = m;  // (where neighbouring numbers are 16 apart the difference may be 16, and f16 has no 2^16)
+        top = fmaxf(w.top[e][c], top);
+        corr[c] = ex2(w.top[e][c] - top);
+        w.top[e][c] = top;
         w.l[e][c] *= corr[c];
       }
 #pragma unroll
@@ -323,18 +328,11 @@ __device__ __forceinline__ void softmax64(WarpState<D, NT>& w, float (&s)[NT][4]
 #pragma unroll
         for (int k = 0; k < 4; k++) w.o[e][i][k] *= corr[k & 1];
     }
-    // (where neighbouring numbers are 16 apart the difference may be 16, and f16 has no 2^16)
-    float top[2];
-#pragma unroll
-    for (int c = 0; c < 2; c++) {
-      top[c] = w.m[e][c] - P_UP;
-      if (w.m[e][c] - top[c] > 15.f) top[c] = w.m[e][c];
-    }
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        s[e][i][k] = ex2(fmaf(s[e][i][k], w.s_scale[e][k & 1], -top[k & 1]));
+        s[e][i][k] = ex2(fmaf(s[e][i][k], w.s_scale[e][k & 1], -w.top[e][k & 1]));
         w.l[e][k & 1] += s[e][i][k];
       }
   }
@@ -927,7 +925,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
 #pragma unroll
                 for (int x = 0; x < NB; x++)
                   *reinterpret_cast<float4*>(record + 32 * x + 4 * g) = make_float4(w.o[e][2 * x][c], w.o[e][2 * x][c + 2], w.o[e][2 * x + 1][c], w.o[e][2 * x + 1][c + 2]);
-                if (g == 0) end_record<D>(record, w.m[e][c], w.l[e][c]);
+                if (g == 0) end_record<D>(record, w.top[e][c], w.l[e][c]);
                 continue;
               }
               const float inv = w.l[e][c] == 0.f ? 0.f : 1.f / w.l[e][c];
@@ -948,7 +946,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, 1) kv4_attention_kernel
 #pragma unroll
               for (int x = 0; x < NB; x++)
                 *reinterpret_cast<float4*>(p + 32 * x + 4 * g) = make_float4(w.o[e][2 * x][c], w.o[e][2 * x][c + 2], w.o[e][2 * x + 1][c], w.o[e][2 * x + 1][c + 2]);
-              if (g == 0) *reinterpret_cast<float2*>(p + D) = make_float2(w.m[e][c], w.l[e][c]);
+              if (g == 0) *reinterpret_cast<float2*>(p + D) = make_float2(w.top[e][c], w.l[e][c]);
             }
           if (lane == 0)
             pieces[2 * warp + (last ? 1 : 0)] = Piece{1, plan[0] + begin + first - cur.unit, cur.q.units, cur.head, row0, min(S::ROWS, n_rows - row0), cur.q.q0, !cur.q.causal};

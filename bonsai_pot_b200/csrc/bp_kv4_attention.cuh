@@ -18,7 +18,7 @@ enum Mode {
   BEHIND,  // requests whose keys are their prefix's and then their own: two rows of pages; their outputs are written
   CHOSEN,  // tokens that see every key of pages chosen for each KV head; their outputs are written
 };
-// A partial result of a row: [0, D) the values' sum, [D] the largest score (log2 units), [D + 1] the sum of the weights, then as whole numbers [D + 2] c and
+// A partial result of a row: [0, D) the values' sum, [D] the score (log2 units) that its weights refer to, 2^(score - [D]), [D + 1] the sum of the weights, then as whole numbers [D + 2] c and
 // [D + 3] n << 16 | r. n = 0: that is it. n > 0: n CTAs from c on have a piece of it each, at row r of their place for pieces (piece_at).
 // bp_kv4_shared.cu puts them together.
 template <int D>

@@ -609,6 +609,10 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
         uint8_t* stage = smem + x * S::Q_B;
         const uint32_t rows = min(BM, q.rows - min(tile_row, q.rows));
         records[x * BM + r] = to;
+        // What is summed refers to the maximum: without P_UP, which a large maximum would swallow. The maximum's product with the scale is rounded; what it lost goes into the sums where
+        // both parts are this kernel's (beside it are the other kernel's scores, each rounded the same way). From 2^31 on what is lost no longer fits.
+        const float m = m_run * scale, lost = a.first ? 0.f : fmaf(m_run, scale, -m);
+        const float down_by = ex2(fminf(fmaxf(lost, -60.f), 60.f) - P_UP);
 #pragma unroll 1
         for (uint32_t half = 0; half < 2; half++) {
           if (half) named_bar_sync(1 + x, 128);  // (what was staged before has gone)
@@ -622,7 +626,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
             for (int e = 0; e < 4; e++) {
               float v[4];
 #pragma unroll
-              for (int j = 0; j < 4; j++) v[j] = none ? __int_as_float(0x7fffffff) : __uint_as_float(o[8 * (e >> 1) + column_of(4 * (e & 1) + j)]);
+              for (int j = 0; j < 4; j++) v[j] = none ? __int_as_float(0x7fffffff) : __uint_as_float(o[8 * (e >> 1) + column_of(4 * (e & 1) + j)]) * down_by;
               *reinterpret_cast<float4*>(stage + r * (2 * D) + (((4 * k + e) ^ (r & (U - 1))) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
             }
           }
@@ -636,7 +640,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
           }
         }
         if (there) {
-          end_record<D>(to, l_run == 0.f ? NEG_BIG : m_run * scale, l_run);
+          end_record<D>(to, l_run == 0.f ? NEG_BIG : m, l_run * down_by);
           if (!all && blockIdx.x == first_cta) end_record<D>(record, NEG_BIG, 0.f, first_cta, parts, x * BM + r);
         }
       } else if (first == 0 && n == keys.tiles) {

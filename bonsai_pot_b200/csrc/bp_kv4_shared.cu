@@ -1,7 +1,7 @@
 // Attention of requests behind prefixes that several of them have in common (include/bonsai_pages.h).
 //
-// The keys that a query sees are those of its prefix and its request's own. With o_i = sum of 2^(s - m_i) v, l_i = sum of 2^(s - m_i) and m_i = the
-// largest score (log2 units) over part i of the keys, the output is sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, m = the largest m_i. Prefixes are items whose rows
+// The keys that a query sees are those of its prefix and its request's own. With o_i = sum of 2^(s - m_i) v, l_i = sum of 2^(s - m_i) and m_i near the
+// largest score s (log2 units) over part i of the keys, the output is sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, m = the largest m_i. Prefixes are items whose rows
 // are those of all their requests, so that their codes are read and expanded once for all of them; own keys are items of each request. Both are the attention
 // kernels' (bp_kv4_attention.cu, bp_kv4_prefill.cu), which leave (o, m, l) of whole items in the caller's work memory and of pieces of items in the context's, in 32 bits;
 // the kernel here joins them all, in the order of the keys.
