@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
             to[(4 * k + e) * S::ROWS] = make_float4(v[0], v[1], v[2], v[3]);  // (a warp's 32 rows are 512 bytes)
           }
         }
-        reinterpret_cast<float2*>(mine + D * S::ROWS)[x * BM + r] = make_float2(l_run == 0.f ? NEG_BIG : m_run * scale, l_run);
+        reinterpret_cast<float2*>(mine + D * S::ROWS)[x * BM + r] = make_float2(l_run == 0.f ? NEG_BIG : m_run, l_run);
       }
     }
     done += n;
@@ -729,15 +729,16 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
       const uint32_t rows = min(S::ROWS, q.rows - row0);
       auto piece = [&](uint32_t k) { return from + static_cast<size_t>(2 * k + (k == 0)) * S::PARTIAL; };
       auto ml = [&](uint32_t k, uint32_t r) { return reinterpret_cast<const float2*>(piece(k) + D * S::ROWS)[r]; };
-      // the rows' maxima and 1 / sums, in the dead K tiles; then a thread per four dims of a row, the rows of a warp side by side
+      // the rows' maxima (before the scale, as in the tiles: scaled ones would be rounded) and 1 / sums, in the dead K tiles; then a thread per four dims of a row, the rows of a warp side by side
       float2* joined = reinterpret_cast<float2*>(smem + S::OFF_K);
       for (uint32_t r = threadIdx.x; r < S::ROWS; r += THREADS) {
         float m = NEG_BIG, l = 0.f;
+        const float scale = row_scale[r];
 #pragma unroll 4
         for (uint32_t k = 0; k < j.n; k++) {
           const float2 e = ml(k, r);
           const float top = fmaxf(m, e.x);
-          l = l * ex2(m - top) + e.y * ex2(e.x - top);
+          l = l * ex2((m - top) * scale) + e.y * ex2((e.x - top) * scale);
           m = top;
         }
         joined[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
@@ -751,7 +752,7 @@ __global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1) kv4_prefill_kernel(c
 #pragma unroll 2
         for (uint32_t k = 0; k < j.n; k++) {
           const float4 v = reinterpret_cast<const float4*>(piece(k))[c * S::ROWS + r];
-          const float w = ex2(ml(k, r).x - all.x) * all.y;
+          const float w = ex2((ml(k, r).x - all.x) * row_scale[r]) * all.y;
           o = make_float4(fmaf(v.x, w, o.x), fmaf(v.y, w, o.y), fmaf(v.z, w, o.z), fmaf(v.w, w, o.w));
         }
         // staged in the dead Q tiles: whole rows go to memory

@@ -77,6 +77,17 @@ def test_many_rows(ctx, power, order, q, heads, hkv, dim, kv):
     ctx.status()
 
 
+@pytest.mark.parametrize("power", POWERS)
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed"])
+@pytest.mark.parametrize("q,heads,hkv,dim,kv", [(40, 2, 2, 128, 3000), (130, 4, 1, 64, 900), (300, 1, 1, 64, 1500)])
+def test_many_rows_of_any_scale(ctx, power, order, q, heads, hkv, dim, kv):
+    """This kernel takes the maximum off before the scale comes in: no product is rounded before its difference is taken, in the joins neither."""
+    r = exact(Requests(6, "f16", [q, q], [kv, kv // 3], heads, hkv, dim, 32), 1, order)
+    for scale in (0.7 * 2.0 ** power, 1.13 * 2.0 ** power):
+        r.check(r.run(ctx, scale=scale), scale=scale)
+    ctx.status()
+
+
 FORMS = [(1, 64, 4), (1, 5, 4), (3, 30, 4), (40, 5, 4), (450, 2, 4)]  # two launches side by side, one for few rows, two, one for many rows in parts, prefix and own keys in one item
 
 
@@ -89,6 +100,18 @@ def test_behind_a_prefix(ctx, power, order, q, n, heads):
     s = exact(Shared(3, "f16", [q] * n, [own if i % 3 else max(own, q) + 500 for i in range(n)], [0, n - 1], [prefix], heads, 2, 128 if q == 3 else 64, 32), 1, order)
     scale = scale_of(2.0 ** power)
     s.check(s.run(ctx, scale=scale), scale=scale)
+    ctx.status()
+
+
+@pytest.mark.parametrize("power", POWERS)
+@pytest.mark.parametrize("order", ["rising", "mixed", "level"])
+@pytest.mark.parametrize("q,n,heads", FORMS[3:])
+def test_behind_a_prefix_with_any_scale(ctx, power, order, q, n, heads):
+    """The same of the kernel for many rows alone; in parts its records hold what their maxima's products lose, up to 2^31."""
+    s = exact(Shared(7, "f16", [q] * n, [590 if i % 3 else q + 500 for i in range(n)], [0, n - 1], [700], heads, 2, 64, 32), 1, order)
+    for scale in (0.7 * 2.0 ** power, 1.13 * 2.0 ** power):
+        if power < 9 or q > 40:
+            s.check(s.run(ctx, scale=scale), scale=scale)
     ctx.status()
 
 
