@@ -259,7 +259,7 @@ __device__ __forceinline__ uint32_t entries_of(const Tables& t, uint32_t tokens)
 
 constexpr uint32_t ROW_THREADS = 512;
 
-// A CTA per row. (A row that is there twice has been emptied by who came first.)
+// A CTA per row. A row whose length can be none is left; one that is there twice has been emptied by who came first.
 __global__ void __launch_bounds__(ROW_THREADS) pages_release_kernel(const __grid_constant__ Tables t, const int32_t* __restrict__ rows) {
   __shared__ int32_t tokens_s;
   pdl_launch_dependents();
@@ -270,11 +270,14 @@ __global__ void __launch_bounds__(ROW_THREADS) pages_release_kernel(const __grid
     if (threadIdx.x == 0) note_range(t.err);
     return;
   }
-  if (threadIdx.x == 0) tokens_s = atomicExch(&t.kv_len[r], 0);
+  if (threadIdx.x == 0) {
+    const int32_t tokens = *reinterpret_cast<volatile int32_t*>(&t.kv_len[r]);
+    const bool good = tokens >= 0 && t.pages_of(tokens) <= t.row_pages;
+    if (!good) note_range(t.err);
+    tokens_s = good && atomicCAS(&t.kv_len[r], tokens, 0) == tokens ? tokens : 0;
+  }
   __syncthreads();
-  const int32_t tokens = tokens_s;
-  if (tokens < 0 && threadIdx.x == 0) note_range(t.err);
-  const uint32_t n = entries_of(t, max(tokens, 0));
+  const uint32_t n = t.pages_of(tokens_s);
   const int32_t* row = t.row(r);
   for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 4 * ROW_THREADS) {  // four of a thread on their way
     int32_t page[4], refs[4];

@@ -30,7 +30,7 @@ typedef struct bp_page_tables {
  * = page * page_tokens + place in the page. Places from q_start[n_rows] on become -1 in both: padding, as for bp_rope and
  * bp_kv4_append. A row that is refused (no room, no pages) keeps its length, and its tokens become padding too. */
 int bp_pages_grow(bp_paged_ctx* ctx, void* stream, const bp_page_tables* tables, const void* n_new, void* q_start, void* positions, void* slots, uint32_t n_out);
-/* The rows rows[0 .. n - 1] (device int32; negative: none) give their pages back: refs - 1 for each, kv_len 0. */
+/* The rows rows[0 .. n - 1] (device int32; negative: none) give their pages back: refs - 1 for each, kv_len 0. Entries that are no pages, and counts that are 0 already, are passed over. */
 int bp_pages_release(bp_paged_ctx* ctx, void* stream, const bp_page_tables* tables, const void* rows, uint32_t n);
 /* Row children[i] (which must be empty) becomes what row parents[i] is (device int32 [n] both; a negative one of either: no pair). Full pages are
  * shared; a last page that is not full is to be copied, into the lowest free pages in the order of the pairs: src[i], dst[i] (device

@@ -1,0 +1,36 @@
+"""Page tables whose numbers are not what a server keeps in them: what a call refuses it reports and leaves."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import bonsai_pot_b200 as bp  # noqa: E402
+from tests.test_gpu_pages import Both, ctx, dev  # noqa: E402, F401
+
+pytestmark = pytest.mark.gpu
+
+
+def reported(ctx, call):
+    call()
+    with pytest.raises(bp.ContextOverflow):
+        ctx.status()
+    ctx.status()
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("length", [-1, -(1 << 31), "one more", (1 << 31) - 1])
+def test_a_row_of_no_possible_length_is_not_given_back(ctx, page, length):
+    """Its length, its entries and every count stay; the other rows of the call end, one that is there twice once."""
+    b = Both(1, 4, 5, 40, page, [3 * page + 1, 5 * page, 7, 2 * page])
+    length = 5 * page + 1 if length == "one more" else length
+    b.kv[1] = length
+    table = b.table.clone()
+    reported(ctx, lambda: ctx.release(b.gpu, dev([0, 1, 1, 3, 3])))
+    assert b.kv.tolist() == [0, length, 7, 0] and torch.equal(b.table, table)
+    b.kv[1] = 5 * page
+    b.ref.release([0, 3])
+    b.check()
+    ctx.release(b.gpu, dev([1]))  # put right it ends like any other
+    b.ref.release([1])
+    b.check()
+    ctx.status()
