@@ -416,7 +416,7 @@ struct CompactArgs {
   uint32_t most;
   uint32_t* counter;
 };
-// What moves where, by one CTA. The count of a page that moves becomes -1 - (where it goes) for the tables' entries.
+// What moves where, by one CTA. The count of a page that moves becomes -1 - (which move it is) for the tables' entries; src tells it from a count that was negative before.
 __device__ __forceinline__ void plan_moves(const CompactArgs& c, uint32_t* smem, uint32_t* sums) {
   const Tables& t = c.t;
   Look<false> first;
@@ -430,7 +430,7 @@ __device__ __forceinline__ void plan_moves(const CompactArgs& c, uint32_t* smem,
     const int32_t from = i < high ? c.src[i] : -1, to = i < low ? c.dst[i] : -1;
     if (from >= 0 && to >= 0 && from > to) {
       t.refs[to] = t.refs[from];
-      t.refs[from] = -1 - to;
+      t.refs[from] = -1 - static_cast<int32_t>(i);
     } else {
       c.src[i] = c.dst[i] = -1;
     }
@@ -449,10 +449,18 @@ __device__ __forceinline__ void follow_moves(const CompactArgs& c, uint32_t r, u
     for (uint32_t k = 0; k < 4; k++) page[k] = i0 + 32 * k < n ? row[i0 + 32 * k] : 0;
 #pragma unroll
     for (uint32_t k = 0; k < 4; k++) refs[k] = static_cast<uint32_t>(page[k]) < t.n_pages ? t.refs[page[k]] : 0;
+    int32_t from[4], to[4];
 #pragma unroll
     for (uint32_t k = 0; k < 4; k++) {
-      if (static_cast<uint32_t>(page[k]) >= t.n_pages) note_range(t.err);
-      if (refs[k] < 0 && i0 + 32 * k < n) row[i0 + 32 * k] = -1 - refs[k];
+      const uint32_t move = static_cast<uint32_t>(-1 - refs[k]);  // (of a count that is none: beyond `most`)
+      from[k] = move < c.most ? c.src[move] : -1;
+      to[k] = move < c.most ? c.dst[move] : -1;
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) {
+      if (i0 + 32 * k >= n) continue;
+      if (static_cast<uint32_t>(page[k]) >= t.n_pages || (refs[k] < 0 && from[k] != page[k])) note_range(t.err);
+      else if (refs[k] < 0) row[i0 + 32 * k] = to[k];
     }
   }
 }

@@ -34,3 +34,20 @@ def test_a_row_of_no_possible_length_is_not_given_back(ctx, page, length):
     b.ref.release([1])
     b.check()
     ctx.status()
+
+
+@pytest.mark.parametrize("rows,width", [(4, 30), (300, 1000)])
+@pytest.mark.parametrize("count", [-1, -2, -6, -(1 << 31)])
+def test_compaction_tells_counts_below_zero_from_moves(ctx, rows, width, count):
+    """A page of such a count neither moves nor sends a row's entry elsewhere; it is reported. The others move."""
+    page, n_pages = 16, 30000
+    b = Both(2, rows, width, n_pages, page, [page * 20] + [page * 3] * (rows - 1))
+    held = int(b.ref.table[0, 7])
+    b.ref.refs[held] = count
+    b.refs.copy_(dev(b.ref.refs))
+    src, dst = dev([5] * 50), dev([5] * 50)
+    reported(ctx, lambda: ctx.compact(b.gpu, src, dst))
+    want = b.ref.compact(50)  # (which leaves alone what is neither free nor held)
+    assert np.array_equal(src.cpu().numpy(), want[0]) and np.array_equal(dst.cpu().numpy(), want[1])
+    assert (want[0] >= 0).sum() == min(50, 20 + 3 * (rows - 1) - 1) and b.ref.table[0, 7] == held
+    b.check()
