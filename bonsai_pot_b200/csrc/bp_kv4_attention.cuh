@@ -252,6 +252,7 @@ cudaError_t bp_launch_kv4_prefill(bp_paged_ctx* c, cudaStream_t s, uint32_t head
                                   const float** slots = nullptr, uint32_t* piece = nullptr);
 cudaError_t bp_launch_kv4_few_rows(bp_paged_ctx* c, cudaStream_t s, uint32_t head_dim, int mode, uint64_t rows, uint32_t ctas, const bp::kv4::AttnArgs& a,
                                    const float** slots = nullptr, uint32_t* piece = nullptr);
+constexpr uint32_t BP_KV4_ITEM_COST_IN_PARTS = 10;  // what an item of the kernel for many rows costs in PARTS besides its tiles of 64 keys, in such tiles (bp_kv4_prefill.cu)
 constexpr uint64_t BP_KV4_FEW_ROWS = 32;  // of a request, that the kernel for few rows takes (bp_kv4_attention.cu has the reason)
 // The scale and what belongs to the context and the pool.
 uint32_t bp_kv4_table_pages(const bp::Pool& pool, uint32_t stride);

@@ -44,7 +44,7 @@ constexpr uint32_t MIXED = 11;
 // What beginning and ending an item costs, in key tiles. (In parts its rows are 32-bit records. 4 chunks of 512 behind 16384 keys: with 6, 633 us, as the CTAs with
 // the chunks' own keys, a dozen tiles per item, came last; 10: 444, 14: 451, 18: 455.)
 template <int MODE>
-constexpr uint32_t ITEM_COST = MODE == PARTS ? 10 : 6;
+constexpr uint32_t ITEM_COST = MODE == PARTS ? BP_KV4_ITEM_COST_IN_PARTS : 6;
 constexpr float GROW = 5.f;            // log2 by which a maximum may grow before O is rescaled; P_UP + GROW stays below 16
 
 template <int D, uint32_t NQ>

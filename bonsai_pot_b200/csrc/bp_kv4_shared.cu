@@ -107,9 +107,10 @@ int bp_kv4_attention_shared(bp_paged_ctx* c, void* stream, uint32_t dtype, const
   if (in->n_req > 65535 || in->n_prefix > 65535) return fail_config(c, "at most 65535 requests and prefixes");
   if (static_cast<uint64_t>(in->total_q) * in->n_head > 0x7fffffffull || in->max_kv > 0x7fffff00u || in->max_prefix > 0x7fffff00u)
     return fail_config(c, "total_q * n_head, max_kv and max_prefix must be < 2^31");
-  // units of 64 keys of 8 rows, and what an item of the kernel for many queries costs besides, are counted in 32 bits, those of both parts together
-  const uint64_t rows8 = static_cast<uint64_t>(in->total_q) * (in->n_head / p.n_kv_head) / 8;
-  if ((rows8 + in->n_req) * p.n_kv_head > 0x7fffffffull / (in->max_kv / 64 + 8) || (rows8 + in->n_prefix) * p.n_kv_head > 0x7fffffffull / (in->max_prefix / 64 + 8))
+  // Units of 64 keys of 8 rows, and what an item of the kernel for many queries costs besides, are counted in 32 bits, those of both parts together. (Prefix and own keys in one
+  // item are no more: that is for hundreds of rows per request, of which an item has 128 or 256.)
+  const uint64_t rows8 = static_cast<uint64_t>(in->total_q) * (in->n_head / p.n_kv_head) / 8, cost = 1 + BP_KV4_ITEM_COST_IN_PARTS;
+  if ((rows8 + in->n_req) * p.n_kv_head * (in->max_kv / 64 + cost) + (rows8 + in->n_prefix) * p.n_kv_head * (in->max_prefix / 64 + cost) > 0xffffffffull)  // (no more than 2^59 each)
     return fail_config(c, "total_q * n_head * max_kv or max_prefix is too large for one call");
   if (!rq.data || !ro.data || !in->q_start || !in->kv_len || !in->work || (in->max_kv != 0 && (!p.data || !in->page_table)) ||
       (in->n_prefix != 0 && (!in->prefix_start || !in->prefix_len || (in->max_prefix != 0 && (!p.data || !in->prefix_table)))))
