@@ -55,7 +55,7 @@ class Server:
         i32 = dict(dtype=torch.int32, device="cuda")
         positions, slots = torch.tensor(positions, **i32), torch.tensor(slots, device="cuda")
         q, k, v = qkv[:, :N_HEAD], qkv[:, N_HEAD:N_HEAD + N_KV_HEAD], qkv[:, N_HEAD + N_KV_HEAD:]
-        turned, out = torch.empty_like(q), torch.empty(q.shape, dtype=q.dtype, device="cuda")
+        turned, out = torch.empty_like(q), torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda")  # (so that a row nobody writes shows)
         self.ctx.rope(q, turned, positions, self.rope, w_norm=self.w_q)
         self.ctx.append(self.pool, k, v, positions, slots, self.rope, w_k_norm=self.w_k)
         self.ctx.attention(self.pool, turned, out, torch.tensor(starts, **i32), torch.tensor(lengths, **i32),
@@ -76,14 +76,16 @@ def projections(n):
 
 
 def deviation(server, request, q, out):
-    """Of `out`, the outputs of the request's last tokens q, from the plain softmax: the largest, and the largest in parts of sum p |v|."""
+    """Of `out`, the outputs of the request's last tokens q, from the plain softmax: the largest, and the largest in parts of sum p |v|; infinite where an output is no number."""
     k, v = (t.repeat_interleave(N_HEAD // N_KV_HEAD, 1) for t in server.keys(request))
     n, total = q.shape[0], k.shape[0]
     scores = torch.einsum("qhd,thd->qht", q.float(), k) / HEAD_DIM ** 0.5
-    hidden = torch.arange(total, device="cuda") > torch.arange(total - n, total, device="cuda")[:, None]
+    hidden = torch.arange(total, device=q.device) > torch.arange(total - n, total, device=q.device)[:, None]
     p = torch.softmax(scores.masked_fill(hidden[:, None], float("-inf")), -1)
     off = (torch.einsum("qht,thd->qhd", p, v) - out.float()).abs()
-    return off.max().item(), (off / torch.einsum("qht,thd->qhd", p, v.abs())).max().item()
+    weight = torch.einsum("qht,thd->qhd", p, v.abs())
+    both = off.max().item(), torch.where(off == 0, 0.0, off / weight).max().item()  # (a token that sees one key may have a value of 0, and a weight of 0 with it)
+    return tuple(x if x == x else float("inf") for x in both)  # (max() would pass over what is no number)
 
 
 def run(steps=64, prompts=(700, 37, 1, 1300), seed=0):

@@ -77,7 +77,7 @@ def projections(n):
 
 
 def deviation(server, layer, row, q, out, alone=False):
-    """The largest deviation of `out`, the outputs of the row's last tokens q, from the plain softmax, in parts of sum p |v|."""
+    """The largest deviation of `out`, the outputs of the row's last tokens q, from the plain softmax, in parts of sum p |v|; infinite where an output is no number."""
     k, v = server.keys(layer, row)
     own = k.shape[0]
     if row and not alone:
@@ -85,11 +85,13 @@ def deviation(server, layer, row, q, out, alone=False):
     k, v = (t.repeat_interleave(N_HEAD // N_KV_HEAD, 1) for t in (k, v))
     n, total = q.shape[0], k.shape[0]
     scores = torch.einsum("qhd,thd->qht", q.float(), k) / HEAD_DIM ** 0.5
-    hidden = torch.arange(total, device="cuda") > torch.arange(total - n, total, device="cuda")[:, None]
+    hidden = torch.arange(total, device=q.device) > torch.arange(total - n, total, device=q.device)[:, None]
     p = torch.softmax(scores.masked_fill(hidden[:, None], float("-inf")), -1)
     off = (torch.einsum("qht,thd->qhd", p, v) - out.float()).abs()
     assert own >= n
-    return (off / torch.einsum("qht,thd->qhd", p, v.abs())).max().item()
+    weight = torch.einsum("qht,thd->qhd", p, v.abs())
+    largest = torch.where(off == 0, 0.0, off / weight).max().item()  # (a token that sees one key may have a value of 0, and a weight of 0 with it)
+    return largest if largest == largest else float("inf")  # (max() would pass over what is no number)
 
 
 def run(steps=32, instruction=1000, questions=(37, 160, 5), answers=3, seed=0):
@@ -102,7 +104,7 @@ def run(steps=32, instruction=1000, questions=(37, 160, 5), answers=3, seed=0):
         nonlocal worst
         n = sum(n_new)
         qkv = projections(n)
-        turned, out = (torch.empty(LAYERS, n, N_HEAD, HEAD_DIM, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        turned, out = (torch.full((LAYERS, n, N_HEAD, HEAD_DIM), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(2))  # (so that a row nobody writes shows)
         server.step(torch.tensor(n_new, **I32), qkv, turned, out, ROW_PAGES * PAGE, instruction)
         at = 0
         for r, k in enumerate(n_new):
@@ -130,6 +132,7 @@ def run(steps=32, instruction=1000, questions=(37, 160, 5), answers=3, seed=0):
         n_new.zero_()
         n_new[live] = 1
         qkv.copy_(projections(len(children)))
+        out.fill_(float("nan"))
         graph.replay()
         if step in (0, steps // 2, steps - 1):
             for i, r in enumerate(live):
@@ -140,13 +143,13 @@ def run(steps=32, instruction=1000, questions=(37, 160, 5), answers=3, seed=0):
     for layer in range(LAYERS):
         server.ctx.summarise(server.pools[layer], server.summaries[layer], full)
         for places in (ROW_PAGES, 6):
-            pages, keys, got = torch.empty(1, N_KV_HEAD, places, **I32), torch.empty(1, **I32), torch.empty_like(q)
+            pages, keys, got = torch.empty(1, N_KV_HEAD, places, **I32), torch.empty(1, **I32), torch.full_like(q, float("nan"))
             server.ctx.select(server.pools[layer], server.summaries[layer], q, pages, keys, torch.tensor([0, 1], **I32), server.kv[:1], server.table[:1], max_q=1, max_kv=instruction, first=1, last=2)
             server.ctx.attention_selected(server.pools[layer], q, got, pages, keys)
             if places == ROW_PAGES:
                 worst = max(worst, deviation(server, layer, 0, q, got, alone=True))
-            elif int(keys) != 5 * PAGE + instruction % PAGE:
-                raise RuntimeError("six pages hold five full ones' keys and the last one's")
+            elif int(keys) != 5 * PAGE + instruction % PAGE or not got.isfinite().all():
+                raise RuntimeError("six pages hold five full ones' keys and the last one's, and outputs are numbers")
     server.ctx.status()
     return worst, int((server.refs > 0).sum())
 
