@@ -36,8 +36,9 @@ class Server:
         self.rope = bp.RopeTable(angles)
         self.prefix_start = torch.tensor([1, rows], **I32)  # the rows from 1 on go on where row 0 ends
 
-    def step(self, n_new, qkv, turned, out, most, prefix):
-        """n_new[r] further tokens for every row, packed in qkv [layers, tokens, heads + 2 KV heads, head_dim]; `most`, `prefix`: tokens of a row, of the instruction, at most.
+    def step(self, n_new, qkv, turned, out, each, most, prefix):
+        """n_new[r] further tokens for every row, packed in qkv [layers, tokens, heads + 2 KV heads, head_dim]; `each`, `most`, `prefix`: new tokens of a row, tokens of a row, of the
+        instruction, at most (by `each` and by the rows behind the instruction attention goes to its kernels for single tokens or for prompts: say 1 where it is 1).
         Rows behind the instruction see it, too."""
         n = qkv.shape[1]
         start, positions, slots = torch.empty(self.rows + 1, **I32), torch.empty(n, **I32), torch.empty(n, dtype=torch.int64, device="cuda")
@@ -49,7 +50,7 @@ class Server:
             q, k, v = qkv[layer].split([N_HEAD, N_KV_HEAD, N_KV_HEAD], 1)
             self.ctx.rope(q, turned[layer], where, self.rope)
             self.ctx.append(pool, k, v, where, slots, self.rope)
-            self.ctx.attention_shared(pool, turned[layer], out[layer], start, self.kv, self.table, self.prefix_start, self.kv[:1], self.table[:1], work, max_q=n, max_kv=most, max_prefix=prefix)
+            self.ctx.attention_shared(pool, turned[layer], out[layer], start, self.kv, self.table, self.prefix_start, self.kv[:1], self.table[:1], work, max_q=each, max_kv=most, max_prefix=prefix)
 
     def fork(self, parents, children):
         parents, children = torch.tensor(parents, **I32), torch.tensor(children, **I32)
@@ -105,7 +106,7 @@ def run(steps=32, instruction=1000, questions=(37, 160, 5), answers=3, seed=0):
         n = sum(n_new)
         qkv = projections(n)
         turned, out = (torch.full((LAYERS, n, N_HEAD, HEAD_DIM), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(2))  # (so that a row nobody writes shows)
-        server.step(torch.tensor(n_new, **I32), qkv, turned, out, ROW_PAGES * PAGE, instruction)
+        server.step(torch.tensor(n_new, **I32), qkv, turned, out, max(n_new), ROW_PAGES * PAGE, instruction)
         at = 0
         for r, k in enumerate(n_new):
             if k and r in rows_to_check:
@@ -124,7 +125,7 @@ def run(steps=32, instruction=1000, questions=(37, 160, 5), answers=3, seed=0):
     turned, out = (torch.zeros(LAYERS, len(children), N_HEAD, HEAD_DIM, dtype=torch.bfloat16, device="cuda") for _ in range(2))
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        server.step(n_new, qkv, turned, out, ROW_PAGES * PAGE, instruction)
+        server.step(n_new, qkv, turned, out, 1, ROW_PAGES * PAGE, instruction)
     for step in range(steps):
         if step == steps // 2 and len(live) > 1:
             server.drop([1, live[0], live[-1]])  # a question, whose answers go on, and two answers

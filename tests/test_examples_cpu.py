@@ -55,3 +55,13 @@ def test_outputs_that_nobody_writes_show(monkeypatch):
         monkeypatch.setattr(bp.PagedContext, name, lambda self, *a, **kw: None)
     assert paged_serving.serve(2, (40, 3)) == (float("inf"), float("inf"))
     assert shared_serving.run(2, 1000, (7,), 2)[0] == float("inf")
+
+
+@pytest.mark.gpu
+def test_a_decoded_step_says_that_rows_get_one_token(monkeypatch):
+    """By max_q a call goes to the kernel for single tokens or to the one for prompts."""
+    asked, call = [], bp.PagedContext.attention_shared
+    monkeypatch.setattr(bp.PagedContext, "attention_shared", lambda self, *a, **kw: (asked.append((a[1].shape[0], kw["max_q"])), call(self, *a, **kw))[1])
+    shared_serving.run(2, 1000, (7, 30), 5)
+    layers = shared_serving.LAYERS
+    assert asked == [(1000, 1000)] * layers + [(37, 30)] * layers + [(10, 1)] * layers
