@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(ROW_THREADS) pages_release_kernel(const __grid
 // ---- fork ------------------------------------------------------------------------------------------------------------
 
 // A CTA per pair copies the row's full pages; the CTA that comes last hands out the pages for those that are not full. A child is claimed by -1 - i in its
-// length, so a row that is a child twice is one pair's alone.
+// length, so a row that is a child twice is one pair's alone; whose it is src says until then (a length may have been negative before).
 struct ForkArgs {
   Tables t;
   const int32_t *parents, *children;
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(ROW_THREADS) pages_fork_kernel(const __grid_co
       } else if (f.parents[i] >= 0 && f.children[i] >= 0) {
         note_range(t.err);
       }
-      tokens_s = tokens;
+      tokens_s = f.src[i] = tokens;
     }
     __syncthreads();
     const int32_t tokens = tokens_s;
@@ -367,12 +367,10 @@ __global__ void __launch_bounds__(ROW_THREADS) pages_fork_kernel(const __grid_co
   const uint32_t per = (f.n + ROW_THREADS - 1) / ROW_THREADS, i0 = min(threadIdx.x * per, f.n), i1 = min(i0 + per, f.n);
   Look<false> look;
   look.ask(t, 0);
-  uint32_t need = 0, parent, child;
+  uint32_t need = 0;
   uint2 total;
   for (uint32_t i = i0; i < i1; i++) {
-    int32_t tokens = -1;
-    if (is_pair(f, i, parent, child) && *reinterpret_cast<volatile int32_t*>(&t.kv_len[child]) == -1 - static_cast<int32_t>(i))
-      tokens = max(*reinterpret_cast<volatile int32_t*>(&t.kv_len[parent]), 0);  // (a parent that is somebody's child, too, was empty)
+    const int32_t tokens = *reinterpret_cast<volatile int32_t*>(&f.src[i]);
     lengths[i] = tokens;
     need += tokens > 0 && (tokens & (t.page - 1));
     f.src[i] = f.dst[i] = -1;

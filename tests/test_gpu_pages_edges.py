@@ -51,3 +51,19 @@ def test_compaction_tells_counts_below_zero_from_moves(ctx, rows, width, count):
     assert np.array_equal(src.cpu().numpy(), want[0]) and np.array_equal(dst.cpu().numpy(), want[1])
     assert (want[0] >= 0).sum() == min(50, 20 + 3 * (rows - 1) - 1) and b.ref.table[0, 7] == held
     b.check()
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("pair", [0, 1, 2])
+def test_forks_tell_a_length_below_zero_from_a_claimed_child(ctx, page, pair):
+    """A child of any such length is not empty: its pair is reported, its row and every count stay. The other pairs are made."""
+    b = Both(3, 8, 6, 60, page, [3 * page + 5, 2 * page, 0, 0, 0, 0, 4 * page + 1, 0])
+    parents, children = [0, 1, 6, 0], [2, 3, 4, 5]
+    b.ref.kv[children[pair]] = -1 - pair
+    b.kv.copy_(dev(b.ref.kv))
+    src, dst = dev([5] * 4), dev([5] * 4)
+    reported(ctx, lambda: ctx.fork(b.gpu, dev(parents), dev(children), src, dst))
+    parents[pair] = -1
+    _, s, d = b.ref.fork(parents, children)
+    assert np.array_equal(src.cpu().numpy(), s) and np.array_equal(dst.cpu().numpy(), d)
+    b.check()
