@@ -466,8 +466,10 @@ __device__ __forceinline__ void free_moved(const CompactArgs& c) {
   for (uint32_t i = threadIdx.x; i < c.most; i += blockDim.x)
     if (c.src[i] >= 0) c.t.refs[c.src[i]] = 0;
 }
-// All of it by a cluster, a warp per row: tables of up to COMPACT_ENTRIES entries.
-constexpr uint32_t COMPACT_ENTRIES = 1u << 18;
+// All of it by a cluster, a warp per row: tables of up to COMPACT_ENTRIES entries. us on the device for 64 pages, one launch / two (whose issue takes 3 more of the host):
+//   rows x pages of a row   16 x 64   64 x 256   64 x 1024   256 x 512   64 x 4096   512 x 512   1024 x 512   4096 x 1024
+//                           6.6/7.1   9.1/9.9    14.6/15.1   12.5/12.0   46.2/33.1   18.2/12.3   29.0/12.1    167/20.3
+constexpr uint32_t COMPACT_ENTRIES = 1u << 17;
 __global__ void __launch_bounds__(GROW_THREADS, 1) pages_compact_kernel(const __grid_constant__ CompactArgs c) {
   extern __shared__ uint32_t smem[];
   __shared__ uint32_t sums[GROW_THREADS / 32];
