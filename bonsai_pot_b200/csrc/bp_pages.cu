@@ -120,6 +120,10 @@ __device__ __forceinline__ uint32_t last_begun(const uint32_t* begin, uint32_t n
 // ---- grow ------------------------------------------------------------------------------------------------------------
 
 constexpr uint32_t GROW_THREADS = 1024;
+// Places of new tokens that one CTA fills in; more are spread over a cluster of eight. us on the device, one CTA / eight:
+//   places    512       2048      4096      8192      16384      32768        256 rows: 2048      4096      16384
+//   16 rows   6.4/7.0   7.0/8.0   7.9/8.1   9.9/8.2   14.1/9.2   22.7/10.4              7.6/8.3   8.9/8.7   18.3/10.3
+constexpr uint32_t GROW_ALONE = 4 * GROW_THREADS;
 
 struct GrowArgs {
   Tables t;
@@ -599,7 +603,7 @@ int bp_pages_grow(bp_paged_ctx* c, void* stream, const bp_page_tables* tables, c
   OnDevice on(c->device);
   BP_TRY(c, on.err);
   const uint32_t smem = (GROW_THREADS * WORDS + 2 * (g.t.n_rows + 1)) * 4;
-  BP_TRY(c, launch_cluster(pages_grow_kernel, n_out > 2 * GROW_THREADS ? 8 : 1, smem, static_cast<cudaStream_t>(stream), g));
+  BP_TRY(c, launch_cluster(pages_grow_kernel, n_out > GROW_ALONE ? 8 : 1, smem, static_cast<cudaStream_t>(stream), g));
   return BP_OK;
 }
 
