@@ -21,9 +21,9 @@
 // 1600 for a free buffer, the O issuers 1770 for P, and the expanders 490 for free slots. The row exponentials alone take 1024 cycles at 16 per cycle and SM, the MMAs
 // would take about 1450 at the measured rate of a library product. 2048 queries behind 32768 keys, 32 / 8 heads of 128: 1.21 ms, 881 TFLOP/s, 54 % of that rate
 // (floor 0.65 ms). Four expander warps whose page ids were waited for took 1.39 ms; eight of them, with two softmax threads per row, 1.38; with one softmax
-// thread per row 1.25; with whole lines read and one barrier per slot 1.23. 4 requests of up to 512 queries behind up to 4099 keys: 97 us (floor 32): a tile costs the
+// thread per row 1.25; with whole lines read and one barrier per slot 1.23. 4 requests of up to 512 queries behind up to 4099 keys: 98 us (floor 32): a tile costs the
 // same, beginning and ending an item about 14 us; before the line weighted items and the partial results had whole-warp accesses it was 216. 4 chunks of up to 512 queries with
-// 16384 keys in common and up to 1030 of their own: 412 us, 880 TFLOP/s (BEHIND; both parts in one launch 425, and 20 to join them). One query tile of 128 rows (64 tokens behind 8191 keys in common, 90 CTAs): 33 us, 1.0 to 1.15
+// 16384 keys in common and up to 1030 of their own: 434 us, 836 TFLOP/s (BEHIND; in PARTS, with 20 to join them, 444). One query tile of 128 rows (64 tokens behind 8191 keys in common, 90 CTAs): 33 us, 1.0 to 1.15
 // per key tile (2000 cycles: an expander warp takes 1900 for it, nearly all of them one instruction waiting for another, the softmax 1300), 1.3 before the first item is
 // found, 1.8 for the queries, 2 from there to the first scores, 2.4 to write the rows. (Tried: two key tiles per turn of the expanders, 280 bytes of registers spilled: 45 us; K and V of a tile
 // behind one fence: the same; every 2nd or 4th pair of exponentials by a polynomial on the FMA units: chunks 536 and 487 us instead of 450.)
@@ -41,8 +41,14 @@ constexpr uint32_t SLOTS = 4;          // K and V tiles in shared memory
 // Tiles of which some rows of an item see only a part: its rows are 256 tokens at most, so these are 5 tiles at each end of the keys that they see; where a
 // window is so short that no tile lies between the two ends, the two overlap or are less than two tiles apart: 11 tiles.
 constexpr uint32_t MIXED = 11;
-// What beginning and ending an item costs, in key tiles. (In parts its rows are 32-bit records. 4 chunks of 512 behind 16384 keys: with 6, 633 us, as the CTAs with
-// the chunks' own keys, a dozen tiles per item, came last; 10: 444, 14: 451, 18: 455.)
+// What beginning and ending an item costs, in key tiles. (In parts its rows are 32-bit records.) us in parts, 32 / 8 heads of 128 and 40 / 8 of 64; no number is the best for all, 10 is never
+// more than 16 % from it:
+//   requests x tokens, prefix, own   16 x 16, 8192, 600   16 x 40, 4096, 400   8 x 64, 16384, 700   32 x 40, 1000, 1000   32 x 8, 4096, 500 (64 dims)
+//   cost 4                           86 / 79              110 / 106            238 / 231            139 / 120             69
+//   6                                86 / 81              102 / 99             215 / 210            137 / 119             72
+//   10                               90 / 85              103 / 100            192 / 208            137 / 121             80
+//   14                               96 / 90              111 / 102            196 / 215            134 / 120             89
+//   20                               103 / 96             115 / 108            201 / 224            132 / 120             93
 template <int MODE>
 constexpr uint32_t ITEM_COST = MODE == PARTS ? BP_KV4_ITEM_COST_IN_PARTS : 6;
 constexpr float GROW = 5.f;            // log2 by which a maximum may grow before O is rescaled; P_UP + GROW stays below 16

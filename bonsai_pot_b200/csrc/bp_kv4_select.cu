@@ -166,7 +166,7 @@ __device__ __forceinline__ void store_to_first(uint32_t* at, uint32_t x) {
 // go to the first CTA, which looks for the want-th highest of them: the range in which it lies is cut into up to 256 parts of equal width and counted until one part
 // holds no others than are wanted. Bound by latency: what follows the launch is one chain of accesses to memory (the token's request 0.4 us, its lengths, page ids and summaries
 // 1.6 to 2 for as many pages as are asked for at a time) and of barriers (range and counts 2, the list 1.5). One token of 1024 pages 6.9 us in clusters of eight (0.3 of memory; 23 with a CTA per head that
-// asked for four pages at a time per warp), 53 tokens of up to 512 pages 10.3, 32 tokens of up to 512 pages of twice the bytes 9.3 (5.4 of memory).
+// asked for four pages at a time per warp), 53 tokens of up to 512 pages 10.3, 32 tokens of up to 512 pages of twice the bytes 9.3 (4749 pages of 8 heads: 1.5 of memory).
 template <int D>
 __global__ void __launch_bounds__(CHOICE_THREADS) kv4_select_kernel(const __grid_constant__ ChoiceArgs s) {
   constexpr uint32_t WARPS = CHOICE_THREADS / 32;

@@ -7,7 +7,7 @@
 // the kernel here joins them all, in the order of the keys.
 //
 // Floors: prefix and own keys once, 6.2 us for 64 tokens behind two prefixes of up to 8191 keys (32 / 8 heads of 128, up to 1000 keys of their own), the products, 220 us for 4 chunks of up to 512
-// behind 16384. Measured 41 and 412 us, 16 for 8 tokens behind 2048 keys (bp_kv4_attention over the same keys in rows of pages for each request: 116, 403 and 19).
+// behind 16384. Measured 43.5 and 434 us, 16.9 for 8 tokens behind 2048 keys (bp_kv4_attention over the same keys in rows of pages for each request: 116, 403 and 19.1).
 // Bound by the attention kernels' beginnings and ends and, of chunks, by their softmax. One launch after the other, each joining its items by the CTA that comes last, took 92, 513 and 31; chunks
 // in parts 444.
 #include "bp_kv4_attention.cuh"
@@ -157,7 +157,8 @@ int bp_kv4_attention_shared(bp_paged_ctx* c, void* stream, uint32_t dtype, const
     j.ctas[0] = j.ctas[1] = c->sm_count;
   } else {
     // Side by side, each on its share of the SMs: what a tile of 64 keys takes there (1.2 us of 256 rows, 0.9 of 128) against 0.15 us for a unit of 64 keys of 128 dims here
-    // (0.18, but requests are shorter than the longest), by the lengths that the caller says.
+    // (0.18, but requests are shorter than the longest), by the lengths that the caller says; a unit counts once, whatever a request's rows. 64 tokens, own keys up to 1000, behind 8191 and 5000:
+    // 61 us with max_kv 1000, 98 with 8192, 122 with 32768; 16 requests of 5 tokens (20 rows) behind 8191: 123, most of it the own keys'.
     const float prefix_tiles = static_cast<float>(in->n_prefix) * p.n_kv_head * ((prefix_rows + 255) / 256) * (in->max_prefix / 64 + 6);
     const float prefix_cost = prefix_tiles * (prefix_rows > 128 ? 1.2f : 0.9f), own_cost = static_cast<float>(in->n_req) * p.n_kv_head * (in->max_kv / 64 + 1) * (0.15f / 128) * D;
     const float part = prefix_cost / (prefix_cost + own_cost);

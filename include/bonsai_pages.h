@@ -14,7 +14,8 @@ extern "C" {
 #endif
 
 /* Page tables, all device int32: row r has kv_len[r] tokens in the pages table[r * table_stride + i], i = 0 .. ceil(kv_len / page_tokens) - 1
- * (entries behind these mean nothing, and the calls may overwrite them); refs[p] is how often page p is held, by rows and by whoever
+ * (entries behind these mean nothing, and the calls may overwrite them; whoever shortens a row by hand has to take the pages behind it
+ * from refs, too); refs[p] is how often page p is held, by rows and by whoever
  * else adds to it; a page with refs 0 is free. n_rows <= 16384. A row may be any sequence: a request, a prefix of several, a kept one.
  * The calls below run on the device alone, in the stream's order; what they refuse there they leave as it was, and
  * bp_paged_status reports it (rows, pages or lengths out of range, no free page left, a row that has no room). The results do not depend on how the
@@ -54,7 +55,8 @@ int bp_pages_copy(bp_paged_ctx* ctx, void* stream, const bp_page_array* arrays, 
  * requests before prefix_start[0] and from prefix_start[n_prefix] on have none. Every query of a request sees all keys of its
  * prefix, and of the request's own ones (kv_len[r], in page_table) those that it would see in bp_kv4_attention; so the outputs are those of
  * bp_kv4_attention over prefix and own keys in one row of pages, where a request has no fewer own keys than queries. A query that sees no key
- * gives zeros. max_prefix: no prefix has more keys. work: device memory for 32-bit results of either part, 16-byte aligned, of
+ * gives zeros. What has fewer than 32 bits is what has fewer in bp_kv4_attention (queries, and the weights that multiply values); results of either part are joined in 32.
+ * How the SMs are shared between prefixes and requests goes by max_prefix and max_kv: close ones are worth it. max_prefix: no prefix has more keys. work: device memory for 32-bit results of either part, 16-byte aligned, of
  * bp_kv4_shared_work(total_q, n_head, head_dim) floats; it may serve one call after the other. */
 typedef struct bp_kv4_shared {
   bp_rows q, out;
@@ -94,7 +96,7 @@ typedef struct bp_kv4_choice {
 } bp_kv4_choice;
 int bp_kv4_select(bp_paged_ctx* ctx, void* stream, uint32_t dtype, const bp_kv4_pool* pool, const bp_block_summary* summary, const bp_kv4_choice* args);
 /* Attention of every token over pages of its own for each KV head: pages and keys as bp_kv4_select writes them. Zeros where
- * keys is 0; rows with negative keys are left as they were. total_q <= 65535. */
+ * keys is 0; rows with negative keys are left as they were. Fewer bits: as in bp_kv4_attention. total_q <= 65535. */
 typedef struct bp_kv4_chosen {
   bp_rows q, out;
   const void *pages, *keys;
